@@ -1,0 +1,187 @@
+// What a row's sequence has said so far, and what that and the caller's rules do to its logits.
+//
+// A row's history is a bit per token of the vocabulary (it occurred, in the prompt or in the output) and a count per token (times
+// it was generated; only tokens with their bit set have one above 0).  The bits make the counts' table cheap to keep: a step reads
+// the 4 V / 32 bytes of bits and the counts of set bits only, and a row is cleared by its bits.
+//
+//   l <- seen ? (l > 0 ? l / repetition : l * repetition) : l     (wick src/sampler.rs:76-85)
+//   l <- l - (frequency * n + presence * [n > 0])                  n: the count
+//   l <- l + bias of the token
+//   l <- -inf where the row's mask does not allow the token
+//
+// Whole numbers are added with atomics, whose order changes nothing.
+#include "common.cuh"
+
+namespace wick {
+
+constexpr int HT = 256;
+
+// Blocks (chunk of words, row of the list).
+__global__ void __launch_bounds__(HT)
+history_clear_kernel(unsigned* __restrict__ seen, int* __restrict__ counts, const int* __restrict__ rows, int n_rows, int vocab, int words) {
+    pdl_trigger();
+    pdl_wait();
+    const int r = rows[blockIdx.y];
+    if (r < 0 || r >= n_rows) return;
+    for (int i = blockIdx.x * HT + threadIdx.x; i < words; i += gridDim.x * HT) {
+        unsigned w = seen[(int64_t)r * words + i];
+        if (w == 0) continue;
+        seen[(int64_t)r * words + i] = 0;
+        while (w) {
+            const int v = i * 32 + __ffs(w) - 1;
+            if (v < vocab) counts[(int64_t)r * vocab + v] = 0;
+            w &= w - 1;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(HT)
+history_add_kernel(unsigned* seen, int* __restrict__ counts, const int* __restrict__ tokens, const int* __restrict__ rows, int n, int n_rows,
+                   int vocab, int words, int generated) {
+    pdl_trigger();
+    pdl_wait();
+    const int i = blockIdx.x * HT + threadIdx.x;
+    if (i >= n) return;
+    const int r = rows[i], v = tokens[i];
+    if (r < 0 || r >= n_rows || v < 0 || v >= vocab) return;
+    atomicOr(seen + (int64_t)r * words + (v >> 5), 1u << (v & 31));
+    if (generated) atomicAdd(counts + (int64_t)r * vocab + v, 1);
+}
+
+struct Steer {
+    const float* x;            // logits, rows x_stride apart
+    float* y;                  // result, rows y_stride apart (may be x itself)
+    int64_t x_stride, y_stride;
+    int vocab, words, n_rows, n_masks;
+    const int* rows;           // the row's place in the arrays below, or null: its own index
+    const unsigned* seen;      // [n_rows, words], or null: no penalties
+    const int* counts;         // [n_rows, vocab]
+    const float* penalties;    // [n_rows, 3]: repetition, frequency, presence
+    const int *bias_cu, *bias_tokens;
+    const float* bias_values;  // tokens of one row are distinct
+    const unsigned* masks;     // [n_masks, words]
+    const int* mask_of;        // [n_rows], -1: none
+};
+
+// A block takes U groups of four tokens a thread of one row.  VEC: x and y lie alike to 16 bytes, so that a group is one load and
+// one store; a row of odd length begins in the middle of a group, and bits of a group then lie in two words.
+template <int U, bool VEC>
+__global__ void __launch_bounds__(HT) steer_kernel(const Steer a) {
+    constexpr int CH = HT * U * 4;
+    __shared__ float bias[CH];
+    __shared__ unsigned biased[CH / 32];
+    pdl_trigger();
+    pdl_wait();
+    const int i = blockIdx.y, V = a.vocab;
+    const float* x = fresh(a.x) + i * a.x_stride;
+    float* y = a.y + i * a.y_stride;
+    const int skew = VEC ? (int)(((uintptr_t)x >> 2) & 3) : 0;     // tokens of the first group that lie before the row
+    const int e0 = (int)blockIdx.x * CH - skew;                     // the block's first token
+    const int r = a.rows ? a.rows[i] : i;
+    const bool known = r >= 0 && r < a.n_rows;
+    const unsigned* seen = known && a.seen ? a.seen + (int64_t)r * a.words : nullptr;
+    const int* counts = a.counts + (int64_t)(known ? r : 0) * V;
+    float rep = 1.f, freq = 0.f, pres = 0.f;
+    if (seen) rep = a.penalties[r * 3], freq = a.penalties[r * 3 + 1], pres = a.penalties[r * 3 + 2];
+    const int which = known && a.masks ? a.mask_of[r] : -1;
+    const unsigned* mask = which >= 0 && which < a.n_masks ? a.masks + (int64_t)which * a.words : nullptr;
+    int b0 = 0, b1 = 0;
+    if (known && a.bias_cu) b0 = a.bias_cu[r], b1 = a.bias_cu[r + 1];
+    if (b0 < b1) {
+        for (int k = threadIdx.x; k < CH / 32; k += HT) biased[k] = 0;
+        __syncthreads();
+        for (int k = b0 + threadIdx.x; k < b1; k += HT) {
+            const int at = a.bias_tokens[k] - e0;
+            if (at >= 0 && at < CH) {
+                bias[at] = a.bias_values[k];
+                atomicOr(&biased[at >> 5], 1u << (at & 31));
+            }
+        }
+        __syncthreads();
+    }
+    // bits of four tokens from e on (e >= 0, e < V)
+    auto four = [&](const unsigned* w, int e) -> unsigned {
+        const int k = e >> 5, s = e & 31;
+        unsigned v = w[k] >> s;
+        if (s > 28 && k + 1 < a.words) v |= w[k + 1] << (32 - s);
+        return v & 15u;
+    };
+    auto one = [&](float l, int e, bool is_seen, bool is_allowed) -> float {
+        if (!is_allowed) return -INFINITY;
+        if (is_seen) {
+            l = l > 0.f ? __fdiv_rn(l, rep) : l * rep;
+            const int n = counts[e];
+            if (n > 0) l -= fmaf(freq, (float)n, pres);
+        }
+        if (b0 < b1 && (biased[(e - e0) >> 5] >> ((e - e0) & 31) & 1)) l += bias[e - e0];
+        return l;
+    };
+    float4 v[U];
+    unsigned s4[U], a4[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int e = e0 + (u * HT + (int)threadIdx.x) * 4;
+        const bool whole = VEC && e >= 0 && e + 4 <= V;
+        s4[u] = whole && seen ? four(seen, e) : 0u;
+        a4[u] = whole && mask ? four(mask, e) : 15u;
+        if (whole && a4[u]) v[u] = *reinterpret_cast<const float4*>(x + e);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int e = e0 + (u * HT + (int)threadIdx.x) * 4;
+        if (VEC && e >= 0 && e + 4 <= V) {
+            float4 o = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (a4[u] == 15u && s4[u] == 0u && b0 == b1) {
+                o = v[u];
+            } else if (a4[u]) {
+                o.x = one(v[u].x, e, s4[u] & 1, a4[u] & 1);
+                o.y = one(v[u].y, e + 1, s4[u] & 2, a4[u] & 2);
+                o.z = one(v[u].z, e + 2, s4[u] & 4, a4[u] & 4);
+                o.w = one(v[u].w, e + 3, s4[u] & 8, a4[u] & 8);
+            }
+            *reinterpret_cast<float4*>(y + e) = o;
+        } else {
+            for (int k = max(e, 0); k < min(e + 4, V); ++k)
+                y[k] = one(x[k], k, seen && (seen[k >> 5] >> (k & 31) & 1), !mask || (mask[k >> 5] >> (k & 31) & 1));
+        }
+    }
+}
+
+}  // namespace wick
+
+using namespace wick;
+
+// seen: 32-bit words [n_rows, words]; counts: int32 [n_rows, vocab]; rows: int32 [n], rows outside are left out.
+WICK_API int wick_history_clear(void* seen, int* counts, const int* rows, int n, int n_rows, int vocab, int words, void* s) {
+    WICK_REQUIRE(vocab > 0 && words == (vocab + 31) / 32 && n >= 0 && n <= 65535, "history_clear: bad sizes");
+    if (n == 0) return 0;
+    WICK_CUDA(launch(history_clear_kernel, dim3(min(32, ceil_div(words, HT)), n), dim3(HT), 0, (cudaStream_t)s, (unsigned*)seen, counts, rows,
+                     n_rows, vocab, words));
+    return check_launch("history_clear");
+}
+
+// tokens, rows: int32 [n], the row that each token belongs to.  generated: counted, not only marked.
+WICK_API int wick_history_add(void* seen, int* counts, const int* tokens, const int* rows, int n, int n_rows, int vocab, int words,
+                              int generated, void* s) {
+    WICK_REQUIRE(vocab > 0 && words == (vocab + 31) / 32 && n >= 0, "history_add: bad sizes");
+    if (n == 0) return 0;
+    WICK_CUDA(launch(history_add_kernel, dim3(ceil_div(n, HT)), dim3(HT), 0, (cudaStream_t)s, (unsigned*)seen, counts, tokens, rows, n, n_rows,
+                     vocab, words, generated));
+    return check_launch("history_add");
+}
+
+// x, y: float32 [n, vocab], rows x_stride / y_stride apart; the other arrays as in struct Steer.
+WICK_API int wick_steer_logits(const float* x, int64_t x_stride, float* y, int64_t y_stride, int n, int vocab, const int* rows, int n_rows,
+                               const void* seen, const int* counts, const float* penalties, const int* bias_cu, const int* bias_tokens,
+                               const float* bias_values, const void* masks, const int* mask_of, int n_masks, void* s) {
+    WICK_REQUIRE(vocab > 0 && n >= 0 && n <= 65535, "steer_logits: bad sizes");
+    if (n == 0) return 0;
+    Steer a = {x, y, x_stride, y_stride, vocab, (vocab + 31) / 32, n_rows, n_masks, rows, (const unsigned*)seen, counts, penalties,
+               bias_cu, bias_tokens, bias_values, (const unsigned*)masks, mask_of};
+    const bool alike = (((uintptr_t)x ^ (uintptr_t)y) & 15) == 0 && (x_stride - y_stride) % 4 == 0;
+    if (alike)
+        WICK_CUDA(launch(steer_kernel<1, true>, dim3(ceil_div(vocab + 3, HT * 4), n), dim3(HT), 0, (cudaStream_t)s, a));
+    else
+        WICK_CUDA(launch(steer_kernel<1, false>, dim3(ceil_div(vocab, HT * 4), n), dim3(HT), 0, (cudaStream_t)s, a));
+    return check_launch("steer_logits");
+}

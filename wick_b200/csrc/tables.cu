@@ -1,0 +1,145 @@
+// A step's page tables, positions and slots, built on the device from the sequences' lengths.
+//
+// Sequence b holds start_b positions on held_b = ceil(start_b / 64) pages and gets q_b more; need_b = ceil((start_b + q_b) / 64) -
+// held_b pages come from the list of free ones, sequence after sequence:
+//   page of its column j:  tables[source][j]                     j < held_b      (source: its own record, or its parent's)
+//                          free[head + sum_{b' < b} need_b' + j - held_b]        j < held_b + need_b
+//                          0 (the reserved page)                  beyond, and beyond the list's end, which is reported
+// and for its token i, at position p = start_b + i: slot = page of column p / 64, times 64, plus p % 64.
+//
+// One launch: every block makes the sums over all sequences for itself (a few thousand numbers from the L2 cache; a second
+// launch, or blocks that wait for one another, would cost more than that), then a warp fills a sequence's row, a thread a
+// token.  Record 0 is the padding's: it gets no pages.
+#include "common.cuh"
+
+namespace wick {
+
+constexpr int TT = 256;
+constexpr int MAX_TABLE_SEQS = 8192;
+
+struct Tables {
+    const int *start, *q_len, *slots, *parent;
+    int* tables;                                   // [n_slots, table_width]
+    const int *free_pages, *free_head;
+    int *page_table, *cu_seqlens, *kv_len, *positions, *seq_of_token, *head_out;
+    int64_t* slot_map;
+    int n_seqs, n_slots, table_width, width, n_free, n_tokens;
+};
+
+__global__ void __launch_bounds__(TT) step_tables_kernel(const Tables a, int* status) {
+    extern __shared__ int sums[];
+    int* cum_q = sums;                             // tokens of the sequences before each one
+    int* cum_n = sums + a.n_seqs + 1;              // pages that they need
+    __shared__ int warp_q[TT / 32], warp_n[TT / 32];
+    pdl_wait();                                    // (no early start of the next kernel: kernels of a step read these fields before they wait)
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_seqs;
+    auto held_of = [&](int b) { return (max(a.start[b], 0) + kPage - 1) / kPage; };
+    auto slot_of = [&](int b) {                    // -1: outside the table, reported below
+        const int s = a.slots[b];
+        return s >= 0 && s < a.n_slots ? s : -1;
+    };
+    int base_q = 0, base_n = 0;
+    for (int s0 = 0; s0 < B; s0 += TT) {
+        const int b = s0 + tid;
+        int q = 0, n = 0;
+        if (b < B) {
+            q = max(a.q_len[b], 0);
+            if (slot_of(b) > 0) n = (max(a.start[b], 0) + q + kPage - 1) / kPage - held_of(b);
+        }
+        int uq = q, un = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int tq = __shfl_up_sync(0xffffffffu, uq, o), tn = __shfl_up_sync(0xffffffffu, un, o);
+            if (lane >= o) uq += tq, un += tn;
+        }
+        if (lane == 31) warp_q[warp] = uq, warp_n[warp] = un;
+        __syncthreads();
+        int wq = 0, wn = 0, all_q = 0, all_n = 0;
+#pragma unroll
+        for (int w = 0; w < TT / 32; ++w) {
+            if (w < warp) wq += warp_q[w], wn += warp_n[w];
+            all_q += warp_q[w], all_n += warp_n[w];
+        }
+        if (b < B) cum_q[b] = base_q + wq + uq - q, cum_n[b] = base_n + wn + un - n;
+        base_q += all_q, base_n += all_n;
+        __syncthreads();
+    }
+    if (tid == 0) cum_q[B] = base_q, cum_n[B] = base_n;
+    __syncthreads();
+    const int head = *a.free_head;
+
+    // What column j of sequence b holds.
+    auto page_at = [&](int src, int slot, int held, int total, int first, int j) -> int {
+        if (slot <= 0 || j >= total) return 0;
+        if (j < held) return j < a.table_width ? a.tables[(int64_t)src * a.table_width + j] : 0;
+        const int at = first + j - held;
+        return at >= 0 && at < a.n_free ? a.free_pages[at] : 0;
+    };
+    auto source_of = [&](int b, int slot) {
+        const int p = a.parent ? a.parent[b] : -1;
+        return p >= 0 && p < a.n_slots ? p : max(slot, 0);
+    };
+
+    const int gt = (int)blockIdx.x * TT + tid, step = (int)gridDim.x * TT;
+    for (int b = gt; b <= B; b += step) {
+        a.cu_seqlens[b] = cum_q[b];
+        if (b < B) a.kv_len[b] = max(a.start[b], 0) + cum_q[b + 1] - cum_q[b];
+    }
+    if (gt == 0) {
+        *a.head_out = head + cum_n[B];
+        if ((head < 0 || head + cum_n[B] > a.n_free) && cum_n[B] > 0) atomicCAS(status, 0, 12);
+    }
+    for (int b = gt >> 5; b < B; b += step >> 5) {
+        const int slot = slot_of(b), held = held_of(b), total = held + cum_n[b + 1] - cum_n[b], first = head + cum_n[b], src = source_of(b, slot);
+        if (lane == 0 && (slot < 0 || (slot > 0 && total > min(a.width, a.table_width)))) atomicCAS(status, 0, 13);
+        const bool fork = src != slot;
+        for (int j = lane; j < a.width; j += 32) {
+            const int page = page_at(src, slot, held, total, first, j);
+            a.page_table[(int64_t)b * a.width + j] = page;
+            if (slot > 0 && j < total && j < a.table_width && (fork || j >= held)) a.tables[(int64_t)slot * a.table_width + j] = page;
+        }
+    }
+    for (int t = gt; t < a.n_tokens; t += step) {
+        int pos = 0, seq = 0;
+        int64_t at = -1;
+        if (t < cum_q[B]) {
+            int lo = 0, hi = B;                    // cum_q[lo] <= t < cum_q[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (cum_q[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            seq = lo;
+            pos = max(a.start[seq], 0) + t - cum_q[seq];
+            const int slot = slot_of(seq), held = held_of(seq), total = held + cum_n[seq + 1] - cum_n[seq];
+            at = (int64_t)page_at(source_of(seq, slot), slot, held, total, head + cum_n[seq], pos / kPage) * kPage + pos % kPage;
+        }
+        a.positions[t] = pos;
+        a.seq_of_token[t] = seq;
+        a.slot_map[t] = at;
+    }
+}
+
+}  // namespace wick
+
+using namespace wick;
+
+// Arrays as in struct Tables.  status: 12 the list of free pages is too short, 13 a record or a length outside the tables.
+WICK_API int wick_step_tables(const int* start, const int* q_len, const int* slots, const int* parent, int n_seqs, int* tables, int n_slots,
+                              int table_width, const int* free_pages, int n_free, const int* free_head, int* page_table, int width,
+                              int* cu_seqlens, int* kv_len, int* positions, int* seq_of_token, void* slot_map, int n_tokens, int* head_out,
+                              int* status, void* s) {
+    WICK_REQUIRE(n_seqs >= 1 && n_seqs <= MAX_TABLE_SEQS, "step_tables: %d sequences (1 to %d)", n_seqs, MAX_TABLE_SEQS);
+    WICK_REQUIRE(n_slots >= 1 && table_width >= 1 && width >= 1 && n_free >= 0 && n_tokens >= 0, "step_tables: bad sizes");
+    Tables a = {start, q_len, slots, parent, tables, free_pages, free_head, page_table, cu_seqlens, kv_len, positions, seq_of_token, head_out,
+                (int64_t*)slot_map, n_seqs, n_slots, table_width, width, n_free, n_tokens};
+    const int blocks = max(1, min(2 * sm_count(), max(ceil_div((int64_t)n_seqs, TT / 32), ceil_div(n_tokens, TT))));
+    const size_t smem = (size_t)(2 * (n_seqs + 1)) * sizeof(int);
+    static bool raised = false;
+    if (!raised) {
+        WICK_CUDA(cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * (MAX_TABLE_SEQS + 1) * sizeof(int))));
+        raised = true;
+    }
+    WICK_CUDA(launch(step_tables_kernel, dim3(blocks), dim3(TT), smem, (cudaStream_t)s, a, status));
+    return check_launch("step_tables");
+}

@@ -12,7 +12,7 @@ import contextlib
 import ctypes
 import math
 import os
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -86,7 +86,7 @@ def plain_kernels() -> bool:
     return PLAIN_KERNELS
 
 
-CORE_SOURCES = ["core.cu", "sample.cu", "state.cu"]
+CORE_SOURCES = ["core.cu", "sample.cu", "state.cu", "tables.cu", "steer.cu"]
 
 
 def _core() -> _Lib:
@@ -128,6 +128,8 @@ _STATUS_TEXT = {1: "gemm_tc gave up waiting for a free shared-memory stage", 2: 
                 7: "attention (tcgen05) gave up waiting for a copy or an accumulator",
                 8: "attention decode (tensor cores) gave up waiting for its TMA copies",
                 10: "attention decode was given a length or a page outside its page table or its cache",
+                11: "attention over a shared prefix was given a sequence that does not fit its group's pages or its page table",
+                12: "step_tables ran out of free pages", 13: "step_tables was given a record or a length outside its tables",
                 99: "the test kernel gave up waiting for nothing (nobody arrives on its barrier)"}
 
 
@@ -526,6 +528,93 @@ def attention_decode_parts_fused(qkv: torch.Tensor, n_heads: int, n_kv: int, hea
                          _p(k_weight), float(eps), _p(cos), _p(sin), 1 if write_kv else 0, _p(kv), kv.shape[0], _p(out),
                          _p(scratch), scratch.numel(), _p(batch.kv_len), n, mk, _p(batch.page_table), batch.table_width,
                          n_heads, n_kv, float(scale), _p(status_tensor(qkv.device)), _stream(), kernels=2 if mk > 128 else 1)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Attention where groups of a step's sequences share their first pages (csrc/attn_shared.cuh, attn_shared.cu).
+SHARED_SOURCES = ["attn_shared.cu"]
+
+
+def _shared(head_dim: int) -> _Lib:
+    key = f"shared{head_dim}"
+    lib = _libs.get(key)
+    if lib is None:
+        _need(head_dim % 16 == 0 and 16 <= head_dim <= 256,
+              f"attention kernels take a head_dim that is a multiple of 16 between 16 and 256, not {head_dim}")
+        lib = _libs[key] = _Lib(f"wick_shared_hd{head_dim}", SHARED_SOURCES, [f"WICK_HD={head_dim}"])
+        lib._lib.wick_attn_shared_scratch.restype = ctypes.c_longlong
+        lib._lib.wick_attn_shared_scratch.argtypes = [ctypes.c_int] * 8
+    return lib
+
+
+class SharedPrefix(NamedTuple):
+    """Which sequences of a step share their first pages.  Group g is the sequences ``cu_groups[g]`` to ``cu_groups[g + 1]`` of the step
+    (every sequence is in one group), whose page tables begin with the same ``pages[g]`` page ids (0: they share nothing); each
+    of them has cached at least that many whole pages before the step.  ``group_of`` names each sequence's group.  All three
+    are int32 on the device.  ``max_pages`` and ``own_bound`` are upper bounds, for the host: of ``pages``, and of the positions (the
+    step's new ones among them) that a sequence holds behind its group's pages."""
+    cu_groups: torch.Tensor
+    pages: torch.Tensor
+    group_of: torch.Tensor
+    max_pages: int
+    own_bound: int
+
+    @classmethod
+    def of(cls, sizes: Sequence[int], pages: Sequence[int], kv_lens: Sequence[int], device) -> "SharedPrefix":
+        """From host lists: sequences and shared pages of each group, and the sequences' lengths after the step."""
+        _need(len(sizes) == len(pages) and all(n >= 0 for n in sizes) and sum(sizes) == len(kv_lens), "every sequence is in one group")
+        group_of = [g for g, n in enumerate(sizes) for _ in range(n)]
+        own = [k - PAGE * pages[g] for k, g in zip(kv_lens, group_of)]
+        _need(all(p >= 0 for p in pages) and all(n > 0 for n in own), "a group's sequences are longer than the pages that they share")
+        cu = [0]
+        for n in sizes:
+            cu.append(cu[-1] + n)
+        dev = torch.tensor(cu + list(pages) + group_of, dtype=torch.int32).to(device)
+        G = len(sizes)
+        return cls(dev[:G + 1], dev[G + 1:2 * G + 1], dev[2 * G + 1:], max(pages, default=0), max(own, default=0))
+
+
+def attention_shared_scratch(shared: SharedPrefix, batch, n_heads: int, n_kv: int, head_dim: int) -> int:
+    """float32 words of scratch that :func:`attention_shared` needs for this step."""
+    lib = _shared(head_dim)
+    n = lib._lib.wick_attn_shared_scratch(batch.n_tokens, batch.n_seqs, shared.pages.numel(), n_heads, n_kv, shared.max_pages, shared.own_bound,
+                                          batch.max_q_len)
+    if n < 0:
+        raise KernelError(lib._lib.wick_last_error().decode("utf-8", "replace"))
+    return n
+
+
+def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPrefix, scale: float, scratch: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of the step's new tokens (any number a sequence, one each when decoding) over the cache, which already holds their
+    keys and values, reading what a group of sequences shares once for the whole group.  q: [n, heads, d]; kv: [pages, 2,
+    kv_heads, 64, d].  The result is that of the same tokens' ordinary attention over ``batch.page_table``.  scratch: float32, at
+    least :func:`attention_shared_scratch` words (made here if none is given)."""
+    n, n_heads, hd = q.shape
+    _cuda("q", q)
+    _cuda("kv", kv, q.dtype)
+    _need(kv.dim() == 5 and kv.shape[1] == 2 and kv.shape[3] == PAGE and kv.shape[4] == hd,
+          f"kv must be [pages, 2, kv_heads, {PAGE}, {hd}], is {tuple(kv.shape)}")
+    cu_groups, pages, group_of, max_pages, own_bound = shared
+    G, n_seqs = pages.numel(), batch.n_seqs
+    _need(n == batch.n_tokens, f"q has {n} rows, the batch {batch.n_tokens} tokens")
+    _cuda("cu_groups", cu_groups, torch.int32, (G + 1,))
+    _cuda("pages", pages, torch.int32)
+    _cuda("group_of", group_of, torch.int32, (n_seqs,))
+    if scratch is None:
+        scratch = torch.empty(attention_shared_scratch(shared, batch, n_heads, kv.shape[2], hd), dtype=torch.float32, device=q.device)
+    else:
+        _cuda("scratch", scratch, torch.float32)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _cuda("out", out, q.dtype, q.shape)
+    splits = own_bound > 512
+    _shared(hd).call(f"wick_attn_shared_{_dt(q)}", "piplppppipippiiiiiifplpp", _p(q), n, _p(kv), kv.shape[0], _p(out), _p(cu_groups), _p(pages),
+                     _p(group_of), G, _p(batch.cu_seqlens), n_seqs, _p(batch.start), _p(batch.page_table), batch.table_width, n_heads,
+                     kv.shape[2], max_pages, own_bound, batch.max_q_len, float(scale), _p(scratch), scratch.numel(),
+                     _p(status_tensor(q.device)), _stream(), kernels=1 + (max_pages > 0) + splits)
     return out
 
 
@@ -1911,6 +2000,133 @@ def penalty_seen(logits: torch.Tensor, seen: torch.Tensor, state: torch.Tensor, 
     _cuda("slots", slots, torch.int32, (rows,))
     _core().call("wick_penalty_seen", "ppippfip", _p(logits), _p(seen), vocab, _p(state), _p(slots), float(penalty), rows,
                  _stream())
+
+
+# ---------------------------------------------------------------------------
+# A step's description made on the device (csrc/tables.cu).
+def step_tables(start: torch.Tensor, q_len: torch.Tensor, slots: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor,
+                free_head: torch.Tensor, *, page_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_len: torch.Tensor, positions: torch.Tensor,
+                seq_of_token: torch.Tensor, slot_map: torch.Tensor, head_out: torch.Tensor, parent: Optional[torch.Tensor] = None) -> None:
+    """The fields of a step's description from its sequences' lengths, without the host.
+
+    Sequence b (record ``slots[b]``) has cached ``start[b]`` positions and brings ``q_len[b]`` new tokens (0: none).  The pages it holds
+    are in ``tables[slots[b]]`` (int32 [slots, width], in position order); what it needs beyond is handed out from ``free_pages``,
+    beginning at ``free_head[0]``, sequence after sequence, and written to ``tables``.  A sequence with ``parent[b] >= 0`` starts from
+    the pages of that record instead of its own (the pages that hold its ``start[b]`` positions; a parent holds at least those).
+    Record 0 is the padding's: it gets no pages.  A list that is too short gives the reserved page 0 and shows in
+    :func:`check_status`.
+
+    Written: page_table [n, any width], 0 behind a sequence's last page; cu_seqlens [n + 1]; kv_len [n]; for each of the tokens (as many as
+    ``positions`` has places; places beyond the last token get position 0, sequence 0 and slot -1) positions, seq_of_token and
+    slot_map (int64: page * 64 + place in the page); head_out [1], the next step's ``free_head`` (another tensor than ``free_head``)."""
+    n, n_tokens, i32 = slots.numel(), positions.numel(), torch.int32
+    for nm, t in (("start", start), ("q_len", q_len), ("slots", slots), ("kv_len", kv_len)):
+        _cuda(nm, t, i32, (n,))
+    _cuda("tables", tables, i32)
+    _cuda("free_pages", free_pages, i32)
+    _cuda("free_head", free_head, i32, (1,))
+    _cuda("page_table", page_table, i32)
+    _need(tables.dim() == 2 and page_table.dim() == 2 and page_table.shape[0] == n, f"tables must be [slots, width], page_table [{n}, width]")
+    _cuda("cu_seqlens", cu_seqlens, i32, (n + 1,))
+    _cuda("positions", positions, i32)
+    _cuda("seq_of_token", seq_of_token, i32, (n_tokens,))
+    _cuda("slot_map", slot_map, torch.int64, (n_tokens,))
+    _cuda("head_out", head_out, i32, (1,))
+    _need(head_out.data_ptr() != free_head.data_ptr(), "head_out must be another tensor than free_head")
+    if parent is not None:
+        _cuda("parent", parent, i32, (n,))
+    _core().call("wick_step_tables", "ppppipiipippipppppippp", _p(start), _p(q_len), _p(slots), _p(parent), n,
+                 _p(tables), tables.shape[0], tables.shape[1], _p(free_pages), free_pages.numel(), _p(free_head), _p(page_table),
+                 page_table.shape[1], _p(cu_seqlens), _p(kv_len), _p(positions), _p(seq_of_token), _p(slot_map), n_tokens, _p(head_out),
+                 _p(status_tensor(slots.device)), _stream())
+
+
+# ---------------------------------------------------------------------------
+# What a sequence has said, and what that and the caller's rules do to its logits (csrc/steer.cu).
+def bit_words(n: int) -> int:
+    """32-bit words that hold a bit for each of ``n`` tokens."""
+    return (n + 31) // 32
+
+
+def _history(seen: torch.Tensor, counts: torch.Tensor) -> Tuple[int, int, int]:
+    _cuda("counts", counts, torch.int32)
+    _need(counts.dim() == 2, "counts must be [rows, vocab]")
+    n_rows, vocab = counts.shape
+    words = (vocab + 31) // 32
+    _cuda("seen", seen, torch.int32, (n_rows, words))
+    return n_rows, vocab, words
+
+
+def history_clear(seen: torch.Tensor, counts: torch.Tensor, rows: torch.Tensor) -> None:
+    """Forget the histories of ``rows`` (int32).  A history is a bit per token in ``seen`` (int32 [rows, words of 32 tokens]: it occurred, in
+    the prompt or the output) and the times it was generated in ``counts`` (int32 [rows, vocab]; above 0 only where the bit is set)."""
+    n_rows, vocab, words = _history(seen, counts)
+    _cuda("rows", rows, torch.int32)
+    _core().call("wick_history_clear", "pppiiiip", _p(seen), _p(counts), _p(rows), rows.numel(), n_rows, vocab, words, _stream())
+
+
+def history_add(seen: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor, rows: torch.Tensor, generated: bool) -> None:
+    """Add ``tokens`` (int32) to the histories of ``rows`` (int32, a row per token; a row or a token outside the arrays is left out).
+    generated: they are counted, not only marked as seen."""
+    n_rows, vocab, words = _history(seen, counts)
+    _cuda("tokens", tokens, torch.int32)
+    _cuda("rows", rows, torch.int32, tokens.shape)
+    _core().call("wick_history_add", "ppppiiiiip", _p(seen), _p(counts), _p(tokens), _p(rows), tokens.numel(), n_rows, vocab, words,
+                 1 if generated else 0, _stream())
+
+
+def steer_logits(logits: torch.Tensor, rows: Optional[torch.Tensor] = None, *, seen: Optional[torch.Tensor] = None,
+                 counts: Optional[torch.Tensor] = None, penalties: Optional[torch.Tensor] = None,
+                 bias: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, masks: Optional[torch.Tensor] = None,
+                 mask_of: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A step's logits under its sequences' rules, in one pass.  logits: float32 [n, vocab] (rows may lie further apart than vocab).
+    ``rows``: int32 [n], each logits row's place in the arrays below (none: its own index; a place outside them has no rules).
+
+    * ``seen``, ``counts`` (see :func:`history_clear`) with ``penalties``, float32 [rows, 3]: a token that occurred has its logit
+      divided by penalties[:, 0] if positive, multiplied otherwise; then ``penalties[:, 1] * n + penalties[:, 2]`` is taken off one
+      that was generated n > 0 times (repetition, frequency, presence);
+    * ``bias`` = (int32 [rows + 1] ranges, int32 tokens, float32 values): row r's entries, whose tokens differ, are added;
+    * ``masks``, int32 [masks, words]: a token whose bit is 0 in mask ``mask_of[row]`` (int32 [rows]; -1: none) becomes -inf, whatever
+      its logit was.  A mask that allows nothing leaves a row of -inf.
+
+    out: where to write (default: in place)."""
+    n, vocab = logits.shape
+    _need(logits.is_cuda and logits.dtype == torch.float32 and (vocab == 1 or logits.stride(1) == 1) and (n <= 1 or logits.stride(0) >= vocab),
+          "logits must be float32 rows on the CUDA device")
+    if out is None:
+        out = logits
+    else:
+        _need(out.is_cuda and out.dtype == torch.float32 and out.shape == logits.shape and (vocab == 1 or out.stride(1) == 1) and
+              (n <= 1 or out.stride(0) >= vocab), f"out must be float32 rows [{n}, {vocab}] on the CUDA device")
+    n_rows = n_masks = 0
+    if seen is not None:
+        _need(counts is not None and penalties is not None, "seen, counts and penalties come together")
+        n_rows, v, _ = _history(seen, counts)
+        _need(v == vocab, f"counts must be [rows, {vocab}]")
+        _cuda("penalties", penalties, torch.float32, (n_rows, 3))
+    else:
+        _need(counts is None and penalties is None, "seen, counts and penalties come together")
+    cu = tokens = values = None
+    if bias is not None:
+        cu, tokens, values = bias
+        _cuda("bias ranges", cu, torch.int32)
+        _need(n_rows in (0, cu.numel() - 1) and cu.numel() > 0, f"bias ranges must have {n_rows + 1} places")
+        n_rows = cu.numel() - 1
+        _cuda("bias tokens", tokens, torch.int32)
+        _cuda("bias values", values, torch.float32, tokens.shape)
+    if masks is not None:
+        _need(mask_of is not None, "masks and mask_of come together")
+        _cuda("mask_of", mask_of, torch.int32)
+        _need(n_rows in (0, mask_of.numel()), f"mask_of must have {n_rows} places")
+        n_rows, n_masks = mask_of.numel(), masks.shape[0]
+        _cuda("masks", masks, torch.int32, (n_masks, (vocab + 31) // 32))
+    else:
+        _need(mask_of is None, "masks and mask_of come together")
+    if rows is not None:
+        _cuda("rows", rows, torch.int32, (n,))
+    _core().call("wick_steer_logits", "plpliipippppppppip", _p(logits), logits.stride(0), _p(out), out.stride(0), n, vocab, _p(rows), n_rows,
+                 _p(seen), _p(counts), _p(penalties), _p(cu), _p(tokens), _p(values), _p(masks), _p(mask_of), n_masks, _stream())
+    return out
 
 
 def wait_gives_up(limit_ms: float = 1.0) -> bool:
