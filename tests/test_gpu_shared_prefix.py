@@ -199,7 +199,7 @@ def test_attention_shared_in_a_graph_follows_the_description(ops):
     b = case.batch()
     shared = ops.SharedPrefix.of(case.sizes, case.shared, case.kv_lens, "cuda")._replace(max_pages=4, own_bound=900)
     q, kv = case.q.cuda(), case.kv.cuda()
-    scratch = torch.empty(ops.attention_shared_scratch(shared, b, 8, 2, 128), dtype=F32, device="cuda")
+    scratch = torch.empty(ops.attention_shared_scratch(shared, b, 8, 2, 128, BF16), dtype=F32, device="cuda")
     out = torch.empty_like(q)
     ops.attention_shared(q, kv, b, shared, case.scale, scratch, out)
     g = torch.cuda.CUDAGraph()

@@ -613,25 +613,33 @@ constexpr int PER_SM = 2;                          // blocks an SM of the kernel
 
 struct Call {
     Groups G;
+    bool tc;                                       // the shared part's tcgen05 form
     int tiles_own, splits, blocks;                 // tiles of 16 rows of the longest sequence; parts of own keys; blocks for the shared keys
     int64_t plan_words, prefix_floats, own_floats;
 };
 
-static int plan_call(Call& c, int n_tokens, int n_seqs, int n_groups, int heads, int kv_heads, int max_pages, int own_bound, int max_q_len) {
+static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups, int heads, int kv_heads, int max_pages, int own_bound, int max_q_len) {
     WICK_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "attention (shared prefix): %d heads over %d kv heads", heads, kv_heads);
     WICK_REQUIRE(n_seqs >= 1 && n_seqs <= 65535 && n_tokens >= 0, "attention (shared prefix): %d sequences, %d tokens", n_seqs, n_tokens);
     WICK_REQUIRE(n_groups >= 1 && n_groups <= MAX_GROUPS, "attention (shared prefix): %d groups (1 to %d)", n_groups, MAX_GROUPS);
     WICK_REQUIRE(max_pages >= 0 && own_bound >= 0 && max_q_len >= 0, "attention (shared prefix): bad bounds");
     const int group = heads / kv_heads;
     c.G.n = n_groups, c.G.n_seqs = n_seqs, c.G.max_pages = max_pages, c.G.heads = heads, c.G.kv_heads = kv_heads;
-    c.G.rows = R, c.G.gs = group, c.G.per_kv = 1, c.G.columns = kv_heads, c.G.unit_pages = 1;
+    c.tc = half && tc_supported();
+    if (c.tc) {
+        int gs = 1;                                // heads of a tile: as many as fill its rows with whole tokens
+        while (group % (2 * gs) == 0 && 2 * gs <= TC_ROWS) gs *= 2;
+        c.G.rows = TC_ROWS, c.G.gs = gs, c.G.per_kv = group / gs, c.G.columns = heads / gs, c.G.unit_pages = 2;
+    } else {
+        c.G.rows = R, c.G.gs = group, c.G.per_kv = 1, c.G.columns = kv_heads, c.G.unit_pages = 1;
+    }
     c.tiles_own = ceil_div((int64_t)max_q_len * group, R);
     WICK_REQUIRE((int64_t)c.tiles_own * kv_heads <= INT32_MAX / 2, "attention (shared prefix): %d tokens of one sequence are too many", max_q_len);
     c.splits = own_splits(own_bound);
-    c.blocks = PER_SM * sm_count();
+    c.blocks = (c.tc ? 1 : PER_SM) * sm_count();
     c.plan_words = max_pages > 0 ? (2 * (n_groups + 1) + 1 + 3) / 4 * 4 : 0;
-    const int64_t tiles = ceil_div((int64_t)n_tokens * group, R) + n_groups;
-    c.prefix_floats = max_pages > 0 ? (tiles * c.G.columns + c.blocks) * REC : 0;
+    const int64_t tiles = ceil_div((int64_t)n_tokens * c.G.gs, c.G.rows) + n_groups;
+    c.prefix_floats = max_pages > 0 ? (tiles * c.G.columns + c.blocks) * c.G.rows * (HD + 2) : 0;
     c.own_floats = c.splits > 1 ? (int64_t)n_seqs * c.tiles_own * kv_heads * c.splits * REC : 0;
     return 0;
 }
@@ -642,10 +650,11 @@ static int attn_shared(const void* q, int n_tokens, const void* kv, int64_t kv_p
                        int heads, int kv_heads, int max_pages, int own_bound, int max_q_len, float scale, float* scratch, int64_t scratch_floats,
                        int* status, cudaStream_t s) {
     Call c = {};
-    if (int e = plan_call(c, n_tokens, n_seqs, n_groups, heads, kv_heads, max_pages, own_bound, max_q_len)) return e;
+    if (int e = plan_call(c, sizeof(T) == 2, n_tokens, n_seqs, n_groups, heads, kv_heads, max_pages, own_bound, max_q_len)) return e;
     WICK_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "attention (shared prefix): operands must be 16-byte aligned");
     WICK_REQUIRE(scratch_floats >= c.plan_words + c.prefix_floats + c.own_floats, "attention (shared prefix): scratch of %lld floats, %lld needed",
                  (long long)scratch_floats, (long long)(c.plan_words + c.prefix_floats + c.own_floats));
+    WICK_REQUIRE(scale >= 0.f, "attention (shared prefix): a negative scale");
     if (n_tokens == 0) return 0;
     Groups& G = c.G;
     G.cu_groups = cu_groups, G.pages = pages, G.group_of = group_of, G.cu_seqlens = cu_seqlens, G.start = start, G.page_table = page_table;
@@ -659,9 +668,11 @@ static int attn_shared(const void* q, int n_tokens, const void* kv, int64_t kv_p
         WICK_CUDA(cudaFuncSetAttribute(attn_shared_own_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         raised = true;
     }
-    Shared sh = {nullptr, records, R};
-    if (max_pages > 0) {
-        sh.plan = plan;
+    Shared sh = {nullptr, records, G.rows};
+    if (max_pages > 0) sh.plan = plan;
+    if (max_pages > 0 && c.tc) {
+        if (int e = launch_tc(q, n_tokens, kv, kv_pages, G, c.blocks, scale, plan, records, status, s)) return e;
+    } else if (max_pages > 0) {
         WICK_CUDA(launch(attn_shared_prefix_kernel<T>, dim3(c.blocks), dim3(THREADS), (size_t)SMEM, s, (const T*)q, (const T*)kv, kv_pages, G, scale, plan,
                          records, status));
         if (int e = check_launch("attn_shared_prefix")) return e;
@@ -680,10 +691,10 @@ static int attn_shared(const void* q, int n_tokens, const void* kv, int64_t kv_p
 }  // namespace shared_prefix
 }  // namespace wick
 
-// float32 words of scratch that a call of these sizes needs (-1: refused, see wick_last_error).
-WICK_API long long wick_attn_shared_scratch(int n_tokens, int n_seqs, int n_groups, int heads, int kv_heads, int max_pages, int own_bound, int max_q_len) {
+// float32 words of scratch that a call of these sizes needs (half: of the bfloat16 form; -1: refused, see wick_last_error).
+WICK_API long long wick_attn_shared_scratch(int half, int n_tokens, int n_seqs, int n_groups, int heads, int kv_heads, int max_pages, int own_bound, int max_q_len) {
     shared_prefix::Call c = {};
-    if (shared_prefix::plan_call(c, n_tokens, n_seqs, n_groups, heads, kv_heads, max_pages, own_bound, max_q_len)) return -1;
+    if (shared_prefix::plan_call(c, half != 0, n_tokens, n_seqs, n_groups, heads, kv_heads, max_pages, own_bound, max_q_len)) return -1;
     return c.plan_words + c.prefix_floats + c.own_floats;
 }
 

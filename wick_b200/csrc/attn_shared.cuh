@@ -91,5 +91,11 @@ __device__ __forceinline__ Segment segment_at(const Groups& G, const int* units,
     return s;
 }
 
+// The tcgen05 form of the shared part (attn_shared_tc.cu): bfloat16, tiles of TC_ROWS rows, units of two pages.
+constexpr int TC_ROWS = 128;
+bool tc_supported();
+int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, const Groups& G, int blocks, float scale, int* plan, float* records, int* status,
+              cudaStream_t s);
+
 }  // namespace shared_prefix
 }  // namespace wick

@@ -1,0 +1,416 @@
+// The shared keys of groups of sequences on the 5th-generation tensor cores (tcgen05), bfloat16, head sizes 64 and 128: a record
+// (maximum, sum of weights, weighted sum of values) for every run of units of a tile of 128 rows (attn_shared.cuh).
+//
+// A tile's rows are query heads of one key head times the group's tokens, whatever sequences they belong to: all of them see all
+// shared keys, so there is no mask anywhere.  A unit is a block of 128 keys (two pages; the last one of an odd number is half).  Even
+// blocks go to one stream, odd ones to another, each with its own scores and its own sums in tensor memory and four softmax warps, so
+// that one stream's softmax runs beside the other's products; they are joined when a run ends.
+//   * a producer warp fetches the query rows of a run and its key and value tiles through a ring (TMA, 128-byte swizzle);
+//   * an issuing warp alternates between the streams: O += P V of one, then the scores S = Q K^T of its next block (P lies over the
+//     scores it came from, as bfloat16 pairs);
+//   * a softmax thread owns a row.  O and the sum are scaled by a maximum that follows the true one lazily: O is rescaled only when a
+//     block's maximum exceeds it by more than 8 (in units of log2 e).  Warps whose rows are all beyond the group's tokens compute nothing.
+// Every wait is bounded and reports through the status word (code 7).
+#include "tc_attention.cuh"
+#include "attn_shared.cuh"
+
+#ifndef WICK_HD
+#error "compile with -DWICK_HD=<head_dim>"
+#endif
+
+namespace wick {
+namespace shared_prefix {
+
+namespace tc {
+
+constexpr bool SUPPORTED = WICK_HD == 64 || WICK_HD == 128;
+constexpr int HD = SUPPORTED ? WICK_HD : 64;           // other head sizes: never launched
+constexpr int BQ = TC_ROWS, BK = 128;
+constexpr int PANELS = HD / 64;                        // 64-column panels of a head row
+constexpr int PANEL_BYTES = 128 * 128;                 // 128 rows of 128 bytes
+constexpr int TILE_BYTES = PANELS * PANEL_BYTES;       // the tile of queries, or one block of keys or of values
+constexpr int NSLOT = 5;                               // key / value tiles in flight
+constexpr int THREADS = 320;                           // warp 0: TMA, warp 1: MMA + tensor memory, warps 2-5 and 6-9: softmax
+constexpr uint32_t TMEM_COLS = 512;                    // S of both streams | O of both
+constexpr uint32_t COL_S = 0, COL_O = 2 * BK;
+constexpr int P_FIRST = 64;                            // keys of a block whose weights the product begins with
+constexpr int REC = BQ * (HD + 2);
+
+struct Smem {
+    float ml[2][2][BQ];                                // the streams' maxima and sums
+    uint64_t q_full, q_empty, full[NSLOT], empty[NSLOT], s_full[2], p_full[2][2], o_full[2], o_empty[2], join, joined;
+    Cum cum;
+    uint32_t tmem_slot;
+    int abort_flag;
+};
+constexpr int SMEM_BYTES = (1 + NSLOT) * TILE_BYTES + (int)sizeof(Smem);
+static_assert(SMEM_BYTES <= 227 * 1024, "a block's shared memory");
+
+__global__ void __launch_bounds__(THREADS, 1)
+attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const Groups G, int64_t kv_pages, float scale,
+                      int* plan, float* records, int* status) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* q_s = smem_raw;
+    uint8_t* kv_s = q_s + TILE_BYTES;
+    Smem& sh = *reinterpret_cast<Smem*>(kv_s + NSLOT * TILE_BYTES);
+    volatile int* abort_flag = &sh.abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        sh.abort_flag = 0;
+        mbar_init(&sh.q_full, 1), mbar_init(&sh.q_empty, 1);
+        for (int i = 0; i < NSLOT; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
+        // (every waiter below sees every phase of the barrier it waits on, so that a parity is never ambiguous)
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.s_full[i], 1), mbar_init(&sh.o_full[i], 1), mbar_init(&sh.o_empty[i], 4);
+            mbar_init(&sh.p_full[i][0], 4), mbar_init(&sh.p_full[i][1], 4);
+        }
+        mbar_init(&sh.join, 8), mbar_init(&sh.joined, 8);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0 && lane < 2) {
+        const CUtensorMap* map = lane == 0 ? &q_map : &kv_map;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)), "r"(TMEM_COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    pdl_wait();
+    pdl_trigger();                                     // (behind the wait: the next kernel reads what this one reads without a wait of its own)
+    if (warp == 2) make_plan(G, sh.cum.units, sh.cum.items);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem_slot;
+    const int U = sh.cum.units[G.n], S = blocks_used(U, gridDim.x, 1), cta = blockIdx.x;
+    if (cta == 0) {
+        for (int i = threadIdx.x; i <= G.n; i += THREADS) plan[1 + i] = sh.cum.units[i], plan[2 + G.n + i] = sh.cum.items[i];
+        if (threadIdx.x == 0) plan[0] = S;
+    }
+    const int u_begin = cta < S && U > 0 ? run_start(cta, U, S) : 0, u_end = cta < S && U > 0 ? run_start(cta + 1, U, S) : 0;
+    const bool aligned = (smem_u32(smem_raw) & 1023) == 0;   // (always: the block's dynamic shared memory is all there is)
+    if (!aligned && threadIdx.x == 0) atomicCAS(status, 0, 7);
+    // Walks the block's runs: body(segment, its number, units).  Every role walks on its own.
+    auto each = [&](auto body) {
+        int g = 0, k = 0;
+        for (int u = u_begin; aligned && u < u_end; ++k) {
+            const Segment s = segment_at(G, sh.cum.units, sh.cum.items, g, u, u_end, cta);
+            g = s.g;
+            u += s.to - s.from;
+            if (!body(s, k, s.to - s.from)) break;
+        }
+    };
+    // the block of keys that is half: the last one of an odd number of pages
+    auto half = [&](const Segment& s, int j) { return 2 * (s.from + j) + 1 == s.pages; };
+
+    if (warp == 0) {
+        // ---------------- producer ----------------
+        const bool one = elect_one();
+        int slot = 0, turn = 0;                        // of the ring
+        each([&](const Segment& s, int k, int n_blk) {
+            const int* table = G.page_table + (int64_t)G.cu_groups[s.g] * G.table_width;
+            // A lane holds a page number of each of two runs of 32, read ahead.
+            auto pages = [&](int run) {
+                const int at = 2 * s.from + run * 32 + lane;
+                int page = at < s.pages ? table[at] : 0;
+                if (page < 0 || page >= kv_pages) {
+                    atomicCAS(status, 0, 10);
+                    page = 0;
+                }
+                return page;
+            };
+            int even = pages(0), odd = pages(1);
+            if (k > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.q_empty, (k - 1) & 1, abort_flag, status, 7))) return false;
+            if (one) {
+                mbar_expect_tx(&sh.q_full, TILE_BYTES);
+                for (int pn = 0; pn < PANELS; ++pn)
+                    tma_load_3d(&q_map, &sh.q_full, q_s + pn * PANEL_BYTES, pn * 64, s.column * G.gs, first_token(G, s.g) + s.tile * (BQ / G.gs));
+            }
+            // K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1): the order in which the issuing warp uses them
+#pragma unroll 1
+            for (int i = 0; i < 2 * n_blk; ++i) {
+                const bool last = i == 2 * n_blk - 1;
+                const int is_v = last || (i > 0 && !(i & 1));
+                const int j = last ? n_blk - 1 : (is_v ? (i - 2) >> 1 : (i + 1) >> 1);
+                if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.empty[slot], (turn - 1) & 1, abort_flag, status, 7))) return false;
+                const int held = (2 * j >> 5) & 1 ? odd : even;
+                const int page0 = __shfl_sync(0xffffffffu, held, 2 * j & 31), page1 = __shfl_sync(0xffffffffu, held, (2 * j + 1) & 31);
+                if (is_v && j >= 16 && (j & 15) == 0) {            // (keys and values have left the run before)
+                    if ((j >> 4) & 1) even = pages((j >> 4) + 1);
+                    else odd = pages((j >> 4) + 1);
+                }
+                if (one) {
+                    const int n_pages = half(s, j) ? 1 : 2;
+                    mbar_expect_tx(&sh.full[slot], n_pages * (TILE_BYTES / 2));
+                    uint8_t* dst = kv_s + slot * TILE_BYTES;
+#pragma unroll 1
+                    for (int h = 0; h < n_pages; ++h)
+                        for (int pn = 0; pn < PANELS; ++pn)
+                            tma_load_2d(&kv_map, &sh.full[slot], dst + pn * PANEL_BYTES + h * (kPage * 128), pn * 64,
+                                        (((h ? page1 : page0) * 2 + is_v) * G.kv_heads + s.column / G.per_kv) * kPage);
+                }
+                if (++slot == NSLOT) slot = 0, ++turn;
+                __syncwarp();
+            }
+            return true;
+        });
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        // (the whole warp walks through the steps, one elected lane issues)
+        const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BK >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+        const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+        const uint32_t q_lo = desc_lo(smem_u32(q_s), 16), k_lo0 = desc_lo(smem_u32(kv_s), 16), v_lo0 = desc_lo(smem_u32(kv_s), PANEL_BYTES);
+        const bool one = elect_one();
+        int slot = 0, round = 0;                       // of the ring
+        int steps0 = 0, steps1 = 0, uses0 = 0, uses1 = 0;          // blocks and runs of each stream so far
+        bool ok = true;
+        auto take = [&](int& at) {                     // the next tile of the ring, when it has come
+            at = slot;
+            const bool here = __all_sync(0xffffffffu, mbar_wait(&sh.full[slot], round & 1, abort_flag, status, 7));
+            if (++slot == NSLOT) slot = 0, ++round;
+            return here;
+        };
+        each([&](const Segment& seg, int k, int n_blk) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, k & 1, abort_flag, status, 7));
+            // turn t of stream s: the product of its block t, the scores of its block t + 1
+#pragma unroll 1
+            for (int i = -2; ok && i < n_blk; ++i) {
+                const int s = i & 1, t = i >> 1;
+                const bool more = i + 2 < n_blk;
+                if (t >= 0) {
+                    const int steps = s == 0 ? steps0 : steps1, uses = s == 0 ? uses0 : uses1;
+                    int at;
+                    ok = take(at);
+                    // (the sums of the stream's run before have been read)
+                    if (ok && t == 0 && uses > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_empty[s], (uses - 1) & 1, abort_flag, status, 7));
+                    const uint32_t v_lo = v_lo0 + at * (TILE_BYTES >> 4), d = tmem + COL_O + s * HD, pa = tmem + COL_S + s * BK;
+                    const int parts = half(seg, i) ? 1 : 2;
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[s][part], steps & 1, abort_flag, status, 7));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t pp = pa + part * (P_FIRST / 2), vp = v_lo + part * (P_FIRST / 16) * (2048 >> 4);
+                        if (one && part < parts) {
+                            mma_ts(d, pp, vp, idesc_o, t > 0 || part > 0);
+                            static_for<1, P_FIRST / 16>([&](auto ks) { mma_ts(d, pp + (int)ks * 8, vp + (int)ks * (2048 >> 4), idesc_o, 1); });
+                        }
+                    }
+                    if (!ok) break;
+                    if (one) {
+                        tc_commit(&sh.empty[at]);
+                        if (!more) tc_commit(&sh.o_full[s]);
+                    }
+                    if (s == 0) ++steps0, uses0 += more ? 0 : 1;
+                    else ++steps1, uses1 += more ? 0 : 1;
+                }
+                if (more) {
+                    int at;
+                    ok = take(at);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t k_lo = k_lo0 + at * (TILE_BYTES >> 4), d = tmem + COL_S + s * BK;
+                    if (one) {
+                        static_for<0, HD / 16>([&](auto ks) {
+                            constexpr uint32_t off = (((int)ks >> 2) * PANEL_BYTES + ((int)ks & 3) * 32) >> 4;
+                            mma_ss<((int)ks > 0)>(d, q_lo + off, k_lo + off, idesc_s);
+                        });
+                        tc_commit(&sh.s_full[s]);
+                        tc_commit(&sh.empty[at]);
+                        if (i + 2 == n_blk - 1) tc_commit(&sh.q_empty);        // (the run's last scores)
+                    }
+                }
+                __syncwarp();
+            }
+            return ok;
+        });
+    } else {
+        // ---------------- softmax: a row per thread ----------------
+        // (a warp reads the 32 lanes of tensor memory given by its index modulo 4)
+        const int quad = warp & 3, s = (warp - 2) >> 2;
+        const int r = quad * 32 + lane;
+        const float sl2 = scale * 1.4426950408889634f;
+        const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+        const uint32_t s_addr = lane_base + COL_S + s * BK, o_addr = lane_base + COL_O + s * HD;
+        int step = 0, uses0 = 0, uses1 = 0, joins = 0;  // this stream's blocks, both streams' runs, joins so far
+        bool ok = true;
+        each([&](const Segment& seg, int, int n_blk) {
+            const int n_rows = (first_token(G, seg.g + 1) - first_token(G, seg.g)) * G.gs - seg.tile * BQ;   // (of the tile and behind it)
+            const bool store = r < n_rows, busy = quad * 32 < n_rows;
+            float m = -INFINITY, l = 0.f;              // what O and the sum are scaled by (it follows the maximum lazily), the sum
+            for (int j = s; j < n_blk; j += 2) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s], step & 1, abort_flag, status, 7));
+                if (!ok) return false;
+                ++step;
+                tc_fence_after();
+                auto hand_over = [&](int part) {
+                    tc_st_wait();
+                    tc_fence_before();                 // P and the rescaled O before it multiplies and accumulates
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.p_full[s][part]);
+                };
+                if (!busy) {
+                    hand_over(0), hand_over(1);
+                    continue;
+                }
+                const bool whole = !half(seg, j);
+                float y[BK];
+#pragma unroll
+                for (int c = 0; c < BK; c += 32)
+                    if (c < 64 || whole) tc_ld32_nowait(s_addr + c, reinterpret_cast<uint32_t*>(y + c));
+                tc_ld_wait();
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < BK; i += 8)
+                    if (i < 64 || whole) {
+                        mx4[0] = max3(mx4[0], y[i], y[i + 1]);
+                        mx4[1] = max3(mx4[1], y[i + 2], y[i + 3]);
+                        mx4[2] = max3(mx4[2], y[i + 4], y[i + 5]);
+                        mx4[3] = max3(mx4[3], y[i + 6], y[i + 7]);
+                    }
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+                const bool grow = mx > m + 8.0f;
+                float alpha = 1.0f;
+                if (grow) {
+                    alpha = ex2(m - mx);               // 0 for the first block
+                    m = mx;
+                }
+                const float neg_m = m == -INFINITY ? 0.f : -m;
+                if (j > s && __any_sync(0xffffffffu, grow)) {
+                    // Rare.  (O holds the product of the block before: the scores of this one say so.)
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 16) {
+                        float o[16];
+                        tc_ld16(o_addr + c, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] *= alpha;
+                        tc_st16(o_addr + c, reinterpret_cast<uint32_t*>(o));
+                    }
+                }
+                float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+                const float2 sl2_2 = make_float2(sl2, sl2), neg_m2 = make_float2(neg_m, neg_m);
+#pragma unroll
+                for (int c = 0; c < BK; c += 32) {
+                    if (c < 64 || whole) {
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 e = fma2(make_float2(y[c + i], y[c + i + 1]), sl2_2, neg_m2);
+                            const float2 p = make_float2(ex2(e.x), ex2(e.y));
+                            sum2[(i >> 1) & 3] = add2(sum2[(i >> 1) & 3], p);
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(p.x, p.y);      // key 2k in the low half, key 2k + 1 in the high half
+                            packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        tc_st16(s_addr + c / 2, packed);
+                    }
+                    if (c == 32) hand_over(0);
+                    if (c == 96) hand_over(1);
+                }
+                l = l * alpha + (((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y)));
+            }
+            // The record: [HD / 4][128] groups of four sums, [128] pairs of maximum and sum.
+            float* rec = records + (int64_t)seg.record * REC;
+            auto put = [&](int c, const float* v) {    // 32 numbers of the row from column c on
+                if (store) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(rec + ((c + i) / 4 * BQ + r) * 4) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            };
+            if (n_blk == 1) {                          // (the even stream's alone)
+                if (s == 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[0], uses0 & 1, abort_flag, status, 7));
+                    if (!ok) return false;
+                    tc_fence_after();
+                    if (busy) {
+                        if (store) *reinterpret_cast<float2*>(rec + BQ * HD + 2 * r) = make_float2(m, l);
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 32) {
+                            float v[32];
+                            tc_ld32_nowait(o_addr + c, reinterpret_cast<uint32_t*>(v));
+                            tc_ld_wait();
+                            put(c, v);
+                            __syncwarp();
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.o_empty[0]);    // (read before the next run's product writes)
+                }
+                ++uses0;
+                return true;
+            }
+            // both streams hold a part of every row: each stream's warps make half of the columns
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[0], uses0 & 1, abort_flag, status, 7) && mbar_wait(&sh.o_full[1], uses1 & 1, abort_flag, status, 7));
+            if (!ok) return false;
+            ++uses0, ++uses1;
+            sh.ml[s][0][r] = m;
+            sh.ml[s][1][r] = l;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.join);
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.join, joins & 1, abort_flag, status, 7));
+            if (!ok) return false;
+            tc_fence_after();
+            if (busy) {
+                const float m0 = sh.ml[0][0][r], m1 = sh.ml[1][0][r], mm = fmaxf(m0, m1);
+                const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - mm), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
+                if (store && s == 0) *reinterpret_cast<float2*>(rec + BQ * HD + 2 * r) = make_float2(mm, sh.ml[0][1][r] * f0 + sh.ml[1][1][r] * f1);
+                constexpr int HALF = HD / 2;
+#pragma unroll 1
+                for (int c = s * HALF; c < (s + 1) * HALF; c += 32) {
+                    float v[32], w[32];
+                    tc_ld32_nowait(lane_base + COL_O + c, reinterpret_cast<uint32_t*>(v));
+                    tc_ld32_nowait(lane_base + COL_O + HD + c, reinterpret_cast<uint32_t*>(w));
+                    tc_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = fmaf(w[i], f1, v[i] * f0);
+                    put(c, v);
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.joined);    // (both streams' warps have read both sums)
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.joined, joins & 1, abort_flag, status, 7));
+            if (!ok) return false;
+            ++joins;
+            if (lane == 0) mbar_arrive(&sh.o_empty[s]);
+            return true;
+        });
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (sh.abort_flag) {
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 2000000ull) __nanosleep(1000);   // copies in flight land before the block leaves
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+    }
+}
+
+}  // namespace tc
+
+bool tc_supported() { return tc::SUPPORTED; }
+
+int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, const Groups& G, int blocks, float scale, int* plan, float* records, int* status,
+              cudaStream_t s) {
+    using namespace tc;
+    WICK_REQUIRE(kv_pages * 2 * G.kv_heads * kPage <= INT32_MAX, "attention (shared prefix): a cache of %lld pages is beyond the copies' coordinates", (long long)kv_pages);
+    CUtensorMap q_map, kv_map;
+    if (int e = make_heads_map(&q_map, q, n_tokens, G.heads, HD, G.gs, BQ / G.gs)) return e;
+    if (int e = make_bf16_map(&kv_map, kv, kv_pages * 2 * G.kv_heads * kPage, HD, kPage, "attention (shared prefix)")) return e;
+    static bool raised = false;
+    if (!raised) {
+        WICK_CUDA(cudaFuncSetAttribute(attn_shared_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+        raised = true;
+    }
+    WICK_CUDA(launch(attn_shared_tc_kernel, dim3(blocks), dim3(THREADS), (size_t)SMEM_BYTES, s, q_map, kv_map, G, kv_pages, scale, plan, records, status));
+    return check_launch("attn_shared_tc");
+}
+
+}  // namespace shared_prefix
+}  // namespace wick

@@ -533,7 +533,7 @@ def attention_decode_parts_fused(qkv: torch.Tensor, n_heads: int, n_kv: int, hea
 
 # ---------------------------------------------------------------------------
 # Attention where groups of a step's sequences share their first pages (csrc/attn_shared.cuh, attn_shared.cu).
-SHARED_SOURCES = ["attn_shared.cu"]
+SHARED_SOURCES = ["attn_shared.cu", "attn_shared_tc.cu"]
 
 
 def _shared(head_dim: int) -> _Lib:
@@ -544,7 +544,7 @@ def _shared(head_dim: int) -> _Lib:
               f"attention kernels take a head_dim that is a multiple of 16 between 16 and 256, not {head_dim}")
         lib = _libs[key] = _Lib(f"wick_shared_hd{head_dim}", SHARED_SOURCES, [f"WICK_HD={head_dim}"])
         lib._lib.wick_attn_shared_scratch.restype = ctypes.c_longlong
-        lib._lib.wick_attn_shared_scratch.argtypes = [ctypes.c_int] * 8
+        lib._lib.wick_attn_shared_scratch.argtypes = [ctypes.c_int] * 9
     return lib
 
 
@@ -575,11 +575,11 @@ class SharedPrefix(NamedTuple):
         return cls(dev[:G + 1], dev[G + 1:2 * G + 1], dev[2 * G + 1:], max(pages, default=0), max(own, default=0))
 
 
-def attention_shared_scratch(shared: SharedPrefix, batch, n_heads: int, n_kv: int, head_dim: int) -> int:
+def attention_shared_scratch(shared: SharedPrefix, batch, n_heads: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> int:
     """float32 words of scratch that :func:`attention_shared` needs for this step."""
     lib = _shared(head_dim)
-    n = lib._lib.wick_attn_shared_scratch(batch.n_tokens, batch.n_seqs, shared.pages.numel(), n_heads, n_kv, shared.max_pages, shared.own_bound,
-                                          batch.max_q_len)
+    n = lib._lib.wick_attn_shared_scratch(dtype == torch.bfloat16, batch.n_tokens, batch.n_seqs, shared.pages.numel(), n_heads, n_kv,
+                                          shared.max_pages, shared.own_bound, batch.max_q_len)
     if n < 0:
         raise KernelError(lib._lib.wick_last_error().decode("utf-8", "replace"))
     return n
@@ -603,7 +603,7 @@ def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPre
     _cuda("pages", pages, torch.int32)
     _cuda("group_of", group_of, torch.int32, (n_seqs,))
     if scratch is None:
-        scratch = torch.empty(attention_shared_scratch(shared, batch, n_heads, kv.shape[2], hd), dtype=torch.float32, device=q.device)
+        scratch = torch.empty(attention_shared_scratch(shared, batch, n_heads, kv.shape[2], hd, q.dtype), dtype=torch.float32, device=q.device)
     else:
         _cuda("scratch", scratch, torch.float32)
     if out is None:
