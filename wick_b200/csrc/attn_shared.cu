@@ -394,36 +394,23 @@ __global__ void __launch_bounds__(THREADS)
 attn_shared_prefix_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, const Groups G, float scale, int* plan, float* records, int* status) {
     extern __shared__ __align__(16) uint8_t smem[];
     Work<T>& w = *reinterpret_cast<Work<T>*>(smem);
-    __shared__ Cum cum;
     __shared__ Rows<T> rows;
     pdl_wait();
     pdl_trigger();                                  // (behind the wait: the next kernel reads what this one reads without a wait of its own)
     q = fresh(q);
-    if (threadIdx.x < 32) make_plan(G, cum.units, cum.items);
-    __syncthreads();
-    const int U = cum.units[G.n];
-    const int S = blocks_used(U, gridDim.x, 1);
-    if (blockIdx.x == 0) {
-        for (int i = threadIdx.x; i <= G.n; i += THREADS) plan[1 + i] = cum.units[i], plan[2 + G.n + i] = cum.items[i];
-        if (threadIdx.x == 0) plan[0] = S;
-    }
-    if ((int)blockIdx.x >= S) return;
-    const int end = run_start(blockIdx.x + 1, U, S);
-    int g = 0;
-    for (int u = run_start(blockIdx.x, U, S); u < end;) {
-        const Segment s = segment_at(G, cum.units, cum.items, g, u, end, blockIdx.x);
-        g = s.g;
-        u += s.to - s.from;
+    Walk walk(G, gridDim.x, blockIdx.x == 0 && threadIdx.x < 32 ? plan : nullptr);
+    Segment s;
+    while (walk.segment(s)) {                       // (every warp walks the same way)
         __syncthreads();                            // (the rows and the work of the segment before)
         if (threadIdx.x < R) {
-            const int tok0 = first_token(G, g), n = first_token(G, g + 1) - tok0, idx = s.tile * R + threadIdx.x;
-            const bool there = idx < n * G.gs;
-            rows.q[threadIdx.x] = there ? q + ((int64_t)(tok0 + idx / G.gs) * G.heads + s.column * G.gs + idx % G.gs) * HD : nullptr;
+            const int idx = s.tile * R + threadIdx.x;
+            const bool there = idx < s.n_tok * G.gs;
+            rows.q[threadIdx.x] = there ? q + ((int64_t)(s.tok0 + idx / G.gs) * G.heads + s.column * G.gs + idx % G.gs) * HD : nullptr;
             rows.last[threadIdx.x] = there ? s.pages * kPage - 1 : -1;
         }
         __syncthreads();
-        attend(w, rows, kv, kv_pages, G.page_table + (int64_t)G.cu_groups[g] * G.table_width, s.column / G.per_kv, G.kv_heads,
-               s.from * G.unit_pages * kPage, min(s.to * G.unit_pages, s.pages) * kPage, scale, status);
+        attend(w, rows, kv, kv_pages, G.page_table + (int64_t)G.cu_groups[s.g] * G.table_width, s.column / G.per_kv, G.kv_heads,
+               s.from * kPage, s.to * kPage, scale, status);
         write_record(w, records + (int64_t)s.record * REC);
     }
 }
@@ -433,7 +420,7 @@ attn_shared_prefix_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages
 struct Shared {
     const int* plan;                               // null: nothing is shared
     const float* records;
-    int rows;                                      // of a record
+    int rows;                                      // that a record has room for
 };
 
 // Row `row` of the tile (token tok, head) joined with the shared part's records: the factors of the own part (M -> its weight) and
@@ -444,17 +431,17 @@ struct Joined {
 __device__ __forceinline__ Joined records_of(const Groups& G, const Shared& sh, int g, int tok, int head, int kvh) {
     Joined j = {0, 0, 0};
     if (!sh.plan) return j;
-    const int pages = pages_of(G, g);
-    if (pages == 0) return j;
+    const Cut c = cut_of(G, g);
+    if (c.pages == 0) return j;
     const int *units = sh.plan + 1, *items = sh.plan + 2 + G.n;
     const int S = __ldcg(sh.plan), U = __ldcg(units + G.n);
-    const int h = head - kvh * (G.heads / G.kv_heads);
-    const int idx = (tok - first_token(G, g)) * G.gs + h % G.gs, item = idx / sh.rows * G.columns + kvh * G.per_kv + h / G.gs;
-    const int per = units_per_item(G, pages), u = __ldcg(units + g) + item * per;
-    const int c0 = block_of(u, U, S), c1 = block_of(u + per - 1, U, S);
-    j.first = __ldcg(items + g) + item + c0;
+    const int h = head - kvh * (G.heads / G.kv_heads), column = kvh * G.per_kv + h / G.gs;
+    const int idx = (tok - c.tok0) * G.gs + h % G.gs, tile = idx / G.rows, pair = tile / G.pair, w = c.width(G, pair);
+    const int u = __ldcg(units + g) + c.before(G, pair, column);
+    const int c0 = block_of(u + w - 1, U, S), c1 = block_of(u + w * c.blocks - 1, U, S);
+    j.first = (__ldcg(items + g) + pair * G.columns + column + c0) * G.pair + tile - pair * G.pair;
     j.n = c1 - c0 + 1;
-    j.r = idx % sh.rows;
+    j.r = idx - tile * G.rows;
     return j;
 }
 
@@ -464,7 +451,7 @@ __device__ __forceinline__ void finish(const Groups& G, const Shared& sh, T* __r
                                        Cols cols) {
     __shared__ Joined parts[R];
     __shared__ float most[R], over[R];
-    const int tid = threadIdx.x, group = G.heads / G.kv_heads, row_floats = sh.rows * (HD + 2);
+    const int tid = threadIdx.x, group = G.heads / G.kv_heads, rec_floats = sh.rows * (HD + 2), step = rec_floats * G.pair;   // (of an item's records)
     auto tok_of = [&](int r) { return tok0 + (row0 + r) / group; };
     auto head_of = [&](int r) { return kvh * group + (row0 + r) % group; };
     {
@@ -476,12 +463,12 @@ __device__ __forceinline__ void finish(const Groups& G, const Shared& sh, T* __r
             j = records_of(G, sh, g, tok_of(r), head_of(r), kvh);
         }
         const float m_own = m, l_own = l;
-        for (int i = k; i < j.n; i += 8) m = fmaxf(m, __ldcg(sh.records + (int64_t)(j.first + i) * row_floats + sh.rows * HD + 2 * j.r));
+        for (int i = k; i < j.n; i += 8) m = fmaxf(m, __ldcg(sh.records + (int64_t)j.first * rec_floats + (int64_t)i * step + sh.rows * HD + 2 * j.r));
 #pragma unroll
         for (int d = 1; d < 8; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         l = k == 0 ? l_own * weight(m_own, m) : 0.f;
         for (int i = k; i < j.n; i += 8) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(sh.records + (int64_t)(j.first + i) * row_floats + sh.rows * HD + 2 * j.r));
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(sh.records + (int64_t)j.first * rec_floats + (int64_t)i * step + sh.rows * HD + 2 * j.r));
             l = fmaf(ml.y, weight(ml.x, m), l);
         }
 #pragma unroll
@@ -494,9 +481,9 @@ __device__ __forceinline__ void finish(const Groups& G, const Shared& sh, T* __r
         const Joined j = parts[r];
         const float m = most[r];
         float4 s = cols(r, c * 4, m);
-        const float* rec = sh.records + (int64_t)j.first * row_floats;
+        const float* rec = sh.records + (int64_t)j.first * rec_floats;
 #pragma unroll 4
-        for (int k = 0; k < j.n; ++k, rec += row_floats) {
+        for (int k = 0; k < j.n; ++k, rec += step) {
             const float4 o = __ldcg(reinterpret_cast<const float4*>(rec + ((int64_t)c * sh.rows + j.r) * 4));
             const float a = weight(__ldcg(rec + sh.rows * HD + 2 * j.r), m);
             s.x = fmaf(o.x, a, s.x), s.y = fmaf(o.y, a, s.y), s.z = fmaf(o.z, a, s.z), s.w = fmaf(o.w, a, s.w);
@@ -627,11 +614,13 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
     c.G.n = n_groups, c.G.n_seqs = n_seqs, c.G.max_pages = max_pages, c.G.heads = heads, c.G.kv_heads = kv_heads;
     c.tc = half && tc_supported();
     if (c.tc) {
-        int gs = 1;                                // heads of a tile: as many as fill its rows with whole tokens
-        while (group % (2 * gs) == 0 && 2 * gs <= TC_ROWS) gs *= 2;
-        c.G.rows = TC_ROWS, c.G.gs = gs, c.G.per_kv = group / gs, c.G.columns = heads / gs, c.G.unit_pages = 2;
+        // heads of a tile: all of a key head's, or as many as 128 rows hold of more
+        int gs = group;
+        for (int n = 2; gs > TC_ROWS; ++n)
+            if (group % n == 0) gs = group / n;
+        c.G.rows = TC_ROWS / gs * gs, c.G.gs = gs, c.G.per_kv = group / gs, c.G.columns = heads / gs, c.G.block = 2, c.G.pair = 2;
     } else {
-        c.G.rows = R, c.G.gs = group, c.G.per_kv = 1, c.G.columns = kv_heads, c.G.unit_pages = 1;
+        c.G.rows = R, c.G.gs = group, c.G.per_kv = 1, c.G.columns = kv_heads, c.G.block = 1, c.G.pair = 1;
     }
     c.tiles_own = ceil_div((int64_t)max_q_len * group, R);
     WICK_REQUIRE((int64_t)c.tiles_own * kv_heads <= INT32_MAX / 2, "attention (shared prefix): %d tokens of one sequence are too many", max_q_len);
@@ -639,7 +628,7 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
     c.blocks = (c.tc ? 1 : PER_SM) * sm_count();
     c.plan_words = max_pages > 0 ? (2 * (n_groups + 1) + 1 + 3) / 4 * 4 : 0;
     const int64_t tiles = ceil_div((int64_t)n_tokens * c.G.gs, c.G.rows) + n_groups;
-    c.prefix_floats = max_pages > 0 ? (tiles * c.G.columns + c.blocks) * c.G.rows * (HD + 2) : 0;
+    c.prefix_floats = max_pages > 0 ? ((tiles / c.G.pair + n_groups) * c.G.columns + c.blocks) * c.G.pair * (c.tc ? TC_ROWS : R) * (HD + 2) : 0;
     c.own_floats = c.splits > 1 ? (int64_t)n_seqs * c.tiles_own * kv_heads * c.splits * REC : 0;
     return 0;
 }
@@ -668,7 +657,7 @@ static int attn_shared(const void* q, int n_tokens, const void* kv, int64_t kv_p
         WICK_CUDA(cudaFuncSetAttribute(attn_shared_own_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         raised = true;
     }
-    Shared sh = {nullptr, records, G.rows};
+    Shared sh = {nullptr, records, c.tc ? TC_ROWS : R};
     if (max_pages > 0) sh.plan = plan;
     if (max_pages > 0 && c.tc) {
         if (int e = launch_tc(q, n_tokens, kv, kv_pages, G, c.blocks, scale, plan, records, status, s)) return e;

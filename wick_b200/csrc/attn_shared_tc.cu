@@ -2,9 +2,12 @@
 // (maximum, sum of weights, weighted sum of values) for every run of units of a tile of 128 rows (attn_shared.cuh).
 //
 // A tile's rows are query heads of one key head times the group's tokens, whatever sequences they belong to: all of them see all
-// shared keys, so there is no mask anywhere.  A unit is a block of 128 keys (two pages; the last one of an odd number is half).  Even
-// blocks go to one stream, odd ones to another, each with its own scores and its own sums in tensor memory and four softmax warps, so
-// that one stream's softmax runs beside the other's products; they are joined when a run ends.
+// shared keys, so there is no mask anywhere.  A block of keys is two pages (the last one of an odd number: one).  There are two streams, each
+// with its own scores and its own sums in tensor memory and four softmax warps, so that one stream's softmax runs beside the other's
+// products:
+//   * a group of more than 128 rows: two tiles of rows, a stream each, that share every tile of keys and values;
+//   * the last tile of an odd number: even blocks of keys go to one stream, odd ones to the other, joined when the run ends.
+// Roles:
 //   * a producer warp fetches the query rows of a run and its key and value tiles through a ring (TMA, 128-byte swizzle);
 //   * an issuing warp alternates between the streams: O += P V of one, then the scores S = Q K^T of its next block (P lies over the
 //     scores it came from, as bfloat16 pairs);
@@ -28,7 +31,7 @@ constexpr int HD = SUPPORTED ? WICK_HD : 64;           // other head sizes: neve
 constexpr int BQ = TC_ROWS, BK = 128;
 constexpr int PANELS = HD / 64;                        // 64-column panels of a head row
 constexpr int PANEL_BYTES = 128 * 128;                 // 128 rows of 128 bytes
-constexpr int TILE_BYTES = PANELS * PANEL_BYTES;       // the tile of queries, or one block of keys or of values
+constexpr int TILE_BYTES = PANELS * PANEL_BYTES;       // a tile of queries, or one block of keys or of values
 constexpr int NSLOT = 5;                               // key / value tiles in flight
 constexpr int THREADS = 320;                           // warp 0: TMA, warp 1: MMA + tensor memory, warps 2-5 and 6-9: softmax
 constexpr uint32_t TMEM_COLS = 512;                    // S of both streams | O of both
@@ -39,11 +42,10 @@ constexpr int REC = BQ * (HD + 2);
 struct Smem {
     float ml[2][2][BQ];                                // the streams' maxima and sums
     uint64_t q_full, q_empty, full[NSLOT], empty[NSLOT], s_full[2], p_full[2][2], o_full[2], o_empty[2], join, joined;
-    Cum cum;
     uint32_t tmem_slot;
     int abort_flag;
 };
-constexpr int SMEM_BYTES = (1 + NSLOT) * TILE_BYTES + (int)sizeof(Smem);
+constexpr int SMEM_BYTES = (2 + NSLOT) * TILE_BYTES + (int)sizeof(Smem);
 static_assert(SMEM_BYTES <= 227 * 1024, "a block's shared memory");
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -51,7 +53,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                       int* plan, float* records, int* status) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* q_s = smem_raw;
-    uint8_t* kv_s = q_s + TILE_BYTES;
+    uint8_t* kv_s = q_s + 2 * TILE_BYTES;
     Smem& sh = *reinterpret_cast<Smem*>(kv_s + NSLOT * TILE_BYTES);
     volatile int* abort_flag = &sh.abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -78,42 +80,32 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     }
     pdl_wait();
     pdl_trigger();                                     // (behind the wait: the next kernel reads what this one reads without a wait of its own)
-    if (warp == 2) make_plan(G, sh.cum.units, sh.cum.items);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem_slot;
-    const int U = sh.cum.units[G.n], S = blocks_used(U, gridDim.x, 1), cta = blockIdx.x;
-    if (cta == 0) {
-        for (int i = threadIdx.x; i <= G.n; i += THREADS) plan[1 + i] = sh.cum.units[i], plan[2 + G.n + i] = sh.cum.items[i];
-        if (threadIdx.x == 0) plan[0] = S;
-    }
-    const int u_begin = cta < S && U > 0 ? run_start(cta, U, S) : 0, u_end = cta < S && U > 0 ? run_start(cta + 1, U, S) : 0;
     const bool aligned = (smem_u32(smem_raw) & 1023) == 0;   // (always: the block's dynamic shared memory is all there is)
     if (!aligned && threadIdx.x == 0) atomicCAS(status, 0, 7);
-    // Walks the block's runs: body(segment, its number, units).  Every role walks on its own.
-    auto each = [&](auto body) {
-        int g = 0, k = 0;
-        for (int u = u_begin; aligned && u < u_end; ++k) {
-            const Segment s = segment_at(G, sh.cum.units, sh.cum.items, g, u, u_end, cta);
-            g = s.g;
-            u += s.to - s.from;
-            if (!body(s, k, s.to - s.from)) break;
-        }
-    };
-    // the block of keys that is half: the last one of an odd number of pages
+    Walk walk(G, gridDim.x, blockIdx.x == 0 && warp == 2 ? plan : nullptr);   // (every warp walks on its own)
+    // the block of keys that is one page: the last one of an odd number
     auto half = [&](const Segment& s, int j) { return 2 * (s.from + j) + 1 == s.pages; };
+    Segment seg;
+    int k = 0;                                         // segments so far
+    bool ok = aligned;
 
     if (warp == 0) {
         // ---------------- producer ----------------
         const bool one = elect_one();
         int slot = 0, turn = 0;                        // of the ring
-        each([&](const Segment& s, int k, int n_blk) {
-            const int* table = G.page_table + (int64_t)G.cu_groups[s.g] * G.table_width;
+#pragma unroll 1
+        for (; ok && walk.segment(seg); ++k) {
+            const int n = seg.to - seg.from;
+            const bool split = seg.tiles == 1;
+            const int* table = G.page_table + (int64_t)G.cu_groups[seg.g] * G.table_width;
             // A lane holds a page number of each of two runs of 32, read ahead.
             auto pages = [&](int run) {
-                const int at = 2 * s.from + run * 32 + lane;
-                int page = at < s.pages ? table[at] : 0;
+                const int at = 2 * seg.from + run * 32 + lane;
+                int page = at < seg.pages ? table[at] : 0;
                 if (page < 0 || page >= kv_pages) {
                     atomicCAS(status, 0, 10);
                     page = 0;
@@ -121,19 +113,25 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                 return page;
             };
             int even = pages(0), odd = pages(1);
-            if (k > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.q_empty, (k - 1) & 1, abort_flag, status, 7))) return false;
+            if (k > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty, (k - 1) & 1, abort_flag, status, 7));
+            if (!ok) break;
             if (one) {
-                mbar_expect_tx(&sh.q_full, TILE_BYTES);
-                for (int pn = 0; pn < PANELS; ++pn)
-                    tma_load_3d(&q_map, &sh.q_full, q_s + pn * PANEL_BYTES, pn * 64, s.column * G.gs, first_token(G, s.g) + s.tile * (BQ / G.gs));
+                mbar_expect_tx(&sh.q_full, seg.tiles * PANELS * G.rows * 128);
+                for (int i = 0; i < seg.tiles; ++i)
+                    for (int pn = 0; pn < PANELS; ++pn)
+                        tma_load_3d(&q_map, &sh.q_full, q_s + i * TILE_BYTES + pn * PANEL_BYTES, pn * 64, seg.column * G.gs,
+                                    seg.tok0 + (seg.tile + i) * (G.rows / G.gs));
             }
-            // K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1): the order in which the issuing warp uses them
+            // K0 V0 K1 V1 .., or, split, K0 K1 V0 K2 V1 K3 .. V(n-2) V(n-1): the order in which the issuing warp uses them
 #pragma unroll 1
-            for (int i = 0; i < 2 * n_blk; ++i) {
-                const bool last = i == 2 * n_blk - 1;
-                const int is_v = last || (i > 0 && !(i & 1));
-                const int j = last ? n_blk - 1 : (is_v ? (i - 2) >> 1 : (i + 1) >> 1);
-                if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.empty[slot], (turn - 1) & 1, abort_flag, status, 7))) return false;
+            for (int i = 0; i < 2 * n; ++i) {
+                const bool last = split && i == 2 * n - 1;
+                const int is_v = split ? (last || (i > 0 && !(i & 1))) : (i & 1);
+                const int j = last ? n - 1 : (split ? (is_v ? (i - 2) >> 1 : (i + 1) >> 1) : i >> 1);
+                if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.empty[slot], (turn - 1) & 1, abort_flag, status, 7))) {
+                    ok = false;
+                    break;
+                }
                 const int held = (2 * j >> 5) & 1 ? odd : even;
                 const int page0 = __shfl_sync(0xffffffffu, held, 2 * j & 31), page1 = __shfl_sync(0xffffffffu, held, (2 * j + 1) & 31);
                 if (is_v && j >= 16 && (j & 15) == 0) {            // (keys and values have left the run before)
@@ -141,51 +139,53 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                     else odd = pages((j >> 4) + 1);
                 }
                 if (one) {
-                    const int n_pages = half(s, j) ? 1 : 2;
+                    const int n_pages = half(seg, j) ? 1 : 2;
                     mbar_expect_tx(&sh.full[slot], n_pages * (TILE_BYTES / 2));
                     uint8_t* dst = kv_s + slot * TILE_BYTES;
 #pragma unroll 1
                     for (int h = 0; h < n_pages; ++h)
                         for (int pn = 0; pn < PANELS; ++pn)
                             tma_load_2d(&kv_map, &sh.full[slot], dst + pn * PANEL_BYTES + h * (kPage * 128), pn * 64,
-                                        (((h ? page1 : page0) * 2 + is_v) * G.kv_heads + s.column / G.per_kv) * kPage);
+                                        (((h ? page1 : page0) * 2 + is_v) * G.kv_heads + seg.column / G.per_kv) * kPage);
                 }
                 if (++slot == NSLOT) slot = 0, ++turn;
                 __syncwarp();
             }
-            return true;
-        });
+        }
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         // (the whole warp walks through the steps, one elected lane issues)
         const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BK >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
         const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-        const uint32_t q_lo = desc_lo(smem_u32(q_s), 16), k_lo0 = desc_lo(smem_u32(kv_s), 16), v_lo0 = desc_lo(smem_u32(kv_s), PANEL_BYTES);
+        const uint32_t q_lo0 = desc_lo(smem_u32(q_s), 16), k_lo0 = desc_lo(smem_u32(kv_s), 16), v_lo0 = desc_lo(smem_u32(kv_s), PANEL_BYTES);
         const bool one = elect_one();
         int slot = 0, round = 0;                       // of the ring
         int steps0 = 0, steps1 = 0, uses0 = 0, uses1 = 0;          // blocks and runs of each stream so far
-        bool ok = true;
+        int k_at = 0, v_at = 0;                        // where the keys and values at hand lie
         auto take = [&](int& at) {                     // the next tile of the ring, when it has come
             at = slot;
             const bool here = __all_sync(0xffffffffu, mbar_wait(&sh.full[slot], round & 1, abort_flag, status, 7));
             if (++slot == NSLOT) slot = 0, ++round;
             return here;
         };
-        each([&](const Segment& seg, int k, int n_blk) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, k & 1, abort_flag, status, 7));
-            // turn t of stream s: the product of its block t, the scores of its block t + 1
 #pragma unroll 1
-            for (int i = -2; ok && i < n_blk; ++i) {
-                const int s = i & 1, t = i >> 1;
-                const bool more = i + 2 < n_blk;
-                if (t >= 0) {
+        for (; ok && walk.segment(seg); ++k) {
+            const int n = seg.to - seg.from;
+            const bool split = seg.tiles == 1;
+            const int N = split ? n : 2 * n;           // turns
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, k & 1, abort_flag, status, 7));
+            // turn i: stream i & 1's product of one block, then its scores of the next
+#pragma unroll 1
+            for (int i = -2; ok && i < N; ++i) {
+                const int s = i & 1;
+                const bool more = i + 2 < N;
+                if (i >= 0) {
                     const int steps = s == 0 ? steps0 : steps1, uses = s == 0 ? uses0 : uses1;
-                    int at;
-                    ok = take(at);
+                    if (split || s == 0) ok = take(v_at);
                     // (the sums of the stream's run before have been read)
-                    if (ok && t == 0 && uses > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_empty[s], (uses - 1) & 1, abort_flag, status, 7));
-                    const uint32_t v_lo = v_lo0 + at * (TILE_BYTES >> 4), d = tmem + COL_O + s * HD, pa = tmem + COL_S + s * BK;
-                    const int parts = half(seg, i) ? 1 : 2;
+                    if (ok && i < 2 && uses > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_empty[s], (uses - 1) & 1, abort_flag, status, 7));
+                    const uint32_t v_lo = v_lo0 + v_at * (TILE_BYTES >> 4), d = tmem + COL_O + s * HD, pa = tmem + COL_S + s * BK;
+                    const int parts = half(seg, split ? i : i >> 1) ? 1 : 2;
 #pragma unroll
                     for (int part = 0; part < 2; ++part) {
                         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[s][part], steps & 1, abort_flag, status, 7));
@@ -193,38 +193,36 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                         tc_fence_after();
                         const uint32_t pp = pa + part * (P_FIRST / 2), vp = v_lo + part * (P_FIRST / 16) * (2048 >> 4);
                         if (one && part < parts) {
-                            mma_ts(d, pp, vp, idesc_o, t > 0 || part > 0);
+                            mma_ts(d, pp, vp, idesc_o, i >= 2 || part > 0);
                             static_for<1, P_FIRST / 16>([&](auto ks) { mma_ts(d, pp + (int)ks * 8, vp + (int)ks * (2048 >> 4), idesc_o, 1); });
                         }
                     }
                     if (!ok) break;
                     if (one) {
-                        tc_commit(&sh.empty[at]);
+                        if (split || s == 1) tc_commit(&sh.empty[v_at]);       // a tile is free behind its last reader
                         if (!more) tc_commit(&sh.o_full[s]);
                     }
                     if (s == 0) ++steps0, uses0 += more ? 0 : 1;
                     else ++steps1, uses1 += more ? 0 : 1;
                 }
                 if (more) {
-                    int at;
-                    ok = take(at);
+                    if (split || s == 0) ok = take(k_at);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t k_lo = k_lo0 + at * (TILE_BYTES >> 4), d = tmem + COL_S + s * BK;
+                    const uint32_t k_lo = k_lo0 + k_at * (TILE_BYTES >> 4), q_lo = q_lo0 + (split ? 0 : s * (TILE_BYTES >> 4)), d = tmem + COL_S + s * BK;
                     if (one) {
                         static_for<0, HD / 16>([&](auto ks) {
                             constexpr uint32_t off = (((int)ks >> 2) * PANEL_BYTES + ((int)ks & 3) * 32) >> 4;
                             mma_ss<((int)ks > 0)>(d, q_lo + off, k_lo + off, idesc_s);
                         });
                         tc_commit(&sh.s_full[s]);
-                        tc_commit(&sh.empty[at]);
-                        if (i + 2 == n_blk - 1) tc_commit(&sh.q_empty);        // (the run's last scores)
+                        if (split || s == 1) tc_commit(&sh.empty[k_at]);
+                        if (i + 2 == N - 1) tc_commit(&sh.q_empty);            // (the run's last scores)
                     }
                 }
                 __syncwarp();
             }
-            return ok;
-        });
+        }
     } else {
         // ---------------- softmax: a row per thread ----------------
         // (a warp reads the 32 lanes of tensor memory given by its index modulo 4)
@@ -233,15 +231,18 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const float sl2 = scale * 1.4426950408889634f;
         const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
         const uint32_t s_addr = lane_base + COL_S + s * BK, o_addr = lane_base + COL_O + s * HD;
-        int step = 0, uses0 = 0, uses1 = 0, joins = 0;  // this stream's blocks, both streams' runs, joins so far
-        bool ok = true;
-        each([&](const Segment& seg, int, int n_blk) {
-            const int n_rows = (first_token(G, seg.g + 1) - first_token(G, seg.g)) * G.gs - seg.tile * BQ;   // (of the tile and behind it)
+        int step = 0, uses0 = 0, uses1 = 0, joins = 0; // this stream's blocks, both streams' runs, joins so far
+#pragma unroll 1
+        for (; ok && walk.segment(seg); ++k) {
+            const int n = seg.to - seg.from;
+            const bool split = seg.tiles == 1;
+            const int tile = seg.tile + (split ? 0 : s), n_rows = min(G.rows, seg.n_tok * G.gs - tile * G.rows);
             const bool store = r < n_rows, busy = quad * 32 < n_rows;
             float m = -INFINITY, l = 0.f;              // what O and the sum are scaled by (it follows the maximum lazily), the sum
-            for (int j = s; j < n_blk; j += 2) {
+#pragma unroll 1
+            for (int j = split ? s : 0, first = 1; j < n; j += split ? 2 : 1, first = 0) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s], step & 1, abort_flag, status, 7));
-                if (!ok) return false;
+                if (!ok) break;
                 ++step;
                 tc_fence_after();
                 auto hand_over = [&](int part) {
@@ -277,7 +278,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                     m = mx;
                 }
                 const float neg_m = m == -INFINITY ? 0.f : -m;
-                if (j > s && __any_sync(0xffffffffu, grow)) {
+                if (!first && __any_sync(0xffffffffu, grow)) {
                     // Rare.  (O holds the product of the block before: the scores of this one say so.)
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 16) {
@@ -309,18 +310,20 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                 }
                 l = l * alpha + (((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y)));
             }
+            if (!ok) break;
             // The record: [HD / 4][128] groups of four sums, [128] pairs of maximum and sum.
-            float* rec = records + (int64_t)seg.record * REC;
+            float* rec = records + (int64_t)(seg.record + tile - seg.tile) * REC;
             auto put = [&](int c, const float* v) {    // 32 numbers of the row from column c on
                 if (store) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(rec + ((c + i) / 4 * BQ + r) * 4) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                 }
             };
-            if (n_blk == 1) {                          // (the even stream's alone)
-                if (s == 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[0], uses0 & 1, abort_flag, status, 7));
-                    if (!ok) return false;
+            if (!split || n == 1) {
+                // the row is the stream's own (of one block: the even stream's)
+                if (!split || s == 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[s], (s == 0 ? uses0 : uses1) & 1, abort_flag, status, 7));
+                    if (!ok) break;
                     tc_fence_after();
                     if (busy) {
                         if (store) *reinterpret_cast<float2*>(rec + BQ * HD + 2 * r) = make_float2(m, l);
@@ -335,21 +338,21 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.o_empty[0]);    // (read before the next run's product writes)
+                    if (lane == 0) mbar_arrive(&sh.o_empty[s]);    // (read before the next run's product writes)
                 }
-                ++uses0;
-                return true;
+                ++uses0, uses1 += split ? 0 : 1;
+                continue;
             }
             // both streams hold a part of every row: each stream's warps make half of the columns
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[0], uses0 & 1, abort_flag, status, 7) && mbar_wait(&sh.o_full[1], uses1 & 1, abort_flag, status, 7));
-            if (!ok) return false;
+            if (!ok) break;
             ++uses0, ++uses1;
             sh.ml[s][0][r] = m;
             sh.ml[s][1][r] = l;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.join);
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.join, joins & 1, abort_flag, status, 7));
-            if (!ok) return false;
+            if (!ok) break;
             tc_fence_after();
             if (busy) {
                 const float m0 = sh.ml[0][0][r], m1 = sh.ml[1][0][r], mm = fmaxf(m0, m1);
@@ -372,11 +375,10 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.joined);    // (both streams' warps have read both sums)
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.joined, joins & 1, abort_flag, status, 7));
-            if (!ok) return false;
+            if (!ok) break;
             ++joins;
             if (lane == 0) mbar_arrive(&sh.o_empty[s]);
-            return true;
-        });
+        }
     }
 
     tc_fence_before();
@@ -401,7 +403,7 @@ int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, con
     using namespace tc;
     WICK_REQUIRE(kv_pages * 2 * G.kv_heads * kPage <= INT32_MAX, "attention (shared prefix): a cache of %lld pages is beyond the copies' coordinates", (long long)kv_pages);
     CUtensorMap q_map, kv_map;
-    if (int e = make_heads_map(&q_map, q, n_tokens, G.heads, HD, G.gs, BQ / G.gs)) return e;
+    if (int e = make_heads_map(&q_map, q, n_tokens, G.heads, HD, G.gs, G.rows / G.gs)) return e;
     if (int e = make_bf16_map(&kv_map, kv, kv_pages * 2 * G.kv_heads * kPage, HD, kPage, "attention (shared prefix)")) return e;
     static bool raised = false;
     if (!raised) {
