@@ -1,12 +1,10 @@
 // Attention over a prefix that groups of sequences share, and over each sequence's own keys behind it (attn_shared.cuh has the
-// mathematics and how the shared part is cut).
+// mathematics and how the work is cut): the entry points, and the form for any head size in float32, and in bfloat16 for head sizes
+// other than 64 and 128 (those: attn_shared_tc.cu, attn_shared_own.cu).
 //
-//   1. the shared keys: attn_shared_prefix_kernel here (any head size, bfloat16 and float32, tiles of 16 rows), or the tcgen05 kernel
-//      of attn_shared_tc.cu (bfloat16, head sizes 64 and 128, tiles of 128 rows); a record (m, l, o) per run of units;
-//   2. attn_shared_own_kernel: a block per sequence, key head and 16 rows (and part of the own keys, where they are many): the
-//      own keys, then all parts joined and written.  It starts while the first kernel's last blocks run and waits for them only
-//      before it joins;
-//   3. where a sequence's own keys are cut into parts: attn_shared_join_kernel.
+//   1. attn_shared_part_kernel over the groups' shared keys, then over the sequences' own ones: tiles of 16 rows, a record (m, l, o) per
+//      run of units;
+//   2. attn_shared_join_kernel: a row's records joined and written.
 //
 // bfloat16: mma.sync on tiles of 16 rows and 16 keys.  Keys and values go from the cache straight to registers: the inner index of
 // q . k is summed over in any order, so a lane takes 16 neighbouring bytes of a key row and the same of its query row as operands of
@@ -28,19 +26,9 @@ constexpr int HD = WICK_HD;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head_dim must be a multiple of 16 in [16, 256]");
 typedef __nv_bfloat16 bf16;
 
-constexpr int R = 16;                              // rows of a tile
+constexpr int R = OWN_ROWS;                        // rows of a tile
 constexpr int W = 4, THREADS = W * 32;
 constexpr int REC = R * (HD + 2);                  // floats of a tile's record: [HD / 4][R][4] sums, [R][2] maximum and sum of weights
-constexpr int SPLIT = 512;                         // own keys from which on a sequence is cut
-constexpr int MAX_SPLITS = 16;
-constexpr float LOG2E = 1.4426950408889634f;
-
-__host__ __device__ inline int own_splits(int n) { return n <= SPLIT ? 1 : min(MAX_SPLITS, (n + SPLIT - 1) / SPLIT); }
-__host__ __device__ inline int split_keys(int n, int splits) { return ((n + 63) / 64 + splits - 1) / splits * 64; }
-
-// 2^(a - b) for maxima that may be -inf (nothing seen): then the weight is 0.
-__device__ __forceinline__ float weight(float a, float b) { return a == -INFINITY ? 0.f : exp2f(a - b); }
-
 // A block's 16 rows, as the cores leave them: in PARTS parts.
 template <typename T> struct Work;
 template <> struct Work<bf16> {
@@ -388,204 +376,113 @@ template <typename T> __device__ __forceinline__ void write_record(const Work<T>
     }
 }
 
-// ---- 1. the shared keys --------------------------------------------------------
-template <typename T>
+// ---- the parts ---------------------------------------------------------------------
+// wait_first: whether something before this kernel may still run that it reads the results of (the own parts' kernel comes behind the
+// shared ones', which has waited for q and the cache).
+template <typename T, typename Parts>
 __global__ void __launch_bounds__(THREADS)
-attn_shared_prefix_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, const Groups G, float scale, int* plan, float* records, int* status) {
+attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, T* __restrict__ out, const Groups G, const Parts parts, int wait_first,
+                        float scale, int* plan, float* records, int* status) {
     extern __shared__ __align__(16) uint8_t smem[];
     Work<T>& w = *reinterpret_cast<Work<T>*>(smem);
     __shared__ Rows<T> rows;
-    pdl_wait();
-    pdl_trigger();                                  // (behind the wait: the next kernel reads what this one reads without a wait of its own)
+    constexpr bool OWN = Parts::OWN;
+    if (wait_first) pdl_wait();
+    pdl_trigger();                                  // (behind the wait, so that the next kernel need not wait for what this one waited for)
     q = fresh(q);
-    Walk walk(G, gridDim.x, blockIdx.x == 0 && threadIdx.x < 32 ? plan : nullptr);
+    const int gs = OWN ? G.heads / G.kv_heads : G.gs;
+    Walk<Parts> walk(parts, gridDim.x, nullptr);
     Segment s;
     while (walk.segment(s)) {                       // (every warp walks the same way)
         __syncthreads();                            // (the rows and the work of the segment before)
         if (threadIdx.x < R) {
-            const int idx = s.tile * R + threadIdx.x;
-            const bool there = idx < s.n_tok * G.gs;
-            rows.q[threadIdx.x] = there ? q + ((int64_t)(s.tok0 + idx / G.gs) * G.heads + s.column * G.gs + idx % G.gs) * HD : nullptr;
-            rows.last[threadIdx.x] = there ? s.pages * kPage - 1 : -1;
+            const int idx = s.tile * R + threadIdx.x, tok = idx / gs;
+            const bool there = idx < s.cut.n_tok * gs;
+            rows.q[threadIdx.x] = there ? q + ((int64_t)(s.cut.tok0 + tok) * G.heads + s.column * gs + idx - tok * gs) * HD : nullptr;
+            rows.last[threadIdx.x] = !there ? -1 : (OWN ? s.cut.end - s.cut.n_tok + tok : s.cut.end - 1);
         }
         __syncthreads();
-        attend(w, rows, kv, kv_pages, G.page_table + (int64_t)G.cu_groups[s.g] * G.table_width, s.column / G.per_kv, G.kv_heads,
-               s.from * kPage, s.to * kPage, scale, status);
+        attend(w, rows, kv, kv_pages, G.page_table + (int64_t)s.cut.seq * G.table_width, s.column / (OWN ? 1 : G.per_kv), G.kv_heads,
+               (s.cut.first + s.from) * kPage, min((s.cut.first + s.to) * kPage, s.cut.end), scale, status);
         write_record(w, records + (int64_t)s.record * REC);
     }
-}
-
-// ---- 2. the own keys, and all parts joined -----------------------------------------
-// What the records of the shared part look like.
-struct Shared {
-    const int* plan;                               // null: nothing is shared
-    const float* records;
-    int rows;                                      // that a record has room for
-};
-
-// Row `row` of the tile (token tok, head) joined with the shared part's records: the factors of the own part (M -> its weight) and
-// of each record are left in f[0] and f[1 ..].  Called by the 8 lanes that share a row; n_seg records from `rec` on, at place r.
-struct Joined {
-    int first, n, r;                               // records, the row's place in them
-};
-__device__ __forceinline__ Joined records_of(const Groups& G, const Shared& sh, int g, int tok, int head, int kvh) {
-    Joined j = {0, 0, 0};
-    if (!sh.plan) return j;
-    const Cut c = cut_of(G, g);
-    if (c.pages == 0) return j;
-    const int *units = sh.plan + 1, *items = sh.plan + 2 + G.n;
-    const int S = __ldcg(sh.plan), U = __ldcg(units + G.n);
-    const int h = head - kvh * (G.heads / G.kv_heads), column = kvh * G.per_kv + h / G.gs;
-    const int idx = (tok - c.tok0) * G.gs + h % G.gs, tile = idx / G.rows, pair = tile / G.pair, w = c.width(G, pair);
-    const int u = __ldcg(units + g) + c.before(G, pair, column);
-    const int c0 = block_of(u + w - 1, U, S), c1 = block_of(u + w * c.blocks - 1, U, S);
-    j.first = (__ldcg(items + g) + pair * G.columns + column + c0) * G.pair + tile - pair * G.pair;
-    j.n = c1 - c0 + 1;
-    j.r = idx - tile * G.rows;
-    return j;
-}
-
-// The 16 rows of a tile written: own(r, m, l) gives the own part's maximum and sum, cols(r, c, m) its columns.
-template <typename T, typename Own, typename Cols>
-__device__ __forceinline__ void finish(const Groups& G, const Shared& sh, T* __restrict__ out, int g, int tok0, int row0, int n_rows, int kvh, Own own,
-                                       Cols cols) {
-    __shared__ Joined parts[R];
-    __shared__ float most[R], over[R];
-    const int tid = threadIdx.x, group = G.heads / G.kv_heads, rec_floats = sh.rows * (HD + 2), step = rec_floats * G.pair;   // (of an item's records)
-    auto tok_of = [&](int r) { return tok0 + (row0 + r) / group; };
-    auto head_of = [&](int r) { return kvh * group + (row0 + r) % group; };
-    {
-        const int r = tid / 8, k = tid % 8;        // 8 lanes a row
-        Joined j = {0, 0, 0};
-        float m = -INFINITY, l = 0.f;
-        if (r < n_rows) {
-            own(r, m, l);
-            j = records_of(G, sh, g, tok_of(r), head_of(r), kvh);
-        }
-        const float m_own = m, l_own = l;
-        for (int i = k; i < j.n; i += 8) m = fmaxf(m, __ldcg(sh.records + (int64_t)j.first * rec_floats + (int64_t)i * step + sh.rows * HD + 2 * j.r));
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        l = k == 0 ? l_own * weight(m_own, m) : 0.f;
-        for (int i = k; i < j.n; i += 8) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(sh.records + (int64_t)j.first * rec_floats + (int64_t)i * step + sh.rows * HD + 2 * j.r));
-            l = fmaf(ml.y, weight(ml.x, m), l);
-        }
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-        if (k == 0) parts[r] = j, most[r] = m, over[r] = l != 0.f ? __fdiv_rn(1.0f, l) : 0.f;     // (a sum that is no number shows)
-    }
-    __syncthreads();
-    for (int i = tid; i < n_rows * (HD / 4); i += THREADS) {
-        const int r = i % n_rows, c = i / n_rows;
-        const Joined j = parts[r];
-        const float m = most[r];
-        float4 s = cols(r, c * 4, m);
-        const float* rec = sh.records + (int64_t)j.first * rec_floats;
-#pragma unroll 4
-        for (int k = 0; k < j.n; ++k, rec += step) {
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(rec + ((int64_t)c * sh.rows + j.r) * 4));
-            const float a = weight(__ldcg(rec + sh.rows * HD + 2 * j.r), m);
-            s.x = fmaf(o.x, a, s.x), s.y = fmaf(o.y, a, s.y), s.z = fmaf(o.z, a, s.z), s.w = fmaf(o.w, a, s.w);
-        }
-        const float f = over[r];
-        st4(out + ((int64_t)tok_of(r) * G.heads + head_of(r)) * HD + c * 4, s.x * f, s.y * f, s.z * f, s.w * f);
-    }
-}
-
-// The own keys of sequence b: their first position and the end, or -1 (with a report) where the description cannot be.
-__device__ __forceinline__ int2 own_keys(const Groups& G, int b, int q_len, int* status) {
-    const int g = G.group_of[b];
-    const int begin = g >= 0 && g < G.n ? pages_of(G, g) * kPage : 0, end = G.start[b] + q_len;
-    if (g < 0 || g >= G.n || G.start[b] < begin || (end + kPage - 1) / kPage > G.table_width) {
-        if (threadIdx.x == 0) atomicCAS(status, 0, 11);
-        return make_int2(-1, -1);
-    }
-    return make_int2(begin, end);
-}
-
-// Blocks (key head and tile of rows, sequence, part of the own keys).
-template <typename T>
-__global__ void __launch_bounds__(THREADS)
-attn_shared_own_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, T* __restrict__ out, const Groups G, const Shared sh, float scale,
-                       float* own_records, int* status) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    Work<T>& w = *reinterpret_cast<Work<T>*>(smem);
-    __shared__ Rows<T> rows;
-    // (With a shared part the kernel before this one is the one that computes it, and has waited for q and the cache.)
-    if (!sh.plan) pdl_wait();
-    pdl_trigger();
-    q = fresh(q);
-    const int b = blockIdx.y, kvh = blockIdx.x % G.kv_heads, row0 = blockIdx.x / G.kv_heads * R;
-    const int tok0 = G.cu_seqlens[b], q_len = G.cu_seqlens[b + 1] - tok0, group = G.heads / G.kv_heads;
-    const int n_rows = min(R, q_len * group - row0);
-    if (n_rows <= 0) {
-        pdl_wait();                                 // (whoever waits for this kernel waits for the one before it too)
-        return;
-    }
-    const int2 keys = own_keys(G, b, q_len, status);
-    const int n = keys.y - keys.x, splits = min(own_splits(n), (int)gridDim.z), per = split_keys(n, splits);
-    const int key0 = keys.x + (int)blockIdx.z * per, key1 = min(keys.y, key0 + per);
-    if ((int)blockIdx.z >= splits || keys.x < 0) {
+    if (blockIdx.x == 0) {
         pdl_wait();
-        if (keys.x < 0 && blockIdx.z == 0)
-            for (int i = threadIdx.x; i < n_rows * HD; i += THREADS)
-                st(out + ((int64_t)(tok0 + (row0 + i / HD) / group) * G.heads + kvh * group + (row0 + i / HD) % group) * HD + i % HD, 0.f);
-        return;
+        if (threadIdx.x < 32) Walk<Parts>(parts, gridDim.x, plan);
+        if (OWN)
+            for (int b = 0; b < G.n_seqs; ++b) {    // rows of sequences that do not fit are zeros
+                const Cut c = parts(b);
+                if (c.pages > 0 || c.n_tok <= 0) continue;
+                if (threadIdx.x == 0) atomicCAS(status, 0, 11);
+                for (int64_t i = threadIdx.x; i < (int64_t)c.n_tok * G.heads * HD; i += THREADS) st(out + (int64_t)c.tok0 * G.heads * HD + i, 0.f);
+            }
     }
-    if (threadIdx.x < R) {
-        const int idx = row0 + threadIdx.x;
-        const bool there = (int)threadIdx.x < n_rows;
-        rows.q[threadIdx.x] = there ? q + ((int64_t)(tok0 + idx / group) * G.heads + kvh * group + idx % group) * HD : nullptr;
-        rows.last[threadIdx.x] = there ? keys.y - q_len + idx / group : -1;
-    }
-    __syncthreads();
-    attend(w, rows, kv, kv_pages, G.page_table + (int64_t)b * G.table_width, kvh, G.kv_heads, key0, key1, scale, status);
-    pdl_wait();
-    if (splits > 1) {
-        write_record(w, own_records + (((int64_t)b * gridDim.x + blockIdx.x) * gridDim.z + blockIdx.z) * REC);
-        return;
-    }
-    finish(G, sh, out, G.group_of[b], tok0, row0, n_rows, kvh,
-           [&](int r, float& m, float& l) {
-               m = max_of(w, r);
-               l = sum_of(w, r, m);
-           },
-           [&](int r, int c, float m) { return columns_of(w, r, c, m); });
+    pdl_wait();                                     // (whoever waits for this kernel waits for the one before it too)
 }
 
-// ---- 3. sequences whose own keys were cut ------------------------------------------
-// Blocks (key head and tile of rows, sequence); max_splits: parts that there is room for.
+// ---- the records joined ------------------------------------------------------------
+// Where a row's records of one kind are: n of them, `step` floats apart, the row at place r.
+struct Source {
+    const float* at;
+    int n, step, rows, r;
+    __device__ __forceinline__ float2 ml(int i) const { return *reinterpret_cast<const float2*>(at + (int64_t)i * step + rows * HD + 2 * r); }
+    __device__ __forceinline__ float4 four(int i, int c) const { return *reinterpret_cast<const float4*>(at + (int64_t)i * step + (c * rows + r) * 4); }
+};
+template <typename Parts>
+__device__ __forceinline__ Source source_of(const Parts& parts, const Records& rec, int thing, const Cut& c, int idx, int tile_rows, int column) {
+    Source s = {rec.at, 0, 0, rec.rows, 0};
+    if (!rec.plan || c.pages == 0) return s;
+    const int pair = parts.pair(), columns = parts.columns();
+    const int *units = rec.plan + 1, *items = rec.plan + 2 + parts.n();
+    const Deal deal(units[parts.n()], rec.plan[0], 1);
+    const int tile = idx / tile_rows, k = tile / pair, w = width_of(c, pair, k), u = units[thing] + units_before(c, pair, columns, k, column);
+    const int c0 = deal.block_of(u + w - 1), c1 = deal.block_of(u + w * c.blocks - 1);
+    const int floats = rec.rows * (HD + 2);
+    s.at = rec.at + (int64_t)((items[thing] + k * columns + column + c0) * pair + tile - k * pair) * floats;
+    s.n = c1 - c0 + 1, s.step = floats * pair, s.r = idx - tile * tile_rows;
+    return s;
+}
+
+// Blocks (four rows, sequence): a thread has a row and four columns (of 32, 64 .. further ones too), four neighbouring threads
+// four neighbouring rows, whose sums lie side by side in a record.
+constexpr int JT = 128, JR = 4;
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
-attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Shared sh, const float* own_records, int max_splits, int* status) {
+__global__ void __launch_bounds__(JT)
+attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records shared, const Records own) {
+    const int b = blockIdx.y, row = (int)blockIdx.x * JR + (int)threadIdx.x % JR, group = G.heads / G.kv_heads;
+    const SharedParts sp{G};
+    const OwnParts op{G, R};
+    const Cut mine = op(b);                         // (the description may be read before the wait)
+    const int tok = row / G.heads, head = row - tok * G.heads, kvh = head / group, h = head - kvh * group, g = G.group_of[b];
+    const bool there = tok < mine.n_tok && mine.pages > 0;
+    Cut c = Cut{0, 0, 0, 0, 0, 0, 0, 0};
+    if (there) c = sp(g);
     pdl_wait();
     pdl_trigger();
-    const int b = blockIdx.y, kvh = blockIdx.x % G.kv_heads, row0 = blockIdx.x / G.kv_heads * R;
-    const int tok0 = G.cu_seqlens[b], q_len = G.cu_seqlens[b + 1] - tok0, group = G.heads / G.kv_heads;
-    const int n_rows = min(R, q_len * group - row0);
-    if (n_rows <= 0) return;
-    const int2 keys = own_keys(G, b, q_len, status);
-    const int splits = keys.x < 0 ? 1 : min(own_splits(keys.y - keys.x), max_splits);
-    if (splits <= 1) return;
-    const float* rec = own_records + ((int64_t)b * gridDim.x + blockIdx.x) * max_splits * REC;
-    finish(G, sh, out, G.group_of[b], tok0, row0, n_rows, kvh,
-           [&](int r, float& m, float& l) {
-               for (int i = 0; i < splits; ++i) m = fmaxf(m, __ldcg(rec + (int64_t)i * REC + R * HD + 2 * r));
-               for (int i = 0; i < splits; ++i) {
-                   const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec + (int64_t)i * REC + R * HD + 2 * r));
-                   l = fmaf(ml.y, weight(ml.x, m), l);
-               }
-           },
-           [&](int r, int c, float m) {
-               float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-               for (int i = 0; i < splits; ++i) {
-                   const float4 o = __ldcg(reinterpret_cast<const float4*>(rec + (int64_t)i * REC + (c / 4 * R + r) * 4));
-                   const float a = weight(__ldcg(rec + (int64_t)i * REC + R * HD + 2 * r), m);
-                   s.x = fmaf(o.x, a, s.x), s.y = fmaf(o.y, a, s.y), s.z = fmaf(o.z, a, s.z), s.w = fmaf(o.w, a, s.w);
-               }
-               return s;
-           });
+    if (!there) return;
+    const Source src[2] = {source_of(sp, shared, g, c, (mine.tok0 + tok - c.tok0) * G.gs + h % G.gs, G.rows, kvh * G.per_kv + h / G.gs),
+                           source_of(op, own, b, mine, tok * group + h, R, kvh)};
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll 8
+        for (int i = 0; i < src[k].n; ++i) m = fmaxf(m, src[k].ml(i).x);
+    for (int col = threadIdx.x / JR; col < HD / 4; col += JT / JR) {
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll 8
+            for (int i = 0; i < src[k].n; ++i) {
+                const float2 ml = src[k].ml(i);
+                const float4 o = src[k].four(i, col);
+                const float a = weight(ml.x, m);
+                l = fmaf(ml.y, a, l);
+                s.x = fmaf(o.x, a, s.x), s.y = fmaf(o.y, a, s.y), s.z = fmaf(o.z, a, s.z), s.w = fmaf(o.w, a, s.w);
+            }
+        const float f = l != 0.f ? __fdiv_rn(1.0f, l) : 0.f;       // (a sum that is no number shows)
+        st4(out + ((int64_t)(mine.tok0 + tok) * G.heads + head) * HD + col * 4, s.x * f, s.y * f, s.z * f, s.w * f);
+    }
 }
 
 }  // namespace shared_prefix
@@ -596,85 +493,92 @@ using namespace wick;
 namespace wick {
 namespace shared_prefix {
 
-constexpr int PER_SM = 2;                          // blocks an SM of the kernel for shared keys
+constexpr int PER_SM = 2;                          // thread blocks an SM, where the tcgen05 kernel does not run
 
 struct Call {
     Groups G;
-    bool tc;                                       // the shared part's tcgen05 form
-    int tiles_own, splits, blocks;                 // tiles of 16 rows of the longest sequence; parts of own keys; blocks for the shared keys
-    int64_t plan_words, prefix_floats, own_floats;
+    bool fast;                                     // the forms for bfloat16 at head sizes 64 and 128
+    int blocks, blocks_own;                        // for the shared keys, for the own ones
+    int64_t plan_shared, plan_own, shared_floats, own_floats;
+    int64_t all() const { return plan_shared + plan_own + shared_floats + own_floats; }
 };
 
 static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups, int heads, int kv_heads, int max_pages, int own_bound, int max_q_len) {
     WICK_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "attention (shared prefix): %d heads over %d kv heads", heads, kv_heads);
     WICK_REQUIRE(n_seqs >= 1 && n_seqs <= 65535 && n_tokens >= 0, "attention (shared prefix): %d sequences, %d tokens", n_seqs, n_tokens);
     WICK_REQUIRE(n_groups >= 1 && n_groups <= MAX_GROUPS, "attention (shared prefix): %d groups (1 to %d)", n_groups, MAX_GROUPS);
-    WICK_REQUIRE(max_pages >= 0 && own_bound >= 0 && max_q_len >= 0, "attention (shared prefix): bad bounds");
+    WICK_REQUIRE(max_pages >= 0 && own_bound >= 0 && max_q_len >= 0 && (int64_t)max_q_len * heads <= INT32_MAX / 2, "attention (shared prefix): bad bounds");
     const int group = heads / kv_heads;
-    c.G.n = n_groups, c.G.n_seqs = n_seqs, c.G.max_pages = max_pages, c.G.heads = heads, c.G.kv_heads = kv_heads;
-    c.tc = half && tc_supported();
-    if (c.tc) {
+    Groups& G = c.G;
+    G.n = n_groups, G.n_seqs = n_seqs, G.max_pages = max_pages, G.heads = heads, G.kv_heads = kv_heads;
+    G.single = max_q_len == 1 && n_tokens == n_seqs;
+    c.fast = half && fast_supported();
+    if (c.fast) {
         // heads of a tile: all of a key head's, or as many as 128 rows hold of more
         int gs = group;
         for (int n = 2; gs > TC_ROWS; ++n)
             if (group % n == 0) gs = group / n;
-        c.G.rows = TC_ROWS / gs * gs, c.G.gs = gs, c.G.per_kv = group / gs, c.G.columns = heads / gs, c.G.block = 2, c.G.pair = 2;
+        G.rows = TC_ROWS / gs * gs, G.gs = gs, G.per_kv = group / gs, G.columns = heads / gs, G.block = 2, G.pair = 2;
     } else {
-        c.G.rows = R, c.G.gs = group, c.G.per_kv = 1, c.G.columns = kv_heads, c.G.block = 1, c.G.pair = 1;
+        G.rows = R, G.gs = group, G.per_kv = 1, G.columns = kv_heads, G.block = 1, G.pair = 1;
     }
-    c.tiles_own = ceil_div((int64_t)max_q_len * group, R);
-    WICK_REQUIRE((int64_t)c.tiles_own * kv_heads <= INT32_MAX / 2, "attention (shared prefix): %d tokens of one sequence are too many", max_q_len);
-    c.splits = own_splits(own_bound);
-    c.blocks = (c.tc ? 1 : PER_SM) * sm_count();
-    c.plan_words = max_pages > 0 ? (2 * (n_groups + 1) + 1 + 3) / 4 * 4 : 0;
-    const int64_t tiles = ceil_div((int64_t)n_tokens * c.G.gs, c.G.rows) + n_groups;
-    c.prefix_floats = max_pages > 0 ? ((tiles / c.G.pair + n_groups) * c.G.columns + c.blocks) * c.G.pair * (c.tc ? TC_ROWS : R) * (HD + 2) : 0;
-    c.own_floats = c.splits > 1 ? (int64_t)n_seqs * c.tiles_own * kv_heads * c.splits * REC : 0;
+    // No more thread blocks than there can be runs of work.
+    const int64_t tiles = (int64_t)ceil_div((int64_t)n_tokens * G.gs, G.rows) + n_groups, items = (tiles / G.pair + n_groups) * G.columns;
+    const int64_t units = tiles * G.columns * ceil_div(max_pages, G.block);
+    c.blocks = (int)max((int64_t)1, min((int64_t)(c.fast ? 1 : PER_SM) * sm_count(), units / G.pair));
+    const int64_t items_own = ((int64_t)ceil_div((int64_t)n_tokens * group, R) + n_seqs) * kv_heads;
+    c.blocks_own = (int)max((int64_t)1, min((int64_t)PER_SM * sm_count(), items_own * ceil_div(own_bound, kPage)));
+    WICK_REQUIRE(units <= INT32_MAX / 2 && items_own * ceil_div(own_bound, kPage) <= INT32_MAX / 2, "attention (shared prefix): too much for one step");
+    c.plan_shared = max_pages > 0 ? (2 * n_groups + 3 + 3) / 4 * 4 : 0;
+    c.plan_own = (2 * n_seqs + 3 + 3) / 4 * 4;
+    c.shared_floats = max_pages > 0 ? (items + c.blocks) * G.pair * (c.fast ? TC_ROWS : R) * (HD + 2) : 0;
+    c.own_floats = (items_own + c.blocks_own) * REC;
     return 0;
 }
 
+template <typename T, typename Parts>
+static int launch_part(const T* q, const T* kv, int64_t kv_pages, T* out, const Groups& G, const Parts& parts, bool wait_first, int blocks, float scale,
+                       int* plan, float* records, int* status, cudaStream_t s) {
+    constexpr int SMEM = (int)sizeof(Work<T>);
+    static bool raised = false;
+    if (!raised) {
+        WICK_CUDA(cudaFuncSetAttribute(attn_shared_part_kernel<T, Parts>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        raised = true;
+    }
+    WICK_CUDA(launch(attn_shared_part_kernel<T, Parts>, dim3(blocks), dim3(THREADS), (size_t)SMEM, s, q, kv, kv_pages, out, G, parts, (int)wait_first, scale,
+                     plan, records, status));
+    return check_launch("attn_shared_part");
+}
+
 template <typename T>
-static int attn_shared(const void* q, int n_tokens, const void* kv, int64_t kv_pages, void* out, const int* cu_groups, const int* pages,
+static int attn_shared(const T* q, int n_tokens, const T* kv, int64_t kv_pages, T* out, const int* cu_groups, const int* pages,
                        const int* group_of, int n_groups, const int* cu_seqlens, int n_seqs, const int* start, const int* page_table, int table_width,
                        int heads, int kv_heads, int max_pages, int own_bound, int max_q_len, float scale, float* scratch, int64_t scratch_floats,
                        int* status, cudaStream_t s) {
     Call c = {};
     if (int e = plan_call(c, sizeof(T) == 2, n_tokens, n_seqs, n_groups, heads, kv_heads, max_pages, own_bound, max_q_len)) return e;
     WICK_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "attention (shared prefix): operands must be 16-byte aligned");
-    WICK_REQUIRE(scratch_floats >= c.plan_words + c.prefix_floats + c.own_floats, "attention (shared prefix): scratch of %lld floats, %lld needed",
-                 (long long)scratch_floats, (long long)(c.plan_words + c.prefix_floats + c.own_floats));
+    WICK_REQUIRE(scratch_floats >= c.all(), "attention (shared prefix): scratch of %lld floats, %lld needed", (long long)scratch_floats, (long long)c.all());
     WICK_REQUIRE(scale >= 0.f, "attention (shared prefix): a negative scale");
     if (n_tokens == 0) return 0;
     Groups& G = c.G;
     G.cu_groups = cu_groups, G.pages = pages, G.group_of = group_of, G.cu_seqlens = cu_seqlens, G.start = start, G.page_table = page_table;
     G.table_width = table_width;
-    int* plan = reinterpret_cast<int*>(scratch);
-    float *records = scratch + c.plan_words, *own = records + c.prefix_floats;
-    constexpr int SMEM = (int)sizeof(Work<T>);
-    static bool raised = false;
-    if (!raised) {
-        WICK_CUDA(cudaFuncSetAttribute(attn_shared_prefix_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-        WICK_CUDA(cudaFuncSetAttribute(attn_shared_own_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-        raised = true;
+    int *plan = reinterpret_cast<int*>(scratch), *plan_own = plan + c.plan_shared;
+    float *records = scratch + c.plan_shared + c.plan_own, *own = records + c.shared_floats;
+    const bool any = max_pages > 0;
+    if (fast_supported() && sizeof(T) == 2) {
+        if (any)
+            if (int e = launch_tc(q, n_tokens, kv, kv_pages, G, c.blocks, scale, plan, records, status, s)) return e;
+        if (int e = launch_own(q, kv, kv_pages, out, G, any, c.blocks_own, scale, plan_own, own, status, s)) return e;
+    } else if constexpr (sizeof(T) == 4 || (HD != 64 && HD != 128)) {
+        if (any)
+            if (int e = launch_part(q, kv, kv_pages, out, G, SharedParts{G}, true, c.blocks, scale, plan, records, status, s)) return e;
+        if (int e = launch_part(q, kv, kv_pages, out, G, OwnParts{G, R}, !any, c.blocks_own, scale, plan_own, own, status, s)) return e;
     }
-    Shared sh = {nullptr, records, c.tc ? TC_ROWS : R};
-    if (max_pages > 0) sh.plan = plan;
-    if (max_pages > 0 && c.tc) {
-        if (int e = launch_tc(q, n_tokens, kv, kv_pages, G, c.blocks, scale, plan, records, status, s)) return e;
-    } else if (max_pages > 0) {
-        WICK_CUDA(launch(attn_shared_prefix_kernel<T>, dim3(c.blocks), dim3(THREADS), (size_t)SMEM, s, (const T*)q, (const T*)kv, kv_pages, G, scale, plan,
-                         records, status));
-        if (int e = check_launch("attn_shared_prefix")) return e;
-    }
-    WICK_CUDA(launch(attn_shared_own_kernel<T>, dim3(c.tiles_own * kv_heads, n_seqs, c.splits), dim3(THREADS), (size_t)SMEM, s, (const T*)q, (const T*)kv,
-                     kv_pages, (T*)out, G, sh, scale, own, status));
-    if (int e = check_launch("attn_shared_own")) return e;
-    if (c.splits > 1) {
-        WICK_CUDA(launch(attn_shared_join_kernel<T>, dim3(c.tiles_own * kv_heads, n_seqs), dim3(THREADS), 0, s, (T*)out, G, sh, (const float*)own,
-                         c.splits, status));
-        if (int e = check_launch("attn_shared_join")) return e;
-    }
-    return 0;
+    const Records sh = {any ? plan : nullptr, records, c.fast ? TC_ROWS : R}, ow = {plan_own, own, R};
+    WICK_CUDA(launch(attn_shared_join_kernel<T>, dim3(ceil_div((int64_t)max_q_len * heads, JR), n_seqs), dim3(JT), 0, s, out, G, sh, ow));
+    return check_launch("attn_shared_join");
 }
 
 }  // namespace shared_prefix
@@ -684,7 +588,7 @@ static int attn_shared(const void* q, int n_tokens, const void* kv, int64_t kv_p
 WICK_API long long wick_attn_shared_scratch(int half, int n_tokens, int n_seqs, int n_groups, int heads, int kv_heads, int max_pages, int own_bound, int max_q_len) {
     shared_prefix::Call c = {};
     if (shared_prefix::plan_call(c, half != 0, n_tokens, n_seqs, n_groups, heads, kv_heads, max_pages, own_bound, max_q_len)) return -1;
-    return c.plan_words + c.prefix_floats + c.own_floats;
+    return c.all();
 }
 
 // q, out: [n_tokens, heads, HD]; kv: one schedule entry's cache [kv_pages, 2, kv_heads, 64, HD], which holds the new tokens' keys and
@@ -697,7 +601,7 @@ WICK_API long long wick_attn_shared_scratch(int half, int n_tokens, int n_seqs, 
                       const int* group_of, int n_groups, const int* cu_seqlens, int n_seqs, const int* start, const int* page_table, int table_width,     \
                       int heads, int kv_heads, int max_pages, int own_bound, int max_q_len, float scale, float* scratch, int64_t scratch_floats,          \
                       int* status, void* s) {                                                                                                             \
-        return shared_prefix::attn_shared<T>(q, n_tokens, kv, kv_pages, out, cu_groups, pages, group_of, n_groups, cu_seqlens, n_seqs, start,             \
+        return shared_prefix::attn_shared<T>((const T*)q, n_tokens, (const T*)kv, kv_pages, (T*)out, cu_groups, pages, group_of, n_groups, cu_seqlens, n_seqs, start,             \
                                              page_table, table_width, heads, kv_heads, max_pages, own_bound, max_q_len, scale, scratch, scratch_floats,   \
                                              status, (cudaStream_t)s);                                                                                    \
     }

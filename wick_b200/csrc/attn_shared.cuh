@@ -23,59 +23,107 @@ constexpr int MAX_GROUPS = 1024;
 // The step's description and how the shared part is cut.
 struct Groups {
     const int *cu_groups, *pages, *group_of;       // sequences of group g: cu_groups[g] .. ; its shared pages; the group of a sequence
-    const int *cu_seqlens, *start, *positions, *page_table;
+    const int *cu_seqlens, *start, *page_table;
     int n, n_seqs, table_width, max_pages;
+    int single;                                    // every sequence brings one token: token i is sequence i's
     int heads, kv_heads;
     int rows;                                      // of a tile
     int gs, per_kv, columns;                       // heads of a tile; tiles of heads to a key head, in all
     int block, pair;                               // pages of a block of keys; tiles of an item, at most
 };
+__device__ __forceinline__ int pages_of(const Groups& G, int g) { return max(0, min(min(G.pages[g], G.max_pages), G.table_width)); }
 
-// One group as it is cut.
+// Something whose tiles see the same keys: a group and its shared pages, or a sequence and its own.
 struct Cut {
     int pages, tok0, n_tok, tiles, blocks;
-    __device__ __forceinline__ int items(const Groups& G) const { return (tiles + G.pair - 1) / G.pair * G.columns; }
-    __device__ __forceinline__ int units(const Groups& G) const { return tiles * G.columns * blocks; }
-    // Item i of the group is pair i / columns of tiles: how many they are, and the units of the group before it.
-    __device__ __forceinline__ int width(const Groups& G, int pair) const { return min(G.pair, tiles - pair * G.pair); }
-    __device__ __forceinline__ int before(const Groups& G, int pair, int column) const { return (pair * G.pair * G.columns + column * width(G, pair)) * blocks; }
+    int seq, first, end;                           // the row of the page table, its first column, the end of the positions
 };
-__device__ __forceinline__ int pages_of(const Groups& G, int g) { return max(0, min(min(G.pages[g], G.max_pages), G.table_width)); }
-__device__ __forceinline__ int first_token(const Groups& G, int g) { return G.cu_seqlens[max(0, min(G.cu_groups[g], G.n_seqs))]; }
-__device__ __forceinline__ Cut cut_of(const Groups& G, int g) {
-    Cut c;
-    c.pages = pages_of(G, g);
-    c.tok0 = first_token(G, g);
-    c.n_tok = first_token(G, g + 1) - c.tok0;
-    c.tiles = c.pages > 0 ? (c.n_tok * G.gs + G.rows - 1) / G.rows : 0;
-    c.blocks = (c.pages + G.block - 1) / G.block;
-    return c;
+// How such things are dealt: tiles of an item at most, columns, and the cut of number i of n.
+struct SharedParts {
+    static constexpr bool OWN = false;
+    const Groups G;
+    __device__ __forceinline__ int n() const { return G.n; }
+    __device__ __forceinline__ int pair() const { return G.pair; }
+    __device__ __forceinline__ int columns() const { return G.columns; }
+    __device__ __forceinline__ Cut operator()(int g) const {
+        Cut c;
+        c.pages = pages_of(G, g);
+        const int a = max(0, min(G.cu_groups[g], G.n_seqs)), b = max(a, min(G.cu_groups[g + 1], G.n_seqs));
+        c.seq = a, c.first = 0;
+        c.tok0 = G.single ? a : G.cu_seqlens[a];
+        c.n_tok = (G.single ? b : G.cu_seqlens[b]) - c.tok0;
+        c.tiles = c.pages > 0 ? (c.n_tok * G.gs + G.rows - 1) / G.rows : 0;
+        c.blocks = (c.pages + G.block - 1) / G.block;
+        c.end = c.pages * kPage;
+        return c;
+    }
+};
+// The own keys of a sequence that does not fit its group or its page table: none.
+struct OwnParts {
+    static constexpr bool OWN = true;
+    const Groups G;
+    int rows;                                      // of a tile
+    __device__ __forceinline__ int n() const { return G.n_seqs; }
+    __device__ __forceinline__ int pair() const { return 1; }
+    __device__ __forceinline__ int columns() const { return G.kv_heads; }
+    __device__ __forceinline__ bool fits(int b, const Cut& c) const {
+        return G.group_of[b] >= 0 && G.group_of[b] < G.n && G.start[b] >= c.first * kPage && (c.end + kPage - 1) / kPage <= G.table_width;
+    }
+    __device__ __forceinline__ Cut operator()(int b) const {
+        Cut c;
+        const int g = G.group_of[b];
+        c.seq = b;
+        c.tok0 = G.single ? b : G.cu_seqlens[b];
+        c.n_tok = G.single ? 1 : G.cu_seqlens[b + 1] - c.tok0;
+        c.first = g >= 0 && g < G.n ? pages_of(G, g) : 0;
+        c.end = G.start[b] + c.n_tok;
+        c.blocks = c.pages = c.n_tok > 0 && fits(b, c) ? (c.end + kPage - 1) / kPage - c.first : 0;
+        c.tiles = c.pages > 0 ? (c.n_tok * (G.heads / G.kv_heads) + rows - 1) / rows : 0;
+        return c;
+    }
+};
+// Item i of a thing is pair i / columns of tiles: how many they are, and the units of the thing before it.
+__device__ __forceinline__ int items_of(const Cut& c, int pair, int columns) { return (c.tiles + pair - 1) / pair * columns; }
+__device__ __forceinline__ int width_of(const Cut& c, int pair, int k) { return min(pair, c.tiles - k * pair); }
+__device__ __forceinline__ int units_before(const Cut& c, int pair, int columns, int k, int column) {
+    return (k * pair * columns + column * width_of(c, pair, k)) * c.blocks;
 }
 
-// Thread block c of S takes the units c U / S .. (c + 1) U / S; the block of unit u.  A run has G.pair units at least.
-__device__ __forceinline__ int run_start(int c, int U, int S) { return (int)((int64_t)c * U / S); }
-__device__ __forceinline__ int block_of(int u, int U, int S) { return (int)(((int64_t)S * (u + 1) - 1) / U); }
+// The units dealt: thread block c of S takes those from run_start(c) to run_start(c + 1), U / S of them or one more, and `pair` at least.
+struct Deal {
+    int U, S, per, more;                           // more: thread blocks that have one more than per
+    __device__ __forceinline__ Deal(int units, int blocks, int pair) : U(units) {
+        S = max(1, min(blocks, U / pair));
+        per = U / S, more = U - per * S;
+    }
+    __device__ __forceinline__ int run_start(int c) const { return c * per + min(c, more); }
+    __device__ __forceinline__ int block_of(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
+};
 
 // A run's part of one item: `tiles` tiles from `tile` on, blocks of keys from .. to.
 struct Segment {
-    int g, pages, tok0, n_tok, tile, tiles, column, record;
+    Cut cut;
+    int tile, tiles, column;
     int from, to;
+    int record;                                    // its number among all segments that there can be
+    int item0;                                     // the item's first unit
 };
 
-// A warp's way through its thread block's run.  A lane knows one group of 32.
-struct Walk {
-    const Groups& G;
-    int U, S, cta, u, end;                         // units of all groups; thread blocks that take part; this one, where it is in its run, the run's end
-    int g0, units, items;                          // first group of those known; units and items of the groups before it
+// A warp's way through its thread block's run.  A lane knows one thing of 32.
+template <typename Parts> struct Walk {
+    const Parts parts;
+    Deal deal;
+    int u, end;                                    // where it is in its run, the run's end
+    int g0, units, items;                          // first of the things known; units and items before it
     Cut mine;
-    int upto_units, upto_items;                    // ... and up to this lane's group
+    int upto_units, upto_items;                    // ... and up to this lane's
 
     __device__ __forceinline__ void know(int first) {
         g0 = first;
         const int g = g0 + (int)(threadIdx.x & 31);
-        mine = Cut{0, 0, 0, 0, 0};
-        if (g < G.n) mine = cut_of(G, g);
-        int x = mine.units(G), y = mine.items(G);
+        mine = Cut{0, 0, 0, 0, 0, 0, 0, 0};
+        if (g < parts.n()) mine = parts(g);
+        int x = mine.tiles * parts.columns() * mine.blocks, y = items_of(mine, parts.pair(), parts.columns());
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int tx = __shfl_up_sync(0xffffffffu, x, o), ty = __shfl_up_sync(0xffffffffu, y, o);
@@ -83,46 +131,46 @@ struct Walk {
         }
         upto_units = units + x, upto_items = items + y;
     }
-    // The groups known before become those before the first known.
-    __device__ __forceinline__ void next() {
+    __device__ __forceinline__ void next() {       // what was known becomes what lies before
         units = __shfl_sync(0xffffffffu, upto_units, 31), items = __shfl_sync(0xffffffffu, upto_items, 31);
         know(g0 + 32);
     }
-    // plan: where the thread blocks' number and the units and items before each group are written down, or null.
-    __device__ __forceinline__ Walk(const Groups& groups, int blocks, int* plan) : G(groups), units(0), items(0) {
+    // plan: where the thread blocks' number and the units and items before each thing are written down, or null.
+    __device__ __forceinline__ Walk(const Parts& p, int blocks, int* plan) : parts(p), deal(0, 1, 1), units(0), items(0) {
+        const int lane = threadIdx.x & 31;
         know(0);
         for (;;) {
-            const int g = g0 + (int)(threadIdx.x & 31);
-            if (plan && g < G.n) plan[2 + g] = upto_units, plan[3 + G.n + g] = upto_items;
-            if (g0 + 32 >= G.n) break;
+            const int g = g0 + lane;
+            if (plan && g < parts.n()) plan[2 + g] = upto_units, plan[3 + parts.n() + g] = upto_items;
+            if (g0 + 32 >= parts.n()) break;
             next();
         }
-        U = __shfl_sync(0xffffffffu, upto_units, 31);
-        S = max(1, min(blocks, U / G.pair));
-        if (plan && (threadIdx.x & 31) == 0) plan[0] = S, plan[1] = 0, plan[2 + G.n] = 0;
-        cta = blockIdx.x;
-        u = U > 0 && cta < S ? run_start(cta, U, S) : 0;
-        end = U > 0 && cta < S ? run_start(cta + 1, U, S) : 0;
-        if (G.n > 32) units = items = 0, know(0);
+        deal = Deal(__shfl_sync(0xffffffffu, upto_units, 31), blocks, parts.pair());
+        if (plan && lane == 0) plan[0] = deal.S, plan[1] = 0, plan[2 + parts.n()] = 0;
+        const bool in = deal.U > 0 && (int)blockIdx.x < deal.S;
+        u = in ? deal.run_start(blockIdx.x) : 0;
+        end = in ? deal.run_start(blockIdx.x + 1) : 0;
+        if (parts.n() > 32) units = items = 0, know(0);
     }
     // The next part of the run; false: there is none.
     __device__ __forceinline__ bool segment(Segment& s) {
         while (u < end) {
             while (u >= __shfl_sync(0xffffffffu, upto_units, 31)) next();
-            const int l = __ffs(__ballot_sync(0xffffffffu, u < upto_units)) - 1;
-            Cut c;
+            const int l = __ffs(__ballot_sync(0xffffffffu, u < upto_units)) - 1, pair = parts.pair(), columns = parts.columns();
+            Cut& c = s.cut;
             c.pages = __shfl_sync(0xffffffffu, mine.pages, l), c.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);
             c.n_tok = __shfl_sync(0xffffffffu, mine.n_tok, l), c.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
-            c.blocks = __shfl_sync(0xffffffffu, mine.blocks, l);
-            const int local = u - __shfl_sync(0xffffffffu, upto_units - mine.units(G), l), pair = local / (G.pair * G.columns * c.blocks);
-            const int w = c.width(G, pair), column = (local - c.before(G, pair, 0)) / (w * c.blocks), off = local - c.before(G, pair, column);
-            const int left = min(w * c.blocks - off, end - u);
-            s.g = g0 + l, s.pages = c.pages, s.tok0 = c.tok0, s.n_tok = c.n_tok;
-            s.tile = pair * G.pair, s.tiles = w, s.column = column;
+            c.blocks = __shfl_sync(0xffffffffu, mine.blocks, l), c.seq = __shfl_sync(0xffffffffu, mine.seq, l);
+            c.first = __shfl_sync(0xffffffffu, mine.first, l), c.end = __shfl_sync(0xffffffffu, mine.end, l);
+            const int base = __shfl_sync(0xffffffffu, upto_units - mine.tiles * columns * mine.blocks, l), local = u - base;
+            const int k = local / (pair * columns * c.blocks), w = width_of(c, pair, k), before = units_before(c, pair, columns, k, 0);
+            s.column = (local - before) / (w * c.blocks);
+            const int off = local - before - s.column * w * c.blocks, left = min(w * c.blocks - off, end - u);
+            s.tile = k * pair, s.tiles = w, s.item0 = u - off;
             // (a block of two tiles is done by whoever has the second one's unit)
             s.from = off / w, s.to = (off + left) / w;
             // (items and thread blocks rise together along the runs: no two segments share the sum)
-            s.record = (__shfl_sync(0xffffffffu, upto_items - mine.items(G), l) + pair * G.columns + column + cta) * G.pair;
+            s.record = __shfl_sync(0xffffffffu, upto_items - items_of(mine, pair, columns), l) + k * columns + s.column + (int)blockIdx.x;
             u += left;
             if (s.from < s.to) return true;
         }
@@ -130,11 +178,27 @@ struct Walk {
     }
 };
 
-// The tcgen05 form of the shared part (attn_shared_tc.cu): bfloat16, tiles of up to TC_ROWS rows, two an item, blocks of two pages.
-constexpr int TC_ROWS = 128;
-bool tc_supported();
+// A record: [HD / 4][rows] groups of four sums, then [rows] pairs of maximum and sum.  Records of a kind of parts, and the plan of the Walk
+// that dealt them (null: there are none):
+struct Records {
+    const int* plan;
+    const float* at;
+    int rows;                                      // that a record has room for
+};
+
+// 2^(a - b) for maxima that may be -inf (nothing seen): then the weight is 0.
+__device__ __forceinline__ float weight(float a, float b) { return a == -INFINITY ? 0.f : exp2f(a - b); }
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// The forms for bfloat16 at head sizes 64 and 128: the shared part on tcgen05 (attn_shared_tc.cu; tiles of up to TC_ROWS rows, two an item,
+// blocks of two pages), and the own keys streamed through shared memory (attn_shared_own.cu).
+constexpr int TC_ROWS = 128, OWN_ROWS = 16;
+bool fast_supported();
 int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, const Groups& G, int blocks, float scale, int* plan, float* records, int* status,
               cudaStream_t s);
+int launch_own(const void* q, const void* kv, int64_t kv_pages, void* out, const Groups& G, bool after_shared, int blocks, float scale, int* plan,
+               float* records, int* status, cudaStream_t s);
 
 }  // namespace shared_prefix
 }  // namespace wick

@@ -78,17 +78,19 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    // (The description lies ready before the step's kernels start; the plan is written behind the wait.)
+    Walk<SharedParts> walk(SharedParts{G}, gridDim.x, nullptr);    // (every warp walks on its own)
     pdl_wait();
     pdl_trigger();                                     // (behind the wait: the next kernel reads what this one reads without a wait of its own)
+    if (blockIdx.x == 0 && warp == 2) Walk<SharedParts>(SharedParts{G}, gridDim.x, plan);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem_slot;
     const bool aligned = (smem_u32(smem_raw) & 1023) == 0;   // (always: the block's dynamic shared memory is all there is)
     if (!aligned && threadIdx.x == 0) atomicCAS(status, 0, 7);
-    Walk walk(G, gridDim.x, blockIdx.x == 0 && warp == 2 ? plan : nullptr);   // (every warp walks on its own)
     // the block of keys that is one page: the last one of an odd number
-    auto half = [&](const Segment& s, int j) { return 2 * (s.from + j) + 1 == s.pages; };
+    auto half = [&](const Segment& s, int j) { return 2 * (s.from + j) + 1 == s.cut.pages; };
     Segment seg;
     int k = 0;                                         // segments so far
     bool ok = aligned;
@@ -101,11 +103,11 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         for (; ok && walk.segment(seg); ++k) {
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
-            const int* table = G.page_table + (int64_t)G.cu_groups[seg.g] * G.table_width;
+            const int* table = G.page_table + (int64_t)seg.cut.seq * G.table_width;
             // A lane holds a page number of each of two runs of 32, read ahead.
             auto pages = [&](int run) {
                 const int at = 2 * seg.from + run * 32 + lane;
-                int page = at < seg.pages ? table[at] : 0;
+                int page = at < seg.cut.pages ? table[at] : 0;
                 if (page < 0 || page >= kv_pages) {
                     atomicCAS(status, 0, 10);
                     page = 0;
@@ -120,7 +122,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                 for (int i = 0; i < seg.tiles; ++i)
                     for (int pn = 0; pn < PANELS; ++pn)
                         tma_load_3d(&q_map, &sh.q_full, q_s + i * TILE_BYTES + pn * PANEL_BYTES, pn * 64, seg.column * G.gs,
-                                    seg.tok0 + (seg.tile + i) * (G.rows / G.gs));
+                                    seg.cut.tok0 + (seg.tile + i) * (G.rows / G.gs));
             }
             // K0 V0 K1 V1 .., or, split, K0 K1 V0 K2 V1 K3 .. V(n-2) V(n-1): the order in which the issuing warp uses them
 #pragma unroll 1
@@ -236,7 +238,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         for (; ok && walk.segment(seg); ++k) {
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
-            const int tile = seg.tile + (split ? 0 : s), n_rows = min(G.rows, seg.n_tok * G.gs - tile * G.rows);
+            const int tile = seg.tile + (split ? 0 : s), n_rows = min(G.rows, seg.cut.n_tok * G.gs - tile * G.rows);
             const bool store = r < n_rows, busy = quad * 32 < n_rows;
             float m = -INFINITY, l = 0.f;              // what O and the sum are scaled by (it follows the maximum lazily), the sum
 #pragma unroll 1
@@ -255,21 +257,27 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                     hand_over(0), hand_over(1);
                     continue;
                 }
-                const bool whole = !half(seg, j);
-                float y[BK];
-#pragma unroll
-                for (int c = 0; c < BK; c += 32)
-                    if (c < 64 || whole) tc_ld32_nowait(s_addr + c, reinterpret_cast<uint32_t*>(y + c));
-                tc_ld_wait();
+                // Twice over the scores, 64 at a time, in loops: a run meets this code a few times, and each 128 bytes of it come from the
+                // L2 cache the first time.
+                const int parts = half(seg, j) ? 1 : 2;
+                float y[64];                           // the scores read last
+                auto read = [&](int part) {
+                    tc_ld32_nowait(s_addr + part * P_FIRST, reinterpret_cast<uint32_t*>(y));
+                    tc_ld32_nowait(s_addr + part * P_FIRST + 32, reinterpret_cast<uint32_t*>(y + 32));
+                    tc_ld_wait();
+                };
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int part = parts - 1; part >= 0; --part) {
+                    read(part);
 #pragma unroll
-                for (int i = 0; i < BK; i += 8)
-                    if (i < 64 || whole) {
+                    for (int i = 0; i < 64; i += 8) {
                         mx4[0] = max3(mx4[0], y[i], y[i + 1]);
                         mx4[1] = max3(mx4[1], y[i + 2], y[i + 3]);
                         mx4[2] = max3(mx4[2], y[i + 4], y[i + 5]);
                         mx4[3] = max3(mx4[3], y[i + 6], y[i + 7]);
                     }
+                }
                 const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
                 const bool grow = mx > m + 8.0f;
                 float alpha = 1.0f;
@@ -291,28 +299,31 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                 }
                 float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
                 const float2 sl2_2 = make_float2(sl2, sl2), neg_m2 = make_float2(neg_m, neg_m);
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part) {
+                    if (part < parts) {
+                        if (part > 0) read(part);
 #pragma unroll
-                for (int c = 0; c < BK; c += 32) {
-                    if (c < 64 || whole) {
-                        uint32_t packed[16];
+                        for (int c = 0; c < 64; c += 32) {
+                            uint32_t packed[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float2 e = fma2(make_float2(y[c + i], y[c + i + 1]), sl2_2, neg_m2);
-                            const float2 p = make_float2(ex2(e.x), ex2(e.y));
-                            sum2[(i >> 1) & 3] = add2(sum2[(i >> 1) & 3], p);
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(p.x, p.y);      // key 2k in the low half, key 2k + 1 in the high half
-                            packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 e = fma2(make_float2(y[c + i], y[c + i + 1]), sl2_2, neg_m2);
+                                const float2 p = make_float2(ex2(e.x), ex2(e.y));
+                                sum2[(i >> 1) & 3] = add2(sum2[(i >> 1) & 3], p);
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(p.x, p.y);      // key 2k in the low half, key 2k + 1 in the high half
+                                packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                            tc_st16(s_addr + part * (P_FIRST / 2) + c / 2, packed);
                         }
-                        tc_st16(s_addr + c / 2, packed);
                     }
-                    if (c == 32) hand_over(0);
-                    if (c == 96) hand_over(1);
+                    hand_over(part);
                 }
                 l = l * alpha + (((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y)));
             }
             if (!ok) break;
             // The record: [HD / 4][128] groups of four sums, [128] pairs of maximum and sum.
-            float* rec = records + (int64_t)(seg.record + tile - seg.tile) * REC;
+            float* rec = records + (int64_t)(seg.record * G.pair + tile - seg.tile) * REC;
             auto put = [&](int c, const float* v) {    // 32 numbers of the row from column c on
                 if (store) {
 #pragma unroll
@@ -395,8 +406,6 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
 }
 
 }  // namespace tc
-
-bool tc_supported() { return tc::SUPPORTED; }
 
 int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, const Groups& G, int blocks, float scale, int* plan, float* records, int* status,
               cudaStream_t s) {

@@ -533,7 +533,7 @@ def attention_decode_parts_fused(qkv: torch.Tensor, n_heads: int, n_kv: int, hea
 
 # ---------------------------------------------------------------------------
 # Attention where groups of a step's sequences share their first pages (csrc/attn_shared.cuh, attn_shared.cu).
-SHARED_SOURCES = ["attn_shared.cu", "attn_shared_tc.cu"]
+SHARED_SOURCES = ["attn_shared.cu", "attn_shared_tc.cu", "attn_shared_own.cu"]
 
 
 def _shared(head_dim: int) -> _Lib:
@@ -610,11 +610,10 @@ def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPre
         out = torch.empty_like(q)
     else:
         _cuda("out", out, q.dtype, q.shape)
-    splits = own_bound > 512
     _shared(hd).call(f"wick_attn_shared_{_dt(q)}", "piplppppipippiiiiiifplpp", _p(q), n, _p(kv), kv.shape[0], _p(out), _p(cu_groups), _p(pages),
                      _p(group_of), G, _p(batch.cu_seqlens), n_seqs, _p(batch.start), _p(batch.page_table), batch.table_width, n_heads,
                      kv.shape[2], max_pages, own_bound, batch.max_q_len, float(scale), _p(scratch), scratch.numel(),
-                     _p(status_tensor(q.device)), _stream(), kernels=1 + (max_pages > 0) + splits)
+                     _p(status_tensor(q.device)), _stream(), kernels=2 + (max_pages > 0))
     return out
 
 
