@@ -408,14 +408,10 @@ attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, 
     }
     if (blockIdx.x == 0) {
         pdl_wait();
-        if (threadIdx.x < 32) Walk<Parts>(parts, gridDim.x, plan);
-        if (OWN)
-            for (int b = 0; b < G.n_seqs; ++b) {    // rows of sequences that do not fit are zeros
-                const Cut c = parts(b);
-                if (c.pages > 0 || c.n_tok <= 0) continue;
-                if (threadIdx.x == 0) atomicCAS(status, 0, 11);
-                for (int64_t i = threadIdx.x; i < (int64_t)c.n_tok * G.heads * HD; i += THREADS) st(out + (int64_t)c.tok0 * G.heads * HD + i, 0.f);
-            }
+        if (threadIdx.x < 32) {
+            Walk<Parts>(parts, gridDim.x, plan);
+            if constexpr (OWN) clear_unfit(parts, out, G.heads * HD, status);
+        }
     }
     pdl_wait();                                     // (whoever waits for this kernel waits for the one before it too)
 }
@@ -462,23 +458,36 @@ attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records share
     if (!there) return;
     const Source src[2] = {source_of(sp, shared, g, c, (mine.tok0 + tok - c.tok0) * G.gs + h % G.gs, G.rows, kvh * G.per_kv + h / G.gs),
                            source_of(op, own, b, mine, tok * group + h, R, kvh)};
+    // (eight records at a time, the last one read again behind the end: reads do not wait for one another)
     float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-#pragma unroll 8
-        for (int i = 0; i < src[k].n; ++i) m = fmaxf(m, src[k].ml(i).x);
+#pragma unroll 1
+        for (int i0 = 0; i0 < src[k].n; i0 += 8) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = src[k].ml(min(i0 + i, src[k].n - 1)).x;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, x[i]);
+        }
     for (int col = threadIdx.x / JR; col < HD / 4; col += JT / JR) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         float l = 0.f;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-#pragma unroll 8
-            for (int i = 0; i < src[k].n; ++i) {
-                const float2 ml = src[k].ml(i);
-                const float4 o = src[k].four(i, col);
-                const float a = weight(ml.x, m);
-                l = fmaf(ml.y, a, l);
-                s.x = fmaf(o.x, a, s.x), s.y = fmaf(o.y, a, s.y), s.z = fmaf(o.z, a, s.z), s.w = fmaf(o.w, a, s.w);
+#pragma unroll 1
+            for (int i0 = 0; i0 < src[k].n; i0 += 8) {
+                float2 ml[8];
+                float4 o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ml[i] = src[k].ml(min(i0 + i, src[k].n - 1)), o[i] = src[k].four(min(i0 + i, src[k].n - 1), col);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (i0 + i >= src[k].n) continue;
+                    const float a = weight(ml[i].x, m);
+                    l = fmaf(ml[i].y, a, l);
+                    s.x = fmaf(o[i].x, a, s.x), s.y = fmaf(o[i].y, a, s.y), s.z = fmaf(o[i].z, a, s.z), s.w = fmaf(o[i].w, a, s.w);
+                }
             }
         const float f = l != 0.f ? __fdiv_rn(1.0f, l) : 0.f;       // (a sum that is no number shows)
         st4(out + ((int64_t)(mine.tok0 + tok) * G.heads + head) * HD + col * 4, s.x * f, s.y * f, s.z * f, s.w * f);

@@ -82,6 +82,21 @@ struct OwnParts {
         return c;
     }
 };
+// By a warp: the sequences that do not fit are reported, and their rows are made zero.
+template <typename T> __device__ __forceinline__ void clear_unfit(const OwnParts& parts, T* out, int row_numbers, int* status) {
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < parts.n(); b0 += 32) {
+        Cut c = Cut{0, 0, 0, 0, 0, 0, 0, 0};
+        if (b0 + lane < parts.n()) c = parts(b0 + lane);
+        unsigned bad = __ballot_sync(0xffffffffu, c.n_tok > 0 && c.pages == 0);
+        if (bad && lane == 0) atomicCAS(status, 0, 11);
+        for (; bad; bad &= bad - 1) {
+            const int l = __ffs(bad) - 1;
+            const int64_t at = (int64_t)__shfl_sync(0xffffffffu, c.tok0, l) * row_numbers, n = (int64_t)__shfl_sync(0xffffffffu, c.n_tok, l) * row_numbers;
+            for (int64_t i = lane; i < n; i += 32) st(out + at + i, 0.f);
+        }
+    }
+}
 // Item i of a thing is pair i / columns of tiles: how many they are, and the units of the thing before it.
 __device__ __forceinline__ int items_of(const Cut& c, int pair, int columns) { return (c.tiles + pair - 1) / pair * columns; }
 __device__ __forceinline__ int width_of(const Cut& c, int pair, int k) { return min(pair, c.tiles - k * pair); }

@@ -149,12 +149,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
         if (blockIdx.x == 0) {
             pdl_wait();
             Walk<OwnParts>(parts, gridDim.x, plan);
-            for (int b = 0; b < G.n_seqs; ++b) {                       // rows of sequences that do not fit are zeros
-                const Cut c = parts(b);
-                if (c.pages > 0 || c.n_tok <= 0) continue;
-                if (lane == 0) atomicCAS(status, 0, 11);
-                for (int64_t i = lane; i < (int64_t)c.n_tok * G.heads * HD; i += 32) out[(int64_t)c.tok0 * G.heads * HD + i] = __float2bfloat16_rn(0.f);
-            }
+            clear_unfit(parts, out, G.heads * HD, status);
         }
     } else {
         // ---------------- compute ----------------
