@@ -458,37 +458,38 @@ attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records share
     if (!there) return;
     const Source src[2] = {source_of(sp, shared, g, c, (mine.tok0 + tok - c.tok0) * G.gs + h % G.gs, G.rows, kvh * G.per_kv + h / G.gs),
                            source_of(op, own, b, mine, tok * group + h, R, kvh)};
-    // (eight records at a time, the last one read again behind the end: reads do not wait for one another)
-    float m = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll 1
-        for (int i0 = 0; i0 < src[k].n; i0 += 8) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = src[k].ml(min(i0 + i, src[k].n - 1)).x;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, x[i]);
-        }
+    // Both kinds in one go, eight records at a time (the last one read again behind the end): reads do not wait for one another, and what the
+    // records are scaled by follows their maximum.
+    const int n = src[0].n + src[1].n;
     for (int col = threadIdx.x / JR; col < HD / 4; col += JT / JR) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
+        float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-            for (int i0 = 0; i0 < src[k].n; i0 += 8) {
-                float2 ml[8];
-                float4 o[8];
+        for (int i0 = 0; i0 < n; i0 += 8) {
+            float2 ml[8];
+            float4 o[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ml[i] = src[k].ml(min(i0 + i, src[k].n - 1)), o[i] = src[k].four(min(i0 + i, src[k].n - 1), col);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (i0 + i >= src[k].n) continue;
-                    const float a = weight(ml[i].x, m);
-                    l = fmaf(ml[i].y, a, l);
-                    s.x = fmaf(o[i].x, a, s.x), s.y = fmaf(o[i].y, a, s.y), s.z = fmaf(o[i].z, a, s.z), s.w = fmaf(o[i].w, a, s.w);
-                }
+            for (int i = 0; i < 8; ++i) {
+                const int at = min(i0 + i, n - 1);
+                const bool second = at >= src[0].n;
+                const Source& from = second ? src[1] : src[0];
+                const int k = second ? at - src[0].n : at;
+                ml[i] = from.ml(k), o[i] = from.four(k, col);
             }
+            float most = m;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, ml[i].x);
+            const float before = weight(m, most);
+            m = most;
+            l *= before, s.x *= before, s.y *= before, s.z *= before, s.w *= before;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i0 + i >= n) continue;
+                const float a = weight(ml[i].x, m);
+                l = fmaf(ml[i].y, a, l);
+                s.x = fmaf(o[i].x, a, s.x), s.y = fmaf(o[i].y, a, s.y), s.z = fmaf(o[i].z, a, s.z), s.w = fmaf(o[i].w, a, s.w);
+            }
+        }
         const float f = l != 0.f ? __fdiv_rn(1.0f, l) : 0.f;       // (a sum that is no number shows)
         st4(out + ((int64_t)(mine.tok0 + tok) * G.heads + head) * HD + col * 4, s.x * f, s.y * f, s.z * f, s.w * f);
     }
@@ -531,12 +532,22 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
     } else {
         G.rows = R, G.gs = group, G.per_kv = 1, G.columns = kv_heads, G.block = 1, G.pair = 1;
     }
+    // The own keys' kernel starts as soon as all of the first one's thread blocks run, on the SMs that those leave.  (An
+    // environment variable sets the share, for measurements.)
     // No more thread blocks than there can be runs of work.
     const int64_t tiles = (int64_t)ceil_div((int64_t)n_tokens * G.gs, G.rows) + n_groups, items = (tiles / G.pair + n_groups) * G.columns;
     const int64_t units = tiles * G.columns * ceil_div(max_pages, G.block);
-    c.blocks = (int)max((int64_t)1, min((int64_t)(c.fast ? 1 : PER_SM) * sm_count(), units / G.pair));
+    const int sms = sm_count();
+    const int own_per_sm = c.fast ? OWN_WARPS * (128 / HD) : PER_SM;
+    int first = c.fast ? sms : PER_SM * sms, second = own_per_sm * sms;
+    if (c.fast && max_pages > 0) {
+        const char* e = getenv("WICK_SPLIT");
+        const double share = e ? atof(e) : 1.0;
+        if (share < 1.0) first = max(1, (int)(sms * share)), second = own_per_sm * (sms - first);
+    }
+    c.blocks = (int)max((int64_t)1, min((int64_t)first, units / G.pair));
     const int64_t items_own = ((int64_t)ceil_div((int64_t)n_tokens * group, R) + n_seqs) * kv_heads;
-    c.blocks_own = (int)max((int64_t)1, min((int64_t)PER_SM * sm_count(), items_own * ceil_div(own_bound, kPage)));
+    c.blocks_own = (int)max((int64_t)1, min((int64_t)second, items_own * ceil_div(own_bound, kPage)));
     WICK_REQUIRE(units <= INT32_MAX / 2 && items_own * ceil_div(own_bound, kPage) <= INT32_MAX / 2, "attention (shared prefix): too much for one step");
     c.plan_shared = max_pages > 0 ? (2 * n_groups + 3 + 3) / 4 * 4 : 0;
     c.plan_own = (2 * n_seqs + 3 + 3) / 4 * 4;

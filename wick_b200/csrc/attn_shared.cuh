@@ -208,7 +208,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 // The forms for bfloat16 at head sizes 64 and 128: the shared part on tcgen05 (attn_shared_tc.cu; tiles of up to TC_ROWS rows, two an item,
 // blocks of two pages), and the own keys streamed through shared memory (attn_shared_own.cu).
-constexpr int TC_ROWS = 128, OWN_ROWS = 16;
+constexpr int TC_ROWS = 128, OWN_ROWS = 16, OWN_WARPS = 6;   // (warps an SM at head size 128, twice as many at 64)
 bool fast_supported();
 int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, const Groups& G, int blocks, float scale, int* plan, float* records, int* status,
               cudaStream_t s);
