@@ -13,6 +13,9 @@
 //     scores it came from, as bfloat16 pairs);
 //   * a softmax thread owns a row.  O and the sum are scaled by a maximum that follows the true one lazily: O is rescaled only when a
 //     block's maximum exceeds it by more than 8 (in units of log2 e).  Warps whose rows are all beyond the group's tokens compute nothing.
+// REHEARSE: a run has few blocks, and a block's code is met for the first time while all SMs fill their rings: instructions then
+// come through the same queues as 24 MB of keys and values, and the first block's softmax took 4,300 clocks, the first products 4,100.
+// So the softmax warps go through their code once while there is nothing to do yet, and the issuing warp's code is loops.
 // Every wait is bounded and reports through the status word (code 7).
 #include "tc_attention.cuh"
 #include "attn_shared.cuh"
@@ -47,6 +50,18 @@ struct Smem {
 };
 constexpr int SMEM_BYTES = (2 + NSLOT) * TILE_BYTES + (int)sizeof(Smem);
 static_assert(SMEM_BYTES <= 227 * 1024, "a block's shared memory");
+
+// D (tensor memory) (+)= A (shared memory) * B (shared memory)
+__device__ __forceinline__ void mma_ss_acc(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, int acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
+        ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "r"(acc)
+        : "memory");
+}
 
 __global__ void __launch_bounds__(THREADS, 1)
 attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const Groups G, int64_t kv_pages, float scale,
@@ -92,7 +107,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     // the block of keys that is one page: the last one of an odd number
     auto half = [&](const Segment& s, int j) { return 2 * (s.from + j) + 1 == s.cut.pages; };
     Segment seg;
-    int k = 0;                                         // segments so far
+    int k = 0;                                         // runs so far
     bool ok = aligned;
 
     if (warp == 0) {
@@ -175,8 +190,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
             const int N = split ? n : 2 * n;           // turns
+            // turn i: stream i & 1's product of one block, then its scores of the next.  (Instructions in loops: see REHEARSE.)
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, k & 1, abort_flag, status, 7));
-            // turn i: stream i & 1's product of one block, then its scores of the next
 #pragma unroll 1
             for (int i = -2; ok && i < N; ++i) {
                 const int s = i & 1;
@@ -186,17 +201,21 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                     if (split || s == 0) ok = take(v_at);
                     // (the sums of the stream's run before have been read)
                     if (ok && i < 2 && uses > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_empty[s], (uses - 1) & 1, abort_flag, status, 7));
-                    const uint32_t v_lo = v_lo0 + v_at * (TILE_BYTES >> 4), d = tmem + COL_O + s * HD, pa = tmem + COL_S + s * BK;
+                    uint32_t vp = v_lo0 + v_at * (TILE_BYTES >> 4), pp = tmem + COL_S + s * BK;
+                    const uint32_t d = tmem + COL_O + s * HD;
                     const int parts = half(seg, split ? i : i >> 1) ? 1 : 2;
-#pragma unroll
+#pragma unroll 1
                     for (int part = 0; part < 2; ++part) {
                         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[s][part], steps & 1, abort_flag, status, 7));
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t pp = pa + part * (P_FIRST / 2), vp = v_lo + part * (P_FIRST / 16) * (2048 >> 4);
                         if (one && part < parts) {
-                            mma_ts(d, pp, vp, idesc_o, i >= 2 || part > 0);
-                            static_for<1, P_FIRST / 16>([&](auto ks) { mma_ts(d, pp + (int)ks * 8, vp + (int)ks * (2048 >> 4), idesc_o, 1); });
+                            int begun = i >= 2 || part > 0;
+#pragma unroll 1
+                            for (int ks = 0; ks < P_FIRST / 16; ++ks, pp += 8, vp += 2048 >> 4) {
+                                mma_ts(d, pp, vp, idesc_o, begun);
+                                begun = 1;
+                            }
                         }
                     }
                     if (!ok) break;
@@ -211,12 +230,15 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                     if (split || s == 0) ok = take(k_at);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t k_lo = k_lo0 + k_at * (TILE_BYTES >> 4), q_lo = q_lo0 + (split ? 0 : s * (TILE_BYTES >> 4)), d = tmem + COL_S + s * BK;
+                    uint32_t k_lo = k_lo0 + k_at * (TILE_BYTES >> 4), q_lo = q_lo0 + (split ? 0 : s * (TILE_BYTES >> 4));
+                    const uint32_t d = tmem + COL_S + s * BK;
                     if (one) {
-                        static_for<0, HD / 16>([&](auto ks) {
-                            constexpr uint32_t off = (((int)ks >> 2) * PANEL_BYTES + ((int)ks & 3) * 32) >> 4;
-                            mma_ss<((int)ks > 0)>(d, q_lo + off, k_lo + off, idesc_s);
-                        });
+#pragma unroll 1
+                        for (int ks = 0; ks < HD / 16; ++ks) {
+                            mma_ss_acc(d, q_lo, k_lo, idesc_s, ks > 0);
+                            const uint32_t step = (ks & 3) == 3 ? (PANEL_BYTES - 96) >> 4 : 32 >> 4;   // (four steps of 32 bytes a panel)
+                            q_lo += step, k_lo += step;
+                        }
                         tc_commit(&sh.s_full[s]);
                         if (split || s == 1) tc_commit(&sh.empty[k_at]);
                         if (i + 2 == N - 1) tc_commit(&sh.q_empty);            // (the run's last scores)
@@ -240,14 +262,19 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             const bool split = seg.tiles == 1;
             const int tile = seg.tile + (split ? 0 : s), n_rows = min(G.rows, seg.cut.n_tok * G.gs - tile * G.rows);
             const bool store = r < n_rows, busy = quad * 32 < n_rows;
+            const int dj = split ? 2 : 1;
             float m = -INFINITY, l = 0.f;              // what O and the sum are scaled by (it follows the maximum lazily), the sum
 #pragma unroll 1
-            for (int j = split ? s : 0, first = 1; j < n; j += split ? 2 : 1, first = 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s], step & 1, abort_flag, status, 7));
-                if (!ok) break;
-                ++step;
+            for (int j = (split ? s : 0) - (k == 0 ? dj : 0); j < n; j += dj) {
+                const bool rehearsed = j < 0, first = j < dj;      // (a block before the first: see REHEARSE)
+                if (!rehearsed) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s], step & 1, abort_flag, status, 7));
+                    if (!ok) break;
+                    ++step;
+                }
                 tc_fence_after();
                 auto hand_over = [&](int part) {
+                    if (rehearsed) return;
                     tc_st_wait();
                     tc_fence_before();                 // P and the rescaled O before it multiplies and accumulates
                     __syncwarp();
@@ -314,12 +341,13 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                                 const __nv_bfloat162 h = __floats2bfloat162_rn(p.x, p.y);      // key 2k in the low half, key 2k + 1 in the high half
                                 packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
                             }
-                            tc_st16(s_addr + part * (P_FIRST / 2) + c / 2, packed);
+                            if (!rehearsed) tc_st16(s_addr + part * (P_FIRST / 2) + c / 2, packed);
                         }
                     }
                     hand_over(part);
                 }
                 l = l * alpha + (((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y)));
+                if (rehearsed) m = -INFINITY, l = 0.f;
             }
             if (!ok) break;
             // The record: [HD / 4][128] groups of four sums, [128] pairs of maximum and sum.
