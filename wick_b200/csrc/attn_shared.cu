@@ -26,7 +26,7 @@ constexpr int HD = WICK_HD;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head_dim must be a multiple of 16 in [16, 256]");
 typedef __nv_bfloat16 bf16;
 
-constexpr int R = OWN_ROWS;                        // rows of a tile
+constexpr int R = 16;                              // rows of a tile
 constexpr int W = 4, THREADS = W * 32;
 constexpr int REC = R * (HD + 2);                  // floats of a tile's record: [HD / 4][R][4] sums, [R][2] maximum and sum of weights
 // A block's 16 rows, as the cores leave them: in PARTS parts.
@@ -377,23 +377,21 @@ template <typename T> __device__ __forceinline__ void write_record(const Work<T>
 }
 
 // ---- the parts ---------------------------------------------------------------------
-// wait_first: whether something before this kernel may still run that it reads the results of (the own parts' kernel comes behind the
-// shared ones', which has waited for q and the cache).
-template <typename T, typename Parts>
+// OWN: the own keys, else the shared ones.  wait_first: whether something before this kernel may still run that it reads the results of
+// (the own keys' kernel comes behind the shared ones', which has waited for q and the cache).
+template <typename T, bool OWN>
 __global__ void __launch_bounds__(THREADS)
-attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, T* __restrict__ out, const Groups G, const Parts parts, int wait_first,
+attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, T* __restrict__ out, const Groups G, int wait_first,
                         float scale, int* plan, float* records, int* status) {
     extern __shared__ __align__(16) uint8_t smem[];
     Work<T>& w = *reinterpret_cast<Work<T>*>(smem);
     __shared__ Rows<T> rows;
-    constexpr bool OWN = Parts::OWN;
     if (wait_first) pdl_wait();
     pdl_trigger();                                  // (behind the wait, so that the next kernel need not wait for what this one waited for)
     q = fresh(q);
     const int gs = OWN ? G.heads / G.kv_heads : G.gs;
-    Walk<Parts> walk(parts, gridDim.x, nullptr);
-    Segment s;
-    while (walk.segment(s)) {                       // (every warp walks the same way)
+    const OwnParts own{G, R};
+    auto work = [&](const Segment& s) {
         __syncthreads();                            // (the rows and the work of the segment before)
         if (threadIdx.x < R) {
             const int idx = s.tile * R + threadIdx.x, tok = idx / gs;
@@ -405,12 +403,24 @@ attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, 
         attend(w, rows, kv, kv_pages, G.page_table + (int64_t)s.cut.seq * G.table_width, s.column / (OWN ? 1 : G.per_kv), G.kv_heads,
                (s.cut.first + s.from) * kPage, min((s.cut.first + s.to) * kPage, s.cut.end), scale, status);
         write_record(w, records + (int64_t)s.record * REC);
+    };
+    if constexpr (OWN) {                            // (every warp walks the same way)
+        Walk walk(own, gridDim.x, nullptr);
+        Segment s;
+        while (walk.segment(s)) work(s);
+    } else {
+        Runs runs(G, gridDim.x);
+        for (int r = blockIdx.x; r < runs.all; r += gridDim.x) work(runs.segment(r));
     }
     if (blockIdx.x == 0) {
         pdl_wait();
         if (threadIdx.x < 32) {
-            Walk<Parts>(parts, gridDim.x, plan);
-            if constexpr (OWN) clear_unfit(parts, out, G.heads * HD, status);
+            if constexpr (OWN) {
+                Walk(own, gridDim.x, plan);
+                clear_unfit(own, out, G.heads * HD, status);
+            } else {
+                Runs(G, gridDim.x).write(plan);
+            }
         }
     }
     pdl_wait();                                     // (whoever waits for this kernel waits for the one before it too)
@@ -421,77 +431,79 @@ attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, 
 struct Source {
     const float* at;
     int n, step, rows, r;
-    __device__ __forceinline__ float2 ml(int i) const { return *reinterpret_cast<const float2*>(at + (int64_t)i * step + rows * HD + 2 * r); }
-    __device__ __forceinline__ float4 four(int i, int c) const { return *reinterpret_cast<const float4*>(at + (int64_t)i * step + (c * rows + r) * 4); }
 };
-template <typename Parts>
-__device__ __forceinline__ Source source_of(const Parts& parts, const Records& rec, int thing, const Cut& c, int idx, int tile_rows, int column) {
+__device__ __forceinline__ Source shared_source(const Groups& G, const Records& rec, int g, const Cut& c, int tok, int h, int kvh) {
     Source s = {rec.at, 0, 0, rec.rows, 0};
     if (!rec.plan || c.pages == 0) return s;
-    const int pair = parts.pair(), columns = parts.columns();
-    const int *units = rec.plan + 1, *items = rec.plan + 2 + parts.n();
-    const Deal deal(units[parts.n()], rec.plan[0], 1);
-    const int tile = idx / tile_rows, k = tile / pair, w = width_of(c, pair, k), u = units[thing] + units_before(c, pair, columns, k, column);
-    const int c0 = deal.block_of(u + w - 1), c1 = deal.block_of(u + w * c.blocks - 1);
-    const int floats = rec.rows * (HD + 2);
-    s.at = rec.at + (int64_t)((items[thing] + k * columns + column + c0) * pair + tile - k * pair) * floats;
-    s.n = c1 - c0 + 1, s.step = floats * pair, s.r = idx - tile * tile_rows;
+    const int idx = (tok - c.tok0) * G.gs + h % G.gs, tile = idx / G.rows, floats = rec.rows * (HD + 2);
+    const Place p = place_of(G, c, rec.plan[0], tile, kvh * G.per_kv + h / G.gs);
+    s.at = rec.at + (int64_t)((rec.plan[1 + g] + p.first) * G.pair + tile % G.pair) * floats;
+    s.n = p.n, s.step = floats * G.pair, s.r = idx - tile * G.rows;
     return s;
 }
+__device__ __forceinline__ Source own_source(const OwnParts& parts, const Records& rec, int b, const Cut& c, int idx, int kvh) {
+    const int *units = rec.plan + 1, *items = rec.plan + 2 + parts.n();
+    const Deal deal(units[parts.n()], rec.plan[0]);
+    const int tile = idx / parts.rows, item = tile * parts.columns() + kvh, u = units[b] + item * c.pages, c0 = deal.worker_of(u);
+    const int floats = rec.rows * (HD + 2);
+    return Source{rec.at + (int64_t)(items[b] + item + c0) * floats, deal.worker_of(u + c.pages - 1) - c0 + 1, floats, rec.rows, idx - tile * parts.rows};
+}
 
-// Blocks (four rows, sequence): a thread has a row and four columns (of 32, 64 .. further ones too), four neighbouring threads
-// four neighbouring rows, whose sums lie side by side in a record.
+// Blocks (four rows, sequence): a thread has a row and four columns (and those 128, 256 .. behind), four neighbouring threads four
+// neighbouring rows, whose sums lie side by side in a record.  Eight records at a time: each of the eight threads of a row in a warp
+// finds one's weight, and all read the sums of all of them at once (behind the last one: of that one again, without weight).
 constexpr int JT = 128, JR = 4;
 template <typename T>
 __global__ void __launch_bounds__(JT)
 attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records shared, const Records own) {
     const int b = blockIdx.y, row = (int)blockIdx.x * JR + (int)threadIdx.x % JR, group = G.heads / G.kv_heads;
-    const SharedParts sp{G};
-    const OwnParts op{G, R};
-    const Cut mine = op(b);                         // (the description may be read before the wait)
+    const OwnParts parts{G, own.rows};
+    const Cut mine = parts(b);                      // (the description may be read before the wait)
     const int tok = row / G.heads, head = row - tok * G.heads, kvh = head / group, h = head - kvh * group, g = G.group_of[b];
     const bool there = tok < mine.n_tok && mine.pages > 0;
     Cut c = Cut{0, 0, 0, 0, 0, 0, 0, 0};
-    if (there) c = sp(g);
+    if (there) c = SharedParts{G}(g);
     pdl_wait();
     pdl_trigger();
-    if (!there) return;
-    const Source src[2] = {source_of(sp, shared, g, c, (mine.tok0 + tok - c.tok0) * G.gs + h % G.gs, G.rows, kvh * G.per_kv + h / G.gs),
-                           source_of(op, own, b, mine, tok * group + h, R, kvh)};
-    // Both kinds in one go, eight records at a time (the last one read again behind the end): reads do not wait for one another, and what the
-    // records are scaled by follows their maximum.
-    const int n = src[0].n + src[1].n;
-    for (int col = threadIdx.x / JR; col < HD / 4; col += JT / JR) {
+    Source src = {nullptr, 0, 0, 0, 0};
+    const int k = (threadIdx.x & 31) / JR;          // of the eight threads of a row
+    for (int col = threadIdx.x / JR; col < (HD / 4 + 7) / 8 * 8; col += JT / JR) {     // (whole warps)
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-        for (int i0 = 0; i0 < n; i0 += 8) {
-            float2 ml[8];
-            float4 o[8];
+        for (int kind = 0; kind < 2; ++kind) {
+            if (there) src = kind == 0 ? shared_source(G, shared, g, c, mine.tok0 + tok, h, kvh) : own_source(parts, own, b, mine, tok * group + h, kvh);
+            const float *sums = src.at + (min(col, HD / 4 - 1) * src.rows + src.r) * 4, *ml = src.at + src.rows * HD + 2 * src.r;
+#pragma unroll 1
+            for (int i0 = 0; __any_sync(0xffffffffu, i0 < src.n); i0 += 8) {
+                const int left = src.n - i0;        // (a row without further records: reads the last one again, or none)
+                float2 x = make_float2(-INFINITY, 0.f);
+                float4 o[8];
+                if (k < left) x = *reinterpret_cast<const float2*>(ml + (int64_t)(i0 + k) * src.step);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = min(i0 + i, n - 1);
-                const bool second = at >= src[0].n;
-                const Source& from = second ? src[1] : src[0];
-                const int k = second ? at - src[0].n : at;
-                ml[i] = from.ml(k), o[i] = from.four(k, col);
-            }
-            float most = m;
+                for (int i = 0; i < 8; ++i)
+                    if (left > 0) o[i] = *reinterpret_cast<const float4*>(sums + (int64_t)(i0 + min(i, left - 1)) * src.step);
+                float most = fmaxf(m, x.x);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) most = fmaxf(most, ml[i].x);
-            const float before = weight(m, most);
-            m = most;
-            l *= before, s.x *= before, s.y *= before, s.z *= before, s.w *= before;
+                for (int d = JR; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                const float before = weight(m, most);
+                m = most;
+                l *= before, s.x *= before, s.y *= before, s.z *= before, s.w *= before;
+                const float w = weight(x.x, m);
+                float add = k < left ? x.y * w : 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (i0 + i >= n) continue;
-                const float a = weight(ml[i].x, m);
-                l = fmaf(ml[i].y, a, l);
-                s.x = fmaf(o[i].x, a, s.x), s.y = fmaf(o[i].y, a, s.y), s.z = fmaf(o[i].z, a, s.z), s.w = fmaf(o[i].w, a, s.w);
+                for (int d = JR; d < 32; d <<= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+                l += add;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float a = __shfl_sync(0xffffffffu, w, i * JR + (threadIdx.x % JR));
+                    if (i >= left) continue;
+                    s.x = fmaf(o[i].x, a, s.x), s.y = fmaf(o[i].y, a, s.y), s.z = fmaf(o[i].z, a, s.z), s.w = fmaf(o[i].w, a, s.w);
+                }
             }
         }
         const float f = l != 0.f ? __fdiv_rn(1.0f, l) : 0.f;       // (a sum that is no number shows)
-        st4(out + ((int64_t)(mine.tok0 + tok) * G.heads + head) * HD + col * 4, s.x * f, s.y * f, s.z * f, s.w * f);
+        if (there && col < HD / 4) st4(out + ((int64_t)(mine.tok0 + tok) * G.heads + head) * HD + col * 4, s.x * f, s.y * f, s.z * f, s.w * f);
     }
 }
 
@@ -546,26 +558,27 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
         if (share < 1.0) first = max(1, (int)(sms * share)), second = own_per_sm * (sms - first);
     }
     c.blocks = (int)max((int64_t)1, min((int64_t)first, units / G.pair));
-    const int64_t items_own = ((int64_t)ceil_div((int64_t)n_tokens * group, R) + n_seqs) * kv_heads;
+    const int rows_own = c.fast ? OWN_ROWS : R;
+    const int64_t items_own = ((int64_t)ceil_div((int64_t)n_tokens * group, rows_own) + n_seqs) * kv_heads;
     c.blocks_own = (int)max((int64_t)1, min((int64_t)second, items_own * ceil_div(own_bound, kPage)));
     WICK_REQUIRE(units <= INT32_MAX / 2 && items_own * ceil_div(own_bound, kPage) <= INT32_MAX / 2, "attention (shared prefix): too much for one step");
-    c.plan_shared = max_pages > 0 ? (2 * n_groups + 3 + 3) / 4 * 4 : 0;
+    c.plan_shared = max_pages > 0 ? (n_groups + 2 + 3) / 4 * 4 : 0;
     c.plan_own = (2 * n_seqs + 3 + 3) / 4 * 4;
-    c.shared_floats = max_pages > 0 ? (items + c.blocks) * G.pair * (c.fast ? TC_ROWS : R) * (HD + 2) : 0;
-    c.own_floats = (items_own + c.blocks_own) * REC;
+    c.shared_floats = max_pages > 0 ? max((int64_t)c.blocks, items) * G.pair * (c.fast ? TC_ROWS : R) * (HD + 2) : 0;
+    c.own_floats = (items_own + c.blocks_own) * rows_own * (HD + 2);
     return 0;
 }
 
-template <typename T, typename Parts>
-static int launch_part(const T* q, const T* kv, int64_t kv_pages, T* out, const Groups& G, const Parts& parts, bool wait_first, int blocks, float scale,
-                       int* plan, float* records, int* status, cudaStream_t s) {
+template <typename T, bool OWN>
+static int launch_part(const T* q, const T* kv, int64_t kv_pages, T* out, const Groups& G, bool wait_first, int blocks, float scale, int* plan,
+                       float* records, int* status, cudaStream_t s) {
     constexpr int SMEM = (int)sizeof(Work<T>);
     static bool raised = false;
     if (!raised) {
-        WICK_CUDA(cudaFuncSetAttribute(attn_shared_part_kernel<T, Parts>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        WICK_CUDA(cudaFuncSetAttribute(attn_shared_part_kernel<T, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
         raised = true;
     }
-    WICK_CUDA(launch(attn_shared_part_kernel<T, Parts>, dim3(blocks), dim3(THREADS), (size_t)SMEM, s, q, kv, kv_pages, out, G, parts, (int)wait_first, scale,
+    WICK_CUDA(launch(attn_shared_part_kernel<T, OWN>, dim3(blocks), dim3(THREADS), (size_t)SMEM, s, q, kv, kv_pages, out, G, (int)wait_first, scale,
                      plan, records, status));
     return check_launch("attn_shared_part");
 }
@@ -593,10 +606,10 @@ static int attn_shared(const T* q, int n_tokens, const T* kv, int64_t kv_pages, 
         if (int e = launch_own(q, kv, kv_pages, out, G, any, c.blocks_own, scale, plan_own, own, status, s)) return e;
     } else if constexpr (sizeof(T) == 4 || (HD != 64 && HD != 128)) {
         if (any)
-            if (int e = launch_part(q, kv, kv_pages, out, G, SharedParts{G}, true, c.blocks, scale, plan, records, status, s)) return e;
-        if (int e = launch_part(q, kv, kv_pages, out, G, OwnParts{G, R}, !any, c.blocks_own, scale, plan_own, own, status, s)) return e;
+            if (int e = launch_part<T, false>(q, kv, kv_pages, out, G, true, c.blocks, scale, plan, records, status, s)) return e;
+        if (int e = launch_part<T, true>(q, kv, kv_pages, out, G, !any, c.blocks_own, scale, plan_own, own, status, s)) return e;
     }
-    const Records sh = {any ? plan : nullptr, records, c.fast ? TC_ROWS : R}, ow = {plan_own, own, R};
+    const Records sh = {any ? plan : nullptr, records, c.fast ? TC_ROWS : R}, ow = {plan_own, own, c.fast ? OWN_ROWS : R};
     WICK_CUDA(launch(attn_shared_join_kernel<T>, dim3(ceil_div((int64_t)max_q_len * heads, JR), n_seqs), dim3(JT), 0, s, out, G, sh, ow));
     return check_launch("attn_shared_join");
 }

@@ -6,11 +6,12 @@
 // holds; the rest are the sequence's own.  Each part is kept as (m, l, o) = (maximum, sum of weights, weighted sum of values), all
 // in float32, and parts are joined by M = max m_i, l = sum l_i 2^(m_i - M), o likewise (scores in units of log2 e).
 //
-// A tile's rows see the shared keys in blocks of G.block pages; a tile (or, where a block of threads takes two, a pair of neighbouring
-// tiles) with all its blocks is an ITEM, a tile and block a UNIT of work.  The units of all items, one behind the other, are dealt to
-// the thread blocks in equal contiguous runs, so that no last round is half empty, whatever the groups' sizes; where a run ends inside an
-// item the item has a further record.  Who has which unit follows from the description alone, so the kernel that joins finds the
-// records by arithmetic, in a fixed order.
+// Shared keys: a tile (or, where a thread block takes two, a pair of neighbouring tiles) is an ITEM.  An item's blocks of G.block pages are cut
+// into RUNS of equal length, the longest that still gives every thread block one run (see Runs): what a run costs besides its blocks is
+// as much as three of them, so a thread block should not have two.  Own keys: a sequence's 16 or 8 rows of one key head are an item, whose
+// pages are dealt to the workers in equal contiguous runs, from one item into the next (see Walk).  Either way a record is
+// written per run and item, and who has what follows from the description alone: the kernel that joins finds the records by
+// arithmetic, in a fixed order.
 #pragma once
 
 #include "common.cuh"
@@ -38,13 +39,8 @@ struct Cut {
     int pages, tok0, n_tok, tiles, blocks;
     int seq, first, end;                           // the row of the page table, its first column, the end of the positions
 };
-// How such things are dealt: tiles of an item at most, columns, and the cut of number i of n.
 struct SharedParts {
-    static constexpr bool OWN = false;
-    const Groups G;
-    __device__ __forceinline__ int n() const { return G.n; }
-    __device__ __forceinline__ int pair() const { return G.pair; }
-    __device__ __forceinline__ int columns() const { return G.columns; }
+    const Groups& G;
     __device__ __forceinline__ Cut operator()(int g) const {
         Cut c;
         c.pages = pages_of(G, g);
@@ -60,11 +56,9 @@ struct SharedParts {
 };
 // The own keys of a sequence that does not fit its group or its page table: none.
 struct OwnParts {
-    static constexpr bool OWN = true;
-    const Groups G;
+    const Groups& G;
     int rows;                                      // of a tile
     __device__ __forceinline__ int n() const { return G.n_seqs; }
-    __device__ __forceinline__ int pair() const { return 1; }
     __device__ __forceinline__ int columns() const { return G.kv_heads; }
     __device__ __forceinline__ bool fits(int b, const Cut& c) const {
         return G.group_of[b] >= 0 && G.group_of[b] < G.n && G.start[b] >= c.first * kPage && (c.end + kPage - 1) / kPage <= G.table_width;
@@ -97,48 +91,135 @@ template <typename T> __device__ __forceinline__ void clear_unfit(const OwnParts
         }
     }
 }
-// Item i of a thing is pair i / columns of tiles: how many they are, and the units of the thing before it.
-__device__ __forceinline__ int items_of(const Cut& c, int pair, int columns) { return (c.tiles + pair - 1) / pair * columns; }
-__device__ __forceinline__ int width_of(const Cut& c, int pair, int k) { return min(pair, c.tiles - k * pair); }
-__device__ __forceinline__ int units_before(const Cut& c, int pair, int columns, int k, int column) {
-    return (k * pair * columns + column * width_of(c, pair, k)) * c.blocks;
-}
-
-// The units dealt: thread block c of S takes those from run_start(c) to run_start(c + 1), U / S of them or one more, and `pair` at least.
+// Own pages dealt: worker c of S takes the units (pages of an item) from run_start(c) to run_start(c + 1), U / S of them or one more.
 struct Deal {
-    int U, S, per, more;                           // more: thread blocks that have one more than per
-    __device__ __forceinline__ Deal(int units, int blocks, int pair) : U(units) {
-        S = max(1, min(blocks, U / pair));
+    int U, S, per, more;                           // more: workers that have one more than per
+    __device__ __forceinline__ Deal(int units, int workers) : U(units) {
+        S = max(1, min(workers, U));
         per = U / S, more = U - per * S;
     }
     __device__ __forceinline__ int run_start(int c) const { return c * per + min(c, more); }
-    __device__ __forceinline__ int block_of(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
+    __device__ __forceinline__ int worker_of(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
 };
 
-// A run's part of one item: `tiles` tiles from `tile` on, blocks of keys from .. to.
+// A run's part of one item: `tiles` tiles from `tile` on, blocks (own: pages) from .. to.
 struct Segment {
     Cut cut;
     int tile, tiles, column;
     int from, to;
-    int record;                                    // its number among all segments that there can be
-    int item0;                                     // the item's first unit
+    int record;
 };
 
-// A warp's way through its thread block's run.  A lane knows one thing of 32.
-template <typename Parts> struct Walk {
-    const Parts parts;
-    Deal deal;
-    int u, end;                                    // where it is in its run, the run's end
-    int g0, units, items;                          // first of the things known; units and items before it
+// ---- shared keys -------------------------------------------------------------------
+// The blocks of a run of an item of w tiles: `run` for two tiles, twice as many for one (whose blocks cost half).
+__device__ __forceinline__ int run_blocks(const Groups& G, int run, int w) { return run * G.pair / w; }
+// Runs of an item of w tiles, of all items of a group.
+__device__ __forceinline__ int runs_of_item(const Groups& G, const Cut& c, int run, int w) {
+    const int n = run_blocks(G, run, w);
+    return (c.blocks + n - 1) / n;
+}
+__device__ __forceinline__ int runs_of(const Groups& G, const Cut& c, int run) {
+    const int full = c.tiles / G.pair, rest = c.tiles - full * G.pair;
+    return G.columns * (full * runs_of_item(G, c, run, G.pair) + (rest ? runs_of_item(G, c, run, rest) : 0));
+}
+// Where a tile of a group is: its item's first run (of the group's) and number of runs.
+struct Place {
+    int first, n;
+};
+__device__ __forceinline__ Place place_of(const Groups& G, const Cut& c, int run, int tile, int column) {
+    const int pair = tile / G.pair, w = min(G.pair, c.tiles - pair * G.pair), n = runs_of_item(G, c, run, w);
+    const int before = pair > 0 ? pair * G.columns * runs_of_item(G, c, run, G.pair) : 0;
+    return Place{before + column * n, n};
+}
+
+// A warp's knowledge of all runs.  A lane knows one group of 32.
+struct Runs {
+    const Groups& G;
+    int run, all;                                  // blocks of a run, all runs
+    int g0, before;                                // first of the groups known; runs of the groups before it
     Cut mine;
-    int upto_units, upto_items;                    // ... and up to this lane's
+    int upto;                                      // runs up to this lane's group
 
     __device__ __forceinline__ void know(int first) {
         g0 = first;
         const int g = g0 + (int)(threadIdx.x & 31);
         mine = Cut{0, 0, 0, 0, 0, 0, 0, 0};
-        if (g < parts.n()) mine = parts(g);
-        int x = mine.tiles * parts.columns() * mine.blocks, y = items_of(mine, parts.pair(), parts.columns());
+        if (g < G.n) mine = SharedParts{G}(g);
+    }
+    __device__ __forceinline__ void count() {
+        int x = mine.tiles > 0 ? runs_of(G, mine, run) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, x, o);
+            if ((int)(threadIdx.x & 31) >= o) x += t;
+        }
+        upto = before + x;
+    }
+    __device__ __forceinline__ Runs(const Groups& groups, int blocks) : G(groups), before(0) {
+        // the shortest run that leaves no thread block with two; no shorter than an equal share, no longer than the longest item
+        int cost = 0, most = 1;
+        for (int g = 0; g < G.n; g += 32) {
+            know(g);
+            cost += __reduce_add_sync(0xffffffffu, (unsigned)(mine.tiles * G.columns * mine.blocks));
+            most = max(most, (int)__reduce_max_sync(0xffffffffu, (unsigned)(mine.tiles > 0 ? mine.blocks : 0)));
+        }
+        run = max(1, (cost + blocks * G.pair - 1) / (blocks * G.pair));
+        for (;; run += 1 + run / 16) {
+            all = 0;
+            for (int g = 0; g < G.n; g += 32) {
+                if (G.n > 32) know(g);
+                all += (int)__reduce_add_sync(0xffffffffu, (unsigned)(mine.tiles > 0 ? runs_of(G, mine, run) : 0));
+            }
+            if (all <= blocks || run >= most) break;
+        }
+        if (G.n > 32) know(0);
+        count();
+    }
+    // plan: the blocks of a run, then the runs before each group.
+    __device__ __forceinline__ void write(int* plan) {
+        if ((threadIdx.x & 31) == 0) plan[0] = run, plan[1] = 0;
+        for (int g = 0; g < G.n; g += 32) {
+            if (g > 0) before = __shfl_sync(0xffffffffu, upto, 31), know(g), count();
+            if (g + (int)(threadIdx.x & 31) < G.n) plan[2 + g + (threadIdx.x & 31)] = upto;
+        }
+    }
+    // Run r (of those asked for one after the other, in rising order).
+    __device__ __forceinline__ Segment segment(int r) {
+        while (r >= __shfl_sync(0xffffffffu, upto, 31)) before = __shfl_sync(0xffffffffu, upto, 31), know(g0 + 32), count();
+        const int l = __ffs(__ballot_sync(0xffffffffu, r < upto)) - 1;
+        Segment s;
+        Cut& c = s.cut;
+        c.pages = __shfl_sync(0xffffffffu, mine.pages, l), c.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);
+        c.n_tok = __shfl_sync(0xffffffffu, mine.n_tok, l), c.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
+        c.blocks = __shfl_sync(0xffffffffu, mine.blocks, l), c.seq = __shfl_sync(0xffffffffu, mine.seq, l);
+        c.first = 0, c.end = c.pages * kPage;
+        const int local = r - (l > 0 ? __shfl_sync(0xffffffffu, upto, l - 1) : before);
+        const int per = G.columns * runs_of_item(G, c, run, G.pair), full = c.tiles / G.pair;
+        const int pair = min(full, local / per), w = pair < full ? G.pair : c.tiles - full * G.pair, n = runs_of_item(G, c, run, w), rest = local - pair * per;
+        s.column = rest / n;
+        s.tile = pair * G.pair, s.tiles = w;
+        s.from = (rest - s.column * n) * run_blocks(G, run, w), s.to = min(c.blocks, s.from + run_blocks(G, run, w));
+        s.record = r;
+        return s;
+    }
+};
+
+// ---- own keys ----------------------------------------------------------------------
+// A worker's way through its run; a worker is `blockIdx.x`.  A lane knows one sequence of 32.
+struct Walk {
+    const OwnParts parts;
+    Deal deal;
+    int u, end;                                    // where it is in its run, the run's end
+    int b0, units, items;                          // first of the sequences known; units and items before it
+    Cut mine;
+    int upto_units, upto_items;                    // ... and up to this lane's
+
+    __device__ __forceinline__ void know(int first) {
+        b0 = first;
+        const int b = b0 + (int)(threadIdx.x & 31);
+        mine = Cut{0, 0, 0, 0, 0, 0, 0, 0};
+        if (b < parts.n()) mine = parts(b);
+        int y = mine.tiles * parts.columns(), x = y * mine.pages;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int tx = __shfl_up_sync(0xffffffffu, x, o), ty = __shfl_up_sync(0xffffffffu, y, o);
@@ -148,19 +229,19 @@ template <typename Parts> struct Walk {
     }
     __device__ __forceinline__ void next() {       // what was known becomes what lies before
         units = __shfl_sync(0xffffffffu, upto_units, 31), items = __shfl_sync(0xffffffffu, upto_items, 31);
-        know(g0 + 32);
+        know(b0 + 32);
     }
-    // plan: where the thread blocks' number and the units and items before each thing are written down, or null.
-    __device__ __forceinline__ Walk(const Parts& p, int blocks, int* plan) : parts(p), deal(0, 1, 1), units(0), items(0) {
+    // plan: the workers' number and the units and items before each sequence are written down there (null: not).
+    __device__ __forceinline__ Walk(const OwnParts& p, int workers, int* plan) : parts(p), deal(0, 1), units(0), items(0) {
         const int lane = threadIdx.x & 31;
         know(0);
         for (;;) {
-            const int g = g0 + lane;
-            if (plan && g < parts.n()) plan[2 + g] = upto_units, plan[3 + parts.n() + g] = upto_items;
-            if (g0 + 32 >= parts.n()) break;
+            const int b = b0 + lane;
+            if (plan && b < parts.n()) plan[2 + b] = upto_units, plan[3 + parts.n() + b] = upto_items;
+            if (b0 + 32 >= parts.n()) break;
             next();
         }
-        deal = Deal(__shfl_sync(0xffffffffu, upto_units, 31), blocks, parts.pair());
+        deal = Deal(__shfl_sync(0xffffffffu, upto_units, 31), workers);
         if (plan && lane == 0) plan[0] = deal.S, plan[1] = 0, plan[2 + parts.n()] = 0;
         const bool in = deal.U > 0 && (int)blockIdx.x < deal.S;
         u = in ? deal.run_start(blockIdx.x) : 0;
@@ -169,32 +250,26 @@ template <typename Parts> struct Walk {
     }
     // The next part of the run; false: there is none.
     __device__ __forceinline__ bool segment(Segment& s) {
-        while (u < end) {
-            while (u >= __shfl_sync(0xffffffffu, upto_units, 31)) next();
-            const int l = __ffs(__ballot_sync(0xffffffffu, u < upto_units)) - 1, pair = parts.pair(), columns = parts.columns();
-            Cut& c = s.cut;
-            c.pages = __shfl_sync(0xffffffffu, mine.pages, l), c.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);
-            c.n_tok = __shfl_sync(0xffffffffu, mine.n_tok, l), c.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
-            c.blocks = __shfl_sync(0xffffffffu, mine.blocks, l), c.seq = __shfl_sync(0xffffffffu, mine.seq, l);
-            c.first = __shfl_sync(0xffffffffu, mine.first, l), c.end = __shfl_sync(0xffffffffu, mine.end, l);
-            const int base = __shfl_sync(0xffffffffu, upto_units - mine.tiles * columns * mine.blocks, l), local = u - base;
-            const int k = local / (pair * columns * c.blocks), w = width_of(c, pair, k), before = units_before(c, pair, columns, k, 0);
-            s.column = (local - before) / (w * c.blocks);
-            const int off = local - before - s.column * w * c.blocks, left = min(w * c.blocks - off, end - u);
-            s.tile = k * pair, s.tiles = w, s.item0 = u - off;
-            // (a block of two tiles is done by whoever has the second one's unit)
-            s.from = off / w, s.to = (off + left) / w;
-            // (items and thread blocks rise together along the runs: no two segments share the sum)
-            s.record = __shfl_sync(0xffffffffu, upto_items - items_of(mine, pair, columns), l) + k * columns + s.column + (int)blockIdx.x;
-            u += left;
-            if (s.from < s.to) return true;
-        }
-        return false;
+        if (u >= end) return false;
+        while (u >= __shfl_sync(0xffffffffu, upto_units, 31)) next();
+        const int l = __ffs(__ballot_sync(0xffffffffu, u < upto_units)) - 1, columns = parts.columns();
+        Cut& c = s.cut;
+        c.pages = __shfl_sync(0xffffffffu, mine.pages, l), c.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);
+        c.n_tok = __shfl_sync(0xffffffffu, mine.n_tok, l), c.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
+        c.seq = __shfl_sync(0xffffffffu, mine.seq, l), c.blocks = c.pages;
+        c.first = __shfl_sync(0xffffffffu, mine.first, l), c.end = __shfl_sync(0xffffffffu, mine.end, l);
+        const int local = u - __shfl_sync(0xffffffffu, upto_units - mine.tiles * columns * mine.pages, l), item = local / c.pages;
+        s.tile = item / columns, s.tiles = 1, s.column = item - s.tile * columns;
+        s.from = local - item * c.pages, s.to = min(c.pages, s.from + end - u);
+        // (items and workers rise together along the runs: no two parts share the sum)
+        s.record = __shfl_sync(0xffffffffu, upto_items - mine.tiles * columns, l) + item + (int)blockIdx.x;
+        u += s.to - s.from;
+        return true;
     }
 };
 
-// A record: [HD / 4][rows] groups of four sums, then [rows] pairs of maximum and sum.  Records of a kind of parts, and the plan of the Walk
-// that dealt them (null: there are none):
+// A record: [HD / 4][rows] groups of four sums, then [rows] pairs of maximum and sum.  Records of a kind, and the plan that Runs or Walk wrote
+// (null: there are none):
 struct Records {
     const int* plan;
     const float* at;
@@ -208,7 +283,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 // The forms for bfloat16 at head sizes 64 and 128: the shared part on tcgen05 (attn_shared_tc.cu; tiles of up to TC_ROWS rows, two an item,
 // blocks of two pages), and the own keys streamed through shared memory (attn_shared_own.cu).
-constexpr int TC_ROWS = 128, OWN_ROWS = 16, OWN_WARPS = 6;   // (warps an SM at head size 128, twice as many at 64)
+constexpr int TC_ROWS = 128, OWN_ROWS = 8, OWN_WARPS = 6;    // (warps an SM at head size 128, twice as many at 64)
 bool fast_supported();
 int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, const Groups& G, int blocks, float scale, int* plan, float* records, int* status,
               cudaStream_t s);

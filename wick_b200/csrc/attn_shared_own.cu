@@ -1,11 +1,12 @@
 // The own keys of each sequence behind its group's shared prefix: bfloat16, head sizes 64 and 128.
 //
 // A thread block is ONE warp that feeds itself; six of them (head size 64: twelve) fill an SM's shared memory.  The pages of all items (a
-// sequence's 16 rows of one key head) are dealt to the warps in equal runs (attn_shared.cuh).  A warp has room for one page of keys and
+// sequence's 8 rows of one key head) are dealt to the warps in equal runs (attn_shared.cuh).  A warp has room for one page of keys and
 // one of values: the next page's keys are copied (TMA, 128-byte swizzle) while it turns scores into weights and multiplies the values,
-// the next values while it multiplies the next keys, from one item into the next.  Queries are on the 16-row side of mma.sync, so that weights
-// are the second product's operand as they stand; they enter it rounded to bfloat16, and their sum is taken of the rounded ones.  Every item leaves
-// a record per run that has a part of it.
+// the next values while it multiplies the next keys, from one item into the next.  Keys and value columns are on the 16-row side of mma.sync, the
+// rows on the 8-wide one (with rows on the 16-row side a page took twice the instructions, of which a token of 4 or 8 heads needs half);
+// weights are turned into the second product's operand by movmatrix, rounded to bfloat16; their sum is taken of the rounded ones.  Every item
+// leaves a record per run that has a part of it.
 // Bound by the bytes of the keys and values.  (Measured and left: blocks of four or eight warps that shared a page met three times
 // a page, 2,000 clocks of latency that two blocks an SM could not hide: 64 sequences of 370 own positions, 8 key heads, 28 us.)
 // The kernel of the shared part runs before this one, which starts under its last blocks.
@@ -28,7 +29,7 @@ constexpr int HD = SUPPORTED ? WICK_HD : 64;           // other head sizes: neve
 typedef __nv_bfloat16 bf16;
 constexpr int R = OWN_ROWS;
 constexpr int PANELS = HD / 64, PANEL_BYTES = kPage * 128, TILE_BYTES = PANELS * PANEL_BYTES;   // a page of keys, or of values
-constexpr int KS = HD / 16, NT = HD / 8;               // steps of q . k; tiles of eight value columns
+constexpr int KS = HD / 16, MT = kPage / 16;           // steps of q . k, and tiles of 16 value columns; tiles of 16 keys
 constexpr int REC = R * (HD + 2);
 
 struct Smem {
@@ -53,6 +54,13 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
 // Byte offset, inside a page's tile, of the 16-byte chunk `chunk` (8 numbers) of row `row`.
 __device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
     return (uint32_t)((chunk >> 3) * PANEL_BYTES + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+// An 8 x 8 matrix of 16-bit numbers, a row in four lanes: the transposed matrix in the same layout.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
 }
 
 // The page after the one at hand: the run's part it lies in, its place in it.  A lane holds one of 32 page numbers.
@@ -80,8 +88,8 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
     if (!after_shared) pdl_wait();
     pdl_trigger();
     const OwnParts parts{G, R};
-    Walk<OwnParts> walk(parts, gridDim.x, nullptr);
-    Ahead next;
+    Walk walk(parts, gridDim.x, nullptr);
+    Ahead next = {};
     auto know_ids = [&]() {                            // from page next.j on
         const int* table = G.page_table + (int64_t)next.s.cut.seq * G.table_width + next.s.cut.first;
         int id = next.j + lane < next.s.to ? table[next.j + lane] : 0;
@@ -114,10 +122,9 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
     if (ok) begin();
     if (next.any) copy(0), copy(1);
 
-    uint32_t qa[KS][4];
-    float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    int last0 = -1, last1 = -1;                        // the last position that rows g and g + 8 see
-    bool upper = false;                                // rows 8 to 15 are there
+    uint32_t qb[KS][2];                                // lane: row g
+    float o[KS][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;        // columns 16 i + g and + 8 of rows 2 t and 2 t + 1
+    int last0 = -1, last1 = -1;                        // the last position that rows 2 t and 2 t + 1 see
     const uint32_t k_s = smem_u32(sm.k), v_s = smem_u32(sm.v);
 #pragma unroll 1
     for (int turn = 0; ok && next.any; turn ^= 1) {
@@ -125,23 +132,18 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
         const int key0 = (next.s.cut.first + next.j) * kPage, valid = next.s.cut.end - key0;     // places of the page that hold a token
         const int record = next.s.record;
         if (first) {
-            const int i0 = next.s.tile * R + g, n_rows = next.s.cut.n_tok * group - next.s.tile * R;
-            const bool is0 = g < n_rows, is1 = g + 8 < n_rows;
-            const int tok0 = i0 / group, tok1 = (i0 + 8) / group, p0 = next.s.cut.end - next.s.cut.n_tok, h = next.s.column * group;
-            const bf16* q0 = q + ((int64_t)(next.s.cut.tok0 + tok0) * G.heads + h + i0 - tok0 * group) * HD + 2 * t;
-            const bf16* q1 = q + ((int64_t)(next.s.cut.tok0 + tok1) * G.heads + h + i0 + 8 - tok1 * group) * HD + 2 * t;
-            last0 = is0 ? p0 + tok0 : -1, last1 = is1 ? p0 + tok1 : -1;
-            upper = n_rows > 8;
+            const int row0 = next.s.tile * R, n_rows = next.s.cut.n_tok * group - row0, p0 = next.s.cut.end - next.s.cut.n_tok;
+            const int tok = (row0 + g) / group;
+            const bf16* q0 = q + ((int64_t)(next.s.cut.tok0 + tok) * G.heads + next.s.column * group + row0 + g - tok * group) * HD + 2 * t;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                qa[i][0] = is0 ? *reinterpret_cast<const uint32_t*>(q0 + i * 16) : 0u;
-                qa[i][1] = is1 ? *reinterpret_cast<const uint32_t*>(q1 + i * 16) : 0u;
-                qa[i][2] = is0 ? *reinterpret_cast<const uint32_t*>(q0 + i * 16 + 8) : 0u;
-                qa[i][3] = is1 ? *reinterpret_cast<const uint32_t*>(q1 + i * 16 + 8) : 0u;
+                qb[i][0] = g < n_rows ? *reinterpret_cast<const uint32_t*>(q0 + i * 16) : 0u;
+                qb[i][1] = g < n_rows ? *reinterpret_cast<const uint32_t*>(q0 + i * 16 + 8) : 0u;
             }
+            last0 = 2 * t < n_rows ? p0 + (row0 + 2 * t) / group : -1, last1 = 2 * t + 1 < n_rows ? p0 + (row0 + 2 * t + 1) / group : -1;
             m0 = m1 = -INFINITY, l0 = l1 = 0.f;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+            for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         }
         // the page ahead, before this one is waited for
         if (!last) {
@@ -151,30 +153,29 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&sm.k_full, turn, &sm.abort_flag, status, 7));
         if (!ok) break;
-        float c[kPage / 8][4];
+        float c[MT][4];                                // keys 16 m + g and + 8, rows 2 t and 2 t + 1
 #pragma unroll
-        for (int n = 0; n < kPage / 8; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+        for (int m = 0; m < MT; ++m) c[m][0] = c[m][1] = c[m][2] = c[m][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < KS; ++i)
 #pragma unroll
-            for (int n = 0; n < kPage / 8; n += 2) {
-                uint32_t kb[4];
-                ldsm_x4(kb, k_s + tile_off(n * 8 + (lane >> 4) * 8 + (lane & 7), 2 * i + ((lane >> 3) & 1)));
-                mma16816(c[n], qa[i], kb[0], kb[1]);
-                mma16816(c[n + 1], qa[i], kb[2], kb[3]);
+            for (int m = 0; m < MT; ++m) {
+                uint32_t ka[4];
+                ldsm_x4(ka, k_s + tile_off(m * 16 + (lane & 15), 2 * i + (lane >> 4)));
+                mma16816(c[m], ka, qb[i][0], qb[i][1]);
             }
         if (next.any) copy(0);
         // the rows' maxima, weights and sums
         float x0 = -INFINITY, x1 = -INFINITY;
-        const int lim0 = last0 - key0 - 2 * t, lim1 = last1 - key0 - 2 * t;        // places up to them are seen
+        const int lim0 = last0 - key0 - g, lim1 = last1 - key0 - g;    // places up to them are seen
 #pragma unroll
-        for (int n = 0; n < kPage / 8; ++n) {
-            c[n][0] = 8 * n <= lim0 ? c[n][0] * sl2 : -INFINITY, c[n][1] = 8 * n + 1 <= lim0 ? c[n][1] * sl2 : -INFINITY;
-            c[n][2] = 8 * n <= lim1 ? c[n][2] * sl2 : -INFINITY, c[n][3] = 8 * n + 1 <= lim1 ? c[n][3] * sl2 : -INFINITY;
-            x0 = fmaxf(x0, fmaxf(c[n][0], c[n][1])), x1 = fmaxf(x1, fmaxf(c[n][2], c[n][3]));
+        for (int m = 0; m < MT; ++m) {
+            c[m][0] = 16 * m <= lim0 ? c[m][0] * sl2 : -INFINITY, c[m][1] = 16 * m <= lim1 ? c[m][1] * sl2 : -INFINITY;
+            c[m][2] = 16 * m + 8 <= lim0 ? c[m][2] * sl2 : -INFINITY, c[m][3] = 16 * m + 8 <= lim1 ? c[m][3] * sl2 : -INFINITY;
+            x0 = fmaxf(x0, fmaxf(c[m][0], c[m][2])), x1 = fmaxf(x1, fmaxf(c[m][1], c[m][3]));
         }
 #pragma unroll
-        for (int d = 1; d <= 2; d <<= 1) {
+        for (int d = 4; d <= 16; d <<= 1) {
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
         }
@@ -182,66 +183,57 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
         const float a0 = weight(m0, n0), a1 = weight(m1, n1), z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
         m0 = n0, m1 = n1;
         l0 *= a0, l1 *= a1;
-        uint32_t pa[kPage / 16][4];
+        uint32_t pb[MT][2];
 #pragma unroll
-        for (int n = 0; n < kPage / 8; ++n) {
-            const __nv_bfloat162 p = __floats2bfloat162_rn(exp2f(c[n][0] - z0), exp2f(c[n][1] - z0));
-            const float2 pf = __bfloat1622float2(p);
-            l0 += pf.x + pf.y;
-            pa[n / 2][(n & 1) * 2] = *reinterpret_cast<const uint32_t*>(&p);
-            pa[n / 2][(n & 1) * 2 + 1] = 0u;
-        }
-        if (upper) {
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int n = 0; n < kPage / 8; ++n) {
-                const __nv_bfloat162 r = __floats2bfloat162_rn(exp2f(c[n][2] - z1), exp2f(c[n][3] - z1));
-                const float2 rf = __bfloat1622float2(r);
-                l1 += rf.x + rf.y;
-                pa[n / 2][(n & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&r);
+            for (int h = 0; h < 2; ++h) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(exp2f(c[m][2 * h] - z0), exp2f(c[m][2 * h + 1] - z1));
+                const float2 pf = __bfloat1622float2(p);
+                l0 += pf.x, l1 += pf.y;
+                pb[m][h] = transpose8x8(*reinterpret_cast<const uint32_t*>(&p));
             }
-        }
 #pragma unroll
-        for (int i = 0; i < NT; ++i) o[i][0] *= a0, o[i][1] *= a0, o[i][2] *= a1, o[i][3] *= a1;
+        for (int i = 0; i < KS; ++i) o[i][0] *= a0, o[i][1] *= a1, o[i][2] *= a0, o[i][3] *= a1;
         ok = __all_sync(0xffffffffu, mbar_wait(&sm.v_full, turn, &sm.abort_flag, status, 7));
         if (!ok) break;
+        if (valid < kPage) {                           // places without a token may hold anything: zeros
+            for (int i = max(valid, 0) * (HD / 8) + lane; i < kPage * (HD / 8); i += 32)
+                *reinterpret_cast<uint4*>(sm.v + tile_off(i / (HD / 8), i % (HD / 8))) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+        }
 #pragma unroll
-        for (int ks = 0; ks < kPage / 16; ++ks)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < NT; i += 2) {
-                uint32_t vb[4];
-                ldsm_x4_trans(vb, v_s + tile_off(ks * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), i + (lane >> 4)));
-                if (valid < kPage) {                                   // places without a token may hold anything: zeros
-                    const int left = valid - ks * 16 - 2 * t;
-                    const uint32_t f0 = left >= 2 ? 0xffffffffu : (left == 1 ? 0xffffu : 0u), f1 = left >= 10 ? 0xffffffffu : (left == 9 ? 0xffffu : 0u);
-                    vb[0] &= f0, vb[1] &= f1, vb[2] &= f0, vb[3] &= f1;
-                }
-                mma16816(o[i], pa[ks], vb[0], vb[1]);
-                mma16816(o[i + 1], pa[ks], vb[2], vb[3]);
+            for (int i = 0; i < KS; ++i) {
+                uint32_t va[4];
+                ldsm_x4_trans(va, v_s + tile_off(m * 16 + (lane >> 4) * 8 + (lane & 7), 2 * i + ((lane >> 3) & 1)));
+                mma16816(o[i], va, pb[m][0], pb[m][1]);
             }
         if (next.any) copy(1);
         if (last) {
             float* rec = records + (int64_t)record * REC;
             float s0 = l0, s1 = l1;
 #pragma unroll
-            for (int d = 1; d <= 2; d <<= 1) {
+            for (int d = 4; d <= 16; d <<= 1) {
                 s0 += __shfl_xor_sync(0xffffffffu, s0, d);
                 s1 += __shfl_xor_sync(0xffffffffu, s1, d);
             }
-            if (t == 0) {
-                *reinterpret_cast<float2*>(rec + R * HD + 2 * g) = make_float2(m0, s0);
-                *reinterpret_cast<float2*>(rec + R * HD + 2 * (g + 8)) = make_float2(m1, s1);
-            }
+            if (g == 0) *reinterpret_cast<float4*>(rec + R * HD + 4 * t) = make_float4(m0, s0, m1, s1);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int c0 = j * 8 + 2 * t;
-                if (last0 >= 0) *reinterpret_cast<float2*>(rec + ((c0 >> 2) * R + g) * 4 + (c0 & 3)) = make_float2(o[j][0], o[j][1]);
-                if (last1 >= 0) *reinterpret_cast<float2*>(rec + ((c0 >> 2) * R + g + 8) * 4 + (c0 & 3)) = make_float2(o[j][2], o[j][3]);
-            }
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int col = 16 * i + 8 * h + g;
+                    float* at = rec + ((col >> 2) * R + 2 * t) * 4 + (col & 3);
+                    if (last0 >= 0) at[0] = o[i][2 * h];
+                    if (last1 >= 0) at[4] = o[i][2 * h + 1];
+                }
         }
     }
     if (blockIdx.x == 0) {
         pdl_wait();
-        Walk<OwnParts>(parts, gridDim.x, plan);
+        Walk(parts, gridDim.x, plan);
         clear_unfit(parts, out, G.heads * HD, status);
     }
     pdl_wait();                                        // (whoever waits for this kernel waits for the one before it too)

@@ -94,10 +94,10 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     // (The description lies ready before the step's kernels start; the plan is written behind the wait.)
-    Walk<SharedParts> walk(SharedParts{G}, gridDim.x, nullptr);    // (every warp walks on its own)
+    Runs runs(G, gridDim.x);                           // (every warp knows them on its own)
     pdl_wait();
     pdl_trigger();                                     // (behind the wait: the next kernel reads what this one reads without a wait of its own)
-    if (blockIdx.x == 0 && warp == 2) Walk<SharedParts>(SharedParts{G}, gridDim.x, plan);
+    if (blockIdx.x == 0 && warp == 2) Runs(G, gridDim.x).write(plan);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -115,14 +115,15 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const bool one = elect_one();
         int slot = 0, turn = 0;                        // of the ring
 #pragma unroll 1
-        for (; ok && walk.segment(seg); ++k) {
+        for (int at = blockIdx.x; ok && at < runs.all; at += gridDim.x, ++k) {
+            seg = runs.segment(at);
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
             const int* table = G.page_table + (int64_t)seg.cut.seq * G.table_width;
             // A lane holds a page number of each of two runs of 32, read ahead.
             auto pages = [&](int run) {
-                const int at = 2 * seg.from + run * 32 + lane;
-                int page = at < seg.cut.pages ? table[at] : 0;
+                const int j = 2 * seg.from + run * 32 + lane;
+                int page = j < seg.cut.pages ? table[j] : 0;
                 if (page < 0 || page >= kv_pages) {
                     atomicCAS(status, 0, 10);
                     page = 0;
@@ -186,7 +187,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             return here;
         };
 #pragma unroll 1
-        for (; ok && walk.segment(seg); ++k) {
+        for (int at = blockIdx.x; ok && at < runs.all; at += gridDim.x, ++k) {
+            seg = runs.segment(at);
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
             const int N = split ? n : 2 * n;           // turns
@@ -257,7 +259,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const uint32_t s_addr = lane_base + COL_S + s * BK, o_addr = lane_base + COL_O + s * HD;
         int step = 0, uses0 = 0, uses1 = 0, joins = 0; // this stream's blocks, both streams' runs, joins so far
 #pragma unroll 1
-        for (; ok && walk.segment(seg); ++k) {
+        for (int at = blockIdx.x; ok && at < runs.all; at += gridDim.x, ++k) {
+            seg = runs.segment(at);
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
             const int tile = seg.tile + (split ? 0 : s), n_rows = min(G.rows, seg.cut.n_tok * G.gs - tile * G.rows);
