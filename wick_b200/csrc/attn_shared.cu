@@ -544,18 +544,24 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
     } else {
         G.rows = R, G.gs = group, G.per_kv = 1, G.columns = kv_heads, G.block = 1, G.pair = 1;
     }
-    // The own keys' kernel starts as soon as all of the first one's thread blocks run, on the SMs that those leave.  (An
-    // environment variable sets the share, for measurements.)
-    // No more thread blocks than there can be runs of work.
+    // No more thread blocks than there can be runs of work.  The own keys' kernel starts as soon as all thread blocks of the first one run, on the
+    // SMs that those leave: shares by what each is expected to take, a turn of two blocks (1.2 of them where one tile takes both streams)
+    // 2,300 clocks of an SM, a page of own keys 1,500.  (Lengths are on the device: groups of equal size are assumed, that share half of the most
+    // pages where there are several, and half of the most own positions.)
     const int64_t tiles = (int64_t)ceil_div((int64_t)n_tokens * G.gs, G.rows) + n_groups, items = (tiles / G.pair + n_groups) * G.columns;
     const int64_t units = tiles * G.columns * ceil_div(max_pages, G.block);
-    const int sms = sm_count();
-    const int own_per_sm = c.fast ? OWN_WARPS * (128 / HD) : PER_SM;
-    int first = c.fast ? sms : PER_SM * sms, second = own_per_sm * sms;
+    const int sms = sm_count(), own_per_sm = c.fast ? OWN_WARPS * (128 / HD) : PER_SM;
+    int first = (c.fast ? 1 : PER_SM) * sms, second = own_per_sm * sms;
     if (c.fast && max_pages > 0) {
+        const int per_group = ceil_div(ceil_div(n_tokens, n_groups) * (int64_t)G.gs, G.rows);
+        const double work = (double)n_groups * G.columns * per_group * (per_group == 1 ? 0.6 : 1.0) * ceil_div(max_pages, 2) * (n_groups > 1 ? 0.5 : 1.0) * 2300;
+        const double work_own = (double)n_seqs * kv_heads * (0.5 * own_bound / kPage + 0.5) * 1500;
         const char* e = getenv("WICK_SPLIT");
-        const double share = e ? atof(e) : 1.0;
-        if (share < 1.0) first = max(1, (int)(sms * share)), second = own_per_sm * (sms - first);
+        const double share = e ? atof(e) : work / (work + work_own);
+        if (e && share < 0) fprintf(stderr, "share %.2f\n", work / (work + work_own));
+        const double sh = e && share < 0 ? work / (work + work_own) : share;
+        first = (int)min((int64_t)max(1, min(sms - 8, (int)(sms * sh))), max((int64_t)1, units / G.pair));
+        second = own_per_sm * (sms - first);
     }
     c.blocks = (int)max((int64_t)1, min((int64_t)first, units / G.pair));
     const int rows_own = c.fast ? OWN_ROWS : R;

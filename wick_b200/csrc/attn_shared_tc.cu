@@ -15,7 +15,7 @@
 //     block's maximum exceeds it by more than 8 (in units of log2 e).  Warps whose rows are all beyond the group's tokens compute nothing.
 // REHEARSE: a run has few blocks, and a block's code is met for the first time while all SMs fill their rings: instructions then
 // come through the same queues as 24 MB of keys and values, and the first block's softmax took 4,300 clocks, the first products 4,100.
-// So the softmax warps go through their code once while there is nothing to do yet, and the issuing warp's code is loops.
+// So the softmax warps go through their code once while there is nothing to do yet.
 // Every wait is bounded and reports through the status word (code 7).
 #include "tc_attention.cuh"
 #include "attn_shared.cuh"
@@ -50,18 +50,6 @@ struct Smem {
 };
 constexpr int SMEM_BYTES = (2 + NSLOT) * TILE_BYTES + (int)sizeof(Smem);
 static_assert(SMEM_BYTES <= 227 * 1024, "a block's shared memory");
-
-// D (tensor memory) (+)= A (shared memory) * B (shared memory)
-__device__ __forceinline__ void mma_ss_acc(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, int acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %3};\n\t"
-        "mov.b64 db, {%2, %3};\n\t"
-        "setp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
-        ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "r"(acc)
-        : "memory");
-}
 
 __global__ void __launch_bounds__(THREADS, 1)
 attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const Groups G, int64_t kv_pages, float scale,
@@ -192,7 +180,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
             const int N = split ? n : 2 * n;           // turns
-            // turn i: stream i & 1's product of one block, then its scores of the next.  (Instructions in loops: see REHEARSE.)
+            // turn i: stream i & 1's product of one block, then its scores of the next.
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, k & 1, abort_flag, status, 7));
 #pragma unroll 1
             for (int i = -2; ok && i < N; ++i) {
@@ -213,11 +201,9 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                         tc_fence_after();
                         if (one && part < parts) {
                             int begun = i >= 2 || part > 0;
-#pragma unroll 1
-                            for (int ks = 0; ks < P_FIRST / 16; ++ks, pp += 8, vp += 2048 >> 4) {
-                                mma_ts(d, pp, vp, idesc_o, begun);
-                                begun = 1;
-                            }
+                            mma_ts(d, pp, vp, idesc_o, begun);
+                            static_for<1, P_FIRST / 16>([&](auto ks) { mma_ts(d, pp + (int)ks * 8, vp + (int)ks * (2048 >> 4), idesc_o, 1); });
+                            pp += 8 * (P_FIRST / 16), vp += (P_FIRST / 16) * (2048 >> 4);
                         }
                     }
                     if (!ok) break;
@@ -235,12 +221,10 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                     uint32_t k_lo = k_lo0 + k_at * (TILE_BYTES >> 4), q_lo = q_lo0 + (split ? 0 : s * (TILE_BYTES >> 4));
                     const uint32_t d = tmem + COL_S + s * BK;
                     if (one) {
-#pragma unroll 1
-                        for (int ks = 0; ks < HD / 16; ++ks) {
-                            mma_ss_acc(d, q_lo, k_lo, idesc_s, ks > 0);
-                            const uint32_t step = (ks & 3) == 3 ? (PANEL_BYTES - 96) >> 4 : 32 >> 4;   // (four steps of 32 bytes a panel)
-                            q_lo += step, k_lo += step;
-                        }
+                        static_for<0, HD / 16>([&](auto ks) {
+                            constexpr uint32_t off = (((int)ks >> 2) * PANEL_BYTES + ((int)ks & 3) * 32) >> 4;
+                            mma_ss<((int)ks > 0)>(d, q_lo + off, k_lo + off, idesc_s);
+                        });
                         tc_commit(&sh.s_full[s]);
                         if (split || s == 1) tc_commit(&sh.empty[k_at]);
                         if (i + 2 == N - 1) tc_commit(&sh.q_empty);            // (the run's last scores)
