@@ -2,8 +2,7 @@
 // mathematics and how the work is cut): the entry points, and the form for any head size in float32, and in bfloat16 for head sizes
 // other than 64 and 128 (those: attn_shared_tc.cu, attn_shared_own.cu).
 //
-//   1. attn_shared_part_kernel over the groups' shared keys, then over the sequences' own ones: tiles of 16 rows, a record (m, l, o) per
-//      run of units;
+//   1. attn_shared_part_kernel over the sequences' own keys and the groups' shared ones: tiles of 16 rows, a record (m, l, o) per run;
 //   2. attn_shared_join_kernel: a row's records joined and written.
 //
 // bfloat16: mma.sync on tiles of 16 rows and 16 keys.  Keys and values go from the cache straight to registers: the inner index of
@@ -377,53 +376,37 @@ template <typename T> __device__ __forceinline__ void write_record(const Work<T>
 }
 
 // ---- the parts ---------------------------------------------------------------------
-// OWN: the own keys, else the shared ones.  wait_first: whether something before this kernel may still run that it reads the results of
-// (the own keys' kernel comes behind the shared ones', which has waited for q and the cache).
-template <typename T, bool OWN>
+template <typename T>
 __global__ void __launch_bounds__(THREADS)
-attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, T* __restrict__ out, const Groups G, int wait_first,
-                        float scale, int* plan, float* records, int* status) {
+attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, T* __restrict__ out, const Groups G, int groups, float scale, int* plan,
+                        float* records, int* status) {
     extern __shared__ __align__(16) uint8_t smem[];
     Work<T>& w = *reinterpret_cast<Work<T>*>(smem);
     __shared__ Rows<T> rows;
-    if (wait_first) pdl_wait();
-    pdl_trigger();                                  // (behind the wait, so that the next kernel need not wait for what this one waited for)
+    pdl_trigger();
+    const int group = G.heads / G.kv_heads;
+    const OwnParts parts{G, R, groups};
+    Walk walk(parts, gridDim.x, nullptr);           // (the description may be read before the wait)
+    pdl_wait();
     q = fresh(q);
-    const int gs = OWN ? G.heads / G.kv_heads : G.gs;
-    const OwnParts own{G, R};
-    auto work = [&](const Segment& s) {
+    Segment s;
+    while (walk.segment(s)) {                       // (every warp walks the same way)
         __syncthreads();                            // (the rows and the work of the segment before)
         if (threadIdx.x < R) {
-            const int idx = s.tile * R + threadIdx.x, tok = idx / gs;
-            const bool there = idx < s.cut.n_tok * gs;
-            rows.q[threadIdx.x] = there ? q + ((int64_t)(s.cut.tok0 + tok) * G.heads + s.column * gs + idx - tok * gs) * HD : nullptr;
-            rows.last[threadIdx.x] = !there ? -1 : (OWN ? s.cut.end - s.cut.n_tok + tok : s.cut.end - 1);
+            const int idx = s.tile * R + threadIdx.x, tok = idx / group;
+            const bool there = idx < s.cut.n_tok * group;
+            rows.q[threadIdx.x] = there ? q + ((int64_t)(s.cut.tok0 + tok) * G.heads + s.column * group + idx - tok * group) * HD : nullptr;
+            rows.last[threadIdx.x] = there ? s.last(tok) : -1;
         }
         __syncthreads();
-        attend(w, rows, kv, kv_pages, G.page_table + (int64_t)s.cut.seq * G.table_width, s.column / (OWN ? 1 : G.per_kv), G.kv_heads,
-               (s.cut.first + s.from) * kPage, min((s.cut.first + s.to) * kPage, s.cut.end), scale, status);
+        attend(w, rows, kv, kv_pages, G.page_table + (int64_t)s.cut.seq * G.table_width, s.column, G.kv_heads, (s.cut.first + s.from) * kPage,
+               min((s.cut.first + s.to) * kPage, s.cut.end), scale, status);
         write_record(w, records + (int64_t)s.record * REC);
-    };
-    if constexpr (OWN) {                            // (every warp walks the same way)
-        Walk walk(own, gridDim.x, nullptr);
-        Segment s;
-        while (walk.segment(s)) work(s);
-    } else {
-        Runs runs(G, gridDim.x);
-        for (int r = blockIdx.x; r < runs.all; r += gridDim.x) work(runs.segment(r));
     }
-    if (blockIdx.x == 0) {
-        pdl_wait();
-        if (threadIdx.x < 32) {
-            if constexpr (OWN) {
-                Walk(own, gridDim.x, plan);
-                clear_unfit(own, out, G.heads * HD, status);
-            } else {
-                Runs(G, gridDim.x).write(plan);
-            }
-        }
+    if (blockIdx.x == 0 && threadIdx.x < 32) {
+        Walk(parts, gridDim.x, plan);
+        clear_unfit(parts, out, G.heads * HD, status);
     }
-    pdl_wait();                                     // (whoever waits for this kernel waits for the one before it too)
 }
 
 // ---- the records joined ------------------------------------------------------------
@@ -442,9 +425,10 @@ __device__ __forceinline__ Source shared_source(const Groups& G, const Records& 
     return s;
 }
 __device__ __forceinline__ Source own_source(const OwnParts& parts, const Records& rec, int b, const Cut& c, int idx, int kvh) {
+    if (c.pages == 0) return Source{rec.at, 0, 0, rec.rows, 0};
     const int *units = rec.plan + 1, *items = rec.plan + 2 + parts.n();
     const Deal deal(units[parts.n()], rec.plan[0]);
-    const int tile = idx / parts.rows, item = tile * parts.columns() + kvh, u = units[b] + item * c.pages, c0 = deal.worker_of(u);
+    const int tile = idx / parts.rows, item = tile * parts.G.kv_heads + kvh, u = units[b] + item * c.pages, c0 = deal.worker_of(u);
     const int floats = rec.rows * (HD + 2);
     return Source{rec.at + (int64_t)(items[b] + item + c0) * floats, deal.worker_of(u + c.pages - 1) - c0 + 1, floats, rec.rows, idx - tile * parts.rows};
 }
@@ -455,14 +439,14 @@ __device__ __forceinline__ Source own_source(const OwnParts& parts, const Record
 constexpr int JT = 128, JR = 4;
 template <typename T>
 __global__ void __launch_bounds__(JT)
-attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records shared, const Records own) {
+attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records shared, const Records own, int groups) {
     const int b = blockIdx.y, row = (int)blockIdx.x * JR + (int)threadIdx.x % JR, group = G.heads / G.kv_heads;
-    const OwnParts parts{G, own.rows};
+    const OwnParts parts{G, own.rows, groups};
     const Cut mine = parts(b);                      // (the description may be read before the wait)
     const int tok = row / G.heads, head = row - tok * G.heads, kvh = head / group, h = head - kvh * group, g = G.group_of[b];
     const bool there = tok < mine.n_tok && mine.pages > 0;
     Cut c = Cut{0, 0, 0, 0, 0, 0, 0, 0};
-    if (there) c = SharedParts{G}(g);
+    if (there) c = groups ? parts(G.n_seqs + g) : SharedParts{G}(g);
     pdl_wait();
     pdl_trigger();
     Source src = {nullptr, 0, 0, 0, 0};
@@ -472,7 +456,11 @@ attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records share
         float m = -INFINITY, l = 0.f;
 #pragma unroll 1
         for (int kind = 0; kind < 2; ++kind) {
-            if (there) src = kind == 0 ? shared_source(G, shared, g, c, mine.tok0 + tok, h, kvh) : own_source(parts, own, b, mine, tok * group + h, kvh);
+            if (there) {
+                if (kind == 0 && !groups) src = shared_source(G, shared, g, c, mine.tok0 + tok, h, kvh);
+                else if (kind == 0) src = own_source(parts, own, G.n_seqs + g, c, (mine.tok0 + tok - c.tok0) * group + h, kvh);
+                else src = own_source(parts, own, b, mine, tok * group + h, kvh);
+            }
             const float *sums = src.at + (min(col, HD / 4 - 1) * src.rows + src.r) * 4, *ml = src.at + src.rows * HD + 2 * src.r;
 #pragma unroll 1
             for (int i0 = 0; __any_sync(0xffffffffu, i0 < src.n); i0 += 8) {
@@ -515,11 +503,13 @@ using namespace wick;
 namespace wick {
 namespace shared_prefix {
 
+constexpr int FEW = 2000 * (HD < 128 ? 2 : 1);
 constexpr int PER_SM = 2;                          // thread blocks an SM, where the tcgen05 kernel does not run
 
 struct Call {
     Groups G;
     bool fast;                                     // the forms for bfloat16 at head sizes 64 and 128
+    bool tc;                                       // the shared keys have a kernel of their own
     int blocks, blocks_own;                        // for the shared keys, for the own ones
     int64_t plan_shared, plan_own, shared_floats, own_floats;
     int64_t all() const { return plan_shared + plan_own + shared_floats + own_floats; }
@@ -535,58 +525,44 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
     G.n = n_groups, G.n_seqs = n_seqs, G.max_pages = max_pages, G.heads = heads, G.kv_heads = kv_heads;
     G.single = max_q_len == 1 && n_tokens == n_seqs;
     c.fast = half && fast_supported();
-    if (c.fast) {
-        // heads of a tile: all of a key head's, or as many as 128 rows hold of more
-        int gs = group;
-        for (int n = 2; gs > TC_ROWS; ++n)
-            if (group % n == 0) gs = group / n;
-        G.rows = TC_ROWS / gs * gs, G.gs = gs, G.per_kv = group / gs, G.columns = heads / gs, G.block = 2, G.pair = 2;
-    } else {
-        G.rows = R, G.gs = group, G.per_kv = 1, G.columns = kv_heads, G.block = 1, G.pair = 1;
-    }
-    // No more thread blocks than there can be runs of work.  The own keys' kernel starts as soon as all thread blocks of the first one run, on the
-    // SMs that those leave: shares by what each is expected to take, a turn of two blocks (1.2 of them where one tile takes both streams)
-    // 2,300 clocks of an SM, a page of own keys 1,500.  (Lengths are on the device: groups of equal size are assumed, that share half of the most
-    // pages where there are several, and half of the most own positions.)
-    const int64_t tiles = (int64_t)ceil_div((int64_t)n_tokens * G.gs, G.rows) + n_groups, items = (tiles / G.pair + n_groups) * G.columns;
-    const int64_t units = tiles * G.columns * ceil_div(max_pages, G.block);
-    const int sms = sm_count(), own_per_sm = c.fast ? OWN_WARPS * (128 / HD) : PER_SM;
-    int first = (c.fast ? 1 : PER_SM) * sms, second = own_per_sm * sms;
-    if (c.fast && max_pages > 0) {
-        const int per_group = ceil_div(ceil_div(n_tokens, n_groups) * (int64_t)G.gs, G.rows);
-        const double work = (double)n_groups * G.columns * per_group * (per_group == 1 ? 0.6 : 1.0) * ceil_div(max_pages, 2) * (n_groups > 1 ? 0.5 : 1.0) * 2300;
-        const double work_own = (double)n_seqs * kv_heads * (0.5 * own_bound / kPage + 0.5) * 1500;
-        const char* e = getenv("WICK_SPLIT");
-        const double share = e ? atof(e) : work / (work + work_own);
-        if (e && share < 0) fprintf(stderr, "share %.2f\n", work / (work + work_own));
-        const double sh = e && share < 0 ? work / (work + work_own) : share;
-        first = (int)min((int64_t)max(1, min(sms - 8, (int)(sms * sh))), max((int64_t)1, units / G.pair));
+    // heads of a tcgen05 tile: all of a key head's, or as many as 128 rows hold of more
+    int gs = group;
+    for (int n = 2; gs > TC_ROWS; ++n)
+        if (group % n == 0) gs = group / n;
+    G.rows = TC_ROWS / gs * gs, G.gs = gs, G.per_kv = group / gs, G.columns = heads / gs, G.block = 2, G.pair = 2;
+    const int sms = sm_count(), rows_own = c.fast ? OWN_ROWS : R, own_per_sm = c.fast ? OWN_WARPS * (128 / HD) : PER_SM;
+    const int64_t tiles = (int64_t)ceil_div((int64_t)n_tokens * gs, G.rows) + n_groups, items = (tiles / 2 + n_groups) * G.columns;
+    const int64_t units = tiles * G.columns * ceil_div(max_pages, 2);
+    const int64_t items_seqs = ((int64_t)ceil_div((int64_t)n_tokens * group, rows_own) + n_seqs) * kv_heads, pages_own = ceil_div(own_bound, kPage);
+    const int64_t items_groups = max_pages > 0 ? ((int64_t)ceil_div((int64_t)n_tokens * group, rows_own) + n_groups) * kv_heads : 0;
+    WICK_REQUIRE(units <= INT32_MAX / 2 && items_seqs * pages_own + items_groups * max_pages <= INT32_MAX / 2, "attention (shared prefix): too much for one step");
+    // The shared keys have a kernel of their own from FEW pages of 8 rows on: fewer take the own keys' kernel, and one launch, less time (16
+    // sequences of 32 heads over 8 of 128: behind 1,024 positions 13.1 us together and 15.9 apart, 4,096 21.8 and 18.1; 48 of 24 over 4 of
+    // 64: 1,024 15.1 and 17.5, 4,096 26.7 and 21.4).
+    c.tc = c.fast && items_groups * max_pages > FEW;
+    int first = sms, second = own_per_sm * sms;
+    if (c.tc) {
+        // The own keys' kernel starts as soon as all thread blocks of the first one run, on the SMs that those leave (64 sequences of 370 own
+        // positions behind 8,192 shared ones, 32 heads over 8: one behind the other 54 us, half of the SMs each 42; 24 behind 31,000, 64 over
+        // 8: 72, and 64 on four fifths and one).  Shares by what each is expected to take: a page of own keys a quarter of a turn
+        // of a tile and two pages, which takes 0.6 of one where the tile has both streams.  (Lengths are on the device: groups of equal
+        // size are assumed, that share 0.7 of the most pages where there are several, and half of the most own positions.)
+        const int per_group = ceil_div(ceil_div(n_tokens, n_groups) * (int64_t)gs, G.rows);
+        const double work = (double)n_groups * G.columns * per_group * (per_group == 1 ? 0.6 : 1.0) * ceil_div(max_pages, 2) * (n_groups > 1 ? 0.7 : 1.0);
+        const double tiles_own = G.single ? (double)n_seqs * ceil_div(group, OWN_ROWS) : (double)n_tokens * group / OWN_ROWS + 0.5 * n_seqs;
+        const double work_own = tiles_own * kv_heads * (0.5 * own_bound / kPage + 0.5) * 0.26;
+        first = (int)min((int64_t)max(1, min(sms - 8, (int)(sms * work / (work + work_own)))), max((int64_t)1, units / 2));
         second = own_per_sm * (sms - first);
     }
-    c.blocks = (int)max((int64_t)1, min((int64_t)first, units / G.pair));
-    const int rows_own = c.fast ? OWN_ROWS : R;
-    const int64_t items_own = ((int64_t)ceil_div((int64_t)n_tokens * group, rows_own) + n_seqs) * kv_heads;
-    c.blocks_own = (int)max((int64_t)1, min((int64_t)second, items_own * ceil_div(own_bound, kPage)));
-    WICK_REQUIRE(units <= INT32_MAX / 2 && items_own * ceil_div(own_bound, kPage) <= INT32_MAX / 2, "attention (shared prefix): too much for one step");
-    c.plan_shared = max_pages > 0 ? (n_groups + 2 + 3) / 4 * 4 : 0;
-    c.plan_own = (2 * n_seqs + 3 + 3) / 4 * 4;
-    c.shared_floats = max_pages > 0 ? max((int64_t)c.blocks, items) * G.pair * (c.fast ? TC_ROWS : R) * (HD + 2) : 0;
+    // No more thread blocks than there can be runs of work.
+    const int64_t items_own = items_seqs + (c.tc ? 0 : items_groups);
+    c.blocks = (int)max((int64_t)1, min((int64_t)first, units / 2));
+    c.blocks_own = (int)max((int64_t)1, min((int64_t)second, items_seqs * pages_own + (c.tc ? 0 : items_groups * max_pages)));
+    c.plan_shared = c.tc ? (n_groups + 2 + 3) / 4 * 4 : 0;
+    c.plan_own = (2 * (n_seqs + n_groups) + 3 + 3) / 4 * 4;
+    c.shared_floats = c.tc ? max((int64_t)c.blocks, items) * 2 * TC_ROWS * (HD + 2) : 0;
     c.own_floats = (items_own + c.blocks_own) * rows_own * (HD + 2);
     return 0;
-}
-
-template <typename T, bool OWN>
-static int launch_part(const T* q, const T* kv, int64_t kv_pages, T* out, const Groups& G, bool wait_first, int blocks, float scale, int* plan,
-                       float* records, int* status, cudaStream_t s) {
-    constexpr int SMEM = (int)sizeof(Work<T>);
-    static bool raised = false;
-    if (!raised) {
-        WICK_CUDA(cudaFuncSetAttribute(attn_shared_part_kernel<T, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-        raised = true;
-    }
-    WICK_CUDA(launch(attn_shared_part_kernel<T, OWN>, dim3(blocks), dim3(THREADS), (size_t)SMEM, s, q, kv, kv_pages, out, G, (int)wait_first, scale,
-                     plan, records, status));
-    return check_launch("attn_shared_part");
 }
 
 template <typename T>
@@ -605,18 +581,24 @@ static int attn_shared(const T* q, int n_tokens, const T* kv, int64_t kv_pages, 
     G.table_width = table_width;
     int *plan = reinterpret_cast<int*>(scratch), *plan_own = plan + c.plan_shared;
     float *records = scratch + c.plan_shared + c.plan_own, *own = records + c.shared_floats;
-    const bool any = max_pages > 0;
+    const int groups = c.tc || max_pages == 0 ? 0 : n_groups;      // that the own keys' kernel takes too
     if (fast_supported() && sizeof(T) == 2) {
-        if (any)
+        if (c.tc)
             if (int e = launch_tc(q, n_tokens, kv, kv_pages, G, c.blocks, scale, plan, records, status, s)) return e;
-        if (int e = launch_own(q, kv, kv_pages, out, G, any, c.blocks_own, scale, plan_own, own, status, s)) return e;
+        if (int e = launch_own(q, kv, kv_pages, out, G, groups, c.tc, c.blocks_own, scale, plan_own, own, status, s)) return e;
     } else if constexpr (sizeof(T) == 4 || (HD != 64 && HD != 128)) {
-        if (any)
-            if (int e = launch_part<T, false>(q, kv, kv_pages, out, G, true, c.blocks, scale, plan, records, status, s)) return e;
-        if (int e = launch_part<T, true>(q, kv, kv_pages, out, G, !any, c.blocks_own, scale, plan_own, own, status, s)) return e;
+        constexpr int SMEM = (int)sizeof(Work<T>);
+        static bool raised = false;
+        if (!raised) {
+            WICK_CUDA(cudaFuncSetAttribute(attn_shared_part_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+            raised = true;
+        }
+        WICK_CUDA(launch(attn_shared_part_kernel<T>, dim3(c.blocks_own), dim3(THREADS), (size_t)SMEM, s, q, kv, kv_pages, out, G, groups, scale, plan_own, own,
+                         status));
+        if (int e = check_launch("attn_shared_part")) return e;
     }
-    const Records sh = {any ? plan : nullptr, records, c.fast ? TC_ROWS : R}, ow = {plan_own, own, c.fast ? OWN_ROWS : R};
-    WICK_CUDA(launch(attn_shared_join_kernel<T>, dim3(ceil_div((int64_t)max_q_len * heads, JR), n_seqs), dim3(JT), 0, s, out, G, sh, ow));
+    const Records sh = {c.tc ? plan : nullptr, records, TC_ROWS}, ow = {plan_own, own, c.fast ? OWN_ROWS : R};
+    WICK_CUDA(launch(attn_shared_join_kernel<T>, dim3(ceil_div((int64_t)max_q_len * heads, JR), n_seqs), dim3(JT), 0, s, out, G, sh, ow, groups));
     return check_launch("attn_shared_join");
 }
 

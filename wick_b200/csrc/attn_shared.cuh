@@ -8,8 +8,8 @@
 //
 // Shared keys: a tile (or, where a thread block takes two, a pair of neighbouring tiles) is an ITEM.  An item's blocks of G.block pages are cut
 // into RUNS of equal length, the longest that still gives every thread block one run (see Runs): what a run costs besides its blocks is
-// as much as three of them, so a thread block should not have two.  Own keys: a sequence's 16 or 8 rows of one key head are an item, whose
-// pages are dealt to the workers in equal contiguous runs, from one item into the next (see Walk).  Either way a record is
+// as much as three of them, so a thread block should not have two.  Own keys (and shared ones, where they are few): a sequence's 16 or 8 rows
+// of one key head are an item, whose pages are dealt to the workers in equal contiguous runs, from one item into the next (see Walk).  Either way a record is
 // written per run and item, and who has what follows from the description alone: the kernel that joins finds the records by
 // arithmetic, in a fixed order.
 #pragma once
@@ -54,24 +54,31 @@ struct SharedParts {
         return c;
     }
 };
-// The own keys of a sequence that does not fit its group or its page table: none.
+// What the workers of the own keys' kernel do: the own keys of each sequence (of one that does not fit its group or its page table:
+// none), and behind the last sequence, where no other kernel does them, the shared keys of each group.
 struct OwnParts {
     const Groups& G;
     int rows;                                      // of a tile
-    __device__ __forceinline__ int n() const { return G.n_seqs; }
-    __device__ __forceinline__ int columns() const { return G.kv_heads; }
+    int groups;                                    // that come behind the sequences
+    __device__ __forceinline__ int n() const { return G.n_seqs + groups; }
+    __device__ __forceinline__ bool shared(int i) const { return i >= G.n_seqs; }
     __device__ __forceinline__ bool fits(int b, const Cut& c) const {
         return G.group_of[b] >= 0 && G.group_of[b] < G.n && G.start[b] >= c.first * kPage && (c.end + kPage - 1) / kPage <= G.table_width;
     }
-    __device__ __forceinline__ Cut operator()(int b) const {
+    __device__ __forceinline__ Cut operator()(int i) const {
         Cut c;
-        const int g = G.group_of[b];
-        c.seq = b;
-        c.tok0 = G.single ? b : G.cu_seqlens[b];
-        c.n_tok = G.single ? 1 : G.cu_seqlens[b + 1] - c.tok0;
-        c.first = g >= 0 && g < G.n ? pages_of(G, g) : 0;
-        c.end = G.start[b] + c.n_tok;
-        c.blocks = c.pages = c.n_tok > 0 && fits(b, c) ? (c.end + kPage - 1) / kPage - c.first : 0;
+        if (shared(i)) {
+            c = SharedParts{G}(i - G.n_seqs);
+            c.blocks = c.pages;
+        } else {
+            const int g = G.group_of[i];
+            c.seq = i;
+            c.tok0 = G.single ? i : G.cu_seqlens[i];
+            c.n_tok = G.single ? 1 : G.cu_seqlens[i + 1] - c.tok0;
+            c.first = g >= 0 && g < G.n ? pages_of(G, g) : 0;
+            c.end = G.start[i] + c.n_tok;
+            c.blocks = c.pages = c.n_tok > 0 && fits(i, c) ? (c.end + kPage - 1) / kPage - c.first : 0;
+        }
         c.tiles = c.pages > 0 ? (c.n_tok * (G.heads / G.kv_heads) + rows - 1) / rows : 0;
         return c;
     }
@@ -79,9 +86,9 @@ struct OwnParts {
 // By a warp: the sequences that do not fit are reported, and their rows are made zero.
 template <typename T> __device__ __forceinline__ void clear_unfit(const OwnParts& parts, T* out, int row_numbers, int* status) {
     const int lane = threadIdx.x & 31;
-    for (int b0 = 0; b0 < parts.n(); b0 += 32) {
+    for (int b0 = 0; b0 < parts.G.n_seqs; b0 += 32) {
         Cut c = Cut{0, 0, 0, 0, 0, 0, 0, 0};
-        if (b0 + lane < parts.n()) c = parts(b0 + lane);
+        if (b0 + lane < parts.G.n_seqs) c = parts(b0 + lane);
         unsigned bad = __ballot_sync(0xffffffffu, c.n_tok > 0 && c.pages == 0);
         if (bad && lane == 0) atomicCAS(status, 0, 11);
         for (; bad; bad &= bad - 1) {
@@ -108,6 +115,9 @@ struct Segment {
     int tile, tiles, column;
     int from, to;
     int record;
+    bool shared;                                   // (Walk) a group's keys: every row sees all of them
+    // (Walk) the last position that a row of the thing's token `tok` sees
+    __device__ __forceinline__ int last(int tok) const { return shared ? cut.end - 1 : cut.end - cut.n_tok + tok; }
 };
 
 // ---- shared keys -------------------------------------------------------------------
@@ -205,7 +215,7 @@ struct Runs {
 };
 
 // ---- own keys ----------------------------------------------------------------------
-// A worker's way through its run; a worker is `blockIdx.x`.  A lane knows one sequence of 32.
+// A worker's way through its run; a worker is `blockIdx.x`.  A lane knows one sequence (or group) of 32.
 struct Walk {
     const OwnParts parts;
     Deal deal;
@@ -219,7 +229,7 @@ struct Walk {
         const int b = b0 + (int)(threadIdx.x & 31);
         mine = Cut{0, 0, 0, 0, 0, 0, 0, 0};
         if (b < parts.n()) mine = parts(b);
-        int y = mine.tiles * parts.columns(), x = y * mine.pages;
+        int y = mine.tiles * parts.G.kv_heads, x = y * mine.pages;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int tx = __shfl_up_sync(0xffffffffu, x, o), ty = __shfl_up_sync(0xffffffffu, y, o);
@@ -252,13 +262,14 @@ struct Walk {
     __device__ __forceinline__ bool segment(Segment& s) {
         if (u >= end) return false;
         while (u >= __shfl_sync(0xffffffffu, upto_units, 31)) next();
-        const int l = __ffs(__ballot_sync(0xffffffffu, u < upto_units)) - 1, columns = parts.columns();
+        const int l = __ffs(__ballot_sync(0xffffffffu, u < upto_units)) - 1, columns = parts.G.kv_heads;
         Cut& c = s.cut;
         c.pages = __shfl_sync(0xffffffffu, mine.pages, l), c.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);
         c.n_tok = __shfl_sync(0xffffffffu, mine.n_tok, l), c.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
         c.seq = __shfl_sync(0xffffffffu, mine.seq, l), c.blocks = c.pages;
         c.first = __shfl_sync(0xffffffffu, mine.first, l), c.end = __shfl_sync(0xffffffffu, mine.end, l);
         const int local = u - __shfl_sync(0xffffffffu, upto_units - mine.tiles * columns * mine.pages, l), item = local / c.pages;
+        s.shared = parts.shared(b0 + l);
         s.tile = item / columns, s.tiles = 1, s.column = item - s.tile * columns;
         s.from = local - item * c.pages, s.to = min(c.pages, s.from + end - u);
         // (items and workers rise together along the runs: no two parts share the sum)
@@ -287,7 +298,7 @@ constexpr int TC_ROWS = 128, OWN_ROWS = 8, OWN_WARPS = 6;    // (warps an SM at 
 bool fast_supported();
 int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, const Groups& G, int blocks, float scale, int* plan, float* records, int* status,
               cudaStream_t s);
-int launch_own(const void* q, const void* kv, int64_t kv_pages, void* out, const Groups& G, bool after_shared, int blocks, float scale, int* plan,
+int launch_own(const void* q, const void* kv, int64_t kv_pages, void* out, const Groups& G, int groups, bool after_shared, int blocks, float scale, int* plan,
                float* records, int* status, cudaStream_t s);
 
 }  // namespace shared_prefix

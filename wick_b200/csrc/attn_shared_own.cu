@@ -1,4 +1,5 @@
-// The own keys of each sequence behind its group's shared prefix: bfloat16, head sizes 64 and 128.
+// The own keys of each sequence behind its group's shared prefix, and shared keys that are too few for a kernel of their own: bfloat16,
+// head sizes 64 and 128.
 //
 // A thread block is ONE warp that feeds itself; six of them (head size 64: twelve) fill an SM's shared memory.  The pages of all items (a
 // sequence's 8 rows of one key head) are dealt to the warps in equal runs (attn_shared.cuh).  A warp has room for one page of keys and
@@ -71,7 +72,7 @@ struct Ahead {
 };
 
 __global__ void __launch_bounds__(32)
-attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q, int64_t kv_pages, bf16* __restrict__ out, const Groups G, int after_shared,
+attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q, int64_t kv_pages, bf16* __restrict__ out, const Groups G, int groups, int after_shared,
                        float scale, int* plan, float* records, int* status) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
@@ -87,7 +88,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
     // (With a shared part the kernel before this one is the one that computes it, and has waited for q and the cache.)
     if (!after_shared) pdl_wait();
     pdl_trigger();
-    const OwnParts parts{G, R};
+    const OwnParts parts{G, R, groups};
     Walk walk(parts, gridDim.x, nullptr);
     Ahead next = {};
     auto know_ids = [&]() {                            // from page next.j on
@@ -132,7 +133,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
         const int key0 = (next.s.cut.first + next.j) * kPage, valid = next.s.cut.end - key0;     // places of the page that hold a token
         const int record = next.s.record;
         if (first) {
-            const int row0 = next.s.tile * R, n_rows = next.s.cut.n_tok * group - row0, p0 = next.s.cut.end - next.s.cut.n_tok;
+            const int row0 = next.s.tile * R, n_rows = next.s.cut.n_tok * group - row0;
             const int tok = (row0 + g) / group;
             const bf16* q0 = q + ((int64_t)(next.s.cut.tok0 + tok) * G.heads + next.s.column * group + row0 + g - tok * group) * HD + 2 * t;
 #pragma unroll
@@ -140,7 +141,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
                 qb[i][0] = g < n_rows ? *reinterpret_cast<const uint32_t*>(q0 + i * 16) : 0u;
                 qb[i][1] = g < n_rows ? *reinterpret_cast<const uint32_t*>(q0 + i * 16 + 8) : 0u;
             }
-            last0 = 2 * t < n_rows ? p0 + (row0 + 2 * t) / group : -1, last1 = 2 * t + 1 < n_rows ? p0 + (row0 + 2 * t + 1) / group : -1;
+            last0 = 2 * t < n_rows ? next.s.last((row0 + 2 * t) / group) : -1, last1 = 2 * t + 1 < n_rows ? next.s.last((row0 + 2 * t + 1) / group) : -1;
             m0 = m1 = -INFINITY, l0 = l1 = 0.f;
 #pragma unroll
             for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -245,7 +246,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
 
 }  // namespace own
 
-int launch_own(const void* q, const void* kv, int64_t kv_pages, void* out, const Groups& G, bool after_shared, int blocks, float scale, int* plan,
+int launch_own(const void* q, const void* kv, int64_t kv_pages, void* out, const Groups& G, int groups, bool after_shared, int blocks, float scale, int* plan,
                float* records, int* status, cudaStream_t s) {
     using namespace own;
     CUtensorMap kv_map;
@@ -256,7 +257,7 @@ int launch_own(const void* q, const void* kv, int64_t kv_pages, void* out, const
         raised = true;
     }
     WICK_CUDA(launch(attn_shared_own_kernel, dim3(blocks), dim3(32), (size_t)SMEM_BYTES, s, kv_map, (const bf16*)q, kv_pages, (bf16*)out, G,
-                     (int)after_shared, scale, plan, records, status));
+                     groups, (int)after_shared, scale, plan, records, status));
     return check_launch("attn_shared_own");
 }
 
