@@ -29,6 +29,7 @@ from .models import kikopel as _kikopel  # noqa: F401
 from .models import saposun as _saposun  # noqa: F401
 from .models.model import Model
 from .models.spec import LayerSpec, ModelSpec, PartSpec, ScheduleEntry
+from .sampling.rules import LogitRules
 from .sampling.sampler import Rng, Sampler, SamplerConfig
 from .engine.generate import GenOptions, GenResult, generate
 from .weights.loader import WeightError, load_weights
@@ -42,11 +43,14 @@ def __getattr__(name):
     if name in ("Engine", "parse_dtype"):
         from .engine import engine as _e
         return getattr(_e, name)
+    if name == "sample_many":
+        from .engine.samples import sample_many
+        return sample_many
     raise AttributeError(name)
 
 
-__all__ = ["Architecture", "ConfigError", "Engine", "FasunexConfig", "GenOptions", "GenResult", "KikopelConfig", "LayerSpec", "Model", "ModelConfig",
+__all__ = ["Architecture", "ConfigError", "Engine", "FasunexConfig", "GenOptions", "GenResult", "KikopelConfig", "LayerSpec", "LogitRules", "Model", "ModelConfig",
            "ModelSpec", "NibotarConfig", "PartSpec", "Qwen3Config", "Rng", "SafeTensorsDir", "SafeTensorsError", "Sampler",
            "SamplerConfig", "SaposunConfig", "ScheduleEntry", "SunosunConfig", "TuguvikConfig", "WeightError", "architecture_names", "config_from_json", "generate",
-           "get_architecture", "load_config", "load_weights", "register_architecture", "write_random_model",
+           "get_architecture", "load_config", "load_weights", "register_architecture", "sample_many", "write_random_model",
            "write_safetensors"]

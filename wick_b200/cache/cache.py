@@ -90,6 +90,12 @@ class Storage:
     def open_seq(self, slot: int) -> None:
         """A sequence starts in ``slot``."""
 
+    def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Pages ``dst`` become copies of pages ``src`` (int64 on the device).  A kind without pages copies nothing."""
+
+    def copy_slots(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """The records of slots ``dst`` become copies of those of ``src`` (int64 on the device).  A kind without records copies nothing."""
+
     def read_bytes(self, cached_tokens: int, n_seqs: int) -> int:
         """Bytes a decode step reads from this group for ``n_seqs`` sequences that hold
         ``cached_tokens`` positions between them."""
@@ -99,7 +105,15 @@ class Storage:
         return torch.empty((), dtype=self.dtype).element_size()
 
 
-class PagedKV(Storage):
+class _Paged(Storage):
+    """Storage whose second dimension is the page."""
+
+    def copy_pages(self, src, dst):
+        for entry in self.tensor:                                    # (one entry's pages at a time: the copy in between stays small)
+            entry[dst] = entry[src]
+
+
+class PagedKV(_Paged):
     """Keys and values of every position: [entries, pages, 2, kv_heads, 64, head_dim].  Where
     values have a size of their own, a page is flat: [kv_heads, 64, head_dim] keys, then
     [kv_heads, 64, v_head_dim] values (with equal sizes the two forms are the same memory)."""
@@ -129,7 +143,7 @@ class PagedKV(Storage):
         return cached_tokens * self.bytes_per_token()
 
 
-class PagedRows(Storage):
+class PagedRows(_Paged):
     """One row of the need's ``shape`` per position: [entries, pages, 64, *shape].  A mixer
     sees its entry's part as ``rows``."""
     kind = "paged_rows"
@@ -150,7 +164,7 @@ class PagedRows(Storage):
         return cached_tokens * self.bytes_per_token()
 
 
-class PagedBlocks(Storage):
+class PagedBlocks(_Paged):
     """A key and a value for every whole block of the need's ``block`` positions, on the page that holds the block's last
     position: [entries, pages, kv_heads * rows * (head_dim + v_head_dim)], a page [kv_heads, rows, head_dim] keys, then
     [kv_heads, rows, v_head_dim] values, rows the most blocks that end on one page.  A mixer sees its entry's part as ``blocks``."""
@@ -187,6 +201,10 @@ class StateRecords(Storage):
     def open_seq(self, slot):
         if self.tensor is not None:
             self.tensor[:, slot].zero_()
+
+    def copy_slots(self, src, dst):
+        for entry in self.tensor:
+            entry[dst] = entry[src]
 
     def read_bytes(self, cached_tokens, n_seqs):
         n = self.element_size()
@@ -240,6 +258,7 @@ class Cache:
         self.pages = IndexPool(self.n_pages, reserved=(0,), what="page")
         self.slots = IndexPool(self.max_seqs + 1, reserved=(0,), what="slot")
         self.seqs: Dict[int, SeqRecord] = {}
+        self.lent: set = set()                                       # pages that no sequence holds (see lend)
         self.groups: List[_Group] = []
         # entry -> (group, index in the group), or a list of such for an entry that keeps several things
         self.entry_place: Dict[int, object] = {}
@@ -349,6 +368,32 @@ class Cache:
             self.pages.free(p)
         self.slots.free(slot)
 
+    # ---- pages without a sequence ----------------------------------------------
+    def lend(self, n: int) -> List[int]:
+        """``n`` pages for a batch that deals them to its sequences itself; they come back with :meth:`give_back`."""
+        if n > self.pages.n_free:
+            raise CacheFull(f"the cache is full: {n} pages of {PAGE} tokens wanted, {self.pages.n_free} are free of {self.pages.capacity}")
+        pages = self.pages.alloc_many(n)
+        self.lent.update(pages)
+        return pages
+
+    def give_back(self, pages: Sequence[int]) -> None:
+        for p in pages:
+            if p not in self.lent:
+                raise PoolError(f"page {p} is given back but was not lent")
+            self.lent.remove(p)
+            self.pages.free(p)
+
+    def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Copy the contents of pages ``src`` to pages ``dst`` (int64 on the device) in every group."""
+        for g in self.groups:
+            g.store.copy_pages(src, dst)
+
+    def copy_slots(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Copy the per-sequence records of slots ``src`` to slots ``dst`` (int64 on the device) in every group."""
+        for g in self.groups:
+            g.store.copy_slots(src, dst)
+
     def check(self) -> None:
         """Bookkeeping invariants: no page held by two sequences or by none."""
         self.pages.check()
@@ -363,7 +408,9 @@ class Cache:
                 if not self.pages.is_held(p):
                     raise PoolError(f"page {p} of slot {slot} is not held")
                 seen.add(p)
-        if seen != self.pages.held():
+        if seen & self.lent:
+            raise PoolError("a lent page is held by a sequence")
+        if seen | self.lent != self.pages.held():
             raise PoolError("a held page belongs to no sequence")
         if set(self.seqs) != self.slots.held():
             raise PoolError("a held slot has no record")

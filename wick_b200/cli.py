@@ -31,7 +31,10 @@ options:
   -t, --temperature <x>    sampling temperature, 0 = greedy (default 0.7)
       --top-k <n>          (default 40)     --top-p <x>   (default 0.9)
       --min-p <x>          (default 0)      --repeat-penalty <x> (default 1.0)
-      --seed <n>           RNG seed
+      --frequency-penalty <x>, --presence-penalty <x>       taken off the logits of generated tokens (default 0)
+      --logit-bias <id:x,...>  added to tokens' logits      --allow <a,b,c>  the only tokens that may be sampled
+      --samples <n>        continuations of every prompt, over one copy of its cache (default 1)
+      --seed <n>           RNG seed (continuation k: seed + k)
       --stop-id <id>       extra stop token (repeatable; the config's eos ids always stop)
   -q, --quant <fmt>        weights and activations: bf16 (default) or f32
   -c, --context <n>        context length per sequence (default 4096)
@@ -54,6 +57,8 @@ class Args:
         self.max_tokens = 256
         self.sampler = SamplerConfig()
         self.stop_ids: List[int] = []
+        self.rules: dict = {}
+        self.samples = 1
         self.quant = "bf16"
         self.context = 4096
         self.batch: Optional[int] = None
@@ -108,6 +113,20 @@ def parse_args(argv: List[str]) -> Args:
             a.sampler.min_p = num(float, arg)
         elif arg == "--repeat-penalty":
             a.sampler.repetition_penalty = num(float, arg)
+        elif arg in ("--frequency-penalty", "--presence-penalty"):
+            a.rules[arg[2:].replace("-", "_")] = num(float, arg)
+        elif arg == "--logit-bias":
+            text = num(str, arg)
+            try:
+                a.rules.setdefault("bias", {}).update((int(t), float(x)) for t, x in (pair.split(":") for pair in text.split(",") if pair))
+            except ValueError:
+                raise UsageError(f"bad value for {arg}: {text}") from None
+        elif arg == "--allow":
+            a.rules["allowed"] = a.rules.get("allowed", []) + _ids(num(str, arg))
+        elif arg == "--samples":
+            a.samples = num(int, arg)
+            if a.samples < 1:
+                raise UsageError(f"bad value for --samples: {a.samples}")
         elif arg == "--seed":
             a.sampler.seed = num(int, arg)
         elif arg == "--stop-id":
@@ -160,11 +179,19 @@ def cmd_run(a: Args) -> None:
     batch = a.batch or 64
     per_seq = [min(a.context, len(p) + a.max_tokens) for p in a.prompts]
     need = sum(sorted(((n + 63) // 64 * 64 for n in per_seq), reverse=True)[:batch])
+    if a.samples > 1:
+        # each prompt once, and its continuations' own positions (one batch of them at a time, as many prompts as it holds)
+        from .engine.samples import pages_of_batch
+        each = sorted((64 * pages_of_batch(len(p), n - len(p), min(a.samples, batch)) for p, n in zip(a.prompts, per_seq)), reverse=True)
+        need = sum(each[:max(1, batch // a.samples)])
     eng = _load(a, max(need, 64))
     # (the model's own end-of-sequence ids are added by the generation loop)
     opts = wick.GenOptions(max_tokens=a.max_tokens, sampler=a.sampler, stop_token_ids=a.stop_ids, context=a.context,
-                           max_batch=batch)
-    res = wick.generate(eng, a.prompts, opts)
+                           max_batch=batch, rules=wick.LogitRules(**a.rules) if a.rules else None)
+    if a.samples > 1:
+        res = [r for rs in wick.sample_many(eng, a.prompts, a.samples, opts) for r in rs]
+    else:
+        res = wick.generate(eng, a.prompts, opts)
     for r in res:
         print(json.dumps(r.tokens))
     for r in res:

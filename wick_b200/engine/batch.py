@@ -95,6 +95,8 @@ class StepBatch:
         self.slots = v(L.slots, L.n_seqs)
         self.page_table = v(L.page_table, L.n_seqs * L.table_width).view(L.n_seqs, L.table_width)
         self.want = v(L.want, L.n_want)
+        # Which sequences share their first pages (an ops.SharedPrefix), for mixers that read them once; None: nobody is known to.
+        self.shared = None
         # Values that several layers share within the step (position tables and
         # the like), keyed by whoever computes them.
         self.memo: Dict[object, object] = {}

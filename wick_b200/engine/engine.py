@@ -136,6 +136,7 @@ class Engine:
             use_graphs = os.environ.get("WICK_B200_NO_GRAPHS", "") == ""
         self.use_graphs = use_graphs
         self._graphs: Dict[Tuple[int, int], _DecodeGraph] = {}
+        self._shared_graphs: Dict[Tuple[int, int, int, int, int], _DecodeGraph] = {}
         # Short prompt steps are bound by the host's time per launch: they are captured too,
         # where every part of the model allows it (WICK_B200_NO_PROMPT_GRAPHS=1: never).
         self.prompt_graphs = (os.environ.get("WICK_B200_NO_PROMPT_GRAPHS", "") == "") and model.prompt_capturable()
@@ -222,11 +223,11 @@ class Engine:
         consecutive prompts in the same way).  Pages beyond the new length are given back."""
         self.cache.truncate(slot, length)
 
-    def begin_run(self, sampler, stop_token_ids=()):
+    def begin_run(self, sampler, stop_token_ids=(), rules=None):
         """A batch of sequences that start together and then decode on the device: see
         :class:`~wick_b200.engine.run.DeviceRun`."""
         from .run import DeviceRun
-        return DeviceRun(self, sampler, stop_token_ids)
+        return DeviceRun(self, sampler, stop_token_ids, rules)
 
     # ---- the step ------------------------------------------------------------
     def _check(self, slots, tokens, want) -> None:
@@ -401,6 +402,30 @@ class Engine:
             self._upload(g.layout, g.buffer, tokens=[[0]] * n_pad, starts=[0] * n_pad, slots=[0] * n_pad,
                          pages=[[0]] * n_pad, want=[[0]] * n_pad)
             self._capture(g)
+        return g
+
+    def shared_graph(self, n_seqs: int, width: int, n_groups: int, max_pages: int, own_bound: int) -> _DecodeGraph:
+        """The captured decode step for ``n_seqs`` sequences (padded, see :meth:`_bucket`) in ``n_groups`` groups that share up to
+        ``max_pages`` pages and hold up to ``own_bound`` positions behind them, with page tables of ``width`` columns; captured on
+        first use.  Beside the step's description it has ``batch.shared`` (whose tensors say who shares what, see
+        :class:`~wick_b200.ops.SharedPrefix`), ``rows`` (int32, of a sampler's rows), ``ones`` and ``slot_map`` for
+        :func:`~wick_b200.ops.step_tables`.  Graphs switched off: the same, not captured."""
+        n_pad = self._bucket(n_seqs)
+        key = (n_pad, width, n_groups, max_pages, own_bound)
+        g = self._shared_graphs.get(key)
+        if g is None:
+            g = _DecodeGraph(n_pad, width)
+            g.buffer = torch.zeros(g.layout.size, dtype=torch.int32, device=self.device)
+            g.batch = StepBatch(g.layout, g.buffer, q_lens=[1] * n_pad, starts=[0] * n_pad, workspace=self.workspace, kv_bound=width * PAGE)
+            make = lambda v: torch.tensor(v, dtype=torch.int32).to(self.device)      # noqa: E731
+            # (until told otherwise: padding entries, all of them in the last group)
+            g.batch.shared = ops.SharedPrefix(make([0] * n_groups + [n_pad]), make([0] * n_groups), make([n_groups - 1] * n_pad), max_pages, own_bound)
+            g.rows, g.ones = make([-1] * n_pad), make([1] * n_pad)
+            g.slot_map = torch.zeros(n_pad, dtype=torch.int64, device=self.device)
+            self._upload(g.layout, g.buffer, tokens=[[0]] * n_pad, starts=[0] * n_pad, slots=[0] * n_pad, pages=[[0]] * n_pad, want=[[0]] * n_pad)
+            if self.use_graphs:
+                self._capture(g)
+            self._shared_graphs[key] = g
         return g
 
     def _fill_graph_batch(self, g: _DecodeGraph, slots, tokens, starts) -> None:

@@ -25,6 +25,7 @@ import dataclasses
 import time
 from typing import Callable, List, Optional, Sequence
 
+from ..sampling.rules import LogitRules
 from ..sampling.sampler import Sampler, SamplerConfig
 from .run import StepRun
 
@@ -38,6 +39,7 @@ class GenOptions:
     stop_token_ids: Sequence[int] = ()
     context: int = 4096                 # tokens a sequence may hold (prompt + generated)
     max_batch: int = 64                 # sequences that start together
+    rules: Optional[LogitRules] = None  # penalties, biases and allowed tokens of every sequence, beside the sampler's options
 
 
 @dataclasses.dataclass
@@ -126,7 +128,9 @@ def generate(engine, prompts: Sequence[Sequence[int]], opts: Optional[GenOptions
         if run_factory is not None:
             return run_factory(engine, opts, stops, k)
         if sampler_factory is None and hasattr(engine, "begin_run"):
-            return engine.begin_run(opts.sampler, stops)
+            return engine.begin_run(opts.sampler, stops) if opts.rules is None else engine.begin_run(opts.sampler, stops, opts.rules)
+        if opts.rules is not None:
+            raise ValueError("rules on the logits need a batch that is stepped on the device")
         make_sampler = sampler_factory or (lambda cfg, m: Sampler(cfg, m))
         return StepRun(engine, make_sampler(opts.sampler, k), opts.sampler.repetition_penalty != 1.0)
 

@@ -35,6 +35,7 @@ import torch
 
 from .. import ops
 from ..cache import PAGE
+from ..sampling.rules import LogitRules, Steering
 from ..sampling.sampler import SamplerConfig, rng_state, sample_on_device
 
 
@@ -74,8 +75,11 @@ class StepRun:
 class DeviceRun:
     depth = 1
 
-    def __init__(self, engine, cfg: SamplerConfig, stop_token_ids: Sequence[int] = ()):
-        self.engine, self.cfg = engine, cfg
+    def __init__(self, engine, cfg: SamplerConfig, stop_token_ids: Sequence[int] = (), rules: Optional[LogitRules] = None):
+        self.engine, self.cfg, self.rules = engine, cfg, rules
+        self.steering: Optional[Steering] = None     # (with rules; they and the repetition penalty then go through one kernel)
+        self.row_of: Dict[int, int] = {}
+        self.rows: Optional[torch.Tensor] = None     # the step's rows, as far as a steering needs them
         dev = engine.device
         stops = sorted(set(int(t) for t in stop_token_ids))
         self.stops = torch.tensor(stops, dtype=torch.int32, device=dev) if stops else None
@@ -91,21 +95,32 @@ class DeviceRun:
         self.uploads = 0                     # descriptions copied to the device (a test reads it)
         self.h2d_bytes = 0
         self.left: Dict[int, int] = {}       # tokens each sequence may still be given, as far as the host knows
+        self._rows_for: Optional[tuple] = None
         self.last_logits: Optional[torch.Tensor] = None   # the last step's rows (a view: the next step overwrites them)
+
+    def _buffers(self, B: int) -> None:
+        """For the tokens of up to B rows a step."""
+        self.ids = torch.zeros(B + 1, dtype=torch.int32, device=self.engine.device)
+        self.uniforms = torch.zeros(B, dtype=torch.float32, device=self.engine.device)
+        for _ in range(self.depth + 2):
+            self._pinned.append(torch.zeros(B + 1, dtype=torch.int32, pin_memory=True))
+            self._events.append(torch.cuda.Event())
 
     # ---- the first step: all prompts ----
     def start(self, slots: Sequence[int], prompts: Sequence[Sequence[int]], limits: Sequence[int]) -> None:
         e = self.engine
         B = len(slots)
         dev = e.device
-        self.ids = torch.zeros(B + 1, dtype=torch.int32, device=dev)
-        self.uniforms = torch.zeros(B, dtype=torch.float32, device=dev)
-        for _ in range(self.depth + 2):
-            self._pinned.append(torch.zeros(B + 1, dtype=torch.int32, pin_memory=True))
-            self._events.append(torch.cuda.Event())
+        self._buffers(B)
         if self.cfg.temperature > 0.0:
             self.rng = torch.tensor([rng_state(self.cfg.seed)] * B, dtype=torch.int64).to(dev)
-        if self.cfg.repetition_penalty != 1.0:
+        if self.rules is not None:
+            self.steering = Steering([self.rules] * B, self.cfg.repetition_penalty, self.vocab, dev)
+            self.row_of = {s: i for i, s in enumerate(slots)}
+            told = torch.tensor([t for p in prompts for t in p], dtype=torch.int32).to(dev)
+            self.steering.said(told, torch.tensor([i for i, p in enumerate(prompts) for _ in p], dtype=torch.int32).to(dev), generated=False)
+            self.rows = torch.arange(B, dtype=torch.int32, device=dev)
+        elif self.cfg.repetition_penalty != 1.0:
             self.seen = torch.zeros((B, self.vocab), dtype=torch.uint8, device=dev)
         # the sequences' records: nothing cached, nothing generated, their limits and rows
         rec = np.zeros((B, ops.SEQ_STATE_WORDS + 1), dtype=np.int32)
@@ -124,7 +139,7 @@ class DeviceRun:
         with ops.stream_scope():
             if self.seen is not None:                    # (a captured step's padding tokens belong to slot 0: not marked)
                 ops.seen_prompt(self.seen, e.seq_state, batch.slots, batch.tokens, batch.seq_of_token)
-            self._sample_and_advance(logits[:B], batch.slots[:B], batch.kv_len[:B], B)
+            self._sample_and_advance(logits[:B], batch.slots[:B], batch.kv_len[:B], B, self.rows)
         self.last_logits = logits[:B]
         for s, q, lim in zip(slots, q_lens, limits):
             e.cache.advance(s, q)
@@ -150,6 +165,9 @@ class DeviceRun:
             g.composition = composition
             self.uploads += 1
             self.h2d_bytes += g.layout.size * 4
+        if self.steering is not None and self._rows_for != tuple(slots):
+            self.rows = torch.tensor([self.row_of[s] for s in slots], dtype=torch.int32).pin_memory().to(e.device, non_blocking=True)
+            self._rows_for = tuple(slots)
         b = g.batch
         with ops.stream_scope():
             ops.step_prepare(e.seq_state, b.slots, b.tokens, b.positions, b.start, b.kv_len)
@@ -160,19 +178,24 @@ class DeviceRun:
             else:                                        # (graphs switched off: the same step as separate launches)
                 b.memo.clear()
                 logits = e.model.forward(b, cache)
-            self._sample_and_advance(logits[:B], b.slots[:B], b.kv_len[:B], B)
+            self._sample_and_advance(logits[:B], b.slots[:B], b.kv_len[:B], B, self.rows)
         self.last_logits = logits[:B]
         for s in slots:
             cache.advance(s, 1)
             self.left[s] = self.left.get(s, 1) - 1
 
-    def _sample_and_advance(self, logits: torch.Tensor, slots_dev: torch.Tensor, kv_len_dev: torch.Tensor, B: int) -> None:
+    def _sample_and_advance(self, logits: torch.Tensor, slots_dev: torch.Tensor, kv_len_dev: torch.Tensor, B: int,
+                            rows: Optional[torch.Tensor] = None) -> None:
         e = self.engine
+        if self.steering is not None:
+            self.steering.apply(logits, rows)
         if self.seen is not None:
             ops.penalty_seen(logits, self.seen, e.seq_state, slots_dev, self.cfg.repetition_penalty)
         ids = self.ids[:B + 1]                       # the sampled tokens, then the kernels' status word
         sample_on_device(self.cfg, logits, lambda: ops.rng_uniforms(self.rng, e.seq_state, slots_dev, self.uniforms[:B]),
                          out=ids[:B])
+        if self.steering is not None:
+            self.steering.said(ids[:B], rows, generated=True)
         ops.step_advance(e.seq_state, slots_dev, ids, kv_len_dev, self.stops, self.seen, self.vocab)
         i = self._turn
         self._turn = (i + 1) % len(self._pinned)

@@ -312,7 +312,8 @@ class GQAttention(Mixer):
             cos = sin = None
             if inv_freq is not None:
                 cos, sin = self.position.tables(batch)
-            if batch.is_decode and qkv.shape[0] <= 8 and not ops.plain_kernels() and ops.attention_decode_parts_supported(
+            shared = getattr(batch, "shared", None) is not None and not ops.plain_kernels()
+            if batch.is_decode and not shared and qkv.shape[0] <= 8 and not ops.plain_kernels() and ops.attention_decode_parts_supported(
                     batch.n_seqs, self.heads, self.kv_heads, self.head_dim, self.ctx.dtype):
                 # the tensor-core decode attention: the projection's sums, the q/k norm, the rotation,
                 # the cache append, the attention and the merge in one or two launches
@@ -332,7 +333,11 @@ class GQAttention(Mixer):
                 cos=cos, sin=sin, kv=cache.kv, page_table=batch.page_table,
                 seq_of_token=batch.seq_of_token, positions=batch.positions, write_kv=write_cache,
                 dtype=self.ctx.dtype)
-        if batch.is_decode:
+        if getattr(batch, "shared", None) is not None and not ops.plain_kernels():
+            # groups of sequences share their first pages, which are read once for all of a group
+            need = ops.attention_shared_scratch(batch.shared, batch, self.heads, self.kv_heads, self.head_dim, self.ctx.dtype)
+            att = ops.attention_shared(q, cache.kv, batch, batch.shared, self.scale, batch.workspace.get("attention_shared", need, torch.float32))
+        elif batch.is_decode:
             need = ops.attention_decode_scratch_floats(batch.n_seqs, self.heads, self.head_dim, batch.kv_bound,
                                                        self.ctx.dtype)
             att = ops.attention_decode(q, cache.kv, batch, self.scale,
