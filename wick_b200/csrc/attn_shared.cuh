@@ -224,11 +224,12 @@ struct Walk {
     Cut mine;
     int upto_units, upto_items;                    // ... and up to this lane's
 
-    __device__ __forceinline__ void know(int first) {
-        b0 = first;
-        const int b = b0 + (int)(threadIdx.x & 31);
-        mine = Cut{0, 0, 0, 0, 0, 0, 0, 0};
-        if (b < parts.n()) mine = parts(b);
+    __device__ __forceinline__ Cut cut(int first) const {
+        const int b = first + (int)(threadIdx.x & 31);
+        return b < parts.n() ? parts(b) : Cut{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+    __device__ __forceinline__ void know(int first, const Cut& c) {
+        b0 = first, mine = c;
         int y = mine.tiles * parts.G.kv_heads, x = y * mine.pages;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -237,31 +238,32 @@ struct Walk {
         }
         upto_units = units + x, upto_items = items + y;
     }
-    __device__ __forceinline__ void next() {       // what was known becomes what lies before
+    __device__ __forceinline__ void next(const Cut& c) {       // what was known becomes what lies before
         units = __shfl_sync(0xffffffffu, upto_units, 31), items = __shfl_sync(0xffffffffu, upto_items, 31);
-        know(b0 + 32);
+        know(b0 + 32, c);
     }
     // plan: the workers' number and the units and items before each sequence are written down there (null: not).
     __device__ __forceinline__ Walk(const OwnParts& p, int workers, int* plan) : parts(p), deal(0, 1), units(0), items(0) {
         const int lane = threadIdx.x & 31;
-        know(0);
+        know(0, cut(0));
         for (;;) {
+            const Cut ahead = b0 + 32 < parts.n() ? cut(b0 + 32) : mine;       // (read beside what is counted now)
             const int b = b0 + lane;
             if (plan && b < parts.n()) plan[2 + b] = upto_units, plan[3 + parts.n() + b] = upto_items;
             if (b0 + 32 >= parts.n()) break;
-            next();
+            next(ahead);
         }
         deal = Deal(__shfl_sync(0xffffffffu, upto_units, 31), workers);
         if (plan && lane == 0) plan[0] = deal.S, plan[1] = 0, plan[2 + parts.n()] = 0;
         const bool in = deal.U > 0 && (int)blockIdx.x < deal.S;
         u = in ? deal.run_start(blockIdx.x) : 0;
         end = in ? deal.run_start(blockIdx.x + 1) : 0;
-        if (parts.n() > 32) units = items = 0, know(0);
+        if (u < units) units = items = 0, know(0, cut(0));                     // (else it begins among those known last)
     }
     // The next part of the run; false: there is none.
     __device__ __forceinline__ bool segment(Segment& s) {
         if (u >= end) return false;
-        while (u >= __shfl_sync(0xffffffffu, upto_units, 31)) next();
+        while (u >= __shfl_sync(0xffffffffu, upto_units, 31)) next(cut(b0 + 32));
         const int l = __ffs(__ballot_sync(0xffffffffu, u < upto_units)) - 1, columns = parts.G.kv_heads;
         Cut& c = s.cut;
         c.pages = __shfl_sync(0xffffffffu, mine.pages, l), c.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);

@@ -63,11 +63,11 @@ struct Steer {
     const int* mask_of;        // [n_rows], -1: none
 };
 
-// A block takes U groups of four tokens a thread of one row.  VEC: x and y lie alike to 16 bytes, so that a group is one load and
-// one store; a row of odd length begins in the middle of a group, and bits of a group then lie in two words.
-template <int U, bool VEC>
+// A block takes four tokens a thread of one row.  VEC: x and y lie alike to 16 bytes, so that the four are one load and one store; a row of
+// odd length begins in the middle of four, and their bits then lie in two words.
+template <bool VEC>
 __global__ void __launch_bounds__(HT) steer_kernel(const Steer a) {
-    constexpr int CH = HT * U * 4;
+    constexpr int CH = HT * 4;
     __shared__ float bias[CH];
     __shared__ unsigned biased[CH / 32];
     pdl_trigger();
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(HT) steer_kernel(const Steer a) {
     const int i = blockIdx.y, V = a.vocab;
     const float* x = fresh(a.x) + i * a.x_stride;
     float* y = a.y + i * a.y_stride;
-    const int skew = VEC ? (int)(((uintptr_t)x >> 2) & 3) : 0;     // tokens of the first group that lie before the row
+    const int skew = VEC ? (int)(((uintptr_t)x >> 2) & 3) : 0;     // tokens of the first four that lie before the row
     const int e0 = (int)blockIdx.x * CH - skew;                     // the block's first token
     const int r = a.rows ? a.rows[i] : i;
     const bool known = r >= 0 && r < a.n_rows;
@@ -87,17 +87,19 @@ __global__ void __launch_bounds__(HT) steer_kernel(const Steer a) {
     const unsigned* mask = which >= 0 && which < a.n_masks ? a.masks + (int64_t)which * a.words : nullptr;
     int b0 = 0, b1 = 0;
     if (known && a.bias_cu) b0 = a.bias_cu[r], b1 = a.bias_cu[r + 1];
+    bool biases = false;       // of tokens of this block
     if (b0 < b1) {
         for (int k = threadIdx.x; k < CH / 32; k += HT) biased[k] = 0;
         __syncthreads();
         for (int k = b0 + threadIdx.x; k < b1; k += HT) {
             const int at = a.bias_tokens[k] - e0;
             if (at >= 0 && at < CH) {
+                biases = true;
                 bias[at] = a.bias_values[k];
                 atomicOr(&biased[at >> 5], 1u << (at & 31));
             }
         }
-        __syncthreads();
+        biases = __syncthreads_or(biases);
     }
     // bits of four tokens from e on (e >= 0, e < V)
     auto four = [&](const unsigned* w, int e) -> unsigned {
@@ -106,43 +108,36 @@ __global__ void __launch_bounds__(HT) steer_kernel(const Steer a) {
         if (s > 28 && k + 1 < a.words) v |= w[k + 1] << (32 - s);
         return v & 15u;
     };
-    auto one = [&](float l, int e, bool is_seen, bool is_allowed) -> float {
-        if (!is_allowed) return -INFINITY;
-        if (is_seen) {
-            l = l > 0.f ? __fdiv_rn(l, rep) : l * rep;
-            const int n = counts[e];
-            if (n > 0) l -= fmaf(freq, (float)n, pres);
-        }
-        if (b0 < b1 && (biased[(e - e0) >> 5] >> ((e - e0) & 31) & 1)) l += bias[e - e0];
-        return l;
+    // n: the token's count if it was seen, else 0
+    auto one = [&](float l, int e, bool is_seen, bool is_allowed, int n) -> float {
+        if (is_seen) l = l > 0.f ? __fdiv_rn(l, rep) : l * rep;
+        if (n > 0) l -= fmaf(freq, (float)n, pres);
+        if (biases && (biased[(e - e0) >> 5] >> ((e - e0) & 31) & 1)) l += bias[e - e0];
+        return is_allowed ? l : -INFINITY;
     };
-    float4 v[U];
-    unsigned s4[U], a4[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int e = e0 + (u * HT + (int)threadIdx.x) * 4;
-        const bool whole = VEC && e >= 0 && e + 4 <= V;
-        s4[u] = whole && seen ? four(seen, e) : 0u;
-        a4[u] = whole && mask ? four(mask, e) : 15u;
-        if (whole && a4[u]) v[u] = *reinterpret_cast<const float4*>(x + e);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int e = e0 + (u * HT + (int)threadIdx.x) * 4;
-        if (VEC && e >= 0 && e + 4 <= V) {
-            float4 o = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (a4[u] == 15u && s4[u] == 0u && b0 == b1) {
-                o = v[u];
-            } else if (a4[u]) {
-                o.x = one(v[u].x, e, s4[u] & 1, a4[u] & 1);
-                o.y = one(v[u].y, e + 1, s4[u] & 2, a4[u] & 2);
-                o.z = one(v[u].z, e + 2, s4[u] & 4, a4[u] & 4);
-                o.w = one(v[u].w, e + 3, s4[u] & 8, a4[u] & 8);
+    const int e = e0 + (int)threadIdx.x * 4;
+    if (VEC && e >= 0 && e + 4 <= V) {
+        const unsigned s4 = seen ? four(seen, e) : 0u, a4 = mask ? four(mask, e) : 15u;
+        float4 o = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (a4) {
+            const float4 v = *reinterpret_cast<const float4*>(x + e);
+            // (the four counts are asked for together: behind one another they took longer than all the rest)
+            const unsigned want = s4 & a4;
+            const int n0 = want & 1 ? counts[e] : 0, n1 = want & 2 ? counts[e + 1] : 0, n2 = want & 4 ? counts[e + 2] : 0,
+                      n3 = want & 8 ? counts[e + 3] : 0;
+            o = v;
+            if (a4 != 15u || s4 != 0u || biases) {
+                o.x = one(v.x, e, s4 & 1, a4 & 1, n0);
+                o.y = one(v.y, e + 1, s4 & 2, a4 & 2, n1);
+                o.z = one(v.z, e + 2, s4 & 4, a4 & 4, n2);
+                o.w = one(v.w, e + 3, s4 & 8, a4 & 8, n3);
             }
-            *reinterpret_cast<float4*>(y + e) = o;
-        } else {
-            for (int k = max(e, 0); k < min(e + 4, V); ++k)
-                y[k] = one(x[k], k, seen && (seen[k >> 5] >> (k & 31) & 1), !mask || (mask[k >> 5] >> (k & 31) & 1));
+        }
+        *reinterpret_cast<float4*>(y + e) = o;
+    } else {
+        for (int k = max(e, 0); k < min(e + 4, V); ++k) {
+            const bool is_seen = seen && (seen[k >> 5] >> (k & 31) & 1);
+            y[k] = one(x[k], k, is_seen, !mask || (mask[k >> 5] >> (k & 31) & 1), is_seen ? counts[k] : 0);
         }
     }
 }
@@ -180,8 +175,8 @@ WICK_API int wick_steer_logits(const float* x, int64_t x_stride, float* y, int64
                bias_cu, bias_tokens, bias_values, (const unsigned*)masks, mask_of};
     const bool alike = (((uintptr_t)x ^ (uintptr_t)y) & 15) == 0 && (x_stride - y_stride) % 4 == 0;
     if (alike)
-        WICK_CUDA(launch(steer_kernel<1, true>, dim3(ceil_div(vocab + 3, HT * 4), n), dim3(HT), 0, (cudaStream_t)s, a));
+        WICK_CUDA(launch(steer_kernel<true>, dim3(ceil_div(vocab + 3, HT * 4), n), dim3(HT), 0, (cudaStream_t)s, a));
     else
-        WICK_CUDA(launch(steer_kernel<1, false>, dim3(ceil_div(vocab, HT * 4), n), dim3(HT), 0, (cudaStream_t)s, a));
+        WICK_CUDA(launch(steer_kernel<false>, dim3(ceil_div(vocab, HT * 4), n), dim3(HT), 0, (cudaStream_t)s, a));
     return check_launch("steer_logits");
 }

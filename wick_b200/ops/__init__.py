@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 import os
 from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
@@ -135,7 +136,7 @@ _STATUS_TEXT = {1: "gemm_tc gave up waiting for a free shared-memory stage", 2: 
 
 def status_tensor(device) -> torch.Tensor:
     global _status
-    if _status is None or _status.device != torch.device(device):
+    if _status is None or (_status.device != device and _status.device != torch.device(device)):
         _status = torch.zeros(1, dtype=torch.int32, device=device)
     return _status
 
@@ -185,6 +186,8 @@ def _need(cond: bool, msg: str) -> None:
 
 
 def _cuda(name: str, t: torch.Tensor, dtype=None, shape=None) -> None:
+    if t.is_cuda and t.is_contiguous() and (dtype is None or t.dtype is dtype) and (shape is None or t.shape == shape):
+        return
     if not t.is_cuda:
         raise KernelError(f"{name} must be a CUDA tensor (the kernels have no CPU form)")
     if not t.is_contiguous():
@@ -580,14 +583,19 @@ class SharedPrefix(NamedTuple):
         return cls(dev[:G + 1], dev[G + 1:2 * G + 1], dev[2 * G + 1:], max(pages, default=0), max(own, default=0))
 
 
-def attention_shared_scratch(shared: SharedPrefix, batch, n_heads: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> int:
-    """float32 words of scratch that :func:`attention_shared` needs for this step."""
+@functools.lru_cache(maxsize=4096)
+def _shared_scratch(head_dim: int, *sizes: int) -> int:
     lib = _shared(head_dim)
-    n = lib._lib.wick_attn_shared_scratch(dtype == torch.bfloat16, batch.n_tokens, batch.n_seqs, shared.pages.numel(), n_heads, n_kv,
-                                          shared.max_pages, shared.own_bound, batch.max_q_len)
+    n = lib._lib.wick_attn_shared_scratch(*sizes)
     if n < 0:
         raise KernelError(lib._lib.wick_last_error().decode("utf-8", "replace"))
     return n
+
+
+def attention_shared_scratch(shared: SharedPrefix, batch, n_heads: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> int:
+    """float32 words of scratch that :func:`attention_shared` needs for this step."""
+    return _shared_scratch(head_dim, dtype is torch.bfloat16, batch.n_tokens, batch.n_seqs, shared.pages.numel(), n_heads, n_kv, shared.max_pages,
+                           shared.own_bound, batch.max_q_len)
 
 
 def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPrefix, scale: float, scratch: Optional[torch.Tensor] = None,
@@ -599,26 +607,28 @@ def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPre
     n, n_heads, hd = q.shape
     _cuda("q", q)
     _cuda("kv", kv, q.dtype)
-    _need(kv.dim() == 5 and kv.shape[1] == 2 and kv.shape[3] == PAGE and kv.shape[4] == hd,
-          f"kv must be [pages, 2, kv_heads, {PAGE}, {hd}], is {tuple(kv.shape)}")
+    if kv.dim() != 5 or kv.shape[1:] != (2, kv.shape[2], PAGE, hd):
+        raise KernelError(f"kv must be [pages, 2, kv_heads, {PAGE}, {hd}], is {tuple(kv.shape)}")
+    kv_pages, n_kv = kv.shape[0], kv.shape[2]
     cu_groups, pages, group_of, max_pages, own_bound = shared
-    G, n_seqs = pages.numel(), batch.n_seqs
-    _need(n == batch.n_tokens, f"q has {n} rows, the batch {batch.n_tokens} tokens")
-    _cuda("cu_groups", cu_groups, torch.int32, (G + 1,))
-    _cuda("pages", pages, torch.int32)
-    _cuda("group_of", group_of, torch.int32, (n_seqs,))
+    G, n_seqs, i32 = pages.numel(), batch.n_seqs, torch.int32
+    if n != batch.n_tokens:
+        raise KernelError(f"q has {n} rows, the batch {batch.n_tokens} tokens")
+    _cuda("cu_groups", cu_groups, i32, (G + 1,))
+    _cuda("pages", pages, i32)
+    _cuda("group_of", group_of, i32, (n_seqs,))
     if scratch is None:
-        scratch = torch.empty(attention_shared_scratch(shared, batch, n_heads, kv.shape[2], hd, q.dtype), dtype=torch.float32, device=q.device)
+        scratch = torch.empty(attention_shared_scratch(shared, batch, n_heads, n_kv, hd, q.dtype), dtype=torch.float32, device=q.device)
     else:
         _cuda("scratch", scratch, torch.float32)
     if out is None:
         out = torch.empty_like(q)
     else:
         _cuda("out", out, q.dtype, q.shape)
-    _shared(hd).call(f"wick_attn_shared_{_dt(q)}", "piplppppipippiiiiiifplpp", _p(q), n, _p(kv), kv.shape[0], _p(out), _p(cu_groups), _p(pages),
-                     _p(group_of), G, _p(batch.cu_seqlens), n_seqs, _p(batch.start), _p(batch.page_table), batch.table_width, n_heads,
-                     kv.shape[2], max_pages, own_bound, batch.max_q_len, float(scale), _p(scratch), scratch.numel(),
-                     _p(status_tensor(q.device)), _stream(), kernels=2)
+    _shared(hd).call(f"wick_attn_shared_{_dt(q)}", "piplppppipippiiiiiifplpp", q.data_ptr(), n, kv.data_ptr(), kv_pages, out.data_ptr(),
+                     cu_groups.data_ptr(), pages.data_ptr(), group_of.data_ptr(), G, batch.cu_seqlens.data_ptr(), n_seqs, batch.start.data_ptr(),
+                     batch.page_table.data_ptr(), batch.table_width, n_heads, n_kv, max_pages, own_bound, batch.max_q_len, scale, scratch.data_ptr(),
+                     scratch.numel(), status_tensor(q.device).data_ptr(), _stream(), kernels=2)
     return out
 
 
@@ -2030,19 +2040,23 @@ def step_tables(start: torch.Tensor, q_len: torch.Tensor, slots: torch.Tensor, t
     _cuda("free_pages", free_pages, i32)
     _cuda("free_head", free_head, i32, (1,))
     _cuda("page_table", page_table, i32)
-    _need(tables.dim() == 2 and page_table.dim() == 2 and page_table.shape[0] == n, f"tables must be [slots, width], page_table [{n}, width]")
+    if tables.dim() != 2 or page_table.dim() != 2 or page_table.shape[0] != n:
+        raise KernelError(f"tables must be [slots, width], page_table [{n}, width]")
     _cuda("cu_seqlens", cu_seqlens, i32, (n + 1,))
     _cuda("positions", positions, i32)
     _cuda("seq_of_token", seq_of_token, i32, (n_tokens,))
     _cuda("slot_map", slot_map, torch.int64, (n_tokens,))
     _cuda("head_out", head_out, i32, (1,))
-    _need(head_out.data_ptr() != free_head.data_ptr(), "head_out must be another tensor than free_head")
+    head, taken = free_head.data_ptr(), head_out.data_ptr()
+    if head == taken:
+        raise KernelError("head_out must be another tensor than free_head")
     if parent is not None:
         _cuda("parent", parent, i32, (n,))
-    _core().call("wick_step_tables", "ppppipiipippipppppippp", _p(start), _p(q_len), _p(slots), _p(parent), n,
-                 _p(tables), tables.shape[0], tables.shape[1], _p(free_pages), free_pages.numel(), _p(free_head), _p(page_table),
-                 page_table.shape[1], _p(cu_seqlens), _p(kv_len), _p(positions), _p(seq_of_token), _p(slot_map), n_tokens, _p(head_out),
-                 _p(status_tensor(slots.device)), _stream())
+    n_slots, table_width = tables.shape
+    _core().call("wick_step_tables", "ppppipiipippipppppippp", start.data_ptr(), q_len.data_ptr(), slots.data_ptr(), _p(parent), n, tables.data_ptr(),
+                 n_slots, table_width, free_pages.data_ptr(), free_pages.numel(), head, page_table.data_ptr(), page_table.shape[1],
+                 cu_seqlens.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), slot_map.data_ptr(), n_tokens, taken,
+                 status_tensor(slots.device).data_ptr(), _stream())
 
 
 # ---------------------------------------------------------------------------
@@ -2095,13 +2109,15 @@ def steer_logits(logits: torch.Tensor, rows: Optional[torch.Tensor] = None, *, s
 
     out: where to write (default: in place)."""
     n, vocab = logits.shape
-    _need(logits.is_cuda and logits.dtype == torch.float32 and (vocab == 1 or logits.stride(1) == 1) and (n <= 1 or logits.stride(0) >= vocab),
-          "logits must be float32 rows on the CUDA device")
+    far, step = logits.stride()
+    if not (logits.is_cuda and logits.dtype is torch.float32 and (vocab == 1 or step == 1) and (n <= 1 or far >= vocab)):
+        raise KernelError("logits must be float32 rows on the CUDA device")
     if out is None:
-        out = logits
+        out, out_far = logits, far
     else:
-        _need(out.is_cuda and out.dtype == torch.float32 and out.shape == logits.shape and (vocab == 1 or out.stride(1) == 1) and
-              (n <= 1 or out.stride(0) >= vocab), f"out must be float32 rows [{n}, {vocab}] on the CUDA device")
+        out_far, step = out.stride() if out.dim() == 2 else (0, 0)
+        if not (out.is_cuda and out.dtype is torch.float32 and out.shape == logits.shape and (vocab == 1 or step == 1) and (n <= 1 or out_far >= vocab)):
+            raise KernelError(f"out must be float32 rows [{n}, {vocab}] on the CUDA device")
     n_rows = n_masks = 0
     if seen is not None:
         _need(counts is not None and penalties is not None, "seen, counts and penalties come together")
@@ -2128,7 +2144,7 @@ def steer_logits(logits: torch.Tensor, rows: Optional[torch.Tensor] = None, *, s
         _need(mask_of is None, "masks and mask_of come together")
     if rows is not None:
         _cuda("rows", rows, torch.int32, (n,))
-    _core().call("wick_steer_logits", "plpliipippppppppip", _p(logits), logits.stride(0), _p(out), out.stride(0), n, vocab, _p(rows), n_rows,
+    _core().call("wick_steer_logits", "plpliipippppppppip", logits.data_ptr(), far, out.data_ptr(), out_far, n, vocab, _p(rows), n_rows,
                  _p(seen), _p(counts), _p(penalties), _p(cu), _p(tokens), _p(values), _p(masks), _p(mask_of), n_masks, _stream())
     return out
 
