@@ -434,10 +434,12 @@ __device__ __forceinline__ Source own_source(const OwnParts& parts, const Record
 }
 
 // Blocks (four rows, sequence): a thread has a row and four columns (and those 128, 256 .. behind), four neighbouring threads four
-// neighbouring rows, whose sums lie side by side in a record.  Eight records at a time: each of the eight threads of a row in a warp
-// finds one's weight, and all read the sums of all of them at once (behind the last one: of that one again, without weight).
+// neighbouring rows, whose sums lie side by side in a record.  JN records at a time (16 where all blocks run at once, and 8, for more of them on
+// an SM, where they do not), the shared keys' and the own ones' in one
+// list, so that all reads of a row that has no more stand side by side: each of the eight threads of a row in a warp finds a weight or two,
+// and all read the sums of all JN at once (behind the last one: of that one again, without weight).
 constexpr int JT = 128, JR = 4;
-template <typename T>
+template <typename T, int JN>
 __global__ void __launch_bounds__(JT)
 attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records shared, const Records own, int groups) {
     const int b = blockIdx.y, row = (int)blockIdx.x * JR + (int)threadIdx.x % JR, group = G.heads / G.kv_heads;
@@ -449,45 +451,57 @@ attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records share
     if (there) c = groups ? parts(G.n_seqs + g) : SharedParts{G}(g);
     pdl_wait();
     pdl_trigger();
-    Source src = {nullptr, 0, 0, 0, 0};
-    const int k = (threadIdx.x & 31) / JR;          // of the eight threads of a row
+    Source s0 = {shared.at, 0, 0, 0, 0}, s1 = s0;
+    if (there) {
+        s0 = groups ? own_source(parts, own, G.n_seqs + g, c, (mine.tok0 + tok - c.tok0) * group + h, kvh) : shared_source(G, shared, g, c, mine.tok0 + tok, h, kvh);
+        s1 = own_source(parts, own, b, mine, tok * group + h, kvh);
+    }
+    const int k = (threadIdx.x & 31) / JR, n = s0.n + s1.n;        // k: of the eight threads of a row
+    // number `at` of a record of s0's, `at1` of one of s1's, of record i of both
+    auto place = [&](int i, int at, int at1) {
+        const bool first = i < s0.n;
+        return (first ? s0.at + at : s1.at + at1) + (int64_t)(first ? i : i - s0.n) * (first ? s0.step : s1.step);
+    };
+    const int ml0 = s0.rows * HD + 2 * s0.r, ml1 = s1.rows * HD + 2 * s1.r;
     for (int col = threadIdx.x / JR; col < (HD / 4 + 7) / 8 * 8; col += JT / JR) {     // (whole warps)
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         float m = -INFINITY, l = 0.f;
+        const int at0 = (min(col, HD / 4 - 1) * s0.rows + s0.r) * 4, at1 = (min(col, HD / 4 - 1) * s1.rows + s1.r) * 4;
 #pragma unroll 1
-        for (int kind = 0; kind < 2; ++kind) {
-            if (there) {
-                if (kind == 0 && !groups) src = shared_source(G, shared, g, c, mine.tok0 + tok, h, kvh);
-                else if (kind == 0) src = own_source(parts, own, G.n_seqs + g, c, (mine.tok0 + tok - c.tok0) * group + h, kvh);
-                else src = own_source(parts, own, b, mine, tok * group + h, kvh);
+        for (int i0 = 0; __any_sync(0xffffffffu, i0 < n); i0 += JN) {
+            const int left = n - i0;                // (a row without further records: reads the last one again, or none)
+            float2 x[JN / 8];
+            float4 o[JN];
+#pragma unroll
+            for (int i = 0; i < JN / 8; ++i) {
+                x[i] = make_float2(-INFINITY, 0.f);
+                if (k + 8 * i < left) x[i] = *reinterpret_cast<const float2*>(place(i0 + k + 8 * i, ml0, ml1));
             }
-            const float *sums = src.at + (min(col, HD / 4 - 1) * src.rows + src.r) * 4, *ml = src.at + src.rows * HD + 2 * src.r;
-#pragma unroll 1
-            for (int i0 = 0; __any_sync(0xffffffffu, i0 < src.n); i0 += 8) {
-                const int left = src.n - i0;        // (a row without further records: reads the last one again, or none)
-                float2 x = make_float2(-INFINITY, 0.f);
-                float4 o[8];
-                if (k < left) x = *reinterpret_cast<const float2*>(ml + (int64_t)(i0 + k) * src.step);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (left > 0) o[i] = *reinterpret_cast<const float4*>(sums + (int64_t)(i0 + min(i, left - 1)) * src.step);
-                float most = fmaxf(m, x.x);
+            for (int i = 0; i < JN; ++i)
+                if (left > 0) o[i] = *reinterpret_cast<const float4*>(place(i0 + min(i, left - 1), at0, at1));
+            float most = m;
 #pragma unroll
-                for (int d = JR; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                const float before = weight(m, most);
-                m = most;
-                l *= before, s.x *= before, s.y *= before, s.z *= before, s.w *= before;
-                const float w = weight(x.x, m);
-                float add = k < left ? x.y * w : 0.f;
+            for (int i = 0; i < JN / 8; ++i) most = fmaxf(most, x[i].x);
 #pragma unroll
-                for (int d = JR; d < 32; d <<= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
-                l += add;
+            for (int d = JR; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            const float before = weight(m, most);
+            m = most;
+            l *= before, s.x *= before, s.y *= before, s.z *= before, s.w *= before;
+            float w[JN / 8], add = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float a = __shfl_sync(0xffffffffu, w, i * JR + (threadIdx.x % JR));
-                    if (i >= left) continue;
-                    s.x = fmaf(o[i].x, a, s.x), s.y = fmaf(o[i].y, a, s.y), s.z = fmaf(o[i].z, a, s.z), s.w = fmaf(o[i].w, a, s.w);
-                }
+            for (int i = 0; i < JN / 8; ++i) {
+                w[i] = weight(x[i].x, m);
+                if (k + 8 * i < left) add += x[i].y * w[i];
+            }
+#pragma unroll
+            for (int d = JR; d < 32; d <<= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+            l += add;
+#pragma unroll
+            for (int i = 0; i < JN; ++i) {
+                const float a = __shfl_sync(0xffffffffu, w[i / 8], i % 8 * JR + (threadIdx.x % JR));
+                if (i >= left) continue;
+                s.x = fmaf(o[i].x, a, s.x), s.y = fmaf(o[i].y, a, s.y), s.z = fmaf(o[i].z, a, s.z), s.w = fmaf(o[i].w, a, s.w);
             }
         }
         const float f = l != 0.f ? __fdiv_rn(1.0f, l) : 0.f;       // (a sum that is no number shows)
@@ -529,10 +543,10 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
     int gs = group;
     for (int n = 2; gs > TC_ROWS; ++n)
         if (group % n == 0) gs = group / n;
-    G.rows = TC_ROWS / gs * gs, G.gs = gs, G.per_kv = group / gs, G.columns = heads / gs, G.block = 2, G.pair = 2;
+    G.rows = TC_ROWS / gs * gs, G.gs = gs, G.per_kv = group / gs, G.columns = heads / gs, G.block = 1, G.pair = 2;
     const int sms = sm_count(), rows_own = c.fast ? OWN_ROWS : R, own_per_sm = c.fast ? OWN_WARPS * (128 / HD) : PER_SM;
     const int64_t tiles = (int64_t)ceil_div((int64_t)n_tokens * gs, G.rows) + n_groups, items = (tiles / 2 + n_groups) * G.columns;
-    const int64_t units = tiles * G.columns * ceil_div(max_pages, 2);
+    const int64_t units = tiles * G.columns * max_pages;
     const int64_t items_seqs = ((int64_t)ceil_div((int64_t)n_tokens * group, rows_own) + n_seqs) * kv_heads, pages_own = ceil_div(own_bound, kPage);
     const int64_t items_groups = max_pages > 0 ? ((int64_t)ceil_div((int64_t)n_tokens * group, rows_own) + n_groups) * kv_heads : 0;
     WICK_REQUIRE(units <= INT32_MAX / 2 && items_seqs * pages_own + items_groups * max_pages <= INT32_MAX / 2, "attention (shared prefix): too much for one step");
@@ -598,7 +612,9 @@ static int attn_shared(const T* q, int n_tokens, const T* kv, int64_t kv_pages, 
         if (int e = check_launch("attn_shared_part")) return e;
     }
     const Records sh = {c.tc ? plan : nullptr, records, TC_ROWS}, ow = {plan_own, own, c.fast ? OWN_ROWS : R};
-    WICK_CUDA(launch(attn_shared_join_kernel<T>, dim3(ceil_div((int64_t)max_q_len * heads, JR), n_seqs), dim3(JT), 0, s, out, G, sh, ow, groups));
+    const dim3 grid(ceil_div((int64_t)max_q_len * heads, JR), n_seqs);
+    if ((int64_t)grid.x * grid.y <= 4 * sm_count()) WICK_CUDA(launch(attn_shared_join_kernel<T, 16>, grid, dim3(JT), 0, s, out, G, sh, ow, groups));
+    else WICK_CUDA(launch(attn_shared_join_kernel<T, 8>, grid, dim3(JT), 0, s, out, G, sh, ow, groups));
     return check_launch("attn_shared_join");
 }
 

@@ -63,7 +63,8 @@ struct OwnParts {
     __device__ __forceinline__ int n() const { return G.n_seqs + groups; }
     __device__ __forceinline__ bool shared(int i) const { return i >= G.n_seqs; }
     __device__ __forceinline__ bool fits(int b, const Cut& c) const {
-        return G.group_of[b] >= 0 && G.group_of[b] < G.n && G.start[b] >= c.first * kPage && (c.end + kPage - 1) / kPage <= G.table_width;
+        const int g = G.group_of[b];
+        return g >= 0 && g < G.n && b >= G.cu_groups[g] && b < G.cu_groups[g + 1] && G.start[b] >= c.first * kPage && (c.end + kPage - 1) / kPage <= G.table_width;
     }
     __device__ __forceinline__ Cut operator()(int i) const {
         Cut c;

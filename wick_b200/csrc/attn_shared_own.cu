@@ -85,9 +85,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    // (With a shared part the kernel before this one is the one that computes it, and has waited for q and the cache.)
-    if (!after_shared) pdl_wait();
-    pdl_trigger();
+    // (The description lies ready before the step's kernels start.)
     const OwnParts parts{G, R, groups};
     Walk walk(parts, gridDim.x, nullptr);
     Ahead next = {};
@@ -121,6 +119,9 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
     if (!ok && lane == 0) atomicCAS(status, 0, 7);
     next.any = false;
     if (ok) begin();
+    // (With a shared part the kernel before this one is the one that computes it, and has waited for q and the cache.)
+    if (!after_shared) pdl_wait();
+    pdl_trigger();
     if (next.any) copy(0), copy(1);
 
     uint32_t qb[KS][2];                                // lane: row g

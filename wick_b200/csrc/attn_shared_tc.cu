@@ -31,24 +31,24 @@ namespace tc {
 
 constexpr bool SUPPORTED = WICK_HD == 64 || WICK_HD == 128;
 constexpr int HD = SUPPORTED ? WICK_HD : 64;           // other head sizes: never launched
-constexpr int BQ = TC_ROWS, BK = 128;
+constexpr int BQ = TC_ROWS, BK = kPage;
 constexpr int PANELS = HD / 64;                        // 64-column panels of a head row
-constexpr int PANEL_BYTES = 128 * 128;                 // 128 rows of 128 bytes
-constexpr int TILE_BYTES = PANELS * PANEL_BYTES;       // a tile of queries, or one block of keys or of values
-constexpr int NSLOT = 5;                               // key / value tiles in flight
+constexpr int Q_PANEL = BQ * 128, KV_PANEL = BK * 128; // bytes: rows of 128
+constexpr int Q_BYTES = PANELS * Q_PANEL, KV_BYTES = PANELS * KV_PANEL;        // a tile of queries, of keys or of values
+constexpr int NSLOT = 5;                               // pairs of a value and a key tile in flight
+constexpr int AHEAD = 4;                               // turns that the scores are ahead of the products (two a stream)
 constexpr int THREADS = 320;                           // warp 0: TMA, warp 1: MMA + tensor memory, warps 2-5 and 6-9: softmax
 constexpr uint32_t TMEM_COLS = 512;                    // S of both streams | O of both
-constexpr uint32_t COL_S = 0, COL_O = 2 * BK;
-constexpr int P_FIRST = 64;                            // keys of a block whose weights the product begins with
+constexpr uint32_t COL_S = 0, COL_O = 4 * BK;          // S: two of either stream
 constexpr int REC = BQ * (HD + 2);
 
 struct Smem {
     float ml[2][2][BQ];                                // the streams' maxima and sums
-    uint64_t q_full, q_empty, full[NSLOT], empty[NSLOT], s_full[2], p_full[2][2], o_full[2], o_empty[2], join, joined;
+    uint64_t q_full, q_empty, full[NSLOT], empty[NSLOT], s_full[2][2], p_full[2][2], before_last[2], o_full[2], o_empty[2], join, joined;
     uint32_t tmem_slot;
     int abort_flag;
 };
-constexpr int SMEM_BYTES = (2 + NSLOT) * TILE_BYTES + (int)sizeof(Smem);
+constexpr int SMEM_BYTES = 2 * Q_BYTES + NSLOT * 2 * KV_BYTES + (int)sizeof(Smem);
 static_assert(SMEM_BYTES <= 227 * 1024, "a block's shared memory");
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -56,8 +56,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                       int* plan, float* records, int* status) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* q_s = smem_raw;
-    uint8_t* kv_s = q_s + 2 * TILE_BYTES;
-    Smem& sh = *reinterpret_cast<Smem*>(kv_s + NSLOT * TILE_BYTES);
+    uint8_t* kv_s = q_s + 2 * Q_BYTES;
+    Smem& sh = *reinterpret_cast<Smem*>(kv_s + NSLOT * 2 * KV_BYTES);
     volatile int* abort_flag = &sh.abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -67,8 +67,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         for (int i = 0; i < NSLOT; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
         // (every waiter below sees every phase of the barrier it waits on, so that a parity is never ambiguous)
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.s_full[i], 1), mbar_init(&sh.o_full[i], 1), mbar_init(&sh.o_empty[i], 4);
-            mbar_init(&sh.p_full[i][0], 4), mbar_init(&sh.p_full[i][1], 4);
+            mbar_init(&sh.o_full[i], 1), mbar_init(&sh.o_empty[i], 4), mbar_init(&sh.before_last[i], 1);
+            for (int b = 0; b < 2; ++b) mbar_init(&sh.s_full[i][b], 1), mbar_init(&sh.p_full[i][b], 4);
         }
         mbar_init(&sh.join, 8), mbar_init(&sh.joined, 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -83,6 +83,19 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     }
     // (The description lies ready before the step's kernels start; the plan is written behind the wait.)
     Runs runs(G, gridDim.x);                           // (every warp knows them on its own)
+    Segment seg;
+    // The producer's lanes hold a page number of each of two runs of 32, read ahead.
+    auto pages = [&](int run) {
+        const int j = seg.from + run * 32 + lane;
+        int page = j < seg.to ? G.page_table[(int64_t)seg.cut.seq * G.table_width + j] : 0;
+        if (page < 0 || page >= kv_pages) {
+            atomicCAS(status, 0, 10);
+            page = 0;
+        }
+        return page;
+    };
+    int even = 0, odd = 0;
+    if (warp == 0 && blockIdx.x < runs.all) seg = runs.segment(blockIdx.x), even = pages(0), odd = pages(1);
     pdl_wait();
     pdl_trigger();                                     // (behind the wait: the next kernel reads what this one reads without a wait of its own)
     if (blockIdx.x == 0 && warp == 2) Runs(G, gridDim.x).write(plan);
@@ -92,9 +105,6 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     const uint32_t tmem = sh.tmem_slot;
     const bool aligned = (smem_u32(smem_raw) & 1023) == 0;   // (always: the block's dynamic shared memory is all there is)
     if (!aligned && threadIdx.x == 0) atomicCAS(status, 0, 7);
-    // the block of keys that is one page: the last one of an odd number
-    auto half = [&](const Segment& s, int j) { return 2 * (s.from + j) + 1 == s.cut.pages; };
-    Segment seg;
     int k = 0;                                         // runs so far
     bool ok = aligned;
 
@@ -104,55 +114,39 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         int slot = 0, turn = 0;                        // of the ring
 #pragma unroll 1
         for (int at = blockIdx.x; ok && at < runs.all; at += gridDim.x, ++k) {
-            seg = runs.segment(at);
+            if (k > 0) seg = runs.segment(at), even = pages(0), odd = pages(1);
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
-            const int* table = G.page_table + (int64_t)seg.cut.seq * G.table_width;
-            // A lane holds a page number of each of two runs of 32, read ahead.
-            auto pages = [&](int run) {
-                const int j = 2 * seg.from + run * 32 + lane;
-                int page = j < seg.cut.pages ? table[j] : 0;
-                if (page < 0 || page >= kv_pages) {
-                    atomicCAS(status, 0, 10);
-                    page = 0;
-                }
-                return page;
-            };
-            int even = pages(0), odd = pages(1);
             if (k > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty, (k - 1) & 1, abort_flag, status, 7));
             if (!ok) break;
             if (one) {
                 mbar_expect_tx(&sh.q_full, seg.tiles * PANELS * G.rows * 128);
                 for (int i = 0; i < seg.tiles; ++i)
                     for (int pn = 0; pn < PANELS; ++pn)
-                        tma_load_3d(&q_map, &sh.q_full, q_s + i * TILE_BYTES + pn * PANEL_BYTES, pn * 64, seg.column * G.gs,
+                        tma_load_3d(&q_map, &sh.q_full, q_s + i * Q_BYTES + pn * Q_PANEL, pn * 64, seg.column * G.gs,
                                     seg.cut.tok0 + (seg.tile + i) * (G.rows / G.gs));
             }
-            // K0 V0 K1 V1 .., or, split, K0 K1 V0 K2 V1 K3 .. V(n-2) V(n-1): the order in which the issuing warp uses them
+            // A slot: the values of block i beside the keys of the block that the issuing warp scores in the same turn.
+            const int ahead = split ? AHEAD : AHEAD / 2;
 #pragma unroll 1
-            for (int i = 0; i < 2 * n; ++i) {
-                const bool last = split && i == 2 * n - 1;
-                const int is_v = split ? (last || (i > 0 && !(i & 1))) : (i & 1);
-                const int j = last ? n - 1 : (split ? (is_v ? (i - 2) >> 1 : (i + 1) >> 1) : i >> 1);
-                if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.empty[slot], (turn - 1) & 1, abort_flag, status, 7))) {
-                    ok = false;
-                    break;
-                }
-                const int held = (2 * j >> 5) & 1 ? odd : even;
-                const int page0 = __shfl_sync(0xffffffffu, held, 2 * j & 31), page1 = __shfl_sync(0xffffffffu, held, (2 * j + 1) & 31);
-                if (is_v && j >= 16 && (j & 15) == 0) {            // (keys and values have left the run before)
-                    if ((j >> 4) & 1) even = pages((j >> 4) + 1);
-                    else odd = pages((j >> 4) + 1);
+            for (int i = -ahead; i < n; ++i) {
+                if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[slot], (turn - 1) & 1, abort_flag, status, 7));
+                if (!ok) break;
+                const int j = i + ahead, v = max(i, 0);
+                const int k_page = __shfl_sync(0xffffffffu, j >> 5 & 1 ? odd : even, j & 31), v_page = __shfl_sync(0xffffffffu, v >> 5 & 1 ? odd : even, v & 31);
+                if (i >= 32 && (i & 31) == 0) {        // (keys and values have left the run before)
+                    if (i >> 5 & 1) even = pages((i >> 5) + 1);
+                    else odd = pages((i >> 5) + 1);
                 }
                 if (one) {
-                    const int n_pages = half(seg, j) ? 1 : 2;
-                    mbar_expect_tx(&sh.full[slot], n_pages * (TILE_BYTES / 2));
-                    uint8_t* dst = kv_s + slot * TILE_BYTES;
+                    mbar_expect_tx(&sh.full[slot], ((i >= 0) + (j < n)) * KV_BYTES);
 #pragma unroll 1
-                    for (int h = 0; h < n_pages; ++h)
+                    for (int is_v = 0; is_v < 2; ++is_v) {
+                        if (is_v ? i < 0 : j >= n) continue;
+                        const int y = (((is_v ? v_page : k_page) * 2 + is_v) * G.kv_heads + seg.column / G.per_kv) * kPage;
                         for (int pn = 0; pn < PANELS; ++pn)
-                            tma_load_2d(&kv_map, &sh.full[slot], dst + pn * PANEL_BYTES + h * (kPage * 128), pn * 64,
-                                        (((h ? page1 : page0) * 2 + is_v) * G.kv_heads + seg.column / G.per_kv) * kPage);
+                            tma_load_2d(&kv_map, &sh.full[slot], kv_s + (2 * slot + is_v) * KV_BYTES + pn * KV_PANEL, pn * 64, y);
+                    }
                 }
                 if (++slot == NSLOT) slot = 0, ++turn;
                 __syncwarp();
@@ -160,78 +154,66 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
-        // (the whole warp walks through the steps, one elected lane issues)
+        // (One lane by itself, without a vote or a shuffle: what it does between its instructions bounds the kernel.)
         const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BK >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
         const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-        const uint32_t q_lo0 = desc_lo(smem_u32(q_s), 16), k_lo0 = desc_lo(smem_u32(kv_s), 16), v_lo0 = desc_lo(smem_u32(kv_s), PANEL_BYTES);
+        const uint32_t q_lo0 = desc_lo(smem_u32(q_s), 16), k_lo0 = desc_lo(smem_u32(kv_s), 16), v_lo0 = desc_lo(smem_u32(kv_s) + KV_BYTES, KV_PANEL);
         const bool one = elect_one();
         int slot = 0, round = 0;                       // of the ring
-        int steps0 = 0, steps1 = 0, uses0 = 0, uses1 = 0;          // blocks and runs of each stream so far
-        int k_at = 0, v_at = 0;                        // where the keys and values at hand lie
-        auto take = [&](int& at) {                     // the next tile of the ring, when it has come
-            at = slot;
-            const bool here = __all_sync(0xffffffffu, mbar_wait(&sh.full[slot], round & 1, abort_flag, status, 7));
-            if (++slot == NSLOT) slot = 0, ++round;
-            return here;
-        };
+        int scores[2] = {0, 0}, steps[2] = {0, 0}, uses[2] = {0, 0};           // scores, products and runs of each stream so far
 #pragma unroll 1
         for (int at = blockIdx.x; ok && at < runs.all; at += gridDim.x, ++k) {
             seg = runs.segment(at);
             const int n = seg.to - seg.from;
             const bool split = seg.tiles == 1;
             const int N = split ? n : 2 * n;           // turns
-            // turn i: stream i & 1's product of one block, then its scores of the next.
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full, k & 1, abort_flag, status, 7));
-#pragma unroll 1
-            for (int i = -2; ok && i < N; ++i) {
-                const int s = i & 1;
-                const bool more = i + 2 < N;
+            // turn i: stream i & 1's product of one block, then its scores of the block after the next.
+            auto turn = [&](int i, auto stream) {
+                constexpr int s = (int)stream;
+                if (split || s == 0) {
+                    if (!mbar_wait(&sh.full[slot], round & 1, abort_flag, status, 7)) return false;
+                }
                 if (i >= 0) {
-                    const int steps = s == 0 ? steps0 : steps1, uses = s == 0 ? uses0 : uses1;
-                    if (split || s == 0) ok = take(v_at);
+                    const int at_s = steps[s] & 1;
                     // (the sums of the stream's run before have been read)
-                    if (ok && i < 2 && uses > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_empty[s], (uses - 1) & 1, abort_flag, status, 7));
-                    uint32_t vp = v_lo0 + v_at * (TILE_BYTES >> 4), pp = tmem + COL_S + s * BK;
-                    const uint32_t d = tmem + COL_O + s * HD;
-                    const int parts = half(seg, split ? i : i >> 1) ? 1 : 2;
-#pragma unroll 1
-                    for (int part = 0; part < 2; ++part) {
-                        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[s][part], steps & 1, abort_flag, status, 7));
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (one && part < parts) {
-                            int begun = i >= 2 || part > 0;
-                            mma_ts(d, pp, vp, idesc_o, begun);
-                            static_for<1, P_FIRST / 16>([&](auto ks) { mma_ts(d, pp + (int)ks * 8, vp + (int)ks * (2048 >> 4), idesc_o, 1); });
-                            pp += 8 * (P_FIRST / 16), vp += (P_FIRST / 16) * (2048 >> 4);
-                        }
-                    }
-                    if (!ok) break;
-                    if (one) {
-                        if (split || s == 1) tc_commit(&sh.empty[v_at]);       // a tile is free behind its last reader
-                        if (!more) tc_commit(&sh.o_full[s]);
-                    }
-                    if (s == 0) ++steps0, uses0 += more ? 0 : 1;
-                    else ++steps1, uses1 += more ? 0 : 1;
-                }
-                if (more) {
-                    if (split || s == 0) ok = take(k_at);
-                    if (!ok) break;
+                    if (i < 2 && uses[s] > 0 && !mbar_wait(&sh.o_empty[s], (uses[s] - 1) & 1, abort_flag, status, 7)) return false;
+                    if (!mbar_wait(&sh.p_full[s][at_s], (steps[s] >> 1) & 1, abort_flag, status, 7)) return false;
                     tc_fence_after();
-                    uint32_t k_lo = k_lo0 + k_at * (TILE_BYTES >> 4), q_lo = q_lo0 + (split ? 0 : s * (TILE_BYTES >> 4));
-                    const uint32_t d = tmem + COL_S + s * BK;
-                    if (one) {
-                        static_for<0, HD / 16>([&](auto ks) {
-                            constexpr uint32_t off = (((int)ks >> 2) * PANEL_BYTES + ((int)ks & 3) * 32) >> 4;
-                            mma_ss<((int)ks > 0)>(d, q_lo + off, k_lo + off, idesc_s);
-                        });
-                        tc_commit(&sh.s_full[s]);
-                        if (split || s == 1) tc_commit(&sh.empty[k_at]);
-                        if (i + 2 == N - 1) tc_commit(&sh.q_empty);            // (the run's last scores)
-                    }
+                    const uint32_t vp = v_lo0 + slot * (2 * KV_BYTES >> 4), pp = tmem + COL_S + (2 * s + at_s) * BK, d = tmem + COL_O + s * HD;
+                    mma_ts(d, pp, vp, idesc_o, i >= 2);
+                    static_for<1, BK / 16>([&](auto ks) { mma_ts(d, pp + (int)ks * 8, vp + (int)ks * (2048 >> 4), idesc_o, 1); });
+                    ++steps[s];
+                    if (i + 2 >= N) tc_commit(&sh.o_full[s]), ++uses[s];
+                    else if (i + 4 >= N) tc_commit(&sh.before_last[s]);
                 }
-                __syncwarp();
+                if (i + AHEAD < N) {
+                    const int at_s = scores[s] & 1;
+                    if (i < 0) tc_fence_after();
+                    const uint32_t k_lo = k_lo0 + slot * (2 * KV_BYTES >> 4), q_lo = q_lo0 + (split ? 0 : s * (Q_BYTES >> 4));
+                    const uint32_t d = tmem + COL_S + (2 * s + at_s) * BK;
+                    static_for<0, HD / 16>([&](auto ks) {
+                        constexpr uint32_t in = ((int)ks & 3) * 32, pn = (int)ks >> 2;
+                        mma_ss<((int)ks > 0)>(d, q_lo + ((pn * Q_PANEL + in) >> 4), k_lo + ((pn * KV_PANEL + in) >> 4), idesc_s);
+                    });
+                    tc_commit(&sh.s_full[s][at_s]);
+                    ++scores[s];
+                    if (i + AHEAD == N - 1) tc_commit(&sh.q_empty);            // (the run's last scores)
+                }
+                if (split || s == 1) {
+                    tc_commit(&sh.empty[slot]);        // (behind the last reader of both tiles)
+                    if (++slot == NSLOT) slot = 0, ++round;
+                }
+                return true;
+            };
+            if (one) {
+                ok = mbar_wait(&sh.q_full, k & 1, abort_flag, status, 7);
+#pragma unroll 1
+                for (int i = -AHEAD; ok && i < N; i += 2) {
+                    ok = turn(i, std::integral_constant<int, 0>{});
+                    if (ok && i + 1 < N) ok = turn(i + 1, std::integral_constant<int, 1>{});
+                }
             }
+            ok = __any_sync(0xffffffffu, one && ok);
         }
     } else {
         // ---------------- softmax: a row per thread ----------------
@@ -240,8 +222,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const int r = quad * 32 + lane;
         const float sl2 = scale * 1.4426950408889634f;
         const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-        const uint32_t s_addr = lane_base + COL_S + s * BK, o_addr = lane_base + COL_O + s * HD;
-        int step = 0, uses0 = 0, uses1 = 0, joins = 0; // this stream's blocks, both streams' runs, joins so far
+        const uint32_t o_addr = lane_base + COL_O + s * HD;
+        int step = 0, lasts = 0, uses0 = 0, uses1 = 0, joins = 0;  // this stream's blocks, its runs of two blocks or more, both streams' runs, joins so far
 #pragma unroll 1
         for (int at = blockIdx.x; ok && at < runs.all; at += gridDim.x, ++k) {
             seg = runs.segment(at);
@@ -254,43 +236,41 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
 #pragma unroll 1
             for (int j = (split ? s : 0) - (k == 0 ? dj : 0); j < n; j += dj) {
                 const bool rehearsed = j < 0, first = j < dj;      // (a block before the first: see REHEARSE)
+                const int at_s = step & 1;
+                const uint32_t s_addr = lane_base + COL_S + (2 * s + at_s) * BK;
                 if (!rehearsed) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s], step & 1, abort_flag, status, 7));
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s][at_s], (step >> 1) & 1, abort_flag, status, 7));
                     if (!ok) break;
                     ++step;
                 }
                 tc_fence_after();
-                auto hand_over = [&](int part) {
+                auto hand_over = [&]() {
                     if (rehearsed) return;
                     tc_st_wait();
                     tc_fence_before();                 // P and the rescaled O before it multiplies and accumulates
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.p_full[s][part]);
+                    if (lane == 0) mbar_arrive(&sh.p_full[s][at_s]);
                 };
+                if (!first && !rehearsed && j + dj >= n) {             // (no scores come behind the last block's: its rescaling waits here)
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.before_last[s], lasts & 1, abort_flag, status, 7));
+                    if (!ok) break;
+                    ++lasts;
+                }
                 if (!busy) {
-                    hand_over(0), hand_over(1);
+                    hand_over();
                     continue;
                 }
-                // Twice over the scores, 64 at a time, in loops: a run meets this code a few times, and each 128 bytes of it come from the
-                // L2 cache the first time.
-                const int parts = half(seg, j) ? 1 : 2;
-                float y[64];                           // the scores read last
-                auto read = [&](int part) {
-                    tc_ld32_nowait(s_addr + part * P_FIRST, reinterpret_cast<uint32_t*>(y));
-                    tc_ld32_nowait(s_addr + part * P_FIRST + 32, reinterpret_cast<uint32_t*>(y + 32));
-                    tc_ld_wait();
-                };
+                float y[BK];
+                tc_ld32_nowait(s_addr, reinterpret_cast<uint32_t*>(y));
+                tc_ld32_nowait(s_addr + 32, reinterpret_cast<uint32_t*>(y + 32));
+                tc_ld_wait();
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                for (int part = parts - 1; part >= 0; --part) {
-                    read(part);
 #pragma unroll
-                    for (int i = 0; i < 64; i += 8) {
-                        mx4[0] = max3(mx4[0], y[i], y[i + 1]);
-                        mx4[1] = max3(mx4[1], y[i + 2], y[i + 3]);
-                        mx4[2] = max3(mx4[2], y[i + 4], y[i + 5]);
-                        mx4[3] = max3(mx4[3], y[i + 6], y[i + 7]);
-                    }
+                for (int i = 0; i < BK; i += 8) {
+                    mx4[0] = max3(mx4[0], y[i], y[i + 1]);
+                    mx4[1] = max3(mx4[1], y[i + 2], y[i + 3]);
+                    mx4[2] = max3(mx4[2], y[i + 4], y[i + 5]);
+                    mx4[3] = max3(mx4[3], y[i + 6], y[i + 7]);
                 }
                 const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
                 const bool grow = mx > m + 8.0f;
@@ -301,7 +281,10 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                 }
                 const float neg_m = m == -INFINITY ? 0.f : -m;
                 if (!first && __any_sync(0xffffffffu, grow)) {
-                    // Rare.  (O holds the product of the block before: the scores of this one say so.)
+                    // Rare.  O must hold the product of the block before, which the next block's scores come behind.
+                    if (j + dj < n) ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[s][at_s ^ 1], (step >> 1) & 1, abort_flag, status, 7));
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 16) {
                         float o[16];
@@ -313,26 +296,20 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                 }
                 float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
                 const float2 sl2_2 = make_float2(sl2, sl2), neg_m2 = make_float2(neg_m, neg_m);
-#pragma unroll 1
-                for (int part = 0; part < 2; ++part) {
-                    if (part < parts) {
-                        if (part > 0) read(part);
 #pragma unroll
-                        for (int c = 0; c < 64; c += 32) {
-                            uint32_t packed[16];
+                for (int c = 0; c < BK; c += 32) {
+                    uint32_t packed[16];
 #pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                const float2 e = fma2(make_float2(y[c + i], y[c + i + 1]), sl2_2, neg_m2);
-                                const float2 p = make_float2(ex2(e.x), ex2(e.y));
-                                sum2[(i >> 1) & 3] = add2(sum2[(i >> 1) & 3], p);
-                                const __nv_bfloat162 h = __floats2bfloat162_rn(p.x, p.y);      // key 2k in the low half, key 2k + 1 in the high half
-                                packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
-                            }
-                            if (!rehearsed) tc_st16(s_addr + part * (P_FIRST / 2) + c / 2, packed);
-                        }
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 e = fma2(make_float2(y[c + i], y[c + i + 1]), sl2_2, neg_m2);
+                        const float2 p = make_float2(ex2(e.x), ex2(e.y));
+                        sum2[(i >> 1) & 3] = add2(sum2[(i >> 1) & 3], p);
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(p.x, p.y);      // key 2k in the low half, key 2k + 1 in the high half
+                        packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
                     }
-                    hand_over(part);
+                    if (!rehearsed) tc_st16(s_addr + c / 2, packed);
                 }
+                hand_over();
                 l = l * alpha + (((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y)));
                 if (rehearsed) m = -INFINITY, l = 0.f;
             }
@@ -428,7 +405,7 @@ int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, con
     WICK_REQUIRE(kv_pages * 2 * G.kv_heads * kPage <= INT32_MAX, "attention (shared prefix): a cache of %lld pages is beyond the copies' coordinates", (long long)kv_pages);
     CUtensorMap q_map, kv_map;
     if (int e = make_heads_map(&q_map, q, n_tokens, G.heads, HD, G.gs, G.rows / G.gs)) return e;
-    if (int e = make_bf16_map(&kv_map, kv, kv_pages * 2 * G.kv_heads * kPage, HD, kPage, "attention (shared prefix)")) return e;
+    if (int e = make_bf16_map(&kv_map, kv, kv_pages * 2 * G.kv_heads * kPage, HD, BK, "attention (shared prefix)")) return e;
     static bool raised = false;
     if (!raised) {
         WICK_CUDA(cudaFuncSetAttribute(attn_shared_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
