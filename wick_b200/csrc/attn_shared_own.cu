@@ -108,7 +108,6 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
         __syncwarp();
         if (lane == 0) {
             uint64_t* bar = v ? &sm.v_full : &sm.k_full;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_expect_tx(bar, TILE_BYTES);
             for (int pn = 0; pn < PANELS; ++pn)
                 tma_load_2d(&kv_map, bar, (v ? sm.v : sm.k) + pn * PANEL_BYTES, pn * 64, ((page * 2 + v) * G.kv_heads + next.s.column) * kPage);
@@ -202,6 +201,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
         if (valid < kPage) {                           // places without a token may hold anything: zeros
             for (int i = max(valid, 0) * (HD / 8) + lane; i < kPage * (HD / 8); i += 32)
                 *reinterpret_cast<uint4*>(sm.v + tile_off(i / (HD / 8), i % (HD / 8))) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // (before the next copy writes there)
             __syncwarp();
         }
 #pragma unroll
