@@ -88,6 +88,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
     // (The description lies ready before the step's kernels start.)
     const OwnParts parts{G, R, groups};
     Walk walk(parts, gridDim.x, nullptr);
+    const uint64_t policy = read_once_policy();
     Ahead next = {};
     auto know_ids = [&]() {                            // from page next.j on
         const int* table = G.page_table + (int64_t)next.s.cut.seq * G.table_width + next.s.cut.first;
@@ -110,7 +111,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
             uint64_t* bar = v ? &sm.v_full : &sm.k_full;
             mbar_expect_tx(bar, TILE_BYTES);
             for (int pn = 0; pn < PANELS; ++pn)
-                tma_load_2d(&kv_map, bar, (v ? sm.v : sm.k) + pn * PANEL_BYTES, pn * 64, ((page * 2 + v) * G.kv_heads + next.s.column) * kPage);
+                tma_load_2d(&kv_map, bar, (v ? sm.v : sm.k) + pn * PANEL_BYTES, pn * 64, ((page * 2 + v) * G.kv_heads + next.s.column) * kPage, policy);
         }
         __syncwarp();
     };

@@ -112,6 +112,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         // ---------------- producer ----------------
         const bool one = elect_one();
         int slot = 0, turn = 0;                        // of the ring
+        const uint64_t policy = read_once_policy();
 #pragma unroll 1
         for (int at = blockIdx.x; ok && at < runs.all; at += gridDim.x, ++k) {
             if (k > 0) seg = runs.segment(at), even = pages(0), odd = pages(1);
@@ -145,7 +146,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                         if (is_v ? i < 0 : j >= n) continue;
                         const int y = (((is_v ? v_page : k_page) * 2 + is_v) * G.kv_heads + seg.column / G.per_kv) * kPage;
                         for (int pn = 0; pn < PANELS; ++pn)
-                            tma_load_2d(&kv_map, &sh.full[slot], kv_s + (2 * slot + is_v) * KV_BYTES + pn * KV_PANEL, pn * 64, y);
+                            tma_load_2d(&kv_map, &sh.full[slot], kv_s + (2 * slot + is_v) * KV_BYTES + pn * KV_PANEL, pn * 64, y, policy);
                     }
                 }
                 if (++slot == NSLOT) slot = 0, ++turn;
