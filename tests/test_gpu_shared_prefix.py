@@ -181,6 +181,87 @@ def test_attention_shared_shows_infinities_and_nan(ops, dtype):
     assert bool(torch.isfinite(got).all())
 
 
+# Prefixes long enough for the kernel that computes them by themselves.
+LONG = {
+    # one tile of rows (both streams on it), an odd number of pages; one sequence brings nothing new
+    "one_tile": ([(63, [(3, 1), (0, 1), (130, 1), (64, 0), (17, 1), (9, 1), (1, 1)])], 32, 8),
+    # two tiles of rows, a stream each; heads that are no power of two, so that a tile has fewer than 128 rows
+    "two_tiles": ([(40, [(i % 70, 1) for i in range(37)])], 12, 2),
+    # three tiles: a pair and one by itself
+    "three_tiles": ([(30, [(i * 13 % 200, 1) for i in range(41)])], 16, 2),
+    # several tokens a sequence, groups of different lengths, one that shares nothing, an empty one
+    "tokens": ([(33, [(5, 9), (70, 1), (0, 30)]), (0, [(40, 3)]), (19, []), (52, [(64, 17), (1, 1)])], 16, 4),
+    # more items than thread blocks: some blocks have several runs, of one tile and of two
+    "many_runs": ([(1 + i * 7 % 9, [(i % 5, 1)] * (1 + i * 11 % 4)) for i in range(60)] + [(7, [(2, 9)] * 5)], 64, 16),
+    # one block of keys more than there are page numbers in a run of 32, two more
+    "runs_of_32": ([(33, [(3, 1)] * 8), (34, [(3, 1)] * 8), (65, [(0, 1)] * 40)], 32, 4),
+}
+
+
+def kernels_of(ops, call):
+    before = ops.launches[0]
+    call()
+    return ops.launches[0] - before
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shape", sorted(LONG))
+def test_attention_shared_behind_long_prefixes(ops, shape, dim):
+    groups, heads, kv_heads = LONG[shape]
+    if dim == 64:                                               # (the prefixes have to be twice as long there)
+        groups = [(2 * p + (p > 0), s) for p, s in groups]
+    case = Case(groups, heads, kv_heads, dim, BF16, seed=len(shape) + dim, more_width=1)
+    assert kernels_of(ops, lambda: check(case.run(ops), case)) == 3
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [5, 30])
+@pytest.mark.parametrize("slope", [12.0, -12.0, 300.0])
+def test_attention_shared_with_scores_that_rise(ops, slope, rows, dim):
+    """Scores that rise, or fall, by a multiple of the slope from page to page, so that the maximum moves in every block, or never."""
+    pages = 90 * 128 // dim
+    case = Case([(pages, [(i % 40, 1) for i in range(rows)])], 32, 8, dim, BF16, seed=rows)
+    u = torch.zeros(dim)
+    u[::2] = 1.0
+    case.q = (case.q.float() * 0.1 + 0.5 * u).to(BF16)
+    for j, page in enumerate(case.tables[0][:pages]):
+        case.kv[page, 0] = (case.kv[page, 0].float() + u * (slope * j / pages)).to(BF16)
+    assert kernels_of(ops, lambda: check(case.run(ops), case)) == 3
+    ops.check_status()
+
+
+def test_attention_shared_behind_a_long_prefix_shows_infinities_and_nan(ops):
+    case = Case([(60, [(10, 1), (70, 1), (5, 1), (9, 1)] * 4)], 16, 4, 128, BF16, seed=2)
+    page = case.tables[0][37]
+    case.kv[page, 1, 0, 7, 5] = math.inf
+    case.q[1, 5] = math.nan
+    got = case.run(ops).float().cpu()
+    assert bool((got[:, :4, 5] == math.inf).all()), "heads of key head 0 read it"
+    assert bool(torch.isnan(got[1, 5]).all())
+    got[:, :4, 5] = 0
+    got[1, 5] = 0
+    assert bool(torch.isfinite(got).all())
+
+
+def test_attention_shared_behind_a_long_prefix_same_bits_again(ops):
+    groups, heads, kv_heads = LONG["tokens"]
+    case = Case(groups, heads, kv_heads, 128, BF16, seed=4)
+    a = case.run(ops)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = case.run(ops, out=torch.empty_like(a))
+    s.synchronize()
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dim,dtype,kernels", [(64, BF16, 2), (128, BF16, 2), (48, BF16, 2), (128, F32, 2)])
+def test_attention_shared_counts_its_kernels(ops, dim, dtype, kernels):
+    case = Case([(2, [(10, 1), (70, 1)])], 4, 2, dim, dtype, seed=1)
+    assert kernels_of(ops, lambda: case.run(ops)) == kernels
+
+
 def test_attention_shared_same_bits_again_and_on_another_stream(ops):
     case = Case(SHAPES["groups"], 8, 2, 128, BF16, seed=4)
     a = case.run(ops)
@@ -224,6 +305,19 @@ def test_attention_shared_reports_a_sequence_that_is_shorter_than_its_group(ops)
     with pytest.raises(ops.KernelError, match="does not fit"):
         ops.check_status()
     assert bool((got[1] == 0).all())
+    ops.check_status()
+
+
+def test_attention_shared_reports_a_sequence_outside_its_group(ops):
+    case = Case([(2, [(10, 1), (70, 1)]), (2, [(3, 1)])], 4, 2, 64, BF16, seed=1)
+    shared = ops.SharedPrefix.of(case.sizes, case.shared, case.kv_lens, "cuda")
+    shared = shared._replace(group_of=ints([0, 1, 1]))          # (group 1 begins with the sequence behind)
+    got = ops.attention_shared(case.q.cuda(), case.kv.cuda(), case.batch(), shared, case.scale)
+    with pytest.raises(ops.KernelError, match="does not fit"):
+        ops.check_status()
+    assert bool((got[1] == 0).all())
+    want, most = case.want()
+    assert bool((((got.double().cpu() - want).abs() / most)[[0, 2]] <= 1.0).all()), "the others' are their own"
     ops.check_status()
 
 

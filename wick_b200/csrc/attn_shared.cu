@@ -621,10 +621,13 @@ static int attn_shared(const T* q, int n_tokens, const T* kv, int64_t kv_pages, 
 }  // namespace shared_prefix
 }  // namespace wick
 
-// float32 words of scratch that a call of these sizes needs (half: of the bfloat16 form; -1: refused, see wick_last_error).
-WICK_API long long wick_attn_shared_scratch(int half, int n_tokens, int n_seqs, int n_groups, int heads, int kv_heads, int max_pages, int own_bound, int max_q_len) {
+// float32 words of scratch that a call of these sizes needs (half: of the bfloat16 form; -1: refused, see wick_last_error), and the
+// kernels that it launches.
+WICK_API long long wick_attn_shared_scratch(int half, int n_tokens, int n_seqs, int n_groups, int heads, int kv_heads, int max_pages, int own_bound, int max_q_len,
+                                            int* kernels) {
     shared_prefix::Call c = {};
     if (shared_prefix::plan_call(c, half != 0, n_tokens, n_seqs, n_groups, heads, kv_heads, max_pages, own_bound, max_q_len)) return -1;
+    *kernels = n_tokens == 0 ? 0 : 2 + c.tc;
     return c.all();
 }
 

@@ -552,7 +552,7 @@ def _shared(head_dim: int) -> _Lib:
               f"attention kernels take a head_dim that is a multiple of 16 between 16 and 256, not {head_dim}")
         lib = _libs[key] = _Lib(f"wick_shared_hd{head_dim}", SHARED_SOURCES, [f"WICK_HD={head_dim}"])
         lib._lib.wick_attn_shared_scratch.restype = ctypes.c_longlong
-        lib._lib.wick_attn_shared_scratch.argtypes = [ctypes.c_int] * 9
+        lib._lib.wick_attn_shared_scratch.argtypes = [ctypes.c_int] * 9 + [ctypes.POINTER(ctypes.c_int)]
     return lib
 
 
@@ -584,18 +584,20 @@ class SharedPrefix(NamedTuple):
 
 
 @functools.lru_cache(maxsize=4096)
-def _shared_scratch(head_dim: int, *sizes: int) -> int:
+def _shared_scratch(head_dim: int, *sizes: int) -> Tuple[int, int]:
+    """float32 words of scratch of a call of these sizes, and the kernels that it launches."""
     lib = _shared(head_dim)
-    n = lib._lib.wick_attn_shared_scratch(*sizes)
+    kernels = ctypes.c_int(0)
+    n = lib._lib.wick_attn_shared_scratch(*sizes, ctypes.byref(kernels))
     if n < 0:
         raise KernelError(lib._lib.wick_last_error().decode("utf-8", "replace"))
-    return n
+    return n, kernels.value
 
 
 def attention_shared_scratch(shared: SharedPrefix, batch, n_heads: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> int:
     """float32 words of scratch that :func:`attention_shared` needs for this step."""
     return _shared_scratch(head_dim, dtype is torch.bfloat16, batch.n_tokens, batch.n_seqs, shared.pages.numel(), n_heads, n_kv, shared.max_pages,
-                           shared.own_bound, batch.max_q_len)
+                           shared.own_bound, batch.max_q_len)[0]
 
 
 def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPrefix, scale: float, scratch: Optional[torch.Tensor] = None,
@@ -617,8 +619,9 @@ def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPre
     _cuda("cu_groups", cu_groups, i32, (G + 1,))
     _cuda("pages", pages, i32)
     _cuda("group_of", group_of, i32, (n_seqs,))
+    words, kernels = _shared_scratch(hd, q.dtype is torch.bfloat16, n, n_seqs, G, n_heads, n_kv, max_pages, own_bound, batch.max_q_len)
     if scratch is None:
-        scratch = torch.empty(attention_shared_scratch(shared, batch, n_heads, n_kv, hd, q.dtype), dtype=torch.float32, device=q.device)
+        scratch = torch.empty(words, dtype=torch.float32, device=q.device)
     else:
         _cuda("scratch", scratch, torch.float32)
     if out is None:
@@ -628,7 +631,7 @@ def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPre
     _shared(hd).call(f"wick_attn_shared_{_dt(q)}", "piplppppipippiiiiiifplpp", q.data_ptr(), n, kv.data_ptr(), kv_pages, out.data_ptr(),
                      cu_groups.data_ptr(), pages.data_ptr(), group_of.data_ptr(), G, batch.cu_seqlens.data_ptr(), n_seqs, batch.start.data_ptr(),
                      batch.page_table.data_ptr(), batch.table_width, n_heads, n_kv, max_pages, own_bound, batch.max_q_len, scale, scratch.data_ptr(),
-                     scratch.numel(), status_tensor(q.device).data_ptr(), _stream(), kernels=2)
+                     scratch.numel(), status_tensor(q.device).data_ptr(), _stream(), kernels=kernels)
     return out
 
 
