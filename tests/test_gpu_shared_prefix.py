@@ -184,11 +184,11 @@ def test_attention_shared_shows_infinities_and_nan(ops, dtype):
 # Prefixes long enough for the kernel that computes them by themselves.
 LONG = {
     # one tile of rows (both streams on it), an odd number of pages; one sequence brings nothing new
-    "one_tile": ([(63, [(3, 1), (0, 1), (130, 1), (64, 0), (17, 1), (9, 1), (1, 1)])], 32, 8),
+    "one_tile": ([(127, [(3, 1), (0, 1), (130, 1), (64, 0), (17, 1), (9, 1), (1, 1)])], 32, 8),
     # two tiles of rows, a stream each; heads that are no power of two, so that a tile has fewer than 128 rows
-    "two_tiles": ([(40, [(i % 70, 1) for i in range(37)])], 12, 2),
+    "two_tiles": ([(70, [(i % 70, 1) for i in range(37)])], 12, 2),
     # three tiles: a pair and one by itself
-    "three_tiles": ([(30, [(i * 13 % 200, 1) for i in range(41)])], 16, 2),
+    "three_tiles": ([(50, [(i * 13 % 200, 1) for i in range(41)])], 16, 2),
     # several tokens a sequence, groups of different lengths, one that shares nothing, an empty one
     "tokens": ([(33, [(5, 9), (70, 1), (0, 30)]), (0, [(40, 3)]), (19, []), (52, [(64, 17), (1, 1)])], 16, 4),
     # more items than thread blocks: some blocks have several runs, of one tile and of two
@@ -220,7 +220,7 @@ def test_attention_shared_behind_long_prefixes(ops, shape, dim):
 @pytest.mark.parametrize("slope", [12.0, -12.0, 300.0])
 def test_attention_shared_with_scores_that_rise(ops, slope, rows, dim):
     """Scores that rise, or fall, by a multiple of the slope from page to page, so that the maximum moves in every block, or never."""
-    pages = 90 * 128 // dim
+    pages = 120 * 128 // dim
     case = Case([(pages, [(i % 40, 1) for i in range(rows)])], 32, 8, dim, BF16, seed=rows)
     u = torch.zeros(dim)
     u[::2] = 1.0
@@ -232,7 +232,7 @@ def test_attention_shared_with_scores_that_rise(ops, slope, rows, dim):
 
 
 def test_attention_shared_behind_a_long_prefix_shows_infinities_and_nan(ops):
-    case = Case([(60, [(10, 1), (70, 1), (5, 1), (9, 1)] * 4)], 16, 4, 128, BF16, seed=2)
+    case = Case([(110, [(10, 1), (70, 1), (5, 1), (9, 1)] * 4)], 16, 4, 128, BF16, seed=2)
     page = case.tables[0][37]
     case.kv[page, 1, 0, 7, 5] = math.inf
     case.q[1, 5] = math.nan

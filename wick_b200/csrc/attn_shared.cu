@@ -447,7 +447,7 @@ attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records share
     const Cut mine = parts(b);                      // (the description may be read before the wait)
     const int tok = row / G.heads, head = row - tok * G.heads, kvh = head / group, h = head - kvh * group, g = G.group_of[b];
     const bool there = tok < mine.n_tok && mine.pages > 0;
-    Cut c = Cut{0, 0, 0, 0, 0, 0, 0, 0};
+    Cut c = Cut{0, 0, 0, 0, 0, 0, 0};
     if (there) c = groups ? parts(G.n_seqs + g) : SharedParts{G}(g);
     pdl_wait();
     pdl_trigger();
@@ -517,7 +517,7 @@ using namespace wick;
 namespace wick {
 namespace shared_prefix {
 
-constexpr int FEW = 2000 * (HD < 128 ? 2 : 1);
+constexpr int FEW = 3500 * (HD < 128 ? 2 : 1);
 constexpr int PER_SM = 2;                          // thread blocks an SM, where the tcgen05 kernel does not run
 
 struct Call {
@@ -543,7 +543,7 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
     int gs = group;
     for (int n = 2; gs > TC_ROWS; ++n)
         if (group % n == 0) gs = group / n;
-    G.rows = TC_ROWS / gs * gs, G.gs = gs, G.per_kv = group / gs, G.columns = heads / gs, G.block = 1, G.pair = 2;
+    G.rows = TC_ROWS / gs * gs, G.gs = gs, G.per_kv = group / gs, G.columns = heads / gs, G.pair = 2;
     const int sms = sm_count(), rows_own = c.fast ? OWN_ROWS : R, own_per_sm = c.fast ? OWN_WARPS * (128 / HD) : PER_SM;
     const int64_t tiles = (int64_t)ceil_div((int64_t)n_tokens * gs, G.rows) + n_groups, items = (tiles / 2 + n_groups) * G.columns;
     const int64_t units = tiles * G.columns * max_pages;
@@ -551,8 +551,8 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
     const int64_t items_groups = max_pages > 0 ? ((int64_t)ceil_div((int64_t)n_tokens * group, rows_own) + n_groups) * kv_heads : 0;
     WICK_REQUIRE(units <= INT32_MAX / 2 && items_seqs * pages_own + items_groups * max_pages <= INT32_MAX / 2, "attention (shared prefix): too much for one step");
     // The shared keys have a kernel of their own from FEW pages of 8 rows on: fewer take the own keys' kernel, and one launch, less time (16
-    // sequences of 32 heads over 8 of 128: behind 1,024 positions 13.1 us together and 15.9 apart, 4,096 21.8 and 18.1; 48 of 24 over 4 of
-    // 64: 1,024 15.1 and 17.5, 4,096 26.7 and 21.4).
+    // sequences of 32 heads over 8 of 128: behind 2,048 positions 14.6 us together and 16.3 apart, 4,096 20.1 and 18.9; 48 of 24 over 4 of
+    // 64: 2,048 17.5 and 19.8, 4,096 24.9 and 21.3; over 120 sizes the better of the two is missed by 0.2 % and 0.7 % on average).
     c.tc = c.fast && items_groups * max_pages > FEW;
     int first = sms, second = own_per_sm * sms;
     if (c.tc) {
@@ -568,10 +568,13 @@ static int plan_call(Call& c, bool half, int n_tokens, int n_seqs, int n_groups,
         first = (int)min((int64_t)max(1, min(sms - 8, (int)(sms * work / (work + work_own)))), max((int64_t)1, units / 2));
         second = own_per_sm * (sms - first);
     }
-    // No more thread blocks than there can be runs of work.
-    const int64_t items_own = items_seqs + (c.tc ? 0 : items_groups);
+    // No more thread blocks than there can be runs of work; and few items with many pages are cut into longer runs than one page, since a row's
+    // records are joined sixteen at a time (4 sequences of 8 heads of 64 behind 16,384 positions: runs of one page 42 us, of seven 23; 4 of
+    // 32 over 8 of 128 behind 4,096: 14.8, 12.1).
+    const int64_t items_own = items_seqs + (c.tc ? 0 : items_groups), most = max(pages_own, c.tc ? (int64_t)0 : (int64_t)max_pages);
+    const int run = max(1, (int)sqrt(most / 5.0));
     c.blocks = (int)max((int64_t)1, min((int64_t)first, units / 2));
-    c.blocks_own = (int)max((int64_t)1, min((int64_t)second, items_seqs * pages_own + (c.tc ? 0 : items_groups * max_pages)));
+    c.blocks_own = (int)max((int64_t)1, min((int64_t)second, (items_seqs * pages_own + (c.tc ? 0 : items_groups * max_pages)) / run));
     c.plan_shared = c.tc ? (n_groups + 2 + 3) / 4 * 4 : 0;
     c.plan_own = (2 * (n_seqs + n_groups) + 3 + 3) / 4 * 4;
     c.shared_floats = c.tc ? max((int64_t)c.blocks, items) * 2 * TC_ROWS * (HD + 2) : 0;

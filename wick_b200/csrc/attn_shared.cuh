@@ -6,9 +6,9 @@
 // holds; the rest are the sequence's own.  Each part is kept as (m, l, o) = (maximum, sum of weights, weighted sum of values), all
 // in float32, and parts are joined by M = max m_i, l = sum l_i 2^(m_i - M), o likewise (scores in units of log2 e).
 //
-// Shared keys: a tile (or, where a thread block takes two, a pair of neighbouring tiles) is an ITEM.  An item's blocks of G.block pages are cut
-// into RUNS of equal length, the longest that still gives every thread block one run (see Runs): what a run costs besides its blocks is
-// as much as three of them, so a thread block should not have two.  Own keys (and shared ones, where they are few): a sequence's 16 or 8 rows
+// Shared keys: a tile (or, where a thread block takes two, a pair of neighbouring tiles) is an ITEM.  An item's pages are cut
+// into RUNS of equal length, the shortest that leaves no thread block with two (see Runs): what a run costs besides its pages (its
+// start and its record) is as much as ten of them.  Own keys (and shared ones, where they are few): a sequence's 16 or 8 rows
 // of one key head are an item, whose pages are dealt to the workers in equal contiguous runs, from one item into the next (see Walk).  Either way a record is
 // written per run and item, and who has what follows from the description alone: the kernel that joins finds the records by
 // arithmetic, in a fixed order.
@@ -30,13 +30,13 @@ struct Groups {
     int heads, kv_heads;
     int rows;                                      // of a tile
     int gs, per_kv, columns;                       // heads of a tile; tiles of heads to a key head, in all
-    int block, pair;                               // pages of a block of keys; tiles of an item, at most
+    int pair;                                      // tiles of an item, at most
 };
 __device__ __forceinline__ int pages_of(const Groups& G, int g) { return max(0, min(min(G.pages[g], G.max_pages), G.table_width)); }
 
 // Something whose tiles see the same keys: a group and its shared pages, or a sequence and its own.
 struct Cut {
-    int pages, tok0, n_tok, tiles, blocks;
+    int pages, tok0, n_tok, tiles;
     int seq, first, end;                           // the row of the page table, its first column, the end of the positions
 };
 struct SharedParts {
@@ -49,7 +49,6 @@ struct SharedParts {
         c.tok0 = G.single ? a : G.cu_seqlens[a];
         c.n_tok = (G.single ? b : G.cu_seqlens[b]) - c.tok0;
         c.tiles = c.pages > 0 ? (c.n_tok * G.gs + G.rows - 1) / G.rows : 0;
-        c.blocks = (c.pages + G.block - 1) / G.block;
         c.end = c.pages * kPage;
         return c;
     }
@@ -70,7 +69,6 @@ struct OwnParts {
         Cut c;
         if (shared(i)) {
             c = SharedParts{G}(i - G.n_seqs);
-            c.blocks = c.pages;
         } else {
             const int g = G.group_of[i];
             c.seq = i;
@@ -78,7 +76,7 @@ struct OwnParts {
             c.n_tok = G.single ? 1 : G.cu_seqlens[i + 1] - c.tok0;
             c.first = g >= 0 && g < G.n ? pages_of(G, g) : 0;
             c.end = G.start[i] + c.n_tok;
-            c.blocks = c.pages = c.n_tok > 0 && fits(i, c) ? (c.end + kPage - 1) / kPage - c.first : 0;
+            c.pages = c.n_tok > 0 && fits(i, c) ? (c.end + kPage - 1) / kPage - c.first : 0;
         }
         c.tiles = c.pages > 0 ? (c.n_tok * (G.heads / G.kv_heads) + rows - 1) / rows : 0;
         return c;
@@ -88,7 +86,7 @@ struct OwnParts {
 template <typename T> __device__ __forceinline__ void clear_unfit(const OwnParts& parts, T* out, int row_numbers, int* status) {
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < parts.G.n_seqs; b0 += 32) {
-        Cut c = Cut{0, 0, 0, 0, 0, 0, 0, 0};
+        Cut c = Cut{0, 0, 0, 0, 0, 0, 0};
         if (b0 + lane < parts.G.n_seqs) c = parts(b0 + lane);
         unsigned bad = __ballot_sync(0xffffffffu, c.n_tok > 0 && c.pages == 0);
         if (bad && lane == 0) atomicCAS(status, 0, 11);
@@ -110,7 +108,7 @@ struct Deal {
     __device__ __forceinline__ int worker_of(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
 };
 
-// A run's part of one item: `tiles` tiles from `tile` on, blocks (own: pages) from .. to.
+// A run's part of one item: `tiles` tiles from `tile` on, pages from .. to.
 struct Segment {
     Cut cut;
     int tile, tiles, column;
@@ -122,12 +120,12 @@ struct Segment {
 };
 
 // ---- shared keys -------------------------------------------------------------------
-// The blocks of a run of an item of w tiles: `run` for two tiles, twice as many for one (whose blocks cost half).
-__device__ __forceinline__ int run_blocks(const Groups& G, int run, int w) { return run * G.pair / w; }
+// The pages of a run of an item of w tiles: `run` for two tiles, twice as many for one (whose pages cost half).
+__device__ __forceinline__ int run_pages(const Groups& G, int run, int w) { return run * G.pair / w; }
 // Runs of an item of w tiles, of all items of a group.
 __device__ __forceinline__ int runs_of_item(const Groups& G, const Cut& c, int run, int w) {
-    const int n = run_blocks(G, run, w);
-    return (c.blocks + n - 1) / n;
+    const int n = run_pages(G, run, w);
+    return (c.pages + n - 1) / n;
 }
 __device__ __forceinline__ int runs_of(const Groups& G, const Cut& c, int run) {
     const int full = c.tiles / G.pair, rest = c.tiles - full * G.pair;
@@ -146,7 +144,7 @@ __device__ __forceinline__ Place place_of(const Groups& G, const Cut& c, int run
 // A warp's knowledge of all runs.  A lane knows one group of 32.
 struct Runs {
     const Groups& G;
-    int run, all;                                  // blocks of a run, all runs
+    int run, all;                                  // pages of a run, all runs
     int g0, before;                                // first of the groups known; runs of the groups before it
     Cut mine;
     int upto;                                      // runs up to this lane's group
@@ -154,7 +152,7 @@ struct Runs {
     __device__ __forceinline__ void know(int first) {
         g0 = first;
         const int g = g0 + (int)(threadIdx.x & 31);
-        mine = Cut{0, 0, 0, 0, 0, 0, 0, 0};
+        mine = Cut{0, 0, 0, 0, 0, 0, 0};
         if (g < G.n) mine = SharedParts{G}(g);
     }
     __device__ __forceinline__ void count() {
@@ -171,8 +169,8 @@ struct Runs {
         int cost = 0, most = 1;
         for (int g = 0; g < G.n; g += 32) {
             know(g);
-            cost += __reduce_add_sync(0xffffffffu, (unsigned)(mine.tiles * G.columns * mine.blocks));
-            most = max(most, (int)__reduce_max_sync(0xffffffffu, (unsigned)(mine.tiles > 0 ? mine.blocks : 0)));
+            cost += __reduce_add_sync(0xffffffffu, (unsigned)(mine.tiles * G.columns * mine.pages));
+            most = max(most, (int)__reduce_max_sync(0xffffffffu, (unsigned)(mine.tiles > 0 ? mine.pages : 0)));
         }
         run = max(1, (cost + blocks * G.pair - 1) / (blocks * G.pair));
         for (;; run += 1 + run / 16) {
@@ -186,7 +184,7 @@ struct Runs {
         if (G.n > 32) know(0);
         count();
     }
-    // plan: the blocks of a run, then the runs before each group.
+    // plan: the pages of a run, then the runs before each group.
     __device__ __forceinline__ void write(int* plan) {
         if ((threadIdx.x & 31) == 0) plan[0] = run, plan[1] = 0;
         for (int g = 0; g < G.n; g += 32) {
@@ -202,14 +200,14 @@ struct Runs {
         Cut& c = s.cut;
         c.pages = __shfl_sync(0xffffffffu, mine.pages, l), c.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);
         c.n_tok = __shfl_sync(0xffffffffu, mine.n_tok, l), c.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
-        c.blocks = __shfl_sync(0xffffffffu, mine.blocks, l), c.seq = __shfl_sync(0xffffffffu, mine.seq, l);
+        c.seq = __shfl_sync(0xffffffffu, mine.seq, l);
         c.first = 0, c.end = c.pages * kPage;
         const int local = r - (l > 0 ? __shfl_sync(0xffffffffu, upto, l - 1) : before);
         const int per = G.columns * runs_of_item(G, c, run, G.pair), full = c.tiles / G.pair;
         const int pair = min(full, local / per), w = pair < full ? G.pair : c.tiles - full * G.pair, n = runs_of_item(G, c, run, w), rest = local - pair * per;
         s.column = rest / n;
         s.tile = pair * G.pair, s.tiles = w;
-        s.from = (rest - s.column * n) * run_blocks(G, run, w), s.to = min(c.blocks, s.from + run_blocks(G, run, w));
+        s.from = (rest - s.column * n) * run_pages(G, run, w), s.to = min(c.pages, s.from + run_pages(G, run, w));
         s.record = r;
         return s;
     }
@@ -227,7 +225,7 @@ struct Walk {
 
     __device__ __forceinline__ Cut cut(int first) const {
         const int b = first + (int)(threadIdx.x & 31);
-        return b < parts.n() ? parts(b) : Cut{0, 0, 0, 0, 0, 0, 0, 0};
+        return b < parts.n() ? parts(b) : Cut{0, 0, 0, 0, 0, 0, 0};
     }
     __device__ __forceinline__ void know(int first, const Cut& c) {
         b0 = first, mine = c;
@@ -269,7 +267,7 @@ struct Walk {
         Cut& c = s.cut;
         c.pages = __shfl_sync(0xffffffffu, mine.pages, l), c.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);
         c.n_tok = __shfl_sync(0xffffffffu, mine.n_tok, l), c.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
-        c.seq = __shfl_sync(0xffffffffu, mine.seq, l), c.blocks = c.pages;
+        c.seq = __shfl_sync(0xffffffffu, mine.seq, l);
         c.first = __shfl_sync(0xffffffffu, mine.first, l), c.end = __shfl_sync(0xffffffffu, mine.end, l);
         const int local = u - __shfl_sync(0xffffffffu, upto_units - mine.tiles * columns * mine.pages, l), item = local / c.pages;
         s.shared = parts.shared(b0 + l);
@@ -295,8 +293,8 @@ __device__ __forceinline__ float weight(float a, float b) { return a == -INFINIT
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// The forms for bfloat16 at head sizes 64 and 128: the shared part on tcgen05 (attn_shared_tc.cu; tiles of up to TC_ROWS rows, two an item,
-// blocks of two pages), and the own keys streamed through shared memory (attn_shared_own.cu).
+// The forms for bfloat16 at head sizes 64 and 128: the shared part on tcgen05 (attn_shared_tc.cu; tiles of up to TC_ROWS rows, two an
+// item), and the own keys streamed through shared memory (attn_shared_own.cu).
 constexpr int TC_ROWS = 128, OWN_ROWS = 8, OWN_WARPS = 6;    // (warps an SM at head size 128, twice as many at 64)
 bool fast_supported();
 int launch_tc(const void* q, int n_tokens, const void* kv, int64_t kv_pages, const Groups& G, int blocks, float scale, int* plan, float* records, int* status,
