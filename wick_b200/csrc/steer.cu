@@ -63,11 +63,15 @@ struct Steer {
     const int* mask_of;        // [n_rows], -1: none
 };
 
-// A block takes four tokens a thread of one row.  VEC: x and y lie alike to 16 bytes, so that the four are one load and one store; a row of
-// odd length begins in the middle of four, and their bits then lie in two words.
-template <bool VEC>
+// A block takes G tokens a thread of one row: four, or, where that is more than two rounds of blocks, eight, whose bits, block's prologue and
+// turn cost half as many instructions, which bound a large call (61 rows of 100,003, half of them masked: 16.1 us and 15.0; 8 of
+// 151,936: 4.3 and 5.0).
+// VEC: x and y lie alike to 16 bytes, so that four tokens are one load and one store; a row of odd length begins in the middle of four, and
+// the bits of a thread's tokens then lie in two words.
+template <int G, bool VEC>
 __global__ void __launch_bounds__(HT) steer_kernel(const Steer a) {
-    constexpr int CH = HT * 4;
+    constexpr int CH = HT * G;
+    constexpr unsigned ALL = (1u << G) - 1;
     __shared__ float bias[CH];
     __shared__ unsigned biased[CH / 32];
     pdl_trigger();
@@ -101,43 +105,50 @@ __global__ void __launch_bounds__(HT) steer_kernel(const Steer a) {
         }
         biases = __syncthreads_or(biases);
     }
-    // bits of four tokens from e on (e >= 0, e < V)
-    auto four = [&](const unsigned* w, int e) -> unsigned {
+    // bits of the G tokens from e on (0 <= e, e + G <= V)
+    auto bits = [&](const unsigned* w, int e) -> unsigned {
         const int k = e >> 5, s = e & 31;
-        unsigned v = w[k] >> s;
-        if (s > 28 && k + 1 < a.words) v |= w[k + 1] << (32 - s);
-        return v & 15u;
+        return __funnelshift_r(w[k], s > 32 - G ? w[k + 1] : 0u, s) & ALL;
     };
-    // n: the token's count if it was seen, else 0
-    auto one = [&](float l, int e, bool is_seen, bool is_allowed, int n) -> float {
-        if (is_seen) l = l > 0.f ? __fdiv_rn(l, rep) : l * rep;
-        if (n > 0) l -= fmaf(freq, (float)n, pres);
-        if (biases && (biased[(e - e0) >> 5] >> ((e - e0) & 31) & 1)) l += bias[e - e0];
-        return is_allowed ? l : -INFINITY;
-    };
-    const int e = e0 + (int)threadIdx.x * 4;
-    if (VEC && e >= 0 && e + 4 <= V) {
-        const unsigned s4 = seen ? four(seen, e) : 0u, a4 = mask ? four(mask, e) : 15u;
-        float4 o = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (a4) {
-            const float4 v = *reinterpret_cast<const float4*>(x + e);
-            // (the four counts are asked for together: behind one another they took longer than all the rest)
-            const unsigned want = s4 & a4;
-            const int n0 = want & 1 ? counts[e] : 0, n1 = want & 2 ? counts[e + 1] : 0, n2 = want & 4 ? counts[e + 2] : 0,
-                      n3 = want & 8 ? counts[e + 3] : 0;
-            o = v;
-            if (a4 != 15u || s4 != 0u || biases) {
-                o.x = one(v.x, e, s4 & 1, a4 & 1, n0);
-                o.y = one(v.y, e + 1, s4 & 2, a4 & 2, n1);
-                o.z = one(v.z, e + 2, s4 & 4, a4 & 4, n2);
-                o.w = one(v.w, e + 3, s4 & 8, a4 & 8, n3);
-            }
+    auto one = [&](float l, int e, bool is_seen, bool is_biased) -> float {
+        if (is_seen) {
+            const int n = counts[e];
+            l = l > 0.f ? __fdiv_rn(l, rep) : l * rep;
+            if (n > 0) l -= fmaf(freq, (float)n, pres);
         }
-        *reinterpret_cast<float4*>(y + e) = o;
+        return is_biased ? l + bias[e - e0] : l;
+    };
+    const int at = (int)threadIdx.x * G, e = e0 + at;
+    const unsigned biased_bits = biases ? biased[at >> 5] >> (at & 31) & ALL : 0u;
+    if (VEC && e >= 0 && e + G <= V) {
+        const unsigned seen_bits = seen ? bits(seen, e) : 0u, allowed = mask ? bits(mask, e) : ALL;
+        float o[G];
+#pragma unroll
+        for (int h = 0; h < G; h += 4) {           // (four that are left out are not read)
+            float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (allowed >> h & 15) v = *reinterpret_cast<const float4*>(x + e + h);
+            o[h] = v.x, o[h + 1] = v.y, o[h + 2] = v.z, o[h + 3] = v.w;
+        }
+        // Few tokens are seen or biased: a turn for each of the thread's, which is one or none nearly always.
+        for (unsigned w = (seen_bits | biased_bits) & allowed; w; w &= w - 1) {
+            const int k = __ffs(w) - 1;
+            float l = o[0];
+#pragma unroll
+            for (int i = 1; i < G; ++i) l = k == i ? o[i] : l;
+            l = one(l, e + k, seen_bits >> k & 1, biased_bits >> k & 1);
+#pragma unroll
+            for (int i = 0; i < G; ++i) o[i] = k == i ? l : o[i];
+        }
+        if (allowed != ALL) {
+#pragma unroll
+            for (int i = 0; i < G; ++i) o[i] = allowed >> i & 1 ? o[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < G; h += 4) *reinterpret_cast<float4*>(y + e + h) = make_float4(o[h], o[h + 1], o[h + 2], o[h + 3]);
     } else {
-        for (int k = max(e, 0); k < min(e + 4, V); ++k) {
-            const bool is_seen = seen && (seen[k >> 5] >> (k & 31) & 1);
-            y[k] = one(x[k], k, is_seen, !mask || (mask[k >> 5] >> (k & 31) & 1), is_seen ? counts[k] : 0);
+        for (int k = max(e, 0); k < min(e + G, V); ++k) {
+            const float l = one(x[k], k, seen && (seen[k >> 5] >> (k & 31) & 1), biased_bits >> (k - e) & 1);
+            y[k] = !mask || (mask[k >> 5] >> (k & 31) & 1) ? l : -INFINITY;
         }
     }
 }
@@ -174,9 +185,10 @@ WICK_API int wick_steer_logits(const float* x, int64_t x_stride, float* y, int64
     Steer a = {x, y, x_stride, y_stride, vocab, (vocab + 31) / 32, n_rows, n_masks, rows, (const unsigned*)seen, counts, penalties,
                bias_cu, bias_tokens, bias_values, (const unsigned*)masks, mask_of};
     const bool alike = (((uintptr_t)x ^ (uintptr_t)y) & 15) == 0 && (x_stride - y_stride) % 4 == 0;
-    if (alike)
-        WICK_CUDA(launch(steer_kernel<true>, dim3(ceil_div(vocab + 3, HT * 4), n), dim3(HT), 0, (cudaStream_t)s, a));
-    else
-        WICK_CUDA(launch(steer_kernel<false>, dim3(ceil_div(vocab, HT * 4), n), dim3(HT), 0, (cudaStream_t)s, a));
+    const bool eight = alike && (int64_t)ceil_div(vocab, HT * 4) * n > 16 * sm_count();
+    const dim3 grid(ceil_div(vocab + (alike ? 3 : 0), HT * (eight ? 8 : 4)), n);
+    if (eight) WICK_CUDA(launch(steer_kernel<8, true>, grid, dim3(HT), 0, (cudaStream_t)s, a));
+    else if (alike) WICK_CUDA(launch(steer_kernel<4, true>, grid, dim3(HT), 0, (cudaStream_t)s, a));
+    else WICK_CUDA(launch(steer_kernel<4, false>, grid, dim3(HT), 0, (cudaStream_t)s, a));
     return check_launch("steer_logits");
 }
