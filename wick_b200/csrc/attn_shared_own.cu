@@ -8,9 +8,14 @@
 // rows on the 8-wide one (with rows on the 16-row side a page took twice the instructions, of which a token of 4 or 8 heads needs half);
 // weights are turned into the second product's operand by movmatrix, rounded to bfloat16; their sum is taken of the rounded ones.  Every item
 // leaves a record per run that has a part of it.
-// Bound by the bytes of the keys and values.  (Measured and left: blocks of four or eight warps that shared a page met three times
-// a page, 2,000 clocks of latency that two blocks an SM could not hide: 64 sequences of 370 own positions, 8 key heads, 28 us.)
-// The kernel of the shared part runs before this one, which starts under its last blocks.
+// Bound by the bytes of the keys and values: with all SMs a page takes a warp 4 us, 7 TB/s, behind a start of 3 us (the description, then the
+// first page); on the 65 SMs that the shared part leaves by one warp's chain, copy - scores - weights - values, 2.2 us a page.  64 sequences of
+// 370 own positions, 8 key heads of 128 (97 MB): 23 us there; 4 sequences behind 512 positions, both parts: 5.6 us.
+// (Measured and left: blocks of four or eight warps that shared a page met three times a page, 2,000 clocks of latency that two blocks an SM
+// could not hide, 28 us; half a page a turn and twice the warps, 24 us in place of 26, but twice the records: steps of few keys lost 10 to
+// 25 %.)
+// The kernel of the shared part runs before this one, which starts under its last blocks.  A page's place is read by the warp that has the next
+// page copied there, before; only where zeros were written there does a fence stand between.
 #include "tcgen05.cuh"
 #include "attn_shared.cuh"
 

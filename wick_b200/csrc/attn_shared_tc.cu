@@ -2,20 +2,28 @@
 // (maximum, sum of weights, weighted sum of values) for every run of units of a tile of 128 rows (attn_shared.cuh).
 //
 // A tile's rows are query heads of one key head times the group's tokens, whatever sequences they belong to: all of them see all
-// shared keys, so there is no mask anywhere.  A block of keys is two pages (the last one of an odd number: one).  There are two streams, each
-// with its own scores and its own sums in tensor memory and four softmax warps, so that one stream's softmax runs beside the other's
-// products:
+// shared keys, so there is no mask anywhere.  A block of keys is a page.  There are two streams, each with its own sums and two places for
+// scores in tensor memory (4 x 64 columns, and twice the head size) and four softmax warps, so that one stream's softmax runs beside the
+// other's products, and a stream's softmax of one block beside the scores of its next:
 //   * a group of more than 128 rows: two tiles of rows, a stream each, that share every tile of keys and values;
 //   * the last tile of an odd number: even blocks of keys go to one stream, odd ones to the other, joined when the run ends.
 // Roles:
-//   * a producer warp fetches the query rows of a run and its key and value tiles through a ring (TMA, 128-byte swizzle);
-//   * an issuing warp alternates between the streams: O += P V of one, then the scores S = Q K^T of its next block (P lies over the
-//     scores it came from, as bfloat16 pairs);
+//   * a producer warp fetches the query rows of a run and its key and value tiles through a ring (TMA, 128-byte swizzle, first to leave the
+//     L2 cache: each is read once, and the records, which are read again, stay there; 24 sequences behind 31,000 positions 60.7 and 55.6 us);
+//   * an issuing lane alternates between the streams: O += P V of one, then the scores S = Q K^T of its block after the next (P lies over
+//     the scores it came from, as bfloat16 pairs).  It waits by itself, without votes, and arrives once a block for both of its tiles:
+//     with a whole warp's votes and an arrival for each tile and product a turn took 1,400 clocks, of which 580 were its instructions;
 //   * a softmax thread owns a row.  O and the sum are scaled by a maximum that follows the true one lazily: O is rescaled only when a
 //     block's maximum exceeds it by more than 8 (in units of log2 e).  Warps whose rows are all beyond the group's tokens compute nothing.
+//     Weights enter the second product rounded to bfloat16, as its operand has to be; their sum is taken of the unrounded ones, in 32 bits.
 // REHEARSE: a run has few blocks, and a block's code is met for the first time while all SMs fill their rings: instructions then
-// come through the same queues as 24 MB of keys and values, and the first block's softmax took 4,300 clocks, the first products 4,100.
-// So the softmax warps go through their code once while there is nothing to do yet.
+// come through the same queues as 24 MB of keys and values, and the first block's softmax took 4,300 clocks.  So the softmax warps go through
+// their code once while there is nothing to do yet.  (The issuing lane does not: it changed nothing.)
+// What bounds it: the start of a run (10 to 15 thousand clocks until four turns are through, of which the kernel before hides 4), then the
+// tensor pipe, 830 clocks a turn of 12 products (64 keys of a stream; the softmax beside it 550; scores of 64 columns cost as much as of
+// 128, but with 128 there is room for one place each, and a stream then stands still between its softmax and its next scores: 1,100).  64
+// sequences behind 8,192 positions, 32 heads over 8 of 128, on 83 SMs: 24.8 us; 24 behind 31,000, 64 over 8, on 128 SMs: 46 us.
+// (Measured and left: an issuing warp for either stream, 1 to 2 % of long runs and as much slower short ones.)
 // Every wait is bounded and reports through the status word (code 7).
 #include "tc_attention.cuh"
 #include "attn_shared.cuh"

@@ -10,6 +10,7 @@
 // One launch: every block makes the sums over all sequences for itself (a few thousand numbers from the L2 cache; a second
 // launch, or blocks that wait for one another, would cost more than that), then a warp fills a sequence's row, a thread a
 // token.  Record 0 is the padding's: it gets no pages.
+// Bound by that chain: 48 sequences of a token each 3.5 us, 700 with 300 forks and up to 400 tokens each (5 MB written) 9.1.
 #include "common.cuh"
 
 namespace wick {
