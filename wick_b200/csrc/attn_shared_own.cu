@@ -256,6 +256,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
 int launch_own(const void* q, const void* kv, int64_t kv_pages, void* out, const Groups& G, int groups, bool after_shared, int blocks, float scale, int* plan,
                float* records, int* status, cudaStream_t s) {
     using namespace own;
+    WICK_REQUIRE(kv_pages * 2 * G.kv_heads * kPage <= INT32_MAX, "attention (shared prefix): a cache of %lld pages is beyond the copies' coordinates", (long long)kv_pages);
     CUtensorMap kv_map;
     if (int e = make_bf16_map(&kv_map, kv, kv_pages * 2 * G.kv_heads * kPage, HD, kPage, "attention (shared prefix)")) return e;
     static bool raised = false;
