@@ -11,7 +11,7 @@
 // keys' rows and pairs them by byte permutation.  No shared memory, no barrier until the warps' parts are joined.  Weights enter the second
 // product rounded to bfloat16, and their sum is taken of the rounded ones, so that a row of equal values keeps them.
 // float32: products and sums on the CUDA cores, keys and values through shared memory, 32 keys at a time: bound by the shared memory's reads
-// for them (6 sequences behind 1,000 positions, 16 heads over 4 of 128: 14.1 us, 7 MB).
+// for them (6 sequences behind 1,000 positions, 16 heads over 4 of 128: 12.2 us, 7 MB).
 // The join is bound by a chain (plan, then records that other SMs have just written) and, where there are many, by the records' bytes: 64
 // sequences of 32 heads with ten records a row of the shared keys, 11 MB, 7 us; 4 of 16 heads 4.5.
 #include "common.cuh"
@@ -233,10 +233,14 @@ __device__ __forceinline__ void copy16(void* dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(n) : "memory");
 }
 
-// A warp has the scores of four rows with a tile's 32 keys, a thread the sums of four rows and four columns.
+// A warp has the scores of four rows with a tile's 32 keys, a thread the sums of four rows and four columns.  FEW: where there are four rows at
+// most (a token of up to four heads), a warp has a quarter of the tile's keys, a lane one row's score with one of them, then four columns of
+// all four rows; the warps' parts are joined at the end (11 sequences of up to 1,085 own positions behind 732, 8 heads of 64 over 8: 24.5 us,
+// and 27.8 with a quarter of the warps at work).
+template <bool FEW>
 __device__ void attend(Work<float>& w, const Rows<float>& rows, const float* __restrict__ kv, int64_t kv_pages, const int* __restrict__ tab, int kvh,
                        int n_kv, int key0, int key1, float scale, int* status) {
-    constexpr int KT = Work<float>::KT, ITEMS = (HD + THREADS - 1) / THREADS;
+    constexpr int KT = Work<float>::KT, ITEMS = FEW ? (HD / 4 + 31) / 32 : (HD + THREADS - 1) / THREADS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float sl2 = scale * LOG2E;
     for (int i = tid; i < R * HD / 4; i += THREADS) {
@@ -280,6 +284,52 @@ __device__ void attend(Work<float>& w, const Rows<float>& rows, const float* __r
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         __syncthreads();
+        if constexpr (FEW) {
+            const int mine = warp * 8 + (lane & 7), row = lane >> 3;
+            float t4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 4) {
+                const float4 k4 = *reinterpret_cast<const float4*>(&w.k[i & 1][mine][d]), q4 = *reinterpret_cast<const float4*>(&w.q[row][d]);
+                t4[0] = fmaf(q4.x, k4.x, t4[0]), t4[1] = fmaf(q4.y, k4.y, t4[1]), t4[2] = fmaf(q4.z, k4.z, t4[2]), t4[3] = fmaf(q4.w, k4.w, t4[3]);
+            }
+            const int key = key0 + i * KT + mine;
+            const float x = key < key1 && key <= rows.last[row] ? ((t4[0] + t4[1]) + (t4[2] + t4[3])) * sl2 : -INFINITY;
+            float n = x;
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, o));
+            n = fmaxf(m[0], n);
+            const float a = weight(m[0], n), p = weight(x, n);
+            l[0] = l[0] * a + p;                       // (of this lane's keys)
+            m[0] = n;
+            float ar[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ar[r] = __shfl_sync(0xffffffffu, a, r * 8);
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[it][r][e] *= ar[r];
+#pragma unroll
+            for (int key = 0; key < 8; ++key) {
+                float pr[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) pr[r] = __shfl_sync(0xffffffffu, p, r * 8 + key);
+#pragma unroll
+                for (int it = 0; it < ITEMS; ++it) {
+                    const int c = (it * 32 + lane) * 4;
+                    if (c >= HD) continue;
+                    const float4 v4 = *reinterpret_cast<const float4*>(&w.v[i & 1][warp * 8 + key][c]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        acc[it][r][0] = fmaf(pr[r], v4.x, acc[it][r][0]), acc[it][r][1] = fmaf(pr[r], v4.y, acc[it][r][1]);
+                        acc[it][r][2] = fmaf(pr[r], v4.z, acc[it][r][2]), acc[it][r][3] = fmaf(pr[r], v4.w, acc[it][r][3]);
+                    }
+                }
+            }
+            __syncthreads();
+            continue;
+        }
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int d = 0; d < HD; d += 4) {
@@ -328,6 +378,39 @@ __device__ void attend(Work<float>& w, const Rows<float>& rows, const float* __r
         }
         __syncthreads();
     }
+    if constexpr (FEW) {
+        // the warps' parts, in the place of the keys: [W][4][HD] sums, [W][4] maxima and sums of weights
+        float *parts = &w.k[0][0][0], *ml = parts + W * 4 * HD;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+        if ((lane & 7) == 0) ml[(warp * 4 + (lane >> 3)) * 2] = m[0], ml[(warp * 4 + (lane >> 3)) * 2 + 1] = l[0];
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            const int c = (it * 32 + lane) * 4;
+            if (c >= HD) continue;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<float4*>(parts + (warp * 4 + r) * HD + c) = make_float4(acc[it][r][0], acc[it][r][1], acc[it][r][2], acc[it][r][3]);
+        }
+        __syncthreads();
+        for (int idx = tid; idx < 4 * HD; idx += THREADS) {
+            const int r = idx / HD, c = idx % HD;
+            float mm = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < W; ++k) mm = fmaxf(mm, ml[(k * 4 + r) * 2]);
+#pragma unroll
+            for (int k = 0; k < W; ++k) sum = fmaf(parts[(k * 4 + r) * HD + c], weight(ml[(k * 4 + r) * 2], mm), sum);
+            w.o[0][r][c] = sum;
+        }
+        if (tid < 4) {
+            float mm = -INFINITY, sum = 0.f;
+            for (int k = 0; k < W; ++k) mm = fmaxf(mm, ml[(k * 4 + tid) * 2]);
+            for (int k = 0; k < W; ++k) sum = fmaf(ml[(k * 4 + tid) * 2 + 1], weight(ml[(k * 4 + tid) * 2], mm), sum);
+            w.m[0][tid] = mm, w.l[0][tid] = sum;
+        }
+        __syncthreads();
+        return;
+    }
     if (lane == 0) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) w.m[0][warp * 4 + r] = m[r], w.l[0][warp * 4 + r] = l[r];
@@ -367,12 +450,13 @@ template <typename T> __device__ __forceinline__ float4 columns_of(const Work<T>
     }
     return s;
 }
-template <typename T> __device__ __forceinline__ void write_record(const Work<T>& w, float* rec) {
+template <typename T> __device__ __forceinline__ void write_record(const Work<T>& w, float* rec, int n_rows) {
     for (int i = threadIdx.x; i < R * HD / 4; i += THREADS) {
         const int r = i % R, c = i / R;
+        if (r >= n_rows) continue;
         *reinterpret_cast<float4*>(rec + i * 4) = columns_of(w, r, c * 4, max_of(w, r));
     }
-    if (threadIdx.x < R) {
+    if ((int)threadIdx.x < min(R, n_rows)) {
         const float m = max_of(w, threadIdx.x);
         *reinterpret_cast<float2*>(rec + R * HD + 2 * threadIdx.x) = make_float2(m, sum_of(w, threadIdx.x, m));
     }
@@ -402,9 +486,12 @@ attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, 
             rows.last[threadIdx.x] = there ? s.last(tok) : -1;
         }
         __syncthreads();
-        attend(w, rows, kv, kv_pages, G.page_table + (int64_t)s.cut.seq * G.table_width, s.column, G.kv_heads, (s.cut.first + s.from) * kPage,
-               min((s.cut.first + s.to) * kPage, s.cut.end), scale, status);
-        write_record(w, records + (int64_t)s.record * REC);
+        const int* table = G.page_table + (int64_t)s.cut.seq * G.table_width;
+        const int n_rows = s.cut.n_tok * group - s.tile * R, key0 = (s.cut.first + s.from) * kPage, key1 = min((s.cut.first + s.to) * kPage, s.cut.end);
+        if constexpr (sizeof(T) == 2) attend(w, rows, kv, kv_pages, table, s.column, G.kv_heads, key0, key1, scale, status);
+        else if (n_rows <= 4) attend<true>(w, rows, kv, kv_pages, table, s.column, G.kv_heads, key0, key1, scale, status);
+        else attend<false>(w, rows, kv, kv_pages, table, s.column, G.kv_heads, key0, key1, scale, status);
+        write_record(w, records + (int64_t)s.record * REC, n_rows);
     }
     if (blockIdx.x == 0 && threadIdx.x < 32) {
         Walk(parts, gridDim.x, plan);
@@ -521,7 +608,9 @@ namespace wick {
 namespace shared_prefix {
 
 constexpr int FEW = 3500 * (HD < 128 ? 2 : 1);
-constexpr int PER_SM = 2;                          // thread blocks an SM, where the tcgen05 kernel does not run
+// Thread blocks an SM of the form for any head size: what its shared memory holds (the same: 20.5 us, and 24.5 with two everywhere; 24 sequences
+// behind 3,000 positions, 24 heads over 4 of 64, float32: 38.9 and 50.4).
+constexpr int PER_SM = HD > 128 ? 1 : 256 / HD < 8 ? 256 / HD : 8;
 
 struct Call {
     Groups G;
