@@ -16,6 +16,7 @@
 // sequences of 32 heads with ten records a row of the shared keys, 11 MB, 7 us; 4 of 16 heads 4.5.
 #include "common.cuh"
 #include "attn_shared.cuh"
+#include "packed.cuh"
 
 #ifndef WICK_HD
 #error "compile with -DWICK_HD=<head_dim>"
@@ -742,3 +743,5 @@ WICK_API long long wick_attn_shared_scratch(int half, int n_tokens, int n_seqs, 
     }
 WICK_ATTN_SHARED(wick_attn_shared_bf16, __nv_bfloat16)
 WICK_ATTN_SHARED(wick_attn_shared_f32, float)
+WICK_PACKED(wick_attn_shared_bf16)
+WICK_PACKED(wick_attn_shared_f32)

@@ -14,6 +14,7 @@
 // 14.6 us, where what stands behind the bytes is 190 instructions a warp) and by one chain of dependent reads in small ones (place, mask,
 // bits, count: 8 rows of 151,936 in 4.5 us, one of 32,768 in 2.6).  History calls are a launch (2.4 us each in a graph).
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace wick {
 
@@ -194,3 +195,6 @@ WICK_API int wick_steer_logits(const float* x, int64_t x_stride, float* y, int64
     else WICK_CUDA(launch(steer_kernel<4, false>, grid, dim3(HT), 0, (cudaStream_t)s, a));
     return check_launch("steer_logits");
 }
+WICK_PACKED(wick_history_clear)
+WICK_PACKED(wick_history_add)
+WICK_PACKED(wick_steer_logits)

@@ -12,6 +12,7 @@
 // token.  Record 0 is the padding's: it gets no pages.
 // Bound by that chain: 48 sequences of a token each 3.5 us, 700 with 300 forks and up to 400 tokens each (5 MB written) 9.1.
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace wick {
 
@@ -144,3 +145,4 @@ WICK_API int wick_step_tables(const int* start, const int* q_len, const int* slo
     WICK_CUDA(launch(step_tables_kernel, dim3(blocks), dim3(TT), smem, (cudaStream_t)s, a, status));
     return check_launch("step_tables");
 }
+WICK_PACKED(wick_step_tables)

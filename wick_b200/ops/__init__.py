@@ -13,6 +13,7 @@ import ctypes
 import functools
 import math
 import os
+import struct
 from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -26,7 +27,7 @@ class KernelError(RuntimeError):
     pass
 
 
-_CT = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "f": ctypes.c_float}
+_CT = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "f": ctypes.c_float, "b": ctypes.c_char_p}
 
 # Argument kinds of an exported function: p pointer, i int32, l int64, f float; the
 # last pointer is always the stream.
@@ -65,6 +66,18 @@ class _Lib:
 
     def call(self, name: str, sig: str, *args, kernels: int = 1):
         rc = self.fn(name, sig)(*args)
+        if rc != 0:
+            raise KernelError(self._lib.wick_last_error().decode("utf-8", "replace"))
+        launches[0] += kernels
+
+    def call_packed(self, name: str, sig: str, *args, kernels: int = 1):
+        """:meth:`call` of an entry point that the library exports packed (csrc/packed.cuh; no pointer: 0): a call of 25 arguments in a
+        quarter of the time that ctypes takes to convert them."""
+        f = self._fns.get((name,))
+        if f is None:
+            fn = self.fn(name + "_packed", "b")
+            f = self._fns[(name,)] = (fn, struct.Struct("=" + "".join("d" if c == "f" else "q" for c in sig)).pack)
+        rc = f[0](f[1](*args))
         if rc != 0:
             raise KernelError(self._lib.wick_last_error().decode("utf-8", "replace"))
         launches[0] += kernels
@@ -628,7 +641,7 @@ def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPre
         out = torch.empty_like(q)
     else:
         _cuda("out", out, q.dtype, q.shape)
-    _shared(hd).call(f"wick_attn_shared_{_dt(q)}", "piplppppipippiiiiiifplpp", q.data_ptr(), n, kv.data_ptr(), kv_pages, out.data_ptr(),
+    _shared(hd).call_packed(f"wick_attn_shared_{_dt(q)}", "piplppppipippiiiiiifplpp", q.data_ptr(), n, kv.data_ptr(), kv_pages, out.data_ptr(),
                      cu_groups.data_ptr(), pages.data_ptr(), group_of.data_ptr(), G, batch.cu_seqlens.data_ptr(), n_seqs, batch.start.data_ptr(),
                      batch.page_table.data_ptr(), batch.table_width, n_heads, n_kv, max_pages, own_bound, batch.max_q_len, scale, scratch.data_ptr(),
                      scratch.numel(), status_tensor(q.device).data_ptr(), _stream(), kernels=kernels)
@@ -2056,7 +2069,7 @@ def step_tables(start: torch.Tensor, q_len: torch.Tensor, slots: torch.Tensor, t
     if parent is not None:
         _cuda("parent", parent, i32, (n,))
     n_slots, table_width = tables.shape
-    _core().call("wick_step_tables", "ppppipiipippipppppippp", start.data_ptr(), q_len.data_ptr(), slots.data_ptr(), _p(parent), n, tables.data_ptr(),
+    _core().call_packed("wick_step_tables", "ppppipiipippipppppippp", start.data_ptr(), q_len.data_ptr(), slots.data_ptr(), 0 if parent is None else parent.data_ptr(), n, tables.data_ptr(),
                  n_slots, table_width, free_pages.data_ptr(), free_pages.numel(), head, page_table.data_ptr(), page_table.shape[1],
                  cu_seqlens.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), slot_map.data_ptr(), n_tokens, taken,
                  status_tensor(slots.device).data_ptr(), _stream())
@@ -2083,7 +2096,7 @@ def history_clear(seen: torch.Tensor, counts: torch.Tensor, rows: torch.Tensor) 
     the prompt or the output) and the times it was generated in ``counts`` (int32 [rows, vocab]; above 0 only where the bit is set)."""
     n_rows, vocab, words = _history(seen, counts)
     _cuda("rows", rows, torch.int32)
-    _core().call("wick_history_clear", "pppiiiip", _p(seen), _p(counts), _p(rows), rows.numel(), n_rows, vocab, words, _stream())
+    _core().call_packed("wick_history_clear", "pppiiiip", seen.data_ptr(), counts.data_ptr(), rows.data_ptr(), rows.numel(), n_rows, vocab, words, _stream())
 
 
 def history_add(seen: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor, rows: torch.Tensor, generated: bool) -> None:
@@ -2092,7 +2105,7 @@ def history_add(seen: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor, 
     n_rows, vocab, words = _history(seen, counts)
     _cuda("tokens", tokens, torch.int32)
     _cuda("rows", rows, torch.int32, tokens.shape)
-    _core().call("wick_history_add", "ppppiiiiip", _p(seen), _p(counts), _p(tokens), _p(rows), tokens.numel(), n_rows, vocab, words,
+    _core().call_packed("wick_history_add", "ppppiiiiip", seen.data_ptr(), counts.data_ptr(), tokens.data_ptr(), rows.data_ptr(), tokens.numel(), n_rows, vocab, words,
                  1 if generated else 0, _stream())
 
 
@@ -2147,8 +2160,9 @@ def steer_logits(logits: torch.Tensor, rows: Optional[torch.Tensor] = None, *, s
         _need(mask_of is None, "masks and mask_of come together")
     if rows is not None:
         _cuda("rows", rows, torch.int32, (n,))
-    _core().call("wick_steer_logits", "plpliipippppppppip", logits.data_ptr(), far, out.data_ptr(), out_far, n, vocab, _p(rows), n_rows,
-                 _p(seen), _p(counts), _p(penalties), _p(cu), _p(tokens), _p(values), _p(masks), _p(mask_of), n_masks, _stream())
+    ptrs = [0 if t is None else t.data_ptr() for t in (rows, seen, counts, penalties, cu, tokens, values, masks, mask_of)]
+    _core().call_packed("wick_steer_logits", "plpliipippppppppip", logits.data_ptr(), far, out.data_ptr(), out_far, n, vocab, ptrs[0], n_rows,
+                        *ptrs[1:], n_masks, _stream())
     return out
 
 
