@@ -198,6 +198,14 @@ def _need(cond: bool, msg: str) -> None:
         raise KernelError(msg)
 
 
+def _ready(dtype: torch.dtype, *tensors: torch.Tensor) -> bool:
+    """Whether all are contiguous CUDA tensors of ``dtype`` (a third of what as many calls of :func:`_cuda`, which says what is wrong, take)."""
+    for t in tensors:
+        if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
+            return False
+    return True
+
+
 def _cuda(name: str, t: torch.Tensor, dtype=None, shape=None) -> None:
     if t.is_cuda and t.is_contiguous() and (dtype is None or t.dtype is dtype) and (shape is None or t.shape == shape):
         return
@@ -620,18 +628,20 @@ def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPre
     kv_heads, 64, d].  The result is that of the same tokens' ordinary attention over ``batch.page_table``.  scratch: float32, at
     least :func:`attention_shared_scratch` words (made here if none is given)."""
     n, n_heads, hd = q.shape
-    _cuda("q", q)
-    _cuda("kv", kv, q.dtype)
+    if not _ready(q.dtype, q, kv):
+        _cuda("q", q)
+        _cuda("kv", kv, q.dtype)
     if kv.dim() != 5 or kv.shape[1:] != (2, kv.shape[2], PAGE, hd):
         raise KernelError(f"kv must be [pages, 2, kv_heads, {PAGE}, {hd}], is {tuple(kv.shape)}")
-    kv_pages, n_kv = kv.shape[0], kv.shape[2]
+    kv_pages, _, n_kv, _, _ = kv.shape
     cu_groups, pages, group_of, max_pages, own_bound = shared
     G, n_seqs, i32 = pages.numel(), batch.n_seqs, torch.int32
     if n != batch.n_tokens:
         raise KernelError(f"q has {n} rows, the batch {batch.n_tokens} tokens")
-    _cuda("cu_groups", cu_groups, i32, (G + 1,))
-    _cuda("pages", pages, i32)
-    _cuda("group_of", group_of, i32, (n_seqs,))
+    if not (_ready(i32, cu_groups, pages, group_of) and cu_groups.shape == (G + 1,) and group_of.shape == (n_seqs,)):
+        _cuda("cu_groups", cu_groups, i32, (G + 1,))
+        _cuda("pages", pages, i32)
+        _cuda("group_of", group_of, i32, (n_seqs,))
     words, kernels = _shared_scratch(hd, q.dtype is torch.bfloat16, n, n_seqs, G, n_heads, n_kv, max_pages, own_bound, batch.max_q_len)
     if scratch is None:
         scratch = torch.empty(words, dtype=torch.float32, device=q.device)
@@ -642,9 +652,10 @@ def attention_shared(q: torch.Tensor, kv: torch.Tensor, batch, shared: SharedPre
     else:
         _cuda("out", out, q.dtype, q.shape)
     _shared(hd).call_packed(f"wick_attn_shared_{_dt(q)}", "piplppppipippiiiiiifplpp", q.data_ptr(), n, kv.data_ptr(), kv_pages, out.data_ptr(),
-                     cu_groups.data_ptr(), pages.data_ptr(), group_of.data_ptr(), G, batch.cu_seqlens.data_ptr(), n_seqs, batch.start.data_ptr(),
-                     batch.page_table.data_ptr(), batch.table_width, n_heads, n_kv, max_pages, own_bound, batch.max_q_len, scale, scratch.data_ptr(),
-                     scratch.numel(), status_tensor(q.device).data_ptr(), _stream(), kernels=kernels)
+                            cu_groups.data_ptr(), pages.data_ptr(), group_of.data_ptr(), G, batch.cu_seqlens.data_ptr(), n_seqs,
+                            batch.start.data_ptr(), batch.page_table.data_ptr(), batch.table_width, n_heads, n_kv, max_pages, own_bound,
+                            batch.max_q_len, scale, scratch.data_ptr(), scratch.numel(), status_tensor(q.device).data_ptr(), _stream(),
+                            kernels=kernels)
     return out
 
 
@@ -2050,29 +2061,33 @@ def step_tables(start: torch.Tensor, q_len: torch.Tensor, slots: torch.Tensor, t
     ``positions`` has places; places beyond the last token get position 0, sequence 0 and slot -1) positions, seq_of_token and
     slot_map (int64: page * 64 + place in the page); head_out [1], the next step's ``free_head`` (another tensor than ``free_head``)."""
     n, n_tokens, i32 = slots.numel(), positions.numel(), torch.int32
-    for nm, t in (("start", start), ("q_len", q_len), ("slots", slots), ("kv_len", kv_len)):
-        _cuda(nm, t, i32, (n,))
-    _cuda("tables", tables, i32)
-    _cuda("free_pages", free_pages, i32)
-    _cuda("free_head", free_head, i32, (1,))
-    _cuda("page_table", page_table, i32)
+    each, places = (n,), (n_tokens,)
+    if not (_ready(i32, start, q_len, slots, kv_len, tables, free_pages, free_head, page_table, cu_seqlens, positions, seq_of_token, head_out)
+            and _ready(torch.int64, slot_map) and start.shape == each and q_len.shape == each and slots.shape == each and kv_len.shape == each
+            and cu_seqlens.shape == (n + 1,) and seq_of_token.shape == places and slot_map.shape == places and free_head.shape == (1,)
+            and head_out.shape == (1,)):
+        for nm, t in (("start", start), ("q_len", q_len), ("slots", slots), ("kv_len", kv_len)):
+            _cuda(nm, t, i32, each)
+        for nm, t in (("tables", tables), ("free_pages", free_pages), ("page_table", page_table), ("positions", positions)):
+            _cuda(nm, t, i32)
+        _cuda("free_head", free_head, i32, (1,))
+        _cuda("cu_seqlens", cu_seqlens, i32, (n + 1,))
+        _cuda("seq_of_token", seq_of_token, i32, places)
+        _cuda("slot_map", slot_map, torch.int64, places)
+        _cuda("head_out", head_out, i32, (1,))
     if tables.dim() != 2 or page_table.dim() != 2 or page_table.shape[0] != n:
         raise KernelError(f"tables must be [slots, width], page_table [{n}, width]")
-    _cuda("cu_seqlens", cu_seqlens, i32, (n + 1,))
-    _cuda("positions", positions, i32)
-    _cuda("seq_of_token", seq_of_token, i32, (n_tokens,))
-    _cuda("slot_map", slot_map, torch.int64, (n_tokens,))
-    _cuda("head_out", head_out, i32, (1,))
     head, taken = free_head.data_ptr(), head_out.data_ptr()
     if head == taken:
         raise KernelError("head_out must be another tensor than free_head")
     if parent is not None:
-        _cuda("parent", parent, i32, (n,))
+        _cuda("parent", parent, i32, each)
     n_slots, table_width = tables.shape
-    _core().call_packed("wick_step_tables", "ppppipiipippipppppippp", start.data_ptr(), q_len.data_ptr(), slots.data_ptr(), 0 if parent is None else parent.data_ptr(), n, tables.data_ptr(),
-                 n_slots, table_width, free_pages.data_ptr(), free_pages.numel(), head, page_table.data_ptr(), page_table.shape[1],
-                 cu_seqlens.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), slot_map.data_ptr(), n_tokens, taken,
-                 status_tensor(slots.device).data_ptr(), _stream())
+    _core().call_packed("wick_step_tables", "ppppipiipippipppppippp", start.data_ptr(), q_len.data_ptr(), slots.data_ptr(),
+                        0 if parent is None else parent.data_ptr(), n, tables.data_ptr(), n_slots, table_width, free_pages.data_ptr(),
+                        free_pages.numel(), head, page_table.data_ptr(), page_table.shape[1], cu_seqlens.data_ptr(), kv_len.data_ptr(),
+                        positions.data_ptr(), seq_of_token.data_ptr(), slot_map.data_ptr(), n_tokens, taken, status_tensor(slots.device).data_ptr(),
+                        _stream())
 
 
 # ---------------------------------------------------------------------------
