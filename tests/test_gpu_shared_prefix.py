@@ -296,6 +296,34 @@ def test_attention_shared_in_a_graph_follows_the_description(ops):
     check(out, case)
 
 
+def test_attention_shared_in_a_graph_behind_a_long_prefix(ops):
+    """The same where the shared keys have a kernel of their own; twice in the graph, each beginning before the one before it has ended."""
+    case = Case([(130, [(10, 1), (70, 1), (600, 1)] * 3), (3, [(5, 1)])], 32, 8, 128, BF16, seed=6, more_width=2)
+    b = case.batch()
+    shared = ops.SharedPrefix.of(case.sizes, case.shared, case.kv_lens, "cuda")._replace(max_pages=140, own_bound=900)
+    q, kv = case.q.cuda(), case.kv.cuda()
+    scratch = torch.empty(ops.attention_shared_scratch(shared, b, 32, 8, 128, BF16), dtype=F32, device="cuda")
+    outs = [torch.empty_like(q), torch.empty_like(q)]
+    ops.attention_shared(q, kv, b, shared, case.scale, scratch, outs[0])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for out in outs:
+            assert kernels_of(ops, lambda: ops.attention_shared(q, kv, b, shared, case.scale, scratch, out)) == 3      # noqa: B023
+    for out in outs:
+        out.zero_()
+    g.replay()
+    for out in outs:
+        check(out, case)
+    # the group shares less now (its sequences hold the rest as their own), a sequence has become shorter
+    shared.pages.copy_(ints([127, 3]))
+    case.starts[1] -= 60
+    b.start.copy_(ints(case.starts))
+    g.replay()
+    for out in outs:
+        check(out, case)
+    ops.check_status()
+
+
 def test_attention_shared_reports_a_sequence_that_is_shorter_than_its_group(ops):
     case = Case([(2, [(10, 1), (70, 1)])], 4, 2, 64, BF16, seed=1)
     b = case.batch()
