@@ -5,6 +5,7 @@
 // the draw exactly as the reference does.  One block of 1024 threads per row;
 // every reduction and scan has a fixed order, so a row's result depends on that
 // row alone.
+#include <float.h>
 #include <limits.h>
 
 #include "common.cuh"
@@ -76,18 +77,23 @@ __device__ __forceinline__ float block_scan(float v, float* warp_tot, float* tot
     return v;
 }
 
+// The weight of a logit beside the row's maximum.  Logits equal to it weigh 1, whatever they are: one of +inf takes the draw, several share it.
+__device__ __forceinline__ float weight_of(float x, float m, float inv_t) { return x == m ? 1.f : expf((x - m) * inv_t); }
+
+// A token without weight (a logit of -inf, or one so far below the maximum) is never drawn: not where the sums' rounding leaves a thread's walk
+// short of the target (then its last token with weight is), not by the uniform number 0 (the target is then the smallest there is).
 __global__ void __launch_bounds__(ST)
 sample_temperature_kernel(const float* __restrict__ logits, const float* __restrict__ uniforms,
                           int* __restrict__ out, int vocab, float inv_t) {
     __shared__ float red[40];
     __shared__ float warp_tot[32];
-    __shared__ int chosen;
+    __shared__ int chosen, behind, last;
     const float* x = logits + (int64_t)blockIdx.x * vocab;
     float m = -INFINITY;
     for (int i = threadIdx.x; i < vocab; i += ST) m = fmaxf(m, x[i]);
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-    if (threadIdx.x == 0) chosen = INT_MAX;
+    if (threadIdx.x == 0) chosen = behind = INT_MAX, last = -1;
     __syncthreads();
     m = red[0];
     for (int w = 1; w < 32; ++w) m = fmaxf(m, red[w]);
@@ -95,22 +101,32 @@ sample_temperature_kernel(const float* __restrict__ logits, const float* __restr
     const int chunk = (vocab + ST - 1) / ST;
     const int lo = min(threadIdx.x * chunk, vocab), hi = min(lo + chunk, vocab);
     float mine = 0.f;
-    for (int i = lo; i < hi; ++i) mine += expf((x[i] - m) * inv_t);
+    int first = INT_MAX, heavy = -1;               // the first and the last of this thread's tokens with weight
+    for (int i = lo; i < hi; ++i) {
+        const float w = weight_of(x[i], m, inv_t);
+        mine += w;
+        if (w > 0.f) first = min(first, i), heavy = i;
+    }
     float total;
     const float incl = block_scan(mine, warp_tot, &total);
     const float excl = incl - mine;
-    const float target = uniforms[blockIdx.x] * total;
-    if ((excl < target || threadIdx.x == 0) && incl >= target && hi > lo) {
+    float target = uniforms[blockIdx.x] * total;
+    if (target < FLT_MIN) target = FLT_MIN;        // (a sum that is no number stays one)
+    if (excl < target && incl >= target && heavy >= 0) {
         float run = excl;
-        int pick = hi - 1;
-        for (int i = lo; i < hi; ++i) {
-            run += expf((x[i] - m) * inv_t);
-            if (run >= target) { pick = i; break; }
+        for (int i = lo; i <= heavy; ++i) {
+            const float w = weight_of(x[i], m, inv_t);
+            run += w;
+            if (w > 0.f && run >= target) { heavy = i; break; }
         }
-        atomicMin(&chosen, pick);
+        atomicMin(&chosen, heavy);
     }
+    // Where two threads' rounded sums leave a gap at their border and the target lies in it, the token behind it is taken; where it lies behind
+    // the last sum, the last with weight.
+    const int after = __reduce_min_sync(0xffffffffu, incl >= target ? first : INT_MAX), of_warp = __reduce_max_sync(0xffffffffu, heavy);
+    if ((threadIdx.x & 31) == 0) atomicMin(&behind, after), atomicMax(&last, of_warp);
     __syncthreads();
-    if (threadIdx.x == 0) out[blockIdx.x] = chosen == INT_MAX ? vocab - 1 : chosen;
+    if (threadIdx.x == 0) out[blockIdx.x] = chosen != INT_MAX ? chosen : behind != INT_MAX ? behind : last >= 0 && total == total ? last : vocab - 1;
 }
 
 // Each (row, token) pair once: logit > 0 ? logit / penalty : logit * penalty
@@ -222,6 +238,8 @@ top_k_kernel(const float* __restrict__ logits, float* __restrict__ vals, int* __
 // r = u * (sum of what is left) walked down the candidates (wick src/sampler.rs:95-125).
 // One thread per row does the sums one after the other in float32, as the reference's
 // iterator sums do (k <= 1024 on the usual path; nothing here is worth more threads).
+// A candidate of -inf (a token that the caller has ruled out) is never drawn: what the sums' rounding leaves over at the walk's end goes to the
+// last one kept that is larger.  Candidates equal to the largest weigh 1, so that those of +inf share the draw.
 // probs: scratch [rows, k].
 __global__ void pick_sorted_kernel(const float* __restrict__ vals, const int* __restrict__ idxs, const float* __restrict__ uniforms,
                                    float* __restrict__ probs, int* __restrict__ out, int rows, int k, float temperature,
@@ -238,7 +256,7 @@ __global__ void pick_sorted_kernel(const float* __restrict__ vals, const int* __
     const float top = v[0];
     float total = 0.f;
     for (int i = 0; i < k; ++i) {
-        p[i] = expf(__fdiv_rn(__fsub_rn(v[i], top), temperature));
+        p[i] = v[i] == top ? 1.f : expf(__fdiv_rn(__fsub_rn(v[i], top), temperature));
         total = __fadd_rn(total, p[i]);
     }
     for (int i = 0; i < k; ++i) p[i] = __fdiv_rn(p[i], total);
@@ -258,12 +276,14 @@ __global__ void pick_sorted_kernel(const float* __restrict__ vals, const int* __
     float tot = 0.f;
     for (int i = 0; i < keep; ++i) tot = __fadd_rn(tot, p[i]);
     float r = __fmul_rn(uniforms[row], tot);
-    int pick = ix[keep - 1];
+    int pick = 0;
     for (int i = 0; i < keep; ++i) {
+        if (i > 0 && v[i] == -INFINITY) break;     // (sorted: nothing but such behind it)
+        pick = i;
         r = __fsub_rn(r, p[i]);
-        if (r <= 0.f) { pick = ix[i]; break; }
+        if (r <= 0.f) break;
     }
-    out[row] = pick;
+    out[row] = ix[pick];
 }
 
 }  // namespace wick

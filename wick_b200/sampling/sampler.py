@@ -78,10 +78,14 @@ class Rng:
 
 def pick_from_sorted(vals: np.ndarray, idx: np.ndarray, cfg: SamplerConfig, rng: Rng) -> int:
     """vals: float32 candidates sorted descending, idx their token ids.  Steps
-    sampler.rs:95-125 in float32."""
+    sampler.rs:95-125 in float32.  A candidate of -inf, which no logit of a model is but one that the caller has
+    ruled out, is never drawn; candidates equal to the largest weigh 1, so that those of +inf share the draw."""
     f = np.float32
     t = f(cfg.temperature)
-    probs = np.exp(((vals.astype(f) - vals[0]) / t).astype(f)).astype(f)
+    vals = vals.astype(f)
+    less = vals != vals[0]
+    probs = np.ones(len(vals), dtype=f)
+    probs[less] = np.exp(((vals[less] - vals[0]) / t).astype(f))
     total = f(0)
     for p in probs:                      # sequential float32 sum, as the reference's iterator sum
         total = f(total + p)
@@ -102,11 +106,15 @@ def pick_from_sorted(vals: np.ndarray, idx: np.ndarray, cfg: SamplerConfig, rng:
     for p in probs[:keep]:
         tot = f(tot + p)
     r = f(f(rng.next_f32()) * tot)
+    pick = 0
     for i in range(keep):
+        if i > 0 and vals[i] == -np.inf:
+            break
+        pick = i
         r = f(r - probs[i])
         if r <= 0:
-            return int(idx[i])
-    return int(idx[keep - 1])
+            break
+    return int(idx[pick])
 
 
 def rng_state(seed: int) -> List[int]:
