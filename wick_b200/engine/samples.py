@@ -50,6 +50,7 @@ class SampleRun(DeviceRun):
         self.lent: List[int] = []
         self.slots: List[int] = []
         self.parents: List[int] = []
+        self.mark = object()         # of this batch, on the captured step that holds its description
 
     def start(self, prompts: Sequence[Sequence[int]], numbers: Sequence[Sequence[int]], limits: Sequence[int]) -> None:      # type: ignore[override]
         """numbers[i]: which continuations of prompt i (their generators are seeded by them); limits[i]: the tokens each may have."""
@@ -108,7 +109,7 @@ class SampleRun(DeviceRun):
         rec = np.zeros((R, ops.SEQ_STATE_WORDS), dtype=np.int32)
         rec[:, ops.SEQ_LIMIT], rec[:, ops.SEQ_ROW] = self.limit, np.arange(R)
         ops.seq_state_set(e.seq_state, slots, up(rec))
-        self.graph, self.composition = None, None
+        self.graph = None
         first = logits[:P].repeat_interleave(up([len(k) for k in numbers]), 0)
         with ops.stream_scope():
             self._sample_and_advance(first, slots, up(self.length), R, rows)
@@ -117,7 +118,8 @@ class SampleRun(DeviceRun):
     def launch(self, live: Sequence[int]) -> None:                   # type: ignore[override]
         e = self.engine
         B = len(live)
-        if self.composition != tuple(live):
+        # (The step is the engine's: another batch may have written its own description there since.)
+        if self.graph is None or self.graph.composition != (self.mark, tuple(live)):
             self._compose(live)
         g, b = self.graph, self.graph.batch
         with ops.stream_scope():
@@ -152,7 +154,7 @@ class SampleRun(DeviceRun):
             at += dst.numel()
         self.uploads += 1
         self.h2d_bytes += flat.numel() * 4
-        self.composition = tuple(live)
+        g.composition = (self.mark, tuple(live))
 
     def close(self) -> None:
         """Give back every slot and page."""
