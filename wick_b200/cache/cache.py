@@ -68,7 +68,10 @@ class Storage:
     including the padding page 0, slots including the padding slot 0), the element type
     and the device; it allocates in :meth:`allocate`, hands one entry's part of itself to
     a mixer in :meth:`view`, prepares a slot for a new sequence in :meth:`open_seq`, and
-    says how many bytes a step reads from it in :meth:`read_bytes`."""
+    says how many bytes a step reads from it in :meth:`read_bytes`.  One whose sequences can be
+    forked (several continuations of one prompt) says in :meth:`copy_pages` and
+    :meth:`copy_slots` how; there is no default, since what is kept per page and what per slot
+    only the kind knows."""
 
     kind = ""
 
@@ -91,10 +94,16 @@ class Storage:
         """A sequence starts in ``slot``."""
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        """Pages ``dst`` become copies of pages ``src`` (int64 on the device).  A kind without pages copies nothing."""
+        """Pages ``dst`` become copies of pages ``src`` (int64 on the device); a kind without pages has nothing to do here."""
+        raise NotImplementedError(f"{type(self).__name__} ({self.need.kind}) does not say how its pages are copied")
 
     def copy_slots(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        """The records of slots ``dst`` become copies of those of ``src`` (int64 on the device).  A kind without records copies nothing."""
+        """The records of slots ``dst`` become copies of those of ``src`` (int64 on the device); a kind without records has nothing to do here."""
+        raise NotImplementedError(f"{type(self).__name__} ({self.need.kind}) does not say how its records are copied")
+
+    def can_copy(self) -> bool:
+        """Whether the kind says how its pages and its records are copied."""
+        return type(self).copy_pages is not Storage.copy_pages and type(self).copy_slots is not Storage.copy_slots
 
     def read_bytes(self, cached_tokens: int, n_seqs: int) -> int:
         """Bytes a decode step reads from this group for ``n_seqs`` sequences that hold
@@ -106,11 +115,14 @@ class Storage:
 
 
 class _Paged(Storage):
-    """Storage whose second dimension is the page."""
+    """Storage whose second dimension is the page, and nothing else per sequence."""
 
     def copy_pages(self, src, dst):
         for entry in self.tensor:                                    # (one entry's pages at a time: the copy in between stays small)
             entry[dst] = entry[src]
+
+    def copy_slots(self, src, dst):
+        pass
 
 
 class PagedKV(_Paged):
@@ -201,6 +213,9 @@ class StateRecords(Storage):
     def open_seq(self, slot):
         if self.tensor is not None:
             self.tensor[:, slot].zero_()
+
+    def copy_pages(self, src, dst):
+        pass
 
     def copy_slots(self, src, dst):
         for entry in self.tensor:
@@ -383,6 +398,10 @@ class Cache:
                 raise PoolError(f"page {p} is given back but was not lent")
             self.lent.remove(p)
             self.pages.free(p)
+
+    def cannot_copy(self) -> List[str]:
+        """The kinds of storage in use whose sequences cannot be forked (see :meth:`Storage.can_copy`)."""
+        return sorted({g.need.kind for g in self.groups if not g.store.can_copy()})
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Copy the contents of pages ``src`` to pages ``dst`` (int64 on the device) in every group."""

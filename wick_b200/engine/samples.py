@@ -169,7 +169,7 @@ def sample_many(engine, prompts: Sequence[Sequence[int]], n: int, opts: Optional
     """``n`` continuations of every prompt, each prompt's in order.  Continuation k of a prompt draws with the generator of seed
     ``opts.sampler.seed + k``.  rules: for all prompts, or one for each (default: ``opts.rules``).  As many prompts as the batch limit
     (counted in continuations), the cache's slots and its free pages allow are decoded together; a prompt with more continuations than the
-    batch limit is run again for the rest of them."""
+    batch limit is run again for the rest of them.  A cache with a kind of storage that cannot be copied is refused."""
     opts = opts or GenOptions()
     if n < 1:
         raise ValueError(f"{n} continuations (at least 1)")
@@ -179,6 +179,9 @@ def sample_many(engine, prompts: Sequence[Sequence[int]], n: int, opts: Optional
         raise ValueError("one set of rules for all prompts, or one for each")
     stops = stop_set(engine, opts)
     cache = engine.cache
+    if cache.cannot_copy():
+        raise RuntimeError("the cache cannot be forked: storage of kind " + ", ".join(cache.cannot_copy()) + " does not say how its pages and records "
+                           "are copied (Storage.copy_pages, Storage.copy_slots)")
     context = min(opts.context, cache.max_position or opts.context)
     results: List[List[Optional[GenResult]]] = [[None] * n for _ in prompts]
     waiting: List[Tuple[int, List[int], int]] = []                 # prompt, continuations, tokens each
