@@ -7,10 +7,15 @@
 //                          0 (the reserved page)                  beyond, and beyond the list's end, which is reported
 // and for its token i, at position p = start_b + i: slot = page of column p / 64, times 64, plus p % 64.
 //
-// One launch: every block makes the sums over all sequences for itself (a few thousand numbers from the L2 cache; a second
-// launch, or blocks that wait for one another, would cost more than that), then a warp fills a sequence's row, a thread a
-// token.  Record 0 is the padding's: it gets no pages.
-// Bound by that chain: 48 sequences of a token each 3.5 us, 700 with 300 forks and up to 400 tokens each (5 MB written) 9.1.
+// Forks read what their parents held BEFORE the call, whatever becomes of the parents in it (two sequences may change places): a call with
+// parents first makes the rows from the tables as they are, and writes them into the tables in a second launch.  A fork begins on a page of its
+// own (start_b a multiple of 64): in the middle of one, it and its parent would write to the same places.
+//
+// Every block makes the sums over all sequences for itself (a few thousand numbers from the L2 cache; a launch for them, or blocks that wait
+// for one another, would cost more than that), then a warp fills a sequence's row, a thread a token.  Record 0 is the padding's: it gets no
+// pages.
+// Bound by that chain, and in a large call by its rows, a warp each, whose reads and writes wait for one another: 48 sequences of a token each
+// 3.5 us, 700 with 300 forks and up to 400 tokens each (5 MB written) 9.1.
 #include "common.cuh"
 #include "packed.cuh"
 
@@ -26,27 +31,47 @@ struct Tables {
     int *page_table, *cu_seqlens, *kv_len, *positions, *seq_of_token, *head_out;
     int64_t* slot_map;
     int n_seqs, n_slots, table_width, width, n_free, n_tokens;
+
+    // The record of sequence b; -1 (reported, no pages): outside the tables, a parent outside them, a fork that begins inside a page.
+    __device__ __forceinline__ int slot_of(int b) const {
+        const int s = slots[b], p = parent ? parent[b] : -1;
+        return s != 0 && (s < 0 || s >= n_slots || p >= n_slots || (p >= 0 && p != s && start[b] % kPage != 0)) ? -1 : s;
+    }
+    __device__ __forceinline__ int source_of(int b, int slot) const {
+        const int p = parent ? parent[b] : -1;
+        return p >= 0 && p < n_slots ? p : max(slot, 0);
+    }
 };
+
+// The rows that step_tables_kernel has made, into the tables: a warp a sequence.
+__global__ void __launch_bounds__(TT) store_tables_kernel(const Tables a) {
+    pdl_wait();                                    // (no early start of the next kernel, as below)
+    const int lane = threadIdx.x & 31;
+    for (int b = ((int)blockIdx.x * TT + (int)threadIdx.x) >> 5; b < a.n_seqs; b += (int)gridDim.x * (TT / 32)) {
+        const int slot = a.slot_of(b), start = max(a.start[b], 0), held = (start + kPage - 1) / kPage;
+        if (slot <= 0) continue;
+        const int from = a.source_of(b, slot) != slot ? 0 : held, to = min((start + max(a.q_len[b], 0) + kPage - 1) / kPage, min(a.width, a.table_width));
+        const int* row = a.page_table + (int64_t)b * a.width;
+        for (int j = from + lane; j < to; j += 32) a.tables[(int64_t)slot * a.table_width + j] = row[j];
+    }
+}
 
 __global__ void __launch_bounds__(TT) step_tables_kernel(const Tables a, int* status) {
     extern __shared__ int sums[];
     int* cum_q = sums;                             // tokens of the sequences before each one
     int* cum_n = sums + a.n_seqs + 1;              // pages that they need
     __shared__ int warp_q[TT / 32], warp_n[TT / 32];
-    pdl_wait();                                    // (no early start of the next kernel: kernels of a step read these fields before they wait)
+    if (a.parent) pdl_trigger();                   // (of store_tables_kernel, which waits before all else)
+    pdl_wait();                                    // (no early start of another kernel: kernels of a step read these fields before they wait)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_seqs;
     auto held_of = [&](int b) { return (max(a.start[b], 0) + kPage - 1) / kPage; };
-    auto slot_of = [&](int b) {                    // -1: outside the table, reported below
-        const int s = a.slots[b];
-        return s >= 0 && s < a.n_slots ? s : -1;
-    };
     int base_q = 0, base_n = 0;
     for (int s0 = 0; s0 < B; s0 += TT) {
         const int b = s0 + tid;
         int q = 0, n = 0;
         if (b < B) {
             q = max(a.q_len[b], 0);
-            if (slot_of(b) > 0) n = (max(a.start[b], 0) + q + kPage - 1) / kPage - held_of(b);
+            if (a.slot_of(b) > 0) n = (max(a.start[b], 0) + q + kPage - 1) / kPage - held_of(b);
         }
         int uq = q, un = n;
 #pragma unroll
@@ -77,10 +102,6 @@ __global__ void __launch_bounds__(TT) step_tables_kernel(const Tables a, int* st
         const int at = first + j - held;
         return at >= 0 && at < a.n_free ? a.free_pages[at] : 0;
     };
-    auto source_of = [&](int b, int slot) {
-        const int p = a.parent ? a.parent[b] : -1;
-        return p >= 0 && p < a.n_slots ? p : max(slot, 0);
-    };
 
     const int gt = (int)blockIdx.x * TT + tid, step = (int)gridDim.x * TT;
     for (int b = gt; b <= B; b += step) {
@@ -90,15 +111,15 @@ __global__ void __launch_bounds__(TT) step_tables_kernel(const Tables a, int* st
     if (gt == 0) {
         *a.head_out = head + cum_n[B];
         if ((head < 0 || head + cum_n[B] > a.n_free) && cum_n[B] > 0) atomicCAS(status, 0, 12);
+        if (cum_q[B] > a.n_tokens) atomicCAS(status, 0, 14);
     }
     for (int b = gt >> 5; b < B; b += step >> 5) {
-        const int slot = slot_of(b), held = held_of(b), total = held + cum_n[b + 1] - cum_n[b], first = head + cum_n[b], src = source_of(b, slot);
+        const int slot = a.slot_of(b), held = held_of(b), total = held + cum_n[b + 1] - cum_n[b], first = head + cum_n[b], src = a.source_of(b, slot);
         if (lane == 0 && (slot < 0 || (slot > 0 && total > min(a.width, a.table_width)))) atomicCAS(status, 0, 13);
-        const bool fork = src != slot;
         for (int j = lane; j < a.width; j += 32) {
             const int page = page_at(src, slot, held, total, first, j);
             a.page_table[(int64_t)b * a.width + j] = page;
-            if (slot > 0 && j < total && j < a.table_width && (fork || j >= held)) a.tables[(int64_t)slot * a.table_width + j] = page;
+            if (!a.parent && slot > 0 && j >= held && j < total && j < a.table_width) a.tables[(int64_t)slot * a.table_width + j] = page;
         }
     }
     for (int t = gt; t < a.n_tokens; t += step) {
@@ -113,8 +134,8 @@ __global__ void __launch_bounds__(TT) step_tables_kernel(const Tables a, int* st
             }
             seq = lo;
             pos = max(a.start[seq], 0) + t - cum_q[seq];
-            const int slot = slot_of(seq), held = held_of(seq), total = held + cum_n[seq + 1] - cum_n[seq];
-            at = (int64_t)page_at(source_of(seq, slot), slot, held, total, head + cum_n[seq], pos / kPage) * kPage + pos % kPage;
+            const int slot = a.slot_of(seq), held = held_of(seq), total = held + cum_n[seq + 1] - cum_n[seq];
+            at = (int64_t)page_at(a.source_of(seq, slot), slot, held, total, head + cum_n[seq], pos / kPage) * kPage + pos % kPage;
         }
         a.positions[t] = pos;
         a.seq_of_token[t] = seq;
@@ -126,7 +147,8 @@ __global__ void __launch_bounds__(TT) step_tables_kernel(const Tables a, int* st
 
 using namespace wick;
 
-// Arrays as in struct Tables.  status: 12 the list of free pages is too short, 13 a record or a length outside the tables.
+// Arrays as in struct Tables.  status: 12 the list of free pages is too short, 13 a record, a parent or a length outside the tables, or a fork
+// that begins inside a page, 14 more tokens than places.  Two launches with parents, one without.
 WICK_API int wick_step_tables(const int* start, const int* q_len, const int* slots, const int* parent, int n_seqs, int* tables, int n_slots,
                               int table_width, const int* free_pages, int n_free, const int* free_head, int* page_table, int width,
                               int* cu_seqlens, int* kv_len, int* positions, int* seq_of_token, void* slot_map, int n_tokens, int* head_out,
@@ -143,6 +165,9 @@ WICK_API int wick_step_tables(const int* start, const int* q_len, const int* slo
         raised = true;
     }
     WICK_CUDA(launch(step_tables_kernel, dim3(blocks), dim3(TT), smem, (cudaStream_t)s, a, status));
-    return check_launch("step_tables");
+    if (int e = check_launch("step_tables")) return e;
+    if (!parent) return 0;
+    WICK_CUDA(launch(store_tables_kernel, dim3(ceil_div(n_seqs, TT / 32)), dim3(TT), 0, (cudaStream_t)s, a));
+    return check_launch("store_tables");
 }
 WICK_PACKED(wick_step_tables)

@@ -143,7 +143,9 @@ _STATUS_TEXT = {1: "gemm_tc gave up waiting for a free shared-memory stage", 2: 
                 8: "attention decode (tensor cores) gave up waiting for its TMA copies",
                 10: "attention decode was given a length or a page outside its page table or its cache",
                 11: "attention over a shared prefix was given a sequence that does not fit its group's pages or its page table",
-                12: "step_tables ran out of free pages", 13: "step_tables was given a record or a length outside its tables",
+                12: "step_tables ran out of free pages",
+                13: "step_tables was given a record, a parent or a length outside its tables, or a fork that begins inside a page",
+                14: "step_tables was given more tokens than places for them",
                 99: "the test kernel gave up waiting for nothing (nobody arrives on its barrier)"}
 
 
@@ -2053,9 +2055,10 @@ def step_tables(start: torch.Tensor, q_len: torch.Tensor, slots: torch.Tensor, t
     Sequence b (record ``slots[b]``) has cached ``start[b]`` positions and brings ``q_len[b]`` new tokens (0: none).  The pages it holds
     are in ``tables[slots[b]]`` (int32 [slots, width], in position order); what it needs beyond is handed out from ``free_pages``,
     beginning at ``free_head[0]``, sequence after sequence, and written to ``tables``.  A sequence with ``parent[b] >= 0`` starts from
-    the pages of that record instead of its own (the pages that hold its ``start[b]`` positions; a parent holds at least those).
-    Record 0 is the padding's: it gets no pages.  A list that is too short gives the reserved page 0 and shows in
-    :func:`check_status`.
+    the pages that this record held before the call instead of its own (those of its ``start[b]`` positions, a multiple of 64: what it writes is
+    on pages of its own; a parent holds at least those).  A parent may be forked, or grow, in the same call.
+    Record 0 is the padding's: it gets no pages.  A list that is too short gives the reserved page 0, a sequence whose record or parent is
+    outside the tables, or whose fork begins inside a page, gets no pages; these, and more tokens than places, show in :func:`check_status`.
 
     Written: page_table [n, any width], 0 behind a sequence's last page; cu_seqlens [n + 1]; kv_len [n]; for each of the tokens (as many as
     ``positions`` has places; places beyond the last token get position 0, sequence 0 and slot -1) positions, seq_of_token and
@@ -2087,7 +2090,7 @@ def step_tables(start: torch.Tensor, q_len: torch.Tensor, slots: torch.Tensor, t
                         0 if parent is None else parent.data_ptr(), n, tables.data_ptr(), n_slots, table_width, free_pages.data_ptr(),
                         free_pages.numel(), head, page_table.data_ptr(), page_table.shape[1], cu_seqlens.data_ptr(), kv_len.data_ptr(),
                         positions.data_ptr(), seq_of_token.data_ptr(), slot_map.data_ptr(), n_tokens, taken, status_tensor(slots.device).data_ptr(),
-                        _stream())
+                        _stream(), kernels=1 if parent is None else 2)
 
 
 # ---------------------------------------------------------------------------
