@@ -476,7 +476,7 @@ attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, 
     const OwnParts parts{G, R, groups};
     Walk walk(parts, gridDim.x, nullptr);           // (the description may be read before the wait)
     pdl_wait();
-    q = fresh(q);
+    q = fresh(q), kv = fresh(kv);                   // (the step's own keys and values have just been appended)
     Segment s;
     while (walk.segment(s)) {                       // (every warp walks the same way)
         __syncthreads();                            // (the rows and the work of the segment before)

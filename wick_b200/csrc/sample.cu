@@ -248,6 +248,7 @@ __global__ void pick_sorted_kernel(const float* __restrict__ vals, const int* __
     pdl_wait();
     vals = fresh(vals);
     idxs = fresh(idxs);
+    uniforms = fresh(uniforms);
     const int row = blockIdx.x * blockDim.x + threadIdx.x;
     if (row >= rows) return;
     const float* v = vals + (int64_t)row * k;

@@ -135,6 +135,7 @@ __global__ void penalty_seen_kernel(float* logits, const uint8_t* __restrict__ s
     pdl_wait();
     logits = fresh(logits);
     state = fresh(state);
+    seen = fresh(seen);
     const int row = blockIdx.y;
     const int slot = slots[row];
     if (slot == 0) return;

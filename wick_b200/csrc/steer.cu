@@ -22,9 +22,10 @@ constexpr int HT = 256;
 
 // Blocks (chunk of words, row of the list).
 __global__ void __launch_bounds__(HT)
-history_clear_kernel(unsigned* __restrict__ seen, int* __restrict__ counts, const int* __restrict__ rows, int n_rows, int vocab, int words) {
+history_clear_kernel(unsigned* seen, int* counts, const int* rows, int n_rows, int vocab, int words) {
     pdl_trigger();
     pdl_wait();
+    seen = fresh(seen), counts = fresh(counts), rows = fresh(rows);
     const int r = rows[blockIdx.y];
     if (r < 0 || r >= n_rows) return;
     for (int i = blockIdx.x * HT + threadIdx.x; i < words; i += gridDim.x * HT) {
@@ -40,10 +41,10 @@ history_clear_kernel(unsigned* __restrict__ seen, int* __restrict__ counts, cons
 }
 
 __global__ void __launch_bounds__(HT)
-history_add_kernel(unsigned* seen, int* __restrict__ counts, const int* __restrict__ tokens, const int* __restrict__ rows, int n, int n_rows,
-                   int vocab, int words, int generated) {
+history_add_kernel(unsigned* seen, int* counts, const int* tokens, const int* rows, int n, int n_rows, int vocab, int words, int generated) {
     pdl_trigger();
     pdl_wait();
+    tokens = fresh(tokens), rows = fresh(rows);    // (the sampler before this kernel has just written the tokens)
     const int i = blockIdx.x * HT + threadIdx.x;
     if (i >= n) return;
     const int r = rows[i], v = tokens[i];
