@@ -168,8 +168,8 @@ def sample_many(engine, prompts: Sequence[Sequence[int]], n: int, opts: Optional
                 rules: Optional[Sequence[Optional[LogitRules]] | LogitRules] = None) -> List[List[GenResult]]:
     """``n`` continuations of every prompt, each prompt's in order.  Continuation k of a prompt draws with the generator of seed
     ``opts.sampler.seed + k``.  rules: for all prompts, or one for each (default: ``opts.rules``).  As many prompts as the batch limit
-    (counted in continuations), the cache's slots and its free pages allow are decoded together; a prompt with more continuations than the
-    batch limit is run again for the rest of them.  A cache with a kind of storage that cannot be copied is refused."""
+    (counted in continuations, 8,192 at the most), 1,023 of them, the cache's slots and its free pages allow are decoded together; a prompt with
+    more continuations than the batch limit is run again for the rest of them.  A cache with a kind of storage that cannot be copied is refused."""
     opts = opts or GenOptions()
     if n < 1:
         raise ValueError(f"{n} continuations (at least 1)")
@@ -183,6 +183,9 @@ def sample_many(engine, prompts: Sequence[Sequence[int]], n: int, opts: Optional
         raise RuntimeError("the cache cannot be forked: storage of kind " + ", ".join(cache.cannot_copy()) + " does not say how its pages and records "
                            "are copied (Storage.copy_pages, Storage.copy_slots)")
     context = min(opts.context, cache.max_position or opts.context)
+    most = min(opts.max_batch, ops.MAX_TABLE_SEQS)                  # continuations of a batch
+    if most < 1:
+        raise ValueError(f"a batch of {opts.max_batch} (at least 1)")
     results: List[List[Optional[GenResult]]] = [[None] * n for _ in prompts]
     waiting: List[Tuple[int, List[int], int]] = []                 # prompt, continuations, tokens each
     for i, p in enumerate(prompts):
@@ -194,12 +197,12 @@ def sample_many(engine, prompts: Sequence[Sequence[int]], n: int, opts: Optional
         if limit == 0:
             results[i] = [GenResult([], len(p), "length") for _ in range(n)]
             continue
-        waiting += [(i, list(range(k, min(n, k + opts.max_batch))), limit) for k in range(0, n, opts.max_batch)]
+        waiting += [(i, list(range(k, min(n, k + most))), limit) for k in range(0, n, most)]
     while waiting:
         chosen, rows, pages, slots = 0, 0, 0, 0
-        for i, ks, limit in waiting:
+        for i, ks, limit in waiting[:ops.MAX_SHARED_GROUPS - 1]:     # (one group is the padding's)
             rows, slots, pages = rows + len(ks), slots + 1 + len(ks), pages + pages_of_batch(len(prompts[i]), limit, len(ks))
-            if rows > max(opts.max_batch, len(ks)) or slots > cache.slots.n_free or pages > cache.pages.n_free:
+            if rows > most or slots > cache.slots.n_free or pages > cache.pages.n_free:
                 break
             chosen += 1
         if chosen == 0:

@@ -565,6 +565,8 @@ def attention_decode_parts_fused(qkv: torch.Tensor, n_heads: int, n_kv: int, hea
 # ---------------------------------------------------------------------------
 # Attention where groups of a step's sequences share their first pages (csrc/attn_shared.cuh, attn_shared.cu).
 SHARED_SOURCES = ["attn_shared.cu", "attn_shared_tc.cu", "attn_shared_own.cu"]
+MAX_SHARED_GROUPS = 1024      # groups of a step (csrc/attn_shared.cuh)
+MAX_TABLE_SEQS = 8192         # sequences of a step whose tables are made on the device (csrc/tables.cu)
 
 
 def _shared(head_dim: int) -> _Lib:
