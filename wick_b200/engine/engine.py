@@ -100,6 +100,7 @@ class _DecodeGraph:
 PROMPT_GRAPH_TOKENS = 512     # prompt steps of up to this many tokens are captured, padded to a multiple of 64
 PROMPT_GRAPH_SEQS = 64        # ... and of up to this many sequences (padded to a power of two or three quarters of one)
 PROMPT_GRAPH_COUNT = 24       # captured prompt steps an engine keeps (each holds its output rows); further shapes are launched
+SHARED_GRAPH_COUNT = 24       # captured steps of continuations an engine keeps (each holds its output rows); the one used longest ago makes room
 
 
 class _PromptGraph:
@@ -136,7 +137,8 @@ class Engine:
             use_graphs = os.environ.get("WICK_B200_NO_GRAPHS", "") == ""
         self.use_graphs = use_graphs
         self._graphs: Dict[Tuple[int, int], _DecodeGraph] = {}
-        self._shared_graphs: Dict[Tuple[int, int, int, int, int], _DecodeGraph] = {}
+        self._shared_graphs: Dict[Tuple[int, int, int, int, int], _DecodeGraph] = {}      # (in the order of their last use)
+        self._shared_pool = None
         # Short prompt steps are bound by the host's time per launch: they are captured too,
         # where every part of the model allows it (WICK_B200_NO_PROMPT_GRAPHS=1: never).
         self.prompt_graphs = (os.environ.get("WICK_B200_NO_PROMPT_GRAPHS", "") == "") and model.prompt_capturable()
@@ -404,16 +406,23 @@ class Engine:
             self._capture(g)
         return g
 
-    def shared_graph(self, n_seqs: int, width: int, n_groups: int, max_pages: int, own_bound: int) -> _DecodeGraph:
-        """The captured decode step for ``n_seqs`` sequences (padded, see :meth:`_bucket`) in ``n_groups`` groups that share up to
-        ``max_pages`` pages and hold up to ``own_bound`` positions behind them, with page tables of ``width`` columns; captured on
-        first use.  Beside the step's description it has ``batch.shared`` (whose tensors say who shares what, see
-        :class:`~wick_b200.ops.SharedPrefix`), ``rows`` (int32, of a sampler's rows), ``ones`` and ``slot_map`` for
-        :func:`~wick_b200.ops.step_tables`.  Graphs switched off: the same, not captured."""
+    def shared_graph(self, n_seqs: int, width: int, n_groups: int, max_pages: int, own_bound: int, prefer_captured: bool = False) -> _DecodeGraph:
+        """The captured decode step for ``n_seqs`` sequences (padded, see :meth:`_bucket`) in up to ``n_groups`` groups (a power of two) that share
+        up to ``max_pages`` pages and hold up to ``own_bound`` positions behind them, with page tables of ``width`` columns; captured on
+        first use, kept while it is among the :data:`SHARED_GRAPH_COUNT` used last.  Beside the step's description it has ``batch.shared``
+        (whose tensors say who shares what, see :class:`~wick_b200.ops.SharedPrefix`), ``rows`` (int32, of a sampler's rows), ``ones`` and
+        ``slot_map`` for :func:`~wick_b200.ops.step_tables`.  Graphs switched off: the same, not captured.  prefer_captured: a captured step of
+        more sequences serves as well (a batch that is about to end)."""
         n_pad = self._bucket(n_seqs)
         key = (n_pad, width, n_groups, max_pages, own_bound)
-        g = self._shared_graphs.get(key)
+        if prefer_captured and key not in self._shared_graphs:
+            key = min((k for k in self._shared_graphs if k[0] > n_pad and k[1:] == key[1:]), default=key)
+        g = self._shared_graphs.pop(key, None)
         if g is None:
+            if len(self._shared_graphs) >= SHARED_GRAPH_COUNT:
+                torch.cuda.synchronize(self.device)                  # (none of those that go is in flight)
+                while len(self._shared_graphs) >= SHARED_GRAPH_COUNT:
+                    del self._shared_graphs[next(iter(self._shared_graphs))]
             g = _DecodeGraph(n_pad, width)
             g.buffer = torch.zeros(g.layout.size, dtype=torch.int32, device=self.device)
             g.batch = StepBatch(g.layout, g.buffer, q_lens=[1] * n_pad, starts=[0] * n_pad, workspace=self.workspace, kv_bound=width * PAGE)
@@ -424,8 +433,10 @@ class Engine:
             g.slot_map = torch.zeros(n_pad, dtype=torch.int64, device=self.device)
             self._upload(g.layout, g.buffer, tokens=[[0]] * n_pad, starts=[0] * n_pad, slots=[0] * n_pad, pages=[[0]] * n_pad, want=[[0]] * n_pad)
             if self.use_graphs:
-                self._capture(g)
-            self._shared_graphs[key] = g
+                if self._shared_pool is None:
+                    self._shared_pool = torch.cuda.graph_pool_handle()
+                self._capture(g, pool=self._shared_pool)
+        self._shared_graphs[key] = g
         return g
 
     def _fill_graph_batch(self, g: _DecodeGraph, slots, tokens, starts) -> None:
@@ -469,7 +480,7 @@ class Engine:
         self.workspace.frozen = True
         before = ops.launches[0]
         try:
-            with torch.cuda.graph(graph, pool=pool):     # (prompt steps share one pool: they never run at the same time)
+            with torch.cuda.graph(graph, pool=pool):     # (prompt steps share one pool, steps of continuations another: none run at the same time)
                 g.logits = run()
         finally:
             self.workspace.frozen = False

@@ -60,7 +60,8 @@ class SampleRun(DeviceRun):
         self.whole = whole
         self.prompt_of = [i for i in range(P) for _ in numbers[i]]
         R = len(self.prompt_of)
-        self.length = [lens[i] for i in self.prompt_of]            # positions cached, of each continuation
+        self.prompt_len = [lens[i] for i in self.prompt_of]
+        self.length = list(self.prompt_len)                        # positions cached, of each continuation
         self.limit = [limits[i] for i in self.prompt_of]
         # the prompts, once each
         self.parents = [e.open_seq() for _ in prompts]
@@ -141,12 +142,17 @@ class SampleRun(DeviceRun):
 
     def _compose(self, live: Sequence[int]) -> None:
         """The description of a step of these continuations; padded entries are a last group that shares nothing."""
-        e, P = self.engine, len(self.parents)
-        g = self.graph = e.shared_graph(len(live), self.width, P + 1, _power(max(max(self.whole), 1)) if max(self.whole) else 0, self.own_bound)
+        e, P, G = self.engine, len(self.parents), _power(len(self.parents) + 1)
+        # (A batch that has shrunk and will end within 64 steps keeps the captured step it has.)
+        ending = max(self.prompt_len[r] + self.limit[r] - self.length[r] for r in live) < 64
+        g = self.graph = e.shared_graph(len(live), self.width, G, _power(max(self.whole)) if max(self.whole) else 0, self.own_bound, prefer_captured=ending)
         pad = g.n_pad - len(live)
-        sizes = [sum(self.prompt_of[r] == i for r in live) for i in range(P)] + [pad]
-        fields = [[self.slots[r] for r in live] + [0] * pad, np.cumsum([0] + sizes), self.whole + [0],
-                  [self.prompt_of[r] for r in live] + [P] * pad, list(live) + [-1] * pad]
+        sizes = [0] * G
+        for r in live:
+            sizes[self.prompt_of[r]] += 1
+        sizes[G - 1] = pad
+        fields = [[self.slots[r] for r in live] + [0] * pad, np.cumsum([0] + sizes), self.whole + [0] * (G - P),
+                  [self.prompt_of[r] for r in live] + [G - 1] * pad, list(live) + [-1] * pad]
         flat = torch.from_numpy(np.concatenate([np.asarray(f, dtype=np.int32) for f in fields])).pin_memory().to(e.device, non_blocking=True)
         at = 0
         for dst in (g.batch.slots, g.batch.shared.cu_groups, g.batch.shared.pages, g.batch.shared.group_of, g.rows):
