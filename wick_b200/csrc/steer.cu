@@ -64,6 +64,7 @@ struct Steer {
     const float* penalties;    // [n_rows, 3]: repetition, frequency, presence
     const int *bias_cu, *bias_tokens;
     const float* bias_values;  // tokens of one row are distinct
+    int n_bias;                // entries there are: ranges end there
     const unsigned* masks;     // [n_masks, words]
     const int* mask_of;        // [n_rows], -1: none
 };
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(HT) steer_kernel(const Steer a) {
     const int which = known && a.masks ? a.mask_of[r] : -1;
     const unsigned* mask = which >= 0 && which < a.n_masks ? a.masks + (int64_t)which * a.words : nullptr;
     int b0 = 0, b1 = 0;
-    if (known && a.bias_cu) b0 = a.bias_cu[r], b1 = a.bias_cu[r + 1];
+    if (known && a.bias_cu) b0 = max(a.bias_cu[r], 0), b1 = min(a.bias_cu[r + 1], a.n_bias);
     bool biases = false;       // of tokens of this block
     if (b0 < b1) {
         for (int k = threadIdx.x; k < CH / 32; k += HT) biased[k] = 0;
@@ -183,11 +184,11 @@ WICK_API int wick_history_add(void* seen, int* counts, const int* tokens, const 
 // x, y: float32 [n, vocab], rows x_stride / y_stride apart; the other arrays as in struct Steer.
 WICK_API int wick_steer_logits(const float* x, int64_t x_stride, float* y, int64_t y_stride, int n, int vocab, const int* rows, int n_rows,
                                const void* seen, const int* counts, const float* penalties, const int* bias_cu, const int* bias_tokens,
-                               const float* bias_values, const void* masks, const int* mask_of, int n_masks, void* s) {
-    WICK_REQUIRE(vocab > 0 && n >= 0 && n <= 65535, "steer_logits: bad sizes");
+                               const float* bias_values, int n_bias, const void* masks, const int* mask_of, int n_masks, void* s) {
+    WICK_REQUIRE(vocab > 0 && n >= 0 && n <= 65535 && n_bias >= 0, "steer_logits: bad sizes");
     if (n == 0) return 0;
     Steer a = {x, y, x_stride, y_stride, vocab, (vocab + 31) / 32, n_rows, n_masks, rows, (const unsigned*)seen, counts, penalties,
-               bias_cu, bias_tokens, bias_values, (const unsigned*)masks, mask_of};
+               bias_cu, bias_tokens, bias_values, n_bias, (const unsigned*)masks, mask_of};
     const bool alike = (((uintptr_t)x ^ (uintptr_t)y) & 15) == 0 && (x_stride - y_stride) % 4 == 0;
     const bool eight = alike && (int64_t)ceil_div(vocab, HT * 4) * n > 16 * sm_count();
     const dim3 grid(ceil_div(vocab + (alike ? 3 : 0), HT * (eight ? 8 : 4)), n);

@@ -2139,7 +2139,8 @@ def steer_logits(logits: torch.Tensor, rows: Optional[torch.Tensor] = None, *, s
     * ``seen``, ``counts`` (see :func:`history_clear`) with ``penalties``, float32 [rows, 3]: a token that occurred has its logit
       divided by penalties[:, 0] if positive, multiplied otherwise; then ``penalties[:, 1] * n + penalties[:, 2]`` is taken off one
       that was generated n > 0 times (repetition, frequency, presence);
-    * ``bias`` = (int32 [rows + 1] ranges, int32 tokens, float32 values): row r's entries, whose tokens differ, are added;
+    * ``bias`` = (int32 [rows + 1] ranges, int32 tokens, float32 values): row r's entries, whose tokens differ, are added (what a range names
+      beyond the entries there are, and tokens outside the vocabulary, is left out);
     * ``masks``, int32 [masks, words]: a token whose bit is 0 in mask ``mask_of[row]`` (int32 [rows]; -1: none) becomes -inf, whatever
       its logit was.  A mask that allows nothing leaves a row of -inf.
 
@@ -2181,8 +2182,8 @@ def steer_logits(logits: torch.Tensor, rows: Optional[torch.Tensor] = None, *, s
     if rows is not None:
         _cuda("rows", rows, torch.int32, (n,))
     ptrs = [0 if t is None else t.data_ptr() for t in (rows, seen, counts, penalties, cu, tokens, values, masks, mask_of)]
-    _core().call_packed("wick_steer_logits", "plpliipippppppppip", logits.data_ptr(), far, out.data_ptr(), out_far, n, vocab, ptrs[0], n_rows,
-                        *ptrs[1:], n_masks, _stream())
+    _core().call_packed("wick_steer_logits", "plpliipippppppippip", logits.data_ptr(), far, out.data_ptr(), out_far, n, vocab, ptrs[0], n_rows,
+                        *ptrs[1:7], 0 if tokens is None else tokens.numel(), *ptrs[7:], n_masks, _stream())
     return out
 
 
