@@ -495,8 +495,8 @@ attn_shared_part_kernel(const T* q, const T* __restrict__ kv, int64_t kv_pages, 
         write_record(w, records + (int64_t)s.record * REC, n_rows);
     }
     if (blockIdx.x == 0 && threadIdx.x < 32) {
-        Walk(parts, gridDim.x, plan);
-        clear_unfit(parts, out, G.heads * HD, status);
+        const Walk all(parts, gridDim.x, plan);
+        clear_unfit(parts, out, G.heads * HD, all.wrong, status);
     }
 }
 
@@ -510,18 +510,20 @@ __device__ __forceinline__ Source shared_source(const Groups& G, const Records& 
     Source s = {rec.at, 0, 0, rec.rows, 0};
     if (!rec.plan || c.pages == 0) return s;
     const int idx = (tok - c.tok0) * G.gs + h % G.gs, tile = idx / G.rows, floats = rec.rows * (HD + 2);
-    const Place p = place_of(G, c, rec.plan[0], tile, kvh * G.per_kv + h / G.gs);
+    const int run = rec.plan[0];                   // (0, no records: looked at last, beside the other reads)
+    const Place p = place_of(G, c, max(run, 1), tile, kvh * G.per_kv + h / G.gs);
     s.at = rec.at + (int64_t)((rec.plan[1 + g] + p.first) * G.pair + tile % G.pair) * floats;
-    s.n = p.n, s.step = floats * G.pair, s.r = idx - tile * G.rows;
+    s.n = run > 0 ? p.n : 0, s.step = floats * G.pair, s.r = idx - tile * G.rows;
     return s;
 }
 __device__ __forceinline__ Source own_source(const OwnParts& parts, const Records& rec, int b, const Cut& c, int idx, int kvh) {
     if (c.pages == 0) return Source{rec.at, 0, 0, rec.rows, 0};
     const int *units = rec.plan + 1, *items = rec.plan + 2 + parts.n();
-    const Deal deal(units[parts.n()], rec.plan[0]);
+    const int workers = rec.plan[0];               // (0, no records: looked at last, beside the other reads)
+    const Deal deal(units[parts.n()], max(workers, 1));
     const int tile = idx / parts.rows, item = tile * parts.G.kv_heads + kvh, u = units[b] + item * c.pages, c0 = deal.worker_of(u);
     const int floats = rec.rows * (HD + 2);
-    return Source{rec.at + (int64_t)(items[b] + item + c0) * floats, deal.worker_of(u + c.pages - 1) - c0 + 1, floats, rec.rows, idx - tile * parts.rows};
+    return Source{rec.at + (int64_t)(items[b] + item + c0) * floats, workers > 0 ? deal.worker_of(u + c.pages - 1) - c0 + 1 : 0, floats, rec.rows, idx - tile * parts.rows};
 }
 
 // Blocks (four rows, sequence): a thread has a row and four columns (and those 128, 256 .. behind), four neighbouring threads four
@@ -538,7 +540,7 @@ attn_shared_join_kernel(T* __restrict__ out, const Groups G, const Records share
     const Cut mine = parts(b);                      // (the description may be read before the wait)
     const int tok = row / G.heads, head = row - tok * G.heads, kvh = head / group, h = head - kvh * group, g = G.group_of[b];
     const bool there = tok < mine.n_tok && mine.pages > 0;
-    Cut c = Cut{0, 0, 0, 0, 0, 0, 0};
+    Cut c = Cut{};
     if (there) c = groups ? parts(G.n_seqs + g) : SharedParts{G}(g);
     pdl_wait();
     pdl_trigger();
@@ -731,7 +733,8 @@ WICK_API long long wick_attn_shared_scratch(int half, int n_tokens, int n_seqs, 
 // values; cu_groups: int32 [n_groups + 1], the sequences of each group; pages: int32 [n_groups], the leading pages that a group's
 // sequences have in common (each holds that many whole pages before this step); group_of: int32 [n_seqs].  max_pages, own_bound,
 // max_q_len: upper bounds of pages, of a sequence's positions behind its group's pages, and of a sequence's new tokens.
-// status: 10 a page outside the cache, 11 a sequence that does not fit its group or its page table (its rows become zeros).
+// status: 10 a page outside the cache, 11 a sequence that does not fit its group or its page table (its rows become zeros), or groups in no order
+// (where the own keys' kernel does them too all rows become zeros, else they lack the shared keys).
 #define WICK_ATTN_SHARED(NAME, T)                                                                                                                        \
     WICK_API int NAME(const void* q, int n_tokens, const void* kv, int64_t kv_pages, void* out, const int* cu_groups, const int* pages,                   \
                       const int* group_of, int n_groups, const int* cu_seqlens, int n_seqs, const int* start, const int* page_table, int table_width,     \

@@ -38,13 +38,18 @@ __device__ __forceinline__ int pages_of(const Groups& G, int g) { return max(0, 
 struct Cut {
     int pages, tok0, n_tok, tiles;
     int seq, first, end;                           // the row of the page table, its first column, the end of the positions
+    // A group that ends before it begins.  Scratch has room for groups that are one behind the other; in any other order a sequence could be in
+    // many.  Then nothing is computed for groups, which is reported.
+    bool wrong;
 };
 struct SharedParts {
     const Groups& G;
     __device__ __forceinline__ Cut operator()(int g) const {
         Cut c;
         c.pages = pages_of(G, g);
-        const int a = max(0, min(G.cu_groups[g], G.n_seqs)), b = max(a, min(G.cu_groups[g + 1], G.n_seqs));
+        const int from = G.cu_groups[g], to = G.cu_groups[g + 1];
+        const int a = max(0, min(from, G.n_seqs)), b = max(a, min(to, G.n_seqs));
+        c.wrong = to < from;
         c.seq = a, c.first = 0;
         c.tok0 = G.single ? a : G.cu_seqlens[a];
         c.n_tok = (G.single ? b : G.cu_seqlens[b]) - c.tok0;
@@ -71,7 +76,7 @@ struct OwnParts {
             c = SharedParts{G}(i - G.n_seqs);
         } else {
             const int g = G.group_of[i];
-            c.seq = i;
+            c.seq = i, c.wrong = false;
             c.tok0 = G.single ? i : G.cu_seqlens[i];
             c.n_tok = G.single ? 1 : G.cu_seqlens[i + 1] - c.tok0;
             c.first = g >= 0 && g < G.n ? pages_of(G, g) : 0;
@@ -82,14 +87,14 @@ struct OwnParts {
         return c;
     }
 };
-// By a warp: the sequences that do not fit are reported, and their rows are made zero.
-template <typename T> __device__ __forceinline__ void clear_unfit(const OwnParts& parts, T* out, int row_numbers, int* status) {
+// By a warp: the sequences that do not fit are reported, and groups in no order (wrong); the sequences' rows are made zero.
+template <typename T> __device__ __forceinline__ void clear_unfit(const OwnParts& parts, T* out, int row_numbers, bool wrong, int* status) {
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < parts.G.n_seqs; b0 += 32) {
-        Cut c = Cut{0, 0, 0, 0, 0, 0, 0};
+        Cut c = Cut{};
         if (b0 + lane < parts.G.n_seqs) c = parts(b0 + lane);
         unsigned bad = __ballot_sync(0xffffffffu, c.n_tok > 0 && c.pages == 0);
-        if (bad && lane == 0) atomicCAS(status, 0, 11);
+        if ((bad || wrong) && lane == 0) atomicCAS(status, 0, 11);
         for (; bad; bad &= bad - 1) {
             const int l = __ffs(bad) - 1;
             const int64_t at = (int64_t)__shfl_sync(0xffffffffu, c.tok0, l) * row_numbers, n = (int64_t)__shfl_sync(0xffffffffu, c.n_tok, l) * row_numbers;
@@ -144,7 +149,7 @@ __device__ __forceinline__ Place place_of(const Groups& G, const Cut& c, int run
 // A warp's knowledge of all runs.  A lane knows one group of 32.
 struct Runs {
     const Groups& G;
-    int run, all;                                  // pages of a run, all runs
+    int run, all;                                  // pages of a run (0: the groups are in no order), all runs
     int g0, before;                                // first of the groups known; runs of the groups before it
     Cut mine;
     int upto;                                      // runs up to this lane's group
@@ -152,7 +157,7 @@ struct Runs {
     __device__ __forceinline__ void know(int first) {
         g0 = first;
         const int g = g0 + (int)(threadIdx.x & 31);
-        mine = Cut{0, 0, 0, 0, 0, 0, 0};
+        mine = Cut{};
         if (g < G.n) mine = SharedParts{G}(g);
     }
     __device__ __forceinline__ void count() {
@@ -167,8 +172,10 @@ struct Runs {
     __device__ __forceinline__ Runs(const Groups& groups, int blocks) : G(groups), before(0) {
         // the shortest run that leaves no thread block with two; no shorter than an equal share, no longer than the longest item
         int cost = 0, most = 1;
+        bool wrong = false;
         for (int g = 0; g < G.n; g += 32) {
             know(g);
+            wrong |= mine.wrong;
             cost += __reduce_add_sync(0xffffffffu, (unsigned)(mine.tiles * G.columns * mine.pages));
             most = max(most, (int)__reduce_max_sync(0xffffffffu, (unsigned)(mine.tiles > 0 ? mine.pages : 0)));
         }
@@ -183,10 +190,15 @@ struct Runs {
         }
         if (G.n > 32) know(0);
         count();
+        if (__any_sync(0xffffffffu, wrong)) all = run = 0;
     }
     // plan: the pages of a run, then the runs before each group.
-    __device__ __forceinline__ void write(int* plan) {
-        if ((threadIdx.x & 31) == 0) plan[0] = run, plan[1] = 0;
+    __device__ __forceinline__ void write(int* plan, int* status) {
+        if ((threadIdx.x & 31) == 0) {
+            plan[0] = run, plan[1] = 0;
+            if (run == 0) atomicCAS(status, 0, 11);
+        }
+        if (run == 0) return;
         for (int g = 0; g < G.n; g += 32) {
             if (g > 0) before = __shfl_sync(0xffffffffu, upto, 31), know(g), count();
             if (g + (int)(threadIdx.x & 31) < G.n) plan[2 + g + (threadIdx.x & 31)] = upto;
@@ -222,10 +234,11 @@ struct Walk {
     int b0, units, items;                          // first of the sequences known; units and items before it
     Cut mine;
     int upto_units, upto_items;                    // ... and up to this lane's
+    bool wrong;                                    // the groups are in no order
 
     __device__ __forceinline__ Cut cut(int first) const {
         const int b = first + (int)(threadIdx.x & 31);
-        return b < parts.n() ? parts(b) : Cut{0, 0, 0, 0, 0, 0, 0};
+        return b < parts.n() ? parts(b) : Cut{};
     }
     __device__ __forceinline__ void know(int first, const Cut& c) {
         b0 = first, mine = c;
@@ -241,20 +254,22 @@ struct Walk {
         units = __shfl_sync(0xffffffffu, upto_units, 31), items = __shfl_sync(0xffffffffu, upto_items, 31);
         know(b0 + 32, c);
     }
-    // plan: the workers' number and the units and items before each sequence are written down there (null: not).
-    __device__ __forceinline__ Walk(const OwnParts& p, int workers, int* plan) : parts(p), deal(0, 1), units(0), items(0) {
+    // plan: the workers' number (0: the groups are in no order) and the units and items before each sequence are written down there (null: not).
+    __device__ __forceinline__ Walk(const OwnParts& p, int workers, int* plan) : parts(p), deal(0, 1), units(0), items(0), wrong(false) {
         const int lane = threadIdx.x & 31;
         know(0, cut(0));
         for (;;) {
             const Cut ahead = b0 + 32 < parts.n() ? cut(b0 + 32) : mine;       // (read beside what is counted now)
             const int b = b0 + lane;
+            wrong |= mine.wrong;
             if (plan && b < parts.n()) plan[2 + b] = upto_units, plan[3 + parts.n() + b] = upto_items;
             if (b0 + 32 >= parts.n()) break;
             next(ahead);
         }
         deal = Deal(__shfl_sync(0xffffffffu, upto_units, 31), workers);
-        if (plan && lane == 0) plan[0] = deal.S, plan[1] = 0, plan[2 + parts.n()] = 0;
-        const bool in = deal.U > 0 && (int)blockIdx.x < deal.S;
+        wrong = __any_sync(0xffffffffu, wrong);
+        if (plan && lane == 0) plan[0] = wrong ? 0 : deal.S, plan[1] = 0, plan[2 + parts.n()] = 0;
+        const bool in = !wrong && deal.U > 0 && (int)blockIdx.x < deal.S;
         u = in ? deal.run_start(blockIdx.x) : 0;
         end = in ? deal.run_start(blockIdx.x + 1) : 0;
         if (u < units) units = items = 0, know(0, cut(0));                     // (else it begins among those known last)

@@ -241,8 +241,8 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
     }
     if (blockIdx.x == 0) {
         pdl_wait();
-        Walk(parts, gridDim.x, plan);
-        clear_unfit(parts, out, G.heads * HD, status);
+        const Walk all(parts, gridDim.x, plan);
+        clear_unfit(parts, out, G.heads * HD, all.wrong, status);
     }
     pdl_wait();                                        // (whoever waits for this kernel waits for the one before it too)
     if (sm.abort_flag) {

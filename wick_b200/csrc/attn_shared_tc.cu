@@ -108,7 +108,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     if (warp == 0 && blockIdx.x < runs.all) seg = runs.segment(blockIdx.x), even = pages(0), odd = pages(1);
     pdl_wait();
     pdl_trigger();                                     // (behind the wait: the next kernel reads what this one reads without a wait of its own)
-    if (blockIdx.x == 0 && warp == 2) Runs(G, gridDim.x).write(plan);
+    if (blockIdx.x == 0 && warp == 2) Runs(G, gridDim.x).write(plan, status);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

@@ -142,7 +142,7 @@ _STATUS_TEXT = {1: "gemm_tc gave up waiting for a free shared-memory stage", 2: 
                 7: "attention (tcgen05) gave up waiting for a copy or an accumulator",
                 8: "attention decode (tensor cores) gave up waiting for its TMA copies",
                 10: "attention decode was given a length or a page outside its page table or its cache",
-                11: "attention over a shared prefix was given a sequence that does not fit its group's pages or its page table",
+                11: "attention over a shared prefix was given a sequence that does not fit its group's pages or its page table, or groups in no order",
                 12: "step_tables ran out of free pages",
                 13: "step_tables was given a record, a parent or a length outside its tables, or a fork that begins inside a page",
                 14: "step_tables was given more tokens than places for them",
