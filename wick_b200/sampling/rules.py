@@ -36,7 +36,8 @@ class LogitRules:
                     raise ValueError(f"token id {t} of {what} is outside the vocabulary of {vocab}")
         if any(math.isnan(float(b)) for b in self.bias.values()):
             raise ValueError("a bias is not a number")
-        if self.allowed is not None and len(self.allowed) == 0:
+        ruled_out = {int(t) for t, b in self.bias.items() if float(b) == -math.inf}
+        if len(ruled_out) >= vocab or (self.allowed is not None and ruled_out.issuperset(int(t) for t in self.allowed)):
             raise ValueError("no token is allowed")
 
 
