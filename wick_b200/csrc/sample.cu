@@ -77,56 +77,65 @@ __device__ __forceinline__ float block_scan(float v, float* warp_tot, float* tot
     return v;
 }
 
-// The weight of a logit beside the row's maximum.  Logits equal to it weigh 1, whatever they are: one of +inf takes the draw, several share it.
-__device__ __forceinline__ float weight_of(float x, float m, float inv_t) { return x == m ? 1.f : expf((x - m) * inv_t); }
-
 // A token without weight (a logit of -inf, or one so far below the maximum) is never drawn: not where the sums' rounding leaves a thread's walk
-// short of the target (then its last token with weight is), not by the uniform number 0 (the target is then the smallest there is).
+// short of the target (then its last token with weight is), not by the uniform number 0 (the target is then the smallest there is).  BOUNDLESS:
+// the maximum is +inf; the logits equal to it share the draw.
+template <bool BOUNDLESS>
+__device__ __forceinline__ int draw_all(const float* __restrict__ x, float m, float uniform, int vocab, float inv_t, float* warp_tot, int* found) {
+    auto weight = [&](int i) { return BOUNDLESS ? (x[i] == m ? 1.f : 0.f) : expf((x[i] - m) * inv_t); };
+    const int chunk = (vocab + ST - 1) / ST;
+    const int lo = min(threadIdx.x * chunk, vocab), hi = min(lo + chunk, vocab);
+    float mine = 0.f;
+    for (int i = lo; i < hi; ++i) mine += weight(i);
+    float total;
+    const float incl = block_scan(mine, warp_tot, &total);
+    const float excl = incl - mine;
+    float target = uniform * total;
+    if (target < FLT_MIN) target = FLT_MIN;        // (a sum that is no number stays one)
+    if (excl < target && incl >= target && mine > 0.f) {
+        float run = excl;
+        int pick = hi;
+        for (int i = lo; i < hi; ++i) {
+            const float w = weight(i);
+            run += w;
+            if (w > 0.f) pick = i;
+            if (w > 0.f && run >= target) break;
+        }
+        atomicMin(&found[0], pick);
+    }
+    __syncthreads();
+    if (found[0] != INT_MAX) return found[0];
+    // Rare.  The target lies in a gap that rounding left between two threads' sums: the token behind it; or behind the last sum: the last with
+    // weight.  (Or the sum is no number: the last token.)
+    if (mine > 0.f) {
+        int first = hi, last = -1;
+        for (int i = lo; i < hi; ++i)
+            if (weight(i) > 0.f) first = min(first, i), last = i;
+        if (incl >= target) atomicMin(&found[1], first);
+        atomicMax(&found[2], last);
+    }
+    __syncthreads();
+    return found[1] != INT_MAX ? found[1] : found[2] >= 0 && total == total ? found[2] : vocab - 1;
+}
+
 __global__ void __launch_bounds__(ST)
 sample_temperature_kernel(const float* __restrict__ logits, const float* __restrict__ uniforms,
                           int* __restrict__ out, int vocab, float inv_t) {
     __shared__ float red[40];
     __shared__ float warp_tot[32];
-    __shared__ int chosen, behind, last;
+    __shared__ int found[3];
     const float* x = logits + (int64_t)blockIdx.x * vocab;
     float m = -INFINITY;
     for (int i = threadIdx.x; i < vocab; i += ST) m = fmaxf(m, x[i]);
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-    if (threadIdx.x == 0) chosen = behind = INT_MAX, last = -1;
+    if (threadIdx.x == 0) found[0] = found[1] = INT_MAX, found[2] = -1;
     __syncthreads();
     m = red[0];
     for (int w = 1; w < 32; ++w) m = fmaxf(m, red[w]);
-
-    const int chunk = (vocab + ST - 1) / ST;
-    const int lo = min(threadIdx.x * chunk, vocab), hi = min(lo + chunk, vocab);
-    float mine = 0.f;
-    int first = INT_MAX, heavy = -1;               // the first and the last of this thread's tokens with weight
-    for (int i = lo; i < hi; ++i) {
-        const float w = weight_of(x[i], m, inv_t);
-        mine += w;
-        if (w > 0.f) first = min(first, i), heavy = i;
-    }
-    float total;
-    const float incl = block_scan(mine, warp_tot, &total);
-    const float excl = incl - mine;
-    float target = uniforms[blockIdx.x] * total;
-    if (target < FLT_MIN) target = FLT_MIN;        // (a sum that is no number stays one)
-    if (excl < target && incl >= target && heavy >= 0) {
-        float run = excl;
-        for (int i = lo; i <= heavy; ++i) {
-            const float w = weight_of(x[i], m, inv_t);
-            run += w;
-            if (w > 0.f && run >= target) { heavy = i; break; }
-        }
-        atomicMin(&chosen, heavy);
-    }
-    // Where two threads' rounded sums leave a gap at their border and the target lies in it, the token behind it is taken; where it lies behind
-    // the last sum, the last with weight.
-    const int after = __reduce_min_sync(0xffffffffu, incl >= target ? first : INT_MAX), of_warp = __reduce_max_sync(0xffffffffu, heavy);
-    if ((threadIdx.x & 31) == 0) atomicMin(&behind, after), atomicMax(&last, of_warp);
-    __syncthreads();
-    if (threadIdx.x == 0) out[blockIdx.x] = chosen != INT_MAX ? chosen : behind != INT_MAX ? behind : last >= 0 && total == total ? last : vocab - 1;
+    const float u = uniforms[blockIdx.x];
+    const int pick = m == INFINITY ? draw_all<true>(x, m, u, vocab, inv_t, warp_tot, found) : draw_all<false>(x, m, u, vocab, inv_t, warp_tot, found);
+    if (threadIdx.x == 0) out[blockIdx.x] = pick;
 }
 
 // Each (row, token) pair once: logit > 0 ? logit / penalty : logit * penalty
@@ -257,8 +266,12 @@ __global__ void pick_sorted_kernel(const float* __restrict__ vals, const int* __
     const float top = v[0];
     float total = 0.f;
     for (int i = 0; i < k; ++i) {
-        p[i] = v[i] == top ? 1.f : expf(__fdiv_rn(__fsub_rn(v[i], top), temperature));
+        p[i] = expf(__fdiv_rn(__fsub_rn(v[i], top), temperature));
         total = __fadd_rn(total, p[i]);
+    }
+    if (top == INFINITY) {
+        total = 0.f;
+        for (int i = 0; i < k; ++i) p[i] = v[i] == top ? 1.f : 0.f, total += p[i];
     }
     for (int i = 0; i < k; ++i) p[i] = __fdiv_rn(p[i], total);
     int keep = k;
@@ -277,13 +290,13 @@ __global__ void pick_sorted_kernel(const float* __restrict__ vals, const int* __
     float tot = 0.f;
     for (int i = 0; i < keep; ++i) tot = __fadd_rn(tot, p[i]);
     float r = __fmul_rn(uniforms[row], tot);
-    int pick = 0;
+    int pick = -1;
     for (int i = 0; i < keep; ++i) {
-        if (i > 0 && v[i] == -INFINITY) break;     // (sorted: nothing but such behind it)
-        pick = i;
         r = __fsub_rn(r, p[i]);
-        if (r <= 0.f) break;
+        if (r <= 0.f) { pick = i; break; }         // (never by a weight of zero: r was above it before)
     }
+    if (pick < 0)
+        for (pick = keep - 1; pick > 0 && v[pick] == -INFINITY; --pick) {}
     out[row] = ix[pick];
 }
 
