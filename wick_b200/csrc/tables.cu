@@ -43,17 +43,27 @@ struct Tables {
     }
 };
 
-// The rows that step_tables_kernel has made, into the tables: a warp a sequence.
-__global__ void __launch_bounds__(TT) store_tables_kernel(const Tables a) {
-    pdl_wait();                                    // (no early start of the next kernel, as below)
-    const int lane = threadIdx.x & 31;
-    for (int b = ((int)blockIdx.x * TT + (int)threadIdx.x) >> 5; b < a.n_seqs; b += (int)gridDim.x * (TT / 32)) {
-        const int slot = a.slot_of(b), start = max(a.start[b], 0), held = (start + kPage - 1) / kPage;
-        if (slot <= 0) continue;
-        const int from = a.source_of(b, slot) != slot ? 0 : held, to = min((start + max(a.q_len[b], 0) + kPage - 1) / kPage, min(a.width, a.table_width));
-        const int* row = a.page_table + (int64_t)b * a.width;
-        for (int j = from + lane; j < to; j += 32) a.tables[(int64_t)slot * a.table_width + j] = row[j];
+// The rows that step_tables_kernel has made, into the tables: a warp has COLUMNS columns of a sequence, a lane four, read before one is written.
+constexpr int COLUMNS = 128;
+__global__ void __launch_bounds__(TT) store_tables_kernel(const Tables a, int pieces) {
+    const int at = ((int)blockIdx.x * TT + (int)threadIdx.x) >> 5, b = at / pieces;
+    int slot = 0, from = 0, to = 0;
+    if (b < a.n_seqs) {                            // (what the call was given may be read before the wait: the kernel before has waited for it)
+        const int start = max(a.start[b], 0);
+        slot = a.slot_of(b);
+        if (a.source_of(b, slot) == slot) from = (start + kPage - 1) / kPage;
+        to = min((start + max(a.q_len[b], 0) + kPage - 1) / kPage, min(a.width, a.table_width));
     }
+    pdl_wait();                                    // (no early start of the next kernel, as below)
+    if (slot <= 0) return;
+    const int* row = a.page_table + (int64_t)b * a.width;
+    const int j0 = (at - b * pieces) * COLUMNS + (int)(threadIdx.x & 31);
+    int page[COLUMNS / 32];
+#pragma unroll
+    for (int k = 0; k < COLUMNS / 32; ++k) page[k] = j0 + 32 * k < to ? row[j0 + 32 * k] : 0;
+#pragma unroll
+    for (int k = 0; k < COLUMNS / 32; ++k)
+        if (j0 + 32 * k >= from && j0 + 32 * k < to) a.tables[(int64_t)slot * a.table_width + j0 + 32 * k] = page[k];
 }
 
 __global__ void __launch_bounds__(TT) step_tables_kernel(const Tables a, int* status) {
@@ -61,8 +71,8 @@ __global__ void __launch_bounds__(TT) step_tables_kernel(const Tables a, int* st
     int* cum_q = sums;                             // tokens of the sequences before each one
     int* cum_n = sums + a.n_seqs + 1;              // pages that they need
     __shared__ int warp_q[TT / 32], warp_n[TT / 32];
-    if (a.parent) pdl_trigger();                   // (of store_tables_kernel, which waits before all else)
-    pdl_wait();                                    // (no early start of another kernel: kernels of a step read these fields before they wait)
+    pdl_wait();
+    if (a.parent) pdl_trigger();                   // (store_tables_kernel; no other kernel starts early: kernels of a step read these fields before they wait)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.n_seqs;
     auto held_of = [&](int b) { return (max(a.start[b], 0) + kPage - 1) / kPage; };
     int base_q = 0, base_n = 0;
@@ -157,6 +167,8 @@ WICK_API int wick_step_tables(const int* start, const int* q_len, const int* slo
     WICK_REQUIRE(n_slots >= 1 && table_width >= 1 && width >= 1 && n_free >= 0 && n_tokens >= 0, "step_tables: bad sizes");
     Tables a = {start, q_len, slots, parent, tables, free_pages, free_head, page_table, cu_seqlens, kv_len, positions, seq_of_token, head_out,
                 (int64_t*)slot_map, n_seqs, n_slots, table_width, width, n_free, n_tokens};
+    const int pieces = ceil_div(min(width, table_width), COLUMNS);
+    WICK_REQUIRE((int64_t)n_seqs * pieces <= INT32_MAX / 32, "step_tables: %d sequences of %d columns", n_seqs, width);
     const int blocks = max(1, min(2 * sm_count(), max(ceil_div((int64_t)n_seqs, TT / 32), ceil_div(n_tokens, TT))));
     const size_t smem = (size_t)(2 * (n_seqs + 1)) * sizeof(int);
     static bool raised = false;
@@ -167,7 +179,7 @@ WICK_API int wick_step_tables(const int* start, const int* q_len, const int* slo
     WICK_CUDA(launch(step_tables_kernel, dim3(blocks), dim3(TT), smem, (cudaStream_t)s, a, status));
     if (int e = check_launch("step_tables")) return e;
     if (!parent) return 0;
-    WICK_CUDA(launch(store_tables_kernel, dim3(ceil_div(n_seqs, TT / 32)), dim3(TT), 0, (cudaStream_t)s, a));
+    WICK_CUDA(launch(store_tables_kernel, dim3(ceil_div((int64_t)n_seqs * pieces, TT / 32)), dim3(TT), 0, (cudaStream_t)s, a, pieces));
     return check_launch("store_tables");
 }
 WICK_PACKED(wick_step_tables)
