@@ -10,8 +10,9 @@
 // two instructions; and a value row's numbers may stand in any order of columns, so a lane takes 16 neighbouring bytes of each of four
 // keys' rows and pairs them by byte permutation.  No shared memory, no barrier until the warps' parts are joined.  Weights enter the second
 // product rounded to bfloat16, and their sum is taken of the rounded ones, so that a row of equal values keeps them.
-// float32: products and sums on the CUDA cores, keys and values through shared memory, 32 keys at a time: bound by the shared memory's reads
-// for them (6 sequences behind 1,000 positions, 16 heads over 4 of 128: 12.2 us, 7 MB).
+// float32: products and sums on the CUDA cores, keys and values through shared memory, 32 keys at a time: bound by the chain of a page, two
+// times 64 rounds through shared memory by four warps (6 sequences behind 1,000 positions, 16 heads over 4 of 128: 12.2 us, 7 MB; the reads
+// at the shared memory's rate would be 2).
 // The join is bound by a chain (plan, then records that other SMs have just written) and, where there are many, by the records' bytes: 64
 // sequences of 32 heads with ten records a row of the shared keys, 11 MB, 7 us; 4 of 16 heads 4.5.
 #include "common.cuh"

@@ -93,7 +93,7 @@ attn_shared_own_kernel(const __grid_constant__ CUtensorMap kv_map, const bf16* q
     // (The description lies ready before the step's kernels start.)
     const OwnParts parts{G, R, groups};
     Walk walk(parts, gridDim.x, nullptr);
-    const uint64_t policy = read_once_policy();
+    const uint64_t policy = read_once_policy();        // (once for 8 rows: the records, which are read again, are to stay)
     Ahead next = {};
     auto know_ids = [&]() {                            // from page next.j on
         const int* table = G.page_table + (int64_t)next.s.cut.seq * G.table_width + next.s.cut.first;

@@ -9,7 +9,8 @@
 //   * the last tile of an odd number: even blocks of keys go to one stream, odd ones to the other, joined when the run ends.
 // Roles:
 //   * a producer warp fetches the query rows of a run and its key and value tiles through a ring (TMA, 128-byte swizzle, first to leave the
-//     L2 cache: each is read once, and the records, which are read again, stay there; 24 sequences behind 31,000 positions 60.7 and 55.6 us);
+//     L2 cache: each is read once for 256 rows, and the records, which are read again, stay there; 24 sequences behind 31,000 positions 60.7
+//     and 55.6 us);
 //   * an issuing lane alternates between the streams: O += P V of one, then the scores S = Q K^T of its block after the next (P lies over
 //     the scores it came from, as bfloat16 pairs).  It waits by itself, without votes, and arrives once a block for both of its tiles:
 //     with a whole warp's votes and an arrival for each tile and product a turn took 1,400 clocks, of which 580 were its instructions;

@@ -10,9 +10,9 @@
 //   l <- -inf where the row's mask does not allow the token
 //
 // Whole numbers are added with atomics, whose order changes nothing.  All arithmetic is in 32 bits, as the logits are.
-// Steering is bound by its bytes in large calls (4 read and 4 written a token, at 3.3 TB/s: 61 rows of 100,003 tokens, half of them masked, in
-// 14.6 us, beside some 200 instructions a warp) and by one chain of dependent reads in small ones (place, mask,
-// bits, count: 8 rows of 151,936 in 4.5 us, one of 32,768 in 2.6).  History calls are a launch (2.4 us each in a graph).
+// Steering is bound by one chain of dependent reads (place, mask, bits, count: 8 rows of 151,936 in 4.5 us, one of 32,768 in 2.6), which in
+// large calls every round of blocks goes through: 61 rows of 100,003 tokens, half of them masked, 14.6 us, of which the bytes (4 read and 4
+// written a token) are 7.6 and the instructions, some 200 a warp, 4.1.  History calls are a launch (2.4 us each in a graph).
 #include "common.cuh"
 #include "packed.cuh"
 

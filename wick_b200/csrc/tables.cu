@@ -15,7 +15,7 @@
 // for one another, would cost more than that), then a warp fills a sequence's row, a thread a token.  Record 0 is the padding's: it gets no
 // pages.
 // Bound by that chain, and in a large call by its rows, a warp each, whose reads and writes wait for one another: 48 sequences of a token each
-// 3.5 us, 700 with 300 forks and up to 400 tokens each (5 MB written) 9.1.
+// 3.3 to 3.7 us (with parents, and so a second launch, 4.2), 700 with 300 forks and up to 400 tokens each (5 MB written) 10.3.
 #include "common.cuh"
 #include "packed.cuh"
 

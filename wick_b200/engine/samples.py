@@ -1,10 +1,12 @@
 """Several continuations of every prompt, decoded together over ONE copy of the prompt's cache.
 
 :func:`sample_many` runs each prompt once.  Its continuations share the prompt's whole pages (``csrc/attn_shared.cuh``: a step reads them
-once for all continuations); the rest of the prompt's last page is copied, and per-sequence records are, so that what a
+once for all continuations, short ones once per eight rows); the rest of the prompt's last page is copied, and per-sequence records are, so that what a
 continuation writes is its own.  From then on a step needs nothing from the host: the page tables grow on the device, out of a list of
 pages lent to the batch (``ops.step_tables``), the rules are applied and the token is drawn there, and the host, one step behind, reads the
-ids.  A step's description is uploaded only when a continuation has ended.
+ids.  A step's description is uploaded only when a continuation has ended, or another batch has decoded by the same captured step.
+
+Attention is cut by the lengths of the whole batch: in its last places a continuation's logits depend on what is decoded beside it.
 
 Models whose attention is not over paged keys and values, or has options that the shared form does not take, decode the same way: their
 mixers read the page tables, in which the shared pages stand like any others.
