@@ -415,7 +415,7 @@ class Engine:
         more sequences serves as well (a batch that is about to end)."""
         n_pad = self._bucket(n_seqs)
         key = (n_pad, width, n_groups, max_pages, own_bound)
-        if prefer_captured and key not in self._shared_graphs:
+        if prefer_captured and self.use_graphs and key not in self._shared_graphs:
             key = min((k for k in self._shared_graphs if k[0] > n_pad and k[1:] == key[1:]), default=key)
         g = self._shared_graphs.pop(key, None)
         if g is None:
