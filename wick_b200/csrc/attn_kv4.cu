@@ -1,0 +1,767 @@
+// Causal attention over a cache that holds keys and values in 4 bits (kv4.cuh), for any number of new tokens a sequence.
+//
+//   out[i, h] = sum_t p_t v_t,  p = softmax over t <= position(i) of scale q[i, h] . k_t,  k_t and v_t the bfloat16 values that the codes stand for.
+//
+// How the work is cut.  The rows of a (sequence, key head) are its new tokens times the query heads of the key head; they come in tiles of eight or
+// sixteen.  The sequence's pages are cut by its OWN length and the number of key heads alone: into leaves of as many pages (one, for up to 8 most_nodes
+// pages) and nodes of eight leaves.  A leaf is computed by one warp, page by page, into a running maximum, sum and accumulator; a node's leaves
+// are folded in order, a row's nodes likewise.  Which warp computes what changes no bit, so that a sequence's result does not depend on the batch it is
+// in.  The kernel for bfloat16 has a block per node and a warp per leaf; the leaves meet in shared memory.  Nodes leave records (accumulator, maximum, sum) that a
+// second, small kernel joins; a sequence with one node is written directly.
+//
+// The kernel on the tensor cores.  Keys and values stand on the 16-row side of mma.sync (16 positions, or 16 channels), the rows on the 8-column side, so
+// that the eight rows of most head layouts fill it.  A page of one key head (80 d bytes) comes in one bulk copy.  Values are made from codes in registers, in
+// the layout that the instruction wants: what a lane reads of a key are d / 4 neighbouring channels of a position (the queries are permuted to match),
+// and of a value d / 8 neighbouring channels of four positions.  Rows 0, 1, ... 7 of the instruction's position side are
+// the positions 0, 1, 3, 2, 4, 5, 7, 6 of eight, so that either reading touches every bank of the shared memory once.
+//
+// The float32 form (and the plain twin of the other): CUDA cores, the same leaves' values, everything in 32 bits.
+#include "kv4.cuh"
+#include "packed.cuh"
+#include "sm100.cuh"
+
+#ifndef WICK_HD
+#error "compile with -DWICK_HD=<head_dim>"
+#endif
+
+namespace wick {
+namespace kv4 {
+
+constexpr int D = WICK_HD;
+static_assert(D % 64 == 0 && D >= 64 && D <= 256, "head sizes of 64, 128, 192 and 256");
+typedef __nv_bfloat16 bf16;
+
+constexpr int LEAVES = 8;                                        // of a node; warps of a block
+constexpr int THREADS = LEAVES * 32;
+constexpr int TILE = head_bytes(D);                              // a page of one key head
+constexpr int NW = D / 32;                                       // words of a key that a lane reads (its quarter of the row)
+constexpr int NV = D / 64;                                       // words of a value that a lane reads (its eighth)
+constexpr int MAX_STAGES = D <= 128 ? 2 : 1;                      // of a warp's ring (eight rings of two larger tiles are more than an SM has)
+constexpr int MT = D / 16;                                       // tiles of 16 channels
+
+// Nodes of the longest sequences: enough that one sequence alone gives nearly every SM a block (8 key heads: 16), no more (each costs a record).
+__host__ __device__ inline int most_nodes(int n_kv) {
+    const int n = 128 / n_kv;
+    return n < 4 ? 4 : (n > 64 ? 64 : n);
+}
+__host__ __device__ inline int leaf_pages(int n_pages, int n_kv) {
+    const int most = LEAVES * most_nodes(n_kv);
+    return n_pages <= most ? 1 : (n_pages + most - 1) / most;
+}
+__host__ __device__ inline int nodes_of(int n_pages, int n_kv) {
+    const int n = LEAVES * leaf_pages(n_pages, n_kv);
+    return (n_pages + n - 1) / n;
+}
+
+struct Args {
+    const void* q;                                               // [n_tokens, n_heads, d]
+    void* out;
+    const uint8_t* kv;
+    int64_t kv_pages;
+    const int* cu_seqlens;
+    const int* start;
+    const int* page_table;
+    int table_width, n_seqs, n_heads, n_kv, group;
+    float scale2;                                                // scale log2 e
+    int n_tokens;
+    float* rec;                                                  // records: accumulators [row, node, d], then maximum and sum [row, node, 2]; a row is a (token, head)
+    int64_t rec_rows;
+    int nodes;                                                   // places for nodes in a row's records
+    int tiles;                                                   // row tiles of a (sequence, key head) that the grid has
+    int stages;                                                  // of a warp's ring
+    int* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^(a - b) for maxima that may be -inf (nothing seen yet): then the weight is 0.
+__device__ __forceinline__ float weight(float a, float b) { return a == -INFINITY ? 0.f : ex2(a - b); }
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// An 8 x 8 matrix of 16-bit elements, a row per four lanes: the transposed one in the same layout.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ bool no_number(uint32_t scale) { return (scale & 0x7F80u) == 0x7F80u || (scale & 0x7F800000u) == 0x7F800000u; }
+// The position (of 8) in row i of the instruction's position side.
+__device__ __forceinline__ int position_of(int i) { return i ^ ((i >> 1) & 1); }
+
+// A sequence's place in the step, as far as its rows see it.
+struct Seq {
+    int first, new_tokens, start, len, pages;                    // flat number of its first new token; ...; pages that fit its table
+};
+__device__ __forceinline__ Seq sequence(const Args& a, int b) {
+    Seq s;
+    s.first = a.cu_seqlens[b];
+    s.new_tokens = a.cu_seqlens[b + 1] - s.first;
+    s.start = a.start[b];
+    s.len = s.start + s.new_tokens;
+    s.pages = (s.len + kPage - 1) / kPage;
+    return s;
+}
+// Whether a sequence fits the step, its page table and the records' places (else it is left out, and said).
+__device__ __forceinline__ bool fits(const Args& a, const Seq& s) {
+    const bool ok = s.start >= 0 && s.first >= 0 && s.first + s.new_tokens <= a.n_tokens && s.pages <= a.table_width && nodes_of(s.pages, a.n_kv) <= a.nodes;
+    if (!ok) atomicCAS(a.status, 0, 15);
+    return ok;
+}
+// A page id, within the cache (else reported, and page 0).
+__device__ __forceinline__ int checked_page(const Args& a, int id) {
+    if (id < 0 || id >= a.kv_pages) {
+        atomicCAS(a.status, 0, 15);
+        return 0;
+    }
+    return id;
+}
+__device__ __forceinline__ void start_copy(const Args& a, int page, int kvh, uint8_t* dst, uint64_t* bar) {
+    mbar_expect_tx(bar, TILE);
+    bulk_load(dst, a.kv + ((int64_t)page * a.n_kv + kvh) * TILE, TILE, bar);
+}
+
+// ---- one page on the tensor cores -------------------------------------------------------
+template <int NT> struct Sum {                                   // of a leaf or a node: lane (r, j) = (lane / 4, lane % 4) holds rows 2 j, 2 j + 1 of every eight,
+    float o[MT][NT][4];                                          //   channels r d / 8 + 2 m (o[m][.][0], [1]) and + 1 ([2], [3])
+    float m[NT][2], l[NT][2];                                    //   (l: the lane's share until finish_leaf)
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+        }
+    }
+};
+
+template <int NT> struct Rows {
+    uint32_t q[2 * NW][NT][2];                                   // the second operand of the scores, channels in the order of the keys' codes
+    int limit[NT][2];                                            // the last position that rows 2 j, 2 j + 1 see
+};
+
+// Rows row0 .. of a (sequence, key head): row i is head i % group of new token i / group.
+template <int NT>
+__device__ __forceinline__ void load_rows(const Args& a, const Seq& s, int kvh, int row0, Rows<NT>& w) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, n_rows = s.new_tokens * a.group;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int row = row0 + 8 * n + r;
+        const int tok = row / a.group, g = row - tok * a.group;
+        const uint4* src = reinterpret_cast<const uint4*>((const bf16*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + g) * D + 8 * j * NW);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row < n_rows) x = src[i];
+            w.q[2 * i][n][0] = low_halves(x.x, x.z);
+            w.q[2 * i][n][1] = high_halves(x.x, x.z);
+            w.q[2 * i + 1][n][0] = low_halves(x.y, x.w);
+            w.q[2 * i + 1][n][1] = high_halves(x.y, x.w);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) w.limit[n][c] = s.start + min(row0 + 8 * n + 2 * j + c, n_rows - 1) / a.group;
+    }
+}
+
+template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 x = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const uint2 x = reinterpret_cast<const uint2*>(p)[i];
+            w[2 * i] = x.x; w[2 * i + 1] = x.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+
+// One page (in shared memory) into a leaf.  MASK: some of its positions are not seen by some row; first: the position of the page's first row, len: the
+// sequence's length; several: rows of several tokens.  fresh: the leaf's first page.
+template <int NT, bool MASK>
+__device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w, float scale2, int first, int len, bool several, bool fresh, Sum<NT>& sum) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
+    const int tr = position_of(r), ta = position_of(2 * j), tb = position_of(2 * j + 1);
+    float s[4][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.f;
+        uint32_t k[2][NW];
+        const uint8_t* sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int t = mt * 16 + 8 * u + tr;
+            load_words<NW>(tile + t * (D / 2) + j * (D / 8), k[u]);
+            sc[u] = tile + key_scales(D) + t * (D / 8);
+        }
+        uint32_t a2[2], b2[2];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            if (i % (D == 192 ? 2 : 4) == 0) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t x = *reinterpret_cast<const uint32_t*>(sc[u] + ((j * NW + i) >> 2) * 4);
+                    a2[u] = low_halves(x, x);
+                    b2[u] = high_halves(x, x);
+                }
+            }
+            uint32_t v0[4], v1[4];
+            key_word(k[0][i], a2[0], b2[0], v0);
+            key_word(k[1][i], a2[1], b2[1], v1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma16816(s[mt][n], v0[0], v1[0], v0[1], v1[1], w.q[2 * i][n][0], w.q[2 * i][n][1]);
+                mma16816(s[mt][n], v0[2], v1[2], v0[3], v1[3], w.q[2 * i + 1][n][0], w.q[2 * i + 1][n][1]);
+            }
+        }
+    }
+    // scores in units of log2 e, the running maximum, weights
+    uint32_t p[4][NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x = s[mt][n][e] * scale2;
+                if (MASK && first + mt * 16 + 8 * (e >> 1) + tr > w.limit[n][e & 1]) x = -INFINITY;
+                s[mt][n][e] = x;
+                top[e & 1] = fmaxf(top[e & 1], x);
+            }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+            const float m = fmaxf(sum.m[n][c], top[c]), was = weight(sum.m[n][c], m);
+            const float ref = m == -INFINITY ? 0.f : m;          // (nothing seen: weights 0; a score that is no number still shows)
+            sum.m[n][c] = m;
+            float l = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+                s[mt][n][c] = ex2(s[mt][n][c] - ref);
+                s[mt][n][c + 2] = ex2(s[mt][n][c + 2] - ref);
+                l += s[mt][n][c] + s[mt][n][c + 2];
+            }
+            sum.l[n][c] = sum.l[n][c] * was + l;
+            if (!fresh) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    sum.o[i][n][c] *= was;
+                    sum.o[i][n][c + 2] *= was;
+                }
+            }
+        }
+        // The weights enter the second product as bfloat16 numbers (the sum above has them unrounded: at most 2^-9 each, as in the other kernels).
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+            p[mt][n][0] = transpose8x8(pack_bf16(s[mt][n][0], s[mt][n][1]));
+            p[mt][n][1] = transpose8x8(pack_bf16(s[mt][n][2], s[mt][n][3]));
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+        uint32_t v[4][NV];                                       // positions ta, tb of the first eight, of the second
+        const uint8_t* sc[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int t = mt * 16 + 8 * (u >> 1) + (u & 1 ? tb : ta);
+            load_words<NV>(tile + value_codes(D) + t * (D / 2) + value_byte<D>(t, r * (D / 16)), v[u]);
+            sc[u] = tile + value_scales(D) + t * (D / 8);
+        }
+        uint32_t a2[2], b2[2];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i == 0 || D == 192) {
+                uint32_t x[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    x[u] = *reinterpret_cast<const uint32_t*>(sc[u] + ((r * NV + i) >> 2) * 4);
+                    if (MASK) {                                  // (behind the sequence's end: anything may lie there; a value that is no number: see below)
+                        const int t = first + mt * 16 + 8 * (u >> 1) + (u & 1 ? tb : ta);
+                        if (t >= len || (several && no_number(x[u]))) x[u] = 0;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    a2[u] = low_halves(x[2 * u], x[2 * u + 1]);
+                    b2[u] = high_halves(x[2 * u], x[2 * u + 1]);
+                }
+            }
+            uint32_t e[4][2], o[4][2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                value_pair<0>(v[2 * u][i], v[2 * u + 1][i], a2[u], b2[u], e[0][u], o[0][u]);
+                value_pair<1>(v[2 * u][i], v[2 * u + 1][i], a2[u], b2[u], e[1][u], o[1][u]);
+                value_pair<2>(v[2 * u][i], v[2 * u + 1][i], a2[u], b2[u], e[2][u], o[2][u]);
+                value_pair<3>(v[2 * u][i], v[2 * u + 1][i], a2[u], b2[u], e[3][u], o[3][u]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816(sum.o[4 * i + k][n], e[k][0], o[k][0], e[k][1], o[k][1], p[mt][n][0], p[mt][n][1]);
+        }
+    }
+    if (MASK && several) {
+        // A value that is no number shows in the rows that see its position, and in no others (a weight of 0 would not hide it in the product).
+        const uint32_t* all = reinterpret_cast<const uint32_t*>(tile + value_scales(D));
+        bool any = false;
+        for (int i = lane; i < kPage * NW; i += 32) any |= first + i / NW < len && no_number(all[i]);
+        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll 1
+            for (int t = 0; t < kPage && first + t < len; ++t)
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (no_number(all[t * NW + ((r * NV + i) >> 2)]))
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                if (first + t <= w.limit[n][c])
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) sum.o[4 * i + k][n][c] = sum.o[4 * i + k][n][c + 2] = __int_as_float(0x7FFFFFFF);
+        }
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ void leaf_page(const Args& a, const uint8_t* tile, const Rows<NT>& w, const Seq& s, int page, bool fresh, Sum<NT>& sum) {
+    const int first = page * kPage;
+    if (first + kPage - 1 > s.start) page_step<NT, true>(tile, w, a.scale2, first, s.len, s.new_tokens > 1, fresh, sum);
+    else page_step<NT, false>(tile, w, a.scale2, first, s.len, false, fresh, sum);
+}
+
+// A leaf's sum over its positions: every lane gets its rows'.
+template <int NT> __device__ __forceinline__ void finish_leaf(Sum<NT>& sum) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) sum.l[n][c] += __shfl_xor_sync(0xffffffffu, sum.l[n][c], o);
+}
+
+// The fold of a leaf (or a node) p into what came before, each product and sum rounded on its own, so that it is the same wherever it is done:
+//   M' = max(M, m_p);  l = l 2^(M - M') + l_p 2^(m_p - M');  o likewise.
+struct Fold {
+    float m, l, was, now;
+    __device__ __forceinline__ void step(float mp, float lp) {
+        const float t = fmaxf(m, mp);
+        was = weight(m, t);
+        now = weight(mp, t);
+        l = __fadd_rn(__fmul_rn(l, was), __fmul_rn(lp, now));
+        m = t;
+    }
+    __device__ __forceinline__ float of(float o, float op) const { return __fadd_rn(__fmul_rn(o, was), __fmul_rn(op, now)); }
+};
+__device__ __forceinline__ float result(float o, float l) { return __fmul_rn(o, __fdiv_rn(1.0f, l)); }
+
+// ---- a block per node ---------------------------------------------------------------------
+template <int NT>
+__global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_kernel(const Args a) {
+    extern __shared__ __align__(128) uint8_t ring_all[];
+    __shared__ uint64_t full[LEAVES][2];
+    __shared__ float stat_m[LEAVES][8 * NT], stat_l[LEAVES][8 * NT];
+    __shared__ int abort_flag;
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
+    // (nodes innermost, then tiles, heads, sequences)
+    int64_t at = blockIdx.x;
+    const int node = (int)(at % a.nodes);
+    at /= a.nodes;
+    const int tile = (int)(at % a.tiles);
+    at /= a.tiles;
+    const int kvh = (int)(at % a.n_kv), b = (int)(at / a.n_kv);
+    const Seq s = sequence(a, b);
+    const int n_rows = s.new_tokens * a.group, row0 = tile * 8 * NT;
+    if (row0 >= n_rows || !fits(a, s)) return;
+    const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + 8 * NT, n_rows) - 1) / a.group;
+    const int seen = (s.start + last) / kPage + 1;               // pages that any row of the tile sees
+    const int first_page = node * LEAVES * lp;
+    if (first_page >= seen) return;
+    const int n_nodes = nodes_of(s.pages, a.n_kv);
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int w = 0; w < LEAVES; ++w) {
+            mbar_init(&full[w][0], 1);
+            mbar_init(&full[w][1], 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_wait();
+    const int p0 = first_page + warp * lp, count = max(0, min(seen, p0 + lp) - p0);
+    uint8_t* ring = ring_all + (size_t)warp * a.stages * TILE;
+    int ids = 0;
+    auto issue = [&](int k) {                                    // (in order; the lanes hold 32 page ids at a time)
+        if ((k & 31) == 0 && k + lane < count) ids = checked_page(a, a.page_table[(int64_t)b * a.table_width + p0 + k + lane]);
+        const int id = __shfl_sync(0xffffffffu, ids, k & 31);
+        if (lane == 0) start_copy(a, id, kvh, ring + (k % a.stages) * TILE, &full[warp][k % a.stages]);
+    };
+    for (int k = 0; k < min(a.stages, count); ++k) issue(k);
+    Sum<NT> sum;
+    sum.clear();
+    if (count > 0) {
+        Rows<NT> w;
+        load_rows<NT>(a, s, kvh, row0, w);
+#pragma unroll 1
+        for (int k = 0; k < count; ++k) {
+            if (!mbar_wait(&full[warp][k % a.stages], (k / a.stages) & 1, &abort_flag, a.status, 16)) {
+                // (what is on its way has to arrive before this block's shared memory is somebody else's; again with a limit)
+                for (int i = k; i < min(count, k + a.stages); ++i) {
+                    int mine = 0;
+                    mbar_wait(&full[warp][i % a.stages], (i / a.stages) & 1, &mine, a.status, 16);
+                }
+                break;
+            }
+            leaf_page<NT>(a, ring + (k % a.stages) * TILE, w, s, p0 + k, k == 0, sum);
+            __syncwarp();
+            if (k + a.stages < count) issue(k + a.stages);
+        }
+        finish_leaf<NT>(sum);
+    }
+    // The leaves meet: registers as they are, behind one another, in each warp's own part of the ring.
+    if (r == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                stat_m[warp][8 * n + 2 * j + c] = sum.m[n][c];
+                stat_l[warp][8 * n + 2 * j + c] = sum.l[n][c];
+            }
+    }
+    if (count > 0) {
+        float* mine = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mine[((i * NT + n) * 4 + e) * 32 + lane] = sum.o[i][n][e];
+    }
+    __syncthreads();
+    const int leaves = min(LEAVES, (seen - first_page + lp - 1) / lp);
+#pragma unroll 1
+    for (int u = warp; u < MT * NT; u += LEAVES) {
+        const int i = u / NT, n = u % NT;
+        Fold f[2];
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+        f[0].m = f[1].m = -INFINITY;
+        f[0].l = f[1].l = 0.f;
+        for (int p = 0; p < leaves; ++p) {
+            const float* theirs = reinterpret_cast<const float*>(ring_all + (size_t)p * a.stages * TILE) + u * 4 * 32 + lane;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                f[c].step(stat_m[p][8 * n + 2 * j + c], stat_l[p][8 * n + 2 * j + c]);
+                o[c] = f[c].of(o[c], theirs[c * 32]);
+                o[c + 2] = f[c].of(o[c + 2], theirs[(c + 2) * 32]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int row = row0 + 8 * n + 2 * j + c, tok = row / a.group;
+            if (row >= n_rows) continue;
+            const int64_t flat = (int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group);
+            const int ch = r * (D / 8) + 2 * i;
+            if (n_nodes == 1) {
+                *reinterpret_cast<uint32_t*>((bf16*)a.out + flat * D + ch) = pack_bf16(result(o[c], f[c].l), result(o[c + 2], f[c].l));
+            } else {
+                const int64_t rec = flat * a.nodes + node;
+                *reinterpret_cast<float2*>(a.rec + rec * D + ch) = make_float2(o[c], o[c + 2]);
+                if (i == 0 && r == 0) *reinterpret_cast<float2*>(a.rec + a.rec_rows * a.nodes * D + rec * 2) = make_float2(f[c].m, f[c].l);
+            }
+        }
+    }
+}
+
+// ---- joining the nodes ----------------------------------------------------------------------
+// A warp per row (a token's head): its records folded in order.  Sequences with one node have been written already.
+template <typename T>
+__global__ void __launch_bounds__(128) join_kernel(const Args a, const int* __restrict__ seq_of_token, int n_tokens) {
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= (int64_t)n_tokens * a.n_heads) return;
+    const int tok = (int)(row / a.n_heads), b = seq_of_token[tok];
+    if (b < 0 || b >= a.n_seqs) return;
+    const Seq s = sequence(a, b);
+    if (tok < s.first || tok >= s.first + s.new_tokens) return;  // (a token that fills the step up)
+    if (!fits(a, s) || nodes_of(s.pages, a.n_kv) < 2) return;
+    const int seen = (s.start + tok - s.first) / kPage + 1, per = LEAVES * leaf_pages(s.pages, a.n_kv), n = (seen + per - 1) / per;
+    pdl_wait();
+    const float* o_rec = fresh(a.rec) + row * a.nodes * D;
+    const float* m_rec = fresh(a.rec) + a.rec_rows * a.nodes * D + row * a.nodes * 2;
+    Fold f;
+    f.m = -INFINITY;
+    f.l = 0.f;
+    float2 o[D / 64];
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int p = 0; p < n; ++p) {
+        const float2 ml = *reinterpret_cast<const float2*>(m_rec + 2 * p);
+        f.step(ml.x, ml.y);
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) {
+            const float2 x = *reinterpret_cast<const float2*>(o_rec + (int64_t)p * D + 64 * e + 2 * lane);
+            o[e].x = f.of(o[e].x, x.x);
+            o[e].y = f.of(o[e].y, x.y);
+        }
+    }
+    T* dst = (T*)a.out + row * D;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+        st(dst + 64 * e + 2 * lane, result(o[e].x, f.l));
+        st(dst + 64 * e + 2 * lane + 1, result(o[e].y, f.l));
+    }
+}
+
+// ---- CUDA cores --------------------------------------------------------------------------------
+// A block per (node, tile of eight rows, key head, sequence); its warps take the node's pages in turn.  A lane computes the scores of two positions, then
+// sums D / 32 channels of all.  Queries and weights lie in shared memory; codes are read where they are.
+constexpr int PLAIN_WARPS = 4, PR = 8, CH = D / 32;
+
+template <typename T>
+__global__ void __launch_bounds__(PLAIN_WARPS * 32) plain_kernel(const Args a) {
+    __shared__ __align__(16) float ps[PLAIN_WARPS][kPage][PR];
+    __shared__ __align__(16) float so[PLAIN_WARPS][PR][D];       // (the queries while pages are read, then what the warps have summed)
+    __shared__ float sm[PLAIN_WARPS][PR], sl[PLAIN_WARPS][PR];
+    float (&qs)[PR][D] = so[0];
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t at = blockIdx.x;
+    const int node = (int)(at % a.nodes);
+    at /= a.nodes;
+    const int tile = (int)(at % a.tiles);
+    at /= a.tiles;
+    const int kvh = (int)(at % a.n_kv), b = (int)(at / a.n_kv);
+    const Seq s = sequence(a, b);
+    const int n_rows = s.new_tokens * a.group, row0 = tile * PR;
+    if (row0 >= n_rows || !fits(a, s)) return;
+    const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + PR, n_rows) - 1) / a.group;
+    const int seen = (s.start + last) / kPage + 1, first_page = node * LEAVES * lp;
+    if (first_page >= seen) return;
+    const int n_nodes = nodes_of(s.pages, a.n_kv);
+    pdl_wait();
+    for (int i = threadIdx.x; i < PR * D; i += PLAIN_WARPS * 32) {
+        const int row = row0 + i / D, tok = row / a.group;
+        qs[i / D][i % D] = row < n_rows ? ld((const T*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group)) * D + i % D) : 0.f;
+    }
+    __syncthreads();
+    float o[PR][CH], m[PR], l[PR];
+    int limit[PR];
+#pragma unroll
+    for (int u = 0; u < PR; ++u) {
+        m[u] = -INFINITY;
+        l[u] = 0.f;
+        limit[u] = s.start + min(row0 + u, n_rows - 1) / a.group;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) o[u][e] = 0.f;
+    }
+    const int stop = min(seen, first_page + LEAVES * lp);
+#pragma unroll 1
+    for (int page = first_page + warp; page < stop; page += PLAIN_WARPS) {
+        const int id = checked_page(a, a.page_table[(int64_t)b * a.table_width + page]), first = page * kPage;
+        const uint8_t* head = a.kv + ((int64_t)id * a.n_kv + kvh) * TILE;
+        float sc[PR][2];
+#pragma unroll
+        for (int u = 0; u < PR; ++u) sc[u][0] = sc[u][1] = 0.f;
+#pragma unroll 1
+        for (int w = 0; w < D / 8; ++w) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int t = lane + 32 * h;
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(head + key_scales(D) + (t * (D / GROUP) + w / 4) * 4);
+                uint32_t v[4];
+                key_word(*reinterpret_cast<const uint32_t*>(head + t * (D / 2) + 4 * w), low_halves(x, x), high_halves(x, x), v);
+                float k[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v[i]));
+                    k[i] = f.x;
+                    k[i + 4] = f.y;
+                }
+#pragma unroll
+                for (int u = 0; u < PR; ++u) {
+                    const float4 x0 = *reinterpret_cast<const float4*>(&qs[u][8 * w]), x1 = *reinterpret_cast<const float4*>(&qs[u][8 * w + 4]);
+                    sc[u][h] += x0.x * k[0] + x0.y * k[1] + x0.z * k[2] + x0.w * k[3] + x1.x * k[4] + x1.y * k[5] + x1.z * k[6] + x1.w * k[7];
+                }
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < PR; ++u) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                sc[u][h] = first + lane + 32 * h > limit[u] ? -INFINITY : sc[u][h] * a.scale2;
+                top = fmaxf(top, sc[u][h]);
+            }
+            const float mn = fmaxf(m[u], warp_max(top)), was = m[u] == -INFINITY ? 0.f : exp2f(m[u] - mn), ref = mn == -INFINITY ? 0.f : mn;
+            m[u] = mn;
+            const float e0 = exp2f(sc[u][0] - ref), e1 = exp2f(sc[u][1] - ref);
+            l[u] = l[u] * was + warp_sum(e0 + e1);
+            ps[warp][lane][u] = e0;
+            ps[warp][lane + 32][u] = e1;
+#pragma unroll
+            for (int e = 0; e < CH; ++e) o[u][e] *= was;
+        }
+        __syncwarp();
+        const int rows = min(kPage, s.len - first);
+#pragma unroll 1
+        for (int t = 0; t < rows; ++t) {
+            float v[CH];
+            uint32_t x = 0;
+#pragma unroll
+            for (int e = 0; e < CH; e += 2) {
+                // (six channels can lie in two groups)
+                if (e == 0 || D == 192) x = *reinterpret_cast<const uint32_t*>(head + value_scales(D) + (t * (D / GROUP) + (lane * CH + e) / GROUP) * 4);
+                const uint32_t byte = head[value_codes(D) + t * (D / 2) + value_byte<D>(t, (lane * CH + e) / 2)];
+                uint32_t even, odd;
+                value_pair<0>(byte, byte, low_halves(x, x), high_halves(x, x), even, odd);
+                v[e] = __uint_as_float(even << 16);
+                v[e + 1] = __uint_as_float(odd << 16);
+            }
+#pragma unroll
+            for (int u = 0; u < PR; ++u) {
+                const float p = ps[warp][t][u];
+                if (first + t <= limit[u])                       // (a value that is no number does not show in rows that do not see it)
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) o[u][e] += p * v[e];
+            }
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < PR; ++u) {
+#pragma unroll
+        for (int e = 0; e < CH; ++e) so[warp][u][lane * CH + e] = o[u][e];
+        if (lane == 0) {
+            sm[warp][u] = m[u];
+            sl[warp][u] = l[u];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < PR * D; i += PLAIN_WARPS * 32) {
+        const int u = i / D, ch = i % D, row = row0 + u, tok = row / a.group;
+        if (row >= n_rows) continue;
+        Fold f;
+        f.m = -INFINITY;
+        f.l = 0.f;
+        float x = 0.f;
+        for (int p = 0; p < PLAIN_WARPS; ++p) {
+            f.step(sm[p][u], sl[p][u]);
+            x = f.of(x, so[p][u][ch]);
+        }
+        const int64_t flat = (int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group);
+        if (n_nodes == 1) {
+            st((T*)a.out + flat * D + ch, result(x, f.l));
+        } else {
+            const int64_t rec = flat * a.nodes + node;
+            a.rec[rec * D + ch] = x;
+            if (ch == 0) *reinterpret_cast<float2*>(a.rec + a.rec_rows * a.nodes * D + rec * 2) = make_float2(f.m, f.l);
+        }
+    }
+}
+
+static int64_t scratch_floats(int n_tokens, int n_heads, int n_kv, int kv_bound) {
+    const int nodes = nodes_of((kv_bound + kPage - 1) / kPage, n_kv);
+    return nodes < 2 ? 0 : (int64_t)n_tokens * n_heads * nodes * (D + 2);
+}
+
+// form: 0 as the sizes say, 1 CUDA cores, 2 a block per node.
+template <typename T>
+static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pages, void* out, const int* cu_seqlens, int n_seqs, const int* start,
+                     const int* seq_of_token, const int* page_table, int table_width, int n_heads, int n_kv, int max_q, int kv_bound, float scale,
+                     float* scratch, int64_t scratch_size, int form, int* status, void* stream) {
+    WICK_REQUIRE(n_tokens >= 0 && n_seqs > 0 && n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && table_width > 0 && max_q >= 0 && kv_bound >= 0,
+                 "attention_kv4: bad sizes");
+    WICK_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "attention_kv4: arrays must begin on multiples of 16 bytes");
+    if (n_tokens == 0 || max_q == 0 || kv_bound == 0) return 0;
+    const int64_t need = scratch_floats(n_tokens, n_heads, n_kv, kv_bound);
+    WICK_REQUIRE(scratch_size >= need, "attention_kv4: scratch of %lld floats, %lld needed", (long long)scratch_size, (long long)need);
+    Args a;
+    a.q = q;
+    a.out = out;
+    a.kv = (const uint8_t*)kv;
+    a.kv_pages = kv_pages;
+    a.cu_seqlens = cu_seqlens;
+    a.start = start;
+    a.page_table = page_table;
+    a.table_width = table_width;
+    a.n_seqs = n_seqs;
+    a.n_tokens = n_tokens;
+    a.n_heads = n_heads;
+    a.n_kv = n_kv;
+    a.group = n_heads / n_kv;
+    a.scale2 = scale * 1.44269504088896340736f;
+    a.rec = scratch;
+    a.rec_rows = (int64_t)n_tokens * n_heads;
+    const int pages = (kv_bound + kPage - 1) / kPage;
+    a.nodes = nodes_of(pages, n_kv);
+    a.status = status;
+    const int64_t rows = (int64_t)max_q * a.group;
+    const bool plain = form == 1 || sizeof(T) == 4;
+    const int nt = rows > 8 ? 2 : 1;
+    a.tiles = (int)((rows + 8 * (plain ? 1 : nt) - 1) / (8 * (plain ? 1 : nt)));
+    a.stages = leaf_pages(pages, n_kv) > 1 ? MAX_STAGES : 1;
+    const int64_t blocks = (int64_t)n_seqs * n_kv * a.tiles * a.nodes;
+    WICK_REQUIRE(blocks < (1ll << 31), "attention_kv4: %lld blocks are beyond the grid's limit", (long long)blocks);
+    if (plain) {
+        WICK_CUDA(launch(plain_kernel<T>, dim3((unsigned)blocks), dim3(PLAIN_WARPS * 32), 0, (cudaStream_t)stream, a));
+    } else {
+        const size_t smem = (size_t)LEAVES * a.stages * TILE;
+        static bool raised[2] = {false, false};
+        if (!raised[nt - 1]) {
+            WICK_CUDA(cudaFuncSetAttribute(nt == 1 ? leaves_kernel<1> : leaves_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, LEAVES * MAX_STAGES * TILE));
+            raised[nt - 1] = true;
+        }
+        WICK_CUDA(launch(nt == 1 ? leaves_kernel<1> : leaves_kernel<2>, dim3((unsigned)blocks), dim3(THREADS), smem, (cudaStream_t)stream, a));
+    }
+    if (int rc = check_launch("attention_kv4")) return rc;
+    if (a.nodes > 1) {
+        WICK_CUDA(launch(join_kernel<T>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, (cudaStream_t)stream, a, seq_of_token, n_tokens));
+        return check_launch("attention_kv4 (join)");
+    }
+    return 0;
+}
+
+}  // namespace kv4
+}  // namespace wick
+
+using namespace wick;
+typedef __nv_bfloat16 bf16;
+
+// float32 words of scratch of a call of these sizes.
+WICK_API long long wick_attn_kv4_scratch(int n_tokens, int n_heads, int n_kv, int kv_bound) {
+    return n_kv > 0 && kv_bound >= 0 ? (long long)kv4::scratch_floats(n_tokens, n_heads, n_kv, kv_bound) : 0;
+}
+
+#define WICK_KV4_ATTENTION(NAME, T)                                                                                                                  \
+    WICK_API int NAME(const void* q, int n_tokens, const void* kv, int64_t kv_pages, void* out, const int* cu_seqlens, int n_seqs, const int* start, \
+                      const int* seq_of_token, const int* page_table, int table_width, int n_heads, int n_kv, int max_q, int kv_bound, float scale,  \
+                      float* scratch, int64_t scratch_size, int form, int* status, void* stream) {                                                  \
+        return kv4::attention<T>(q, n_tokens, kv, kv_pages, out, cu_seqlens, n_seqs, start, seq_of_token, page_table, table_width, n_heads, n_kv,    \
+                                 max_q, kv_bound, scale, scratch, scratch_size, form, status, stream);                                              \
+    }                                                                                                                                                \
+    WICK_PACKED(NAME)
+WICK_KV4_ATTENTION(wick_attn_kv4_bf16, bf16)
+WICK_KV4_ATTENTION(wick_attn_kv4_f32, float)

@@ -146,6 +146,8 @@ _STATUS_TEXT = {1: "gemm_tc gave up waiting for a free shared-memory stage", 2: 
                 12: "step_tables ran out of free pages",
                 13: "step_tables was given a record, a parent or a length outside its tables, or a fork that begins inside a page",
                 14: "step_tables was given more tokens than places for them",
+                15: "a 4-bit cache was given a position, a length or a page outside its page table or its cache",
+                16: "attention over a 4-bit cache gave up waiting for its bulk copies",
                 99: "the test kernel gave up waiting for nothing (nobody arrives on its barrier)"}
 
 
@@ -2195,3 +2197,8 @@ def wait_gives_up(limit_ms: float = 1.0) -> bool:
     flag = torch.zeros(1, dtype=torch.int32, device=st.device)
     _core().call("wick_wait_gives_up", "pilpp", _p(st), 99, int(limit_ms * 1e6), _p(flag), _stream())
     return bool(flag.item())
+
+
+# A cache in 4 bits, and the attention over it (ops/kv4.py).
+from .kv4 import (KV4_HEAD_DIMS, KV4_SOURCES, attention_kv4, attention_kv4_scratch, kv4_page_bytes, kv4_read,      # noqa: E402,F401
+                  qk_norm_rope_append_kv4)
