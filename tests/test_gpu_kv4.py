@@ -231,6 +231,19 @@ def test_attention(case, dtype):
     for plain in (True, False):
         out = o.attention_kv4(q, kv.cuda(), b, scale, plain=plain)
         check_attention(q, out, cache, b, scale, d)
+    if dtype == BF16:
+        # which kernel computes what changes no bit
+        want = o.attention_kv4(q, kv.cuda(), b, scale, kind="records")
+        check_attention(q, want, cache, b, scale, d)
+        for kind in ("clusters", "stay"):
+            try:
+                o.attention_kv4_scratch(b, H, KV, d, dtype, kind=kind)
+            except o.KernelError:
+                assert kind == "clusters" and max(starts) > 500 or kind == "stay" and max(new) * H // KV > 8
+                continue
+            assert torch.equal(o.attention_kv4(q, kv.cuda(), b, scale, kind=kind), want), kind
+        if d in (64, 128):
+            check_attention(q, o.attention_kv4(q, kv.cuda(), b, scale, kind="opened"), cache, b, scale, d)
     o.check_status()
 
 
@@ -243,7 +256,12 @@ def test_long_sequences(dtype):
         pages, b = step([length, 3], [1, 1], g)
         kv, cache = random_cache(pages, KV, 64, g)
         q = torch.randn((2, H, 64), generator=g).to(dtype).cuda()
-        check_attention(q, o.attention_kv4(q, kv.cuda(), b, 0.125, plain=dtype == F32), cache, b, 0.125, 64)
+        out = o.attention_kv4(q, kv.cuda(), b, 0.125)
+        check_attention(q, out, cache, b, 0.125, 64)
+        if dtype == BF16:
+            assert torch.equal(o.attention_kv4(q, kv.cuda(), b, 0.125, kind="records"), out)
+            if H // KV <= 8:
+                assert torch.equal(o.attention_kv4(q, kv.cuda(), b, 0.125, kind="stay"), out)
     o.check_status()
 
 
@@ -252,11 +270,12 @@ def test_alone_and_among_others(dtype):
     o = ops()
     g = torch.Generator().manual_seed(5)
     starts, new = [2000, 10, 700, 64, 5000, 0, 130], [1] * 7
+    starts, new = starts + [900 + 7 * i for i in range(83)], new + [1] * 83      # (together: blocks that stay)
     pages, b = step(starts, new, g)
     kv = random_cache(pages, 2, 128, g)[0].cuda()
-    q = torch.randn((7, 8, 128), generator=g).to(dtype).cuda()
+    q = torch.randn((90, 8, 128), generator=g).to(dtype).cuda()
     out = o.attention_kv4(q, kv, b, 0.09)
-    for i in range(7):
+    for i in list(range(7)) + [40, 89]:
         one = types.SimpleNamespace(**vars(b))
         one.n_seqs = one.n_tokens = 1
         one.q_lens, one.starts, one.kv_bound = [1], [starts[i]], starts[i] + 1
@@ -472,10 +491,13 @@ def test_refusals():
             o.attention_kv4(q, kv, broken, 0.1)
     with pytest.raises(o.KernelError):
         o.attention_kv4(q, kv, b, 0.1, out=q.float())
+    for bad in (q, q.float()):
+        with pytest.raises(o.KernelError):
+            o.attention_kv4(bad, kv, b, 0.1, kind="other" if bad is q else "stay")
     long_pages, long = step([700, 7], [1, 1], g)
     kv2 = random_cache(long_pages, 2, 64, g)[0].cuda()
     with pytest.raises(o.KernelError):
-        o.attention_kv4(q, kv2, long, 0.1, torch.empty(3, device="cuda"))
+        o.attention_kv4(q, kv2, long, 0.1, torch.empty(3, device="cuda"), kind="records")
     for bad in (kv[:, :, 1:], kv.view(pages, -1), kv.cpu()):
         with pytest.raises(o.KernelError):
             o.kv4_read(bad, 64, b.page_table, b.seq_of_token, b.positions)

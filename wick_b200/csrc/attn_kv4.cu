@@ -6,8 +6,13 @@
 // sixteen.  The sequence's pages are cut by its OWN length and the number of key heads alone: into leaves of as many pages (one, for up to 8 most_nodes
 // pages) and nodes of eight leaves.  A leaf is computed by one warp, page by page, into a running maximum, sum and accumulator; a node's leaves
 // are folded in order, a row's nodes likewise.  Which warp computes what changes no bit, so that a sequence's result does not depend on the batch it is
-// in.  The kernel for bfloat16 has a block per node and a warp per leaf; the leaves meet in shared memory.  Nodes leave records (accumulator, maximum, sum) that a
-// second, small kernel joins; a sequence with one node is written directly.
+// in.  Three forms for bfloat16 (Plan has the rule):
+//   * a block per node, a warp per leaf: the leaves meet in shared memory.  A sequence's nodes, where they are up to CLUSTER, are a cluster whose blocks
+//     read each other's results and write the outcome; more leave records (accumulator, maximum, sum) that a second, small kernel joins.  Few nodes:
+//     as many warps as there are leaves work on a sequence;
+//   * blocks that stay, one per SM, to whose warps all nodes of the step are dealt in equal runs: a warp folds a node's leaves in registers, and its next
+//     pages are on their way across the ends of its nodes.  Many nodes of one row tile each (decode steps); records as above.
+// A sequence with one node is written directly.
 //
 // The kernel on the tensor cores.  Keys and values stand on the 16-row side of mma.sync (16 positions, or 16 channels), the rows on the 8-column side, so
 // that the eight rows of most head layouts fill it.  A page of one key head (80 d bytes) comes in one bulk copy.  Values are made from codes in registers, in
@@ -37,6 +42,8 @@ constexpr int TILE = head_bytes(D);                              // a page of on
 constexpr int NW = D / 32;                                       // words of a key that a lane reads (its quarter of the row)
 constexpr int NV = D / 64;                                       // words of a value that a lane reads (its eighth)
 constexpr int MAX_STAGES = D <= 128 ? 2 : 1;                      // of a warp's ring (eight rings of two larger tiles are more than an SM has)
+constexpr int CLUSTER = 8;                                       // nodes that a cluster joins at most
+constexpr int MAX_SEQS = 1024;                                   // of the form whose blocks stay
 constexpr int MT = D / 16;                                       // tiles of 16 channels
 
 // Nodes of the longest sequences: enough that one sequence alone gives nearly every SM a block (8 key heads: 16), no more (each costs a record).
@@ -63,7 +70,7 @@ struct Args {
     const int* page_table;
     int table_width, n_seqs, n_heads, n_kv, group;
     float scale2;                                                // scale log2 e
-    int n_tokens;
+    int n_tokens, max_q;                                         // (max_q: the most new tokens of a sequence)
     float* rec;                                                  // records: accumulators [row, node, d], then maximum and sum [row, node, 2]; a row is a (token, head)
     int64_t rec_rows;
     int nodes;                                                   // places for nodes in a row's records
@@ -113,7 +120,7 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
 }
 // Whether a sequence fits the step, its page table and the records' places (else it is left out, and said).
 __device__ __forceinline__ bool fits(const Args& a, const Seq& s) {
-    const bool ok = s.start >= 0 && s.first >= 0 && s.first + s.new_tokens <= a.n_tokens && s.pages <= a.table_width && nodes_of(s.pages, a.n_kv) <= a.nodes;
+    const bool ok = s.start >= 0 && s.first >= 0 && s.first + s.new_tokens <= a.n_tokens && s.new_tokens <= a.max_q && s.pages <= a.table_width && nodes_of(s.pages, a.n_kv) <= a.nodes;
     if (!ok) atomicCAS(a.status, 0, 15);
     return ok;
 }
@@ -373,30 +380,64 @@ struct Fold {
 };
 __device__ __forceinline__ float result(float o, float l) { return __fmul_rn(o, __fdiv_rn(1.0f, l)); }
 
+// Row i of a tile's unit n (rows 8 n ..): where its token's head lies in the step, or -1.
+__device__ __forceinline__ int64_t flat_row(const Args& a, const Seq& s, int kvh, int row) {
+    if (row >= s.new_tokens * a.group) return -1;
+    const int tok = row / a.group;
+    return (int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group);
+}
+// A lane's four numbers of tile i (channels r d / 8 + 2 i and + 1 of rows 2 j and 2 j + 1): the result, or a node's record.
+__device__ __forceinline__ void write_result(const Args& a, int64_t flat, int ch, float x, float y, float l) {
+    *reinterpret_cast<uint32_t*>((bf16*)a.out + flat * D + ch) = pack_bf16(result(x, l), result(y, l));
+}
+__device__ __forceinline__ void write_record(const Args& a, int64_t flat, int node, int ch, float x, float y) {
+    *reinterpret_cast<float2*>(a.rec + (flat * a.nodes + node) * D + ch) = make_float2(x, y);
+}
+__device__ __forceinline__ void write_weights(const Args& a, int64_t flat, int node, float m, float l) {
+    *reinterpret_cast<float2*>(a.rec + a.rec_rows * a.nodes * D + (flat * a.nodes + node) * 2) = make_float2(m, l);
+}
+
 // ---- a block per node ---------------------------------------------------------------------
-template <int NT>
+__device__ __forceinline__ uint32_t in_block(uint32_t smem, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+constexpr int leaves_smem(int nt, int stages, bool clusters) { return LEAVES * stages * TILE + (clusters ? nt * 8 * D * 4 : 0); }
+
+// The grid: nodes innermost, then tiles, heads, sequences.  CLUSTERS: a sequence's nodes are a cluster.
+template <int NT, bool CLUSTERS>
 __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_kernel(const Args a) {
     extern __shared__ __align__(128) uint8_t ring_all[];
     __shared__ uint64_t full[LEAVES][2];
     __shared__ float stat_m[LEAVES][8 * NT], stat_l[LEAVES][8 * NT];
+    __shared__ float node_m[8 * NT], node_l[8 * NT];
     __shared__ int abort_flag;
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
-    // (nodes innermost, then tiles, heads, sequences)
-    int64_t at = blockIdx.x;
-    const int node = (int)(at % a.nodes);
-    at /= a.nodes;
-    const int tile = (int)(at % a.tiles);
-    at /= a.tiles;
-    const int kvh = (int)(at % a.n_kv), b = (int)(at / a.n_kv);
+    unsigned at = blockIdx.x;
+    const int node = (int)(at % (unsigned)a.nodes);
+    at /= (unsigned)a.nodes;
+    const int tile = (int)(at % (unsigned)a.tiles);
+    at /= (unsigned)a.tiles;
+    const int kvh = (int)(at % (unsigned)a.n_kv), b = (int)(at / (unsigned)a.n_kv);
     const Seq s = sequence(a, b);
     const int n_rows = s.new_tokens * a.group, row0 = tile * 8 * NT;
-    if (row0 >= n_rows || !fits(a, s)) return;
+    if (row0 >= n_rows || !fits(a, s)) return;                   // (so do all blocks of its cluster)
     const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + 8 * NT, n_rows) - 1) / a.group;
     const int seen = (s.start + last) / kPage + 1;               // pages that any row of the tile sees
     const int first_page = node * LEAVES * lp;
-    if (first_page >= seen) return;
-    const int n_nodes = nodes_of(s.pages, a.n_kv);
+    const bool work = first_page < seen;
+    if (!CLUSTERS && !work) return;
+    const int n_nodes = CLUSTERS ? (seen + LEAVES * lp - 1) / (LEAVES * lp) : nodes_of(s.pages, a.n_kv);
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int w = 0; w < LEAVES; ++w) {
@@ -457,37 +498,272 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
                 for (int e = 0; e < 4; ++e) mine[((i * NT + n) * 4 + e) * 32 + lane] = sum.o[i][n][e];
     }
     __syncthreads();
-    const int leaves = min(LEAVES, (seen - first_page + lp - 1) / lp);
+    const int leaves = work ? min(LEAVES, (seen - first_page + lp - 1) / lp) : 0;
+    float* rec = reinterpret_cast<float*>(ring_all + LEAVES * a.stages * TILE);
 #pragma unroll 1
-    for (int u = warp; u < MT * NT; u += LEAVES) {
+    for (int u = warp; work && u < MT * NT; u += LEAVES) {
         const int i = u / NT, n = u % NT;
-        Fold f[2];
+        // Lane (p, j) has the fold's step of leaf p for rows 2 j, 2 j + 1: the maxima so far by a scan over the leaves.
+        float was[2], now[2], m[2], l[2] = {0.f, 0.f}, lp_[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const float mine = r < leaves ? stat_m[r][8 * n + 2 * j + c] : -INFINITY;
+            lp_[c] = r < leaves ? stat_l[r][8 * n + 2 * j + c] : 0.f;
+            float upto = mine;
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                const float t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto = fmaxf(upto, t);
+            }
+            float before = __shfl_up_sync(0xffffffffu, upto, 4);
+            if (r == 0) before = -INFINITY;
+            was[c] = weight(before, upto);
+            now[c] = weight(mine, upto);
+            m[c] = __shfl_sync(0xffffffffu, upto, 28 + j);
+        }
         float o[4] = {0.f, 0.f, 0.f, 0.f};
-        f[0].m = f[1].m = -INFINITY;
-        f[0].l = f[1].l = 0.f;
+#pragma unroll 4
         for (int p = 0; p < leaves; ++p) {
             const float* theirs = reinterpret_cast<const float*>(ring_all + (size_t)p * a.stages * TILE) + u * 4 * 32 + lane;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                f[c].step(stat_m[p][8 * n + 2 * j + c], stat_l[p][8 * n + 2 * j + c]);
-                o[c] = f[c].of(o[c], theirs[c * 32]);
-                o[c + 2] = f[c].of(o[c + 2], theirs[(c + 2) * 32]);
+                Fold f;
+                f.was = __shfl_sync(0xffffffffu, was[c], 4 * p + j);
+                f.now = __shfl_sync(0xffffffffu, now[c], 4 * p + j);
+                l[c] = f.of(l[c], __shfl_sync(0xffffffffu, lp_[c], 4 * p + j));
+                o[c] = f.of(o[c], theirs[c * 32]);
+                o[c + 2] = f.of(o[c + 2], theirs[(c + 2) * 32]);
+            }
+        }
+        if (CLUSTERS && n_nodes > 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rec[(u * 4 + e) * 32 + lane] = o[e];
+            if (i == 0 && r == 0) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    node_m[8 * n + 2 * j + c] = m[c];
+                    node_l[8 * n + 2 * j + c] = l[c];
+                }
+            }
+            continue;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int64_t flat = flat_row(a, s, kvh, row0 + 8 * n + 2 * j + c);
+            if (flat < 0) continue;
+            const int ch = r * (D / 8) + 2 * i;
+            if (n_nodes == 1) {
+                write_result(a, flat, ch, o[c], o[c + 2], l[c]);
+            } else {
+                write_record(a, flat, node, ch, o[c], o[c + 2]);
+                if (i == 0 && r == 0) write_weights(a, flat, node, m[c], l[c]);
+            }
+        }
+    }
+    if constexpr (CLUSTERS) {
+        if (n_nodes == 1) return;                                // (all blocks of the cluster know)
+        // The nodes meet: unit u is joined by warp u / nodes of block u % nodes, out of all blocks' shared memory, in the nodes' order.
+        cluster_sync();
+#pragma unroll 1
+        for (int u = warp * a.nodes + node; u < MT * NT; u += LEAVES * a.nodes) {
+            const int i = u / NT, n = u % NT;
+            Fold f[2];
+            float o[4] = {0.f, 0.f, 0.f, 0.f};
+            f[0].m = f[1].m = -INFINITY;
+            f[0].l = f[1].l = 0.f;
+#pragma unroll 4
+            for (int p = 0; p < n_nodes; ++p) {
+                const uint32_t theirs = in_block(smem_u32(rec + u * 4 * 32 + lane), p);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    f[c].step(ld_cluster(in_block(smem_u32(&node_m[8 * n + 2 * j + c]), p)), ld_cluster(in_block(smem_u32(&node_l[8 * n + 2 * j + c]), p)));
+                    o[c] = f[c].of(o[c], ld_cluster(theirs + c * 128));
+                    o[c + 2] = f[c].of(o[c + 2], ld_cluster(theirs + (c + 2) * 128));
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int64_t flat = flat_row(a, s, kvh, row0 + 8 * n + 2 * j + c);
+                if (flat >= 0) write_result(a, flat, r * (D / 8) + 2 * i, o[c], o[c + 2], f[c].l);
+            }
+        }
+        cluster_sync();                                          // (nobody leaves while others read)
+    }
+}
+
+// ---- blocks that stay ------------------------------------------------------------------------
+// One row tile a sequence and key head (one new token, up to eight heads).
+struct Node {
+    int u;                                                       // its number among all of the step
+    int b, kvh, node, nodes, lp;
+    int page, end;                                               // of the sequence
+};
+
+__global__ void __launch_bounds__(THREADS, 1) nodes_kernel(const Args a) {
+    extern __shared__ __align__(128) uint8_t ring_all[];
+    __shared__ uint64_t full[LEAVES][MAX_STAGES];
+    __shared__ int cum[MAX_SEQS + 1], lens[MAX_SEQS], firsts[MAX_SEQS];      // nodes before a sequence; its length (with a new token) and the token
+    __shared__ int abort_flag;
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int w = 0; w < LEAVES; ++w)
+            for (int i = 0; i < MAX_STAGES; ++i) mbar_init(&full[w][i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        int before = 0;
+#pragma unroll 1
+        for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+            const int b = s0 + lane;
+            int mine = 0;
+            if (b < a.n_seqs) {
+                const Seq s = sequence(a, b);
+                if (s.new_tokens > 0 && fits(a, s)) mine = nodes_of(s.pages, a.n_kv) * a.n_kv;
+                lens[b] = s.len;
+                firsts[b] = s.first;
+            }
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += t;
+            }
+            if (b < a.n_seqs) cum[b + 1] = before + upto;
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) cum[0] = 0;
+    }
+    __syncthreads();
+    const int64_t U = cum[a.n_seqs], S = (int64_t)gridDim.x * LEAVES, slot = (int64_t)warp * gridDim.x + blockIdx.x;
+    const int u0 = (int)(slot * U / S), u1 = (int)((slot + 1) * U / S);
+    pdl_wait();
+    if (u0 >= u1) return;
+    uint8_t* ring = ring_all + (size_t)warp * MAX_STAGES * TILE;
+
+    auto open = [&](Node& n) {                                   // (nodes are visited in order: b only moves forward)
+        while (n.u >= cum[n.b + 1]) ++n.b;
+        const int pages = (lens[n.b] + kPage - 1) / kPage, local = n.u - cum[n.b];
+        n.lp = leaf_pages(pages, a.n_kv);
+        n.nodes = (pages + LEAVES * n.lp - 1) / (LEAVES * n.lp);
+        n.kvh = local / n.nodes;
+        n.node = local - n.kvh * n.nodes;
+        n.page = n.node * LEAVES * n.lp;
+        n.end = min(pages, n.page + LEAVES * n.lp);
+    };
+    auto page_ids = [&](const Node& n) {
+        return n.page + lane < n.end ? checked_page(a, a.page_table[(int64_t)n.b * a.table_width + n.page + lane]) : 0;
+    };
+    Node cn;                                                     // the node that is computed
+    {
+        int lo = 0, hi = a.n_seqs - 1;                           // the sequence of node u0: the last b with cum[b] <= u0
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (cum[mid] <= u0) lo = mid;
+            else hi = mid - 1;
+        }
+        cn.u = u0;
+        cn.b = lo;
+        open(cn);
+    }
+    // Copies run ahead, page by page.  The lanes hold the ids of up to 32 of a node's pages; those of the next node are asked for while this one's
+    // pages are copied.
+    Node pn = cn, nn = cn;
+    int ids = page_ids(pn), next_ids = 0, held = 0, issued = 0;
+    auto peek = [&]() {
+        if (nn.u + 1 >= u1) return;
+        ++nn.u;
+        open(nn);
+        next_ids = page_ids(nn);
+    };
+    auto issue = [&]() {
+        if (pn.page >= pn.end) {
+            if (pn.u + 1 >= u1) return;
+            pn = nn;
+            ids = next_ids;
+            held = 0;
+            peek();
+        } else if (held == 32) {
+            ids = page_ids(pn);
+            held = 0;
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, held), stage = issued % MAX_STAGES;
+        if (lane == 0) start_copy(a, id, pn.kvh, ring + stage * TILE, &full[warp][stage]);
+        ++held;
+        ++pn.page;
+        ++issued;
+    };
+    peek();
+#pragma unroll
+    for (int k = 0; k < MAX_STAGES; ++k) issue();
+
+    Rows<1> w;
+    int rows_of = -1, done = 0;
+    Seq s;
+#pragma unroll 1
+    while (true) {
+        if (cn.b * a.n_kv + cn.kvh != rows_of) {
+            rows_of = cn.b * a.n_kv + cn.kvh;
+            s.first = firsts[cn.b];
+            s.new_tokens = 1;
+            s.len = lens[cn.b];
+            s.start = s.len - 1;
+            s.pages = (s.len + kPage - 1) / kPage;
+            load_rows<1>(a, s, cn.kvh, 0, w);
+        }
+        Fold f[2];
+        float o[MT][4];
+        f[0].m = f[1].m = -INFINITY;
+        f[0].l = f[1].l = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll 1
+        for (int page = cn.page; page < cn.end;) {
+            Sum<1> sum;
+            sum.clear();
+            const int stop = min(cn.end, page + cn.lp);
+            bool fresh = true;
+#pragma unroll 1
+            for (; page < stop; ++page) {
+                const int stage = done % MAX_STAGES;
+                if (!mbar_wait(&full[warp][stage], (done / MAX_STAGES) & 1, &abort_flag, a.status, 16)) {
+                    for (; done < issued; ++done) {              // (as above)
+                        int mine = 0;
+                        mbar_wait(&full[warp][done % MAX_STAGES], (done / MAX_STAGES) & 1, &mine, a.status, 16);
+                    }
+                    return;
+                }
+                leaf_page<1>(a, ring + stage * TILE, w, s, page, fresh, sum);
+                fresh = false;
+                __syncwarp();
+                ++done;
+                issue();
+            }
+            finish_leaf<1>(sum);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                f[c].step(sum.m[0][c], sum.l[0][c]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    o[i][c] = f[c].of(o[i][c], sum.o[i][0][c]);
+                    o[i][c + 2] = f[c].of(o[i][c + 2], sum.o[i][0][c + 2]);
+                }
             }
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const int row = row0 + 8 * n + 2 * j + c, tok = row / a.group;
-            if (row >= n_rows) continue;
-            const int64_t flat = (int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group);
-            const int ch = r * (D / 8) + 2 * i;
-            if (n_nodes == 1) {
-                *reinterpret_cast<uint32_t*>((bf16*)a.out + flat * D + ch) = pack_bf16(result(o[c], f[c].l), result(o[c + 2], f[c].l));
-            } else {
-                const int64_t rec = flat * a.nodes + node;
-                *reinterpret_cast<float2*>(a.rec + rec * D + ch) = make_float2(o[c], o[c + 2]);
-                if (i == 0 && r == 0) *reinterpret_cast<float2*>(a.rec + a.rec_rows * a.nodes * D + rec * 2) = make_float2(f[c].m, f[c].l);
+            const int64_t flat = flat_row(a, s, cn.kvh, 2 * j + c);
+            if (flat < 0) continue;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if (cn.nodes == 1) write_result(a, flat, r * (D / 8) + 2 * i, o[i][c], o[i][c + 2], f[c].l);
+                else write_record(a, flat, cn.node, r * (D / 8) + 2 * i, o[i][c], o[i][c + 2]);
             }
+            if (cn.nodes > 1 && r == 0) write_weights(a, flat, cn.node, f[c].m, f[c].l);
         }
+        if (++cn.u >= u1) break;
+        open(cn);
     }
 }
 
@@ -682,12 +958,47 @@ __global__ void __launch_bounds__(PLAIN_WARPS * 32) plain_kernel(const Args a) {
     }
 }
 
-static int64_t scratch_floats(int n_tokens, int n_heads, int n_kv, int kv_bound) {
-    const int nodes = nodes_of((kv_bound + kPage - 1) / kPage, n_kv);
-    return nodes < 2 ? 0 : (int64_t)n_tokens * n_heads * nodes * (D + 2);
+// Which kernels a call of these sizes launches, and what they need.
+enum Form { AUTO = 0, PLAIN = 1, RECORDS = 2, CLUSTERS = 3, STAY = 4 };
+struct Plan {
+    bool possible;
+    int form, nt, tiles, nodes, stages, kernels;
+    int64_t scratch, blocks;
+};
+static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int kv_bound, bool f32, int form) {
+    Plan p = {};
+    const int pages = (kv_bound + kPage - 1) / kPage;
+    const int64_t rows = (int64_t)max_q * (n_heads / n_kv);
+    p.nodes = nodes_of(pages, n_kv);
+    p.form = f32 && form == AUTO ? PLAIN : form;
+    const bool can_stay = rows <= 8 && n_seqs <= MAX_SEQS;
+    p.possible = p.form >= AUTO && p.form <= STAY && !(f32 && p.form != PLAIN) && !(p.form == STAY && !can_stay) && !(p.form == CLUSTERS && p.nodes > CLUSTER);
+    if (p.form == AUTO)
+        p.form = can_stay && (int64_t)n_seqs * n_kv * p.nodes >= 2 * (int64_t)LEAVES * sm_count() ? STAY : (p.nodes <= CLUSTER ? CLUSTERS : RECORDS);
+    p.nt = p.form != PLAIN && rows > 8 ? 2 : 1;
+    p.tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
+    p.stages = p.form == STAY || leaf_pages(pages, n_kv) > 1 ? MAX_STAGES : 1;
+    p.blocks = p.form == STAY ? sm_count() : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
+    const bool records = p.nodes > 1 && p.form != CLUSTERS;
+    p.scratch = records ? (int64_t)n_tokens * n_heads * p.nodes * (D + 2) : 0;
+    p.kernels = records ? 2 : 1;
+    return p;
 }
 
-// form: 0 as the sizes say, 1 CUDA cores, 2 a block per node.
+// Dynamic shared memory beyond what a kernel has without asking.
+static int allow(void (*kernel)(Args), int bytes) {
+    static void (*asked[8])(Args) = {};                          // (two host threads may both ask: it does no harm)
+    for (int i = 0; i < 8; ++i) {
+        if (asked[i] == kernel) return 0;
+        if (asked[i] == nullptr) {
+            WICK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+            asked[i] = kernel;
+            return 0;
+        }
+    }
+    return 0;
+}
+
 template <typename T>
 static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pages, void* out, const int* cu_seqlens, int n_seqs, const int* start,
                      const int* seq_of_token, const int* page_table, int table_width, int n_heads, int n_kv, int max_q, int kv_bound, float scale,
@@ -696,8 +1007,10 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
                  "attention_kv4: bad sizes");
     WICK_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "attention_kv4: arrays must begin on multiples of 16 bytes");
     if (n_tokens == 0 || max_q == 0 || kv_bound == 0) return 0;
-    const int64_t need = scratch_floats(n_tokens, n_heads, n_kv, kv_bound);
-    WICK_REQUIRE(scratch_size >= need, "attention_kv4: scratch of %lld floats, %lld needed", (long long)scratch_size, (long long)need);
+    const Plan p = plan(n_tokens, n_seqs, n_heads, n_kv, max_q, kv_bound, sizeof(T) == 4, form);
+    WICK_REQUIRE(p.possible, "attention_kv4: the kernel asked for (%d) does not take these sizes", form);
+    WICK_REQUIRE(scratch_size >= p.scratch, "attention_kv4: scratch of %lld floats, %lld needed", (long long)scratch_size, (long long)p.scratch);
+    WICK_REQUIRE(p.blocks < (1ll << 31), "attention_kv4: %lld blocks are beyond the grid's limit", (long long)p.blocks);
     Args a;
     a.q = q;
     a.out = out;
@@ -709,36 +1022,47 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     a.table_width = table_width;
     a.n_seqs = n_seqs;
     a.n_tokens = n_tokens;
+    a.max_q = max_q;
     a.n_heads = n_heads;
     a.n_kv = n_kv;
     a.group = n_heads / n_kv;
     a.scale2 = scale * 1.44269504088896340736f;
     a.rec = scratch;
     a.rec_rows = (int64_t)n_tokens * n_heads;
-    const int pages = (kv_bound + kPage - 1) / kPage;
-    a.nodes = nodes_of(pages, n_kv);
+    a.nodes = p.nodes;
+    a.tiles = p.tiles;
+    a.stages = p.stages;
     a.status = status;
-    const int64_t rows = (int64_t)max_q * a.group;
-    const bool plain = form == 1 || sizeof(T) == 4;
-    const int nt = rows > 8 ? 2 : 1;
-    a.tiles = (int)((rows + 8 * (plain ? 1 : nt) - 1) / (8 * (plain ? 1 : nt)));
-    a.stages = leaf_pages(pages, n_kv) > 1 ? MAX_STAGES : 1;
-    const int64_t blocks = (int64_t)n_seqs * n_kv * a.tiles * a.nodes;
-    WICK_REQUIRE(blocks < (1ll << 31), "attention_kv4: %lld blocks are beyond the grid's limit", (long long)blocks);
-    if (plain) {
-        WICK_CUDA(launch(plain_kernel<T>, dim3((unsigned)blocks), dim3(PLAIN_WARPS * 32), 0, (cudaStream_t)stream, a));
+    const cudaStream_t st = (cudaStream_t)stream;
+    const dim3 grid((unsigned)p.blocks);
+    if (p.form == PLAIN) {
+        WICK_CUDA(launch(plain_kernel<T>, grid, dim3(PLAIN_WARPS * 32), 0, st, a));
+    } else if (p.form == STAY) {
+        const int smem = LEAVES * MAX_STAGES * TILE;
+        if (int rc = allow(nodes_kernel, smem)) return rc;
+        WICK_CUDA(launch(nodes_kernel, grid, dim3(THREADS), smem, st, a));
     } else {
-        const size_t smem = (size_t)LEAVES * a.stages * TILE;
-        static bool raised[2] = {false, false};
-        if (!raised[nt - 1]) {
-            WICK_CUDA(cudaFuncSetAttribute(nt == 1 ? leaves_kernel<1> : leaves_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, LEAVES * MAX_STAGES * TILE));
-            raised[nt - 1] = true;
-        }
-        WICK_CUDA(launch(nt == 1 ? leaves_kernel<1> : leaves_kernel<2>, dim3((unsigned)blocks), dim3(THREADS), smem, (cudaStream_t)stream, a));
+        const bool clusters = p.form == CLUSTERS && p.nodes > 1;
+        void (*kernel)(Args) = p.nt == 1 ? (clusters ? leaves_kernel<1, true> : leaves_kernel<1, false>) : (clusters ? leaves_kernel<2, true> : leaves_kernel<2, false>);
+        if (int rc = allow(kernel, leaves_smem(p.nt, MAX_STAGES, true))) return rc;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = leaves_smem(p.nt, p.stages, clusters);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = clusters ? p.nodes : 1;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_enabled() ? 2 : 1;
+        WICK_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
     }
     if (int rc = check_launch("attention_kv4")) return rc;
-    if (a.nodes > 1) {
-        WICK_CUDA(launch(join_kernel<T>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, (cudaStream_t)stream, a, seq_of_token, n_tokens));
+    if (p.kernels == 2) {
+        WICK_CUDA(launch(join_kernel<T>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, st, a, seq_of_token, n_tokens));
         return check_launch("attention_kv4 (join)");
     }
     return 0;
@@ -750,9 +1074,19 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
 using namespace wick;
 typedef __nv_bfloat16 bf16;
 
-// float32 words of scratch of a call of these sizes.
-WICK_API long long wick_attn_kv4_scratch(int n_tokens, int n_heads, int n_kv, int kv_bound) {
-    return n_kv > 0 && kv_bound >= 0 ? (long long)kv4::scratch_floats(n_tokens, n_heads, n_kv, kv_bound) : 0;
+// float32 words of scratch of a call of these sizes, and the kernels that it launches.  form: 0 as the sizes say, or one of Form where it is possible.
+WICK_API long long wick_attn_kv4_scratch(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int kv_bound, int f32, int form, int* kernels) {
+    if (n_seqs < 1 || n_heads < 1 || n_kv < 1 || n_heads % n_kv || max_q < 0 || kv_bound < 0) {
+        fail("attention_kv4: bad sizes");
+        return -1;
+    }
+    const kv4::Plan p = kv4::plan(n_tokens, n_seqs, n_heads, n_kv, max_q, kv_bound, f32 != 0, form);
+    if (!p.possible) {
+        fail("attention_kv4: the kernel asked for (%d) does not take these sizes", form);
+        return -1;
+    }
+    *kernels = p.kernels;
+    return (long long)p.scratch;
 }
 
 #define WICK_KV4_ATTENTION(NAME, T)                                                                                                                  \

@@ -78,8 +78,9 @@ __device__ __forceinline__ void encode(const double (&x)[8], unsigned mask, bool
         hi = fmax(hi, __shfl_xor_sync(mask, hi, o));
         bad |= __shfl_xor_sync(mask, (int)bad, o) != 0;
     }
-    bf16 a = __double2bfloat16((hi - lo) * (16.0 / 15.0));
-    bf16 b = __double2bfloat16(lo - (double)__bfloat162float(a));
+    // (to bfloat16 by way of 32 bits, as conversions from 64 bits go elsewhere)
+    bf16 a = __float2bfloat16_rn((float)((hi - lo) * (16.0 / 15.0)));
+    bf16 b = __float2bfloat16_rn((float)(lo - (double)__bfloat162float(a)));
     // (2^127: so that no value that a code stands for is infinite either)
     if (bad || fmax(fabs(lo), fabs(hi)) > 0x1p127 || !isfinite(__bfloat162float(a))) {
         a = __float2bfloat16_rn(0.f);
