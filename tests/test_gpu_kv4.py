@@ -235,11 +235,11 @@ def test_attention(case, dtype):
         # which kernel computes what changes no bit
         want = o.attention_kv4(q, kv.cuda(), b, scale, kind="records")
         check_attention(q, want, cache, b, scale, d)
-        for kind in ("clusters", "stay"):
+        for kind in ("clusters", "stay", "stay_leaves"):
             try:
                 o.attention_kv4_scratch(b, H, KV, d, dtype, kind=kind)
             except o.KernelError:
-                assert kind == "clusters" and max(starts) > 500 or kind == "stay" and max(new) * H // KV > 8
+                assert kind == "clusters" and max(starts) > 500 or "stay" in kind and max(new) * H // KV > 8
                 continue
             assert torch.equal(o.attention_kv4(q, kv.cuda(), b, scale, kind=kind), want), kind
         if d in (64, 128):
@@ -261,7 +261,8 @@ def test_long_sequences(dtype):
         if dtype == BF16:
             assert torch.equal(o.attention_kv4(q, kv.cuda(), b, 0.125, kind="records"), out)
             if H // KV <= 8:
-                assert torch.equal(o.attention_kv4(q, kv.cuda(), b, 0.125, kind="stay"), out)
+                for kind in ("stay", "stay_leaves"):
+                    assert torch.equal(o.attention_kv4(q, kv.cuda(), b, 0.125, kind=kind), out)
     o.check_status()
 
 
@@ -318,6 +319,18 @@ def test_what_is_not_seen_does_not_show(new, d):
         want[new[0] - 1, :2] = True
         for plain in (False, True):
             assert torch.equal(o.attention_kv4(q, kv.cuda(), b, 0.1, plain=plain).isnan(), want)
+
+
+@pytest.mark.parametrize("scale", [-0.07, 0.0])
+def test_scales(scale):
+    """A negative scale turns the order of the scores around, one of 0 weighs all alike."""
+    o = ops()
+    g = torch.Generator().manual_seed(8)
+    pages, b = step([100, 700, 0], [1, 1, 1], g)
+    kv, cache = random_cache(pages, 2, 128, g)
+    q = torch.randn((3, 8, 128), generator=g).to(BF16).cuda()
+    for kind in ("plain", "records", "clusters", "stay", "stay_leaves"):
+        check_attention(q, o.attention_kv4(q, kv.cuda(), b, scale, kind=kind if kind != "clusters" else None), cache, b, scale, 128)
 
 
 def test_rows_behind_the_last_sequence_stay():

@@ -10,8 +10,8 @@
 //   * a block per node, a warp per leaf: the leaves meet in shared memory.  A sequence's nodes, where they are up to CLUSTER, are a cluster whose blocks
 //     read each other's results and write the outcome; more leave records (accumulator, maximum, sum) that a second, small kernel joins.  Few nodes:
 //     as many warps as there are leaves work on a sequence;
-//   * blocks that stay, one per SM, to whose warps all nodes of the step are dealt in equal runs: a warp folds a node's leaves in registers, and its next
-//     pages are on their way across the ends of its nodes.  Many nodes of one row tile each (decode steps); records as above.
+//   * blocks that stay, one per SM, with an equal run of all nodes (or leaves) of the step each, which their warps take one by one: a warp folds a node's
+//     leaves in registers, and its next page is on its way while it computes one.  Many nodes of one row tile each (decode steps); records as above.
 // A sequence with one node is written directly.
 //
 // The kernel on the tensor cores.  Keys and values stand on the 16-row side of mma.sync (16 positions, or 16 channels), the rows on the 8-column side, so
@@ -42,6 +42,7 @@ constexpr int TILE = head_bytes(D);                              // a page of on
 constexpr int NW = D / 32;                                       // words of a key that a lane reads (its quarter of the row)
 constexpr int NV = D / 64;                                       // words of a value that a lane reads (its eighth)
 constexpr int MAX_STAGES = D <= 128 ? 2 : 1;                      // of a warp's ring (eight rings of two larger tiles are more than an SM has)
+constexpr int STAY_WARPS = D == 64 ? 16 : (D == 128 ? 12 : 8);   // of a block that stays (as many as registers allow)
 constexpr int CLUSTER = 8;                                       // nodes that a cluster joins at most
 constexpr int MAX_SEQS = 1024;                                   // of the form whose blocks stay
 constexpr int MT = D / 16;                                       // tiles of 16 channels
@@ -69,8 +70,9 @@ struct Args {
     const int* start;
     const int* page_table;
     int table_width, n_seqs, n_heads, n_kv, group;
-    float scale2;                                                // scale log2 e
-    int n_tokens, max_q;                                         // (max_q: the most new tokens of a sequence)
+    float scale2;                                                // |scale| log2 e
+    uint32_t flip;                                               // sign bits of two bfloat16 numbers if the scale is negative (the queries then change sign), else 0
+    int n_tokens, max_q, pages;                                  // the most new tokens of a sequence, and the most pages that there are places for
     float* rec;                                                  // records: accumulators [row, node, d], then maximum and sum [row, node, 2]; a row is a (token, head)
     int64_t rec_rows;
     int nodes;                                                   // places for nodes in a row's records
@@ -120,7 +122,7 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
 }
 // Whether a sequence fits the step, its page table and the records' places (else it is left out, and said).
 __device__ __forceinline__ bool fits(const Args& a, const Seq& s) {
-    const bool ok = s.start >= 0 && s.first >= 0 && s.first + s.new_tokens <= a.n_tokens && s.new_tokens <= a.max_q && s.pages <= a.table_width && nodes_of(s.pages, a.n_kv) <= a.nodes;
+    const bool ok = s.start >= 0 && s.first >= 0 && s.first + s.new_tokens <= a.n_tokens && s.new_tokens <= a.max_q && s.pages <= a.table_width && s.pages <= a.pages;
     if (!ok) atomicCAS(a.status, 0, 15);
     return ok;
 }
@@ -156,25 +158,34 @@ template <int NT> struct Rows {
     uint32_t q[2 * NW][NT][2];                                   // the second operand of the scores, channels in the order of the keys' codes
     int limit[NT][2];                                            // the last position that rows 2 j, 2 j + 1 see
 };
+__device__ __forceinline__ uint4 flipped(uint4 x, uint32_t flip) { return make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip); }
 
-// Rows row0 .. of a (sequence, key head): row i is head i % group of new token i / group.
+// Rows row0 .. of a (sequence, key head): row i is head i % group of new token i / group.  As they are in memory: a lane has its quarter of row r.
+__device__ __forceinline__ void load_row(const Args& a, const Seq& s, int kvh, int row, uint4 (&x)[NW]) {
+    const int j = threadIdx.x & 3, tok = row / a.group, g = row - tok * a.group;
+    const uint4* src = reinterpret_cast<const uint4*>((const bf16*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + g) * D + 8 * j * NW);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) x[i] = row < s.new_tokens * a.group ? src[i] : make_uint4(0, 0, 0, 0);
+}
+template <int NT>
+__device__ __forceinline__ void order_row(const Args& a, const uint4 (&x)[NW], int n, Rows<NT>& w) {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        const uint4 y = flipped(x[i], a.flip);
+        w.q[2 * i][n][0] = low_halves(y.x, y.z);
+        w.q[2 * i][n][1] = high_halves(y.x, y.z);
+        w.q[2 * i + 1][n][0] = low_halves(y.y, y.w);
+        w.q[2 * i + 1][n][1] = high_halves(y.y, y.w);
+    }
+}
 template <int NT>
 __device__ __forceinline__ void load_rows(const Args& a, const Seq& s, int kvh, int row0, Rows<NT>& w) {
     const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, n_rows = s.new_tokens * a.group;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int row = row0 + 8 * n + r;
-        const int tok = row / a.group, g = row - tok * a.group;
-        const uint4* src = reinterpret_cast<const uint4*>((const bf16*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + g) * D + 8 * j * NW);
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (row < n_rows) x = src[i];
-            w.q[2 * i][n][0] = low_halves(x.x, x.z);
-            w.q[2 * i][n][1] = high_halves(x.x, x.z);
-            w.q[2 * i + 1][n][0] = low_halves(x.y, x.w);
-            w.q[2 * i + 1][n][1] = high_halves(x.y, x.w);
-        }
+        uint4 x[NW];
+        load_row(a, s, kvh, row0 + 8 * n + r, x);
+        order_row<NT>(a, x, n, w);
 #pragma unroll
         for (int c = 0; c < 2; ++c) w.limit[n][c] = s.start + min(row0 + 8 * n + 2 * j + c, n_rows - 1) / a.group;
     }
@@ -200,9 +211,11 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, ui
 }
 
 // One page (in shared memory) into a leaf.  MASK: some of its positions are not seen by some row; first: the position of the page's first row, len: the
-// sequence's length; several: rows of several tokens.  fresh: the leaf's first page.
-template <int NT, bool MASK>
-__device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w, float scale2, int first, int len, bool several, bool fresh, Sum<NT>& sum) {
+// sequence's length; several: rows of several tokens.  fresh: the leaf's first page.  between: what is to be done when the keys have been read and before
+// the values are.
+template <int NT, bool MASK, typename Between>
+__device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w, float scale2, int first, int len, bool several, bool fresh, Sum<NT>& sum,
+                                          Between between) {
     const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
     const int tr = position_of(r), ta = position_of(2 * j), tb = position_of(2 * j + 1);
     float s[4][NT][4];
@@ -239,7 +252,8 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
             }
         }
     }
-    // scores in units of log2 e, the running maximum, weights
+    between();
+    // the running maximum in units of log2 e, weights
     uint32_t p[4][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -248,24 +262,26 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float x = s[mt][n][e] * scale2;
-                if (MASK && first + mt * 16 + 8 * (e >> 1) + tr > w.limit[n][e & 1]) x = -INFINITY;
-                s[mt][n][e] = x;
-                top[e & 1] = fmaxf(top[e & 1], x);
+                if (MASK && first + mt * 16 + 8 * (e >> 1) + tr > w.limit[n][e & 1]) s[mt][n][e] = -INFINITY;
+                top[e & 1] = fmaxf(top[e & 1], s[mt][n][e]);
             }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-            const float m = fmaxf(sum.m[n][c], top[c]), was = weight(sum.m[n][c], m);
+            const float m = fmaxf(sum.m[n][c], top[c] == -INFINITY ? top[c] : top[c] * scale2), was = weight(sum.m[n][c], m);
             const float ref = m == -INFINITY ? 0.f : m;          // (nothing seen: weights 0; a score that is no number still shows)
             sum.m[n][c] = m;
             float l = 0.f;
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-                s[mt][n][c] = ex2(s[mt][n][c] - ref);
-                s[mt][n][c + 2] = ex2(s[mt][n][c + 2] - ref);
-                l += s[mt][n][c] + s[mt][n][c + 2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float& x = s[mt][n][c + 2 * h];
+                    const float y = ex2(fmaf(x, scale2, -ref));
+                    x = MASK && x == -INFINITY ? 0.f : y;        // (a scale of 0 and nothing else makes a difference)
+                    l += x;
+                }
             }
             sum.l[n][c] = sum.l[n][c] * was + l;
             if (!fresh) {
@@ -348,11 +364,15 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
     }
 }
 
-template <int NT>
-__device__ __forceinline__ void leaf_page(const Args& a, const uint8_t* tile, const Rows<NT>& w, const Seq& s, int page, bool fresh, Sum<NT>& sum) {
+struct Nothing {
+    __device__ __forceinline__ void operator()() const {}
+};
+template <int NT, typename Between = Nothing>
+__device__ __forceinline__ void leaf_page(const Args& a, const uint8_t* tile, const Rows<NT>& w, const Seq& s, int page, bool fresh, Sum<NT>& sum,
+                                          Between between = Nothing()) {
     const int first = page * kPage;
-    if (first + kPage - 1 > s.start) page_step<NT, true>(tile, w, a.scale2, first, s.len, s.new_tokens > 1, fresh, sum);
-    else page_step<NT, false>(tile, w, a.scale2, first, s.len, false, fresh, sum);
+    if (first + kPage - 1 > s.start) page_step<NT, true>(tile, w, a.scale2, first, s.len, s.new_tokens > 1, fresh, sum, between);
+    else page_step<NT, false>(tile, w, a.scale2, first, s.len, false, fresh, sum, between);
 }
 
 // A leaf's sum over its positions: every lane gets its rows'.
@@ -365,7 +385,7 @@ template <int NT> __device__ __forceinline__ void finish_leaf(Sum<NT>& sum) {
             for (int o = 4; o < 32; o <<= 1) sum.l[n][c] += __shfl_xor_sync(0xffffffffu, sum.l[n][c], o);
 }
 
-// The fold of a leaf (or a node) p into what came before, each product and sum rounded on its own, so that it is the same wherever it is done:
+// The fold of a leaf (or a node) p into what came before, the same operations wherever it is done:
 //   M' = max(M, m_p);  l = l 2^(M - M') + l_p 2^(m_p - M');  o likewise.
 struct Fold {
     float m, l, was, now;
@@ -373,10 +393,10 @@ struct Fold {
         const float t = fmaxf(m, mp);
         was = weight(m, t);
         now = weight(mp, t);
-        l = __fadd_rn(__fmul_rn(l, was), __fmul_rn(lp, now));
+        l = of(l, lp);
         m = t;
     }
-    __device__ __forceinline__ float of(float o, float op) const { return __fadd_rn(__fmul_rn(o, was), __fmul_rn(op, now)); }
+    __device__ __forceinline__ float of(float o, float op) const { return __fmaf_rn(op, now, __fmul_rn(o, was)); }
 };
 __device__ __forceinline__ float result(float o, float l) { return __fmul_rn(o, __fdiv_rn(1.0f, l)); }
 
@@ -435,8 +455,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
     const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + 8 * NT, n_rows) - 1) / a.group;
     const int seen = (s.start + last) / kPage + 1;               // pages that any row of the tile sees
     const int first_page = node * LEAVES * lp;
-    const bool work = first_page < seen;
-    if (!CLUSTERS && !work) return;
+    if (first_page >= seen) return;                                          // (a cluster does not wait for blocks that have left)
     const int n_nodes = CLUSTERS ? (seen + LEAVES * lp - 1) / (LEAVES * lp) : nodes_of(s.pages, a.n_kv);
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -498,10 +517,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
                 for (int e = 0; e < 4; ++e) mine[((i * NT + n) * 4 + e) * 32 + lane] = sum.o[i][n][e];
     }
     __syncthreads();
-    const int leaves = work ? min(LEAVES, (seen - first_page + lp - 1) / lp) : 0;
+    const int leaves = min(LEAVES, (seen - first_page + lp - 1) / lp);
     float* rec = reinterpret_cast<float*>(ring_all + LEAVES * a.stages * TILE);
 #pragma unroll 1
-    for (int u = warp; work && u < MT * NT; u += LEAVES) {
+    for (int u = warp; u < MT * NT; u += LEAVES) {
         const int i = u / NT, n = u % NT;
         // Lane (p, j) has the fold's step of leaf p for rows 2 j, 2 j + 1: the maxima so far by a scan over the leaves.
         float was[2], now[2], m[2], l[2] = {0.f, 0.f}, lp_[2];
@@ -562,10 +581,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
     }
     if constexpr (CLUSTERS) {
         if (n_nodes == 1) return;                                // (all blocks of the cluster know)
-        // The nodes meet: unit u is joined by warp u / nodes of block u % nodes, out of all blocks' shared memory, in the nodes' order.
+        // The nodes meet: the tiles of 16 channels are shared out among the blocks' warps, and joined out of all blocks' shared memory, in the nodes' order.
         cluster_sync();
 #pragma unroll 1
-        for (int u = warp * a.nodes + node; u < MT * NT; u += LEAVES * a.nodes) {
+        for (int u = warp * n_nodes + node; u < MT * NT; u += LEAVES * n_nodes) {
             const int i = u / NT, n = u % NT;
             Fold f[2];
             float o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -592,24 +611,29 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
 }
 
 // ---- blocks that stay ------------------------------------------------------------------------
-// One row tile a sequence and key head (one new token, up to eight heads).
-struct Node {
-    int u;                                                       // its number among all of the step
-    int b, kvh, node, nodes, lp;
+// One row tile a sequence and key head (one new token, up to eight heads).  A block has an equal run of the step's nodes (BY_LEAF: of its leaves), and its
+// warps take the next one whenever they are done with one.  A warp's tile is filled again while it is read: the next page's keys as soon as the scores are
+// there, its values when the page is done.
+struct Item {
+    int b, kvh, place, nodes, lp;                                // place: the node's number in the sequence (BY_LEAF: the leaf's); none left: b < 0
     int page, end;                                               // of the sequence
 };
 
-__global__ void __launch_bounds__(THREADS, 1) nodes_kernel(const Args a) {
+template <bool BY_LEAF>
+__global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) {
     extern __shared__ __align__(128) uint8_t ring_all[];
-    __shared__ uint64_t full[LEAVES][MAX_STAGES];
-    __shared__ int cum[MAX_SEQS + 1], lens[MAX_SEQS], firsts[MAX_SEQS];      // nodes before a sequence; its length (with a new token) and the token
-    __shared__ int abort_flag;
+    __shared__ uint64_t full[STAY_WARPS][2];                     // keys, values
+    __shared__ int cum[MAX_SEQS + 1], lens[MAX_SEQS], firsts[MAX_SEQS];      // items before a sequence; its length (with a new token) and the token
+    __shared__ int abort_flag, taken;
+    constexpr int PER = BY_LEAF ? 1 : LEAVES;                    // leaves of an item
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int w = 0; w < LEAVES; ++w)
-            for (int i = 0; i < MAX_STAGES; ++i) mbar_init(&full[w][i], 1);
+        for (int w = 0; w < STAY_WARPS; ++w) {
+            mbar_init(&full[w][0], 1);
+            mbar_init(&full[w][1], 1);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -620,7 +644,10 @@ __global__ void __launch_bounds__(THREADS, 1) nodes_kernel(const Args a) {
             int mine = 0;
             if (b < a.n_seqs) {
                 const Seq s = sequence(a, b);
-                if (s.new_tokens > 0 && fits(a, s)) mine = nodes_of(s.pages, a.n_kv) * a.n_kv;
+                if (s.new_tokens > 0 && fits(a, s)) {
+                    const int lp = PER * leaf_pages(s.pages, a.n_kv);
+                    mine = (s.pages + lp - 1) / lp * a.n_kv;
+                }
                 lens[b] = s.len;
                 firsts[b] = s.first;
             }
@@ -633,112 +660,120 @@ __global__ void __launch_bounds__(THREADS, 1) nodes_kernel(const Args a) {
             if (b < a.n_seqs) cum[b + 1] = before + upto;
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (lane == 0) cum[0] = 0;
+        if (lane == 0) {
+            cum[0] = 0;
+            taken = (int)((int64_t)blockIdx.x * before / gridDim.x);
+        }
     }
     __syncthreads();
-    const int64_t U = cum[a.n_seqs], S = (int64_t)gridDim.x * LEAVES, slot = (int64_t)warp * gridDim.x + blockIdx.x;
-    const int u0 = (int)(slot * U / S), u1 = (int)((slot + 1) * U / S);
+    const int stop = (int)((int64_t)(blockIdx.x + 1) * cum[a.n_seqs] / gridDim.x);
     pdl_wait();
-    if (u0 >= u1) return;
-    uint8_t* ring = ring_all + (size_t)warp * MAX_STAGES * TILE;
+    uint8_t* tile = ring_all + (size_t)warp * TILE;
 
-    auto open = [&](Node& n) {                                   // (nodes are visited in order: b only moves forward)
-        while (n.u >= cum[n.b + 1]) ++n.b;
-        const int pages = (lens[n.b] + kPage - 1) / kPage, local = n.u - cum[n.b];
-        n.lp = leaf_pages(pages, a.n_kv);
-        n.nodes = (pages + LEAVES * n.lp - 1) / (LEAVES * n.lp);
-        n.kvh = local / n.nodes;
-        n.node = local - n.kvh * n.nodes;
-        n.page = n.node * LEAVES * n.lp;
-        n.end = min(pages, n.page + LEAVES * n.lp);
-    };
-    auto page_ids = [&](const Node& n) {
-        return n.page + lane < n.end ? checked_page(a, a.page_table[(int64_t)n.b * a.table_width + n.page + lane]) : 0;
-    };
-    Node cn;                                                     // the node that is computed
-    {
-        int lo = 0, hi = a.n_seqs - 1;                           // the sequence of node u0: the last b with cum[b] <= u0
+    auto take = [&](Item& n, int& ids) {
+        int u = 0;
+        if (lane == 0) u = atomicAdd(&taken, 1);
+        u = __shfl_sync(0xffffffffu, u, 0);
+        n.b = -1;
+        if (u >= stop) return;
+        int lo = 0, hi = a.n_seqs - 1;                           // the last sequence with cum[b] <= u
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (cum[mid] <= u0) lo = mid;
+            if (cum[mid] <= u) lo = mid;
             else hi = mid - 1;
         }
-        cn.u = u0;
-        cn.b = lo;
-        open(cn);
-    }
-    // Copies run ahead, page by page.  The lanes hold the ids of up to 32 of a node's pages; those of the next node are asked for while this one's
-    // pages are copied.
-    Node pn = cn, nn = cn;
-    int ids = page_ids(pn), next_ids = 0, held = 0, issued = 0;
-    auto peek = [&]() {
-        if (nn.u + 1 >= u1) return;
-        ++nn.u;
-        open(nn);
-        next_ids = page_ids(nn);
+        n.b = lo;
+        const int pages = (lens[lo] + kPage - 1) / kPage, local = u - cum[lo];
+        n.lp = leaf_pages(pages, a.n_kv);
+        const int items = (pages + PER * n.lp - 1) / (PER * n.lp);
+        n.nodes = (pages + LEAVES * n.lp - 1) / (LEAVES * n.lp);
+        n.kvh = local / items;
+        n.place = local - n.kvh * items;
+        n.page = n.place * PER * n.lp;
+        n.end = min(pages, n.page + PER * n.lp);
+        ids = n.page + lane < n.end ? checked_page(a, a.page_table[(int64_t)lo * a.table_width + n.page + lane]) : 0;
     };
-    auto issue = [&]() {
-        if (pn.page >= pn.end) {
-            if (pn.u + 1 >= u1) return;
-            pn = nn;
-            ids = next_ids;
-            held = 0;
-            peek();
-        } else if (held == 32) {
-            ids = page_ids(pn);
-            held = 0;
+    auto start_half = [&](int id, int kvh, int half) {           // keys or values of a page: their codes and their scales
+        if (lane == 0) {
+            const uint8_t* src = a.kv + ((int64_t)id * a.n_kv + kvh) * TILE;
+            mbar_expect_tx(&full[warp][half], TILE / 2);
+            bulk_load(tile + half * value_codes(D), src + half * value_codes(D), 32 * D, &full[warp][half]);
+            bulk_load(tile + key_scales(D) + half * 8 * D, src + key_scales(D) + half * 8 * D, 8 * D, &full[warp][half]);
         }
-        const int id = __shfl_sync(0xffffffffu, ids, held), stage = issued % MAX_STAGES;
-        if (lane == 0) start_copy(a, id, pn.kvh, ring + stage * TILE, &full[warp][stage]);
-        ++held;
-        ++pn.page;
-        ++issued;
     };
-    peek();
-#pragma unroll
-    for (int k = 0; k < MAX_STAGES; ++k) issue();
-
-    Rows<1> w;
-    int rows_of = -1, done = 0;
+    Item cn, nn;                                                 // the item that is computed, and the next one
+    int ids = 0, next_ids = 0, parity = 0;
+    take(cn, ids);
+    if (cn.b < 0) return;
+    {
+        const int id = __shfl_sync(0xffffffffu, ids, 0);
+        start_half(id, cn.kvh, 0);
+        start_half(id, cn.kvh, 1);
+    }
     Seq s;
+    s.new_tokens = 1;
+    s.first = firsts[cn.b];
+    uint4 raw[NW];
+    load_row(a, s, cn.kvh, r, raw);
+    bool ok = true;
 #pragma unroll 1
     while (true) {
-        if (cn.b * a.n_kv + cn.kvh != rows_of) {
-            rows_of = cn.b * a.n_kv + cn.kvh;
-            s.first = firsts[cn.b];
-            s.new_tokens = 1;
-            s.len = lens[cn.b];
-            s.start = s.len - 1;
-            s.pages = (s.len + kPage - 1) / kPage;
-            load_rows<1>(a, s, cn.kvh, 0, w);
-        }
+        s.len = lens[cn.b];
+        s.start = s.len - 1;
+        s.first = firsts[cn.b];
+        Rows<1> w;
+        order_row<1>(a, raw, 0, w);
+        w.limit[0][0] = w.limit[0][1] = s.start;
+        take(nn, next_ids);
         Fold f[2];
         float o[MT][4];
         f[0].m = f[1].m = -INFINITY;
         f[0].l = f[1].l = 0.f;
 #pragma unroll
         for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        int held = 0;                                            // of the 32 ids that the lanes have
 #pragma unroll 1
         for (int page = cn.page; page < cn.end;) {
             Sum<1> sum;
             sum.clear();
-            const int stop = min(cn.end, page + cn.lp);
+            const int leaf_end = min(cn.end, page + cn.lp);
             bool fresh = true;
 #pragma unroll 1
-            for (; page < stop; ++page) {
-                const int stage = done % MAX_STAGES;
-                if (!mbar_wait(&full[warp][stage], (done / MAX_STAGES) & 1, &abort_flag, a.status, 16)) {
-                    for (; done < issued; ++done) {              // (as above)
+            for (; page < leaf_end; ++page) {
+                int next_id = -1, next_kvh = cn.kvh;
+                ok = ok && mbar_wait(&full[warp][0], parity, &abort_flag, a.status, 16);
+                leaf_page<1>(a, tile, w, s, page, fresh, sum, [&]() {
+                    if (page + 1 < cn.end) {
+                        if (++held == 32) {
+                            held = 0;
+                            ids = page + 1 + lane < cn.end ? checked_page(a, a.page_table[(int64_t)cn.b * a.table_width + page + 1 + lane]) : 0;
+                        }
+                        next_id = __shfl_sync(0xffffffffu, ids, held);
+                    } else if (nn.b >= 0) {
+                        next_id = __shfl_sync(0xffffffffu, next_ids, 0);
+                        next_kvh = nn.kvh;
+                    }
+                    __syncwarp();
+                    if (next_id >= 0) start_half(next_id, next_kvh, 0);
+                    if (page + 1 == cn.end && nn.b >= 0) {       // (the queries are not needed any more: the next item's are asked for)
+                        Seq t;
+                        t.new_tokens = 1;
+                        t.first = firsts[nn.b];
+                        load_row(a, t, nn.kvh, r, raw);
+                    }
+                    ok = mbar_wait(&full[warp][1], parity, &abort_flag, a.status, 16) && ok;
+                });
+                fresh = false;
+                parity ^= 1;
+                __syncwarp();
+                if (next_id >= 0) start_half(next_id, next_kvh, 1);
+                if (!ok) {                                       // (what is on its way has to arrive before this shared memory is somebody else's)
+                    for (int h = 0; h < 2 && next_id >= 0; ++h) {
                         int mine = 0;
-                        mbar_wait(&full[warp][done % MAX_STAGES], (done / MAX_STAGES) & 1, &mine, a.status, 16);
+                        mbar_wait(&full[warp][h], parity, &mine, a.status, 16);
                     }
                     return;
                 }
-                leaf_page<1>(a, ring + stage * TILE, w, s, page, fresh, sum);
-                fresh = false;
-                __syncwarp();
-                ++done;
-                issue();
             }
             finish_leaf<1>(sum);
 #pragma unroll
@@ -751,25 +786,28 @@ __global__ void __launch_bounds__(THREADS, 1) nodes_kernel(const Args a) {
                 }
             }
         }
+        const bool whole = cn.end - cn.page == (s.len + kPage - 1) / kPage;      // (the item is all of the sequence)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const int64_t flat = flat_row(a, s, cn.kvh, 2 * j + c);
+            const int64_t flat = 2 * j + c < a.group ? (int64_t)s.first * a.n_heads + cn.kvh * a.group + 2 * j + c : -1;
             if (flat < 0) continue;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                if (cn.nodes == 1) write_result(a, flat, r * (D / 8) + 2 * i, o[i][c], o[i][c + 2], f[c].l);
-                else write_record(a, flat, cn.node, r * (D / 8) + 2 * i, o[i][c], o[i][c + 2]);
+                if (whole) write_result(a, flat, r * (D / 8) + 2 * i, o[i][c], o[i][c + 2], f[c].l);
+                else write_record(a, flat, cn.place, r * (D / 8) + 2 * i, o[i][c], o[i][c + 2]);
             }
-            if (cn.nodes > 1 && r == 0) write_weights(a, flat, cn.node, f[c].m, f[c].l);
+            if (!whole && r == 0) write_weights(a, flat, cn.place, f[c].m, f[c].l);
         }
-        if (++cn.u >= u1) break;
-        open(cn);
+        if (nn.b < 0) return;
+        cn = nn;
+        ids = next_ids;
     }
 }
 
 // ---- joining the nodes ----------------------------------------------------------------------
-// A warp per row (a token's head): its records folded in order.  Sequences with one node have been written already.
-template <typename T>
+// A warp per row (a token's head): its records folded in order.  BY_LEAF: records of leaves, folded to nodes first.  Sequences with one node (leaf) have
+// been written already.
+template <typename T, bool BY_LEAF>
 __global__ void __launch_bounds__(128) join_kernel(const Args a, const int* __restrict__ seq_of_token, int n_tokens) {
     pdl_trigger();
     const int lane = threadIdx.x & 31;
@@ -779,26 +817,46 @@ __global__ void __launch_bounds__(128) join_kernel(const Args a, const int* __re
     if (b < 0 || b >= a.n_seqs) return;
     const Seq s = sequence(a, b);
     if (tok < s.first || tok >= s.first + s.new_tokens) return;  // (a token that fills the step up)
-    if (!fits(a, s) || nodes_of(s.pages, a.n_kv) < 2) return;
-    const int seen = (s.start + tok - s.first) / kPage + 1, per = LEAVES * leaf_pages(s.pages, a.n_kv), n = (seen + per - 1) / per;
+    if (!fits(a, s)) return;
+    const int seen = (s.start + tok - s.first) / kPage + 1, per = (BY_LEAF ? 1 : LEAVES) * leaf_pages(s.pages, a.n_kv), n = (seen + per - 1) / per;
+    if (s.pages <= per) return;
     pdl_wait();
     const float* o_rec = fresh(a.rec) + row * a.nodes * D;
     const float* m_rec = fresh(a.rec) + a.rec_rows * a.nodes * D + row * a.nodes * 2;
-    Fold f;
-    f.m = -INFINITY;
-    f.l = 0.f;
-    float2 o[D / 64];
+    Fold f, g;
+    g.m = f.m = -INFINITY;
+    g.l = f.l = 0.f;
+    float2 o[D / 64], x[D / 64];
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int p = 0; p < n; ++p) {
-        const float2 ml = *reinterpret_cast<const float2*>(m_rec + 2 * p);
-        f.step(ml.x, ml.y);
+    for (int e = 0; e < D / 64; ++e) x[e] = o[e] = make_float2(0.f, 0.f);
+    auto fold = [](Fold& t, float2 (&into)[D / 64], float m, float l, const float2 (&y)[D / 64]) {
+        t.step(m, l);
 #pragma unroll
         for (int e = 0; e < D / 64; ++e) {
-            const float2 x = *reinterpret_cast<const float2*>(o_rec + (int64_t)p * D + 64 * e + 2 * lane);
-            o[e].x = f.of(o[e].x, x.x);
-            o[e].y = f.of(o[e].y, x.y);
+            into[e].x = t.of(into[e].x, y[e].x);
+            into[e].y = t.of(into[e].y, y[e].y);
+        }
+    };
+#pragma unroll 1
+    for (int p0 = 0; p0 < n; p0 += LEAVES) {                     // (a node's leaves, or eight nodes: asked for together)
+        float2 ml[LEAVES], y[LEAVES][D / 64];
+#pragma unroll
+        for (int p = 0; p < LEAVES; ++p) {
+            if (p0 + p < n) {
+                ml[p] = *reinterpret_cast<const float2*>(m_rec + 2 * (p0 + p));
+#pragma unroll
+                for (int e = 0; e < D / 64; ++e) y[p][e] = *reinterpret_cast<const float2*>(o_rec + (int64_t)(p0 + p) * D + 64 * e + 2 * lane);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < LEAVES; ++p)
+            if (p0 + p < n) fold(BY_LEAF ? g : f, BY_LEAF ? x : o, ml[p].x, ml[p].y, y[p]);
+        if (BY_LEAF) {
+            fold(f, o, g.m, g.l, x);
+            g.m = -INFINITY;
+            g.l = 0.f;
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) x[e] = make_float2(0.f, 0.f);
         }
     }
     T* dst = (T*)a.out + row * D;
@@ -887,7 +945,7 @@ __global__ void __launch_bounds__(PLAIN_WARPS * 32) plain_kernel(const Args a) {
             float top = -INFINITY;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                sc[u][h] = first + lane + 32 * h > limit[u] ? -INFINITY : sc[u][h] * a.scale2;
+                sc[u][h] = first + lane + 32 * h > limit[u] ? -INFINITY : sc[u][h] * (a.flip ? -a.scale2 : a.scale2);
                 top = fmaxf(top, sc[u][h]);
             }
             const float mn = fmaxf(m[u], warp_max(top)), was = m[u] == -INFINITY ? 0.f : exp2f(m[u] - mn), ref = mn == -INFINITY ? 0.f : mn;
@@ -959,7 +1017,7 @@ __global__ void __launch_bounds__(PLAIN_WARPS * 32) plain_kernel(const Args a) {
 }
 
 // Which kernels a call of these sizes launches, and what they need.
-enum Form { AUTO = 0, PLAIN = 1, RECORDS = 2, CLUSTERS = 3, STAY = 4 };
+enum Form { AUTO = 0, PLAIN = 1, RECORDS = 2, CLUSTERS = 3, STAY = 4, STAY_LEAVES = 5 };
 struct Plan {
     bool possible;
     int form, nt, tiles, nodes, stages, kernels;
@@ -972,13 +1030,14 @@ static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int
     p.nodes = nodes_of(pages, n_kv);
     p.form = f32 && form == AUTO ? PLAIN : form;
     const bool can_stay = rows <= 8 && n_seqs <= MAX_SEQS;
-    p.possible = p.form >= AUTO && p.form <= STAY && !(f32 && p.form != PLAIN) && !(p.form == STAY && !can_stay) && !(p.form == CLUSTERS && p.nodes > CLUSTER);
+    p.possible = p.form >= AUTO && p.form <= STAY_LEAVES && !(f32 && p.form != PLAIN) && !(p.form >= STAY && !can_stay) && !(p.form == CLUSTERS && p.nodes > CLUSTER);
     if (p.form == AUTO)
         p.form = can_stay && (int64_t)n_seqs * n_kv * p.nodes >= 2 * (int64_t)LEAVES * sm_count() ? STAY : (p.nodes <= CLUSTER ? CLUSTERS : RECORDS);
     p.nt = p.form != PLAIN && rows > 8 ? 2 : 1;
     p.tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-    p.stages = p.form == STAY || leaf_pages(pages, n_kv) > 1 ? MAX_STAGES : 1;
-    p.blocks = p.form == STAY ? sm_count() : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
+    p.stages = leaf_pages(pages, n_kv) > 1 ? MAX_STAGES : 1;
+    if (p.form == STAY_LEAVES) p.nodes = (pages + leaf_pages(pages, n_kv) - 1) / leaf_pages(pages, n_kv);      // (places for records)
+    p.blocks = p.form >= STAY ? sm_count() : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
     const bool records = p.nodes > 1 && p.form != CLUSTERS;
     p.scratch = records ? (int64_t)n_tokens * n_heads * p.nodes * (D + 2) : 0;
     p.kernels = records ? 2 : 1;
@@ -1023,10 +1082,12 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     a.n_seqs = n_seqs;
     a.n_tokens = n_tokens;
     a.max_q = max_q;
+    a.pages = (kv_bound + kPage - 1) / kPage;
     a.n_heads = n_heads;
     a.n_kv = n_kv;
     a.group = n_heads / n_kv;
-    a.scale2 = scale * 1.44269504088896340736f;
+    a.scale2 = fabsf(scale) * 1.44269504088896340736f;
+    a.flip = scale < 0.f ? 0x80008000u : 0u;
     a.rec = scratch;
     a.rec_rows = (int64_t)n_tokens * n_heads;
     a.nodes = p.nodes;
@@ -1037,10 +1098,10 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     const dim3 grid((unsigned)p.blocks);
     if (p.form == PLAIN) {
         WICK_CUDA(launch(plain_kernel<T>, grid, dim3(PLAIN_WARPS * 32), 0, st, a));
-    } else if (p.form == STAY) {
-        const int smem = LEAVES * MAX_STAGES * TILE;
-        if (int rc = allow(nodes_kernel, smem)) return rc;
-        WICK_CUDA(launch(nodes_kernel, grid, dim3(THREADS), smem, st, a));
+    } else if (p.form >= STAY) {
+        void (*kernel)(Args) = p.form == STAY ? stay_kernel<false> : stay_kernel<true>;
+        if (int rc = allow(kernel, STAY_WARPS * TILE)) return rc;
+        WICK_CUDA(launch(kernel, grid, dim3(STAY_WARPS * 32), STAY_WARPS * TILE, st, a));
     } else {
         const bool clusters = p.form == CLUSTERS && p.nodes > 1;
         void (*kernel)(Args) = p.nt == 1 ? (clusters ? leaves_kernel<1, true> : leaves_kernel<1, false>) : (clusters ? leaves_kernel<2, true> : leaves_kernel<2, false>);
@@ -1062,7 +1123,7 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     }
     if (int rc = check_launch("attention_kv4")) return rc;
     if (p.kernels == 2) {
-        WICK_CUDA(launch(join_kernel<T>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, st, a, seq_of_token, n_tokens));
+        WICK_CUDA(launch(p.form == STAY_LEAVES ? join_kernel<T, true> : join_kernel<T, false>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, st, a, seq_of_token, n_tokens));
         return check_launch("attention_kv4 (join)");
     }
     return 0;

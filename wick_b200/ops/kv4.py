@@ -166,7 +166,7 @@ OPEN_ROWS = 32
 
 
 # The kernels of attention_kv4 by name (csrc/attn_kv4.cu: Plan); "opened": pages opened to bfloat16, then the prompt attention.
-_FORMS = {None: 0, "plain": 1, "records": 2, "clusters": 3, "stay": 4, "opened": -1}
+_FORMS = {None: 0, "plain": 1, "records": 2, "clusters": 3, "stay": 4, "stay_leaves": 5, "opened": -1}
 
 
 @functools.lru_cache(maxsize=4096)
