@@ -93,6 +93,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same with nothing to add to.
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 // An 8 x 8 matrix of 16-bit elements, a row per four lanes: the transposed one in the same layout.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     uint32_t d;
@@ -158,37 +164,49 @@ template <int NT> struct Rows {
     uint32_t q[2 * NW][NT][2];                                   // the second operand of the scores, channels in the order of the keys' codes
     int limit[NT][2];                                            // the last position that rows 2 j, 2 j + 1 see
 };
-__device__ __forceinline__ uint4 flipped(uint4 x, uint32_t flip) { return make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip); }
 
-// Rows row0 .. of a (sequence, key head): row i is head i % group of new token i / group.  As they are in memory: a lane has its quarter of row r.
-__device__ __forceinline__ void load_row(const Args& a, const Seq& s, int kvh, int row, uint4 (&x)[NW]) {
-    const int j = threadIdx.x & 3, tok = row / a.group, g = row - tok * a.group;
-    const uint4* src = reinterpret_cast<const uint4*>((const bf16*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + g) * D + 8 * j * NW);
+// Rows row0 .. of a (sequence, key head): row i is head i % group of new token i / group.  A lane has its quarter of rows r, 8 + r ..; first as they are in
+// memory (fetch_rows), then in the order of the keys' codes (order_rows, in place).
+template <int NT>
+__device__ __forceinline__ void fetch_rows(const Args& a, const Seq& s, int kvh, int row0, Rows<NT>& w) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) x[i] = row < s.new_tokens * a.group ? src[i] : make_uint4(0, 0, 0, 0);
+    for (int n = 0; n < NT; ++n) {
+        const int row = row0 + 8 * n + r, tok = row / a.group, g = row - tok * a.group;
+        const uint4* src = reinterpret_cast<const uint4*>((const bf16*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + g) * D + 8 * j * NW);
+        const bool there = row < s.new_tokens * a.group;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const uint4 x = there ? src[i] : make_uint4(0, 0, 0, 0);
+            w.q[2 * i][n][0] = x.x;
+            w.q[2 * i][n][1] = x.y;
+            w.q[2 * i + 1][n][0] = x.z;
+            w.q[2 * i + 1][n][1] = x.w;
+        }
+    }
 }
 template <int NT>
-__device__ __forceinline__ void order_row(const Args& a, const uint4 (&x)[NW], int n, Rows<NT>& w) {
+__device__ __forceinline__ void order_rows(const Args& a, Rows<NT>& w) {
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
-        const uint4 y = flipped(x[i], a.flip);
-        w.q[2 * i][n][0] = low_halves(y.x, y.z);
-        w.q[2 * i][n][1] = high_halves(y.x, y.z);
-        w.q[2 * i + 1][n][0] = low_halves(y.y, y.w);
-        w.q[2 * i + 1][n][1] = high_halves(y.y, y.w);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const uint32_t x = w.q[2 * i][n][0] ^ a.flip, y = w.q[2 * i][n][1] ^ a.flip, z = w.q[2 * i + 1][n][0] ^ a.flip, v = w.q[2 * i + 1][n][1] ^ a.flip;
+            w.q[2 * i][n][0] = low_halves(x, z);
+            w.q[2 * i][n][1] = high_halves(x, z);
+            w.q[2 * i + 1][n][0] = low_halves(y, v);
+            w.q[2 * i + 1][n][1] = high_halves(y, v);
+        }
 }
 template <int NT>
 __device__ __forceinline__ void load_rows(const Args& a, const Seq& s, int kvh, int row0, Rows<NT>& w) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3, n_rows = s.new_tokens * a.group;
+    const int j = threadIdx.x & 3, n_rows = s.new_tokens * a.group;
+    fetch_rows<NT>(a, s, kvh, row0, w);
+    order_rows<NT>(a, w);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        uint4 x[NW];
-        load_row(a, s, kvh, row0 + 8 * n + r, x);
-        order_row<NT>(a, x, n, w);
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) w.limit[n][c] = s.start + min(row0 + 8 * n + 2 * j + c, n_rows - 1) / a.group;
-    }
 }
 
 template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
@@ -211,18 +229,15 @@ template <int N> __device__ __forceinline__ void load_words(const uint8_t* p, ui
 }
 
 // One page (in shared memory) into a leaf.  MASK: some of its positions are not seen by some row; first: the position of the page's first row, len: the
-// sequence's length; several: rows of several tokens.  fresh: the leaf's first page.  between: what is to be done when the keys have been read and before
+// sequence's length; several: rows of several tokens.  FRESH: the leaf's first page (nothing is in the sum, its members have no value yet).  between: what is to be done when the keys have been read and before
 // the values are.
-template <int NT, bool MASK, typename Between>
-__device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w, float scale2, int first, int len, bool several, bool fresh, Sum<NT>& sum,
-                                          Between between) {
+template <int NT, bool MASK, bool FRESH, typename Between>
+__device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w, float scale2, int first, int len, bool several, Sum<NT>& sum, Between between) {
     const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
     const int tr = position_of(r), ta = position_of(2 * j), tb = position_of(2 * j + 1);
     float s[4][NT][4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.f;
         uint32_t k[2][NW];
         const uint8_t* sc[2];
 #pragma unroll
@@ -247,7 +262,8 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
             key_word(k[1][i], a2[1], b2[1], v1);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                mma16816(s[mt][n], v0[0], v1[0], v0[1], v1[1], w.q[2 * i][n][0], w.q[2 * i][n][1]);
+                if (i == 0) mma16816_first(s[mt][n], v0[0], v1[0], v0[1], v1[1], w.q[2 * i][n][0], w.q[2 * i][n][1]);
+                else mma16816(s[mt][n], v0[0], v1[0], v0[1], v1[1], w.q[2 * i][n][0], w.q[2 * i][n][1]);
                 mma16816(s[mt][n], v0[2], v1[2], v0[3], v1[3], w.q[2 * i + 1][n][0], w.q[2 * i + 1][n][1]);
             }
         }
@@ -269,7 +285,8 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-            const float m = fmaxf(sum.m[n][c], top[c] == -INFINITY ? top[c] : top[c] * scale2), was = weight(sum.m[n][c], m);
+            const float mine = top[c] == -INFINITY ? top[c] : top[c] * scale2, m = FRESH ? mine : fmaxf(sum.m[n][c], mine);
+            const float was = FRESH ? 0.f : weight(sum.m[n][c], m);
             const float ref = m == -INFINITY ? 0.f : m;          // (nothing seen: weights 0; a score that is no number still shows)
             sum.m[n][c] = m;
             float l = 0.f;
@@ -283,8 +300,8 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
                     l += x;
                 }
             }
-            sum.l[n][c] = sum.l[n][c] * was + l;
-            if (!fresh) {
+            sum.l[n][c] = FRESH ? l : sum.l[n][c] * was + l;
+            if (!FRESH) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
                     sum.o[i][n][c] *= was;
@@ -339,7 +356,10 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma16816(sum.o[4 * i + k][n], e[k][0], o[k][0], e[k][1], o[k][1], p[mt][n][0], p[mt][n][1]);
+                for (int n = 0; n < NT; ++n) {
+                    if (FRESH && mt == 0) mma16816_first(sum.o[4 * i + k][n], e[k][0], o[k][0], e[k][1], o[k][1], p[mt][n][0], p[mt][n][1]);
+                    else mma16816(sum.o[4 * i + k][n], e[k][0], o[k][0], e[k][1], o[k][1], p[mt][n][0], p[mt][n][1]);
+                }
         }
     }
     if (MASK && several) {
@@ -371,8 +391,14 @@ template <int NT, typename Between = Nothing>
 __device__ __forceinline__ void leaf_page(const Args& a, const uint8_t* tile, const Rows<NT>& w, const Seq& s, int page, bool fresh, Sum<NT>& sum,
                                           Between between = Nothing()) {
     const int first = page * kPage;
-    if (first + kPage - 1 > s.start) page_step<NT, true>(tile, w, a.scale2, first, s.len, s.new_tokens > 1, fresh, sum, between);
-    else page_step<NT, false>(tile, w, a.scale2, first, s.len, false, fresh, sum, between);
+    if (first + kPage - 1 > s.start) {
+        if (fresh) sum.clear();
+        page_step<NT, true, false>(tile, w, a.scale2, first, s.len, s.new_tokens > 1, sum, between);
+    } else if (fresh) {
+        page_step<NT, false, true>(tile, w, a.scale2, first, s.len, false, sum, between);
+    } else {
+        page_step<NT, false, false>(tile, w, a.scale2, first, s.len, false, sum, between);
+    }
 }
 
 // A leaf's sum over its positions: every lane gets its rows'.
@@ -477,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
     };
     for (int k = 0; k < min(a.stages, count); ++k) issue(k);
     Sum<NT> sum;
-    sum.clear();
+    if (count == 0) sum.clear();
     if (count > 0) {
         Rows<NT> w;
         load_rows<NT>(a, s, kvh, row0, w);
@@ -713,16 +739,15 @@ __global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) 
     Seq s;
     s.new_tokens = 1;
     s.first = firsts[cn.b];
-    uint4 raw[NW];
-    load_row(a, s, cn.kvh, r, raw);
+    Rows<1> w;
+    fetch_rows<1>(a, s, cn.kvh, 0, w);
     bool ok = true;
 #pragma unroll 1
     while (true) {
         s.len = lens[cn.b];
         s.start = s.len - 1;
         s.first = firsts[cn.b];
-        Rows<1> w;
-        order_row<1>(a, raw, 0, w);
+        order_rows<1>(a, w);
         w.limit[0][0] = w.limit[0][1] = s.start;
         take(nn, next_ids);
         Fold f[2];
@@ -735,7 +760,6 @@ __global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) 
 #pragma unroll 1
         for (int page = cn.page; page < cn.end;) {
             Sum<1> sum;
-            sum.clear();
             const int leaf_end = min(cn.end, page + cn.lp);
             bool fresh = true;
 #pragma unroll 1
@@ -759,7 +783,7 @@ __global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) 
                         Seq t;
                         t.new_tokens = 1;
                         t.first = firsts[nn.b];
-                        load_row(a, t, nn.kvh, r, raw);
+                        fetch_rows<1>(a, t, nn.kvh, 0, w);
                     }
                     ok = mbar_wait(&full[warp][1], parity, &abort_flag, a.status, 16) && ok;
                 });

@@ -88,14 +88,20 @@ __device__ __forceinline__ void encode(const double (&x)[8], unsigned mask, bool
         bad = true;
     }
     const double af = (double)__bfloat162float(a), bf = (double)__bfloat162float(b);
+    const bool none = bad || af == 0.0;
+    // 16 (x - b) / a - 16 with 20 bits behind the point, by adding 1.5 2^32: the code is known unless that is next to a half.  There, and where b is so
+    // coarse that the number is large, a division: numbers of few bits often lie halfway between two codes, and the quotient is exact there.
+    const double inv = none ? 0.0 : 16.0 / af;
+    const bool near_all = fmax(fabs(hi - bf), fabs(lo - bf)) * inv >= 1000.0;
     word = 0;
-    // (A division, not a product with the reciprocal: numbers of few bits often lie halfway between two codes, and the quotient is exact there.)
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const double c = fmin(fmax(rint((x[k] - bf) * 16.0 / af - 16.0), 0.0), 15.0);
-        const uint32_t code = bad || af == 0.0 ? 0u : (uint32_t)(int)c;
-        word |= code << (4 * k);
+        const int up = __double2loint(fma(x[k] - bf, inv, 6442450944.0 - 16.0)) + (1 << 19);
+        int code = min(max(up >> 20, 0), 15);
+        if (((up + 1) & 0xFFFFF) <= 2 || near_all) code = (int)fmin(fmax(rint((x[k] - bf) * 16.0 / af - 16.0), 0.0), 15.0);
+        word |= (uint32_t)code << (4 * k);
     }
+    if (none) word = 0;
     if (is_v) word = ((word << 3) & 0xF8F8F8F8u) | ((word >> 5) & 0x07070707u);      // (every byte turned left by 3)
     else word = __funnelshift_l(word, word, 3);
     scale = (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16;
