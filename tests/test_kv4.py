@@ -42,3 +42,45 @@ def test_without_a_device_calls_are_refused():
                                     page_table=i32.view(1, 2), seq_of_token=i32, positions=i32)
     with pytest.raises(ops.KernelError):
         ops.attention_kv4(torch.zeros((2, 4, 64)), kv, None, 0.1)
+
+
+def test_storage_holds_five_bits_a_number():
+    from wick_b200.cache import PAGE, Cache, PagedKV4
+    from wick_b200.parts.base import CacheNeed
+    need = CacheNeed("paged_kv4", kv_heads=3, head_dim=64, dtype=torch.uint8)
+    c = Cache([need, need], max_tokens=640, dtype=torch.float32, device="cpu")
+    store = c.groups[0].store
+    assert isinstance(store, PagedKV4) and store.tensor.shape == (2, 11, 3, 80 * 64) and store.tensor.dtype == torch.uint8
+    assert c.bytes_per_token() == 2 * 3 * 2 * 64 * 5 // 8 and c.read_bytes(70, 2) == 70 * c.bytes_per_token()
+    assert c.storage_bytes() == 11 * PAGE * c.bytes_per_token()
+    store.tensor[:, 3] = 7
+    c.copy_pages(torch.tensor([3]), torch.tensor([5]))
+    assert (store.tensor[:, 5] == 7).all() and (store.tensor[:, 4] == 0).all() and not c.cannot_copy()
+    for bad in (dict(dtype=torch.float32), dict(dtype=torch.uint8, v_head_dim=128), dict(dtype=torch.uint8, window=5)):
+        with pytest.raises(ValueError):
+            Cache([CacheNeed("paged_kv4", kv_heads=3, head_dim=64, **bad)], max_tokens=64, dtype=torch.float32, device="cpu", allocate=False)
+
+
+def test_a_model_says_which_of_its_parts_do_not_take_part():
+    import wick_b200 as wick
+    from helpers import CONFIGS
+    from wick_b200.models.qwen3 import build_spec
+    spec = build_spec(wick.config_from_json(CONFIGS["D"]))
+    m = wick.Model(spec, torch.bfloat16, "cpu", cache_bits=4)
+    assert all(n.kind == "paged_kv4" for n in m.cache_needs())
+    assert all(n.kind == "paged_kv" for n in wick.Model(spec, torch.bfloat16, "cpu").cache_needs())
+    from test_nibotar_config import CONFIG
+    cfg = wick.config_from_json(CONFIG)
+    with pytest.raises(ValueError, match="do not keep their cache in 4 bits"):
+        wick.Model(wick.get_architecture(cfg.architecture).build_spec(cfg), torch.bfloat16, "cpu", cache_bits=4)
+    with pytest.raises(ValueError, match="2 bits"):
+        wick.Model(spec, torch.bfloat16, "cpu", cache_bits=2)
+    with pytest.raises(ValueError, match="head sizes"):
+        wick.Model(build_spec(wick.config_from_json(CONFIGS["A"])), torch.bfloat16, "cpu", cache_bits=4)
+
+
+def test_command_line_option():
+    from wick_b200 import cli
+    assert cli.parse_args(["run", "d", "--cache-bits", "4"]).cache_bits == 4 and cli.parse_args(["run", "d"]).cache_bits is None
+    with pytest.raises(cli.UsageError):
+        cli.parse_args(["run", "d", "--cache-bits", "8"])

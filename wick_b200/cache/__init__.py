@@ -1,6 +1,6 @@
-from .cache import (PAGE, Cache, CacheFull, CacheView, PagedKV, SeqRecord, StateRecords, Storage,
+from .cache import (PAGE, Cache, CacheFull, CacheView, PagedKV, PagedKV4, SeqRecord, StateRecords, Storage,
                     register_storage)
 from .pool import IndexPool, PoolError, PoolExhausted
 
-__all__ = ["PAGE", "Cache", "CacheFull", "CacheView", "PagedKV", "SeqRecord", "StateRecords", "Storage",
+__all__ = ["PAGE", "Cache", "CacheFull", "CacheView", "PagedKV", "PagedKV4", "SeqRecord", "StateRecords", "Storage",
            "register_storage", "IndexPool", "PoolError", "PoolExhausted"]

@@ -11,7 +11,8 @@
 * Schedule entries (layers as they run) with equal needs form a **group** with
   storage of its own, of the class registered for the need's kind
   (:func:`register_storage`): ``paged_kv`` groups [entries, pages, 2, kv_heads,
-  64, head_dim]; ``paged_rows`` groups [entries, pages, 64, *shape], one row of
+  64, head_dim]; ``paged_kv4`` the same in 4 bits [entries, pages, kv_heads,
+  80 head_dim] bytes; ``paged_rows`` groups [entries, pages, 64, *shape], one row of
   fixed shape per position (a latent that keys and values are made from);
   ``paged_blocks`` groups [entries, pages, kv_heads * rows * (head_dim + v_head_dim)], a key and a value for every
   whole block of positions;
@@ -155,6 +156,23 @@ class PagedKV(_Paged):
         return cached_tokens * self.bytes_per_token()
 
 
+class PagedKV4(PagedKV):
+    """Keys and values of every position in 4 bits with a pair of 16-bit scales for every 32 channels (``ops/kv4.py``): bytes [entries, pages,
+    kv_heads, 80 head_dim]."""
+    kind = "paged_kv4"
+
+    def __init__(self, need, n_entries, **kw):
+        super().__init__(need, n_entries, **kw)
+        if self._v_dim() != need.head_dim or self.dtype != torch.uint8:
+            raise ValueError("storage in 4 bits holds keys and values of one size, as bytes")
+
+    def shape(self):
+        return (self.n_entries, self.n_pages, self.need.kv_heads, 80 * self.need.head_dim)
+
+    def bytes_per_token(self) -> int:
+        return self.n_entries * self.need.kv_heads * 80 * self.need.head_dim // PAGE
+
+
 class PagedRows(_Paged):
     """One row of the need's ``shape`` per position: [entries, pages, 64, *shape].  A mixer
     sees its entry's part as ``rows``."""
@@ -237,6 +255,7 @@ def register_storage(kind: str, cls: type) -> type:
 
 
 register_storage("paged_kv", PagedKV)
+register_storage("paged_kv4", PagedKV4)
 register_storage("paged_rows", PagedRows)
 register_storage("paged_blocks", PagedBlocks)
 register_storage("state", StateRecords)

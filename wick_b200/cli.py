@@ -37,6 +37,7 @@ options:
       --seed <n>           RNG seed (continuation k: seed + k)
       --stop-id <id>       extra stop token (repeatable; the config's eos ids always stop)
   -q, --quant <fmt>        weights and activations: bf16 (default) or f32
+      --cache-bits <n>     4: the cache holds keys and values in 4 bits (Qwen3; default: as the activations)
   -c, --context <n>        context length per sequence (default 4096)
       --batch <n>          sequences that start together (default 64; bench: 1)
       --prompt-len <n>     bench: prompt tokens (default 128)
@@ -60,6 +61,7 @@ class Args:
         self.rules: dict = {}
         self.samples = 1
         self.quant = "bf16"
+        self.cache_bits: Optional[int] = None
         self.context = 4096
         self.batch: Optional[int] = None
         self.prompt_len = 128
@@ -138,6 +140,10 @@ def parse_args(argv: List[str]) -> Args:
             if v not in ("bf16", "f32"):
                 raise UsageError(f"unknown format {v} (bf16, f32)")
             a.quant = v
+        elif arg == "--cache-bits":
+            a.cache_bits = num(int, arg)
+            if a.cache_bits != 4:
+                raise UsageError(f"bad value for --cache-bits: {a.cache_bits} (4, or leave it out)")
         elif arg in ("-c", "--context"):
             a.context = num(int, arg)
         elif arg == "--batch":
@@ -161,13 +167,13 @@ def _load(a: Args, max_tokens: int):
 
     import wick_b200 as wick
     t0 = time.perf_counter()
-    eng = wick.Engine.from_dir(a.dir, dtype=a.quant, max_tokens=max_tokens)
+    eng = wick.Engine.from_dir(a.dir, dtype=a.quant, max_tokens=max_tokens, cache_bits=a.cache_bits)
     cfg = eng.config
     name = os.path.basename(os.path.normpath(a.dir)) or "model"
     params = cfg.param_count(getattr(eng.model.head, "is_tied", None)) if hasattr(cfg, "param_count") else 0
     print(f"wick: {name} ({params / 1e6:.0f}M params, {len(eng.spec.schedule)} layers, "
           f"{eng.spec.architecture}) as {a.quant}, {eng.model.weight_bytes_per_step() / 2**30:.1f} GiB, "
-          f"sm_100a kernels, cache of {eng.cache.max_tokens} tokens, loaded in "
+          f"sm_100a kernels, cache of {eng.cache.max_tokens} tokens{'' if a.cache_bits is None else f' in {a.cache_bits} bits'}, loaded in "
           f"{(time.perf_counter() - t0) * 1e3:.0f} ms", file=sys.stderr)
     return eng
 

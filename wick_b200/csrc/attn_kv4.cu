@@ -476,13 +476,6 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
     at /= (unsigned)a.tiles;
     const int kvh = (int)(at % (unsigned)a.n_kv), b = (int)(at / (unsigned)a.n_kv);
     const Seq s = sequence(a, b);
-    const int n_rows = s.new_tokens * a.group, row0 = tile * 8 * NT;
-    if (row0 >= n_rows || !fits(a, s)) return;                   // (so do all blocks of its cluster)
-    const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + 8 * NT, n_rows) - 1) / a.group;
-    const int seen = (s.start + last) / kPage + 1;               // pages that any row of the tile sees
-    const int first_page = node * LEAVES * lp;
-    if (first_page >= seen) return;                                          // (a cluster does not wait for blocks that have left)
-    const int n_nodes = CLUSTERS ? (seen + LEAVES * lp - 1) / (LEAVES * lp) : nodes_of(s.pages, a.n_kv);
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int w = 0; w < LEAVES; ++w) {
@@ -492,7 +485,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    const int n_rows = s.new_tokens * a.group, row0 = tile * 8 * NT;
+    const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + 8 * NT, n_rows) - 1) / a.group;
+    const int seen = (s.start + last) / kPage + 1;               // pages that any row of the tile sees
+    const int first_page = node * LEAVES * lp;
     pdl_wait();
+    if (row0 >= n_rows || !fits(a, s)) return;                   // (so do all blocks of its cluster)
+    if (first_page >= seen) return;                              // (a cluster does not wait for blocks that have left)
+    const int n_nodes = CLUSTERS ? (seen + LEAVES * lp - 1) / (LEAVES * lp) : nodes_of(s.pages, a.n_kv);
     const int p0 = first_page + warp * lp, count = max(0, min(seen, p0 + lp) - p0);
     uint8_t* ring = ring_all + (size_t)warp * a.stages * TILE;
     int ids = 0;
@@ -836,15 +836,14 @@ __global__ void __launch_bounds__(128) join_kernel(const Args a, const int* __re
     pdl_trigger();
     const int lane = threadIdx.x & 31;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= (int64_t)n_tokens * a.n_heads) return;
-    const int tok = (int)(row / a.n_heads), b = seq_of_token[tok];
-    if (b < 0 || b >= a.n_seqs) return;
-    const Seq s = sequence(a, b);
+    const int tok = (int)min(row / a.n_heads, (int64_t)n_tokens - 1), b = seq_of_token[tok];
+    const Seq s = sequence(a, min(max(b, 0), a.n_seqs - 1));
+    pdl_wait();
+    if (row >= (int64_t)n_tokens * a.n_heads || b < 0 || b >= a.n_seqs) return;
     if (tok < s.first || tok >= s.first + s.new_tokens) return;  // (a token that fills the step up)
     if (!fits(a, s)) return;
     const int seen = (s.start + tok - s.first) / kPage + 1, per = (BY_LEAF ? 1 : LEAVES) * leaf_pages(s.pages, a.n_kv), n = (seen + per - 1) / per;
     if (s.pages <= per) return;
-    pdl_wait();
     const float* o_rec = fresh(a.rec) + row * a.nodes * D;
     const float* m_rec = fresh(a.rec) + a.rec_rows * a.nodes * D + row * a.nodes * 2;
     Fold f, g;
@@ -912,12 +911,12 @@ __global__ void __launch_bounds__(PLAIN_WARPS * 32) plain_kernel(const Args a) {
     const int kvh = (int)(at % a.n_kv), b = (int)(at / a.n_kv);
     const Seq s = sequence(a, b);
     const int n_rows = s.new_tokens * a.group, row0 = tile * PR;
+    pdl_wait();
     if (row0 >= n_rows || !fits(a, s)) return;
     const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + PR, n_rows) - 1) / a.group;
     const int seen = (s.start + last) / kPage + 1, first_page = node * LEAVES * lp;
     if (first_page >= seen) return;
     const int n_nodes = nodes_of(s.pages, a.n_kv);
-    pdl_wait();
     for (int i = threadIdx.x; i < PR * D; i += PLAIN_WARPS * 32) {
         const int row = row0 + i / D, tok = row / a.group;
         qs[i / D][i % D] = row < n_rows ? ld((const T*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group)) * D + i % D) : 0.f;

@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(256)
 open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const int* __restrict__ page_table, int table_width,
             const int* __restrict__ cu_seqlens, const int* __restrict__ start, int n_seqs, bf16* __restrict__ out,
             int* __restrict__ out_table, int* status) {
-    pdl_trigger();
+    // (No pdl_trigger: the kernel behind this one may read the page table before it waits, and this one writes it.)
     __shared__ int found[3];
     const int p = blockIdx.x, h = blockIdx.y;
     if (threadIdx.x < 32) {
@@ -350,8 +350,8 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
     }
     __syncthreads();
     const int b = found[0], j = found[1], len = found[2];
-    if (b < 0) return;
     pdl_wait();
+    if (b < 0) return;
     kv = fresh(kv);
     int64_t page = page_of(page_table, table_width, kv_pages, b, j * kPage, status);
     if (page < 0) page = 0;

@@ -154,10 +154,12 @@ class Engine:
 
     # ---- construction ----------------------------------------------------
     @classmethod
-    def from_dir(cls, model_dir: str, *, dtype="bfloat16", max_tokens: int = 4096, device="cuda:0", **kw) -> "Engine":
+    def from_dir(cls, model_dir: str, *, dtype="bfloat16", max_tokens: int = 4096, device="cuda:0", cache_bits: Optional[int] = None,
+                 **kw) -> "Engine":
+        """cache_bits: 4 for a cache that holds keys and values in 4 bits (``ops/kv4.py``), None for one in ``dtype``."""
         cfg = load_config(model_dir)
         arch = get_architecture(cfg.architecture)
-        model = Model(arch.build_spec(cfg), parse_dtype(dtype), device)
+        model = Model(arch.build_spec(cfg), parse_dtype(dtype), device, cache_bits)
         load_weights(model, model_dir)
         eng = cls(model, max_tokens=max_tokens, **kw)
         eng.config = cfg
@@ -165,10 +167,10 @@ class Engine:
 
     @classmethod
     def from_config(cls, cfg: ModelConfig, seed: int, *, dtype="bfloat16", max_tokens: int = 4096, device="cuda:0",
-                    **kw) -> "Engine":
-        """Random weights drawn on the device (no files)."""
+                    cache_bits: Optional[int] = None, **kw) -> "Engine":
+        """Random weights drawn on the device (no files).  cache_bits: as in :meth:`from_dir`."""
         arch = get_architecture(cfg.architecture)
-        model = Model(arch.build_spec(cfg), parse_dtype(dtype), device)
+        model = Model(arch.build_spec(cfg), parse_dtype(dtype), device, cache_bits)
         model.load(random_fetch(model, seed))
         eng = cls(model, max_tokens=max_tokens, **kw)
         eng.config = cfg

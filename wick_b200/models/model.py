@@ -19,17 +19,22 @@ from .spec import ModelSpec
 
 
 class Model:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device: torch.device | str):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device: torch.device | str, cache_bits: Optional[int] = None):
+        """cache_bits: 4 to keep keys and values in 4 bits (mixers that do not take part refuse it), None to keep them in ``dtype``."""
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"compute dtype {dtype} is not built (bfloat16 or float32)")
         spec.validate()
         self.spec = spec
-        self.ctx = BuildContext(dtype=dtype, device=torch.device(device))
+        if cache_bits not in (None, 4):
+            raise ValueError(f"a cache in {cache_bits} bits is not built (4, or None for the compute dtype's)")
+        self.ctx = BuildContext(dtype=dtype, device=torch.device(device), cache_bits=cache_bits)
         ctx = self.ctx
         self.embedding = build_part("embedding", spec.embedding, ctx)
         self.blocks: List[Block] = []
         for ls in spec.layers:
             mixer = build_part("mixer", ls.mixer, ctx)
+            if cache_bits is not None and cache_bits not in mixer.CACHE_BITS:
+                raise ValueError(f"mixers of kind {ls.mixer.kind} do not keep their cache in {cache_bits} bits")
             mixer_norm = build_part("norm", ls.mixer_norm, ctx)
             ffn = build_part("ffn", ls.ffn, ctx)
             ffn_norm = build_part("norm", ls.ffn_norm, ctx)

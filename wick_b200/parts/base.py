@@ -63,6 +63,7 @@ class TensorSpec:
 class BuildContext:
     dtype: torch.dtype            # torch.bfloat16 or torch.float32
     device: torch.device
+    cache_bits: Optional[int] = None   # 4: mixers that can (Mixer.CACHE_BITS) keep their keys and values in 4 bits; None: in the compute dtype
 
     def hold(self, t: torch.Tensor, role: str) -> torch.Tensor:
         """Move a loaded tensor to the device in the dtype its role asks for."""
@@ -88,7 +89,7 @@ class CacheNeed:
 
     kind ``paged_kv``: keys and values of every position, ``kv_heads`` x
     ``head_dim`` each, in pages (values ``v_head_dim`` each, if that is given and
-    differs); ``window`` (tokens) if only the last ones are ever read.  kind ``paged_blocks``: a key and a value for every
+    differs); ``window`` (tokens) if only the last ones are ever read.  kind ``paged_kv4``: the same in 4 bits (``dtype`` uint8).  kind ``paged_blocks``: a key and a value for every
     whole block of ``block`` positions, on the page of the block's last position.  kind ``paged_rows``:
     one row of ``shape`` per position, in the same pages.  kind ``state``: one record of fixed
     ``shape`` and ``dtype`` per sequence, zeroed when the sequence starts.  kind ``several``:
@@ -198,6 +199,9 @@ class Position(Part):
 
 class Mixer(Part):
     category = "mixer"
+    # The numbers of bits, besides those of the compute dtype, that the mixer can keep its cache in (``ctx.cache_bits``; a model whose mixers cannot
+    # is refused).
+    CACHE_BITS: Tuple[int, ...] = ()
 
     def cache_need(self) -> Optional[CacheNeed]:
         return None

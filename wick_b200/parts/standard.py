@@ -239,7 +239,12 @@ class GQAttention(Mixer):
     (one weight vector shared by all heads) before the position encoding; k and v
     are appended to the cache; every new token attends to positions 0..its own;
     the result goes through Wo.  The three projections are held as one matrix.
+
+    With ``ctx.cache_bits`` 4 keys and values are stored in 4 bits (five with their scales, see ``ops/kv4.py``) and every token, the step's
+    own included, reads what the cache holds of them.
     """
+
+    CACHE_BITS = (4,)
 
     def __init__(self, params, ctx):
         super().__init__(params, ctx)
@@ -251,6 +256,9 @@ class GQAttention(Mixer):
         if self.head_dim % 16 != 0 or not 16 <= self.head_dim <= 256:
             raise ValueError(f"the attention kernels take a head_dim that is a multiple of 16 between 16 and 256, "
                              f"not {self.head_dim}")
+        self.cache_bits = ctx.cache_bits
+        if self.cache_bits == 4 and self.head_dim not in ops.KV4_HEAD_DIMS:
+            raise ValueError(f"a cache in 4 bits takes head sizes of {', '.join(map(str, ops.KV4_HEAD_DIMS))}, not {self.head_dim}")
         self.q_dim, self.kv_dim = self.heads * self.head_dim, self.kv_heads * self.head_dim
         self.scale = float(p["scale"]) if p.get("scale") is not None else 1.0 / math.sqrt(self.head_dim)
         self.window = p.get("window")
@@ -296,6 +304,8 @@ class GQAttention(Mixer):
         return None
 
     def cache_need(self):
+        if self.cache_bits == 4:
+            return CacheNeed("paged_kv4", kv_heads=self.kv_heads, head_dim=self.head_dim, window=self.window, dtype=torch.uint8)
         return CacheNeed("paged_kv", kv_heads=self.kv_heads, head_dim=self.head_dim, window=self.window)
 
     def weight_bytes(self):
@@ -313,6 +323,13 @@ class GQAttention(Mixer):
             if inv_freq is not None:
                 cos, sin = self.position.tables(batch)
             shared = getattr(batch, "shared", None) is not None and not ops.plain_kernels()
+            if self.cache_bits == 4:
+                q = ops.qk_norm_rope_append_kv4(
+                    qkv, self.heads, self.kv_heads, self.head_dim, q_weight=self.q_norm.weight if self.q_norm else None,
+                    k_weight=self.k_norm.weight if self.k_norm else None, eps=self.q_norm.eps if self.q_norm else 0.0, cos=cos, sin=sin,
+                    kv=cache.kv, page_table=batch.page_table, seq_of_token=batch.seq_of_token, positions=batch.positions,
+                    write_kv=write_cache, dtype=self.ctx.dtype)
+                return self._attend_kv4(q, batch, cache, residual)
             if batch.is_decode and not shared and qkv.shape[0] <= 8 and not ops.plain_kernels() and ops.attention_decode_parts_supported(
                     batch.n_seqs, self.heads, self.kv_heads, self.head_dim, self.ctx.dtype):
                 # the tensor-core decode attention: the projection's sums, the q/k norm, the rotation,
@@ -333,6 +350,8 @@ class GQAttention(Mixer):
                 cos=cos, sin=sin, kv=cache.kv, page_table=batch.page_table,
                 seq_of_token=batch.seq_of_token, positions=batch.positions, write_kv=write_cache,
                 dtype=self.ctx.dtype)
+        if self.cache_bits == 4:
+            return self._attend_kv4(q, batch, cache, residual)
         if getattr(batch, "shared", None) is not None and not ops.plain_kernels():
             # groups of sequences share their first pages, which are read once for all of a group
             need = ops.attention_shared_scratch(batch.shared, batch, self.heads, self.kv_heads, self.head_dim, self.ctx.dtype)
@@ -347,6 +366,11 @@ class GQAttention(Mixer):
             att = ops.attention_prompt(q, cache.kv, batch, self.scale)
         return self.o.forward_delta(att.view(batch.n_tokens, self.q_dim), residual)
 
+    def _attend_kv4(self, q, batch, cache, residual):
+        # (pages that sequences share are read once for each of them: the 4-bit form knows page tables only)
+        need = ops.attention_kv4_scratch(batch, self.heads, self.kv_heads, self.head_dim, self.ctx.dtype)
+        att = ops.attention_kv4(q, cache.kv, batch, self.scale, batch.workspace.get("attention_kv4", need, torch.float32))
+        return self.o.forward_delta(att.view(batch.n_tokens, self.q_dim), residual)
 
     def _encode_unfused(self, x, batch, cache, write_cache):
         """The way for a position encoding that the fused kernel does not know:
@@ -363,7 +387,12 @@ class GQAttention(Mixer):
             k = self.k_norm.forward(k, torch.float32)
         q, k = q.view(n, self.heads, self.head_dim), k.view(n, self.kv_heads, self.head_dim)
         self.position.apply(q, k, batch.positions)
-        encoded = torch.cat([q.view(n, -1), k.view(n, -1), v], dim=1).to(self.ctx.dtype)
+        encoded = torch.cat([q.view(n, -1), k.view(n, -1), v], dim=1)
+        if self.cache_bits == 4:                         # (32-bit sums, in one part)
+            return ops.qk_norm_rope_append_kv4(
+                encoded[None], self.heads, self.kv_heads, self.head_dim, q_weight=None, k_weight=None, eps=0.0, cos=None, sin=None, kv=cache.kv,
+                page_table=batch.page_table, seq_of_token=batch.seq_of_token, positions=batch.positions, write_kv=write_cache, dtype=self.ctx.dtype)
+        encoded = encoded.to(self.ctx.dtype)
         return ops.qk_norm_rope_append(
             encoded, self.heads, self.kv_heads, self.head_dim, q_weight=None, k_weight=None, eps=0.0, cos=None,
             sin=None, kv=cache.kv, page_table=batch.page_table, seq_of_token=batch.seq_of_token,
