@@ -232,16 +232,20 @@ def test_attention(case, dtype):
         out = o.attention_kv4(q, kv.cuda(), b, scale, plain=plain)
         check_attention(q, out, cache, b, scale, d)
     if dtype == BF16:
-        # which kernel computes what changes no bit
-        want = o.attention_kv4(q, kv.cuda(), b, scale, kind="records")
-        check_attention(q, want, cache, b, scale, d)
-        for kind in ("clusters", "stay", "stay_leaves"):
-            try:
-                o.attention_kv4_scratch(b, H, KV, d, dtype, kind=kind)
-            except o.KernelError:
-                assert kind == "clusters" and max(starts) > 500 or "stay" in kind and max(new) * H // KV > 8
-                continue
-            assert torch.equal(o.attention_kv4(q, kv.cuda(), b, scale, kind=kind), want), kind
+        # how the work is shared out changes no bit
+        for kinds in (("records", "clusters", "stay", "stay_leaves"), ("tc", "tc_clusters")):
+            want = None
+            for kind in kinds:
+                try:
+                    o.attention_kv4_scratch(b, H, KV, d, dtype, kind=kind)
+                except o.KernelError:
+                    assert "tc" in kind and d != 128 or "clusters" in kind and max(starts) > 500 or "stay" in kind and max(new) * H // KV > 8
+                    continue
+                got = o.attention_kv4(q, kv.cuda(), b, scale, kind=kind)
+                if want is None:
+                    check_attention(q, got, cache, b, scale, d)
+                    want = got
+                assert torch.equal(got, want), kind
         if d in (64, 128):
             check_attention(q, o.attention_kv4(q, kv.cuda(), b, scale, kind="opened"), cache, b, scale, d)
     o.check_status()
@@ -263,6 +267,12 @@ def test_long_sequences(dtype):
             if H // KV <= 8:
                 for kind in ("stay", "stay_leaves"):
                     assert torch.equal(o.attention_kv4(q, kv.cuda(), b, 0.125, kind=kind), out)
+    for H, KV, length, new in ((16, 1, 70000, 1), (8, 8, 9001, 1), (16, 2, 40001, 3)):
+        g = torch.Generator().manual_seed(length)
+        pages, b = step([length, 3], [new, 1], g)
+        kv, cache = random_cache(pages, KV, 128, g)
+        q = torch.randn((new + 1, H, 128), generator=g).to(dtype).cuda()
+        check_attention(q, o.attention_kv4(q, kv.cuda(), b, 0.1), cache, b, 0.1, 128)
     o.check_status()
 
 
@@ -329,8 +339,8 @@ def test_scales(scale):
     pages, b = step([100, 700, 0], [1, 1, 1], g)
     kv, cache = random_cache(pages, 2, 128, g)
     q = torch.randn((3, 8, 128), generator=g).to(BF16).cuda()
-    for kind in ("plain", "records", "clusters", "stay", "stay_leaves"):
-        check_attention(q, o.attention_kv4(q, kv.cuda(), b, scale, kind=kind if kind != "clusters" else None), cache, b, scale, 128)
+    for kind in ("plain", "records", "stay", "stay_leaves", "tc", "tc_clusters"):
+        check_attention(q, o.attention_kv4(q, kv.cuda(), b, scale, kind=kind), cache, b, scale, 128)
 
 
 def test_rows_behind_the_last_sequence_stay():
