@@ -728,150 +728,156 @@ __global__ void __launch_bounds__(128) join_kernel(const Args a, const int* __re
 }
 
 // ---- CUDA cores --------------------------------------------------------------------------------
-// A block per (node, tile of eight rows, key head, sequence); its warps take the node's pages in turn.  A lane computes the scores of two positions, then
-// sums D / 32 channels of all.  Queries and weights lie in shared memory; codes are read where they are.
-constexpr int PLAIN_WARPS = 4, PR = 8, CH = D / 32;
+// A block of eight warps per (leaf, tile of eight rows, key head, sequence): page by page the scores (four lanes a position, a quarter of the channels each, the
+// queries in shared memory), the rows' weights (a warp a row), the weighted values (a thread two channels, the positions shared out among D / 2
+// threads' worth of groups).  Everything in 32 bits; a leaf leaves a record.  6 sequences of up to 1,000 positions, 16 heads over 2 of 128: the four warps a
+// node that this took the place of 46 us, now 16.
+constexpr int PR = 8;                                            // rows of a tile
+constexpr int Q_PAD = D / 4 + 4;                                 // a quarter of a query, so that quarters lie in different banks
+constexpr int V_GROUPS = 256 / (D / 2);                          // groups of positions (192: two, and 64 threads without)
 
 template <typename T>
-__global__ void __launch_bounds__(PLAIN_WARPS * 32) plain_kernel(const Args a) {
-    __shared__ __align__(16) float ps[PLAIN_WARPS][kPage][PR];
-    __shared__ __align__(16) float so[PLAIN_WARPS][PR][D];       // (the queries while pages are read, then what the warps have summed)
-    __shared__ float sm[PLAIN_WARPS][PR], sl[PLAIN_WARPS][PR];
-    float (&qs)[PR][D] = so[0];
+__global__ void __launch_bounds__(256) plain_kernel(const Args a) {
+    __shared__ __align__(16) float qs[PR][4][Q_PAD];
+    __shared__ __align__(16) float ps[kPage][PR];                // scores, then weights
+    __shared__ float so[V_GROUPS][PR][D];
+    __shared__ float sm[PR], sl[PR], sa[PR];
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t at = blockIdx.x;
-    const int node = (int)(at % a.nodes);
-    at /= a.nodes;
-    const int tile = (int)(at % a.tiles);
-    at /= a.tiles;
-    const int kvh = (int)(at % a.n_kv), b = (int)(at / a.n_kv);
+    unsigned at = blockIdx.x;
+    const int leaf = (int)(at % (unsigned)a.nodes);
+    at /= (unsigned)a.nodes;
+    const int tile = (int)(at % (unsigned)a.tiles);
+    at /= (unsigned)a.tiles;
+    const int kvh = (int)(at % (unsigned)a.n_kv), b = (int)(at / (unsigned)a.n_kv);
     const Seq s = sequence(a, b);
     const int n_rows = s.new_tokens * a.group, row0 = tile * PR;
-    pdl_wait();
-    if (row0 >= n_rows || !fits(a, s)) return;
     const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + PR, n_rows) - 1) / a.group;
-    const int seen = (s.start + last) / kPage + 1, first_page = node * LEAVES * lp;
-    if (first_page >= seen) return;
-    const int n_nodes = nodes_of(s.pages, a.n_kv);
-    for (int i = threadIdx.x; i < PR * D; i += PLAIN_WARPS * 32) {
-        const int row = row0 + i / D, tok = row / a.group;
-        qs[i / D][i % D] = row < n_rows ? ld((const T*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group)) * D + i % D) : 0.f;
+    const int seen = (s.start + last) / kPage + 1, first_page = leaf * lp;
+    pdl_wait();
+    if (row0 >= n_rows || !fits(a, s) || first_page >= seen) return;
+    for (int i = threadIdx.x; i < PR * D; i += 256) {
+        const int row = row0 + i / D, tok = row / a.group, ch = i % D;
+        qs[i / D][ch / (D / 4)][ch % (D / 4)] =
+            row < n_rows ? ld((const T*)a.q + ((int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group)) * D + ch) : 0.f;
     }
-    __syncthreads();
-    float o[PR][CH], m[PR], l[PR];
-    int limit[PR];
-#pragma unroll
-    for (int u = 0; u < PR; ++u) {
-        m[u] = -INFINITY;
-        l[u] = 0.f;
-        limit[u] = s.start + min(row0 + u, n_rows - 1) / a.group;
-#pragma unroll
-        for (int e = 0; e < CH; ++e) o[u][e] = 0.f;
+    if (threadIdx.x < PR) {
+        sm[threadIdx.x] = -INFINITY;
+        sl[threadIdx.x] = 0.f;
     }
-    const int stop = min(seen, first_page + LEAVES * lp);
+    const float scale2 = a.flip ? -a.scale2 : a.scale2;
+    const int pair = threadIdx.x % (D / 2), part = threadIdx.x / (D / 2);
+    float o[PR][2];
+#pragma unroll
+    for (int u = 0; u < PR; ++u) o[u][0] = o[u][1] = 0.f;
+    const int stop = min(seen, first_page + lp);
 #pragma unroll 1
-    for (int page = first_page + warp; page < stop; page += PLAIN_WARPS) {
+    for (int page = first_page; page < stop; ++page) {
         const int id = checked_page(a, a.page_table[(int64_t)b * a.table_width + page]), first = page * kPage;
         const uint8_t* head = a.kv + ((int64_t)id * a.n_kv + kvh) * TILE;
-        float sc[PR][2];
+        const int rows = min(kPage, s.len - first);
+        __syncthreads();                                         // (queries are there; the weights of the page before have been used)
+        {
+            const int t = warp * 8 + (lane >> 2), j = lane & 3;
+            uint32_t w[NW], x = 0;
+            load_words<NW>(head + t * (D / 2) + j * (D / 8), w);
+            float sc[PR];
 #pragma unroll
-        for (int u = 0; u < PR; ++u) sc[u][0] = sc[u][1] = 0.f;
-#pragma unroll 1
-        for (int w = 0; w < D / 8; ++w) {
+            for (int u = 0; u < PR; ++u) sc[u] = 0.f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int t = lane + 32 * h;
-                const uint32_t x = *reinterpret_cast<const uint32_t*>(head + key_scales(D) + (t * (D / GROUP) + w / 4) * 4);
+            for (int i = 0; i < NW; ++i) {
+                if (i % (D == 192 ? 2 : 4) == 0) x = *reinterpret_cast<const uint32_t*>(head + key_scales(D) + (t * (D / GROUP) + ((j * NW + i) >> 2)) * 4);
                 uint32_t v[4];
-                key_word(*reinterpret_cast<const uint32_t*>(head + t * (D / 2) + 4 * w), low_halves(x, x), high_halves(x, x), v);
+                key_word(w[i], low_halves(x, x), high_halves(x, x), v);
                 float k[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v[i]));
-                    k[i] = f.x;
-                    k[i + 4] = f.y;
+                for (int e = 0; e < 4; ++e) {
+                    k[e] = __uint_as_float(v[e] << 16);
+                    k[e + 4] = __uint_as_float(v[e] & 0xFFFF0000u);
                 }
 #pragma unroll
                 for (int u = 0; u < PR; ++u) {
-                    const float4 x0 = *reinterpret_cast<const float4*>(&qs[u][8 * w]), x1 = *reinterpret_cast<const float4*>(&qs[u][8 * w + 4]);
-                    sc[u][h] += x0.x * k[0] + x0.y * k[1] + x0.z * k[2] + x0.w * k[3] + x1.x * k[4] + x1.y * k[5] + x1.z * k[6] + x1.w * k[7];
+                    const float4 x0 = *reinterpret_cast<const float4*>(&qs[u][j][8 * i]), x1 = *reinterpret_cast<const float4*>(&qs[u][j][8 * i + 4]);
+                    sc[u] += x0.x * k[0] + x0.y * k[1] + x0.z * k[2] + x0.w * k[3] + x1.x * k[4] + x1.y * k[5] + x1.z * k[6] + x1.w * k[7];
                 }
-            }
-        }
-        __syncwarp();
-#pragma unroll
-        for (int u = 0; u < PR; ++u) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                sc[u][h] = first + lane + 32 * h > limit[u] ? -INFINITY : sc[u][h] * (a.flip ? -a.scale2 : a.scale2);
-                top = fmaxf(top, sc[u][h]);
-            }
-            const float mn = fmaxf(m[u], warp_max(top)), was = m[u] == -INFINITY ? 0.f : exp2f(m[u] - mn), ref = mn == -INFINITY ? 0.f : mn;
-            m[u] = mn;
-            const float e0 = exp2f(sc[u][0] - ref), e1 = exp2f(sc[u][1] - ref);
-            l[u] = l[u] * was + warp_sum(e0 + e1);
-            ps[warp][lane][u] = e0;
-            ps[warp][lane + 32][u] = e1;
-#pragma unroll
-            for (int e = 0; e < CH; ++e) o[u][e] *= was;
-        }
-        __syncwarp();
-        const int rows = min(kPage, s.len - first);
-#pragma unroll 1
-        for (int t = 0; t < rows; ++t) {
-            float v[CH];
-            uint32_t x = 0;
-#pragma unroll
-            for (int e = 0; e < CH; e += 2) {
-                // (six channels can lie in two groups)
-                if (e == 0 || D == 192) x = *reinterpret_cast<const uint32_t*>(head + value_scales(D) + (t * (D / GROUP) + (lane * CH + e) / GROUP) * 4);
-                const uint32_t byte = head[value_codes(D) + t * (D / 2) + value_byte<D>(t, (lane * CH + e) / 2)];
-                uint32_t even, odd;
-                value_pair<0>(byte, byte, low_halves(x, x), high_halves(x, x), even, odd);
-                v[e] = __uint_as_float(even << 16);
-                v[e + 1] = __uint_as_float(odd << 16);
             }
 #pragma unroll
             for (int u = 0; u < PR; ++u) {
-                const float p = ps[warp][t][u];
-                if (first + t <= limit[u])                       // (a value that is no number does not show in rows that do not see it)
+                sc[u] += __shfl_xor_sync(0xffffffffu, sc[u], 1);
+                sc[u] += __shfl_xor_sync(0xffffffffu, sc[u], 2);
+            }
+            if (j == 0) {
 #pragma unroll
-                    for (int e = 0; e < CH; ++e) o[u][e] += p * v[e];
+                for (int u = 0; u < PR; ++u)
+                    ps[t][u] = first + t > s.start + min(row0 + u, n_rows - 1) / a.group ? -INFINITY : sc[u] * scale2;
             }
         }
-        __syncwarp();
-    }
-    __syncthreads();
+        __syncthreads();
+        {
+            const int u = warp;                                  // (eight warps, eight rows)
+            const float x = ps[lane][u], y = ps[lane + 32][u];
+            const float m0 = sm[u], m = fmaxf(m0, warp_max(fmaxf(x, y))), ref = m == -INFINITY ? 0.f : m;
+            const float e0 = exp2f(x - ref), e1 = exp2f(y - ref), sum = warp_sum(e0 + e1), was = m0 == -INFINITY ? 0.f : exp2f(m0 - m);
+            ps[lane][u] = e0;
+            ps[lane + 32][u] = e1;
+            __syncwarp();
+            if (lane == 0) {
+                sm[u] = m;
+                sl[u] = sl[u] * was + sum;
+                sa[u] = was;
+            }
+        }
+        __syncthreads();
+        if (part < V_GROUPS) {
 #pragma unroll
-    for (int u = 0; u < PR; ++u) {
+            for (int u = 0; u < PR; ++u) {
+                o[u][0] *= sa[u];
+                o[u][1] *= sa[u];
+            }
+            const bool all = first + kPage - 1 <= s.start;       // every row sees every position
+            // A position's two values, and their part in the rows that see it (a value that is no number does not show in the others).
+            auto add = [&](int t, bool check) {
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(head + value_scales(D) + (t * (D / GROUP) + pair / 16) * 4);
+                const uint32_t byte = head[value_codes(D) + t * (D / 2) + value_byte<D>(t, pair)];
+                uint32_t even, odd;
+                value_pair<0>(byte, byte, low_halves(x, x), high_halves(x, x), even, odd);
+                const float v0 = __uint_as_float(even << 16), v1 = __uint_as_float(odd << 16);
+                const float4 p0 = *reinterpret_cast<const float4*>(&ps[t][0]), p1 = *reinterpret_cast<const float4*>(&ps[t][4]);
+                const float p[PR] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
 #pragma unroll
-        for (int e = 0; e < CH; ++e) so[warp][u][lane * CH + e] = o[u][e];
-        if (lane == 0) {
-            sm[warp][u] = m[u];
-            sl[warp][u] = l[u];
+                for (int u = 0; u < PR; ++u) {
+                    if (check && first + t > s.start + min(row0 + u, n_rows - 1) / a.group) continue;
+                    o[u][0] += p[u] * v0;
+                    o[u][1] += p[u] * v1;
+                }
+            };
+            if (all) {
+#pragma unroll 8
+                for (int t = part; t < kPage; t += V_GROUPS) add(t, false);
+            } else {
+#pragma unroll 1
+                for (int t = part; t < rows; t += V_GROUPS) add(t, true);
+            }
         }
     }
+    if (part < V_GROUPS) {
+#pragma unroll
+        for (int u = 0; u < PR; ++u) *reinterpret_cast<float2*>(&so[part][u][2 * pair]) = make_float2(o[u][0], o[u][1]);
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < PR * D; i += PLAIN_WARPS * 32) {
-        const int u = i / D, ch = i % D, row = row0 + u, tok = row / a.group;
-        if (row >= n_rows) continue;
-        Fold f;
-        f.m = -INFINITY;
-        f.l = 0.f;
-        float x = 0.f;
-        for (int p = 0; p < PLAIN_WARPS; ++p) {
-            f.step(sm[p][u], sl[p][u]);
-            x = f.of(x, so[p][u][ch]);
-        }
-        const int64_t flat = (int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group);
-        if (n_nodes == 1) {
-            st((T*)a.out + flat * D + ch, result(x, f.l));
+    for (int i = threadIdx.x; i < PR * D; i += 256) {
+        const int u = i / D, ch = i % D;
+        const int64_t flat = flat_row(a, s, kvh, row0 + u);
+        if (flat < 0) continue;
+        float x = so[0][u][ch];
+#pragma unroll
+        for (int p = 1; p < V_GROUPS; ++p) x += so[p][u][ch];
+        if (s.pages <= lp) {
+            st((T*)a.out + flat * D + ch, result(x, sl[u]));
         } else {
-            const int64_t rec = flat * a.nodes + node;
+            const int64_t rec = flat * a.nodes + leaf;
             a.rec[rec * D + ch] = x;
-            if (ch == 0) *reinterpret_cast<float2*>(a.rec + a.rec_rows * a.nodes * D + rec * 2) = make_float2(f.m, f.l);
+            if (ch == 0) *reinterpret_cast<float2*>(a.rec + a.rec_rows * a.nodes * D + rec * 2) = make_float2(sm[u], sl[u]);
         }
     }
 }
@@ -896,7 +902,7 @@ static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int
     p.rows = p.form == PLAIN ? 8 : (tc ? (rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 24 ? 24 : 32))) : 8 * p.nt);
     p.tiles = (int)((rows + p.rows - 1) / p.rows);
     p.stages = leaf_pages(pages, n_kv) > 1 ? MAX_STAGES : 1;
-    if (p.form == STAY_LEAVES) p.nodes = (pages + leaf_pages(pages, n_kv) - 1) / leaf_pages(pages, n_kv);      // (places for records)
+    if (p.form == STAY_LEAVES || p.form == PLAIN) p.nodes = (pages + leaf_pages(pages, n_kv) - 1) / leaf_pages(pages, n_kv);      // (places for records)
     p.blocks = p.form == STAY || p.form == STAY_LEAVES || p.form == TC ? sm_count() : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
     const bool records = p.nodes > 1 && p.form != CLUSTERS && p.form != TC_CLUSTERS;
     p.scratch = records ? (int64_t)n_tokens * n_heads * p.nodes * (D + 2) : 0;
@@ -957,7 +963,7 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     const cudaStream_t st = (cudaStream_t)stream;
     const dim3 grid((unsigned)p.blocks);
     if (p.form == PLAIN) {
-        WICK_CUDA(launch(plain_kernel<T>, grid, dim3(PLAIN_WARPS * 32), 0, st, a));
+        WICK_CUDA(launch(plain_kernel<T>, grid, dim3(256), 0, st, a));
     } else if (p.form >= TC) {
         if (int rc = launch_tc(a, p.rows, p.form == TC_CLUSTERS, p.blocks, st)) return rc;
     } else if (p.form >= STAY) {
@@ -985,7 +991,7 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     }
     if (int rc = check_launch("attention_kv4")) return rc;
     if (p.kernels == 2) {
-        WICK_CUDA(launch(p.form == STAY_LEAVES ? join_kernel<T, true> : join_kernel<T, false>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, st, a, seq_of_token, n_tokens));
+        WICK_CUDA(launch(p.form == STAY_LEAVES || p.form == PLAIN ? join_kernel<T, true> : join_kernel<T, false>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, st, a, seq_of_token, n_tokens));
         return check_launch("attention_kv4 (join)");
     }
     return 0;

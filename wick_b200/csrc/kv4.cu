@@ -267,25 +267,29 @@ append_kernel(const T* __restrict__ qkv, const float* __restrict__ parts, int sp
 }
 
 // ---- reading tokens back ---------------------------------------------------------
-// The eight values of channels 8 w .. 8 w + 7 of row t of a head's part of a page.
-__device__ __forceinline__ uint4 eight(const uint8_t* head, int t, int w, bool is_v) {
-    const uint32_t s = *reinterpret_cast<const uint32_t*>(head + (is_v ? value_scales(D) : key_scales(D)) + (t * (D / GROUP) + w / 4) * 4);
-    const uint32_t a2 = low_halves(s, s), b2 = high_halves(s, s);
-    const uint32_t x = *reinterpret_cast<const uint32_t*>(head + (is_v ? value_codes(D) + t * (D / 2) + value_byte<D>(t, 4 * w) : t * (D / 2) + 4 * w));
-    uint4 r;
+// Channels 8 w .. 8 w + 7 of row t of a head's part of a page: their codes and scales, and their values.
+struct Eight {
+    uint32_t codes, scales;
+};
+__device__ __forceinline__ Eight load_eight(const uint8_t* head, int t, int w, bool is_v) {
+    Eight e;
+    e.scales = *reinterpret_cast<const uint32_t*>(head + (is_v ? value_scales(D) : key_scales(D)) + (t * (D / GROUP) + w / 4) * 4);
+    e.codes = *reinterpret_cast<const uint32_t*>(head + (is_v ? value_codes(D) + t * (D / 2) + value_byte<D>(t, 4 * w) : t * (D / 2) + 4 * w));
+    return e;
+}
+__device__ __forceinline__ uint4 values_of(const Eight& c, bool is_v) {
+    const uint32_t a2 = low_halves(c.scales, c.scales), b2 = high_halves(c.scales, c.scales), x = c.codes;
     if (is_v) {
         uint32_t e[4], o[4];                                     // (both halves the same position)
         value_pair<0>(x, x, a2, b2, e[0], o[0]);
         value_pair<1>(x, x, a2, b2, e[1], o[1]);
         value_pair<2>(x, x, a2, b2, e[2], o[2]);
         value_pair<3>(x, x, a2, b2, e[3], o[3]);
-        r = make_uint4(low_halves(e[0], o[0]), low_halves(e[1], o[1]), low_halves(e[2], o[2]), low_halves(e[3], o[3]));
-    } else {
-        uint32_t v[4];
-        key_word(x, a2, b2, v);
-        r = make_uint4(low_halves(v[0], v[1]), low_halves(v[2], v[3]), high_halves(v[0], v[1]), high_halves(v[2], v[3]));
+        return make_uint4(low_halves(e[0], o[0]), low_halves(e[1], o[1]), low_halves(e[2], o[2]), low_halves(e[3], o[3]));
     }
-    return r;
+    uint32_t v[4];
+    key_word(x, a2, b2, v);
+    return make_uint4(low_halves(v[0], v[1]), low_halves(v[2], v[3]), high_halves(v[0], v[1]), high_halves(v[2], v[3]));
 }
 
 __global__ void __launch_bounds__(128)
@@ -304,7 +308,7 @@ read_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
     int64_t page = -1;
     if (seq >= 0 && seq < n_seqs) page = page_of(page_table, table_width, kv_pages, seq, pos, status);
     else atomicCAS(status, 0, 15);
-    if (page >= 0) r = eight(kv + (page * n_kv + h) * head_bytes(D), pos % kPage, w, is_v);
+    if (page >= 0) r = values_of(load_eight(kv + (page * n_kv + h) * head_bytes(D), pos % kPage, w, is_v), is_v);
     *reinterpret_cast<uint4*>(out + (((int64_t)(is_v ? n : 0) + t) * n_kv + h) * D + 8 * w) = r;
 }
 
@@ -370,12 +374,20 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
     }
     const uint8_t* head = kv + (page * n_kv + h) * head_bytes(D);
     const int rows = min(kPage, len - j * kPage);
-    for (int i = threadIdx.x; i < 2 * kPage * (D / 8); i += blockDim.x) {
-        const bool is_v = i >= kPage * (D / 8);
-        const int t = i / (D / 8) % kPage, w = i % (D / 8);
-        uint4 r = make_uint4(0, 0, 0, 0);
-        if (t < rows) r = eight(head, t, w, is_v);
-        *reinterpret_cast<uint4*>(out + ((((int64_t)p * 2 + is_v) * n_kv + h) * kPage + t) * D + 8 * w) = r;
+    // All codes of a page are asked for before the first are used (a loop that used them one by one: 42 us for 562 pages of 8 heads of 128, now 30).
+    constexpr int STEPS = 2 * kPage * (D / 8) / 256;
+    Eight e[STEPS];
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+        const int i = u * 256 + threadIdx.x;
+        e[u] = load_eight(head, i / (D / 8) % kPage, i % (D / 8), u >= STEPS / 2);
+    }
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+        const bool is_v = u >= STEPS / 2;
+        const int i = u * 256 + threadIdx.x, t = i / (D / 8) % kPage;
+        const uint4 v = values_of(e[u], is_v);
+        *reinterpret_cast<uint4*>(out + ((((int64_t)p * 2 + is_v) * n_kv + h) * kPage + t) * D + 8 * (i % (D / 8))) = t < rows ? v : make_uint4(0, 0, 0, 0);
     }
 }
 
