@@ -891,17 +891,16 @@ static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int
     const bool can_stay = rows <= 8 && n_seqs <= MAX_SEQS, can_tc = D == 128 && n_seqs <= MAX_SEQS;
     p.possible = p.form >= AUTO && p.form <= TC_CLUSTERS && !(f32 && p.form != PLAIN) && !((p.form == STAY || p.form == STAY_LEAVES) && !can_stay) &&
                  !(p.form >= TC && !can_tc) && !((p.form == CLUSTERS || p.form == TC_CLUSTERS) && p.nodes > CLUSTER);
-    if (p.form == AUTO && can_tc) {
-        const int nr = rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 24 ? 24 : 32));
-        p.form = p.nodes <= CLUSTER && (int64_t)n_seqs * n_kv * p.nodes * ((rows + nr - 1) / nr) <= 2 * sm_count() ? TC_CLUSTERS : TC;
-    } else if (p.form == AUTO) {
-        p.form = can_stay && (int64_t)n_seqs * n_kv * p.nodes >= 2 * (int64_t)LEAVES * sm_count() ? STAY : (p.nodes <= CLUSTER ? CLUSTERS : RECORDS);
-    }
+    const int64_t nodes = (int64_t)n_seqs * n_kv * p.nodes;
+    if (p.form == AUTO && can_tc && rows > 8)
+        p.form = p.nodes <= CLUSTER && nodes <= 2 * sm_count() ? TC_CLUSTERS : TC;
+    else if (p.form == AUTO)
+        p.form = can_stay && nodes >= 2 * (int64_t)LEAVES * sm_count() ? STAY : (p.nodes <= CLUSTER && nodes <= 2 * sm_count() ? CLUSTERS : RECORDS);
     const bool tc = p.form >= TC;
-    p.nt = p.form != PLAIN && rows > 8 ? 2 : 1;
+    p.nt = p.form == PLAIN || rows <= 8 ? 1 : (rows <= 16 || D > 128 ? 2 : 3);
     p.rows = p.form == PLAIN ? 8 : (tc ? (rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 24 ? 24 : 32))) : 8 * p.nt);
     p.tiles = (int)((rows + p.rows - 1) / p.rows);
-    p.stages = leaf_pages(pages, n_kv) > 1 ? MAX_STAGES : 1;
+    p.stages = leaf_pages(pages, n_kv) > 1 || p.nt == 3 ? MAX_STAGES : 1;
     if (p.form == STAY_LEAVES || p.form == PLAIN) p.nodes = (pages + leaf_pages(pages, n_kv) - 1) / leaf_pages(pages, n_kv);      // (places for records)
     p.blocks = p.form == STAY || p.form == STAY_LEAVES || p.form == TC ? sm_count() : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
     const bool records = p.nodes > 1 && p.form != CLUSTERS && p.form != TC_CLUSTERS;
@@ -972,7 +971,7 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
         WICK_CUDA(launch(kernel, grid, dim3(STAY_WARPS * 32), STAY_WARPS * TILE, st, a));
     } else {
         const bool clusters = p.form == CLUSTERS && p.nodes > 1;
-        void (*kernel)(Args) = p.nt == 1 ? (clusters ? leaves_kernel<1, true> : leaves_kernel<1, false>) : (clusters ? leaves_kernel<2, true> : leaves_kernel<2, false>);
+        void (*kernel)(Args) = p.nt == 1 ? (clusters ? leaves_kernel<1, true> : leaves_kernel<1, false>) : p.nt == 2 ? (clusters ? leaves_kernel<2, true> : leaves_kernel<2, false>) : (clusters ? leaves_kernel<D <= 128 ? 3 : 2, true> : leaves_kernel<D <= 128 ? 3 : 2, false>);
         if (int rc = allow(kernel, leaves_smem(p.nt, MAX_STAGES, true))) return rc;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = grid;

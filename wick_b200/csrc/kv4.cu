@@ -52,18 +52,55 @@ __device__ __forceinline__ int64_t page_of(const int* page_table, int table_widt
 // L lanes per vector (one head of q, k or v of one token): a lane holds 8 neighbouring channels i0 .. and their partners in the rotation, i0 + d / 2 ..;
 // four neighbouring lanes hold a group of 32 channels in either half.
 //   q:  x / sqrt(mean x^2 + eps) w, rotated, in 32 bits, rounded to the activations' type
-//   k:  the same in 64 bits, then codes;   v: codes
-// Codes are decided in 64 bits (sums over the projection's runs, norm, rotation, division): 32 would put a few numbers in a million, those next
-// to the border between two codes, on the wrong side of it, another few for every other order of the same operations.
+//   k:  the same, then codes;   v: codes
+// A code is that of the number that 64-bit arithmetic gives (sums over the projection's runs, norm, rotation, range, division).  32 bits would put a few
+// numbers in a million, those next to the border between two codes, on the wrong side of it, another few for every other order of the same operations.  So a
+// vector is computed in 32 bits with a bound on what they can be off by; where every decision (both scales' roundings, every code) is the same
+// anywhere within the bound, it stands, and only where one is not (one key in some 60) the vector is computed again in 64.  3,900 tokens, 32 heads
+// over 8 of 128: all in 64 bits 46 us, now 42 (the queries alone 21).
 constexpr int L = D == 192 ? 16 : D / 16;
 
-struct Codes {
-    uint32_t word[2];                                            // of the lane's channels i0 .. and of their partners
-    uint32_t scale[2];                                           // a | b << 16 of their groups
+struct Source {                                                  // where a lane's numbers of a key or a value come from, and where its codes go
+    const float* parts;                                          // the float32 partial sums, or null
+    const void* qkv;                                             // the activations, or null
+    int splits;
+    int64_t split_stride, base;
+    const float *w, *cos_t, *sin_t;                              // of this lane's channels; null: no norm, no rotation
+    float eps;
+    unsigned mask;                                               // the vector's lanes
+    bool is_v;
+    uint8_t* head;                                               // the head's part of the page; null: nowhere
+    int row, i0;
 };
 
-// One half of a vector: 8 numbers a lane, 4 lanes a group.
-__device__ __forceinline__ void encode(const double (&x)[8], unsigned mask, bool is_v, uint32_t& word, uint32_t& scale) {
+// The sum over a vector's lanes.
+template <typename T> __device__ __forceinline__ T vector_sum(T x, unsigned mask) {
+    if constexpr (D == 192) {                                    // (12 lanes: each of 4, then the three)
+        x += __shfl_xor_sync(mask, x, 1);
+        x += __shfl_xor_sync(mask, x, 2);
+        const int l0 = (threadIdx.x & 31) / L * L;
+        return __shfl_sync(mask, x, l0) + __shfl_sync(mask, x, l0 + 4) + __shfl_sync(mask, x, l0 + 8);
+    } else {
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) x += __shfl_xor_sync(mask, x, o);
+        return x;
+    }
+}
+__device__ __forceinline__ void store_codes(uint8_t* head, int row, int i0, bool is_v, int half, uint32_t word, uint32_t scale) {
+    if (head == nullptr) return;
+    if (is_v) word = ((word << 3) & 0xF8F8F8F8u) | ((word >> 5) & 0x07070707u);      // (every byte turned left by 3)
+    else word = __funnelshift_l(word, word, 3);
+    const int ch = i0 + half * (D / 2), o = ch / 2;
+    uint8_t* codes = head + (is_v ? value_codes(D) + row * (D / 2) + value_byte<D>(row, o) : row * (D / 2) + o);
+    *reinterpret_cast<uint32_t*>(codes) = word;
+    if ((ch & (GROUP - 1)) == 0) *reinterpret_cast<uint32_t*>(head + (is_v ? value_scales(D) : key_scales(D)) + (row * (D / GROUP) + ch / GROUP) * 4) = scale;
+}
+__device__ __forceinline__ uint32_t pair_of(bf16 a, bf16 b) { return (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16; }
+__device__ __forceinline__ int exact_code(double x, double a, double b) { return (int)fmin(fmax(rint((x - b) * 16.0 / a - 16.0), 0.0), 15.0); }
+constexpr float LARGEST = 1.7014118346046923e38f;                // 2^127: beyond it values that codes stand for could be infinite
+
+// One half of a vector, 8 numbers a lane, 4 lanes a group, in 64 bits.
+__device__ __forceinline__ void encode_exactly(const double (&x)[8], const Source& s, int half) {
     double lo = x[0], hi = x[0];
     bool bad = false;
 #pragma unroll
@@ -74,41 +111,144 @@ __device__ __forceinline__ void encode(const double (&x)[8], unsigned mask, bool
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        lo = fmin(lo, __shfl_xor_sync(mask, lo, o));
-        hi = fmax(hi, __shfl_xor_sync(mask, hi, o));
-        bad |= __shfl_xor_sync(mask, (int)bad, o) != 0;
+        lo = fmin(lo, __shfl_xor_sync(s.mask, lo, o));
+        hi = fmax(hi, __shfl_xor_sync(s.mask, hi, o));
+        bad |= __shfl_xor_sync(s.mask, (int)bad, o) != 0;
     }
     // (to bfloat16 by way of 32 bits, as conversions from 64 bits go elsewhere)
     bf16 a = __float2bfloat16_rn((float)((hi - lo) * (16.0 / 15.0)));
     bf16 b = __float2bfloat16_rn((float)(lo - (double)__bfloat162float(a)));
-    // (2^127: so that no value that a code stands for is infinite either)
-    if (bad || fmax(fabs(lo), fabs(hi)) > 0x1p127 || !isfinite(__bfloat162float(a))) {
+    if (bad || fmax(fabs(lo), fabs(hi)) > (double)LARGEST || !isfinite(__bfloat162float(a))) {
         a = __float2bfloat16_rn(0.f);
         b = __ushort_as_bfloat16(0x7FFF);
-        bad = true;
     }
     const double af = (double)__bfloat162float(a), bf = (double)__bfloat162float(b);
-    const bool none = bad || af == 0.0;
     // 16 (x - b) / a - 16 with 20 bits behind the point, by adding 1.5 2^32: the code is known unless that is next to a half.  There, and where b is so
     // coarse that the number is large, a division: numbers of few bits often lie halfway between two codes, and the quotient is exact there.
-    const double inv = none ? 0.0 : 16.0 / af;
-    const bool near_all = fmax(fabs(hi - bf), fabs(lo - bf)) * inv >= 1000.0;
-    word = 0;
+    const double inv = af == 0.0 ? 0.0 : 16.0 / af;
+    const bool all = fmax(fabs(hi - bf), fabs(lo - bf)) * inv >= 1000.0;
+    uint32_t word = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const int up = __double2loint(fma(x[k] - bf, inv, 6442450944.0 - 16.0)) + (1 << 19);
         int code = min(max(up >> 20, 0), 15);
-        if (((up + 1) & 0xFFFFF) <= 2 || near_all) code = (int)fmin(fmax(rint((x[k] - bf) * 16.0 / af - 16.0), 0.0), 15.0);
+        if (((up + 1) & 0xFFFFF) <= 2 || all) code = exact_code(x[k], af, bf);
         word |= (uint32_t)code << (4 * k);
     }
-    if (none) word = 0;
-    if (is_v) word = ((word << 3) & 0xF8F8F8F8u) | ((word >> 5) & 0x07070707u);      // (every byte turned left by 3)
-    else word = __funnelshift_l(word, word, 3);
-    scale = (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16;
+    if (af == 0.0) word = 0;
+    store_codes(s.head, s.row, s.i0, s.is_v, half, word, pair_of(a, b));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(128)
+template <typename T> __device__ __forceinline__ void vector_exactly(const Source& s) {
+    double a[8], b[8];
+    {
+        float fa[8], fb[8];
+        if (s.parts) {
+            load8(s.parts + s.base, fa);
+            load8(s.parts + s.base + D / 2, fb);
+        } else {
+            load8((const T*)s.qkv + s.base, fa);
+            load8((const T*)s.qkv + s.base + D / 2, fb);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            a[k] = (double)fa[k];
+            b[k] = (double)fb[k];
+        }
+        for (int sp = 1; s.parts && sp < s.splits; ++sp) {
+            load8(s.parts + sp * s.split_stride + s.base, fa);
+            load8(s.parts + sp * s.split_stride + s.base + D / 2, fb);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                a[k] += (double)fa[k];
+                b[k] += (double)fb[k];
+            }
+        }
+    }
+    if (s.w) {
+        double ss = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ss += a[k] * a[k] + b[k] * b[k];
+        ss = vector_sum(ss, s.mask);
+        const double scale = 1.0 / sqrt(ss / (double)D + (double)s.eps);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            a[k] = (a[k] * scale) * (double)s.w[k];
+            b[k] = (b[k] * scale) * (double)s.w[k + D / 2];
+        }
+    }
+    if (s.cos_t) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const double c = (double)s.cos_t[k], sn = (double)s.sin_t[k];
+            const double ra = a[k] * c - b[k] * sn, rb = b[k] * c + a[k] * sn;
+            a[k] = ra;
+            b[k] = rb;
+        }
+    }
+    encode_exactly(a, s, 0);
+    encode_exactly(b, s, 1);
+}
+template <typename T> __device__ __noinline__ void vector_again(const Source* s) { vector_exactly<T>(*s); }
+
+// One half in 32 bits, its numbers off by `off` at most from what 64 bits give.  Returns whether every decision is sure.  With u = 2^-24:
+//   range and 16 / 15 of it: 2 off, and four roundings;   min - a: off, and a rounding;   the 64-bit path rounds either to 32 bits before bfloat16: one more;
+//   16 (x - b) / a - 16 is taken with 16 bits behind the point from a sum near 192: half of its last place, off 16 / a, and three roundings of at most 48 (its distance from a border is compared with one and a
+//   half of that place more).
+__device__ __forceinline__ bool encode(const float (&x)[8], float off, unsigned mask, uint32_t& word, uint32_t& scale) {
+    constexpr float u = 5.9604645e-8f;
+    float lo = x[0], hi = x[0], all = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        lo = fminf(lo, x[k]);
+        hi = fmaxf(hi, x[k]);
+        all += x[k] * 0.f;                                       // (0, or no number if one of them is infinite or none)
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+    }
+    const float range = (hi - lo) * (16.0f / 15.0f), da = 2.2f * off + 6.f * u * range;
+    const bf16 a = __float2bfloat16_rn(range - da);
+    const float af = __bfloat162float(a), least = lo - af, db = 1.1f * off + 3.f * u * fabsf(least);
+    const bf16 b = __float2bfloat16_rn(least - db);
+    const float bf = __bfloat162float(b), inv = 16.0f / af;
+    bool sure = all == 0.f && af >= 1e-30f && fmaxf(fabsf(lo), fabsf(hi)) < 1e38f && fmaxf(fabsf(hi - bf), fabsf(lo - bf)) * inv < 48.f &&
+                __bfloat16_as_ushort(a) == __bfloat16_as_ushort(__float2bfloat16_rn(range + da)) &&
+                __bfloat16_as_ushort(b) == __bfloat16_as_ushort(__float2bfloat16_rn(least + db));
+    const float wide = off * inv * 65536.0f;
+    sure = sure && wide < 8000.f;
+    const int d = sure ? (int)wide + 2 : 0;
+    // The code with 16 bits behind the point, and a half: the low 20 bits of the number's, since 192 has none there; the least distance from a border.
+    constexpr int ZERO = 0x43400000;
+    int nearest = 0xFFFF;
+    word = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int y = __float_as_int(fmaf(x[k] - bf, inv, 176.5f)), kept = min(max(y, ZERO), ZERO + 0xFFFFF);
+        nearest = min(nearest, (y + d) & 0xFFFF);
+        word |= k < 4 ? (uint32_t)kept >> (16 - 4 * k) & 0xFu << (4 * k) : (uint32_t)kept << (4 * k - 16) & 0xFu << (4 * k);
+    }
+    scale = pair_of(a, b);
+    if (sure && nearest <= 2 * d) {
+        if (off != 0.f) return false;
+        // (the numbers are what they are, and those of few bits lie on borders)
+        word = 0;
+#pragma unroll 1
+        for (int k = 0; k < 8; ++k) {
+            float y = x[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) y = k == e ? x[e] : y;
+            word |= (uint32_t)exact_code((double)y, (double)af, (double)bf) << (4 * k);
+        }
+    }
+    return sure;
+}
+
+// EXACTLY: all keys and values in 64 bits at once.
+template <typename T, bool EXACTLY>
+__global__ void __launch_bounds__(128, EXACTLY ? 4 : 8)
 append_kernel(const T* __restrict__ qkv, const float* __restrict__ parts, int splits, int64_t split_stride, int n_tokens, int n_heads, int n_kv,
               const float* __restrict__ q_w, const float* __restrict__ k_w, float eps, const float* __restrict__ cos_t,
               const float* __restrict__ sin_t, T* __restrict__ q_out, uint8_t* __restrict__ kv, int64_t kv_pages, const int* __restrict__ page_table,
@@ -130,20 +270,45 @@ append_kernel(const T* __restrict__ qkv, const float* __restrict__ parts, int sp
     const float* w = is_q ? q_w : (is_v ? nullptr : k_w);
     const bool rotate = !is_v && cos_t != nullptr;
     const int64_t base = ((int64_t)t * (n_heads + 2 * n_kv) + h) * D + i0;
-    float c[8], sn[8], wa[8], wb[8];
-    if (rotate) {
-        load8(cos_t + (int64_t)t * half + i0, c);
-        load8(sin_t + (int64_t)t * half + i0, sn);
+    uint8_t* head = nullptr;                                     // the head's part of the page; null: nowhere
+    int row = 0;
+    if (!is_q) {
+        const int pos = positions[t], seq = seq_of_token[t];
+        if (seq < 0 || seq >= n_seqs) {
+            atomicCAS(status, 0, 15);
+        } else {
+            const int64_t page = page_of(page_table, table_width, kv_pages, seq, pos, status);
+            if (page >= 0) head = kv + (page * n_kv + (h - n_heads - (is_v ? n_kv : 0))) * head_bytes(D);
+        }
+        row = pos & (kPage - 1);
     }
-    if (w) {
-        load8(w + i0, wa);
-        load8(w + i0 + half, wb);
+    auto source = [&]() {
+        Source s;
+        s.parts = parts;
+        s.qkv = qkv;
+        s.splits = splits;
+        s.split_stride = split_stride;
+        s.base = base;
+        s.w = w ? w + i0 : nullptr;
+        s.cos_t = rotate ? cos_t + (int64_t)t * half + i0 : nullptr;
+        s.sin_t = rotate ? sin_t + (int64_t)t * half + i0 : nullptr;
+        s.eps = eps;
+        s.mask = mask;
+        s.is_v = is_v;
+        s.head = head;
+        s.row = row;
+        s.i0 = i0;
+        return s;
+    };
+    if (EXACTLY && !is_q) {
+        vector_exactly<T>(source());
+        return;
     }
-    if (is_q) {
-        float a[8], b[8];
-        if (parts) {
-            load8(parts + base, a);
-            load8(parts + base + half, b);
+    float a[8], b[8];
+    if (parts) {
+        load8(parts + base, a);
+        load8(parts + base + half, b);
+        if (is_q) {
             for (int sp = 1; sp < splits; ++sp) {
                 float da[8], db[8];
                 load8(parts + sp * split_stride + base, da);
@@ -154,116 +319,96 @@ append_kernel(const T* __restrict__ qkv, const float* __restrict__ parts, int sp
                     b[k] += db[k];
                 }
             }
-        } else {
-            load8(qkv + base, a);
-            load8(qkv + base + half, b);
+        } else if (splits > 1) {
+            // (in 64 bits: in 32 a sum of large runs of opposite signs would be off by more than a rounding of itself)
+            double sa[8], sb[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                sa[k] = (double)a[k];
+                sb[k] = (double)b[k];
+            }
+            for (int sp = 1; sp < splits; ++sp) {
+                load8(parts + sp * split_stride + base, a);
+                load8(parts + sp * split_stride + base + half, b);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    sa[k] += (double)a[k];
+                    sb[k] += (double)b[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                a[k] = (float)sa[k];
+                b[k] = (float)sb[k];
+            }
         }
-        if (w) {
+    } else {
+        load8(qkv + base, a);
+        load8(qkv + base + half, b);
+    }
+    if (w) {
+        float wa[8], wb[8];
+        load8(w + i0, wa);
+        load8(w + i0 + half, wb);
+        float scale;
+        if (is_q) {
             float ss = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) ss += a[k] * a[k] + b[k] * b[k];
-            if (D == 192) {                                      // (12 lanes: each of 4, then the three)
-                ss += __shfl_xor_sync(mask, ss, 1);
-                ss += __shfl_xor_sync(mask, ss, 2);
-                const int l0 = (threadIdx.x & 31) / L * L;
-                ss = __shfl_sync(mask, ss, l0) + __shfl_sync(mask, ss, l0 + 4) + __shfl_sync(mask, ss, l0 + 8);
-            } else {
+            scale = 1.0f / sqrtf(vector_sum(ss, mask) / (float)D + eps);
+        } else {
+            // (the sum in 64 bits: in 32 the scale alone would be off by up to 15 roundings, and two to three times as many vectors would not be sure)
+            double ss = 0.0;
 #pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-            }
-            const float scale = 1.0f / sqrtf(ss / (float)D + eps);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                a[k] = (a[k] * scale) * wa[k];
-                b[k] = (b[k] * scale) * wb[k];
-            }
+            for (int k = 0; k < 8; ++k) ss += (double)a[k] * (double)a[k] + (double)b[k] * (double)b[k];
+            scale = 1.0f / sqrtf((float)(vector_sum(ss, mask) * (1.0 / D) + (double)eps));
         }
-        if (rotate) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float ra = a[k] * c[k] - b[k] * sn[k], rb = b[k] * c[k] + a[k] * sn[k];
-                a[k] = ra;
-                b[k] = rb;
-            }
+        for (int k = 0; k < 8; ++k) {
+            a[k] = (a[k] * scale) * wa[k];
+            b[k] = (b[k] * scale) * wb[k];
         }
+    }
+    float largest = 0.f, turn = 1.f;                             // of the numbers before the rotation, and of its cosines and sines
+    if (!is_q) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) largest = fmaxf(largest, fmaxf(fabsf(a[k]), fabsf(b[k])));
+    }
+    if (rotate) {
+        float c[8], sn[8];
+        load8(cos_t + (int64_t)t * half + i0, c);
+        load8(sin_t + (int64_t)t * half + i0, sn);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            turn = fmaxf(turn, fmaxf(fabsf(c[k]), fabsf(sn[k])));
+            const float ra = a[k] * c[k] - b[k] * sn[k], rb = b[k] * c[k] + a[k] * sn[k];
+            a[k] = ra;
+            b[k] = rb;
+        }
+    }
+    if (is_q) {
         T* dst = q_out + ((int64_t)t * n_heads + h) * D + i0;
         store8(dst, a);
         store8(dst + half, b);
         return;
     }
-    const int kh = h - n_heads - (is_v ? n_kv : 0), pos = positions[t], seq = seq_of_token[t];
-    double a[8], b[8];
-    {
-        float fa[8], fb[8];
-        if (parts) {
-            load8(parts + base, fa);
-            load8(parts + base + half, fb);
-        } else {
-            load8(qkv + base, fa);
-            load8(qkv + base + half, fb);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            a[k] = (double)fa[k];
-            b[k] = (double)fb[k];
-        }
-        for (int sp = 1; parts && sp < splits; ++sp) {
-            load8(parts + sp * split_stride + base, fa);
-            load8(parts + sp * split_stride + base + half, fb);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                a[k] += (double)fa[k];
-                b[k] += (double)fb[k];
-            }
-        }
-    }
-    if (w) {
-        double ss = 0.0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ss += a[k] * a[k] + b[k] * b[k];
-        if (D == 192) {
-            ss += __shfl_xor_sync(mask, ss, 1);
-            ss += __shfl_xor_sync(mask, ss, 2);
-            const int l0 = (threadIdx.x & 31) / L * L;
-            ss = __shfl_sync(mask, ss, l0) + __shfl_sync(mask, ss, l0 + 4) + __shfl_sync(mask, ss, l0 + 8);
-        } else {
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        }
-        const double scale = 1.0 / sqrt(ss / (double)D + (double)eps);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            a[k] = (a[k] * scale) * (double)wa[k];
-            b[k] = (b[k] * scale) * (double)wb[k];
-        }
-    }
-    if (rotate) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const double ra = a[k] * (double)c[k] - b[k] * (double)sn[k], rb = b[k] * (double)c[k] + a[k] * (double)sn[k];
-            a[k] = ra;
-            b[k] = rb;
-        }
-    }
-    Codes out;
-    encode(a, mask, is_v, out.word[0], out.scale[0]);
-    encode(b, mask, is_v, out.word[1], out.scale[1]);
-    if (seq < 0 || seq >= n_seqs) {
-        atomicCAS(status, 0, 15);
+    // What the numbers can be off by, in roundings u of 32 bits, from what 64 bits give: their own 1 (0 for one run); the scale's 4 (the sum's
+    // to 32 bits, of which a root keeps half, root, reciprocal, and what the numbers' do to it); two products 2; the rotation's products and sum 2, of two terms.
+    largest = fmaxf(largest, __shfl_xor_sync(mask, largest, 1));
+    largest = fmaxf(largest, __shfl_xor_sync(mask, largest, 2));
+    turn = fmaxf(turn, __shfl_xor_sync(mask, turn, 1));
+    turn = fmaxf(turn, __shfl_xor_sync(mask, turn, 2));
+    const float off = (w ? (rotate ? 18.5f : 7.5f) : (parts && splits > 1 ? (rotate ? 6.5f : 1.5f) : (rotate ? 4.5f : 0.f))) * 5.9604645e-8f * largest * turn;
+    uint32_t word[2], scale[2];
+    bool sure = encode(a, off, mask, word[0], scale[0]);
+    sure = encode(b, off, mask, word[1], scale[1]) && sure;
+    if (__all_sync(mask, sure)) {
+        store_codes(head, row, i0, is_v, 0, word[0], scale[0]);
+        store_codes(head, row, i0, is_v, 1, word[1], scale[1]);
         return;
     }
-    const int64_t page = page_of(page_table, table_width, kv_pages, seq, pos, status);
-    if (page < 0) return;
-    const int row = pos % kPage;
-    uint8_t* dst = kv + (page * n_kv + kh) * head_bytes(D);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const int ch = i0 + s * half, o = ch / 2;
-        uint8_t* codes = dst + (is_v ? value_codes(D) + row * half + value_byte<D>(row, o) : row * half + o);
-        *reinterpret_cast<uint32_t*>(codes) = out.word[s];
-        if ((ch & (GROUP - 1)) == 0)
-            *reinterpret_cast<uint32_t*>(dst + (is_v ? value_scales(D) : key_scales(D)) + (row * (D / GROUP) + ch / GROUP) * 4) = out.scale[s];
-    }
+    const Source s = source();
+    vector_again<T>(&s);
 }
 
 // ---- reading tokens back ---------------------------------------------------------
@@ -403,7 +548,8 @@ static int append(const void* qkv, const float* parts, int splits, int n_tokens,
     const int rows = ceil_div(vectors, 128 / L);
     WICK_REQUIRE(rows <= 65535, "qk_norm_rope_append_kv4: %d heads are beyond the grid's limit", vectors);
     if (n_tokens == 0) return 0;
-    WICK_CUDA(launch(append_kernel<T>, dim3(n_tokens, rows), dim3(128), 0, (cudaStream_t)stream, (const T*)qkv, parts, splits,
+    // (A step of few tokens waits for its slowest vector, which had better not be one that is computed twice: 64 tokens 5.3 us so, 13 with the second look.)
+    WICK_CUDA(launch(n_tokens <= 256 ? append_kernel<T, true> : append_kernel<T, false>, dim3(n_tokens, rows), dim3(128), 0, (cudaStream_t)stream, (const T*)qkv, parts, splits,
                      (int64_t)n_tokens * (n_heads + 2 * n_kv) * D, n_tokens, n_heads, n_kv, q_w, k_w, eps, cos_t, sin_t, (T*)q_out, (uint8_t*)kv,
                      kv_pages, page_table, table_width, n_seqs, seq_of_token, positions, write_kv, status));
     return check_launch("qk_norm_rope_append_kv4");
