@@ -21,11 +21,188 @@
 // the positions 0, 1, 3, 2, 4, 5, 7, 6 of eight, so that either reading touches every bank of the shared memory once.
 //
 // The float32 form (and the plain twin of the other): CUDA cores, the same leaves' values, everything in 32 bits.
-#include "attn_kv4.cuh"
+#include "kv4.cuh"
 #include "packed.cuh"
+#include "tc_attention.cuh"
+
+#ifndef WICK_HD
+#error "compile with -DWICK_HD=<head_dim>"
+#endif
 
 namespace wick {
 namespace kv4 {
+
+constexpr int D = WICK_HD;
+static_assert(D % 64 == 0 && D >= 64 && D <= 256, "head sizes of 64, 128, 192 and 256");
+typedef __nv_bfloat16 bf16;
+
+constexpr int LEAVES = 8;                                        // of a node; warps of a block
+constexpr int THREADS = LEAVES * 32;
+constexpr int TILE = head_bytes(D);                              // a page of one key head
+constexpr int NW = D / 32;                                       // words of a key that a lane reads (its quarter of the row)
+constexpr int NV = D / 64;                                       // words of a value that a lane reads (its eighth)
+constexpr int MAX_STAGES = D <= 128 ? 2 : 1;                      // of a warp's ring (eight rings of two larger tiles are more than an SM has)
+constexpr int CLUSTER = 8;                                       // nodes that a cluster joins at most
+constexpr int MAX_SEQS = 1024;                                   // of the form whose blocks stay
+constexpr int MT = D / 16;                                       // tiles of 16 channels
+
+// Nodes of the longest sequences: enough that one sequence alone gives every SM two blocks (8 key heads: 37), no more (each costs a record).  Two of 131,000
+// positions, 64 heads over 8 of 128: with 16 nodes 90 us (256 blocks on 148 SMs), now 81.
+__host__ __device__ inline int most_nodes(int n_kv) {
+    const int n = 296 / n_kv;
+    return n < 4 ? 4 : (n > 128 ? 128 : n);
+}
+__host__ __device__ inline int leaf_pages(int n_pages, int n_kv) {
+    const int most = LEAVES * most_nodes(n_kv);
+    return n_pages <= most ? 1 : (n_pages + most - 1) / most;
+}
+__host__ __device__ inline int nodes_of(int n_pages, int n_kv) {
+    const int n = LEAVES * leaf_pages(n_pages, n_kv);
+    return (n_pages + n - 1) / n;
+}
+
+struct Args {
+    const void* q;                                               // [n_tokens, n_heads, d]
+    void* out;
+    const uint8_t* kv;
+    int64_t kv_pages;
+    const int* cu_seqlens;
+    const int* start;
+    const int* page_table;
+    int table_width, n_seqs, n_heads, n_kv, group;
+    float scale2;                                                // |scale| log2 e
+    uint32_t flip;                                               // sign bits of two bfloat16 numbers if the scale is negative (the queries then change sign), else 0
+    int n_tokens, max_q, pages;                                  // the most new tokens of a sequence, and the most pages that there are places for
+    float* rec;                                                  // records: accumulators [row, node, d], then maximum and sum [row, node, 2]; a row is a (token, head)
+    int64_t rec_rows;
+    int nodes;                                                   // places for nodes in a row's records
+    int tiles;                                                   // row tiles of a (sequence, key head) that the grid has
+    int stages;                                                  // of a warp's ring
+    int* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^(a - b) for maxima that may be -inf (nothing seen yet): then the weight is 0.
+__device__ __forceinline__ float weight(float a, float b) { return a == -INFINITY ? 0.f : ex2(a - b); }
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same with nothing to add to.
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// An 8 x 8 matrix of 16-bit elements, a row per four lanes: the transposed one in the same layout.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ bool no_number(uint32_t scale) { return (scale & 0x7F80u) == 0x7F80u || (scale & 0x7F800000u) == 0x7F800000u; }
+// The position (of 8) in row i of the instruction's position side.
+__device__ __forceinline__ int position_of(int i) { return i ^ ((i >> 1) & 1); }
+
+// A sequence's place in the step, as far as its rows see it.
+struct Seq {
+    int first, new_tokens, start, len, pages;                    // flat number of its first new token; ...; pages that fit its table
+};
+__device__ __forceinline__ Seq sequence(const Args& a, int b) {
+    Seq s;
+    s.first = a.cu_seqlens[b];
+    s.new_tokens = a.cu_seqlens[b + 1] - s.first;
+    s.start = a.start[b];
+    s.len = s.start + s.new_tokens;
+    s.pages = (s.len + kPage - 1) / kPage;
+    return s;
+}
+// Whether a sequence fits the step, its page table and the records' places (else it is left out, and said).
+__device__ __forceinline__ bool fits(const Args& a, const Seq& s) {
+    const bool ok = s.start >= 0 && s.first >= 0 && s.first + s.new_tokens <= a.n_tokens && s.new_tokens <= a.max_q && s.pages <= a.table_width && s.pages <= a.pages;
+    if (!ok) atomicCAS(a.status, 0, 15);
+    return ok;
+}
+// A page id, within the cache (else reported, and page 0).
+__device__ __forceinline__ int checked_page(const Args& a, int id) {
+    if (id < 0 || id >= a.kv_pages) {
+        atomicCAS(a.status, 0, 15);
+        return 0;
+    }
+    return id;
+}
+__device__ __forceinline__ void start_copy(const Args& a, int page, int kvh, uint8_t* dst, uint64_t* bar) {
+    mbar_expect_tx(bar, TILE);
+    bulk_load(dst, a.kv + ((int64_t)page * a.n_kv + kvh) * TILE, TILE, bar);
+}
+
+// The fold of a leaf (or a node) p into what came before, the same operations wherever it is done:
+//   M' = max(M, m_p);  l = l 2^(M - M') + l_p 2^(m_p - M');  o likewise.
+struct Fold {
+    float m, l, was, now;
+    __device__ __forceinline__ void step(float mp, float lp) {
+        const float t = fmaxf(m, mp);
+        was = weight(m, t);
+        now = weight(mp, t);
+        l = of(l, lp);
+        m = t;
+    }
+    __device__ __forceinline__ float of(float o, float op) const { return __fmaf_rn(op, now, __fmul_rn(o, was)); }
+};
+// The same for the neighbours 2 j, 2 j + 1 of a lane's rows, two numbers an instruction.
+__device__ __forceinline__ void fold_pair(const Fold (&f)[2], float& o0, float& o1, float p0, float p1) {
+    const float2 r = fma2(make_float2(p0, p1), make_float2(f[0].now, f[1].now), mul2(make_float2(o0, o1), make_float2(f[0].was, f[1].was)));
+    o0 = r.x;
+    o1 = r.y;
+}
+__device__ __forceinline__ float result(float o, float l) { return __fmul_rn(o, __fdiv_rn(1.0f, l)); }
+
+// Row i of a tile's unit n (rows 8 n ..): where its token's head lies in the step, or -1.
+__device__ __forceinline__ int64_t flat_row(const Args& a, const Seq& s, int kvh, int row) {
+    if (row >= s.new_tokens * a.group) return -1;
+    const int tok = row / a.group;
+    return (int64_t)(s.first + tok) * a.n_heads + kvh * a.group + (row - tok * a.group);
+}
+// A lane's four numbers of tile i (channels r d / 8 + 2 i and + 1 of rows 2 j and 2 j + 1): the result, or a node's record.
+__device__ __forceinline__ void write_result(const Args& a, int64_t flat, int ch, float x, float y, float l) {
+    *reinterpret_cast<uint32_t*>((bf16*)a.out + flat * D + ch) = pack_bf16(result(x, l), result(y, l));
+}
+__device__ __forceinline__ void write_record(const Args& a, int64_t flat, int node, int ch, float x, float y) {
+    *reinterpret_cast<float2*>(a.rec + (flat * a.nodes + node) * D + ch) = make_float2(x, y);
+}
+__device__ __forceinline__ void write_weights(const Args& a, int64_t flat, int node, float m, float l) {
+    *reinterpret_cast<float2*>(a.rec + a.rec_rows * a.nodes * D + (flat * a.nodes + node) * 2) = make_float2(m, l);
+}
+
+__device__ __forceinline__ uint32_t in_block(uint32_t smem, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Which kernels a call of these sizes launches, and what they need.
+enum Form { AUTO = 0, PLAIN = 1, RECORDS = 2, CLUSTERS = 3, STAY = 4 };
+struct Plan {
+    bool possible;
+    int form, nt, tiles, nodes, stages, kernels;
+    int64_t scratch, blocks;
+};
 
 // ---- one page on the tensor cores -------------------------------------------------------
 template <int NT> struct Sum {                                   // of a leaf or a node: lane (r, j) = (lane / 4, lane % 4) holds rows 2 j, 2 j + 1 of every eight,
@@ -155,41 +332,48 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
     uint32_t p[4][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        float top[2] = {-INFINITY, -INFINITY};
+        if (MASK) {
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (first + mt * 16 + 8 * (e >> 1) + tr > w.limit[n][e & 1]) s[mt][n][e] = -INFINITY;
+        }
+        float was[2], ref[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float top = max3(max3(s[0][n][c], s[0][n][c + 2], s[1][n][c]), max3(s[1][n][c + 2], s[2][n][c], s[2][n][c + 2]), fmaxf(s[3][n][c], s[3][n][c + 2]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float mine = top == -INFINITY ? top : top * scale2, m = FRESH ? mine : fmaxf(sum.m[n][c], mine);
+            was[c] = FRESH ? 0.f : weight(sum.m[n][c], m);
+            ref[c] = m == -INFINITY ? 0.f : -m;                  // (nothing seen: weights 0; a score that is no number still shows)
+            sum.m[n][c] = m;
+        }
+        float2 l = make_float2(0.f, 0.f);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (MASK && first + mt * 16 + 8 * (e >> 1) + tr > w.limit[n][e & 1]) s[mt][n][e] = -INFINITY;
-                top[e & 1] = fmaxf(top[e & 1], s[mt][n][e]);
+            for (int h = 0; h < 4; h += 2) {
+                const float2 x = fma2(make_float2(s[mt][n][h], s[mt][n][h + 1]), make_float2(scale2, scale2), make_float2(ref[0], ref[1]));
+                // (a scale of 0 and a position that is not seen would else give a number that is none)
+                const float2 y = make_float2(MASK && s[mt][n][h] == -INFINITY ? 0.f : ex2(x.x), MASK && s[mt][n][h + 1] == -INFINITY ? 0.f : ex2(x.y));
+                s[mt][n][h] = y.x;
+                s[mt][n][h + 1] = y.y;
+                l = add2(l, y);
             }
+        sum.l[n][0] = FRESH ? l.x : sum.l[n][0] * was[0] + l.x;
+        sum.l[n][1] = FRESH ? l.y : sum.l[n][1] * was[1] + l.y;
+        if (!FRESH && __any_sync(0xffffffffu, was[0] != 1.f || was[1] != 1.f)) {
+            const float2 f = make_float2(was[0], was[1]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-            const float mine = top[c] == -INFINITY ? top[c] : top[c] * scale2, m = FRESH ? mine : fmaxf(sum.m[n][c], mine);
-            const float was = FRESH ? 0.f : weight(sum.m[n][c], m);
-            const float ref = m == -INFINITY ? 0.f : m;          // (nothing seen: weights 0; a score that is no number still shows)
-            sum.m[n][c] = m;
-            float l = 0.f;
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float& x = s[mt][n][c + 2 * h];
-                    const float y = ex2(fmaf(x, scale2, -ref));
-                    x = MASK && x == -INFINITY ? 0.f : y;        // (a scale of 0 and nothing else makes a difference)
-                    l += x;
+                for (int h = 0; h < 4; h += 2) {
+                    const float2 x = mul2(make_float2(sum.o[i][n][h], sum.o[i][n][h + 1]), f);
+                    sum.o[i][n][h] = x.x;
+                    sum.o[i][n][h + 1] = x.y;
                 }
-            }
-            sum.l[n][c] = FRESH ? l : sum.l[n][c] * was + l;
-            if (!FRESH) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    sum.o[i][n][c] *= was;
-                    sum.o[i][n][c + 2] *= was;
-                }
-            }
         }
         // The weights enter the second product as bfloat16 numbers (the sum above has them unrounded: at most 2^-9 each, as in the other kernels).
 #pragma unroll
@@ -474,46 +658,46 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
 }
 
 // ---- blocks that stay ------------------------------------------------------------------------
-// One row tile a sequence and key head (one new token, up to eight heads).  A block has an equal run of the step's nodes (BY_LEAF: of its leaves), and its
-// warps take the next one whenever they are done with one.  A warp's tile is filled again while it is read: the next page's keys as soon as the scores are
-// there, its values when the page is done.
+// A block has an equal run of the step's items (a node of a row tile of a key head of a sequence each), and its warps take the next one whenever they are done
+// with one.  A warp's tile is filled again while it is read: the next page's keys as soon as the scores are there, its values when the page is done.
+// One unit of rows (NT 1): a node's leaves are folded in registers.  More: there is no room for a second accumulator, and a node is one leaf.
 struct Item {
-    int b, kvh, place, nodes, lp;                                // place: the node's number in the sequence (BY_LEAF: the leaf's); none left: b < 0
-    int page, end;                                               // of the sequence
+    int b, kvh, row0, place, lp;                                 // place: the node's number in the sequence; none left: b < 0
+    int page, end;                                               // of the sequence, as far as the row tile sees
+    int alone;                                                   // the sequence has one node
 };
+template <int NT> constexpr int stay_warps() { return NT > 1 || D > 128 ? 8 : (D == 64 ? 16 : 12); }      // (as many as registers allow)
 
-template <bool BY_LEAF>
-__global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) {
+template <int NT>
+__global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Args a) {
+    constexpr int WARPS = stay_warps<NT>();
     extern __shared__ __align__(128) uint8_t ring_all[];
-    __shared__ uint64_t full[STAY_WARPS][2];                     // keys, values
-    __shared__ int cum[MAX_SEQS + 1], lens[MAX_SEQS], firsts[MAX_SEQS];      // items before a sequence; its length (with a new token) and the token
+    __shared__ uint64_t full[WARPS][2];                          // keys, values
+    __shared__ int cum[MAX_SEQS + 1], lens[MAX_SEQS], firsts[MAX_SEQS + 1];  // items before a sequence; its length (with new tokens) and the first of these
     __shared__ int abort_flag, taken;
-    constexpr int PER = BY_LEAF ? 1 : LEAVES;                    // leaves of an item
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int w = 0; w < STAY_WARPS; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             mbar_init(&full[w][0], 1);
             mbar_init(&full[w][1], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    for (int b = threadIdx.x; b < a.n_seqs; b += WARPS * 32) {
+        const Seq s = sequence(a, b);
+        cum[b + 1] = s.new_tokens > 0 && fits(a, s) ? nodes_of(s.pages, a.n_kv) * ((s.new_tokens * a.group + 8 * NT - 1) / (8 * NT)) * a.n_kv : 0;
+        lens[b] = s.len;
+        firsts[b] = s.first;
+        if (b == a.n_seqs - 1) firsts[b + 1] = s.first + s.new_tokens;
+    }
+    __syncthreads();
     if (warp == 0) {
         int before = 0;
 #pragma unroll 1
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-            const int b = s0 + lane;
-            int mine = 0;
-            if (b < a.n_seqs) {
-                const Seq s = sequence(a, b);
-                if (s.new_tokens > 0 && fits(a, s)) {
-                    const int lp = PER * leaf_pages(s.pages, a.n_kv);
-                    mine = (s.pages + lp - 1) / lp * a.n_kv;
-                }
-                lens[b] = s.len;
-                firsts[b] = s.first;
-            }
+            const int b = s0 + lane, mine = b < a.n_seqs ? cum[b + 1] : 0;
             int upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -533,28 +717,43 @@ __global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) 
     pdl_wait();
     uint8_t* tile = ring_all + (size_t)warp * TILE;
 
+    auto place_of = [&](int b) {
+        Seq s;
+        s.first = firsts[b];
+        s.new_tokens = firsts[b + 1] - s.first;
+        s.len = lens[b];
+        s.start = s.len - s.new_tokens;
+        s.pages = (s.len + kPage - 1) / kPage;
+        return s;
+    };
     auto take = [&](Item& n, int& ids) {
-        int u = 0;
-        if (lane == 0) u = atomicAdd(&taken, 1);
-        u = __shfl_sync(0xffffffffu, u, 0);
-        n.b = -1;
-        if (u >= stop) return;
-        int lo = 0, hi = a.n_seqs - 1;                           // the last sequence with cum[b] <= u
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (cum[mid] <= u) lo = mid;
-            else hi = mid - 1;
+        while (true) {
+            int u = 0;
+            if (lane == 0) u = atomicAdd(&taken, 1);
+            u = __shfl_sync(0xffffffffu, u, 0);
+            n.b = -1;
+            if (u >= stop) break;
+            int lo = 0, hi = a.n_seqs - 1;                       // the last sequence with cum[b] <= u
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (cum[mid] <= u) lo = mid;
+                else hi = mid - 1;
+            }
+            n.b = lo;
+            const Seq s = place_of(lo);
+            const int local = u - cum[lo], n_rows = s.new_tokens * a.group, tiles = (n_rows + 8 * NT - 1) / (8 * NT), nodes = nodes_of(s.pages, a.n_kv);
+            n.lp = leaf_pages(s.pages, a.n_kv);
+            n.place = local % nodes;
+            n.row0 = NT == 1 && tiles == 1 ? 0 : local / nodes % tiles * 8 * NT;
+            n.kvh = local / (nodes * tiles);
+            n.alone = nodes == 1;
+            const int seen = (s.start + (min(n.row0 + 8 * NT, n_rows) - 1) / a.group) / kPage + 1;
+            n.page = n.place * LEAVES * n.lp;
+            n.end = min(seen, n.page + LEAVES * n.lp);
+            if (n.page >= seen) continue;                        // (the tile's rows see none of it)
+            ids = n.page + lane < n.end ? checked_page(a, a.page_table[(int64_t)lo * a.table_width + n.page + lane]) : 0;
+            break;
         }
-        n.b = lo;
-        const int pages = (lens[lo] + kPage - 1) / kPage, local = u - cum[lo];
-        n.lp = leaf_pages(pages, a.n_kv);
-        const int items = (pages + PER * n.lp - 1) / (PER * n.lp);
-        n.nodes = (pages + LEAVES * n.lp - 1) / (LEAVES * n.lp);
-        n.kvh = local / items;
-        n.place = local - n.kvh * items;
-        n.page = n.place * PER * n.lp;
-        n.end = min(pages, n.page + PER * n.lp);
-        ids = n.page + lane < n.end ? checked_page(a, a.page_table[(int64_t)lo * a.table_width + n.page + lane]) : 0;
     };
     auto start_half = [&](int id, int kvh, int half) {           // keys or values of a page: their codes and their scales
         if (lane == 0) {
@@ -573,37 +772,38 @@ __global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) 
         start_half(id, cn.kvh, 0);
         start_half(id, cn.kvh, 1);
     }
-    Seq s;
-    s.new_tokens = 1;
-    s.first = firsts[cn.b];
-    Rows<1> w;
-    fetch_rows<1>(a, s, cn.kvh, 0, w);
+    Rows<NT> w;
+    fetch_rows<NT>(a, place_of(cn.b), cn.kvh, cn.row0, w);
     bool ok = true;
 #pragma unroll 1
     while (true) {
-        s.len = lens[cn.b];
-        s.start = s.len - 1;
-        s.first = firsts[cn.b];
-        order_rows<1>(a, w);
-        w.limit[0][0] = w.limit[0][1] = s.start;
+        const Seq s = place_of(cn.b);
+        order_rows<NT>(a, w);
+        const int n_rows = s.new_tokens * a.group;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) w.limit[n][c] = s.start + min(cn.row0 + 8 * n + 2 * j + c, n_rows - 1) / a.group;
         take(nn, next_ids);
         Fold f[2];
-        float o[MT][4];
-        f[0].m = f[1].m = -INFINITY;
-        f[0].l = f[1].l = 0.f;
+        float o[NT == 1 ? MT : 1][4];
+        Sum<NT> sum;
+        if (NT == 1) {
+            f[0].m = f[1].m = -INFINITY;
+            f[0].l = f[1].l = 0.f;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+            for (int i = 0; i < (NT == 1 ? MT : 1); ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        }
         int held = 0;                                            // of the 32 ids that the lanes have
 #pragma unroll 1
         for (int page = cn.page; page < cn.end;) {
-            Sum<1> sum;
-            const int leaf_end = min(cn.end, page + cn.lp);
+            const int leaf_end = NT == 1 ? min(cn.end, page + cn.lp) : cn.end;
             bool fresh = true;
 #pragma unroll 1
             for (; page < leaf_end; ++page) {
                 int next_id = -1, next_kvh = cn.kvh;
                 ok = ok && mbar_wait(&full[warp][0], parity, &abort_flag, a.status, 16);
-                leaf_page<1>(a, tile, w, s, page, fresh, sum, [&]() {
+                leaf_page<NT>(a, tile, w, s, page, fresh, sum, [&]() {
                     if (page + 1 < cn.end) {
                         if (++held == 32) {
                             held = 0;
@@ -616,12 +816,8 @@ __global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) 
                     }
                     __syncwarp();
                     if (next_id >= 0) start_half(next_id, next_kvh, 0);
-                    if (page + 1 == cn.end && nn.b >= 0) {       // (the queries are not needed any more: the next item's are asked for)
-                        Seq t;
-                        t.new_tokens = 1;
-                        t.first = firsts[nn.b];
-                        fetch_rows<1>(a, t, nn.kvh, 0, w);
-                    }
+                    // (the queries are not needed any more behind a node's last scores: the next item's are asked for)
+                    if (NT == 1 && page + 1 == cn.end && nn.b >= 0) fetch_rows<NT>(a, place_of(nn.b), nn.kvh, nn.row0, w);
                     ok = mbar_wait(&full[warp][1], parity, &abort_flag, a.status, 16) && ok;
                 });
                 fresh = false;
@@ -636,30 +832,34 @@ __global__ void __launch_bounds__(STAY_WARPS * 32, 1) stay_kernel(const Args a) 
                     return;
                 }
             }
-            finish_leaf<1>(sum);
+            finish_leaf<NT>(sum);
+            if constexpr (NT == 1) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                f[c].step(sum.m[0][c], sum.l[0][c]);
+                for (int c = 0; c < 2; ++c) f[c].step(sum.m[0][c], sum.l[0][c]);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    o[i][c] = f[c].of(o[i][c], sum.o[i][0][c]);
-                    o[i][c + 2] = f[c].of(o[i][c + 2], sum.o[i][0][c + 2]);
+                    fold_pair(f, o[i][0], o[i][1], sum.o[i][0][0], sum.o[i][0][1]);
+                    fold_pair(f, o[i][2], o[i][3], sum.o[i][0][2], sum.o[i][0][3]);
                 }
             }
         }
-        const bool whole = cn.end - cn.page == (s.len + kPage - 1) / kPage;      // (the item is all of the sequence)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int64_t flat = 2 * j + c < a.group ? (int64_t)s.first * a.n_heads + cn.kvh * a.group + 2 * j + c : -1;
-            if (flat < 0) continue;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if (whole) write_result(a, flat, r * (D / 8) + 2 * i, o[i][c], o[i][c + 2], f[c].l);
-                else write_record(a, flat, cn.place, r * (D / 8) + 2 * i, o[i][c], o[i][c + 2]);
+            for (int c = 0; c < 2; ++c) {
+                const int64_t flat = flat_row(a, s, cn.kvh, cn.row0 + 8 * n + 2 * j + c);
+                if (flat < 0) continue;
+                const float l = NT == 1 ? f[c].l : sum.l[n][c];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const float x = NT == 1 ? o[NT == 1 ? i : 0][c] : sum.o[i][n][c], y = NT == 1 ? o[NT == 1 ? i : 0][c + 2] : sum.o[i][n][c + 2];
+                    if (cn.alone) write_result(a, flat, r * (D / 8) + 2 * i, x, y, l);
+                    else write_record(a, flat, cn.place, r * (D / 8) + 2 * i, x, y);
+                }
+                if (!cn.alone && r == 0) write_weights(a, flat, cn.place, NT == 1 ? f[c].m : sum.m[n][c], l);
             }
-            if (!whole && r == 0) write_weights(a, flat, cn.place, f[c].m, f[c].l);
-        }
         if (nn.b < 0) return;
+        if (NT > 1) fetch_rows<NT>(a, place_of(nn.b), nn.kvh, nn.row0, w);
         cn = nn;
         ids = next_ids;
     }
@@ -888,22 +1088,17 @@ static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int
     const int64_t rows = (int64_t)max_q * (n_heads / n_kv);
     p.nodes = nodes_of(pages, n_kv);
     p.form = f32 && form == AUTO ? PLAIN : form;
-    const bool can_stay = rows <= 8 && n_seqs <= MAX_SEQS, can_tc = D == 128 && n_seqs <= MAX_SEQS;
-    p.possible = p.form >= AUTO && p.form <= TC_CLUSTERS && !(f32 && p.form != PLAIN) && !((p.form == STAY || p.form == STAY_LEAVES) && !can_stay) &&
-                 !(p.form >= TC && !can_tc) && !((p.form == CLUSTERS || p.form == TC_CLUSTERS) && p.nodes > CLUSTER);
-    const int64_t nodes = (int64_t)n_seqs * n_kv * p.nodes;
-    if (p.form == AUTO && can_tc && rows > 8)
-        p.form = p.nodes <= CLUSTER && nodes <= 2 * sm_count() ? TC_CLUSTERS : TC;
-    else if (p.form == AUTO)
-        p.form = can_stay && nodes >= 2 * (int64_t)LEAVES * sm_count() ? STAY : (p.nodes <= CLUSTER && nodes <= 2 * sm_count() ? CLUSTERS : RECORDS);
-    const bool tc = p.form >= TC;
+    const bool can_stay = n_seqs <= MAX_SEQS;
+    p.possible = p.form >= AUTO && p.form <= STAY && !(f32 && p.form != PLAIN) && !(p.form == STAY && !can_stay) && !(p.form == CLUSTERS && p.nodes > CLUSTER);
     p.nt = p.form == PLAIN || rows <= 8 ? 1 : (rows <= 16 || D > 128 ? 2 : 3);
-    p.rows = p.form == PLAIN ? 8 : (tc ? (rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 24 ? 24 : 32))) : 8 * p.nt);
-    p.tiles = (int)((rows + p.rows - 1) / p.rows);
+    p.tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
+    const int64_t nodes = (int64_t)n_seqs * n_kv * p.nodes * p.tiles;
+    if (p.form == AUTO)
+        p.form = can_stay && nodes >= (p.nt == 1 ? 2 : 1) * (int64_t)LEAVES * sm_count() ? STAY : (p.nodes <= CLUSTER && nodes <= 2 * sm_count() ? CLUSTERS : RECORDS);
     p.stages = leaf_pages(pages, n_kv) > 1 || p.nt == 3 ? MAX_STAGES : 1;
-    if (p.form == STAY_LEAVES || p.form == PLAIN) p.nodes = (pages + leaf_pages(pages, n_kv) - 1) / leaf_pages(pages, n_kv);      // (places for records)
-    p.blocks = p.form == STAY || p.form == STAY_LEAVES || p.form == TC ? sm_count() : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
-    const bool records = p.nodes > 1 && p.form != CLUSTERS && p.form != TC_CLUSTERS;
+    if (p.form == PLAIN) p.nodes = (pages + leaf_pages(pages, n_kv) - 1) / leaf_pages(pages, n_kv);      // (places for records)
+    p.blocks = p.form == STAY ? sm_count() : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
+    const bool records = p.nodes > 1 && p.form != CLUSTERS;
     p.scratch = records ? (int64_t)n_tokens * n_heads * p.nodes * (D + 2) : 0;
     p.kernels = records ? 2 : 1;
     return p;
@@ -911,8 +1106,8 @@ static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int
 
 // Dynamic shared memory beyond what a kernel has without asking.
 static int allow(void (*kernel)(Args), int bytes) {
-    static void (*asked[8])(Args) = {};                          // (two host threads may both ask: it does no harm)
-    for (int i = 0; i < 8; ++i) {
+    static void (*asked[16])(Args) = {};                          // (two host threads may both ask: it does no harm)
+    for (int i = 0; i < 16; ++i) {
         if (asked[i] == kernel) return 0;
         if (asked[i] == nullptr) {
             WICK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
@@ -963,12 +1158,11 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     const dim3 grid((unsigned)p.blocks);
     if (p.form == PLAIN) {
         WICK_CUDA(launch(plain_kernel<T>, grid, dim3(256), 0, st, a));
-    } else if (p.form >= TC) {
-        if (int rc = launch_tc(a, p.rows, p.form == TC_CLUSTERS, p.blocks, st)) return rc;
-    } else if (p.form >= STAY) {
-        void (*kernel)(Args) = p.form == STAY ? stay_kernel<false> : stay_kernel<true>;
-        if (int rc = allow(kernel, STAY_WARPS * TILE)) return rc;
-        WICK_CUDA(launch(kernel, grid, dim3(STAY_WARPS * 32), STAY_WARPS * TILE, st, a));
+    } else if (p.form == STAY) {
+        void (*kernel)(Args) = p.nt == 1 ? stay_kernel<1> : (p.nt == 2 ? stay_kernel<2> : stay_kernel<D <= 128 ? 3 : 2>);
+        const int warps = p.nt == 1 ? stay_warps<1>() : stay_warps<2>();
+        if (int rc = allow(kernel, warps * TILE)) return rc;
+        WICK_CUDA(launch(kernel, grid, dim3(warps * 32), warps * TILE, st, a));
     } else {
         const bool clusters = p.form == CLUSTERS && p.nodes > 1;
         void (*kernel)(Args) = p.nt == 1 ? (clusters ? leaves_kernel<1, true> : leaves_kernel<1, false>) : p.nt == 2 ? (clusters ? leaves_kernel<2, true> : leaves_kernel<2, false>) : (clusters ? leaves_kernel<D <= 128 ? 3 : 2, true> : leaves_kernel<D <= 128 ? 3 : 2, false>);
@@ -990,7 +1184,7 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     }
     if (int rc = check_launch("attention_kv4")) return rc;
     if (p.kernels == 2) {
-        WICK_CUDA(launch(p.form == STAY_LEAVES || p.form == PLAIN ? join_kernel<T, true> : join_kernel<T, false>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, st, a, seq_of_token, n_tokens));
+        WICK_CUDA(launch(p.form == PLAIN ? join_kernel<T, true> : join_kernel<T, false>, dim3((unsigned)(((int64_t)n_tokens * n_heads + 3) / 4)), dim3(128), 0, st, a, seq_of_token, n_tokens));
         return check_launch("attention_kv4 (join)");
     }
     return 0;

@@ -18,7 +18,7 @@ from .. import ops
 from ..layout import PAGE, pages_for
 from . import KernelError, _cuda, _Lib, _libs, _need, _stream, attention_prompt, status_tensor
 
-KV4_SOURCES = ["kv4.cu", "attn_kv4.cu", "attn_kv4_tc.cu"]
+KV4_SOURCES = ["kv4.cu", "attn_kv4.cu"]
 KV4_HEAD_DIMS = (64, 128, 192, 256)
 
 _by_size: Dict[int, _Lib] = {}
@@ -166,7 +166,7 @@ OPEN_ROWS = 32
 
 
 # The kernels of attention_kv4 by name (csrc/attn_kv4.cu: Plan); "opened": pages opened to bfloat16, then the prompt attention.
-_FORMS = {None: 0, "plain": 1, "records": 2, "clusters": 3, "stay": 4, "stay_leaves": 5, "tc": 6, "tc_clusters": 7, "opened": -1}
+_FORMS = {None: 0, "plain": 1, "records": 2, "clusters": 3, "stay": 4, "opened": -1}
 
 
 @functools.lru_cache(maxsize=4096)
