@@ -276,6 +276,35 @@ def test_long_sequences(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_shorter_sequence_of_more_pieces(dtype):
+    """80 key heads: 32 pages are cut into 32 pieces, 33 into half as many."""
+    o = ops()
+    g = torch.Generator().manual_seed(33)
+    pages, b = step([33 * PAGE - 1, 32 * PAGE - 3, 31 * PAGE], [1, 2, 1], g)
+    kv, cache = random_cache(pages, 80, 64, g)
+    q = torch.randn((4, 80, 64), generator=g).to(dtype).cuda()
+    for kind in (None, "plain") + (("records", "clusters", "stay") if dtype == BF16 else ()):
+        check_attention(q, o.attention_kv4(q, kv.cuda(), b, 0.125, kind=kind), cache, b, 0.125, 64)
+    o.check_status()
+
+
+@pytest.mark.parametrize("H,KV,d,starts,new,dtype", [(32, 16, 192, [70, 0, 5], [1250, 3, 0], BF16), (32, 16, 64, [0, 900], [150, 61], F32),
+                                                     (32, 16, 128, [0, 900], [150, 61], BF16)])
+def test_prompts_from_the_codes(H, KV, d, starts, new, dtype):
+    """So many row tiles that no sequence is cut."""
+    o = ops()
+    g = torch.Generator().manual_seed(d)
+    pages, b = step(starts, new, g, spare=2)
+    kv, cache = random_cache(pages, KV, d, g)
+    q = torch.randn((b.n_tokens, H, d), generator=g).to(dtype).cuda()
+    for kind in ("plain",) + (("records", "stay") if dtype == BF16 else ()):
+        check_attention(q, o.attention_kv4(q, kv.cuda(), b, 0.11, kind=kind), cache, b, 0.11, d)
+        if kind == "plain" or d == 192:
+            assert o.attention_kv4_scratch(b, H, KV, d, dtype, kind=kind) == 0
+    o.check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_alone_and_among_others(dtype):
     o = ops()
     g = torch.Generator().manual_seed(5)

@@ -84,3 +84,18 @@ def test_command_line_option():
     assert cli.parse_args(["run", "d", "--cache-bits", "4"]).cache_bits == 4 and cli.parse_args(["run", "d"]).cache_bits is None
     with pytest.raises(cli.UsageError):
         cli.parse_args(["run", "d", "--cache-bits", "8"])
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scratch_is_enough_for_shorter_sequences(d, dtype):
+    """A longer sequence may be cut into fewer pieces than a shorter one: a step has places for those of all lengths up to its bound."""
+    import types
+    from wick_b200 import ops
+    for kv in (1, 2, 8, 32, 80):
+        before = 0
+        for pages in list(range(1, 90)) + list(range(90, 3000, 37)):
+            b = types.SimpleNamespace(n_tokens=3, n_seqs=2, table_width=pages, max_q_len=2, kv_bound=64 * pages)
+            words = ops.attention_kv4_scratch(b, 4 * kv, kv, d, dtype, kind="plain" if dtype == torch.float32 else "records")
+            assert words >= before, (kv, pages)
+            before = words

@@ -2,16 +2,16 @@
 //
 //   out[i, h] = sum_t p_t v_t,  p = softmax over t <= position(i) of scale q[i, h] . k_t,  k_t and v_t the bfloat16 values that the codes stand for.
 //
-// How the work is cut.  The rows of a (sequence, key head) are its new tokens times the query heads of the key head; they come in tiles of eight or
-// sixteen.  The sequence's pages are cut by its OWN length and the number of key heads alone: into leaves of as many pages (one, for up to 8 most_nodes
-// pages) and nodes of eight leaves.  A leaf is computed by one warp, page by page, into a running maximum, sum and accumulator; a node's leaves
-// are folded in order, a row's nodes likewise.  Which warp computes what changes no bit, so that a sequence's result does not depend on the batch it is
-// in.  Three forms for bfloat16 (Plan has the rule):
+// How the work is cut.  The rows of a (sequence, key head) are its new tokens times the query heads of the key head; they come in tiles of 8, 16 or
+// 24.  The sequence's pages are cut by its OWN length and the number of key heads alone: into leaves of as many pages (leaf_pages) and nodes of eight
+// leaves.  A leaf is computed by one warp, page by page, into a running maximum, sum and accumulator; a node's leaves are folded in order, a row's nodes
+// likewise.  While all sequences have up to eight rows, which warp computes what changes no bit, and a sequence's result does not depend on the batch
+// it is in; with more rows tile, form and cut follow the whole step.  Three forms for bfloat16 (plan() has the rule):
 //   * a block per node, a warp per leaf: the leaves meet in shared memory.  A sequence's nodes, where they are up to CLUSTER, are a cluster whose blocks
 //     read each other's results and write the outcome; more leave records (accumulator, maximum, sum) that a second, small kernel joins.  Few nodes:
 //     as many warps as there are leaves work on a sequence;
-//   * blocks that stay, one per SM, with an equal run of all nodes (or leaves) of the step each, which their warps take one by one: a warp folds a node's
-//     leaves in registers, and its next page is on its way while it computes one.  Many nodes of one row tile each (decode steps); records as above.
+//   * blocks that stay, one per SM, with an equal run of all nodes of the step each, which their warps take one by one: a warp folds a node's leaves in
+//     registers (with more than eight rows a node is one leaf), and its next page is on its way while it computes one.  Many nodes; records as above.
 // A sequence with one node is written directly.
 //
 // The kernel on the tensor cores.  Keys and values stand on the 16-row side of mma.sync (16 positions, or 16 channels), the rows on the 8-column side, so
@@ -46,20 +46,20 @@ constexpr int CLUSTER = 8;                                       // nodes that a
 constexpr int MAX_SEQS = 1024;                                   // of the form whose blocks stay
 constexpr int MT = D / 16;                                       // tiles of 16 channels
 
-// Nodes of the longest sequences: enough that one sequence alone gives every SM two blocks (8 key heads: 37), no more (each costs a record).  Two of 131,000
-// positions, 64 heads over 8 of 128: with 16 nodes 90 us (256 blocks on 148 SMs), now 81.
-__host__ __device__ inline int most_nodes(int n_kv) {
-    const int n = 296 / n_kv;
-    return n < 4 ? 4 : (n > 128 ? 128 : n);
-}
+// A leaf is one page while one sequence alone so gives every SM up to two blocks (8 key heads: 37 nodes, 296 pages).  Longer sequences have nodes for one block
+// an SM (18) of long leaves, whose next page is on its way.  us, 32 heads over 8 of 128: 8 sequences of up to 12,000 positions, 24 nodes / 12 of twice the
+// leaves 40 / 49, one of 12,000 12.8 / 11.8; one of up to 32,000, 32 nodes of 2 pages a leaf / 16 of 4: 22 / 17; two of up to 131,000, 64 heads, 37 / 18: 80 / 72.
+__host__ __device__ inline int most_nodes(int n_kv, int blocks) { return max(4, min(128, blocks / n_kv)); }
 __host__ __device__ inline int leaf_pages(int n_pages, int n_kv) {
-    const int most = LEAVES * most_nodes(n_kv);
-    return n_pages <= most ? 1 : (n_pages + most - 1) / most;
+    const int most = LEAVES * most_nodes(n_kv, 148);
+    return n_pages <= LEAVES * most_nodes(n_kv, 296) ? 1 : (n_pages + most - 1) / most;
 }
 __host__ __device__ inline int nodes_of(int n_pages, int n_kv) {
     const int n = LEAVES * leaf_pages(n_pages, n_kv);
     return (n_pages + n - 1) / n;
 }
+// The most that a sequence of up to n_pages has (a longer one can have fewer).
+inline int most_leaves(int n_pages, int n_kv) { return min(n_pages, LEAVES * most_nodes(n_kv, 296)); }
 
 struct Args {
     const void* q;                                               // [n_tokens, n_heads, d]
@@ -78,8 +78,11 @@ struct Args {
     int nodes;                                                   // places for nodes in a row's records
     int tiles;                                                   // row tiles of a (sequence, key head) that the grid has
     int stages;                                                  // of a warp's ring
+    int whole;                                                   // sequences are not cut: a row tile is one node
     int* status;
 };
+__device__ __forceinline__ int leaf_pages(const Args& a, int n_pages) { return a.whole ? n_pages : leaf_pages(n_pages, a.n_kv); }
+__device__ __forceinline__ int nodes_of(const Args& a, int n_pages) { return a.whole ? 1 : nodes_of(n_pages, a.n_kv); }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -200,7 +203,7 @@ __device__ __forceinline__ void cluster_sync() {
 enum Form { AUTO = 0, PLAIN = 1, RECORDS = 2, CLUSTERS = 3, STAY = 4 };
 struct Plan {
     bool possible;
-    int form, nt, tiles, nodes, stages, kernels;
+    int form, nt, tiles, nodes, stages, whole, kernels;
     int64_t scratch, blocks;
 };
 
@@ -507,13 +510,14 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
     }
     __syncthreads();
     const int n_rows = s.new_tokens * a.group, row0 = tile * 8 * NT;
-    const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + 8 * NT, n_rows) - 1) / a.group;
+    const int last = (min(row0 + 8 * NT, n_rows) - 1) / a.group;
     const int seen = (s.start + last) / kPage + 1;               // pages that any row of the tile sees
+    const int lp = a.whole ? (seen + LEAVES - 1) / LEAVES : leaf_pages(s.pages, a.n_kv);
     const int first_page = node * LEAVES * lp;
     pdl_wait();
     if (row0 >= n_rows || !fits(a, s)) return;                   // (so do all blocks of its cluster)
     if (first_page >= seen) return;                              // (a cluster does not wait for blocks that have left)
-    const int n_nodes = CLUSTERS ? (seen + LEAVES * lp - 1) / (LEAVES * lp) : nodes_of(s.pages, a.n_kv);
+    const int n_nodes = CLUSTERS ? (seen + LEAVES * lp - 1) / (LEAVES * lp) : nodes_of(a, s.pages);
     const int p0 = first_page + warp * lp, count = max(0, min(seen, p0 + lp) - p0);
     uint8_t* ring = ring_all + (size_t)warp * a.stages * TILE;
     int ids = 0;
@@ -687,7 +691,7 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
     }
     for (int b = threadIdx.x; b < a.n_seqs; b += WARPS * 32) {
         const Seq s = sequence(a, b);
-        cum[b + 1] = s.new_tokens > 0 && fits(a, s) ? nodes_of(s.pages, a.n_kv) * ((s.new_tokens * a.group + 8 * NT - 1) / (8 * NT)) * a.n_kv : 0;
+        cum[b + 1] = s.new_tokens > 0 && fits(a, s) ? nodes_of(a, s.pages) * ((s.new_tokens * a.group + 8 * NT - 1) / (8 * NT)) * a.n_kv : 0;
         lens[b] = s.len;
         firsts[b] = s.first;
         if (b == a.n_seqs - 1) firsts[b + 1] = s.first + s.new_tokens;
@@ -741,8 +745,8 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
             }
             n.b = lo;
             const Seq s = place_of(lo);
-            const int local = u - cum[lo], n_rows = s.new_tokens * a.group, tiles = (n_rows + 8 * NT - 1) / (8 * NT), nodes = nodes_of(s.pages, a.n_kv);
-            n.lp = leaf_pages(s.pages, a.n_kv);
+            const int local = u - cum[lo], n_rows = s.new_tokens * a.group, tiles = (n_rows + 8 * NT - 1) / (8 * NT), nodes = nodes_of(a, s.pages);
+            n.lp = leaf_pages(a, s.pages);
             n.place = local % nodes;
             n.row0 = NT == 1 && tiles == 1 ? 0 : local / nodes % tiles * 8 * NT;
             n.kvh = local / (nodes * tiles);
@@ -952,7 +956,7 @@ __global__ void __launch_bounds__(256) plain_kernel(const Args a) {
     const int kvh = (int)(at % (unsigned)a.n_kv), b = (int)(at / (unsigned)a.n_kv);
     const Seq s = sequence(a, b);
     const int n_rows = s.new_tokens * a.group, row0 = tile * PR;
-    const int lp = leaf_pages(s.pages, a.n_kv), last = (min(row0 + PR, n_rows) - 1) / a.group;
+    const int lp = leaf_pages(a, s.pages), last = (min(row0 + PR, n_rows) - 1) / a.group;
     const int seen = (s.start + last) / kPage + 1, first_page = leaf * lp;
     pdl_wait();
     if (row0 >= n_rows || !fits(a, s) || first_page >= seen) return;
@@ -1085,19 +1089,25 @@ __global__ void __launch_bounds__(256) plain_kernel(const Args a) {
 static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int kv_bound, bool f32, int form) {
     Plan p = {};
     const int pages = (kv_bound + kPage - 1) / kPage;
-    const int64_t rows = (int64_t)max_q * (n_heads / n_kv);
-    p.nodes = nodes_of(pages, n_kv);
+    const int64_t rows = (int64_t)max_q * (n_heads / n_kv), sm = sm_count();
     p.form = f32 && form == AUTO ? PLAIN : form;
-    const bool can_stay = n_seqs <= MAX_SEQS;
-    p.possible = p.form >= AUTO && p.form <= STAY && !(f32 && p.form != PLAIN) && !(p.form == STAY && !can_stay) && !(p.form == CLUSTERS && p.nodes > CLUSTER);
     p.nt = p.form == PLAIN || rows <= 8 ? 1 : (rows <= 16 || D > 128 ? 2 : 3);
     p.tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-    const int64_t nodes = (int64_t)n_seqs * n_kv * p.nodes * p.tiles;
+    // Prompts have enough row tiles without cuts, and would need records beyond measure (a row and node: 4 d bytes); two tiles a warp that stays, four blocks an SM.
+    p.whole = rows > 8 && (int64_t)n_seqs * n_kv * p.tiles >= (p.form == PLAIN ? 4 : 2 * LEAVES) * sm;
+    const int leaves = p.whole ? 1 : most_leaves(pages, n_kv);
+    p.nodes = p.form == PLAIN ? leaves : (leaves + LEAVES - 1) / LEAVES;      // (places for records)
+    // Measured at 1 to 64 sequences of up to 300 to 131,000 positions, heads of 64 to 256, one key head of 1 to 16.  Blocks that stay want many nodes: a warp's first
+    // one takes 15 us.  us a block per node / blocks that stay, heads of 128: eight rows 512 nodes of 8 pages 15 / 16, 512 of 4 19 / 26, 768 of 8 21 / 25, 1,024 of 4 to
+    // 8 28 / 20 to 33 / 29, 2,048 of 8 51 / 39; more rows 64 nodes 9 / 17, 768 42 / 33, heads of 64 512 23 / 23.
+    // Clusters want to run all at once: 256 blocks 11.7 in records / 10.8, 512 19.3 / 20.4; heads of 256 (a block an SM) 64 11.7 / 10.8, 128 12.2 / 15.4.
+    const int64_t nodes = (int64_t)n_seqs * n_kv * (p.whole ? 1 : nodes_of(pages, n_kv)) * p.tiles;
+    const bool can_stay = n_seqs <= MAX_SEQS;
     if (p.form == AUTO)
-        p.form = can_stay && nodes >= (p.nt == 1 ? 2 : 1) * (int64_t)LEAVES * sm_count() ? STAY : (p.nodes <= CLUSTER && nodes <= 2 * sm_count() ? CLUSTERS : RECORDS);
-    p.stages = leaf_pages(pages, n_kv) > 1 || p.nt == 3 ? MAX_STAGES : 1;
-    if (p.form == PLAIN) p.nodes = (pages + leaf_pages(pages, n_kv) - 1) / leaf_pages(pages, n_kv);      // (places for records)
-    p.blocks = p.form == STAY ? sm_count() : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
+        p.form = can_stay && nodes >= (p.nt > 1 ? 4 : 6) * sm ? STAY : (p.nodes <= CLUSTER && nodes <= (D <= 128 ? 2 * sm : sm / 2) ? CLUSTERS : RECORDS);
+    p.possible = p.form >= PLAIN && p.form <= STAY && !(f32 && p.form != PLAIN) && !(p.form == STAY && !can_stay) && !(p.form == CLUSTERS && p.nodes > CLUSTER);
+    p.stages = p.whole || leaf_pages(pages, n_kv) > 1 || p.nt == 3 ? MAX_STAGES : 1;
+    p.blocks = p.form == STAY ? sm : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
     const bool records = p.nodes > 1 && p.form != CLUSTERS;
     p.scratch = records ? (int64_t)n_tokens * n_heads * p.nodes * (D + 2) : 0;
     p.kernels = records ? 2 : 1;
@@ -1153,6 +1163,7 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     a.nodes = p.nodes;
     a.tiles = p.tiles;
     a.stages = p.stages;
+    a.whole = p.whole;
     a.status = status;
     const cudaStream_t st = (cudaStream_t)stream;
     const dim3 grid((unsigned)p.blocks);

@@ -160,9 +160,10 @@ def kv4_read(kv: torch.Tensor, head_dim: int, page_table: torch.Tensor, seq_of_t
     return out
 
 
-# Rows (new tokens times query heads of a key head) of a sequence from which on its pages are opened to bfloat16 and the prompt attention
-# runs over them; fewer are computed from the codes.
-OPEN_ROWS = 32
+# Rows (new tokens times query heads of a key head) of a sequence up to which they are computed from the codes; of more its pages are opened to
+# bfloat16 and the prompt attention runs over them.  us from the codes / opened: 32 heads over 8 of 128, 8 sequences behind 6,000, 64 rows 76 / 83, 96
+# rows 87 / 86; 32 behind 2,000, 96 rows 116 / 96; one behind 2,000, 96 rows 14 / 24; 14 over 2 of 64, 32 behind 2,000, 168 rows 30 / 61.
+OPEN_ROWS = {64: 192, 128: 80}
 
 
 # The kernels of attention_kv4 by name (csrc/attn_kv4.cu: Plan); "opened": pages opened to bfloat16, then the prompt attention.
@@ -193,7 +194,7 @@ def _form(dtype: torch.dtype, head_dim: int, rows: int, kind: Optional[str], pla
         return _FORMS[kind]
     if plain or ops.PLAIN_KERNELS:
         return 1
-    return -1 if rows > OPEN_ROWS and dtype is _BF16 and head_dim in (64, 128) else 0
+    return -1 if dtype is _BF16 and rows > OPEN_ROWS.get(head_dim, rows) else 0
 
 
 def _open_words(batch, pages: int, n_kv: int, head_dim: int) -> Tuple[int, int]:
@@ -217,8 +218,8 @@ def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratc
                   plain: bool = False, kind: Optional[str] = None) -> torch.Tensor:
     """Causal attention of the step's new tokens (any number a sequence) over a cache in 4 bits, which already holds their keys and values.
     q: [n, heads, d], bfloat16 or float32.  scratch: float32, at least :func:`attention_kv4_scratch` words (made here if none is given).
-    A sequence's result does not depend on the batch that it is in.  plain: on the CUDA cores, without bulk copies (float32
-    always is); ``kind`` picks a form by hand.  A sequence that does not fit its page table or ``batch.kv_bound``, or names a page
+    While no sequence has more than eight rows (new tokens times query heads of a key head), a sequence's result does not depend on the batch
+    that it is in.  plain: on the CUDA cores, without bulk copies (float32 always is); ``kind`` picks a form by hand.  A sequence that does not fit its page table or ``batch.kv_bound``, or names a page
     outside the cache, is reported (:func:`~wick_b200.ops.check_status`)."""
     shape = q.shape
     if len(shape) != 3:
