@@ -456,18 +456,16 @@ __device__ __forceinline__ void page_step(const uint8_t* tile, const Rows<NT>& w
 struct Nothing {
     __device__ __forceinline__ void operator()() const {}
 };
+// (single: leaves of one page.  Other leaves take their first page as any other, so that the warps of a block run the same code.)
 template <int NT, typename Between = Nothing>
-__device__ __forceinline__ void leaf_page(const Args& a, const uint8_t* tile, const Rows<NT>& w, const Seq& s, int page, bool fresh, Sum<NT>& sum,
+__device__ __forceinline__ void leaf_page(const Args& a, const uint8_t* tile, const Rows<NT>& w, const Seq& s, int page, bool fresh, bool single, Sum<NT>& sum,
                                           Between between = Nothing()) {
     const int first = page * kPage;
-    if (first + kPage - 1 > s.start) {
-        if (fresh) sum.clear();
-        page_step<NT, true, false>(tile, w, a.scale2, first, s.len, s.new_tokens > 1, sum, between);
-    } else if (fresh) {
-        page_step<NT, false, true>(tile, w, a.scale2, first, s.len, false, sum, between);
-    } else {
-        page_step<NT, false, false>(tile, w, a.scale2, first, s.len, false, sum, between);
-    }
+    const bool mask = first + kPage - 1 > s.start;
+    if (fresh && (mask || !single)) sum.clear();
+    if (mask) page_step<NT, true, false>(tile, w, a.scale2, first, s.len, s.new_tokens > 1, sum, between);
+    else if (single) page_step<NT, false, true>(tile, w, a.scale2, first, s.len, false, sum, between);
+    else page_step<NT, false, false>(tile, w, a.scale2, first, s.len, false, sum, between);
 }
 
 // A leaf's sum over its positions: every lane gets its rows'.
@@ -542,7 +540,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
                 }
                 break;
             }
-            leaf_page<NT>(a, ring + (k % a.stages) * TILE, w, s, p0 + k, k == 0, sum);
+            leaf_page<NT>(a, ring + (k % a.stages) * TILE, w, s, p0 + k, k == 0, lp == 1, sum);
             __syncwarp();
             if (k + a.stages < count) issue(k + a.stages);
         }
@@ -807,7 +805,7 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
             for (; page < leaf_end; ++page) {
                 int next_id = -1, next_kvh = cn.kvh;
                 ok = ok && mbar_wait(&full[warp][0], parity, &abort_flag, a.status, 16);
-                leaf_page<NT>(a, tile, w, s, page, fresh, sum, [&]() {
+                leaf_page<NT>(a, tile, w, s, page, fresh, NT == 1 && cn.lp == 1, sum, [&]() {
                     if (page + 1 < cn.end) {
                         if (++held == 32) {
                             held = 0;
