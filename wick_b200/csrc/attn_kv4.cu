@@ -482,6 +482,8 @@ template <int NT> __device__ __forceinline__ void finish_leaf(Sum<NT>& sum) {
 constexpr int leaves_smem(int nt, int stages, bool clusters) { return LEAVES * stages * TILE + (clusters ? nt * 8 * D * 4 : 0); }
 
 // The grid: nodes innermost, then tiles, heads, sequences.  CLUSTERS: a sequence's nodes are a cluster.
+// What bounds it: with few nodes the way of one page through the warp (table, copy, scores, values, fold, join), 7 us with the launch; with many as above.
+// 8 sequences of up to 4,000 positions, 32 heads over 8 of 128: 17 us.
 template <int NT, bool CLUSTERS>
 __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_kernel(const Args a) {
     extern __shared__ __align__(128) uint8_t ring_all[];
@@ -660,14 +662,24 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
 }
 
 // ---- blocks that stay ------------------------------------------------------------------------
-// A block has an equal run of the step's items (a node of a row tile of a key head of a sequence each), and its warps take the next one whenever they are done
-// with one.  A warp's tile is filled again while it is read: the next page's keys as soon as the scores are there, its values when the page is done.
+// A block has a run of the step's items (a node of a row tile of a key head of a sequence each) with an equal part of the pages, or of the items while each has
+// a warp, and its warps take the next one whenever they are done with one.  64 sequences of 6,000 to 12,000 positions, 16 heads of 128, nodes of 8 to 24
+// pages: equal parts of the nodes 605 us, of the pages 382; 16 of 2,000 to 4,000: 38, 51 (some blocks have more nodes than warps).
+// A warp's tile is filled again while it is read: the next page's keys as soon as the scores are there, its values when the page is done.
 // One unit of rows (NT 1): a node's leaves are folded in registers.  More: there is no room for a second accumulator, and a node is one leaf.
+// What bounds it: the instructions that make values of codes (653 of a page's 1,343, half as fast as the others) and the matrix instructions beside them, which
+// add up: a scheduler needs 2,590 clocks a page, with two warps as with three.  64 sequences of 4,000 to 8,191 positions, 32 heads over 8 of 128 (504 MB of
+// pages): 133 us, 58 % of the copy's rate; 8 warps a block 140, 16 (which spill) 149.
 struct Item {
     int b, kvh, row0, place, lp;                                 // place: the node's number in the sequence; none left: b < 0
     int page, end;                                               // of the sequence, as far as the row tile sees
     int alone;                                                   // the sequence has one node
 };
+// An item's pages, about (nodes of a long sequence have more than those of a short one), and one for what goes with it.
+__device__ __forceinline__ int item_work(const Args& a, int n_pages) {
+    const int nodes = max(1, nodes_of(a, n_pages));
+    return (n_pages + nodes - 1) / nodes + 1;
+}
 template <int NT> constexpr int stay_warps() { return NT > 1 || D > 128 ? 8 : (D == 64 ? 16 : 12); }      // (as many as registers allow)
 
 template <int NT>
@@ -676,7 +688,8 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
     extern __shared__ __align__(128) uint8_t ring_all[];
     __shared__ uint64_t full[WARPS][2];                          // keys, values
     __shared__ int cum[MAX_SEQS + 1], lens[MAX_SEQS], firsts[MAX_SEQS + 1];  // items before a sequence; its length (with new tokens) and the first of these
-    __shared__ int abort_flag, taken;
+    __shared__ int64_t work[MAX_SEQS + 1];                       // pages, about, before a sequence
+    __shared__ int abort_flag, taken, end_of_run;
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
     if (threadIdx.x == 0) {
@@ -690,6 +703,7 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
     for (int b = threadIdx.x; b < a.n_seqs; b += WARPS * 32) {
         const Seq s = sequence(a, b);
         cum[b + 1] = s.new_tokens > 0 && fits(a, s) ? nodes_of(a, s.pages) * ((s.new_tokens * a.group + 8 * NT - 1) / (8 * NT)) * a.n_kv : 0;
+        work[b + 1] = (int64_t)cum[b + 1] * item_work(a, s.pages);
         lens[b] = s.len;
         firsts[b] = s.first;
         if (b == a.n_seqs - 1) firsts[b + 1] = s.first + s.new_tokens;
@@ -697,25 +711,52 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
     __syncthreads();
     if (warp == 0) {
         int before = 0;
+        int64_t work_before = 0;
 #pragma unroll 1
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-            const int b = s0 + lane, mine = b < a.n_seqs ? cum[b + 1] : 0;
-            int upto = mine;
+            const int b = s0 + lane;
+            int upto = b < a.n_seqs ? cum[b + 1] : 0;
+            int64_t work_upto = b < a.n_seqs ? work[b + 1] : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int t = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += t;
+                const int64_t u = __shfl_up_sync(0xffffffffu, work_upto, o);
+                if (lane >= o) {
+                    upto += t;
+                    work_upto += u;
+                }
             }
-            if (b < a.n_seqs) cum[b + 1] = before + upto;
+            if (b < a.n_seqs) {
+                cum[b + 1] = before + upto;
+                work[b + 1] = work_before + work_upto;
+            }
             before += __shfl_sync(0xffffffffu, upto, 31);
+            work_before += __shfl_sync(0xffffffffu, work_upto, 31);
         }
         if (lane == 0) {
             cum[0] = 0;
-            taken = (int)((int64_t)blockIdx.x * before / gridDim.x);
+            work[0] = 0;
+        }
+        __syncwarp();
+        if (lane < 2) {                                          // the first item of this block's run, and of the next one's
+            const int64_t block = blockIdx.x + lane;
+            int first = (int)(block * before / gridDim.x);       // (a warp for every item: equal numbers)
+            if (before > WARPS * (int)gridDim.x && block < gridDim.x) {
+                const int64_t at = (int64_t)((double)work_before * block / gridDim.x);
+                int lo = 0, hi = a.n_seqs - 1;                   // the last sequence with work[b] <= at
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (work[mid] <= at) lo = mid;
+                    else hi = mid - 1;
+                }
+                const int one = item_work(a, (lens[lo] + kPage - 1) / kPage);
+                first = cum[lo] + (int)min((at - work[lo] + one - 1) / one, (int64_t)(cum[lo + 1] - cum[lo]));
+            }
+            *(lane == 0 ? &taken : &end_of_run) = first;
         }
     }
     __syncthreads();
-    const int stop = (int)((int64_t)(blockIdx.x + 1) * cum[a.n_seqs] / gridDim.x);
+    const int stop = end_of_run;
     pdl_wait();
     uint8_t* tile = ring_all + (size_t)warp * TILE;
 
@@ -932,8 +973,9 @@ __global__ void __launch_bounds__(128) join_kernel(const Args a, const int* __re
 // ---- CUDA cores --------------------------------------------------------------------------------
 // A block of eight warps per (leaf, tile of eight rows, key head, sequence): page by page the scores (four lanes a position, a quarter of the channels each, the
 // queries in shared memory), the rows' weights (a warp a row), the weighted values (a thread two channels, the positions shared out among D / 2
-// threads' worth of groups).  Everything in 32 bits; a leaf leaves a record.  6 sequences of up to 1,000 positions, 16 heads over 2 of 128: the four warps a
-// node that this took the place of 46 us, now 16.
+// threads' worth of groups).  Everything in 32 bits; a leaf leaves a record.  What bounds it: three barriers a page, and
+// codes that are asked for when they are needed.  6 float32 sequences of up to 1,000 positions, 16 heads over 2 of 128: a block of four warps per
+// node 49 us, this 13.
 constexpr int PR = 8;                                            // rows of a tile
 constexpr int Q_PAD = D / 4 + 4;                                 // a quarter of a query, so that quarters lie in different banks
 constexpr int V_GROUPS = 256 / (D / 2);                          // groups of positions (192: two, and 64 threads without)
