@@ -454,6 +454,43 @@ def test_another_stream_and_replays():
     o.check_status()
 
 
+def test_many_sequences():
+    """More than the blocks that stay have places for."""
+    o = ops()
+    g = torch.Generator().manual_seed(1030)
+    starts = [(7 * i) % 130 for i in range(1030)]
+    pages, b = step(starts, [1] * 1030, g)
+    kv, cache = random_cache(pages, 1, 64, g)
+    q = torch.randn((1030, 4, 64), generator=g).to(BF16).cuda()
+    for kind in (None, "records"):
+        check_attention(q, o.attention_kv4(q, kv.cuda(), b, 0.125, kind=kind), cache, b, 0.125, 64)
+    with pytest.raises(o.KernelError):
+        o.attention_kv4(q, kv.cuda(), b, 0.125, kind="stay")
+    o.check_status()
+
+
+def test_captured_single_tokens_of_many_heads():
+    """96 heads of one key head, captured at short lengths and replayed at longer ones."""
+    o = ops()
+    g = torch.Generator().manual_seed(96)
+    pages, b = step([900, 130], [1, 1], g)
+    kv, cache = random_cache(pages, 1, 128, g)
+    kv, q = kv.cuda(), torch.randn((2, 96, 128), generator=g).to(BF16).cuda()
+    early = types.SimpleNamespace(**{**vars(b), "starts": [3, 0], "start": ints([3, 0])})
+    o.attention_kv4(q, kv, early, 0.1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = o.attention_kv4(q, kv, early, 0.1)
+        early.start.copy_(b.start)
+        graph.replay()
+    torch.cuda.synchronize()
+    check_attention(q, out, cache, b, 0.1, 128)
+    o.check_status()
+
+
 def test_misfits_are_reported():
     """Pages outside the cache, places outside the page table, sequences longer than said: nothing outside the arrays is touched."""
     o = ops()
@@ -540,6 +577,9 @@ def test_refusals():
         broken = types.SimpleNamespace(**{**vars(b), name: bad})
         with pytest.raises(o.KernelError):
             o.attention_kv4(q, kv, broken, 0.1)
+    for name in ("kv_bound", "max_q_len"):
+        with pytest.raises(o.KernelError):
+            o.attention_kv4(q, kv, types.SimpleNamespace(**{**vars(b), name: 0}), 0.1)
     with pytest.raises(o.KernelError):
         o.attention_kv4(q, kv, b, 0.1, out=q.float())
     for bad in (q, q.float()):

@@ -1175,7 +1175,8 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     WICK_REQUIRE(n_tokens >= 0 && n_seqs > 0 && n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && table_width > 0 && max_q >= 0 && kv_bound >= 0,
                  "attention_kv4: bad sizes");
     WICK_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "attention_kv4: arrays must begin on multiples of 16 bytes");
-    if (n_tokens == 0 || max_q == 0 || kv_bound == 0) return 0;
+    if (n_tokens == 0) return 0;
+    WICK_REQUIRE(max_q > 0 && kv_bound > 0, "attention_kv4: %d tokens, but up to %d a sequence and %d positions", n_tokens, max_q, kv_bound);
     const Plan p = plan(n_tokens, n_seqs, n_heads, n_kv, max_q, kv_bound, sizeof(T) == 4, form);
     WICK_REQUIRE(p.possible, "attention_kv4: the kernel asked for (%d) does not take these sizes", form);
     WICK_REQUIRE(scratch_size >= p.scratch, "attention_kv4: scratch of %lld floats, %lld needed", (long long)scratch_size, (long long)p.scratch);

@@ -91,8 +91,8 @@ def qk_norm_rope_append_kv4(qkv: torch.Tensor, n_heads: int, n_kv: int, head_dim
 
     qkv: [n, (n_heads + 2 n_kv) head_dim] in the activation dtype, or float32 partial sums [splits, n, ...] (then ``dtype`` names
     the activation dtype).  Keys and values are summed, normed, rotated and assigned their codes in 64 bits: a code is that of
-    the exact number, whatever the batch and the number of partial sums.  A place outside the page table or the cache is left
-    out and reported (:func:`~wick_b200.ops.check_status`)."""
+    the exact number, whatever the batch and the number of partial sums.  Two tokens of a step have different places.  A place outside
+    the page table or the cache is left out and reported (:func:`~wick_b200.ops.check_status`)."""
     lib = _kv4(head_dim)
     device = _here("qkv", qkv)
     shape = qkv.shape
@@ -187,14 +187,15 @@ def _bounds(batch) -> Tuple[int, int, int]:
     return batch.max_q_len, batch.kv_bound, -1
 
 
-def _form(dtype: torch.dtype, head_dim: int, rows: int, kind: Optional[str], plain: bool) -> int:
+def _form(dtype: torch.dtype, head_dim: int, max_q: int, group: int, kind: Optional[str], plain: bool) -> int:
     if kind is not None:
         if kind not in _FORMS or (kind == "opened" and (dtype is not _BF16 or head_dim not in (64, 128))):
             raise KernelError(f"no kernel {kind!r} for {dtype}, head size {head_dim} (known: {', '.join(k for k in _FORMS if k)})")
         return _FORMS[kind]
     if plain or ops.PLAIN_KERNELS:
         return 1
-    return -1 if dtype is _BF16 and rows > OPEN_ROWS.get(head_dim, rows) else 0
+    # (single tokens are never opened: a captured step of them is replayed at lengths that the host's copies do not tell)
+    return -1 if dtype is _BF16 and max_q > 1 and head_dim in OPEN_ROWS and max_q * group > OPEN_ROWS[head_dim] else 0
 
 
 def _open_words(batch, pages: int, n_kv: int, head_dim: int) -> Tuple[int, int]:
@@ -208,7 +209,7 @@ def attention_kv4_scratch(batch, n_heads: int, n_kv: int, head_dim: int, dtype: 
     """float32 words of scratch that :func:`attention_kv4` needs for this step."""
     _need(n_heads > 0 and n_kv > 0 and n_heads % n_kv == 0, f"{n_heads} heads over {n_kv} key heads")
     max_q, kv_bound, pages = _bounds(batch)
-    form = _form(dtype, head_dim, max_q * (n_heads // n_kv), kind, plain)
+    form = _form(dtype, head_dim, max_q, n_heads // n_kv, kind, plain)
     if form < 0:
         return _open_words(batch, pages, n_kv, head_dim)[1]
     return _plan(head_dim, batch.n_tokens, batch.n_seqs, n_heads, n_kv, max_q, kv_bound, dtype is _F32, form)[0]
@@ -250,7 +251,7 @@ def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratc
     max_q, kv_bound, pages = _bounds(batch)
     if kv_bound > width * PAGE:
         raise KernelError(f"{kv_bound} positions in page tables of {width} pages")
-    form = _form(dtype, hd, max_q * (n_heads // n_kv), kind, plain)
+    form = _form(dtype, hd, max_q, n_heads // n_kv, kind, plain)
     if form < 0:
         pages, words = _open_words(batch, pages, n_kv, hd)
         kernels = 1
