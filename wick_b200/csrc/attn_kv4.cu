@@ -1137,9 +1137,10 @@ static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int
     p.whole = rows > 8 && (int64_t)n_seqs * n_kv * p.tiles >= (p.form == PLAIN ? 4 : 2 * LEAVES) * sm;
     const int leaves = p.whole ? 1 : most_leaves(pages, n_kv);
     p.nodes = p.form == PLAIN ? leaves : (leaves + LEAVES - 1) / LEAVES;      // (places for records)
-    // Measured at 1 to 64 sequences of up to 300 to 131,000 positions, heads of 64 to 256, one key head of 1 to 16.  Blocks that stay want many nodes: a warp's first
-    // one takes 15 us.  us a block per node / blocks that stay, heads of 128: eight rows 512 nodes of 8 pages 15 / 16, 512 of 4 19 / 26, 768 of 8 21 / 25, 1,024 of 4 to
-    // 8 28 / 20 to 33 / 29, 2,048 of 8 51 / 39; more rows 64 nodes 9 / 17, 768 42 / 33, heads of 64 512 23 / 23.
+    // Measured at 1 to 64 sequences of up to 300 to 131,000 positions, heads of 64 to 256, 2 to 16 key heads.  Blocks that stay want many nodes: a warp's first
+    // one takes 15 us.  us a block per node / blocks that stay, heads of 128, up to eight rows: 512 nodes (one a sequence, 300 positions) 15 / 16, 512 (two a sequence,
+    // 1,000) 20 / 24, 576 (18, 9,000) 21 / 25, 1,024 (one) 29 / 21, (two) 34 / 30, (eight) 30 / 30, 2,048 (eight) 53 / 39; 16 rows: 64 nodes 9 / 17, 768 43 / 33;
+    // heads of 64, 42 rows: 512 24 / 23.
     // Clusters want to run all at once: 256 blocks 11.7 in records / 10.8, 512 19.3 / 20.4; heads of 256 (a block an SM) 64 11.7 / 10.8, 128 12.2 / 15.4.
     const int64_t nodes = (int64_t)n_seqs * n_kv * (p.whole ? 1 : nodes_of(pages, n_kv)) * p.tiles;
     const bool can_stay = n_seqs <= MAX_SEQS;
