@@ -469,6 +469,28 @@ def test_many_sequences():
     o.check_status()
 
 
+@pytest.mark.parametrize("H,KV,d,starts,new", [
+    (32, 32, 64, [100 * (i + 4) for i in range(20)] + [5000, 0, 4607, 4608, 63, 2500, 6001], [1] * 27),      # up to nine nodes of a page a leaf, and four of several
+    (16, 8, 128, [61 * (i + 20) for i in range(60)], [1 + i % 4 for i in range(60)]),
+    (32, 8, 128, [61 * (i + 20) for i in range(45)] + [0], [1 + i % 5 for i in range(45)] + [0]),            # tiles of 24 rows
+])
+def test_more_nodes_than_warps(H, KV, d, starts, new):
+    """Blocks that stay, several rounds of nodes of unequal sequences; 50 pages, which all of them share."""
+    o = ops()
+    g = torch.Generator().manual_seed(H + KV)
+    _, b = step(starts, new, g)
+    b.table = [[p % 50 for p in row] for row in b.table]
+    b.page_table = ints(b.table)
+    kv, cache = random_cache(50, KV, d, g)
+    q = torch.randn((b.n_tokens, H, d), generator=g).to(BF16).cuda()
+    scale = 1.0 / math.sqrt(d)
+    got = o.attention_kv4(q, kv.cuda(), b, scale, kind="stay")
+    check_attention(q, got, cache, b, scale, d)
+    if max(new) * H // KV <= 8:
+        assert torch.equal(o.attention_kv4(q, kv.cuda(), b, scale, kind="records"), got)
+    o.check_status()
+
+
 def test_captured_single_tokens_of_many_heads():
     """96 heads of one key head, captured at short lengths and replayed at longer ones."""
     o = ops()
