@@ -1,0 +1,58 @@
+"""The cache in 4 bits on the device: descriptions that do not fit, numbers at the ends of their ranges, steps of many tokens."""
+import types
+
+import pytest
+import torch
+
+from test_gpu_kv4 import BF16, F32, ints, ops, random_cache, step
+
+pytestmark = pytest.mark.gpu
+
+
+def said():
+    with pytest.raises(ops().KernelError, match="4-bit cache"):
+        ops().check_status()
+    ops().check_status()
+
+
+@pytest.mark.parametrize("kind", ["plain", "records", "clusters", "stay"])
+@pytest.mark.parametrize("start", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 64, 2 ** 31 - 200, 2 ** 30])
+def test_a_start_near_the_end_of_32_bits(start, kind):
+    """The sequence's length is beyond 32 bits: it is left out and reported, the others are what they were."""
+    o = ops()
+    g = torch.Generator().manual_seed(11)
+    pages, b = step([100, 70, 400, 3], [2, 1, 2, 2], g)
+    kv = random_cache(pages, 2, 64, g)[0].cuda()
+    q = torch.randn((7, 4, 64), generator=g).to(BF16).cuda()
+    good = o.attention_kv4(q, kv, b, 0.1, kind=kind)
+    o.check_status()
+    for i in (0, 2, 3):
+        broken = types.SimpleNamespace(**vars(b))
+        broken.start = b.start.clone()
+        broken.start[i] = start
+        out = torch.full_like(q, 7.0)
+        o.attention_kv4(q, kv, broken, 0.1, out=out, kind=kind)
+        said()
+        mine = torch.tensor([x == i for x in b.seq_of_token.tolist()], device="cuda")
+        assert (out[mine] == 7.0).all() and torch.equal(out[~mine], good[~mine])
+
+
+@pytest.mark.parametrize("kind", ["plain", "records", "stay"])
+def test_tokens_beyond_the_step(kind):
+    """A sequence whose tokens lie outside the step's is left out and reported."""
+    o = ops()
+    g = torch.Generator().manual_seed(12)
+    pages, b = step([100, 70], [2, 1], g)
+    kv = random_cache(pages, 2, 64, g)[0].cuda()
+    q = torch.randn((3, 4, 64), generator=g).to(BF16).cuda()
+    good = o.attention_kv4(q, kv, b, 0.1, kind=kind)
+    for cu in ([0, 2, 4], [-1, 0, 1], [2 ** 31 - 2, 2 ** 31 - 1, 3], [0, 2 ** 31 - 1, -2 ** 31]):
+        broken = types.SimpleNamespace(**vars(b))
+        broken.cu_seqlens = ints(cu)
+        out = torch.full_like(q, 7.0)
+        o.attention_kv4(q, kv, broken, 0.1, out=out, kind=kind)
+        said()
+        if cu[:2] == [0, 2]:
+            assert torch.equal(out[:2], good[:2]) and (out[2] == 7.0).all()
+        elif cu[0] != -1:
+            assert (out == 7.0).all()

@@ -129,9 +129,11 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
     s.pages = (s.len + kPage - 1) / kPage;
     return s;
 }
-// Whether a sequence fits the step, its page table and the records' places (else it is left out, and said).
+// Whether a sequence fits the step, its page table and the records' places (else it is left out, and said).  (Sums of two numbers that may be anything
+// are 64 bits wide: a start near 2^31 would else make a length below 0, which passes every bound.)
 __device__ __forceinline__ bool fits(const Args& a, const Seq& s) {
-    const bool ok = s.start >= 0 && s.first >= 0 && s.first + s.new_tokens <= a.n_tokens && s.new_tokens <= a.max_q && s.pages <= a.table_width && s.pages <= a.pages;
+    const bool ok = s.start >= 0 && s.first >= 0 && s.new_tokens >= 0 && (int64_t)s.first + s.new_tokens <= a.n_tokens && s.new_tokens <= a.max_q &&
+                    (int64_t)s.start + s.new_tokens <= (int64_t)min(a.table_width, a.pages) * kPage;
     if (!ok) atomicCAS(a.status, 0, 15);
     return ok;
 }
