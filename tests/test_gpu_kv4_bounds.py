@@ -4,7 +4,7 @@ import types
 import pytest
 import torch
 
-from test_gpu_kv4 import BF16, F32, ints, ops, random_cache, step
+from test_gpu_kv4 import BF16, F32, PAGE, check_attention, ints, ops, random_cache, step
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,32 @@ def test_tokens_beyond_the_step(kind):
             assert torch.equal(out[:2], good[:2]) and (out[2] == 7.0).all()
         elif cu[0] != -1:
             assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("width", [None, 9])
+def test_opened_pages_have_a_name_in_every_place(width):
+    """Whatever the scratch held: behind a sequence's last page, for sequences without a page, and with more room than pages."""
+    from wick_b200.layout import pages_for
+    o = ops()
+    g = torch.Generator().manual_seed(13)
+    for starts, new in (([0, 100, 300], [65, 64, 5]), ([64], [129]), ([0, 0, 7], [70, 0, 3])):
+        pages, b = step(starts, new, g, width=width)
+        kv, cache = random_cache(pages, 2, 64, g)
+        q = torch.randn((b.n_tokens, 4, 64), generator=g).to(BF16).cuda()
+        words = o.attention_kv4_scratch(b, 4, 2, 64, BF16, kind="opened")
+        want = None
+        for junk in (0, -1, 0x7FFFFFFF, 123456789):
+            scratch = torch.full((words + 3,), junk, dtype=torch.int32, device="cuda").view(F32)
+            out = o.attention_kv4(q, kv.cuda(), b, 0.1, scratch, kind="opened")
+            used = [pages_for(s + n) for s, n in zip(starts, new)]
+            at = sum(used) * 2 * PAGE * 64
+            names = scratch.view(torch.int32)[at:at + b.n_seqs * b.table_width].view(b.n_seqs, -1).tolist()
+            first = 0
+            for row, n in zip(names, used):
+                assert row == [first + i for i in range(n)] + [0] * (b.table_width - n)
+                first += n
+            assert (scratch.view(torch.int32)[words:] == junk).all()
+            want = out if want is None else want
+            assert torch.equal(out, want)
+        check_attention(q, want, cache, b, 0.1, 64)
+    o.check_status()

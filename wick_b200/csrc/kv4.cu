@@ -505,14 +505,17 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
     int64_t page = page_of(page_table, table_width, kv_pages, b, j * kPage, status);
     if (page < 0) page = 0;
     if (h == 0 && threadIdx.x == 0 && j < table_width) out_table[(int64_t)b * table_width + j] = p;
+    // The places behind a sequence's last page name page 0: the prompt attention copies pages in pairs, the second of an odd number's last pair with them.
+    if (h == 0 && (j + 1) * kPage >= len)
+        for (int i = j + 1 + threadIdx.x; i < table_width; i += 256) out_table[(int64_t)b * table_width + i] = 0;
     if (p == (int)gridDim.x - 1 && h == 0 && threadIdx.x == 0) {
         // Pages that there is no room for (the caller counted fewer): said, and named by a page that is there.
         int before = 0;
         for (int s = 0; s < n_seqs; ++s) {
-            const int n = (start[s] + cu_seqlens[s + 1] - cu_seqlens[s] + kPage - 1) / kPage;
-            for (int i = max(0, p + 1 - before); i < n; ++i) {
-                if (i < table_width) out_table[(int64_t)s * table_width + i] = 0;
-                atomicCAS(status, 0, 15);
+            const int n = (start[s] + cu_seqlens[s + 1] - cu_seqlens[s] + kPage - 1) / kPage, room = max(0, p + 1 - before);
+            if (room < n || n == 0) {
+                if (n > 0) atomicCAS(status, 0, 15);
+                for (int i = min(room, n); i < table_width; ++i) out_table[(int64_t)s * table_width + i] = 0;
             }
             before += n;
         }
