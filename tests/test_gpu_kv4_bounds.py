@@ -85,3 +85,57 @@ def test_opened_pages_have_a_name_in_every_place(width):
             assert torch.equal(out, want)
         check_attention(q, want, cache, b, 0.1, 64)
     o.check_status()
+
+
+@pytest.mark.parametrize("start", [-5, -2 ** 31, 5 * PAGE - 64, 64 * PAGE, 2 ** 30, 2 ** 31 - 1, 2 ** 31 - 65, 2 ** 31 - 130])
+def test_opened_pages_of_a_sequence_that_does_not_fit(start):
+    """It is reported, the others are what they were."""
+    o = ops()
+    g = torch.Generator().manual_seed(14)
+    pages, b = step([100, 0, 64], [65, 129, 70], g, width=5)
+    kv = random_cache(pages, 2, 64, g)[0].cuda()
+    q = torch.randn((b.n_tokens, 4, 64), generator=g).to(BF16).cuda()
+    good = o.attention_kv4(q, kv, b, 0.1, kind="opened")
+    o.check_status()
+    for i in range(3):
+        broken = types.SimpleNamespace(**vars(b))
+        broken.start = b.start.clone()
+        broken.start[i] = start
+        out = o.attention_kv4(q, kv, broken, 0.1, kind="opened")
+        said()
+        others = torch.tensor([x != i for x in b.seq_of_token.tolist()], device="cuda")
+        assert torch.equal(out[others], good[others]), i
+
+
+def test_opened_pages_of_tokens_in_no_order():
+    """Tokens outside the step, or sequences whose tokens go backwards: reported, and nothing outside the arrays is written."""
+    o = ops()
+    g = torch.Generator().manual_seed(15)
+    pages, b = step([100, 0, 64], [65, 129, 70], g)
+    kv = random_cache(pages, 2, 64, g)[0].cuda()
+    q = torch.randn((b.n_tokens, 4, 64), generator=g).to(BF16).cuda()
+    good = o.attention_kv4(q, kv, b, 0.1, kind="opened")
+    n = b.n_tokens
+    for cu in ([0, 65, 194, n + 1], [0, 65, 194, 2 ** 31 - 1], [0, 65, 194, -2 ** 31], [-1, 65, 194, n], [2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 3], [0, 200, 100, n]):
+        broken = types.SimpleNamespace(**vars(b))
+        broken.cu_seqlens = ints(cu)
+        around = torch.full((n + 200, 4, 64), 7.0, dtype=BF16, device="cuda")
+        o.attention_kv4(q, kv, broken, 0.1, out=around[100:100 + n], kind="opened")
+        said()
+        assert (around[:100] == 7.0).all() and (around[100 + n:] == 7.0).all()
+        if cu[:3] == [0, 65, 194]:
+            assert torch.equal(around[100:294], good[:194])
+
+
+def test_opened_rows_behind_the_last_sequence_stay():
+    o = ops()
+    g = torch.Generator().manual_seed(16)
+    pages, b = step([100, 7], [65, 100], g)
+    kv = random_cache(pages, 2, 64, g)[0].cuda()
+    q = torch.randn((170, 4, 64), generator=g).to(BF16).cuda()
+    want = o.attention_kv4(q[:165].clone(), kv, b, 0.1, kind="opened")
+    b.n_tokens, b.seq_of_token = 170, ints(b.seq_of_token.tolist() + [1] * 5)
+    out = torch.full_like(q, 7.0)
+    o.attention_kv4(q, kv, b, 0.1, out=out, kind="opened")
+    assert (out[165:] == 7.0).all() and torch.equal(out[:165], want)
+    o.check_status()

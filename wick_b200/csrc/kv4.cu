@@ -458,23 +458,36 @@ read_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
 }
 
 // ---- opening pages ----------------------------------------------------------------
-// The pages of all sequences of a step, in order, as bfloat16 pages [2, n_kv, 64, d] one behind the other, and the table that names them there.  Rows
-// behind a sequence's end are zeros.  A block per page and key head.
+// The pages of all sequences of a step, in order, as bfloat16 pages [2, n_kv, 64, d] one behind the other, and a description of the step over them for the
+// attention: the table that names them (every place of it), and the sequences' tokens and starts.  A sequence that does not fit the step or its page table is
+// reported and has no pages; its start there is 0 (its results are nothing, and the attention reads within the arrays for it).  Rows behind a sequence's end are
+// zeros.  A block per page and key head.
+struct OpenSeq {
+    int len, pages;                                              // pages: -1 if it does not fit
+};
+__device__ __forceinline__ OpenSeq open_seq(const int* cu_seqlens, const int* start, int s, int n_tokens, int table_width) {
+    const int first = cu_seqlens[s], end = cu_seqlens[s + 1], from = start[s];
+    const int64_t len = (int64_t)from + end - first;
+    const bool ok = first >= 0 && end >= first && end <= n_tokens && from >= 0 && len <= (int64_t)table_width * kPage;
+    return {ok ? (int)len : 0, ok ? ((int)len + kPage - 1) / kPage : -1};
+}
+
 __global__ void __launch_bounds__(256)
 open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const int* __restrict__ page_table, int table_width,
-            const int* __restrict__ cu_seqlens, const int* __restrict__ start, int n_seqs, bf16* __restrict__ out,
-            int* __restrict__ out_table, int* status) {
+            const int* __restrict__ cu_seqlens, const int* __restrict__ start, int n_seqs, int n_tokens, bf16* __restrict__ out,
+            int* __restrict__ out_table, int* __restrict__ out_cu, int* __restrict__ out_start, int* status) {
     // (No pdl_trigger: the kernel behind this one may read the page table before it waits, and this one writes it.)
-    __shared__ int found[3];
+    __shared__ int found[4];
     const int p = blockIdx.x, h = blockIdx.y;
+    const bool describes = p == 0 && h == 0;                     // (the block that writes what is not a page's)
     if (threadIdx.x < 32) {
         // the sequence of page p of the step, and its first page's number: a scan over the sequences' pages
         const int lane = threadIdx.x;
         int before = 0, b = -1, j = 0, len = 0;
         for (int s0 = 0; s0 < n_seqs; s0 += 32) {
             const int s = s0 + lane;
-            const int mine_len = s < n_seqs ? start[s] + cu_seqlens[s + 1] - cu_seqlens[s] : 0;
-            const int mine = (mine_len + kPage - 1) / kPage;
+            const OpenSeq it = s < n_seqs ? open_seq(cu_seqlens, start, s, n_tokens, table_width) : OpenSeq{0, 0};
+            const int mine = max(it.pages, 0);
             int upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -482,12 +495,12 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
                 if (lane >= o) upto += v;
             }
             const int total = __shfl_sync(0xffffffffu, upto, 31);
-            if (p < before + total) {
+            if (b < 0 && p < before + total) {
                 const int l = __ffs(__ballot_sync(0xffffffffu, p - before < upto)) - 1;
                 b = s0 + l;
                 j = p - before - __shfl_sync(0xffffffffu, upto - mine, l);
-                len = __shfl_sync(0xffffffffu, mine_len, l);
-                break;
+                len = __shfl_sync(0xffffffffu, it.len, l);
+                if (!describes) break;
             }
             before += total;
         }
@@ -495,41 +508,61 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
             found[0] = b;
             found[1] = j;
             found[2] = len;
+            found[3] = before;                                   // (where it describes the step: all pages)
         }
     }
     __syncthreads();
     const int b = found[0], j = found[1], len = found[2];
     pdl_wait();
-    if (b < 0) return;
-    kv = fresh(kv);
-    int64_t page = page_of(page_table, table_width, kv_pages, b, j * kPage, status);
-    if (page < 0) page = 0;
-    if (h == 0 && threadIdx.x == 0 && j < table_width) out_table[(int64_t)b * table_width + j] = p;
-    // The places behind a sequence's last page name page 0: the prompt attention copies pages in pairs, the second of an odd number's last pair with them.
-    if (h == 0 && (j + 1) * kPage >= len)
-        for (int i = j + 1 + threadIdx.x; i < table_width; i += 256) out_table[(int64_t)b * table_width + i] = 0;
-    if (p == (int)gridDim.x - 1 && h == 0 && threadIdx.x == 0) {
-        // Pages that there is no room for (the caller counted fewer): said, and named by a page that is there.
-        int before = 0;
-        for (int s = 0; s < n_seqs; ++s) {
-            const int n = (start[s] + cu_seqlens[s + 1] - cu_seqlens[s] + kPage - 1) / kPage, room = max(0, p + 1 - before);
-            if (room < n || n == 0) {
-                if (n > 0) atomicCAS(status, 0, 15);
-                for (int i = min(room, n); i < table_width; ++i) out_table[(int64_t)s * table_width + i] = 0;
-            }
-            before += n;
-        }
-    }
-    const uint8_t* head = kv + (page * n_kv + h) * head_bytes(D);
-    const int rows = min(kPage, len - j * kPage);
     // All codes of a page are asked for before the first are used (a loop that used them one by one: 42 us for 562 pages of 8 heads of 128, now 30).
     constexpr int STEPS = 2 * kPage * (D / 8) / 256;
     Eight e[STEPS];
+    if (b >= 0) {
+        kv = fresh(kv);
+        int64_t page = page_of(page_table, table_width, kv_pages, b, j * kPage, status);
+        if (page < 0) page = 0;
+        const uint8_t* head = kv + (page * n_kv + h) * head_bytes(D);
 #pragma unroll
-    for (int u = 0; u < STEPS; ++u) {
-        const int i = u * 256 + threadIdx.x;
-        e[u] = load_eight(head, i / (D / 8) % kPage, i % (D / 8), u >= STEPS / 2);
+        for (int u = 0; u < STEPS; ++u) {
+            const int i = u * 256 + threadIdx.x;
+            e[u] = load_eight(head, i / (D / 8) % kPage, i % (D / 8), u >= STEPS / 2);
+        }
+        if (h == 0 && threadIdx.x == 0) out_table[(int64_t)b * table_width + j] = p;
+        // The places behind a sequence's last page name page 0: the prompt attention copies pages in pairs, the second of an odd number's last pair with them.
+        if (h == 0 && (j + 1) * kPage >= len)
+            for (int i = j + 1 + threadIdx.x; i < table_width; i += 256) out_table[(int64_t)b * table_width + i] = 0;
     }
+    if (describes) {                                             // (while the codes are on their way)
+        bool misfit = false;
+        for (int s = threadIdx.x; s < n_seqs; s += 256) {
+            const int n = open_seq(cu_seqlens, start, s, n_tokens, table_width).pages;
+            misfit |= n < 0;
+            out_start[s] = n < 0 ? 0 : start[s];
+            out_cu[s] = cu_seqlens[s];
+            if (s == n_seqs - 1) out_cu[s + 1] = cu_seqlens[s + 1];
+            if (n <= 0)
+                for (int i = 0; i < table_width; ++i) out_table[(int64_t)s * table_width + i] = 0;
+        }
+        misfit = __syncthreads_or(misfit);
+        if (threadIdx.x == 0 && misfit) {
+            // (the tokens in order and within the step)
+            atomicCAS(status, 0, 15);
+            for (int s = 0, upto = 0; s <= n_seqs; ++s) out_cu[s] = upto = max(upto, min(cu_seqlens[s], n_tokens));
+        }
+        if (threadIdx.x == 0 && found[3] > (int)gridDim.x) {
+            // Pages that there is no room for (the caller counted fewer): said, and named by a page that is there.
+            atomicCAS(status, 0, 15);
+            int before = 0;
+            for (int s = 0; s < n_seqs; ++s) {
+                const int n = max(0, open_seq(cu_seqlens, start, s, n_tokens, table_width).pages), room = max(0, (int)gridDim.x - before);
+                if (room < n)
+                    for (int i = room; i < table_width; ++i) out_table[(int64_t)s * table_width + i] = 0;
+                before += n;
+            }
+        }
+    }
+    if (b < 0) return;
+    const int rows = min(kPage, len - j * kPage);
 #pragma unroll
     for (int u = 0; u < STEPS; ++u) {
         const bool is_v = u >= STEPS / 2;
@@ -589,14 +622,14 @@ WICK_API int wick_kv4_read(const void* kv, int64_t kv_pages, int n_kv, const int
 }
 WICK_PACKED(wick_kv4_read)
 
-// out: bfloat16 [out_pages, 2, n_kv, 64, d]; out_table: int32 [n_seqs, table_width].
+// out: bfloat16 [out_pages, 2, n_kv, 64, d]; out_table: int32 [n_seqs, table_width]; out_cu: int32 [n_seqs + 1]; out_start: int32 [n_seqs].
 WICK_API int wick_kv4_open(const void* kv, int64_t kv_pages, int n_kv, const int* page_table, int table_width, const int* cu_seqlens, const int* start,
-                           int n_seqs, void* out, int out_pages, int* out_table, int* status, void* stream) {
-    WICK_REQUIRE(n_kv > 0 && n_kv <= 65535 && table_width > 0 && n_seqs > 0 && out_pages >= 0, "kv4_open: bad sizes");
+                           int n_seqs, int n_tokens, void* out, int out_pages, int* out_table, int* out_cu, int* out_start, int* status, void* stream) {
+    WICK_REQUIRE(n_kv > 0 && n_kv <= 65535 && table_width > 0 && table_width <= INT32_MAX / kPage && n_seqs > 0 && n_tokens >= 0 && out_pages > 0,
+                 "kv4_open: bad sizes");
     WICK_REQUIRE((((uintptr_t)kv | (uintptr_t)out) & 15) == 0, "kv4_open: arrays must begin on multiples of 16 bytes");
-    if (out_pages == 0) return 0;
     WICK_CUDA(launch(kv4::open_kernel, dim3(out_pages, n_kv), dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)kv, kv_pages, n_kv, page_table,
-                     table_width, cu_seqlens, start, n_seqs, (bf16*)out, out_table, status));
+                     table_width, cu_seqlens, start, n_seqs, n_tokens, (bf16*)out, out_table, out_cu, out_start, status));
     return check_launch("kv4_open");
 }
 WICK_PACKED(wick_kv4_open)

@@ -199,10 +199,10 @@ def _form(dtype: torch.dtype, head_dim: int, max_q: int, group: int, kind: Optio
 
 
 def _open_words(batch, pages: int, n_kv: int, head_dim: int) -> Tuple[int, int]:
-    """Opened pages, and the words that they and their tables take."""
+    """Opened pages, and the words that they and the step's description over them (names of pages, cu_seqlens, starts) take."""
     if pages < 0:
         pages = sum(pages_for(s + q) for s, q in zip(batch.starts, batch.q_lens))
-    return pages, pages * n_kv * PAGE * head_dim + batch.n_seqs * batch.table_width
+    return pages, pages * n_kv * PAGE * head_dim + batch.n_seqs * (batch.table_width + 2) + 1
 
 
 def attention_kv4_scratch(batch, n_heads: int, n_kv: int, head_dim: int, dtype: torch.dtype, plain: bool = False, kind: Optional[str] = None) -> int:
@@ -273,9 +273,11 @@ def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratc
                         kv_bound, scale, scratch.data_ptr() if words else 0, words, form, status, _stream(), kernels=kernels)
         return out
     at = pages * n_kv * PAGE * hd
-    opened, names = scratch.view(-1)[:at].view(_BF16).view(pages, 2, n_kv, PAGE, hd), scratch.view(-1)[at:words].view(torch.int32).view(n_seqs, width)
-    lib.call_packed("wick_kv4_open", "plipippipippp", kv.data_ptr(), kv_pages, n_kv, table.data_ptr(), width, cu.data_ptr(), start.data_ptr(), n_seqs,
-                    opened.data_ptr(), pages, names.data_ptr(), status, _stream())
-    return attention_prompt(q, opened, types.SimpleNamespace(
-        n_tokens=n, q_tiles=getattr(batch, "q_tiles", None), q_lens=batch.q_lens, cu_seqlens=cu, n_seqs=n_seqs, start=start, page_table=names,
-        table_width=width), scale, out=out)
+    base, names = scratch.data_ptr(), at + n_seqs * width
+    lib.call_packed("wick_kv4_open", "plipippiipippppp", kv.data_ptr(), kv_pages, n_kv, table.data_ptr(), width, cu.data_ptr(), start.data_ptr(), n_seqs, n,
+                    base, pages, base + 4 * at, base + 4 * names, base + 4 * (names + n_seqs + 1), status, _stream())
+    flat = scratch.view(-1)                                          # (views while the kernel runs)
+    table, cu, start = flat[at:words].view(torch.int32).split([n_seqs * width, n_seqs + 1, n_seqs])
+    return attention_prompt(q, flat[:at].view(_BF16).view(pages, 2, n_kv, PAGE, hd), types.SimpleNamespace(
+        n_tokens=n, q_tiles=getattr(batch, "q_tiles", None), q_lens=batch.q_lens, cu_seqlens=cu, n_seqs=n_seqs, start=start,
+        page_table=table.view(n_seqs, width), table_width=width), scale, out=out)
