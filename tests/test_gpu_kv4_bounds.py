@@ -1,4 +1,5 @@
 """The cache in 4 bits on the device: descriptions that do not fit, numbers at the ends of their ranges, steps of many tokens."""
+import math
 import types
 
 import pytest
@@ -138,4 +139,24 @@ def test_opened_rows_behind_the_last_sequence_stay():
     out = torch.full_like(q, 7.0)
     o.attention_kv4(q, kv, b, 0.1, out=out, kind="opened")
     assert (out[165:] == 7.0).all() and torch.equal(out[:165], want)
+    o.check_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale", [-0.07, -0.4, 0.0, -0.0, 1e-60, -1e-60])
+def test_opened_pages_and_scales(scale, d):
+    """A negative scale turns the order of the scores around, one of 0 (as a float32, too) weighs all alike; the form that the rule takes, and by hand."""
+    o = ops()
+    g = torch.Generator().manual_seed(17)
+    pages, b = step([0, 100, 70], [150, 33, 1], g)
+    kv, cache = random_cache(pages, 2, d, g)
+    q = torch.randn((b.n_tokens, 4, d), generator=g).to(BF16).cuda()
+    for kind in ("opened", None):
+        check_attention(q, o.attention_kv4(q, kv.cuda(), b, scale, kind=kind), cache, b, scale, d)
+    # a key that is no number shows in the rows that see it, with any scale
+    scales = kv[:, :, 64 * d:].view(pages, 2, 2, PAGE, d // 32, 4)
+    scales[b.table[1][132 // PAGE], 1, 0, 132 % PAGE, 0] = torch.tensor([0.0, math.nan], dtype=BF16).view(torch.uint8)
+    want = torch.zeros(q.shape, dtype=torch.bool, device="cuda")
+    want[182, 2:] = True
+    assert torch.equal(o.attention_kv4(q, kv.cuda(), b, scale, kind="opened").isnan(), want)
     o.check_status()

@@ -461,7 +461,7 @@ read_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
 // The pages of all sequences of a step, in order, as bfloat16 pages [2, n_kv, 64, d] one behind the other, and a description of the step over them for the
 // attention: the table that names them (every place of it), and the sequences' tokens and starts.  A sequence that does not fit the step or its page table is
 // reported and has no pages; its start there is 0 (its results are nothing, and the attention reads within the arrays for it).  Rows behind a sequence's end are
-// zeros.  A block per page and key head.
+// zeros.  key_scale: the keys are multiplied by 1, -1 or 0 (the attention wants a scale above 0).  A block per page and key head.
 struct OpenSeq {
     int len, pages;                                              // pages: -1 if it does not fit
 };
@@ -472,10 +472,17 @@ __device__ __forceinline__ OpenSeq open_seq(const int* cu_seqlens, const int* st
     return {ok ? (int)len : 0, ok ? ((int)len + kPage - 1) / kPage : -1};
 }
 
+// Two bfloat16 numbers times -1 or 0 (exact; what is infinite or no number times 0 is none).
+__device__ __forceinline__ uint32_t scaled(uint32_t x, int by) {
+    if (by < 0) return x ^ 0x80008000u;
+    const uint32_t lo = (x & 0x7F80u) == 0x7F80u ? 0x7FFFu : 0u, hi = (x & 0x7F800000u) == 0x7F800000u ? 0x7FFF0000u : 0u;
+    return lo | hi;
+}
+
 __global__ void __launch_bounds__(256)
 open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const int* __restrict__ page_table, int table_width,
             const int* __restrict__ cu_seqlens, const int* __restrict__ start, int n_seqs, int n_tokens, bf16* __restrict__ out,
-            int* __restrict__ out_table, int* __restrict__ out_cu, int* __restrict__ out_start, int* status) {
+            int* __restrict__ out_table, int* __restrict__ out_cu, int* __restrict__ out_start, int key_scale, int* status) {
     // (No pdl_trigger: the kernel behind this one may read the page table before it waits, and this one writes it.)
     __shared__ int found[4];
     const int p = blockIdx.x, h = blockIdx.y;
@@ -567,7 +574,8 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
     for (int u = 0; u < STEPS; ++u) {
         const bool is_v = u >= STEPS / 2;
         const int i = u * 256 + threadIdx.x, t = i / (D / 8) % kPage;
-        const uint4 v = values_of(e[u], is_v);
+        uint4 v = values_of(e[u], is_v);
+        if (!is_v && key_scale != 1) v = make_uint4(scaled(v.x, key_scale), scaled(v.y, key_scale), scaled(v.z, key_scale), scaled(v.w, key_scale));
         *reinterpret_cast<uint4*>(out + ((((int64_t)p * 2 + is_v) * n_kv + h) * kPage + t) * D + 8 * (i % (D / 8))) = t < rows ? v : make_uint4(0, 0, 0, 0);
     }
 }
@@ -622,14 +630,15 @@ WICK_API int wick_kv4_read(const void* kv, int64_t kv_pages, int n_kv, const int
 }
 WICK_PACKED(wick_kv4_read)
 
-// out: bfloat16 [out_pages, 2, n_kv, 64, d]; out_table: int32 [n_seqs, table_width]; out_cu: int32 [n_seqs + 1]; out_start: int32 [n_seqs].
+// out: bfloat16 [out_pages, 2, n_kv, 64, d]; out_table: int32 [n_seqs, table_width]; out_cu: int32 [n_seqs + 1]; out_start: int32 [n_seqs]; key_scale: 1, -1 or 0.
 WICK_API int wick_kv4_open(const void* kv, int64_t kv_pages, int n_kv, const int* page_table, int table_width, const int* cu_seqlens, const int* start,
-                           int n_seqs, int n_tokens, void* out, int out_pages, int* out_table, int* out_cu, int* out_start, int* status, void* stream) {
+                           int n_seqs, int n_tokens, void* out, int out_pages, int* out_table, int* out_cu, int* out_start, int key_scale,
+                           int* status, void* stream) {
     WICK_REQUIRE(n_kv > 0 && n_kv <= 65535 && table_width > 0 && table_width <= INT32_MAX / kPage && n_seqs > 0 && n_tokens >= 0 && out_pages > 0,
                  "kv4_open: bad sizes");
     WICK_REQUIRE((((uintptr_t)kv | (uintptr_t)out) & 15) == 0, "kv4_open: arrays must begin on multiples of 16 bytes");
     WICK_CUDA(launch(kv4::open_kernel, dim3(out_pages, n_kv), dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)kv, kv_pages, n_kv, page_table,
-                     table_width, cu_seqlens, start, n_seqs, n_tokens, (bf16*)out, out_table, out_cu, out_start, status));
+                     table_width, cu_seqlens, start, n_seqs, n_tokens, (bf16*)out, out_table, out_cu, out_start, key_scale, status));
     return check_launch("kv4_open");
 }
 WICK_PACKED(wick_kv4_open)

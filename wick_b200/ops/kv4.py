@@ -274,8 +274,14 @@ def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratc
         return out
     at = pages * n_kv * PAGE * hd
     base, names = scratch.data_ptr(), at + n_seqs * width
-    lib.call_packed("wick_kv4_open", "plipippiipippppp", kv.data_ptr(), kv_pages, n_kv, table.data_ptr(), width, cu.data_ptr(), start.data_ptr(), n_seqs, n,
-                    base, pages, base + 4 * at, base + 4 * names, base + 4 * (names + n_seqs + 1), status, _stream())
+    # (the prompt attention takes scales above 0: of another sign, or 0 as a float32, it goes with the keys)
+    sign = 1
+    if not scale >= 2.0 ** -126:
+        bare = ctypes.c_float(scale).value
+        if bare <= 0:
+            sign, scale = (0, 1.0) if bare == 0 else (-1, -scale)
+    lib.call_packed("wick_kv4_open", "plipippiipipppipp", kv.data_ptr(), kv_pages, n_kv, table.data_ptr(), width, cu.data_ptr(), start.data_ptr(), n_seqs, n,
+                    base, pages, base + 4 * at, base + 4 * names, base + 4 * (names + n_seqs + 1), sign, status, _stream())
     flat = scratch.view(-1)                                          # (views while the kernel runs)
     table, cu, start = flat[at:words].view(torch.int32).split([n_seqs * width, n_seqs + 1, n_seqs])
     return attention_prompt(q, flat[:at].view(_BF16).view(pages, 2, n_kv, PAGE, hd), types.SimpleNamespace(
