@@ -160,3 +160,40 @@ def test_opened_pages_and_scales(scale, d):
     want[182, 2:] = True
     assert torch.equal(o.attention_kv4(q, kv.cuda(), b, scale, kind="opened").isnan(), want)
     o.check_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("starts,new", [([100, 60], [40, 90]), ([0, 64], [300, 65]), ([63], [2])])
+def test_opened_values_that_are_no_numbers(starts, new, d):
+    """A value that is no number shows in the rows of the tokens that see it, and in no others: in its channels where all of the step's tokens see
+    it, else in all of its head's.  Behind a sequence's end and in other pages nothing shows."""
+    o = ops()
+    g = torch.Generator().manual_seed(d + new[0])
+    pages, b = step(starts, new, g, spare=2)
+    kv, cache = random_cache(pages, 2, d, g)
+    q = torch.randn((b.n_tokens, 4, d), generator=g).to(BF16).cuda()
+    nan = torch.tensor([0.0, math.nan], dtype=BF16).view(torch.uint8)
+    used = {b.table[i][p]: (i, p) for i in range(len(new)) for p in range(-(-(starts[i] + new[i]) // PAGE))}
+    clean = o.attention_kv4(q, kv.cuda(), b, 0.1, kind="opened")
+    scales = kv[:, :, 64 * d:].view(pages, 2, 2, PAGE, d // 32, 4)
+    for p in range(pages):
+        end = starts[used[p][0]] + new[used[p][0]] - used[p][1] * PAGE if p in used else 0
+        scales[p, :, :, max(0, min(PAGE, end)):] = nan
+    assert torch.equal(o.attention_kv4(q, kv.cuda(), b, 0.1, kind="opened"), clean)
+    for i in range(len(new)):
+        for pos in {0, starts[i], starts[i] + 1, starts[i] + new[i] // 2, starts[i] + new[i] - 1}:
+            one = kv.clone()
+            at = one[:, :, 64 * d:].view(scales.shape)
+            at[b.table[i][pos // PAGE], 1, 1, pos % PAGE, 1] = nan          # (the second key head, channels 32 to 63)
+            first = max(0, pos - starts[i]) + sum(new[:i])
+            want = torch.zeros(q.shape, dtype=torch.bool, device="cuda")
+            if pos <= starts[i]:
+                want[first:sum(new[:i + 1]), 2:, 32:64] = True
+            else:
+                want[first:sum(new[:i + 1]), 2:] = True
+            for scale in (0.1, -0.1):
+                out = o.attention_kv4(q, one.cuda(), b, scale, kind="opened")
+                assert torch.equal(out.isnan(), want), (i, pos)
+                if scale > 0:
+                    assert torch.equal(out[~want], clean[~want])
+    o.check_status()

@@ -112,7 +112,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&h);
 }
-__device__ __forceinline__ bool no_number(uint32_t scale) { return (scale & 0x7F80u) == 0x7F80u || (scale & 0x7F800000u) == 0x7F800000u; }
 // The position (of 8) in row i of the instruction's position side.
 __device__ __forceinline__ int position_of(int i) { return i ^ ((i >> 1) & 1); }
 

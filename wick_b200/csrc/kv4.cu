@@ -461,15 +461,17 @@ read_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
 // The pages of all sequences of a step, in order, as bfloat16 pages [2, n_kv, 64, d] one behind the other, and a description of the step over them for the
 // attention: the table that names them (every place of it), and the sequences' tokens and starts.  A sequence that does not fit the step or its page table is
 // reported and has no pages; its start there is 0 (its results are nothing, and the attention reads within the arrays for it).  Rows behind a sequence's end are
-// zeros.  key_scale: the keys are multiplied by 1, -1 or 0 (the attention wants a scale above 0).  A block per page and key head.
+// zeros.  key_scale: the keys are multiplied by 1, -1 or 0 (the attention wants a scale above 0).  A value that is no number would show in earlier tokens'
+// rows too (they weigh it with 0, and 0 times it is none): where some token of the step does not see the position, its group is zeros and the position's key
+// no number, which shows in every channel of the rows that see it, and in no others.  A block per page and key head.
 struct OpenSeq {
-    int len, pages;                                              // pages: -1 if it does not fit
+    int start, len, pages;                                       // pages: -1 if it does not fit
 };
 __device__ __forceinline__ OpenSeq open_seq(const int* cu_seqlens, const int* start, int s, int n_tokens, int table_width) {
     const int first = cu_seqlens[s], end = cu_seqlens[s + 1], from = start[s];
     const int64_t len = (int64_t)from + end - first;
     const bool ok = first >= 0 && end >= first && end <= n_tokens && from >= 0 && len <= (int64_t)table_width * kPage;
-    return {ok ? (int)len : 0, ok ? ((int)len + kPage - 1) / kPage : -1};
+    return {from, ok ? (int)len : 0, ok ? ((int)len + kPage - 1) / kPage : -1};
 }
 
 // Two bfloat16 numbers times -1 or 0 (exact; what is infinite or no number times 0 is none).
@@ -484,16 +486,17 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
             const int* __restrict__ cu_seqlens, const int* __restrict__ start, int n_seqs, int n_tokens, bf16* __restrict__ out,
             int* __restrict__ out_table, int* __restrict__ out_cu, int* __restrict__ out_start, int key_scale, int* status) {
     // (No pdl_trigger: the kernel behind this one may read the page table before it waits, and this one writes it.)
-    __shared__ int found[4];
+    __shared__ int found[5];
+    __shared__ uint8_t none[kPage];
     const int p = blockIdx.x, h = blockIdx.y;
     const bool describes = p == 0 && h == 0;                     // (the block that writes what is not a page's)
     if (threadIdx.x < 32) {
         // the sequence of page p of the step, and its first page's number: a scan over the sequences' pages
         const int lane = threadIdx.x;
-        int before = 0, b = -1, j = 0, len = 0;
+        int before = 0, b = -1, j = 0, len = 0, from = 0;
         for (int s0 = 0; s0 < n_seqs; s0 += 32) {
             const int s = s0 + lane;
-            const OpenSeq it = s < n_seqs ? open_seq(cu_seqlens, start, s, n_tokens, table_width) : OpenSeq{0, 0};
+            const OpenSeq it = s < n_seqs ? open_seq(cu_seqlens, start, s, n_tokens, table_width) : OpenSeq{0, 0, 0};
             const int mine = max(it.pages, 0);
             int upto = mine;
 #pragma unroll
@@ -507,6 +510,7 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
                 b = s0 + l;
                 j = p - before - __shfl_sync(0xffffffffu, upto - mine, l);
                 len = __shfl_sync(0xffffffffu, it.len, l);
+                from = __shfl_sync(0xffffffffu, it.start, l);
                 if (!describes) break;
             }
             before += total;
@@ -516,6 +520,7 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
             found[1] = j;
             found[2] = len;
             found[3] = before;                                   // (where it describes the step: all pages)
+            found[4] = from;
         }
     }
     __syncthreads();
@@ -569,7 +574,31 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
         }
     }
     if (b < 0) return;
-    const int rows = min(kPage, len - j * kPage);
+    const int rows = min(kPage, len - j * kPage), hidden = max(0, found[4] + 1 - j * kPage);        // (from row `hidden` on: not seen by all tokens)
+    if (hidden < rows) {
+        bool any = false;
+#pragma unroll
+        for (int u = STEPS / 2; u < STEPS; ++u) {
+            const int t = (u * 256 + (int)threadIdx.x) / (D / 8) % kPage;
+            any |= no_number(e[u].scales) && t >= hidden && t < rows;
+        }
+        if (__syncthreads_or(any)) {
+            if (threadIdx.x < kPage) none[threadIdx.x] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int u = STEPS / 2; u < STEPS; ++u) {
+                const int t = (u * 256 + (int)threadIdx.x) / (D / 8) % kPage;
+                if (no_number(e[u].scales) && t >= hidden) {
+                    e[u].scales = 0;
+                    none[t] = 1;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < STEPS / 2; ++u)
+                if (none[(u * 256 + threadIdx.x) / (D / 8) % kPage]) e[u].scales = 0x7FFF0000u;
+        }
+    }
 #pragma unroll
     for (int u = 0; u < STEPS; ++u) {
         const bool is_v = u >= STEPS / 2;

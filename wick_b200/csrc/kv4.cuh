@@ -49,6 +49,8 @@ __device__ __forceinline__ uint32_t two_values(uint32_t x, uint32_t a2, uint32_t
 }
 __device__ __forceinline__ uint32_t low_halves(uint32_t x, uint32_t y) { return __byte_perm(x, y, 0x5410); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t x, uint32_t y) { return __byte_perm(x, y, 0x7632); }
+// Whether a pair of scales stands for values that are no numbers.
+__device__ __forceinline__ bool no_number(uint32_t scale) { return (scale & 0x7F80u) == 0x7F80u || (scale & 0x7F800000u) == 0x7F800000u; }
 
 // A word of keys' codes: v[i] has channels i and i + 4.
 __device__ __forceinline__ void key_word(uint32_t w, uint32_t a2, uint32_t b2, uint32_t (&v)[4]) {

@@ -220,8 +220,10 @@ def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratc
     """Causal attention of the step's new tokens (any number a sequence) over a cache in 4 bits, which already holds their keys and values.
     q: [n, heads, d], bfloat16 or float32.  scratch: float32, at least :func:`attention_kv4_scratch` words (made here if none is given).
     While no sequence has more than eight rows (new tokens times query heads of a key head), a sequence's result does not depend on the batch
-    that it is in.  plain: on the CUDA cores, without bulk copies (float32 always is); ``kind`` picks a form by hand.  A sequence that does not fit its page table or ``batch.kv_bound``, or names a page
-    outside the cache, is reported (:func:`~wick_b200.ops.check_status`)."""
+    that it is in.   plain: on the CUDA cores, without bulk copies (float32 always is); ``kind`` picks a form by hand.  A value that is no number shows
+    in its channels of the rows that see its position (where pages are opened and it is one of the step's own after the first token's: in all channels of
+    those rows).  A sequence that does not fit its page table or ``batch.kv_bound``, or names a page outside the cache, is reported
+    (:func:`~wick_b200.ops.check_status`); so is one whose tokens are not among the step's."""
     shape = q.shape
     if len(shape) != 3:
         raise KernelError(f"q must be [n, heads, head_dim], is {tuple(shape)}")
