@@ -5,6 +5,7 @@ import types
 import pytest
 import torch
 
+from plain import kv4_plain as P
 from test_gpu_kv4 import BF16, F32, PAGE, check_attention, ints, ops, random_cache, step
 
 pytestmark = pytest.mark.gpu
@@ -197,3 +198,46 @@ def test_opened_values_that_are_no_numbers(starts, new, d):
                 if scale > 0:
                     assert torch.equal(out[~want], clean[~want])
     o.check_status()
+
+
+# ---- append: numbers at the ends of their ranges, and steps of many tokens -------------
+MANY = 300                                                           # tokens, of which a step's keys and values are looked at in 32 bits first
+
+
+def append_rows(k, v, splits=1, w=None, eps=0.0):
+    """Keys and values float32 [splits, n, d] of n tokens, one head each, into a cache of their own: its bytes, and what it holds (float64 [2, n, d])."""
+    o = ops()
+    n, d = k.shape[1:]
+    pages = -(-n // PAGE)
+    at = types.SimpleNamespace(page_table=ints([list(range(1, pages + 1))]), seq_of_token=ints([0] * n), positions=ints(list(range(n))))
+    kv = torch.zeros((pages + 1, 1, 80 * d), dtype=torch.uint8, device="cuda")
+    x = torch.cat([torch.zeros_like(k), k, v], 2).cuda().contiguous()
+    o.qk_norm_rope_append_kv4(x, 1, 1, d, q_weight=w, k_weight=w, eps=eps, cos=None, sin=None, kv=kv, dtype=F32, **vars(at))
+    held = o.kv4_read(kv, d, at.page_table, at.seq_of_token, at.positions).double().cpu()[:, :, 0]
+    o.check_status()
+    return kv.cpu(), held
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_append_of_ranges_that_bfloat16_cannot_hold(many):
+    """32 finite numbers below 2^127 whose b is beyond bfloat16's range are stored as numbers that are none; somewhat smaller ones as ever."""
+    d = 64
+    n = MANY if many else 6
+    x = torch.randn((2, n, d), generator=torch.Generator().manual_seed(21)).double()
+    edges = ((0, -1.2e38, 1.2e38, True), (1, -1.0e38, 1.0e38, False), (2, -1.6e38, 0.2e38, True), (3, 0.0, 1.6e38, False), (4, -1.65e38, -1.6e38, False),
+             (5, -1.1e38, 1.09e38, True))
+    for i in range(2):
+        for row, low, high, _ in edges:
+            x[i, row, 32 * i:32 * i + 32] = torch.linspace(0, 1, 32).double() * (high - low) + low
+    x = x.float()
+    _, held = append_rows(x[:1], x[1:])
+    for i in range(2):
+        for row, low, high, beyond in edges:
+            a = ((torch.tensor(high).float().double() - torch.tensor(low).float().double()) * (16 / 15)).to(BF16).double()
+            b = (torch.tensor(low).float().double() - a).to(BF16)
+            assert a.isfinite() and b.isfinite().item() != beyond, row   # (the table is right)
+            part, rest = held[i, row, 32 * i:32 * i + 32], held[i, row, 32 - 32 * i:64 - 32 * i]
+            assert part.isnan().all() if beyond else part.isfinite().all(), (i, row)
+            assert rest.isfinite().all()
+            if not beyond:
+                assert torch.equal(part, P.decode(*P.encode(x[i, row:row + 1, 32 * i:32 * i + 32].double()))[0])

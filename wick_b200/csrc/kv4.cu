@@ -118,7 +118,8 @@ __device__ __forceinline__ void encode_exactly(const double (&x)[8], const Sourc
     // (to bfloat16 by way of 32 bits, as conversions from 64 bits go elsewhere)
     bf16 a = __float2bfloat16_rn((float)((hi - lo) * (16.0 / 15.0)));
     bf16 b = __float2bfloat16_rn((float)(lo - (double)__bfloat162float(a)));
-    if (bad || fmax(fabs(lo), fabs(hi)) > (double)LARGEST || !isfinite(__bfloat162float(a))) {
+    // (b on its own: from -1.2e38 to 1.2e38, say, a is finite and min - a is not)
+    if (bad || fmax(fabs(lo), fabs(hi)) > (double)LARGEST || !isfinite(__bfloat162float(a)) || !isfinite(__bfloat162float(b))) {
         a = __float2bfloat16_rn(0.f);
         b = __ushort_as_bfloat16(0x7FFF);
     }

@@ -8,7 +8,7 @@
 //   values' scales [64, d / 32]
 // The value of code c is  bf16(b + a (1 + c / 16)),  one rounding.  A group's numbers x are stored with
 //   a = bf16(16 (max - min) / 15),  b = bf16(min - a),  c = the whole number nearest to 16 (x - b) / a - 16, within 0 .. 15 (0 where a is 0);
-// a group with a number that is none or is beyond 2^127, or with a range beyond bfloat16's, is stored as a = 0, b = NaN, so that it shows.
+// a group with a number that is none or is beyond 2^127, or whose a or b is beyond bfloat16's range, is stored as a = 0, b = NaN, so that it shows.
 //
 // Why this form.  1 + c / 16 is the bfloat16 number with the bits of 1 and c in the upper four bits of its mantissa (3 .. 6): two codes that lie
 // there, one in either half of a register, are an AND-OR away from two numbers, and one fused multiply-add from two values.  Turned left by 3, a

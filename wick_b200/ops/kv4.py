@@ -2,8 +2,8 @@
 
 ``kv`` is one entry's part of such a cache: uint8 [pages, kv_heads, 80 d], pages of 64 positions, head sizes d of 64, 128, 192 and 256.  32
 neighbouring channels of a key or a value share a pair of bfloat16 numbers (a, b); the value of a code c (0 to 15) is bfloat16(b + a (1 + c / 16)).
-A number is stored with the nearest code of its group's range; a group with an infinity, with a number that is none or beyond 2 ** 127 is
-stored as numbers that are none.  Five bits a number, in place of 16 or 32.
+A number is stored with the nearest code of its group's range; a group with an infinity, with a number that is none or beyond 2 ** 127,
+or whose a or b bfloat16 cannot hold, is stored as numbers that are none.  Five bits a number, in place of 16 or 32.
 """
 from __future__ import annotations
 
