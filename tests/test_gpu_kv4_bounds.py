@@ -241,3 +241,69 @@ def test_append_of_ranges_that_bfloat16_cannot_hold(many):
             assert rest.isfinite().all()
             if not beyond:
                 assert torch.equal(part, P.decode(*P.encode(x[i, row:row + 1, 32 * i:32 * i + 32].double()))[0])
+
+
+@pytest.mark.parametrize("heads,n_kv,d", [(4, 2, 64), (6, 2, 128), (5, 1, 192), (4, 2, 256)])
+@pytest.mark.parametrize("splits,dtype,norm,turn", [(0, BF16, True, True), (3, BF16, True, True), (1, F32, True, False), (8, BF16, False, True), (2, F32, False, False),
+                                                    (0, BF16, False, False), (0, F32, False, True), (0, F32, True, True)])
+def test_append_of_many_tokens(heads, n_kv, d, splits, dtype, norm, turn):
+    """Steps of more than 256 tokens look at keys and values in 32 bits first: the codes are those of 64 bits, and the same bytes as in smaller steps."""
+    o = ops()
+    g = torch.Generator().manual_seed(heads * d + splits)
+    starts, new = [0, 61, 5], [300, 3, 1]
+    pages, b = step(starts, new, g, spare=2)
+    n = b.n_tokens
+    x = torch.randn((max(splits, 1), n, (heads + 2 * n_kv) * d), generator=g) * 2
+    x[:, 40:60] *= 100.0                                             # (tokens of other sizes)
+    x[:, 60:80] *= 0.01
+    x = x if splits else x[0].to(dtype)
+    w = (torch.rand(d, generator=g) + 0.5) if norm else None
+    angle = b.positions.cpu().double()[:, None] * 1e4 ** (-torch.arange(d // 2).double() / (d // 2))
+    cos, sin = (angle.cos().float(), angle.sin().float()) if turn else (None, None)
+    up = lambda v: None if v is None else v.cuda()      # noqa: E731
+
+    def run(kv, first, last):
+        part = x[:, first:last] if splits else x[first:last]
+        return o.qk_norm_rope_append_kv4(part.contiguous().cuda(), heads, n_kv, d, q_weight=up(w), k_weight=up(w), eps=1e-6,
+                                         cos=None if cos is None else cos[first:last].contiguous().cuda(),
+                                         sin=None if sin is None else sin[first:last].contiguous().cuda(), kv=kv, page_table=b.page_table,
+                                         seq_of_token=b.seq_of_token[first:last].contiguous(), positions=b.positions[first:last].contiguous(), dtype=dtype)
+    kv = torch.full((pages, n_kv, 80 * d), 0x5A, dtype=torch.uint8, device="cuda")
+    pieces = kv.clone()
+    q = run(kv, 0, n)
+    assert torch.equal(q, torch.cat([run(pieces, 0, 100), run(pieces, 100, 290), run(pieces, 290, n)]))
+    assert torch.equal(kv, pieces)
+    eps = torch.tensor(1e-6, dtype=F32).double().item()
+    _, k, v = P.project(x.double().sum(0) if splits else x.double(), heads, n_kv, d, w, w, eps, cos, sin)
+    held = o.kv4_read(kv, d, b.page_table, b.seq_of_token, b.positions).double().cpu()
+    assert torch.equal(held[0], P.decode(*P.encode(k))) and torch.equal(held[1], P.decode(*P.encode(v)))
+    o.check_status()
+
+
+def test_append_of_many_odd_numbers():
+    """Numbers on borders between codes, equal ones, runs that cancel, numbers that are none, in a step of many tokens."""
+    d = 64
+    g = torch.Generator().manual_seed(22)
+    x = torch.randn((2, 3, MANY, d), generator=g)
+    x[:, 1:] = 0
+    whole = torch.arange(d).float()
+    x[:, 0, 0], x[:, 0, 1], x[:, 0, 2] = 0.0, 3.140625, whole
+    x[:, 0, 3] = 1.0 + whole / 4096
+    x[:, 0, 4] = torch.where(whole % 2 == 0, 0.0, 15.0)
+    x[:, 0, 4, 1::4] = torch.arange(16).float() % 15 + 0.5
+    x[0, 0, 5, 5], x[1, 0, 6, 40], x[0, 0, 7, 33] = math.inf, math.nan, -math.inf
+    x[:, 0, 8] *= 1e-38
+    x[:, 0, 9] *= 1e37
+    x[:, 0, 10:40] = torch.randint(-8, 8, (2, 30, d), generator=g).float()            # (few bits: halves between two codes)
+    x[:, 0, 40:70] = (x[:, 0, 40:70] * 16).round() / 16
+    x[:, 1, 100:150] = 1e4 * torch.randn((2, 50, d), generator=g)                     # (runs that cancel)
+    x[:, 2, 100:150] = -x[:, 1, 100:150]
+    x[:, 1, 150:200] = 3e6 * torch.randn((2, 50, d), generator=g)
+    x[:, 2, 150:200] = -x[:, 1, 150:200]
+    x[:, 0, 200:250] += 1e3                                                           # (a range far from zero)
+    for splits in (1, 3):
+        k, v = x[0, :splits], x[1, :splits]
+        _, held = append_rows(k, v)
+        for i, y in enumerate((k, v)):
+            want = P.decode(*P.encode(y.double().sum(0)))
+            assert torch.equal(held[i].isnan(), want.isnan()) and torch.equal(held[i].nan_to_num(7.0), want.nan_to_num(7.0)), (splits, i)
