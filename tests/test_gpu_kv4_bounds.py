@@ -307,3 +307,23 @@ def test_append_of_many_odd_numbers():
         for i, y in enumerate((k, v)):
             want = P.decode(*P.encode(y.double().sum(0)))
             assert torch.equal(held[i].isnan(), want.isnan()) and torch.equal(held[i].nan_to_num(7.0), want.nan_to_num(7.0)), (splits, i)
+
+
+@pytest.mark.parametrize("size,weight,eps", [(1e-18, 1.0, 0.0), (1e-20, 1.0, 0.0), (3e-22, 1.0, 0.0), (1e-24, 1e3, 0.0), (1e-19, 1.0, 1e-38), (1e-38, 1e12, 1e-6),
+                                             (1.0, 1e20, 1e-6), (1e15, 1.0, 1e-6), (1e19, 1e-3, 1e-6), (3e19, 1.0, 1e-6)])
+def test_append_of_many_norms_at_the_ends_of_the_range(size, weight, eps):
+    """Mean squares below the smallest normal 32-bit number (and above the largest) are as good as others."""
+    d = 64
+    g = torch.Generator().manual_seed(23)
+    k = torch.randn((1, MANY, d), generator=g) * size
+    k[:, :, 32:40] *= 1e-4                                           # (some numbers much smaller than their row's size)
+    k[:, 100:, 32:] *= torch.exp2(-torch.arange(MANY - 100).float())[:, None]         # (... and whole groups)
+    w = (torch.rand(d, generator=g) + 0.5) * weight
+    _, held = append_rows(k, torch.zeros_like(k), w=w.cuda(), eps=eps)
+    y = k[0].double()
+    y = y / torch.sqrt(y.pow(2).mean(-1, keepdim=True) + torch.tensor(eps, dtype=F32).double()) * w.double()
+    codes, a, b = P.encode(y)
+    # (scales below the smallest normal number are not held to be kept, see the test of odd numbers)
+    fine = (a >= 2.0 ** -126).repeat_interleave(32, -1)
+    assert torch.equal(held[0][fine], P.decode(codes, a, b)[fine])
+    assert fine[:100].all() or weight * size < 1e-20

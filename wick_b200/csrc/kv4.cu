@@ -347,6 +347,7 @@ append_kernel(const T* __restrict__ qkv, const float* __restrict__ parts, int sp
         load8(qkv + base, a);
         load8(qkv + base + half, b);
     }
+    float largest = 0.f, turn = 1.f;                             // of the numbers before the rotation, and of its cosines and sines
     if (w) {
         float wa[8], wb[8];
         load8(w + i0, wa);
@@ -362,7 +363,14 @@ append_kernel(const T* __restrict__ qkv, const float* __restrict__ parts, int sp
             double ss = 0.0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) ss += (double)a[k] * (double)a[k] + (double)b[k] * (double)b[k];
-            scale = 1.0f / sqrtf((float)(vector_sum(ss, mask) * (1.0 / D) + (double)eps));
+            const float mean = (float)(vector_sum(ss, mask) * (1.0 / D) + (double)eps);
+            scale = 1.0f / sqrtf(mean);
+            // Numbers below the smallest normal one are off by up to 2^-150, however small they are: such a mean proves nothing, and the numbers and their
+            // products with the scale are off by that times what they are multiplied by (1.2e-38 of 7.5 roundings and more is above it).
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, fmaxf(fabsf(wa[k]), fabsf(wb[k])));
+            largest = mean < 1.2e-38f ? INFINITY : 1.2e-38f * top * (scale + 1.f);
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -370,10 +378,11 @@ append_kernel(const T* __restrict__ qkv, const float* __restrict__ parts, int sp
             b[k] = (b[k] * scale) * wb[k];
         }
     }
-    float largest = 0.f, turn = 1.f;                             // of the numbers before the rotation, and of its cosines and sines
     if (!is_q) {
+        float size = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) largest = fmaxf(largest, fmaxf(fabsf(a[k]), fabsf(b[k])));
+        for (int k = 0; k < 8; ++k) size = fmaxf(size, fmaxf(fabsf(a[k]), fabsf(b[k])));
+        largest += size;
     }
     if (rotate) {
         float c[8], sn[8];
