@@ -327,3 +327,20 @@ def test_append_of_many_norms_at_the_ends_of_the_range(size, weight, eps):
     fine = (a >= 2.0 ** -126).repeat_interleave(32, -1)
     assert torch.equal(held[0][fine], P.decode(codes, a, b)[fine])
     assert fine[:100].all() or weight * size < 1e-20
+
+
+# ---- attention: other devices, and no cache at all ----------------------------------------
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="one device")
+def test_on_a_second_device():
+    """Kernels with more shared memory than a device gives unasked, on the first device and then on another."""
+    o = ops()
+    g = torch.Generator().manual_seed(24)
+    pages, b = step([900, 70, 3000], [2, 3, 1], g)
+    kv, cache = random_cache(pages, 2, 128, g)
+    q = torch.randn((6, 8, 128), generator=g).to(BF16)
+    for device in ("cuda:0", "cuda:1"):
+        with torch.cuda.device(device):
+            there = types.SimpleNamespace(**{k: v.to(device) if isinstance(v, torch.Tensor) else v for k, v in vars(b).items()})
+            for kind in ("records", "clusters", "stay", "opened"):
+                check_attention(q, o.attention_kv4(q.to(device), kv.to(device), there, 0.1, kind=kind), cache, b, 0.1, 128)
+            o.check_status()

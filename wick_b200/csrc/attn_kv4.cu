@@ -1156,17 +1156,21 @@ static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int
     return p;
 }
 
-// Dynamic shared memory beyond what a kernel has without asking.
+// Dynamic shared memory beyond what a kernel has without asking (of the current device: each is asked once).
 static int allow(void (*kernel)(Args), int bytes) {
-    static void (*asked[16])(Args) = {};                          // (two host threads may both ask: it does no harm)
-    for (int i = 0; i < 16; ++i) {
-        if (asked[i] == kernel) return 0;
-        if (asked[i] == nullptr) {
+    static void (*asked[64][16])(Args) = {};                      // (two host threads may both ask: it does no harm)
+    int dev = 0;
+    WICK_CUDA(cudaGetDevice(&dev));
+    void (**mine)(Args) = dev >= 0 && dev < 64 ? asked[dev] : nullptr;
+    for (int i = 0; mine && i < 16; ++i) {
+        if (mine[i] == kernel) return 0;
+        if (mine[i] == nullptr) {
             WICK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-            asked[i] = kernel;
+            mine[i] = kernel;
             return 0;
         }
     }
+    WICK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     return 0;
 }
 

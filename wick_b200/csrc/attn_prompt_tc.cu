@@ -814,9 +814,11 @@ static int attn_prompt_tc(const void* q, long long n_tokens, const void* kv, lon
     const bool shorts = !extra && !guard && (long long)table_width * kPage <= (LONG - 1) * BK;
     auto kernel = extra ? (guard ? attn_prompt_tc_kernel<true, true, true> : attn_prompt_tc_kernel<true, false, true>)
                         : (guard ? attn_prompt_tc_kernel<false, true, true> : (shorts ? attn_prompt_tc_kernel<false, false, false> : attn_prompt_tc_kernel<false, false, true>));
-    static bool raised[5] = {false, false, false, false, false};
-    bool& done = raised[shorts ? 4 : (extra ? 2 : 0) + (guard ? 1 : 0)];
-    if (!done) {
+    static bool raised[64][5] = {};                                // (a device's kernels are asked for it once)
+    int dev = 0;
+    WICK_CUDA(cudaGetDevice(&dev));
+    bool& done = raised[dev & 63][shorts ? 4 : (extra ? 2 : 0) + (guard ? 1 : 0)];
+    if (!done || dev > 63) {
         WICK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
         done = true;
     }

@@ -170,9 +170,17 @@ OPEN_ROWS = {64: 192, 128: 80}
 _FORMS = {None: 0, "plain": 1, "records": 2, "clusters": 3, "stay": 4, "opened": -1}
 
 
+def _current() -> int:
+    """The number of the current device, -1 without one."""
+    try:
+        return _device()
+    except RuntimeError:
+        return -1
+
+
 @functools.lru_cache(maxsize=4096)
-def _plan(head_dim: int, *sizes: int) -> Tuple[int, int]:
-    """float32 words of scratch of a call of these sizes, and the kernels that it launches."""
+def _plan(device: int, head_dim: int, *sizes: int) -> Tuple[int, int]:
+    """float32 words of scratch of a call of these sizes, and the kernels that it launches, on ``device``, the current one (its size decides as well)."""
     lib, kernels = _kv4(head_dim), ctypes.c_int(0)
     n = lib._lib.wick_attn_kv4_scratch(*sizes, ctypes.byref(kernels))
     if n < 0:
@@ -212,7 +220,7 @@ def attention_kv4_scratch(batch, n_heads: int, n_kv: int, head_dim: int, dtype: 
     form = _form(dtype, head_dim, max_q, n_heads // n_kv, kind, plain)
     if form < 0:
         return _open_words(batch, pages, n_kv, head_dim)[1]
-    return _plan(head_dim, batch.n_tokens, batch.n_seqs, n_heads, n_kv, max_q, kv_bound, dtype is _F32, form)[0]
+    return _plan(_current(), head_dim, batch.n_tokens, batch.n_seqs, n_heads, n_kv, max_q, kv_bound, dtype is _F32, form)[0]
 
 
 def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratch: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -258,7 +266,7 @@ def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratc
         pages, words = _open_words(batch, pages, n_kv, hd)
         kernels = 1
     else:
-        words, kernels = _plan(hd, n, n_seqs, n_heads, n_kv, max_q, kv_bound, dtype is _F32, form)
+        words, kernels = _plan(device, hd, n, n_seqs, n_heads, n_kv, max_q, kv_bound, dtype is _F32, form)
     if scratch is None:
         if words:
             scratch = torch.empty(words, dtype=_F32, device=q.device)
