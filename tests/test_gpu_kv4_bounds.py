@@ -344,3 +344,22 @@ def test_on_a_second_device():
             for kind in ("records", "clusters", "stay", "opened"):
                 check_attention(q, o.attention_kv4(q.to(device), kv.to(device), there, 0.1, kind=kind), cache, b, 0.1, 128)
             o.check_status()
+
+
+def test_a_cache_without_pages():
+    """There is nothing that a page outside it could be read as: refused, whatever the form; appending to it and reading from it is reported."""
+    o = ops()
+    for new in ([1, 1], [100, 3]):
+        _, b = step([5, 0], new, torch.Generator().manual_seed(25))
+        kv = torch.zeros((0, 2, 80 * 64), dtype=torch.uint8, device="cuda")
+        for dtype, kinds in ((BF16, (None, "plain", "records", "stay", "opened")), (F32, (None, "plain"))):
+            q = torch.zeros((b.n_tokens, 4, 64), dtype=dtype, device="cuda")
+            for kind in kinds:
+                with pytest.raises(o.KernelError, match="without pages"):
+                    o.attention_kv4(q, kv, b, 0.1, kind=kind)
+        o.check_status()
+        o.qk_norm_rope_append_kv4(torch.zeros((b.n_tokens, 8 * 64), device="cuda"), 4, 2, 64, q_weight=None, k_weight=None, eps=0.0, cos=None, sin=None, kv=kv,
+                                  page_table=b.page_table, seq_of_token=b.seq_of_token, positions=b.positions)
+        said()
+        assert (o.kv4_read(kv, 64, b.page_table, b.seq_of_token, b.positions) == 0).all()
+        said()

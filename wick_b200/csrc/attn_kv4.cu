@@ -1182,6 +1182,8 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
                  "attention_kv4: bad sizes");
     WICK_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "attention_kv4: arrays must begin on multiples of 16 bytes");
     if (n_tokens == 0) return 0;
+    // (a page outside the cache is read as page 0)
+    WICK_REQUIRE(kv_pages > 0, "attention_kv4: %d tokens, and a cache without pages", n_tokens);
     WICK_REQUIRE(max_q > 0 && kv_bound > 0, "attention_kv4: %d tokens, but up to %d a sequence and %d positions", n_tokens, max_q, kv_bound);
     const Plan p = plan(n_tokens, n_seqs, n_heads, n_kv, max_q, kv_bound, sizeof(T) == 4, form);
     WICK_REQUIRE(p.possible, "attention_kv4: the kernel asked for (%d) does not take these sizes", form);

@@ -676,6 +676,7 @@ WICK_API int wick_kv4_open(const void* kv, int64_t kv_pages, int n_kv, const int
     WICK_REQUIRE(n_kv > 0 && n_kv <= 65535 && table_width > 0 && table_width <= INT32_MAX / kPage && n_seqs > 0 && n_tokens >= 0 && out_pages > 0,
                  "kv4_open: bad sizes");
     WICK_REQUIRE((((uintptr_t)kv | (uintptr_t)out) & 15) == 0, "kv4_open: arrays must begin on multiples of 16 bytes");
+    WICK_REQUIRE(kv_pages > 0, "kv4_open: a cache without pages");
     WICK_CUDA(launch(kv4::open_kernel, dim3(out_pages, n_kv), dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)kv, kv_pages, n_kv, page_table,
                      table_width, cu_seqlens, start, n_seqs, n_tokens, (bf16*)out, out_table, out_cu, out_start, key_scale, status));
     return check_launch("kv4_open");

@@ -292,8 +292,9 @@ def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratc
             sign, scale = (0, 1.0) if bare == 0 else (-1, -scale)
     lib.call_packed("wick_kv4_open", "plipippiipipppipp", kv.data_ptr(), kv_pages, n_kv, table.data_ptr(), width, cu.data_ptr(), start.data_ptr(), n_seqs, n,
                     base, pages, base + 4 * at, base + 4 * names, base + 4 * (names + n_seqs + 1), sign, status, _stream())
-    flat = scratch.view(-1)                                          # (views while the kernel runs)
-    table, cu, start = flat[at:words].view(torch.int32).split([n_seqs * width, n_seqs + 1, n_seqs])
-    return attention_prompt(q, flat[:at].view(_BF16).view(pages, 2, n_kv, PAGE, hd), types.SimpleNamespace(
+    # (views while the kernel runs, in as few calls as that takes)
+    flat = (scratch if scratch.dim() == 1 else scratch.view(-1)).view(torch.int32)
+    opened, table, cu, start, _ = flat.split_with_sizes([at, n_seqs * width, n_seqs + 1, n_seqs, flat.shape[0] - words])
+    return attention_prompt(q, opened.view(_BF16).view(pages, 2, n_kv, PAGE, hd), types.SimpleNamespace(
         n_tokens=n, q_tiles=getattr(batch, "q_tiles", None), q_lens=batch.q_lens, cu_seqlens=cu, n_seqs=n_seqs, start=start,
-        page_table=table.view(n_seqs, width), table_width=width), scale, out=out)
+        page_table=table, table_width=width), scale, out=out)
