@@ -585,37 +585,30 @@ open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const in
     }
     if (b < 0) return;
     const int rows = min(kPage, len - j * kPage), hidden = max(0, found[4] + 1 - j * kPage);        // (from row `hidden` on: not seen by all tokens)
-    if (hidden < rows) {
-        bool any = false;
-#pragma unroll
-        for (int u = STEPS / 2; u < STEPS; ++u) {
-            const int t = (u * 256 + (int)threadIdx.x) / (D / 8) % kPage;
-            any |= no_number(e[u].scales) && t >= hidden && t < rows;
-        }
-        if (__syncthreads_or(any)) {
-            if (threadIdx.x < kPage) none[threadIdx.x] = 0;
-            __syncthreads();
-#pragma unroll
-            for (int u = STEPS / 2; u < STEPS; ++u) {
-                const int t = (u * 256 + (int)threadIdx.x) / (D / 8) % kPage;
-                if (no_number(e[u].scales) && t >= hidden) {
-                    e[u].scales = 0;
-                    none[t] = 1;
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < STEPS / 2; ++u)
-                if (none[(u * 256 + threadIdx.x) / (D / 8) % kPage]) e[u].scales = 0x7FFF0000u;
-        }
-    }
+    uint32_t lost = 0;                                           // this thread's values, a bit each, that are no numbers in such rows
+    uint4* page_out = reinterpret_cast<uint4*>(out + ((int64_t)p * 2 * n_kv + h) * kPage * D);
 #pragma unroll
     for (int u = 0; u < STEPS; ++u) {
         const bool is_v = u >= STEPS / 2;
-        const int i = u * 256 + threadIdx.x, t = i / (D / 8) % kPage;
+        const int i = u % (STEPS / 2) * 256 + threadIdx.x, t = i / (D / 8);
+        if (is_v && t >= hidden && t < rows && no_number(e[u].scales)) {
+            e[u].scales = 0;
+            lost |= 1u << (u - STEPS / 2);
+        }
         uint4 v = values_of(e[u], is_v);
         if (!is_v && key_scale != 1) v = make_uint4(scaled(v.x, key_scale), scaled(v.y, key_scale), scaled(v.z, key_scale), scaled(v.w, key_scale));
-        *reinterpret_cast<uint4*>(out + ((((int64_t)p * 2 + is_v) * n_kv + h) * kPage + t) * D + 8 * (i % (D / 8))) = t < rows ? v : make_uint4(0, 0, 0, 0);
+        page_out[(is_v ? (int64_t)n_kv * kPage * (D / 8) : 0) + i] = t < rows ? v : make_uint4(0, 0, 0, 0);
+    }
+    if (hidden < rows && __syncthreads_or(lost != 0)) {
+        if (threadIdx.x < kPage) none[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < STEPS / 2; ++u)
+            if (lost >> u & 1) none[(u * 256 + threadIdx.x) / (D / 8)] = 1;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < STEPS / 2; ++u)
+            if (none[(u * 256 + threadIdx.x) / (D / 8)]) page_out[u * 256 + threadIdx.x] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
     }
 }
 
