@@ -535,7 +535,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
         load_rows<NT>(a, s, kvh, row0, w);
 #pragma unroll 1
         for (int k = 0; k < count; ++k) {
-            if (!mbar_wait(&full[warp][k % a.stages], (k / a.stages) & 1, &abort_flag, a.status, 16)) {
+            // (all lanes leave together: those whose wait runs out as those that saw the copy arrive in the same instant)
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[warp][k % a.stages], (k / a.stages) & 1, &abort_flag, a.status, 16))) {
                 // (what is on its way has to arrive before this block's shared memory is somebody else's; again with a limit)
                 for (int i = k; i < min(count, k + a.stages); ++i) {
                     int mine = 0;
@@ -818,7 +819,6 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
     }
     Rows<NT> w;
     fetch_rows<NT>(a, place_of(cn.b), cn.kvh, cn.row0, w);
-    bool ok = true;
 #pragma unroll 1
     while (true) {
         const Seq s = place_of(cn.b);
@@ -846,7 +846,8 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
 #pragma unroll 1
             for (; page < leaf_end; ++page) {
                 int next_id = -1, next_kvh = cn.kvh;
-                ok = ok && mbar_wait(&full[warp][0], parity, &abort_flag, a.status, 16);
+                bool ok = mbar_wait(&full[warp][0], parity, &abort_flag, a.status, 16);
+                const bool keys = ok;                            // (of lane 0, which starts the copies)
                 leaf_page<NT>(a, tile, w, s, page, fresh, NT == 1 && cn.lp == 1, sum, [&]() {
                     if (page + 1 < cn.end) {
                         if (++held == 32) {
@@ -859,22 +860,23 @@ __global__ void __launch_bounds__(stay_warps<NT>() * 32, 1) stay_kernel(const Ar
                         next_kvh = nn.kvh;
                     }
                     __syncwarp();
-                    if (next_id >= 0) start_half(next_id, next_kvh, 0);
+                    if (next_id >= 0 && keys) start_half(next_id, next_kvh, 0);
                     // (the queries are not needed any more behind a node's last scores: the next item's are asked for)
                     if (NT == 1 && page + 1 == cn.end && nn.b >= 0) fetch_rows<NT>(a, place_of(nn.b), nn.kvh, nn.row0, w);
-                    ok = mbar_wait(&full[warp][1], parity, &abort_flag, a.status, 16) && ok;
+                    // (all lanes leave together: a wait may run out for one as the copy arrives for another)
+                    ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][1], parity, &abort_flag, a.status, 16) && ok);
                 });
+                if (!ok) {                                       // (what is on its way has to arrive before this shared memory is somebody else's)
+                    int mine = 0;
+                    if (lane == 0) mbar_wait(&full[warp][0], next_id >= 0 && keys ? parity ^ 1 : parity, &mine, a.status, 16);
+                    mine = 0;
+                    if (lane == 0) mbar_wait(&full[warp][1], parity, &mine, a.status, 16);
+                    return;
+                }
                 fresh = false;
                 parity ^= 1;
                 __syncwarp();
                 if (next_id >= 0) start_half(next_id, next_kvh, 1);
-                if (!ok) {                                       // (what is on its way has to arrive before this shared memory is somebody else's)
-                    for (int h = 0; h < 2 && next_id >= 0; ++h) {
-                        int mine = 0;
-                        mbar_wait(&full[warp][h], parity, &mine, a.status, 16);
-                    }
-                    return;
-                }
             }
             finish_leaf<NT>(sum);
             if constexpr (NT == 1) {
