@@ -363,3 +363,34 @@ def test_a_cache_without_pages():
         said()
         assert (o.kv4_read(kv, 64, b.page_table, b.seq_of_token, b.positions) == 0).all()
         said()
+
+
+@pytest.mark.parametrize("new,heads,d,dtype,kinds", [(130, 16, 256, BF16, (None, "records", "stay", "clusters")), (500, 16, 256, BF16, (None, "records", "stay", "clusters")),
+                                                     (61, 17, 64, F32, (None,)), (2000, 17, 64, F32, (None,))])
+def test_fewer_pieces_for_bounded_records(new, heads, d, dtype, kinds):
+    """So many rows behind so long a cache that its length alone would cut it into records of more than 256 MB; beside a short sequence."""
+    o = ops()
+    g = torch.Generator().manual_seed(new)
+    starts = [65600, 100]
+    pages, b = step(starts, [new, 3], g)
+    kv, cache = random_cache(pages, 1, d, g)
+    n = b.n_tokens
+    q = torch.randn((n, heads, d), generator=g).to(dtype).cuda()
+    scale = 1.0 / math.sqrt(d)
+    some = [0, 1, new // 2, new - 1]
+    for kind in kinds:
+        words = None
+        try:
+            words = o.attention_kv4_scratch(b, heads, 1, d, dtype, kind=kind)
+        except o.KernelError:
+            assert kind == "clusters"
+            continue
+        assert 4 * words <= 256 << 20
+        scratch = torch.full((words + 100,), math.nan, device="cuda")
+        out = o.attention_kv4(q, kv.cuda(), b, scale, scratch, kind=kind)
+        assert scratch[words:].isnan().all()
+        for t in some:
+            one = types.SimpleNamespace(q_lens=[1], starts=[starts[0] + t], table=[b.table[0]])
+            check_attention(q[t:t + 1], out[t:t + 1], cache, one, scale, d)
+        check_attention(q[new:], out[new:], cache, types.SimpleNamespace(q_lens=[3], starts=[100], table=[b.table[1]]), scale, d)
+    o.check_status()

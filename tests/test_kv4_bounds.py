@@ -29,3 +29,29 @@ def test_plans_are_kept_for_each_device(monkeypatch):
         assert asked == [0, 1]
     finally:
         kv4._plan.cache_clear()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+def test_records_have_a_bound(d, dtype):
+    """New tokens of many rows behind a long cache: what lies between the two kernels stays within 256 MB, whatever the length."""
+    from wick_b200 import ops
+    kinds = (None, "plain") if dtype == torch.float32 else (None, "plain", "records", "stay")
+    for heads, kv, new, seqs, length in ((16, 1, 2000, 1, 62000), (16, 1, 290, 1, 65000), (16, 1, 130, 1, 131000), (64, 8, 10, 16, 131000), (32, 2, 100, 3, 1000000),
+                                         (24, 2, 30000, 1, 100000), (9, 1, 1, 4000, 40000), (128, 1, 1, 900, 131000)):
+        b = batch(new * seqs, seqs, -(-(length + new) // 64), new, starts=[length] * seqs, q_lens=[new] * seqs)
+        for kind in kinds:
+            if kind == "stay" and seqs > 1024:
+                continue
+            if kind is None and new > 1 and new * heads // kv > ops.kv4.OPEN_ROWS.get(d, 1 << 30) and dtype == torch.bfloat16:
+                continue                                             # (opened)
+            assert 4 * ops.attention_kv4_scratch(b, heads, kv, d, dtype, kind=kind) <= 256 << 20, (heads, kv, new, kind)
+
+
+def test_records_follow_the_length_alone_up_to_eight_rows():
+    """... where a sequence's result does not depend on the batch that it is in."""
+    from wick_b200 import ops
+    for seqs in (1, 64, 1000):
+        b = batch(seqs, seqs, 2048, 1)
+        assert ops.attention_kv4_scratch(b, 8, 1, 128, torch.bfloat16, kind="records") == seqs * 8 * 128 * 130
+        assert ops.attention_kv4_scratch(b, 8, 1, 128, torch.float32, kind="plain") == seqs * 8 * 1024 * 130

@@ -45,6 +45,10 @@ constexpr int MAX_STAGES = D <= 128 ? 2 : 1;                      // of a warp's
 constexpr int CLUSTER = 8;                                       // nodes that a cluster joins at most
 constexpr int MAX_SEQS = 1024;                                   // of the form whose blocks stay
 constexpr int MT = D / 16;                                       // tiles of 16 channels
+// What records may take.  A step with more than eight rows a sequence and key head whose records would take more is cut into fewer pieces: its row tiles alone are work
+// enough then (2,000 tokens behind 62,000, 16 heads of 256 over one: 2,000 tiles, and records of 4.1 GB as cut by the length alone).  With up to eight rows
+// the cut is the length's, and a node's records are a twentieth of the bytes of its pages at most (a leaf's, on the CUDA cores, two fifths).
+constexpr int64_t RECORD_BYTES = 256 << 20;
 
 // A leaf is one page while one sequence alone so gives every SM up to two blocks (8 key heads: 37 nodes, 296 pages).  Longer sequences have nodes for one block
 // an SM (18) of long leaves, whose next page is on its way.  us, 32 heads over 8 of 128: 8 sequences of up to 12,000 positions, 24 nodes / 12 of twice the
@@ -79,10 +83,19 @@ struct Args {
     int tiles;                                                   // row tiles of a (sequence, key head) that the grid has
     int stages;                                                  // of a warp's ring
     int whole;                                                   // sequences are not cut: a row tile is one node
+    int most;                                                    // leaves of a sequence at most (RECORD_BYTES); 0: as its length says
     int* status;
 };
-__device__ __forceinline__ int leaf_pages(const Args& a, int n_pages) { return a.whole ? n_pages : leaf_pages(n_pages, a.n_kv); }
-__device__ __forceinline__ int nodes_of(const Args& a, int n_pages) { return a.whole ? 1 : nodes_of(n_pages, a.n_kv); }
+__device__ __forceinline__ int leaf_pages(const Args& a, int n_pages) {
+    if (a.whole) return n_pages;
+    const int lp = leaf_pages(n_pages, a.n_kv);
+    return a.most == 0 ? lp : max(lp, (n_pages + a.most - 1) / a.most);
+}
+__device__ __forceinline__ int nodes_of(const Args& a, int n_pages) {
+    if (a.whole) return 1;
+    const int n = LEAVES * leaf_pages(a, n_pages);
+    return (n_pages + n - 1) / n;
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -204,7 +217,7 @@ __device__ __forceinline__ void cluster_sync() {
 enum Form { AUTO = 0, PLAIN = 1, RECORDS = 2, CLUSTERS = 3, STAY = 4 };
 struct Plan {
     bool possible;
-    int form, nt, tiles, nodes, stages, whole, kernels;
+    int form, nt, tiles, nodes, stages, whole, most, kernels;
     int64_t scratch, blocks;
 };
 
@@ -513,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
     const int n_rows = s.new_tokens * a.group, row0 = tile * 8 * NT;
     const int last = (min(row0 + 8 * NT, n_rows) - 1) / a.group;
     const int seen = (s.start + last) / kPage + 1;               // pages that any row of the tile sees
-    const int lp = a.whole ? (seen + LEAVES - 1) / LEAVES : leaf_pages(s.pages, a.n_kv);
+    const int lp = a.whole ? (seen + LEAVES - 1) / LEAVES : leaf_pages(a, s.pages);
     const int first_page = node * LEAVES * lp;
     pdl_wait();
     if (row0 >= n_rows || !fits(a, s)) return;                   // (so do all blocks of its cluster)
@@ -925,7 +938,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Args a, const int* __re
     if (row >= (int64_t)n_tokens * a.n_heads || b < 0 || b >= a.n_seqs) return;
     if (tok < s.first || tok >= s.first + s.new_tokens) return;  // (a token that fills the step up)
     if (!fits(a, s)) return;
-    const int seen = (s.start + tok - s.first) / kPage + 1, per = (BY_LEAF ? 1 : LEAVES) * leaf_pages(s.pages, a.n_kv), n = (seen + per - 1) / per;
+    const int seen = (s.start + tok - s.first) / kPage + 1, per = (BY_LEAF ? 1 : LEAVES) * leaf_pages(a, s.pages), n = (seen + per - 1) / per;
     if (s.pages <= per) return;
     const float* o_rec = fresh(a.rec) + row * a.nodes * D;
     const float* m_rec = fresh(a.rec) + a.rec_rows * a.nodes * D + row * a.nodes * 2;
@@ -1140,17 +1153,23 @@ static Plan plan(int n_tokens, int n_seqs, int n_heads, int n_kv, int max_q, int
     p.whole = rows > 8 && (int64_t)n_seqs * n_kv * p.tiles >= (p.form == PLAIN ? 4 : 2 * LEAVES) * sm;
     const int leaves = p.whole ? 1 : most_leaves(pages, n_kv);
     p.nodes = p.form == PLAIN ? leaves : (leaves + LEAVES - 1) / LEAVES;      // (places for records)
+    const int64_t places = RECORD_BYTES / (4 * (int64_t)max(n_tokens, 1) * n_heads * (D + 2));
+    if (rows > 8 && p.nodes > places) {
+        p.whole = places <= 1;
+        p.nodes = (int)max(places, (int64_t)1);
+        p.most = p.whole ? 0 : p.nodes * (p.form == PLAIN ? 1 : LEAVES);
+    }
     // Measured at 1 to 64 sequences of up to 300 to 131,000 positions, heads of 64 to 256, 2 to 16 key heads.  Blocks that stay want many nodes: a warp's first
     // one takes 15 us.  us a block per node / blocks that stay, heads of 128, up to eight rows: 512 nodes (one a sequence, 300 positions) 15 / 16, 512 (two a sequence,
     // 1,000) 20 / 24, 576 (18, 9,000) 21 / 25, 1,024 (one) 29 / 21, (two) 34 / 30, (eight) 30 / 30, 2,048 (eight) 53 / 39; 16 rows: 64 nodes 9 / 17, 768 43 / 33;
     // heads of 64, 42 rows: 512 24 / 23.
     // Clusters want to run all at once: 256 blocks 11.7 in records / 10.8, 512 19.3 / 20.4; heads of 256 (a block an SM) 64 11.7 / 10.8, 128 12.2 / 15.4.
-    const int64_t nodes = (int64_t)n_seqs * n_kv * (p.whole ? 1 : nodes_of(pages, n_kv)) * p.tiles;
+    const int64_t nodes = (int64_t)n_seqs * n_kv * (p.whole ? 1 : min(p.nodes, nodes_of(pages, n_kv))) * p.tiles;
     const bool can_stay = n_seqs <= MAX_SEQS;
     if (p.form == AUTO)
         p.form = can_stay && nodes >= (p.nt > 1 ? 4 : 6) * sm ? STAY : (p.nodes <= CLUSTER && nodes <= (D <= 128 ? 2 * sm : sm / 2) ? CLUSTERS : RECORDS);
     p.possible = p.form >= PLAIN && p.form <= STAY && !(f32 && p.form != PLAIN) && !(p.form == STAY && !can_stay) && !(p.form == CLUSTERS && p.nodes > CLUSTER);
-    p.stages = p.whole || leaf_pages(pages, n_kv) > 1 || p.nt == 3 ? MAX_STAGES : 1;
+    p.stages = p.whole || p.most > 0 || leaf_pages(pages, n_kv) > 1 || p.nt == 3 ? MAX_STAGES : 1;
     p.blocks = p.form == STAY ? sm : (int64_t)n_seqs * n_kv * p.tiles * p.nodes;
     const bool records = p.nodes > 1 && p.form != CLUSTERS;
     p.scratch = records ? (int64_t)n_tokens * n_heads * p.nodes * (D + 2) : 0;
@@ -1215,6 +1234,7 @@ static int attention(const void* q, int n_tokens, const void* kv, int64_t kv_pag
     a.tiles = p.tiles;
     a.stages = p.stages;
     a.whole = p.whole;
+    a.most = p.most;
     a.status = status;
     const cudaStream_t st = (cudaStream_t)stream;
     const dim3 grid((unsigned)p.blocks);
