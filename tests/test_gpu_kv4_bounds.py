@@ -394,3 +394,29 @@ def test_fewer_pieces_for_bounded_records(new, heads, d, dtype, kinds):
             check_attention(q[t:t + 1], out[t:t + 1], cache, one, scale, d)
         check_attention(q[new:], out[new:], cache, types.SimpleNamespace(q_lens=[3], starts=[100], table=[b.table[1]]), scale, d)
     o.check_status()
+
+
+def test_captured_decode_steps_do_not_keep_a_prompt_s_scratch():
+    import gc
+    import weakref
+
+    from helpers import CONFIGS, random_tokens
+    from test_gpu_kv4_engine import engine
+    eng = engine("D", "bfloat16", max_tokens=16384)
+    vocab = CONFIGS["D"]["vocab_size"]
+
+    def run(n):
+        s = eng.open_seq()
+        toks = random_tokens(vocab, n + 3, n)
+        eng.step([s], [toks[:n]], [[n - 1]])
+        out = [eng.step([s], [[t]], [[0]]).clone() for t in toks[n:]]
+        eng.close_seq(s)
+        return out
+    first = run(900)
+    large = weakref.ref(eng.workspace.buffers["attention_kv4_prompt"])
+    assert eng._graphs and all("attention_kv4_prompt" not in g.keepalive for g in eng._graphs.values())
+    run(2000)                                                        # (a larger one takes its place)
+    gc.collect()
+    assert large() is None
+    assert all(torch.equal(x, y) for x, y in zip(run(900), first))
+    eng.check_kernels()

@@ -55,3 +55,18 @@ def test_records_follow_the_length_alone_up_to_eight_rows():
         b = batch(seqs, seqs, 2048, 1)
         assert ops.attention_kv4_scratch(b, 8, 1, 128, torch.bfloat16, kind="records") == seqs * 8 * 128 * 130
         assert ops.attention_kv4_scratch(b, 8, 1, 128, torch.float32, kind="plain") == seqs * 8 * 1024 * 130
+
+
+def test_what_a_frozen_workspace_gave():
+    """A captured step keeps the scratch that it asked for, and no other's."""
+    from wick_b200.engine.engine import Workspace
+    w = Workspace(torch.device("cpu"))
+    w.get("a", 10, torch.float32)
+    b = w.get("b", 20, torch.float32)
+    w.frozen, w.taken = True, {}
+    assert w.get("b", 5, torch.float32) is b
+    with pytest.raises(RuntimeError):
+        w.get("c", 1, torch.float32)
+    w.frozen = False
+    w.get("a", 100, torch.float32)
+    assert set(w.taken) == {"b"} and w.taken["b"] is b

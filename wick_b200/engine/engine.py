@@ -47,6 +47,7 @@ class Workspace:
         self.device = device
         self.buffers: Dict[str, torch.Tensor] = {}
         self.frozen = False
+        self.taken: Dict[str, torch.Tensor] = {}        # what was asked for since it was frozen last
 
     def get(self, name: str, numel: int, dtype: torch.dtype, zero: bool = False) -> torch.Tensor:
         """zero: the buffer is zero when it is made (its users leave it zero)."""
@@ -57,6 +58,8 @@ class Workspace:
                                    f"graph is being captured")
             make = torch.zeros if zero else torch.empty
             b = self.buffers[name] = make(max(numel, 1), dtype=dtype, device=self.device)
+        if self.frozen:
+            self.taken[name] = b
         return b
 
 
@@ -479,7 +482,7 @@ class Engine:
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
-        self.workspace.frozen = True
+        self.workspace.frozen, self.workspace.taken = True, {}
         before = ops.launches[0]
         try:
             with torch.cuda.graph(graph, pool=pool):     # (prompt steps share one pool, steps of continuations another: none run at the same time)
@@ -488,8 +491,8 @@ class Engine:
             self.workspace.frozen = False
         g.kernels = ops.launches[0] - before
         ops.launches[0] = before
-        # The graph holds raw pointers into the scratch buffers: keep those alive
-        # even if the workspace later replaces them by larger ones.
-        g.keepalive = dict(self.workspace.buffers)
+        # The graph holds raw pointers into the scratch buffers that its step asked for: keep those alive
+        # even if the workspace later replaces them by larger ones.  (Others it leaves alone: a prompt's may be large.)
+        g.keepalive = self.workspace.taken
         g.graph = graph
         self.check_kernels()

@@ -369,7 +369,9 @@ class GQAttention(Mixer):
     def _attend_kv4(self, q, batch, cache, residual):
         # (pages that sequences share are read once for each of them: the 4-bit form knows page tables only)
         need = ops.attention_kv4_scratch(batch, self.heads, self.kv_heads, self.head_dim, self.ctx.dtype)
-        att = ops.attention_kv4(q, cache.kv, batch, self.scale, batch.workspace.get("attention_kv4", need, torch.float32))
+        # (opened pages and prompts' records are large: captured decode steps, which keep their scratch, have one of their own)
+        name = "attention_kv4" if batch.is_decode else "attention_kv4_prompt"
+        att = ops.attention_kv4(q, cache.kv, batch, self.scale, batch.workspace.get(name, need, torch.float32))
         return self.o.forward_delta(att.view(batch.n_tokens, self.q_dim), residual)
 
     def _encode_unfused(self, x, batch, cache, write_cache):
