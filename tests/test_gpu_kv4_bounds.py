@@ -420,3 +420,25 @@ def test_captured_decode_steps_do_not_keep_a_prompt_s_scratch():
     assert large() is None
     assert all(torch.equal(x, y) for x, y in zip(run(900), first))
     eng.check_kernels()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["D", "E"])
+def test_logits_of_prompts_of_many_tokens(name, dtype):
+    """Prompts whose steps decide codes in 32 bits first, alone, behind what is cached, and several together."""
+    from helpers import CONFIGS, random_tokens
+    from test_gpu_kv4_engine import check, engine
+    eng = engine(name, dtype, max_tokens=4096)
+    vocab = CONFIGS[name]["vocab_size"]
+    toks = random_tokens(vocab, 640, 31)
+    s = eng.open_seq()
+    got = [eng.step([s], [toks[:300]], [[0, 150, 299]]).clone(), eng.step([s], [toks[300:]], [[0, 70, 339]]).clone()]
+    check(eng, s, toks, torch.cat(got), [0, 150, 299, 300, 370, 639], name, dtype, (name, "alone"))
+    eng.close_seq(s)
+    lens = (280, 7, 129)
+    toks = [random_tokens(vocab, n, 40 + n) for n in lens]
+    slots = [eng.open_seq() for _ in lens]
+    got = eng.step(slots, toks, [[0, n - 1] for n in lens]).clone()
+    for b, n in enumerate(lens):
+        check(eng, slots[b], toks[b], got[2 * b:2 * b + 2], [0, n - 1], name, dtype, (name, n, "together"))
+    eng.check_kernels()
