@@ -53,6 +53,7 @@ constexpr int64_t RECORD_BYTES = 256 << 20;
 // A leaf is one page while one sequence alone so gives every SM up to two blocks (8 key heads: 37 nodes, 296 pages).  Longer sequences have nodes for one block
 // an SM (18) of long leaves, whose next page is on its way.  us, 32 heads over 8 of 128: 8 sequences of up to 12,000 positions, 24 nodes / 12 of twice the
 // leaves 40 / 49, one of 12,000 12.8 / 11.8; one of up to 32,000, 32 nodes of 2 pages a leaf / 16 of 4: 22 / 17; two of up to 131,000, 64 heads, 37 / 18: 80 / 72.
+// (148 and 296, one and two blocks for each SM of a B200, stand here as numbers: the cut, and with it a sequence's bits, does not follow the device.)
 __host__ __device__ inline int most_nodes(int n_kv, int blocks) { return max(4, min(128, blocks / n_kv)); }
 __host__ __device__ inline int leaf_pages(int n_pages, int n_kv) {
     const int most = LEAVES * most_nodes(n_kv, 148);
@@ -682,9 +683,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 && D <= 128 ? 2 : 1) leaves_k
 // pages: equal parts of the nodes 605 us, of the pages 382; 16 of 2,000 to 4,000: 38, 51 (some blocks have more nodes than warps).
 // A warp's tile is filled again while it is read: the next page's keys as soon as the scores are there, its values when the page is done.
 // One unit of rows (NT 1): a node's leaves are folded in registers.  More: there is no room for a second accumulator, and a node is one leaf.
-// What bounds it: the instructions that make values of codes (653 of a page's 1,343, half as fast as the others) and the matrix instructions beside them, which
-// add up: a scheduler needs 2,590 clocks a page, with two warps as with three.  64 sequences of 4,000 to 8,191 positions, 32 heads over 8 of 128 (504 MB of
-// pages): 133 us, 58 % of the copy's rate; 8 warps a block 140, 16 (which spill) 149.
+// What bounds it: the instructions that make values of codes (654 of a page's 1,331, half as fast as the others) and the matrix instructions beside them, which
+// mostly add up: a scheduler is active for 2,600 clocks a page, with two warps as with three (whose waits for one another are a part of it).  64 sequences of 4,000
+// to 8,191 positions, 32 heads over 8 of 128 (504 MB of pages): 130 us, 59 % of the copy's rate; at 133, 8 warps a block took 140, 16 (which spill) 149.
 struct Item {
     int b, kvh, row0, place, lp;                                 // place: the node's number in the sequence; none left: b < 0
     int page, end;                                               // of the sequence, as far as the row tile sees

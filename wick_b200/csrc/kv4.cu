@@ -56,7 +56,7 @@ __device__ __forceinline__ int64_t page_of(const int* page_table, int table_widt
 // A code is that of the number that 64-bit arithmetic gives (sums over the projection's runs, norm, rotation, range, division).  32 bits would put a few
 // numbers in a million, those next to the border between two codes, on the wrong side of it, another few for every other order of the same operations.  So a
 // vector is computed in 32 bits with a bound on what they can be off by; where every decision (both scales' roundings, every code) is the same
-// anywhere within the bound, it stands, and only where one is not (one key in some 60) the vector is computed again in 64.  3,900 tokens, 32 heads
+// anywhere within the bound, it stands, and only where one is not (one key in some 60) the vector is computed again in 64.  4,425 tokens, 32 heads
 // over 8 of 128: all in 64 bits 46 us, now 42 (the queries alone 21).
 constexpr int L = D == 192 ? 16 : D / 16;
 

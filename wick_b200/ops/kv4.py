@@ -163,6 +163,7 @@ def kv4_read(kv: torch.Tensor, head_dim: int, page_table: torch.Tensor, seq_of_t
 # Rows (new tokens times query heads of a key head) of a sequence up to which they are computed from the codes; of more its pages are opened to
 # bfloat16 and the prompt attention runs over them.  us from the codes / opened: 32 heads over 8 of 128, 8 sequences behind 6,000, 64 rows 71 / 83, 96
 # rows 85 / 87; 32 behind 2,000, 64 rows 89 / 91, 96 rows 115 / 96; one behind 2,000, 96 rows 14 / 24; 14 over 2 of 64, 32 behind 2,000, 168 rows 30 / 61.
+# Heads of 192 and 256 are never opened: the prompt attention has no tensor-core form for them.
 OPEN_ROWS = {64: 192, 128: 80}
 
 
