@@ -442,3 +442,42 @@ def test_logits_of_prompts_of_many_tokens(name, dtype):
     for b, n in enumerate(lens):
         check(eng, slots[b], toks[b], got[2 * b:2 * b + 2], [0, n - 1], name, dtype, (name, n, "together"))
     eng.check_kernels()
+
+
+def test_opened_pages_of_one_step_behind_another():
+    """Two steps of other lengths take turns over one scratch, with no other kernel in between: each finds its own description there."""
+    o = ops()
+    g = torch.Generator().manual_seed(26)
+    d, KV, H = 128, 2, 8
+    steps = []
+    for starts, new in (([0, 500], [300, 100]), ([540, 10], [100, 300])):
+        pages, b = step(starts, new, g, width=10)
+        kv, cache = random_cache(pages, KV, d, g)
+        q = torch.randn((b.n_tokens, H, d), generator=g).to(BF16).cuda()
+        steps.append((q, kv.cuda(), b, cache))
+    words = {o.attention_kv4_scratch(b, H, KV, d, BF16, kind="opened") for _, _, b, _ in steps}
+    assert len(words) == 1                                           # (the descriptions lie in the same places)
+    scratch = torch.empty(words.pop(), dtype=F32, device="cuda")
+    want = []
+    for q, kv, b, cache in steps:
+        want.append(o.attention_kv4(q, kv, b, 0.1, scratch, kind="opened"))
+        torch.cuda.synchronize()
+        check_attention(q, want[-1], cache, b, 0.1, d)
+    outs = [[torch.empty_like(q) for q, *_ in steps] for _ in range(50)]
+
+    def run():
+        for pair in outs:
+            for (q, kv, b, _), out in zip(steps, pair):
+                o.attention_kv4(q, kv, b, 0.1, scratch, out=out, kind="opened")
+    run()
+    assert all(torch.equal(out, w) for pair in outs for out, w in zip(pair, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(20):
+        for pair in outs:
+            for out in pair:
+                out.fill_(7.0)
+        graph.replay()
+        assert all(torch.equal(out, w) for pair in outs for out, w in zip(pair, want))
+    o.check_status()

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 attn_prompt_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
                       bf16* __restrict__ out, const int* __restrict__ cu_seqlens, int n_seqs,
                       const int* __restrict__ start_arr,
-                      const int* __restrict__ page_table, int table_width, int n_heads, int n_kv, int gs, int T, int columns, int per_kv, int tiles, int n_items, int ordered,
+                      const int* __restrict__ page_table, int table_width, int n_heads, int n_kv, int gs, int T, int columns, int per_kv, int tiles, int n_items, int ordered, int late,
                       float scale, int* status, int mask, int mask_size, const float* __restrict__ sink,
                       const __grid_constant__ CUtensorMap pool_map, const TcExtra X) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -251,7 +251,7 @@ attn_prompt_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         pdl_wait();
         return;
     }
-    // (the step's description is written by the host before the step: no kernel produces it)
+    // (the step's description is written by the host before the step: no kernel produces it; late: the kernel before this one does)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // Item k of the block is the one at place(k) of all, the key heads of one item side by side, in falling order of length, dealt
     // to and fro over the blocks.
@@ -278,6 +278,10 @@ attn_prompt_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    if (late) pdl_wait();
+    cu_seqlens = fresh(cu_seqlens);
+    start_arr = fresh(start_arr);
+    page_table = fresh(page_table);
     {
         const Finder finder(cu_seqlens, start_arr, n_seqs, T * tiles, ordered != 0);
 #pragma unroll 1
@@ -769,7 +773,7 @@ WICK_API int wick_attn_prompt_tc_supported() { return prompttc::SUPPORTED ? 1 : 
 // sequence by sequence); status: device int (code 7 if a block gave up waiting).
 static int attn_prompt_tc(const void* q, long long n_tokens, const void* kv, long long kv_pages, void* out, int n_tiles, const int* cu_seqlens,
                           int n_seqs, const int* start, const int* page_table, int table_width, int n_heads, int n_kv, float scale,
-                          int* status, int mask, int mask_size, const float* sink, const void* pool, const prompttc::TcExtra* extra, void* s) {
+                          int* status, int mask, int mask_size, const float* sink, const void* pool, const prompttc::TcExtra* extra, int late, void* s) {
     using namespace prompttc;
     WICK_REQUIRE(mask == 0 || ((mask == 1 || mask == 2) && mask_size > 0), "attention: mask %d of size %d", mask, mask_size);
     WICK_REQUIRE(SUPPORTED, "attention (tcgen05): head_dim %d is not 64 or 128", (int)WICK_HD);
@@ -824,7 +828,7 @@ static int attn_prompt_tc(const void* q, long long n_tokens, const void* kv, lon
     }
     WICK_CUDA(launch(kernel, dim3(blocks), dim3(THREADS), (size_t)SMEM_BYTES, (cudaStream_t)s, q_map,
                      kv_map, (bf16*)out, cu_seqlens, n_seqs, start, page_table, table_width, n_heads,
-                     n_kv, gs, T, columns, group / gs, tiles, n_items, ordered, scale, status, mask, mask_size, sink, pool_map, X));
+                     n_kv, gs, T, columns, group / gs, tiles, n_items, ordered, late, scale, status, mask, mask_size, sink, pool_map, X));
     return check_launch("attn_prompt_tc");
 }
 
@@ -834,7 +838,7 @@ WICK_API int wick_attn_prompt_tc_masked_bf16(const void* q, long long n_tokens, 
                                              const int* start, const int* page_table, int table_width, int n_heads, int n_kv,
                                              float scale, int* status, int mask, int mask_size, const float* sink, void* s) {
     return attn_prompt_tc(q, n_tokens, kv, kv_pages, out, n_tiles, cu_seqlens, n_seqs, start, page_table, table_width, n_heads, n_kv, scale,
-                          status, mask, mask_size, sink, nullptr, nullptr, s);
+                          status, mask, mask_size, sink, nullptr, nullptr, 0, s);
 }
 
 // ... then the blocks' array (bfloat16 [n_seqs * pool_tiles, 2, n_kv, 64, HD], or null), its tiles a sequence and positions a block, the cap
@@ -846,13 +850,14 @@ WICK_API int wick_attn_prompt_tc_pooled_bf16(const void* q, long long n_tokens, 
                                              int pool_tiles, int block, float cap, const float* gate, void* s) {
     const prompttc::TcExtra X = {pool_tiles, block, cap, gate};
     return attn_prompt_tc(q, n_tokens, kv, kv_pages, out, n_tiles, cu_seqlens, n_seqs, start, page_table, table_width, n_heads, n_kv, scale,
-                          status, mask, mask_size, sink, pool, &X, s);
+                          status, mask, mask_size, sink, pool, &X, 0, s);
 }
 
+// late: cu_seqlens, start and page_table are written by the kernel before this one in the stream.
 WICK_API int wick_attn_prompt_tc_bf16(const void* q, long long n_tokens, const void* kv, long long kv_pages, void* out,
                                       int n_tiles, const int* cu_seqlens, int n_seqs,
                                       const int* start, const int* page_table, int table_width, int n_heads, int n_kv,
-                                      float scale, int* status, void* s) {
-    return wick_attn_prompt_tc_masked_bf16(q, n_tokens, kv, kv_pages, out, n_tiles, cu_seqlens, n_seqs, start, page_table,
-                                           table_width, n_heads, n_kv, scale, status, 0, 0, nullptr, s);
+                                      float scale, int* status, int late, void* s) {
+    return attn_prompt_tc(q, n_tokens, kv, kv_pages, out, n_tiles, cu_seqlens, n_seqs, start, page_table, table_width, n_heads, n_kv, scale,
+                          status, 0, 0, nullptr, nullptr, nullptr, late, s);
 }

@@ -495,9 +495,10 @@ __global__ void __launch_bounds__(256)
 open_kernel(const uint8_t* __restrict__ kv, int64_t kv_pages, int n_kv, const int* __restrict__ page_table, int table_width,
             const int* __restrict__ cu_seqlens, const int* __restrict__ start, int n_seqs, int n_tokens, bf16* __restrict__ out,
             int* __restrict__ out_table, int* __restrict__ out_cu, int* __restrict__ out_start, int key_scale, int* status) {
-    // (No pdl_trigger: the kernel behind this one may read the page table before it waits, and this one writes it.)
     __shared__ int found[5];
     __shared__ uint8_t none[kPage];
+    // (No pdl_trigger: the attention's blocks find their items behind their wait, and started early they only stand in these blocks' way: 48.6 us in place of 49.0
+    // for 2,048 tokens, 32 heads over 8 of 128.)
     const int p = blockIdx.x, h = blockIdx.y;
     const bool describes = p == 0 && h == 0;                     // (the block that writes what is not a page's)
     if (threadIdx.x < 32) {

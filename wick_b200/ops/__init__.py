@@ -390,7 +390,8 @@ def attention_prompt(q: torch.Tensor, kv: torch.Tensor, batch, scale: float,
                      out: Optional[torch.Tensor] = None, plain: bool = False, kind: Optional[str] = None) -> torch.Tensor:
     """Causal attention of the step's new tokens over the cache (which already
     holds their keys and values).  q: [n, heads, d]; kv: [pages, 2, kv_heads, 64, d].
-    ``kind`` (see :func:`attention_prompt_kind`) picks a kernel by hand."""
+    ``kind`` (see :func:`attention_prompt_kind`) picks a kernel by hand.  The batch's ``late``, if it has one: whether a kernel of
+    this module has just written its tensors (those of a step are there before its first kernel)."""
     _cuda("q", q)
     n, n_heads, hd = q.shape
     _cuda("kv", kv, q.dtype)
@@ -405,10 +406,10 @@ def attention_prompt(q: torch.Tensor, kv: torch.Tensor, batch, scale: float,
     _need(kind == "plain" or q.dtype == torch.bfloat16, "the tensor-core attention kernels take bfloat16")
     n_tiles = attention_tiles(batch)
     if kind == "tc":
-        _attn(hd).call("wick_attn_prompt_tc_bf16", "plplpipippiiifpp", _p(q), n, _p(kv), kv.shape[0], _p(out),
+        _attn(hd).call("wick_attn_prompt_tc_bf16", "plplpipippiiifpip", _p(q), n, _p(kv), kv.shape[0], _p(out),
                        n_tiles, _p(batch.cu_seqlens), batch.n_seqs, _p(batch.start),
                        _p(batch.page_table), batch.table_width, n_heads, n_kv, float(scale),
-                       _p(status_tensor(q.device)), _stream())
+                       _p(status_tensor(q.device)), 1 if getattr(batch, "late", False) else 0, _stream())
         return out
     _attn(hd).call("wick_attn_prompt_mma_bf16" if kind == "mma" else f"wick_attn_prompt_{_dt(q)}", "pppipippiiifp",
                    _p(q), _p(kv), _p(out), n_tiles, _p(batch.cu_seqlens), batch.n_seqs, _p(batch.start), _p(batch.page_table),

@@ -298,4 +298,4 @@ def attention_kv4(q: torch.Tensor, kv: torch.Tensor, batch, scale: float, scratc
     opened, table, cu, start, _ = flat.split_with_sizes([at, n_seqs * width, n_seqs + 1, n_seqs, flat.shape[0] - words])
     return attention_prompt(q, opened.view(_BF16).view(pages, 2, n_kv, PAGE, hd), types.SimpleNamespace(
         n_tokens=n, q_tiles=getattr(batch, "q_tiles", None), q_lens=batch.q_lens, cu_seqlens=cu, n_seqs=n_seqs, start=start,
-        page_table=table, table_width=width), scale, out=out)
+        page_table=table, table_width=width, late=True), scale, out=out)
